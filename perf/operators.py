@@ -7,7 +7,7 @@ Every case runs in two forms. `own = False`: plain torch arithmetic in 32 bits, 
 
 The 4-bit formats. A code is one of +-{0, 0.5, 1, 1.5, 2, 3, 4, 6}; ties go to the code with an even mantissa bit.
 - "nv": blocks of 16 columns share an unsigned 8-bit scale S (4 exponent, 3 mantissa bits) and every row has a
-  32-bit scale s: s = the smallest power of two with amax(row) <= 2688 s, S = round(amax(block) / (6 s)),
+  32-bit scale s: s = the smallest power of two (2^-110 at least) with amax(row) <= 2688 s, S = round(amax(block) / (6 s)),
   code = round(x / (S s)), saturating at +-6.
 - "mx": blocks of 32 columns share a power of two 2^E, E = floor(log2(amax(block))) - 2, code = round(x / 2^E),
   saturating at +-6.
@@ -188,7 +188,7 @@ def _plain_values(x, fmt):
     top = v.abs().amax(2, keepdim=True)
     if fmt == "nv":
         m, e = torch.frexp(top.amax(1, keepdim=True))  # m in [0.5, 1); NV_TOP = 0.65625 x 2^12
-        e = torch.where(m > NV_TOP / 4096, e - 11, e - 12).clamp(-126, 127)
+        e = torch.where(m > NV_TOP / 4096, e - 11, e - 12).clamp_min(-110)
         six = torch.full_like(top, 6.0)
         scale = torch.ldexp((torch.ldexp(top, -e) / six).to(torch.float8_e4m3fn).float(), e)
     else:
@@ -308,7 +308,7 @@ def _exact_scales(x, fmt):
     if fmt == "mx":
         scale = _floor_power(top.clamp_min(2.0**-125)) / 4
     else:
-        most = top.max(-1, keepdim=True).values.clamp_min(2.0**-110) / 2688
+        most = (top.max(-1, keepdim=True).values / 2688).clamp_min(2.0**-110)
         s = _floor_power(most)
         s = torch.where(most > s, 2 * s, s)
         t = top / (6 * s)
