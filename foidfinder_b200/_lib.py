@@ -33,6 +33,13 @@ TILE_PAIR256 = 512  # ff_gemm_s8 tile_n: 256 x 256 tiles over a cluster of two C
 # ff_engine_profile kernel classes (FF_PROF_*).
 PROF_CLASSES = ("stem_prep", "stem_gemm", "rotate", "gemm_qkv", "attention", "gemm_proj", "gemm_fc1", "gemm_fc2", "head")
 
+# Block-scaled 4-bit operands (FF_FP4_*, FF_F16.., FF_EPI_QKV_NORM_ROPE, FF_NORM_*, FF_ROPE_*).
+FP4_NV, FP4_MX = 0, 1
+F16, BF16, F32 = 0, 1, 2
+EPI_QKV_NORM_ROPE = 8
+NORM_RMS, NORM_LAYER = 1, 2
+ROPE_PAIRS, ROPE_HALVES = 0, 1
+
 vp, i32, i64, f32 = C.c_void_p, C.c_int, C.c_int64, C.c_float
 
 
@@ -101,6 +108,14 @@ class ModelWeights(C.Structure):
     ] + [(name, vp) for name in POOL_FIELDS + PIXAI_FIELDS]
 
 
+class Fp4Epilogue(C.Structure):
+    _fields_ = (
+        [("kind", i32), ("out_dtype", i32), ("out", vp), ("ldo", i64), ("out_cols", i32), ("bias", vp), ("residual", vp),
+         ("ldr", i64), ("norm", i32), ("q_heads", i32), ("k_heads", i32), ("tokens", i32), ("qk_eps", f32)]
+        + [(name, vp) for name in ("q_w", "q_b", "k_w", "k_b", "rope_cos", "rope_sin")]
+    )
+
+
 _SIGNATURES = {
     "ff_last_error": (C.c_char_p, []),
     "ff_version": (i32, []),
@@ -112,6 +127,18 @@ _SIGNATURES = {
     "ff_linear_w8a8_noalloc": (i32, [vp, vp, vp, f32, i32, i32, i32, i32, vp, vp, vp, vp, i32, i32, vp, vp]),
     "ff_rot_q8_1024": (i32, [vp, vp, vp, i32, vp, vp, vp]),
     "ff_rot_q8_h128": (i32, [vp, i32, i32, vp, vp, vp]),
+    "ff_fp4_code_bytes": (i64, [i32, i32]),
+    "ff_fp4_scale_bytes": (i64, [i32, i32, i32]),
+    "ff_quantize_fp4": (i32, [vp, i32, i64, vp, vp, f32, i32, i32, i32, vp, vp, vp, vp]),
+    "ff_dequantize_fp4": (i32, [vp, vp, vp, i32, i32, i32, vp, i32, i64, vp]),
+    "ff_gemm_fp4": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, C.POINTER(Fp4Epilogue), i32, vp]),
+    "ff_linear_fp4_workspace_bytes": (i64, [i32, i32, i32]),
+    "ff_linear_fp4": (
+        i32, [vp, i32, i64, vp, vp, f32, vp, vp, vp, i32, i32, i32, i32, C.POINTER(Fp4Epilogue), vp, i64, vp]
+    ),
+    "ff_qk_norm_rope": (
+        i32, [vp, i32, i64, vp, i64, i32, i32, i32, i32, i32, vp, vp, vp, vp, f32, vp, vp, i32, i32, vp]
+    ),
     "ff_attention": (i32, [vp, vp, i32, i32, i32, vp, vp, f32, vp]),
     "ff_patchify": (i32, [vp, i32, i32, i32, C.POINTER(f32), C.POINTER(f32), vp, i32, vp]),
     "ff_fill_cls": (i32, [vp, vp, i32, i32, i32, vp]),

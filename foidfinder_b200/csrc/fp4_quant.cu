@@ -1,0 +1,553 @@
+// Block-scaled 4-bit quantisation (with an optional LayerNorm in front) and its inverse.
+//
+//   x [rows, cols] -> (LayerNorm over the row, f32 statistics) -> v
+//   FF_FP4_NV: s = smallest power of two (>= 2^-110) with amax(row) <= 2688 s (2688 = 6 * 448)
+//              S = e4m3(amax(block of 16) / (6 s)),  code = e2m1(v / (S s))
+//   FF_FP4_MX: scale = 2^(floor(log2 amax(block of 32)) - 2),  code = e2m1(v / scale)
+//
+// The power-of-two row scale costs no accuracy that the e4m3 block scale would have kept, and makes v / s and
+// S * s exact, so the codes are the correctly rounded quotients: amax / 6 is an IEEE division, and v / S is a
+// product with the rounded reciprocal whose last bits are snapped off for 16-bit inputs (see quotient()).
+// A row (NV) or block (MX) that holds an infinity or NaN gets a NaN scale, so that it shows in every result.
+//
+// Bound by HBM: 2 bytes read and 0.56 (NV) or 0.53 (MX) written per value. The whole row stays in registers,
+// 16 consecutive columns per lane, so a 16-column block never leaves its lane and a 32-column block is a pair
+// of lanes; WPR warps share a row so that a lane holds at most 48 values.
+#include <type_traits>
+
+#include "common.h"
+#include "fp4.cuh"
+
+namespace ff {
+
+namespace {
+
+constexpr int kQuantThreads = 256;
+
+// W 32-bit words starting at byte address `a` (any alignment that is a multiple of 2), words at or past `end`
+// undefined. Reads whole aligned 16-byte granules that hold at least one byte below `end`.
+template <int W>
+__device__ __forceinline__ void load_words(uintptr_t a, uintptr_t end, uint32_t (&w)[W]) {
+  const uint32_t mis = static_cast<uint32_t>(a) & 15u;
+  if (mis == 0) {
+#pragma unroll
+    for (int j = 0; j < W / 4; ++j) {
+      uint4 u = make_uint4(0, 0, 0, 0);
+      if (a + 16 * j < end) u = __ldg(reinterpret_cast<const uint4*>(a) + j);
+      w[4 * j] = u.x;
+      w[4 * j + 1] = u.y;
+      w[4 * j + 2] = u.z;
+      w[4 * j + 3] = u.w;
+    }
+    return;
+  }
+  const uintptr_t base = a - mis;
+  uint32_t t[W + 4];
+#pragma unroll
+  for (int j = 0; j < W / 4 + 1; ++j) {
+    uint4 u = make_uint4(0, 0, 0, 0);
+    if (base + 16 * j < end) u = __ldg(reinterpret_cast<const uint4*>(base) + j);
+    t[4 * j] = u.x;
+    t[4 * j + 1] = u.y;
+    t[4 * j + 2] = u.z;
+    t[4 * j + 3] = u.w;
+  }
+  if (mis & 8u) {
+#pragma unroll
+    for (int i = 0; i < W + 2; ++i) t[i] = t[i + 2];
+  }
+  if (mis & 4u) {
+#pragma unroll
+    for (int i = 0; i < W + 1; ++i) t[i] = t[i + 1];
+  }
+  const uint32_t sh = (mis & 2u) * 8u;  // 0 or 16 bits
+#pragma unroll
+  for (int i = 0; i < W; ++i) w[i] = __funnelshift_r(t[i], t[i + 1], sh);
+}
+
+template <class T>
+__device__ __forceinline__ void load16(const T* __restrict__ xr, int col, int cols, float (&v)[16]) {
+  if (col >= cols) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = 0.f;
+    return;
+  }
+  constexpr int W = sizeof(T) * 4;
+  uint32_t w[W];
+  load_words<W>(reinterpret_cast<uintptr_t>(xr + col), reinterpret_cast<uintptr_t>(xr + cols), w);
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(w[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float2 f = Pair16<T>::unpack(w[e]);
+      v[2 * e] = f.x;
+      v[2 * e + 1] = f.y;
+    }
+  }
+  if (col + 16 > cols) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      if (col + e >= cols) v[e] = 0.f;
+  }
+}
+
+// |.| maximum that keeps a NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float amax16(const float (&v)[16]) {
+  float m = 0.f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) m = max_nan(m, fabsf(v[e]));
+  return m;
+}
+__device__ __forceinline__ bool not_finite(float amax) { return !(amax <= 3.402823466e38f); }
+
+// FF_FP4_NV row scale s = 2^e: e = floor(log2 amax) - 11, one more when amax's mantissa is above 2688's
+// (1.3125), and -110 at least.
+__device__ __forceinline__ float nv_row_scale(float amax) {
+  const int biased = static_cast<int>((__float_as_uint(amax) + (0x7fffffu - 0x280000u)) >> 23) - 11;
+  return __uint_as_float(static_cast<uint32_t>(max(biased, 127 - 110)) << 23);
+}
+__device__ __forceinline__ float inv_pow2(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
+
+// v / (S s) for the code. EXACT16: v came from a 16-bit type, so a quotient that is no rounding tie of e2m1 is
+// at least 2^-13 away from one, while v * (1 / S) is within 2^-20 of the quotient: adding and subtracting 192
+// rounds to multiples of 2^-16, which puts true ties exactly on the tie. EXACT32: IEEE division (checkpoint
+// weights, once per load). Neither: v is itself rounded (after a LayerNorm), the product is enough.
+enum QuotientKind { kPlain, kExact16, kExact32 };
+template <int KIND>
+__device__ __forceinline__ float quotient(float v, float r, float scale) {
+  if constexpr (KIND == kExact32) return scale > 0.f ? __fdiv_rn(v, scale) : 0.f;
+  const float y = __fmul_rn(v, r);
+  if constexpr (KIND == kExact16) return __fsub_rn(__fadd_rn(y, 192.f), 192.f);
+  return y;
+}
+
+template <int KIND>
+__device__ __forceinline__ uint2 codes16(const float (&v)[16], float r, float scale) {
+  float lo[8], hi[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    lo[e] = quotient<KIND>(v[e], r, scale);
+    hi[e] = quotient<KIND>(v[8 + e], r, scale);
+  }
+  return make_uint2(e2m1x8(lo), e2m1x8(hi));
+}
+
+// One 16-column piece of an NV row with row scale s: its scale byte and codes.
+template <int KIND>
+__device__ __forceinline__ uint32_t nv_piece(const float (&v)[16], float s, bool bad, uint2* codes) {
+  const float is = inv_pow2(s);
+  const uint32_t byte = bad ? 0u : e4m3_byte(__fdiv_rn(amax16(v) * is, 6.f));
+  const float S = e4m3_value(byte);
+  const float r = byte ? __frcp_rn(S) * is : 0.f;
+  *codes = bad ? make_uint2(0, 0) : codes16<KIND>(v, r, S * s);
+  return byte;
+}
+// One 16-column piece of an MX block whose 32 columns have maximum amax. Scaling by a power of two is exact.
+__device__ __forceinline__ uint32_t mx_piece(const float (&v)[16], float amax, uint2* codes) {
+  if (not_finite(amax)) {
+    *codes = make_uint2(0, 0);
+    return 255u;
+  }
+  const int byte = max(static_cast<int>(__float_as_uint(amax) >> 23) - 2, 0);
+  *codes = codes16<kPlain>(v, __uint_as_float(static_cast<uint32_t>(254 - byte) << 23), 0.f);
+  return static_cast<uint32_t>(byte);
+}
+
+template <class T, bool NORM>
+__device__ constexpr int quotient_kind() {
+  return NORM ? kPlain : sizeof(T) == 4 ? kExact32 : kExact16;
+}
+
+struct QuantArgs {
+  const void* x;
+  int64_t ldx;
+  const float *gamma, *beta;
+  float eps;
+  int rows, cols;
+  uint8_t *codes, *scales;
+  float* row_scale;
+};
+
+__device__ __forceinline__ void affine16(float (&v)[16], float mean, float rstd, const QuantArgs& a, int col) {
+  if (col + 16 <= a.cols && (reinterpret_cast<uintptr_t>(a.gamma) & 15) == 0 &&
+      (reinterpret_cast<uintptr_t>(a.beta) & 15) == 0) {
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const float4 g = __ldg(reinterpret_cast<const float4*>(a.gamma + col + e));
+      const float4 b = __ldg(reinterpret_cast<const float4*>(a.beta + col + e));
+      v[e] = (v[e] - mean) * rstd * g.x + b.x;
+      v[e + 1] = (v[e + 1] - mean) * rstd * g.y + b.y;
+      v[e + 2] = (v[e + 2] - mean) * rstd * g.z + b.z;
+      v[e + 3] = (v[e + 3] - mean) * rstd * g.w + b.w;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      v[e] = col + e < a.cols ? (v[e] - mean) * rstd * __ldg(a.gamma + col + e) + __ldg(a.beta + col + e) : 0.f;
+  }
+}
+
+// Codes and scale bytes of the piece at 16-column index c; lanes hold consecutive c, and 4 (NV) or 8 (MX)
+// lanes join their bytes into one 32-bit store. Every lane of the warp calls it.
+template <bool MX>
+__device__ __forceinline__ void store_piece(const QuantArgs& a, int row, int c, uint2 codes, uint32_t byte, bool on) {
+  const int lane = threadIdx.x & 31;
+  const int64_t pitch = fp4_row_bytes(a.cols);
+  const int64_t tile = sf_tile_bytes(a.cols, MX);
+  uint32_t u = byte << (8 * (MX ? (lane >> 1) & 3 : lane & 3));
+  u |= __shfl_xor_sync(0xffffffffu, u, MX ? 2 : 1);
+  u |= __shfl_xor_sync(0xffffffffu, u, MX ? 4 : 2);
+  if (!on) return;
+  if (8 * static_cast<int64_t>(c) < pitch) *reinterpret_cast<uint2*>(a.codes + row * pitch + 8 * static_cast<int64_t>(c)) = codes;
+  if ((lane & (MX ? 7 : 3)) == 0)
+    *reinterpret_cast<uint32_t*>(a.scales + sf_offset(row, MX ? c >> 1 : c, tile)) = u;
+}
+
+// WPR warps per row, NC pieces of 16 columns per lane: rows of up to 512 * WPR * NC columns. A CTA takes rows
+// 32 apart (and neighbours), whose scales share 16-byte groups of a chunk.
+template <class T, bool MX, bool NORM, int WPR, int NC>
+__global__ void __launch_bounds__(kQuantThreads) quantize_fp4_kernel(const QuantArgs a) {
+  constexpr int RPC = kQuantThreads / 32 / WPR;  // rows per CTA
+  __shared__ float red[3][kQuantThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int grp = warp / WPR, wr = warp % WPR;
+  constexpr int PER_TILE = 128 / RPC;
+  const int tile = blockIdx.x / PER_TILE, j = blockIdx.x % PER_TILE;
+  int in_tile;
+  if constexpr (RPC == 8)
+    in_tile = 32 * (grp & 3) + 2 * j + (grp >> 2);
+  else if constexpr (RPC == 4)
+    in_tile = 32 * grp + j;
+  else if constexpr (RPC == 2)
+    in_tile = 32 * (2 * (j >> 5) + grp) + (j & 31);
+  else
+    in_tile = j;
+  const int row = tile * 128 + in_tile;
+  const bool on = row < a.rows;
+  auto row_all = [&](float v, int slot, auto op) {  // over the WPR warps of the row, after a warp reduction
+    if constexpr (WPR > 1) {
+      if (lane == 0) red[slot][warp] = v;
+      __syncthreads();
+      v = red[slot][grp * WPR];
+#pragma unroll
+      for (int i = 1; i < WPR; ++i) v = op(v, red[slot][grp * WPR + i]);
+    }
+    return v;
+  };
+  auto plus = [](float p, float q) { return p + q; };
+  pdl_wait();
+  pdl_trigger();
+  const T* xr = static_cast<const T*>(a.x) + (on ? row : 0) * a.ldx;
+  float v[NC][16];
+#pragma unroll
+  for (int i = 0; i < NC; ++i) load16<T>(xr, ((i * WPR + wr) * 32 + lane) * 16, on ? a.cols : 0, v[i]);
+  if constexpr (NORM) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s += v[i][e];
+    const float n = static_cast<float>(a.cols);
+    const float mean = row_all(warp_sum(s), 0, plus) / n;
+    float q = 0.f;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int col = ((i * WPR + wr) * 32 + lane) * 16;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float d = col + e < a.cols ? v[i][e] - mean : 0.f;
+        q += d * d;
+      }
+    }
+    const float rstd = rsqrtf(row_all(warp_sum(q), 1, plus) / n + a.eps);
+#pragma unroll
+    for (int i = 0; i < NC; ++i) affine16(v[i], mean, rstd, a, ((i * WPR + wr) * 32 + lane) * 16);
+  }
+  float s = 1.f;
+  bool bad = false;
+  if constexpr (!MX) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) m = max_nan(m, amax16(v[i]));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    m = row_all(m, 2, [](float p, float q) { return max_nan(p, q); });
+    bad = not_finite(m);
+    s = nv_row_scale(bad ? 0.f : m);
+    if (on && lane == 0 && wr == 0) a.row_scale[row] = bad ? __uint_as_float(0x7fffffffu) : s;
+  }
+  const int pieces = (a.cols + kFp4Step - 1) / kFp4Step * (kFp4Step / 16);
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int c = (i * WPR + wr) * 32 + lane;
+    uint2 codes;
+    uint32_t byte;
+    if constexpr (MX) {
+      float m = amax16(v[i]);
+      m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      byte = mx_piece(v[i], m, &codes);
+    } else {
+      byte = nv_piece<quotient_kind<T, NORM>()>(v[i], s, bad, &codes);
+    }
+    store_piece<MX>(a, row, c, codes, byte, on && c < pieces);
+  }
+}
+
+// Rows too wide for registers: one CTA per row, the row read again for each step (mean, variance, maximum,
+// codes); the later reads hit L2.
+template <class T, bool MX, bool NORM>
+__global__ void __launch_bounds__(kQuantThreads) quantize_fp4_wide_kernel(const QuantArgs a) {
+  __shared__ float red[kQuantThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = blockIdx.x;
+  const T* xr = static_cast<const T*>(a.x) + row * a.ldx;
+  auto cta_all = [&](float v, auto op) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+    __syncthreads();
+    if (lane == 0) red[warp] = v;
+    __syncthreads();
+    v = red[0];
+    for (int i = 1; i < kQuantThreads / 32; ++i) v = op(v, red[i]);
+    return v;
+  };
+  auto plus = [](float p, float q) { return p + q; };
+  pdl_wait();
+  pdl_trigger();
+  const int pieces = (a.cols + kFp4Step - 1) / kFp4Step * (kFp4Step / 16);
+  float mean = 0.f, rstd = 1.f, v[16];
+  if constexpr (NORM) {
+    float s = 0.f;
+    for (int c = threadIdx.x; c * 16 < a.cols; c += kQuantThreads) {
+      load16<T>(xr, c * 16, a.cols, v);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s += v[e];
+    }
+    mean = cta_all(s, plus) / static_cast<float>(a.cols);
+    float q = 0.f;
+    for (int c = threadIdx.x; c * 16 < a.cols; c += kQuantThreads) {
+      load16<T>(xr, c * 16, a.cols, v);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float d = c * 16 + e < a.cols ? v[e] - mean : 0.f;
+        q += d * d;
+      }
+    }
+    rstd = rsqrtf(cta_all(q, plus) / static_cast<float>(a.cols) + a.eps);
+  }
+  float s = 1.f;
+  bool bad = false;
+  if constexpr (!MX) {
+    float m = 0.f;
+    for (int c = threadIdx.x; c * 16 < a.cols; c += kQuantThreads) {
+      load16<T>(xr, c * 16, a.cols, v);
+      if constexpr (NORM) affine16(v, mean, rstd, a, c * 16);
+      m = max_nan(m, amax16(v));
+    }
+    m = cta_all(m, [](float p, float q) { return max_nan(p, q); });
+    bad = not_finite(m);
+    s = nv_row_scale(bad ? 0.f : m);
+    if (threadIdx.x == 0) a.row_scale[row] = bad ? __uint_as_float(0x7fffffffu) : s;
+  }
+  for (int c0 = warp * 32; c0 < pieces; c0 += kQuantThreads) {  // whole warps: the stores join lanes' bytes
+    const int c = c0 + lane;
+    load16<T>(xr, c * 16, a.cols, v);
+    if constexpr (NORM) affine16(v, mean, rstd, a, c * 16);
+    uint2 codes;
+    uint32_t byte;
+    if constexpr (MX) {
+      float m = amax16(v);
+      m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      byte = mx_piece(v, m, &codes);
+    } else {
+      byte = nv_piece<quotient_kind<T, NORM>()>(v, s, bad, &codes);
+    }
+    store_piece<MX>(a, row, c, codes, byte, c < pieces);
+  }
+}
+
+template <class T, bool MX, bool NORM, int WPR, int NC>
+int launch_quant(const QuantArgs& a, cudaStream_t stream) {
+  constexpr int RPC = kQuantThreads / 32 / WPR;
+  const int grid = (a.rows + 127) / 128 * (128 / RPC);
+  launch(quantize_fp4_kernel<T, MX, NORM, WPR, NC>, dim3(grid), dim3(kQuantThreads), 0, stream, a);
+  return check_launch("quantize_fp4_kernel");
+}
+
+template <class T, bool MX, bool NORM>
+int dispatch_quant(const QuantArgs& a, cudaStream_t stream) {
+  const int cols = (a.cols + kFp4Step - 1) / kFp4Step * kFp4Step;  // the padded scales are written too
+  if (cols <= 512) return launch_quant<T, MX, NORM, 1, 1>(a, stream);
+  if (cols <= 1024) return launch_quant<T, MX, NORM, 1, 2>(a, stream);
+  if (cols <= 1536) return launch_quant<T, MX, NORM, 1, 3>(a, stream);
+  if (cols <= 3 * 1024) return launch_quant<T, MX, NORM, 2, 3>(a, stream);
+  if (cols <= 6 * 1024) return launch_quant<T, MX, NORM, 4, 3>(a, stream);
+  if (cols <= 12 * 1024) return launch_quant<T, MX, NORM, 8, 3>(a, stream);
+  launch(quantize_fp4_wide_kernel<T, MX, NORM>, dim3(a.rows), dim3(kQuantThreads), 0, stream, a);
+  return check_launch("quantize_fp4_wide_kernel");
+}
+
+template <class T>
+int dispatch_quant_t(const QuantArgs& a, bool mx, cudaStream_t stream) {
+  if (a.gamma != nullptr) return mx ? dispatch_quant<T, true, true>(a, stream) : dispatch_quant<T, false, true>(a, stream);
+  return mx ? dispatch_quant<T, true, false>(a, stream) : dispatch_quant<T, false, false>(a, stream);
+}
+
+// ---------------------------------------------------------------- dequantisation
+template <class T>
+__device__ __forceinline__ void store_one(T* p, float v) {
+  if constexpr (sizeof(T) == 4)
+    *p = v;
+  else if constexpr (std::is_same<T, __half>::value)
+    *p = __float2half_rn(v);
+  else
+    *p = __float2bfloat16_rn(v);
+}
+
+// A thread writes one aligned 16-byte granule of an output row (its columns need not start at a block), so the
+// stores are whole whatever the row's alignment; granules that stick out of the row are written value by value.
+template <class T, bool MX>
+__global__ void __launch_bounds__(256)
+    dequantize_fp4_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+                          const float* __restrict__ row_scale, int rows, int cols, T* __restrict__ out, int64_t ldo,
+                          int granules) {
+  constexpr int E = 16 / sizeof(T);
+  pdl_wait();
+  pdl_trigger();
+  const int64_t pitch = fp4_row_bytes(cols), tile = sf_tile_bytes(cols, MX);
+  const int64_t total = static_cast<int64_t>(rows) * granules;
+  for (int64_t t = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; t < total;
+       t += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int row = static_cast<int>(t / granules), g = static_cast<int>(t % granules);
+    T* orow = out + row * ldo;
+    const int off = static_cast<int>((reinterpret_cast<uintptr_t>(orow) & 15) / sizeof(T));
+    const int c0 = g * E - off;  // first column of the granule, may be negative
+    if (c0 >= cols || c0 + E <= 0) continue;
+    const uint8_t* crow = codes + row * pitch;
+    const float s = MX || row_scale == nullptr ? 1.f : __ldg(row_scale + row);
+    // codes of columns [c0, c0 + 8): two aligned words, shifted
+    const int w0 = c0 >> 3;  // rounds down
+    const int words = static_cast<int>(pitch / 4);
+    const uint32_t lo = w0 >= 0 ? __ldg(reinterpret_cast<const uint32_t*>(crow) + w0) : 0u;
+    const uint32_t hi = w0 + 1 < words ? __ldg(reinterpret_cast<const uint32_t*>(crow) + w0 + 1) : 0u;
+    uint32_t h[4];
+    e2m1x8_to_half2(__funnelshift_r(lo, hi, 4 * (c0 & 7)), h);
+    // the (at most two) blocks that the granule touches
+    constexpr int B = MX ? 32 : 16;
+    const int b0 = (c0 < 0 ? 0 : c0) / B;
+    const int b1 = (c0 + E - 1 < cols ? c0 + E - 1 : cols - 1) / B;
+    float sc[2];
+    const int blk[2] = {b0, b1};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t byte = __ldg(scales + sf_offset(row, blk[i], tile));
+      sc[i] = MX ? e8m0_value(byte) : e4m3_value(byte) * s;
+    }
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float2 f = unpack_half2(h[e / 2]);
+      v[e] = ((e & 1) ? f.y : f.x) * ((c0 + e) / B > b0 ? sc[1] : sc[0]);
+    }
+    if (c0 >= 0 && c0 + E <= cols) {
+      uint4 u;
+      if constexpr (sizeof(T) == 4)
+        u = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+      else
+        u = make_uint4(Pair16<T>::pack(v[0], v[1]), Pair16<T>::pack(v[2], v[3]), Pair16<T>::pack(v[4], v[5]),
+                       Pair16<T>::pack(v[6], v[7]));
+      *reinterpret_cast<uint4*>(orow + c0) = u;
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (c0 + e >= 0 && c0 + e < cols) store_one(orow + c0 + e, v[e]);
+    }
+  }
+}
+
+template <class T>
+int launch_dequant(const uint8_t* codes, const uint8_t* scales, const float* rs, int rows, int cols, bool mx, void* out,
+                   int64_t ldo, cudaStream_t stream) {
+  constexpr int E = 16 / sizeof(T);
+  const int granules = (cols + 2 * E - 2) / E;  // one more than an aligned row's where the row may start inside one
+  const int64_t total = static_cast<int64_t>(rows) * granules;
+  const int64_t want = (total + 255) / 256, most = static_cast<int64_t>(sm_count()) * 32;
+  const dim3 grid(static_cast<unsigned>(want < most ? want : most));
+  if (mx)
+    launch(dequantize_fp4_kernel<T, true>, grid, dim3(256), 0, stream, codes, scales, rs, rows, cols,
+           static_cast<T*>(out), ldo, granules);
+  else
+    launch(dequantize_fp4_kernel<T, false>, grid, dim3(256), 0, stream, codes, scales, rs, rows, cols,
+           static_cast<T*>(out), ldo, granules);
+  return check_launch("dequantize_fp4_kernel");
+}
+
+}  // namespace
+
+int quantize_fp4(const void* x, int dtype, int64_t ldx, const float* gamma, const float* beta, float eps, int rows,
+                 int cols, int fmt, uint8_t* codes, uint8_t* scales, float* row_scale, cudaStream_t stream) {
+  FF_REQUIRE(fmt == FF_FP4_NV || fmt == FF_FP4_MX, "ff_quantize_fp4: unknown format %d", fmt);
+  FF_REQUIRE(dtype == FF_F16 || dtype == FF_BF16 || dtype == FF_F32, "ff_quantize_fp4: unknown type %d", dtype);
+  FF_REQUIRE(rows >= 0 && cols >= 1 && cols <= (1 << 24) && ldx >= cols, "ff_quantize_fp4: bad shape [%d, %d], row stride %lld", rows,
+             cols, static_cast<long long>(ldx));
+  if (rows == 0) return FF_OK;
+  FF_REQUIRE(x && codes && scales, "ff_quantize_fp4: NULL pointer");
+  FF_REQUIRE(fmt == FF_FP4_MX || row_scale, "ff_quantize_fp4: FF_FP4_NV needs row_scale");
+  FF_REQUIRE((gamma == nullptr) == (beta == nullptr), "ff_quantize_fp4: give both gamma and beta or neither");
+  FF_REQUIRE(reinterpret_cast<uintptr_t>(x) % (dtype == FF_F32 ? 4 : 2) == 0, "ff_quantize_fp4: x is not aligned to its type");
+  FF_REQUIRE(aligned16(codes) && aligned16(scales), "ff_quantize_fp4: codes and scales must be 16-byte aligned");
+  const QuantArgs a{x, ldx, gamma, beta, eps, rows, cols, codes, scales, row_scale};
+  const bool mx = fmt == FF_FP4_MX;
+  switch (dtype) {
+    case FF_F16: return dispatch_quant_t<__half>(a, mx, stream);
+    case FF_BF16: return dispatch_quant_t<__nv_bfloat16>(a, mx, stream);
+    default: return dispatch_quant_t<float>(a, mx, stream);
+  }
+}
+
+}  // namespace ff
+
+using namespace ff;
+
+extern "C" int64_t ff_fp4_code_bytes(int rows, int cols) {
+  return rows < 0 || cols < 1 ? 0 : static_cast<int64_t>(rows) * fp4_row_bytes(cols);
+}
+
+extern "C" int64_t ff_fp4_scale_bytes(int rows, int cols, int fmt) {
+  if (rows < 0 || cols < 1 || (fmt != FF_FP4_NV && fmt != FF_FP4_MX)) return 0;
+  return static_cast<int64_t>((rows + 127) / 128) * sf_tile_bytes(cols, fmt == FF_FP4_MX);
+}
+
+extern "C" int ff_quantize_fp4(const void* x, int dtype, int64_t ldx, const float* gamma, const float* beta, float eps,
+                               int rows, int cols, int fmt, uint8_t* codes, uint8_t* scales, float* row_scale,
+                               void* stream) {
+  return quantize_fp4(x, dtype, ldx, gamma, beta, eps, rows, cols, fmt, codes, scales, row_scale,
+                      static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int ff_dequantize_fp4(const uint8_t* codes, const uint8_t* scales, const float* row_scale, int rows, int cols,
+                                 int fmt, void* out, int dtype, int64_t ldo, void* stream) {
+  FF_REQUIRE(fmt == FF_FP4_NV || fmt == FF_FP4_MX, "ff_dequantize_fp4: unknown format %d", fmt);
+  FF_REQUIRE(dtype == FF_F16 || dtype == FF_BF16 || dtype == FF_F32, "ff_dequantize_fp4: unknown type %d", dtype);
+  FF_REQUIRE(rows >= 0 && cols >= 1 && cols <= (1 << 24) && ldo >= cols, "ff_dequantize_fp4: bad shape [%d, %d], row stride %lld", rows,
+             cols, static_cast<long long>(ldo));
+  if (rows == 0) return FF_OK;
+  FF_REQUIRE(codes && scales && out, "ff_dequantize_fp4: NULL pointer");
+  FF_REQUIRE(fmt == FF_FP4_MX || row_scale, "ff_dequantize_fp4: FF_FP4_NV needs row_scale");
+  FF_REQUIRE(reinterpret_cast<uintptr_t>(out) % (dtype == FF_F32 ? 4 : 2) == 0, "ff_dequantize_fp4: out is not aligned to its type");
+  FF_REQUIRE(aligned16(codes) && aligned16(scales), "ff_dequantize_fp4: codes and scales must be 16-byte aligned");
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool mx = fmt == FF_FP4_MX;
+  switch (dtype) {
+    case FF_F16: return launch_dequant<__half>(codes, scales, row_scale, rows, cols, mx, out, ldo, st);
+    case FF_BF16: return launch_dequant<__nv_bfloat16>(codes, scales, row_scale, rows, cols, mx, out, ldo, st);
+    default: return launch_dequant<float>(codes, scales, row_scale, rows, cols, mx, out, ldo, st);
+  }
+}

@@ -1,0 +1,166 @@
+// Per-head norm of queries and keys with the rotary position rotation in the same pass.
+//   n = RMS:   x / sqrt(mean(x^2) + eps) * w          LAYER: (x - mean) / sqrt(var + eps) * w + b
+//   (y0, y1) -> (y0 cos - y1 sin, y0 sin + y1 cos) for every pair, f32 throughout, one rounding at the end.
+//
+// Bound by HBM: every value is read and written once (4 bytes). One warp per row: 8 values (16 bytes) per lane,
+// D / 8 lanes per head, so the norm is a sum over D / 8 lanes and a pair of FF_ROPE_PAIRS stays in its lane. The
+// row's angles and the weights stay in registers over its heads; a CTA takes 8 neighbouring rows, whose angles
+// share cache sectors of the angle-major tables.
+#include "common.h"
+#include "fp4.cuh"
+
+namespace ff {
+
+namespace {
+
+constexpr int kQkWarps = 8;
+
+struct QkArgs {
+  const void* x;
+  int64_t ldx;
+  void* out;
+  int64_t ldo;
+  int rows, q_heads, k_heads;
+  const float *q_w, *q_b, *k_w, *k_b;
+  float eps;
+  const float *cos, *sin;
+  int tokens;
+};
+
+template <class T, int D, bool LAYER, bool HALVES>
+__global__ void __launch_bounds__(32 * kQkWarps) qk_norm_rope_kernel(const QkArgs a) {
+  constexpr int G = D / 8;       // lanes per head
+  constexpr int HPW = 32 / G;    // heads per warp and step
+  constexpr int NA = HALVES ? 8 : 4;  // angles per lane
+  const int lane = threadIdx.x & 31, l = lane % G, hl = lane / G;
+  const int row = blockIdx.x * kQkWarps + (threadIdx.x >> 5);
+  pdl_wait();
+  pdl_trigger();
+  if (row >= a.rows) return;
+  const int pos = row % a.tokens;
+  float c[NA], s[NA];
+#pragma unroll
+  for (int i = 0; i < NA; ++i) {
+    const int j = HALVES ? (l % (G / 2)) * 8 + i : l * 4 + i;
+    c[i] = __ldg(a.cos + static_cast<int64_t>(j) * a.tokens + pos);
+    s[i] = __ldg(a.sin + static_cast<int64_t>(j) * a.tokens + pos);
+  }
+  const T* xr = static_cast<const T*>(a.x) + row * a.ldx;
+  T* orow = static_cast<T*>(a.out) + row * a.ldo;
+  const int heads = a.q_heads + a.k_heads;
+#pragma unroll 2
+  for (int h0 = 0; h0 < heads; h0 += HPW) {
+    const int h = h0 + hl;
+    const bool on = h < heads;
+    uint4 u = make_uint4(0, 0, 0, 0);
+    if (on) u = *reinterpret_cast<const uint4*>(xr + h * D + l * 8);
+    const uint32_t w4[4] = {u.x, u.y, u.z, u.w};
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = Pair16<T>::unpack(w4[i]);
+      y[2 * i] = f.x;
+      y[2 * i + 1] = f.y;
+    }
+    if constexpr (LAYER) {
+      float m = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m += y[i];
+#pragma unroll
+      for (int o = G / 2; o; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
+      m *= 1.f / D;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] -= m;
+    }
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss = fmaf(y[i], y[i], ss);
+#pragma unroll
+    for (int o = G / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const float rstd = rsqrtf(ss * (1.f / D) + a.eps);
+    const float* w = h < a.q_heads ? a.q_w : a.k_w;
+    const float* b = h < a.q_heads ? a.q_b : a.k_b;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      y[i] = y[i] * rstd * __ldg(w + l * 8 + i);
+      if (LAYER && b != nullptr) y[i] += __ldg(b + l * 8 + i);
+    }
+    if constexpr (HALVES) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float other = __shfl_xor_sync(0xffffffffu, y[i], G / 2);
+        y[i] = l < G / 2 ? y[i] * c[i] - other * s[i] : other * s[i] + y[i] * c[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float y0 = y[2 * i], y1 = y[2 * i + 1];
+        y[2 * i] = y0 * c[i] - y1 * s[i];
+        y[2 * i + 1] = y0 * s[i] + y1 * c[i];
+      }
+    }
+    if (on)
+      *reinterpret_cast<uint4*>(orow + h * D + l * 8) = make_uint4(
+          Pair16<T>::pack(y[0], y[1]), Pair16<T>::pack(y[2], y[3]), Pair16<T>::pack(y[4], y[5]), Pair16<T>::pack(y[6], y[7]));
+  }
+}
+
+template <class T, int D>
+void launch_qk(const QkArgs& a, int norm, int pairing, cudaStream_t s) {
+  const dim3 grid((a.rows + kQkWarps - 1) / kQkWarps), block(32 * kQkWarps);
+  if (norm == FF_NORM_LAYER) {
+    if (pairing == FF_ROPE_HALVES)
+      launch(qk_norm_rope_kernel<T, D, true, true>, grid, block, 0, s, a);
+    else
+      launch(qk_norm_rope_kernel<T, D, true, false>, grid, block, 0, s, a);
+  } else {
+    if (pairing == FF_ROPE_HALVES)
+      launch(qk_norm_rope_kernel<T, D, false, true>, grid, block, 0, s, a);
+    else
+      launch(qk_norm_rope_kernel<T, D, false, false>, grid, block, 0, s, a);
+  }
+}
+
+template <class T>
+void launch_qk_dim(const QkArgs& a, int dim, int norm, int pairing, cudaStream_t s) {
+  switch (dim) {
+    case 32: return launch_qk<T, 32>(a, norm, pairing, s);
+    case 64: return launch_qk<T, 64>(a, norm, pairing, s);
+    case 128: return launch_qk<T, 128>(a, norm, pairing, s);
+    default: return launch_qk<T, 256>(a, norm, pairing, s);
+  }
+}
+
+}  // namespace
+
+}  // namespace ff
+
+using namespace ff;
+
+extern "C" int ff_qk_norm_rope(const void* x, int dtype, int64_t ldx, void* out, int64_t ldo, int rows, int q_heads,
+                               int k_heads, int head_dim, int norm, const float* q_w, const float* q_b,
+                               const float* k_w, const float* k_b, float eps, const float* rope_cos,
+                               const float* rope_sin, int tokens, int pairing, void* stream) {
+  FF_REQUIRE(dtype == FF_F16 || dtype == FF_BF16, "ff_qk_norm_rope: type %d is not fp16 or bf16", dtype);
+  FF_REQUIRE(head_dim == 32 || head_dim == 64 || head_dim == 128 || head_dim == 256,
+             "ff_qk_norm_rope: head_dim %d is not 32, 64, 128 or 256", head_dim);
+  FF_REQUIRE(norm == FF_NORM_RMS || norm == FF_NORM_LAYER, "ff_qk_norm_rope: unknown norm %d", norm);
+  FF_REQUIRE(pairing == FF_ROPE_PAIRS || pairing == FF_ROPE_HALVES, "ff_qk_norm_rope: unknown pairing %d", pairing);
+  FF_REQUIRE(rows >= 0 && q_heads >= 0 && k_heads >= 0 && q_heads <= (1 << 16) && k_heads <= (1 << 16) && tokens >= 1,
+             "ff_qk_norm_rope: bad shape rows=%d heads=%d+%d tokens=%d", rows, q_heads, k_heads, tokens);
+  const int64_t cols = static_cast<int64_t>(q_heads + k_heads) * head_dim;
+  FF_REQUIRE(ldx >= cols && ldo >= cols && ldx % 8 == 0 && ldo % 8 == 0,
+             "ff_qk_norm_rope: row strides %lld and %lld must hold %lld columns and be multiples of 8",
+             static_cast<long long>(ldx), static_cast<long long>(ldo), static_cast<long long>(cols));
+  if (rows == 0 || cols == 0) return FF_OK;
+  FF_REQUIRE(x && out && rope_cos && rope_sin && (q_w || q_heads == 0) && (k_w || k_heads == 0), "ff_qk_norm_rope: NULL pointer");
+  FF_REQUIRE(aligned16(x) && aligned16(out), "ff_qk_norm_rope: x and out must be 16-byte aligned");
+  FF_REQUIRE(x != out || ldx == ldo, "ff_qk_norm_rope: in place needs equal row strides");
+  const QkArgs a{x, ldx, out, ldo, rows, q_heads, k_heads, q_w, q_b, k_w, k_b, eps, rope_cos, rope_sin, tokens};
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == FF_F16)
+    launch_qk_dim<__half>(a, head_dim, norm, pairing, s);
+  else
+    launch_qk_dim<__nv_bfloat16>(a, head_dim, norm, pairing, s);
+  return check_launch("qk_norm_rope_kernel");
+}

@@ -12,13 +12,15 @@ import torch
 
 from . import _lib
 from ._lib import (
-    EPI_BIAS, EPI_GELU, EPI_LOGITS, EPI_QKV_ROPE, EPI_RESIDUAL, EPI_S32, EPI_STEM, EPI_SWIGLU, TILE_PAIR256, check, lib,
+    EPI_BIAS, EPI_GELU, EPI_LOGITS, EPI_QKV_NORM_ROPE, EPI_QKV_ROPE, EPI_RESIDUAL, EPI_S32, EPI_STEM, EPI_SWIGLU, FP4_MX,
+    FP4_NV, TILE_PAIR256, check, lib,
 )
 
 __all__ = [
     "EPI_QKV_ROPE", "EPI_RESIDUAL", "EPI_SWIGLU", "EPI_BIAS", "EPI_S32", "EPI_STEM", "EPI_LOGITS", "EPI_GELU", "TILE_PAIR256",
     "gemm_s8", "gemm_f16", "rot_q8", "rot_q8_1024", "rot_q8_h128", "attention", "patchify", "fill_cls",
     "layernorm", "topk", "tree_pool", "resize_pad", "patchify_windowed", "layernorm_pos", "pool_query_attention",
+    "FP4_NV", "FP4_MX", "EPI_QKV_NORM_ROPE", "quantize_fp4", "dequantize_fp4", "gemm_fp4", "linear_fp4", "qk_norm_rope",
 ]
 
 
@@ -301,3 +303,244 @@ def int8_mma_peak(device: int = 0, iters: int = 200_000) -> float:
         check(lib().ff_int8_mma_peak(iters, C.byref(ms), C.byref(ops), torch.cuda.current_stream(device).cuda_stream),
               "int8_mma_peak")
     return ops.value / (ms.value * 1e-3) / 1e12
+
+
+# ---------------------------------------------------------------- block-scaled 4-bit operands
+_DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
+_NORMS = {"rms": _lib.NORM_RMS, "layer": _lib.NORM_LAYER}
+_PAIRINGS = {"pairs": _lib.ROPE_PAIRS, "halves": _lib.ROPE_HALVES}
+
+
+def _rows_2d(t: torch.Tensor, what: str) -> int:
+    """Row stride of a 2-D tensor whose columns are contiguous."""
+    _need(t.is_cuda and t.dim() == 2 and (t.shape[1] <= 1 or t.stride(1) == 1), f"{what}: expected a 2-D CUDA tensor with contiguous columns")
+    return max(t.stride(0), t.shape[1]) if t.shape[0] <= 1 else t.stride(0)
+
+
+def _params(n: int, device: torch.device, what: str, **ts: torch.Tensor | None) -> None:
+    for name, t in ts.items():
+        if t is not None:
+            _need(t.device == device and t.is_contiguous() and t.dtype == torch.float32 and t.numel() == n, f"{what}: {name} must be {n} contiguous f32 values on {device}")
+
+
+def fp4_sizes(rows: int, cols: int, fmt: int) -> tuple[int, int]:
+    """Bytes of the code and scale buffers of a [rows, cols] operand."""
+    return int(lib().ff_fp4_code_bytes(rows, cols)), int(lib().ff_fp4_scale_bytes(rows, cols, fmt))
+
+
+def _fp4_operand(codes: torch.Tensor, scales: torch.Tensor, row_scale: torch.Tensor | None, rows: int, cols: int, fmt: int, what: str) -> None:
+    _cuda(codes, scales, row_scale)
+    nc, ns = fp4_sizes(rows, cols, fmt)
+    _need(codes.dtype == torch.uint8 and codes.numel() >= nc, f"{what}: codes must be uint8, {nc} bytes for [{rows}, {cols}]")
+    _need(scales.dtype == torch.uint8 and scales.numel() >= ns, f"{what}: scales must be uint8, {ns} bytes for [{rows}, {cols}]")
+    _need(scales.device == codes.device, f"{what}: codes and scales are on different devices")
+    if fmt == FP4_NV:
+        _params(rows, codes.device, what, row_scale=row_scale)
+        _need(row_scale is not None, f"{what}: FP4_NV needs row_scale")
+
+
+def quantize_fp4(
+    x: torch.Tensor,
+    codes: torch.Tensor,
+    scales: torch.Tensor,
+    row_scale: torch.Tensor | None,
+    fmt: int,
+    *,
+    gamma: torch.Tensor | None = None,
+    beta: torch.Tensor | None = None,
+    eps: float = 1e-6,
+) -> None:
+    """x [T, C] fp16, bf16 or f32 (columns contiguous, any row stride) -> (LayerNorm) -> 4-bit codes and block scales
+    (`fp4_sizes` bytes) and, for FP4_NV, row_scale [T] f32."""
+    ldx = _rows_2d(x, "quantize_fp4")
+    _need(x.dtype in _DTYPES, "quantize_fp4: x must be fp16, bf16 or f32")
+    T, cols = x.shape
+    _fp4_operand(codes, scales, row_scale, T, cols, fmt, "quantize_fp4")
+    _need(codes.device == x.device, "quantize_fp4: x and codes are on different devices")
+    _params(cols, x.device, "quantize_fp4", gamma=gamma, beta=beta)
+    with torch.cuda.device(x.device):
+        check(
+            lib().ff_quantize_fp4(
+                _ptr(x), _DTYPES[x.dtype], ldx, _ptr(gamma), _ptr(beta), eps, T, cols, fmt, _ptr(codes), _ptr(scales),
+                _ptr(row_scale), _stream(x),
+            ),
+            "quantize_fp4",
+        )
+
+
+def dequantize_fp4(codes: torch.Tensor, scales: torch.Tensor, row_scale: torch.Tensor | None, out: torch.Tensor, fmt: int) -> None:
+    """The values of a 4-bit operand into out [T, C] (fp16, bf16 or f32; columns contiguous, any row stride)."""
+    ldo = _rows_2d(out, "dequantize_fp4")
+    _need(out.dtype in _DTYPES, "dequantize_fp4: out must be fp16, bf16 or f32")
+    T, cols = out.shape
+    _fp4_operand(codes, scales, row_scale, T, cols, fmt, "dequantize_fp4")
+    _need(codes.device == out.device, "dequantize_fp4: codes and out are on different devices")
+    with torch.cuda.device(out.device):
+        check(
+            lib().ff_dequantize_fp4(
+                _ptr(codes), _ptr(scales), _ptr(row_scale), T, cols, fmt, _ptr(out), _DTYPES[out.dtype], ldo, _stream(out)
+            ),
+            "dequantize_fp4",
+        )
+
+
+def fp4_epilogue(
+    epi: int,
+    N: int,
+    device: torch.device,
+    *,
+    bias: torch.Tensor | None = None,
+    norm: str = "rms",
+    q_heads: int = 0,
+    k_heads: int = 0,
+    q_weight: torch.Tensor | None = None,
+    k_weight: torch.Tensor | None = None,
+    q_bias: torch.Tensor | None = None,
+    k_bias: torch.Tensor | None = None,
+    qk_eps: float = 1e-6,
+    rope_cos: torch.Tensor | None = None,
+    rope_sin: torch.Tensor | None = None,
+) -> _lib.Fp4Epilogue:
+    """The part of a gemm_fp4 epilogue that does not change from call to call (the tensors must outlive it)."""
+    e = _lib.Fp4Epilogue(kind=epi)
+    _params(N, device, "fp4_epilogue", bias=bias)
+    e.bias = _ptr(bias)
+    if epi == EPI_QKV_NORM_ROPE:
+        _need(norm in _NORMS, "fp4_epilogue: norm must be 'rms' or 'layer'")
+        _params(64, device, "fp4_epilogue", q_weight=q_weight, k_weight=k_weight, q_bias=q_bias, k_bias=k_bias)
+        _need(rope_cos is not None and rope_sin is not None and rope_cos.dim() == 2 and rope_cos.shape[0] == 32 and rope_sin.shape == rope_cos.shape,
+              "fp4_epilogue: rotation tables must be [32, tokens]")
+        _params(rope_cos.numel(), device, "fp4_epilogue", rope_cos=rope_cos, rope_sin=rope_sin)
+        e.norm, e.q_heads, e.k_heads, e.tokens, e.qk_eps = _NORMS[norm], q_heads, k_heads, rope_cos.shape[1], qk_eps
+        e.q_w, e.k_w, e.q_b, e.k_b = _ptr(q_weight), _ptr(k_weight), _ptr(q_bias), _ptr(k_bias)
+        e.rope_cos, e.rope_sin = _ptr(rope_cos), _ptr(rope_sin)
+    return e
+
+
+def _bind_out(e: _lib.Fp4Epilogue, M: int, N: int, out: torch.Tensor, residual: torch.Tensor | None, device: torch.device, what: str) -> None:
+    ldo = _rows_2d(out, what)
+    cols = out.shape[1]
+    _need(out.device == device and out.dtype in _DTYPES, f"{what}: out must be fp16, bf16 or f32 on {device}")
+    _need(out.shape[0] == M and (cols <= N // 2 if e.kind == EPI_SWIGLU else cols == N), f"{what}: out has shape {tuple(out.shape)} for M={M} N={N}")
+    e.out_dtype, e.out, e.ldo, e.out_cols = _DTYPES[out.dtype], _ptr(out), ldo, cols
+    e.residual = None
+    if e.kind == EPI_RESIDUAL:
+        _need(residual is not None, f"{what}: EPI_RESIDUAL needs the residual")
+        e.ldr = _rows_2d(residual, what)
+        _need(residual.shape == out.shape and residual.dtype == out.dtype and residual.device == device, f"{what}: the residual must be like out")
+        e.residual = _ptr(residual)
+
+
+def gemm_fp4(
+    A: torch.Tensor,
+    A_scales: torch.Tensor,
+    row_scale: torch.Tensor | None,
+    W: torch.Tensor,
+    W_scales: torch.Tensor,
+    col_scale: torch.Tensor | None,
+    out: torch.Tensor,
+    epilogue: int | _lib.Fp4Epilogue,
+    fmt: int,
+    *,
+    N: int,
+    K: int,
+    bias: torch.Tensor | None = None,
+    residual: torch.Tensor | None = None,
+    tile: int = 0,
+    **heads,
+) -> None:
+    """4-bit A [M, K] x W [N, K] (operands of `quantize_fp4`) -> epilogue into out (see include/foidfinder_b200.h).
+    `epilogue` is an EPI_* number, with `bias` and the head arguments of `fp4_epilogue`, or a prepared
+    `fp4_epilogue`."""
+    M = out.shape[0]
+    _fp4_operand(A, A_scales, row_scale, M, K, fmt, "gemm_fp4")
+    _fp4_operand(W, W_scales, col_scale, N, K, fmt, "gemm_fp4")
+    _need(W.device == A.device, "gemm_fp4: A and W are on different devices")
+    e = fp4_epilogue(epilogue, N, A.device, bias=bias, **heads) if isinstance(epilogue, int) else epilogue
+    _bind_out(e, M, N, out, residual, A.device, "gemm_fp4")
+    with torch.cuda.device(A.device):
+        check(
+            lib().ff_gemm_fp4(
+                _ptr(A), _ptr(A_scales), _ptr(row_scale), _ptr(W), _ptr(W_scales), _ptr(col_scale), fmt, M, N, K,
+                C.byref(e), tile, _stream(A),
+            ),
+            "gemm_fp4",
+        )
+
+
+def linear_fp4(
+    x: torch.Tensor,
+    W: torch.Tensor,
+    W_scales: torch.Tensor,
+    col_scale: torch.Tensor | None,
+    out: torch.Tensor,
+    epilogue: int | _lib.Fp4Epilogue,
+    fmt: int,
+    *,
+    N: int,
+    gamma: torch.Tensor | None = None,
+    beta: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    bias: torch.Tensor | None = None,
+    residual: torch.Tensor | None = None,
+    **heads,
+) -> None:
+    """quantize_fp4 of x [M, K] (with the LayerNorm, if gamma is given) and gemm_fp4 in one call; the codes of x live
+    in a workspace from torch's allocator on the current stream."""
+    ldx = _rows_2d(x, "linear_fp4")
+    M, K = x.shape
+    _need(x.dtype in _DTYPES, "linear_fp4: x must be fp16, bf16 or f32")
+    _fp4_operand(W, W_scales, col_scale, N, K, fmt, "linear_fp4")
+    _need(W.device == x.device, "linear_fp4: x and W are on different devices")
+    _params(K, x.device, "linear_fp4", gamma=gamma, beta=beta)
+    e = fp4_epilogue(epilogue, N, x.device, bias=bias, **heads) if isinstance(epilogue, int) else epilogue
+    _bind_out(e, M, N, out, residual, x.device, "linear_fp4")
+    with torch.cuda.device(x.device):
+        nbytes = lib().ff_linear_fp4_workspace_bytes(M, K, fmt)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        check(
+            lib().ff_linear_fp4(
+                _ptr(x), _DTYPES[x.dtype], ldx, _ptr(gamma), _ptr(beta), eps, _ptr(W), _ptr(W_scales), _ptr(col_scale),
+                fmt, M, N, K, C.byref(e), _ptr(ws), nbytes, _stream(x),
+            ),
+            "linear_fp4",
+        )
+
+
+def qk_norm_rope(
+    x: torch.Tensor,
+    out: torch.Tensor,
+    *,
+    q_heads: int,
+    k_heads: int,
+    head_dim: int,
+    norm: str,
+    q_weight: torch.Tensor | None,
+    k_weight: torch.Tensor | None,
+    rope_cos: torch.Tensor,
+    rope_sin: torch.Tensor,
+    q_bias: torch.Tensor | None = None,
+    k_bias: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    pairing: str = "pairs",
+) -> None:
+    """x [T, >= (q_heads + k_heads) * head_dim] fp16 or bf16, q heads then k heads -> every head normalised ("rms" or
+    "layer") and rotated by position row % tokens, into the first columns of out (x itself: in place). Tables are
+    angle-major [head_dim / 2, tokens] f32; `pairing` "pairs" rotates (2i, 2i + 1), "halves" (i, i + head_dim / 2)."""
+    ldx, ldo = _rows_2d(x, "qk_norm_rope"), _rows_2d(out, "qk_norm_rope")
+    cols = (q_heads + k_heads) * head_dim
+    _need(x.dtype in (torch.float16, torch.bfloat16) and out.dtype == x.dtype, "qk_norm_rope: x and out must be fp16 or bf16, alike")
+    _need(x.shape[1] >= cols and out.shape[1] >= cols and out.shape[0] == x.shape[0] and out.device == x.device, "qk_norm_rope: shapes")
+    _need(norm in _NORMS and pairing in _PAIRINGS, "qk_norm_rope: norm is 'rms' or 'layer', pairing 'pairs' or 'halves'")
+    _params(head_dim, x.device, "qk_norm_rope", q_weight=q_weight, k_weight=k_weight, q_bias=q_bias, k_bias=k_bias)
+    _need(rope_cos.dim() == 2 and rope_cos.shape[0] == head_dim // 2 and rope_sin.shape == rope_cos.shape, "qk_norm_rope: rotation tables must be [head_dim / 2, tokens]")
+    _params(rope_cos.numel(), x.device, "qk_norm_rope", rope_cos=rope_cos, rope_sin=rope_sin)
+    with torch.cuda.device(x.device):
+        check(
+            lib().ff_qk_norm_rope(
+                _ptr(x), _DTYPES[x.dtype], ldx, _ptr(out), ldo, x.shape[0], q_heads, k_heads, head_dim, _NORMS[norm],
+                _ptr(q_weight), _ptr(q_bias), _ptr(k_weight), _ptr(k_bias), eps, _ptr(rope_cos), _ptr(rope_sin),
+                rope_cos.shape[1], _PAIRINGS[pairing], _stream(x),
+            ),
+            "qk_norm_rope",
+        )

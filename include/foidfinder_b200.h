@@ -141,6 +141,102 @@ int ff_linear_w8a8_noalloc(const uint16_t* x, const float* gamma, const float* b
 int ff_attention(const uint16_t* qkv, uint16_t* out, int num_seqs, int seq_len, int heads, const float* rope_cos,
                  const float* rope_sin, float scale, void* stream);
 
+/* ---------------------------------------------------------------- block-scaled 4-bit operands */
+/*
+ * Values of +-{0, 0.5, 1, 1.5, 2, 3, 4, 6} (e2m1, ties to the even mantissa) with a scale per block of columns.
+ *   FF_FP4_NV: blocks of 16 columns, unsigned 8-bit scales S (4 exponent, 3 mantissa bits), and an f32 scale
+ *              per row: s = smallest power of two (>= 2^-110) with amax(row) <= 2688 s,
+ *              S = round(amax(block) / (6 s)), code = round(v / (S s)). A row with an infinity or NaN gets s = NaN.
+ *   FF_FP4_MX: blocks of 32 columns, power-of-two scales 2^(floor(log2 amax(block)) - 2), no row scale.
+ *              A block with an infinity or NaN gets the scale NaN.
+ * Codes: row-major, column 2i in the low and 2i + 1 in the high four bits of byte i, rows padded with zeros to
+ * 32 columns. Scales: 512-byte chunks of 128 rows x 4 blocks (row r at byte (r % 32) * 16 + (r / 32) * 4), the
+ * chunks of a 128-row tile contiguous along the columns, columns padded with zero scales to a multiple of 256.
+ * None of this has a counterpart in the reference, whose quantised products are int8.
+ */
+#define FF_FP4_NV 0
+#define FF_FP4_MX 1
+#define FF_F16 0
+#define FF_BF16 1
+#define FF_F32 2
+/* Buffer sizes; codes and scales must be 16-byte aligned. */
+int64_t ff_fp4_code_bytes(int rows, int cols);
+int64_t ff_fp4_scale_bytes(int rows, int cols, int fmt);
+
+/*
+ * x [rows, cols] of type dtype (FF_F16, FF_BF16, FF_F32), row stride ldx elements (any), -> (LayerNorm over the
+ * row with gamma/beta/eps when gamma != NULL, f32 statistics) -> codes, scales and, for FF_FP4_NV,
+ * row_scale [rows] (unused and may be NULL for FF_FP4_MX). Any rows >= 0 and cols in [1, 2^24].
+ */
+int ff_quantize_fp4(const void* x, int dtype, int64_t ldx, const float* gamma, const float* beta, float eps, int rows,
+                    int cols, int fmt, uint8_t* codes, uint8_t* scales, float* row_scale, void* stream);
+/* The values back: out [rows, cols] of type dtype, row stride ldo elements, = code * (S * s) rounded once. */
+int ff_dequantize_fp4(const uint8_t* codes, const uint8_t* scales, const float* row_scale, int rows, int cols, int fmt,
+                      void* out, int dtype, int64_t ldo, void* stream);
+
+/*
+ * The product of two such operands on the tcgen05 tensor cores, A [M, K] x W [N, K]:
+ *   y[m, n] = (sum over k, block scales included, f32) * row_scale[m] * col_scale[n] + bias[n]
+ * (row_scale and col_scale, the two operands' row scales, are read for FF_FP4_NV only), then one of
+ *   FF_EPI_BIAS           out = y                       (fp16, bf16 or f32)
+ *   FF_EPI_GELU           out = gelu_tanh(y)            (fp16 or bf16, like all below)
+ *   FF_EPI_SWIGLU         W rows interleaved [gate 64 | up 64]; out [M, out_cols] = silu(gate) * up, out_cols <= N / 2
+ *                         (0: N / 2)
+ *   FF_EPI_RESIDUAL       out = residual + y, summed in f32 (residual may be out itself)
+ *   FF_EPI_QKV_NORM_ROPE  heads of 64 columns, q_heads then k_heads of them, are normalised (FF_NORM_RMS:
+ *                         y / rms(y) * w, FF_NORM_LAYER: (y - mean) / std * w + b) and their interleaved pairs
+ *                         rotated by the angles of position m % tokens (rope_cos / rope_sin [32, tokens],
+ *                         angle-major); the columns after them (v) are out = y
+ * Any M, N, K >= 1 (FF_EPI_SWIGLU: N % 128 == 0; FF_EPI_QKV_NORM_ROPE: N % 64 == 0). 16-bit out and residual:
+ * 16-byte aligned, row strides (elements) multiples of 8. f32 out: any row stride. bias may be NULL.
+ * tile: 0 = automatic, 128 = 128 x 128 tiles per CTA, FF_TILE_PAIR256 = 256 x 256 tiles per pair of CTAs.
+ */
+#define FF_EPI_QKV_NORM_ROPE 8
+#define FF_NORM_RMS 1
+#define FF_NORM_LAYER 2
+typedef struct ff_fp4_epilogue {
+  int kind;
+  int out_dtype;
+  void* out;
+  int64_t ldo;
+  int out_cols;
+  const float* bias; /* [N] */
+  const void* residual;
+  int64_t ldr;
+  int norm, q_heads, k_heads, tokens;
+  float qk_eps;
+  const float *q_w, *q_b, *k_w, *k_b; /* [64]; biases may be NULL */
+  const float *rope_cos, *rope_sin;
+} ff_fp4_epilogue;
+int ff_gemm_fp4(const uint8_t* A, const uint8_t* A_scales, const float* row_scale, const uint8_t* W,
+                const uint8_t* W_scales, const float* col_scale, int fmt, int M, int N, int K,
+                const ff_fp4_epilogue* epilogue, int tile, void* stream);
+
+/*
+ * ff_quantize_fp4 of x [M, K] followed by ff_gemm_fp4 in one call. workspace: device memory, 16-byte aligned, of
+ * at least ff_linear_fp4_workspace_bytes(M, K, fmt) bytes, free again once the call's work on the stream is done.
+ */
+int64_t ff_linear_fp4_workspace_bytes(int M, int K, int fmt);
+int ff_linear_fp4(const void* x, int dtype, int64_t ldx, const float* gamma, const float* beta, float eps,
+                  const uint8_t* W, const uint8_t* W_scales, const float* col_scale, int fmt, int M, int N, int K,
+                  const ff_fp4_epilogue* epilogue, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------- query and key heads */
+/*
+ * Per-head norm and rotary position rotation of queries and keys in one pass: x [rows, >= (q_heads + k_heads) *
+ * head_dim] of type dtype (FF_F16, FF_BF16), row stride ldx elements, q heads then k heads. Every head is
+ * normalised (FF_NORM_RMS or FF_NORM_LAYER, f32, weights [head_dim], biases for FF_NORM_LAYER or NULL) and its
+ * pairs rotated by the angles of position row % tokens: rope_cos / rope_sin [head_dim / 2, tokens] f32,
+ * angle-major. pairing FF_ROPE_PAIRS: pair i is columns (2i, 2i + 1); FF_ROPE_HALVES: (i, i + head_dim / 2).
+ * out [rows, (q_heads + k_heads) * head_dim], row stride ldo; out may be x itself (ldo == ldx). head_dim 32, 64,
+ * 128 or 256; x and out 16-byte aligned with row strides that are multiples of 8. No reference counterpart.
+ */
+#define FF_ROPE_PAIRS 0
+#define FF_ROPE_HALVES 1
+int ff_qk_norm_rope(const void* x, int dtype, int64_t ldx, void* out, int64_t ldo, int rows, int q_heads, int k_heads,
+                    int head_dim, int norm, const float* q_w, const float* q_b, const float* k_w, const float* k_b,
+                    float eps, const float* rope_cos, const float* rope_sin, int tokens, int pairing, void* stream);
+
 /* ---------------------------------------------------------------- stem, norm, head */
 /*
  * images [B, S, S, 3] uint8 -> patches [B * (S/p)^2, k_pad] fp16 with (kh, kw, c) column order

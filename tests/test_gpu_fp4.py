@@ -1,0 +1,421 @@
+"""Block-scaled 4-bit quantisation, the 4-bit product with its epilogues and the query/key head norms with rotation,
+against the 64-bit oracle (oracle/fp4.py).
+
+Tolerances. Quantisation without a norm is exact. After a LayerNorm the f32 statistics move a value by up to about
+2^-20 of itself, which moves a code or a block scale only next to a rounding boundary: at most 1 in 1000 codes may
+differ. Products are compared on the same codes: the tensor cores add in f32, one rounding (or truncation) of at most
+2^-22 of the sum of magnitudes per 64-column step, plus the output type's own rounding (half a unit in the last place)
+and, for the epilogues with transcendental functions, their relative error of 2^-18.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from oracle import fp4 as O
+
+pytestmark = pytest.mark.gpu
+
+HALF_ULP = {torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8, torch.float32: 2.0**-24}
+TINY = {torch.float16: 2.0**-25, torch.bfloat16: 2.0**-130, torch.float32: 2.0**-130}
+FMT = {"nv": 0, "mx": 1}
+
+
+def _x(rows, cols, dtype, seed, outliers=True):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, cols, generator=g)
+    if outliers:
+        x = torch.where(torch.rand(rows, cols, generator=g) < 0.01, 20 * x, x)
+    return x.to(dtype)
+
+
+def _read(q):
+    """(codes [T, C], scale bytes of the padded columns [T, blocks], row scale) of an Fp4Tensor."""
+    codes = O.unpack_codes(q.codes, q.rows, q.cols)
+    s = q.scales.cpu()[O.scale_index(q.rows, q.cols, q.fmt)]
+    row = q.row_scale.cpu().double() if q.fmt == "nv" else torch.ones(q.rows, dtype=torch.float64)
+    return codes, s, row
+
+
+def _check_exact(q, x):
+    codes, s, row = _read(q)
+    ec, es, er = O.quantize(x, q.fmt)
+    same = (codes == ec) | ((codes & 7) + (ec & 7) == 0)  # +0 and -0 are one value
+    assert same.all(), f"{(~same).sum()} codes differ"
+    assert torch.equal(s[:, : es.shape[1]], es)
+    assert s[:, es.shape[1] :].count_nonzero() == 0, "padded block scales must be zero"
+    torch.testing.assert_close(row, er, rtol=0, atol=0, equal_nan=True)
+    packed = q.codes.cpu().view(q.rows, -1)
+    if packed.shape[1] * 2 > q.cols:  # padding columns
+        tail = torch.stack([packed & 15, packed >> 4], 2).view(q.rows, -1)[:, q.cols :]
+        assert tail.count_nonzero() == 0
+
+
+@pytest.mark.parametrize("fmt", ["nv", "mx"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize(("rows", "cols"), [(1, 1), (1, 16), (3, 17), (129, 32), (33, 255), (257, 256), (5, 512), (130, 1024), (64, 1100),
+                                            (9, 2730), (4, 4864), (3, 6200), (2, 12289), (2, 20000)])
+def test_quantize_is_exact(cuda_device, no_device_error, fmt, dtype, rows, cols):
+    from foidfinder_b200 import fp4
+
+    x = _x(rows, cols, dtype, rows * 7 + cols)
+    q = fp4.quantize(x.to(cuda_device), fmt)
+    _check_exact(q, x)
+    v = O.values(*O.quantize(x, fmt), fmt)
+    for out in (torch.float16, torch.bfloat16, torch.float32):
+        got = fp4.dequantize(q, out).cpu()
+        ref = v.float().to(out)  # code * scale is exact in f32
+        assert torch.equal(got, ref)
+
+
+@pytest.mark.parametrize("fmt", ["nv", "mx"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shift", [0, 1, 2, 3, 5, 8])
+def test_quantize_and_dequantize_any_alignment(cuda_device, no_device_error, fmt, dtype, shift):
+    """Rows that start anywhere inside a 16-byte granule, with NaN around them that must not be read as data."""
+    from foidfinder_b200 import fp4
+
+    rows, cols = 37, 333
+    x = _x(rows, cols, dtype, 3)
+    big = torch.full((rows, cols + 20), math.nan, dtype=dtype, device=cuda_device)
+    view = big[:, shift : shift + cols]
+    view.copy_(x)
+    flat = torch.full((rows * cols + 32,), math.nan, dtype=dtype, device=cuda_device)
+    dense = flat[shift : shift + rows * cols].view(rows, cols)
+    dense.copy_(x)
+    for t in (view, dense):
+        _check_exact(fp4.quantize(t, fmt), x)
+    q = fp4.quantize(x.to(cuda_device), fmt)
+    ref = O.values(*O.quantize(x, fmt), fmt).float().to(dtype)
+    for buf, t in ((big, view), (flat, dense)):
+        before = torch.isnan(buf).sum().item()
+        fp4.dequantize(q, out=t)
+        assert torch.equal(t.cpu(), ref)
+        assert torch.isnan(buf).sum().item() == before  # nothing outside the rows was written
+
+
+@pytest.mark.parametrize("fmt", ["nv", "mx"])
+def test_quantize_special_values(cuda_device, no_device_error, fmt):
+    from foidfinder_b200 import fp4
+
+    x = _x(140, 96, torch.float32, 5)
+    x[0] = 0
+    x[1, :32] = 0
+    x[2] = -0.0
+    x[3] *= 1e-30
+    x[4] *= 1e36
+    x[5] = 2688.0
+    x[6, 0], x[6, 1:] = 2690.0, 1.0
+    x[7, 5] = math.inf
+    x[8, 40] = math.nan
+    x[9, 95] = -math.inf
+    x[10] = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0]).repeat(12)  # ties
+    x[11] = 1e-42  # below the smallest normal number
+    x[12] = torch.finfo(torch.float32).max
+    q = fp4.quantize(x.to(cuda_device), fmt)
+    _check_exact(q, x)
+    v = fp4.dequantize(q, torch.float32).cpu()
+    if fmt == "nv":
+        assert torch.isnan(v[[7, 8, 9]]).all()
+    else:
+        assert torch.isnan(v[7, :32]).all() and torch.isfinite(v[7, 32:]).all()
+        assert torch.isnan(v[8, 32:64]).all() and torch.isnan(v[9, 64:]).all()
+    assert torch.isfinite(v[[0, 1, 2, 3, 4, 5, 6, 10, 11]]).all()
+    # the largest f32 value may round up to a block scale times 6 beyond f32: whatever the codes stand for, in f32
+    assert torch.equal(v[12], O.values(*O.quantize(x, fmt), fmt)[12].float())
+
+
+@pytest.mark.parametrize("fmt", ["nv", "mx"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize(("rows", "cols"), [(1, 768), (130, 1024), (17, 2730), (5, 13000), (3, 33)])
+def test_layernorm_quantize(cuda_device, no_device_error, fmt, dtype, rows, cols):
+    from foidfinder_b200 import fp4
+
+    x = _x(rows, cols, dtype, cols)
+    g = torch.Generator().manual_seed(9)
+    gamma, beta = 1 + 0.1 * torch.randn(cols, generator=g), 0.1 * torch.randn(cols, generator=g)
+    q = fp4.quantize(x.to(cuda_device), fmt, gamma=gamma.to(cuda_device), beta=beta.to(cuda_device), eps=1e-5)
+    codes, s, row = _read(q)
+    ec, es, er = O.quantize(O.layer_norm(x, gamma, beta, 1e-5), fmt)
+    assert torch.equal(row, er)
+    nb = es.shape[1]
+    assert (s[:, :nb].int() - es.int()).abs().max() <= 1 and (s[:, :nb] != es).float().mean() <= 1e-3
+    assert s[:, nb:].count_nonzero() == 0
+    assert (codes != ec).float().mean() <= 1e-3
+
+
+def _operand(rows, cols, fmt, seed, device, std=1.0, dtype=torch.float32):
+    from foidfinder_b200 import fp4
+
+    x = (_x(rows, cols, torch.float32, seed) * std).to(dtype)
+    q = fp4.quantize(x.to(device), fmt)
+    return q, O.values(*O.quantize(x, fmt), fmt)
+
+
+def _product(av, wv, bias):
+    """Exact product, and the error bound of its f32 accumulation."""
+    y = av @ wv.t()
+    steps = -(-av.shape[1] // 64) + 8
+    tol = steps * 2.0**-22 * (av.abs() @ wv.abs().t())
+    if bias is not None:
+        y = y + bias.double()
+        tol = tol + 2.0**-23 * (y.abs() + bias.double().abs())
+    return y, tol
+
+
+def _close(got, ref, tol, dtype):
+    got = got.cpu().double()
+    limit = tol + HALF_ULP[dtype] * (ref.abs() + tol) + TINY[dtype]
+    bad = ~((got - ref).abs() <= limit)
+    assert not bad.any(), f"{bad.sum()} of {bad.numel()} values off, worst {((got - ref).abs() / limit).max():.3g} x the bound"
+
+
+GEMM_SHAPES = [(1, 1, 1), (1, 7, 32), (2, 129, 64), (3, 64, 65), (127, 128, 256), (128, 128, 512), (129, 100, 300), (200, 257, 768),
+               (300, 520, 1100), (257, 333, 2730), (515, 384, 1600)]
+
+
+@pytest.mark.parametrize("tile", [128, 512])
+@pytest.mark.parametrize("fmt", ["nv", "mx"])
+@pytest.mark.parametrize(("M", "N", "K"), GEMM_SHAPES)
+def test_gemm_bias_f32(cuda_device, no_device_error, M, N, K, fmt, tile):
+    from foidfinder_b200 import ops
+
+    A, av = _operand(M, K, fmt, 1, cuda_device)
+    W, wv = _operand(N, K, fmt, 2, cuda_device, 0.02)
+    bias = torch.randn(N, generator=torch.Generator().manual_seed(4)) * 0.1
+    out = torch.full((M, N), math.nan, device=cuda_device)
+    ops.gemm_fp4(A.codes, A.scales, A.row_scale, W.codes, W.scales, W.row_scale, out, ops.EPI_BIAS, FMT[fmt], N=N, K=K,
+                 bias=bias.to(cuda_device), tile=tile)
+    y, tol = _product(av, wv, bias)
+    _close(out, y, tol, torch.float32)
+
+
+@pytest.mark.parametrize("tile", [128, 512])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("epi", ["bias", "nobias", "gelu", "residual", "inplace"])
+@pytest.mark.parametrize(("M", "N", "K", "fmt"), [(1, 9, 48, "nv"), (130, 200, 320, "mx"), (300, 328, 1024, "nv"), (515, 270, 1500, "mx")])
+def test_gemm_16bit_epilogues(cuda_device, no_device_error, M, N, K, fmt, epi, dtype, tile):
+    from foidfinder_b200 import ops
+
+    A, av = _operand(M, K, fmt, 1, cuda_device)
+    W, wv = _operand(N, K, fmt, 2, cuda_device, 0.05)
+    g = torch.Generator().manual_seed(4)
+    bias = None if epi == "nobias" else torch.randn(N, generator=g) * 0.1
+    pitch = (N + 7) // 8 * 8 + 8
+    buf = torch.full((M, pitch), 77.0, device=cuda_device, dtype=dtype)
+    out = buf[:, :N]
+    y, tol = _product(av, wv, bias)
+    kind, residual = ops.EPI_BIAS, None
+    if epi == "gelu":
+        kind = ops.EPI_GELU
+        tol = 1.13 * tol + 2.0**-18 * y.abs()  # |gelu'| <= 1.13
+        y = O.gelu_tanh(y)
+    elif epi in ("residual", "inplace"):
+        kind = ops.EPI_RESIDUAL
+        r = torch.randn(M, N, generator=g).to(dtype)
+        residual = out if epi == "inplace" else torch.zeros(M, pitch + 16, device=cuda_device, dtype=dtype)[:, :N]
+        residual.copy_(r)
+        y = y + r.double()
+        tol = tol + 2.0**-23 * (y.abs() + r.double().abs())
+    ops.gemm_fp4(A.codes, A.scales, A.row_scale, W.codes, W.scales, W.row_scale, out, kind, FMT[fmt], N=N, K=K,
+                 bias=None if bias is None else bias.to(cuda_device), residual=residual, tile=tile)
+    _close(out, y, tol, dtype)
+    assert (buf[:, N:] == 77.0).all(), "columns past N were written"
+
+
+@pytest.mark.parametrize("tile", [128, 512])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize(("M", "H", "K", "fmt"), [(1, 64, 64, "nv"), (129, 100, 256, "mx"), (300, 330, 768, "nv"), (260, 704, 512, "mx")])
+def test_gemm_swiglu(cuda_device, no_device_error, M, H, K, fmt, dtype, tile):
+    from foidfinder_b200 import fp4, ops
+
+    A, av = _operand(M, K, fmt, 1, cuda_device)
+    g = torch.Generator().manual_seed(4)
+    w = torch.randn(2 * H, K, generator=g) * 0.1
+    bias = torch.randn(2 * H, generator=g) * 0.1
+    wv = O.values(*O.quantize(w, fmt), fmt)
+    layer = fp4.Fp4Linear(w.to(cuda_device), bias.to(cuda_device), fmt=fmt, epilogue="swiglu")
+    W = layer.weight
+    out = torch.full((M, (H + 7) // 8 * 8), 77.0, device=cuda_device, dtype=dtype)
+    ops.gemm_fp4(A.codes, A.scales, A.row_scale, W.codes, W.scales, W.row_scale, out[:, :H], ops.EPI_SWIGLU, FMT[fmt], N=layer.rows, K=K,
+                 bias=layer.bias, tile=tile)
+    y, tol = _product(av, wv, bias)
+    gt, up, tg, tu = y[:, :H], y[:, H:], tol[:, :H], tol[:, H:]
+    ref = O.silu_mul(gt, up)
+    silu = O.silu_mul(gt, torch.ones_like(gt))
+    _close(out[:, :H], ref, 1.1 * tg * (up.abs() + tu) + silu.abs() * tu + 2.0**-18 * ref.abs(), dtype)
+    assert (out[:, H:] == 77.0).all()
+
+
+def _tables(tokens, half, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    a = torch.rand(half, tokens, generator=g) * 6.28
+    return a.cos().contiguous(), a.sin().contiguous()
+
+
+@pytest.mark.parametrize("tile", [128, 512])
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+@pytest.mark.parametrize(("M", "qh", "kh", "vh", "K", "tokens", "fmt", "dtype"), [
+    (1, 1, 1, 1, 64, 1, "nv", torch.float16),
+    (131, 4, 2, 2, 256, 50, "mx", torch.bfloat16),
+    (300, 3, 3, 3, 768, 197, "nv", torch.float16),
+])
+def test_gemm_qkv_norm_rope(cuda_device, no_device_error, M, qh, kh, vh, K, tokens, fmt, dtype, norm, tile):
+    from foidfinder_b200 import ops
+
+    d = cuda_device
+    N = 64 * (qh + kh + vh)
+    A, av = _operand(M, K, fmt, 1, d)
+    W, wv = _operand(N, K, fmt, 2, d, 0.05)
+    g = torch.Generator().manual_seed(4)
+    bias = torch.randn(N, generator=g) * 0.1
+    qw, kw = 1 + 0.1 * torch.randn(64, generator=g), 1 + 0.1 * torch.randn(64, generator=g)
+    qb, kb = (0.1 * torch.randn(64, generator=g), 0.1 * torch.randn(64, generator=g)) if norm == "layer" else (None, None)
+    cos, sin = _tables(tokens, 32)
+    dev = lambda t: None if t is None else t.to(d)  # noqa: E731
+    out = torch.full((M, N), math.nan, device=d, dtype=dtype)
+    ops.gemm_fp4(A.codes, A.scales, A.row_scale, W.codes, W.scales, W.row_scale, out, ops.EPI_QKV_NORM_ROPE, FMT[fmt], N=N, K=K, bias=bias.to(d),
+                 tile=tile, norm=norm, q_heads=qh, k_heads=kh, q_weight=dev(qw), k_weight=dev(kw), q_bias=dev(qb), k_bias=dev(kb), qk_eps=1e-6,
+                 rope_cos=dev(cos), rope_sin=dev(sin))
+    y, tol = _product(av, wv, bias)
+    q = O.heads(y[:, : 64 * qh], qh, 64, qw, qb, norm, 1e-6, cos, sin, "pairs")
+    k = O.heads(y[:, 64 * qh : 64 * (qh + kh)], kh, 64, kw, kb, norm, 1e-6, cos, sin, "pairs")
+    ref = torch.cat([q, k, y[:, 64 * (qh + kh) :]], 1)
+    # The norm divides the product's error by the head's rms and spreads it over the head; f32 arithmetic of the norm
+    # and rotation adds 2^-19 of values of order 1.
+    qk = 64 * (qh + kh)
+    h = y[:, :qk].reshape(M, -1, 64)
+    if norm == "layer":
+        h = h - h.mean(-1, keepdim=True)
+    rms = h.square().mean(-1, keepdim=True).sqrt()
+    spread = tol[:, :qk].reshape(M, -1, 64).amax(-1, keepdim=True) / rms * (2 + 2 * (h / rms).abs().amax(-1, keepdim=True))
+    lim = torch.cat([(1.5 * 1.5 * spread + 2.0**-19 * (1 + (h / rms).abs().amax(-1, keepdim=True))).expand(-1, -1, 64).reshape(M, qk), tol[:, qk:]], 1)
+    _close(out, ref, lim, dtype)
+
+
+@pytest.mark.parametrize("rows", [1, 5, 130])
+def test_nan_rows_stay_in_their_rows(cuda_device, no_device_error, rows):
+    """A row with a NaN input is NaN in the output; the other rows are as without it, whatever the padding rows hold."""
+    from foidfinder_b200 import fp4
+
+    x = _x(rows, 300, torch.float16, 2).to(cuda_device)
+    w = _x(96, 300, torch.float32, 3).to(cuda_device)
+    for fmt in ("nv", "mx"):
+        layer = fp4.Fp4Linear(w, fmt=fmt)
+        good = layer(x)
+        y = x.clone()
+        y[rows // 2, 7] = math.nan
+        got = layer(y)
+        keep = torch.arange(rows, device=cuda_device) != rows // 2
+        assert torch.isnan(got[rows // 2]).all()
+        assert torch.equal(got[keep], good[keep])
+
+
+@pytest.mark.parametrize("fmt", ["nv", "mx"])
+def test_linear_is_quantize_then_gemm(cuda_device, no_device_error, fmt):
+    from foidfinder_b200 import fp4, ops
+
+    d = cuda_device
+    M, K, N = 300, 700, 264
+    x = _x(M, K, torch.bfloat16, 2).to(d)
+    g = torch.Generator().manual_seed(4)
+    gamma, beta, bias = (torch.randn(n, generator=g).to(d) for n in (K, K, N))
+    layer = fp4.Fp4Linear(_x(N, K, torch.float32, 3).to(d), bias, fmt=fmt, gamma=gamma, beta=beta)
+    q = fp4.quantize(x, fmt, gamma=gamma, beta=beta)
+    W = layer.weight
+    out = torch.empty(M, N, device=d, dtype=torch.bfloat16)
+    ops.gemm_fp4(q.codes, q.scales, q.row_scale, W.codes, W.scales, W.row_scale, out, ops.EPI_BIAS, FMT[fmt], N=N, K=K, bias=bias)
+    assert torch.equal(layer(x), out)
+    assert torch.equal(layer(x), layer(x))
+
+
+def test_linear_on_another_stream(cuda_device, no_device_error):
+    """Each call's workspace belongs to the stream it runs on: two streams at once give the single-stream results."""
+    from foidfinder_b200 import fp4
+
+    d = cuda_device
+    layer = fp4.Fp4Linear(_x(512, 1024, torch.float32, 3).to(d))
+    xs = [_x(2000, 1024, torch.float16, s).to(d) for s in (1, 2)]
+    ref = [layer(x) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    outs = [[torch.empty(2000, 512, device=d, dtype=torch.float16) for _ in range(8)] for _ in xs]
+    for i in range(8):
+        for s, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                layer(xs[s], out=outs[s][i])
+    torch.cuda.synchronize()
+    for s in range(2):
+        for o in outs[s]:
+            assert torch.equal(o, ref[s])
+
+
+def test_linear_in_a_cuda_graph(cuda_device, no_device_error):
+    from foidfinder_b200 import fp4
+
+    d = cuda_device
+    layer = fp4.Fp4Linear(_x(384, 768, torch.float32, 3).to(d), epilogue="gelu", fmt="mx")
+    x = _x(700, 768, torch.float16, 1).to(d)
+    out = torch.empty(700, 384, device=d, dtype=torch.float16)
+    layer(x, out=out)  # loads the kernels
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        layer(x, out=out)
+    x.copy_(_x(700, 768, torch.float16, 9))
+    g.replay()
+    torch.cuda.synchronize()
+    got = out.clone()
+    layer(x, out=out)
+    assert torch.equal(got, out)
+    del g
+
+
+@pytest.mark.parametrize("pairing", ["pairs", "halves"])
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize(("rows", "qh", "kh", "dim", "tokens"), [(1, 1, 1, 32, 1), (3, 16, 16, 64, 2), (130, 5, 2, 64, 50), (77, 8, 1, 128, 197),
+                                                                (33, 3, 3, 256, 9), (20, 7, 0, 32, 20)])
+def test_qk_norm_rope(cuda_device, no_device_error, rows, qh, kh, dim, tokens, dtype, norm, pairing):
+    from foidfinder_b200 import ops
+
+    d = cuda_device
+    cols = (qh + kh) * dim
+    x = (_x(rows, cols + 16, torch.float32, rows, outliers=False) * 1.5).to(dtype)
+    g = torch.Generator().manual_seed(4)
+    qw, kw = 1 + 0.1 * torch.randn(dim, generator=g), 1 + 0.1 * torch.randn(dim, generator=g)
+    qb, kb = (0.1 * torch.randn(dim, generator=g), 0.1 * torch.randn(dim, generator=g)) if norm == "layer" else (None, None)
+    cos, sin = _tables(tokens, dim // 2)
+    dev = lambda t: None if t is None else t.to(d)  # noqa: E731
+    args = dict(q_heads=qh, k_heads=kh, head_dim=dim, norm=norm, q_weight=dev(qw), k_weight=dev(kw), q_bias=dev(qb), k_bias=dev(kb), eps=1e-6,
+                rope_cos=dev(cos), rope_sin=dev(sin), pairing=pairing)
+    out = torch.full((rows, cols + 8), 77.0, device=d, dtype=dtype)
+    xd = x.to(d)
+    ops.qk_norm_rope(xd, out, **args)
+    q = O.heads(x[:, : qh * dim], qh, dim, qw, qb, norm, 1e-6, cos, sin, pairing)
+    k = O.heads(x[:, qh * dim : cols], kh, dim, kw, kb, norm, 1e-6, cos, sin, pairing)
+    ref = torch.cat([q, k], 1)
+    # f32 arithmetic on values of order |n| <= 10: 2^-20 of the rotated pair's magnitude, then one rounding
+    _close(out[:, :cols], ref, 2.0**-20 * torch.full_like(ref, 10.0), dtype)
+    assert (out[:, cols:] == 77.0).all()
+    ops.qk_norm_rope(xd, xd, **args)
+    assert torch.equal(xd[:, :cols], out[:, :cols]) and torch.equal(xd[:, cols:].cpu(), x[:, cols:])
+
+
+def test_qk_norm_of_zero_and_huge_heads(cuda_device, no_device_error):
+    from foidfinder_b200 import ops
+
+    d = cuda_device
+    x = torch.zeros(4, 128, dtype=torch.bfloat16)
+    x[1] = 1e18  # squares stay below the f32 maximum
+    x[2, :64] = math.nan
+    cos, sin = torch.ones(32, 4), torch.zeros(32, 4)
+    w = torch.ones(64, device=d)
+    out = torch.empty(4, 128, device=d, dtype=torch.bfloat16)
+    ops.qk_norm_rope(x.to(d), out, q_heads=1, k_heads=1, head_dim=64, norm="rms", q_weight=w, k_weight=w, rope_cos=cos.to(d), rope_sin=sin.to(d))
+    got = out.cpu().float()
+    assert (got[0] == 0).all() and (got[1] == 1).all() and (got[3] == 0).all()
+    assert torch.isnan(got[2, :64]).all() and (got[2, 64:] == 0).all()
