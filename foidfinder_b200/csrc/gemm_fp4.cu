@@ -4,12 +4,12 @@
 // they multiply (kind::mxf4nvf4 / kind::mxf4, f32 accumulators in TMEM); the row scales, which are powers of
 // two, and the bias are applied in f32 in the epilogue, which rounds once, to the output's type.
 //
-// One CTA per SM, 320 threads, persistent over tiles:
+// One CTA per SM, 640 threads, persistent over a run of tiles:
 //   warp 0     TMA producer: per stage 256 columns (128 bytes of codes, 128-byte swizzle) of A and W rows and
 //              their scale chunks
 //   warp 1     TMEM allocator; copies each stage's scale chunks to TMEM (tcgen05.cp, in order with the MMAs of
 //              the same thread) and issues the MMAs, 64 columns each
-//   warps 2-9  epilogue: two warps per TMEM lane quarter, one output row per lane
+//   warps 4-19 epilogue: two groups, one per accumulator, one output row per lane
 // Tiles: 128 x 128 per CTA, or (PAIR) 256 x 256 over a cluster of two CTAs, where each CTA loads its 128 rows
 // of A, half of W's 256 rows and all of the tile's W scales (each SM's tensor core reads them from its own
 // TMEM), and shared memory moves half as many bytes per multiply-add.
@@ -22,106 +22,123 @@ namespace ff {
 
 namespace {
 
-template <bool PAIR, bool RES>
+template <bool PAIR>
 struct Fp4Cfg {
   static constexpr int BN = PAIR ? 256 : 128;
   static constexpr int TILE_M = PAIR ? 256 : 128;
-  static constexpr int HALF = BN / 2;  // columns per epilogue warp
+  static constexpr int HALF = BN / 2;  // tile columns per epilogue warp
   static constexpr int CODE_BYTES = 128 * 128;  // 128 rows of A, or of W, per CTA and stage
   static constexpr int SFA_BYTES = 4 * kSfChunk;
   static constexpr int SFB_BYTES = (BN / 128) * 4 * kSfChunk;
   static constexpr int STAGE_BYTES = 2 * CODE_BYTES + SFA_BYTES + SFB_BYTES;
-  static constexpr int STAGES = PAIR || RES ? 4 : 5;
-  static constexpr int EPI_WARPS = 8;
-  static constexpr int THREADS = 64 + 32 * EPI_WARPS;
-  static constexpr int STAGING = RES ? 8192 : 4096;  // per epilogue warp: 32 rows x 128 B, twice with a residual
-  static constexpr int COLP = 2 * HALF * 4;          // per epilogue warp: column scales and biases of its columns
-  static constexpr int NORM_BYTES = 4 * 64 * 4;      // q and k norm weights and biases
+  static constexpr int STAGES = 4;
+  static constexpr int GROUP_WARPS = 8;  // epilogue warps of one accumulator
+  static constexpr int THREADS = 128 + 2 * 32 * GROUP_WARPS;
+  static constexpr int STAGING = 4096;      // per epilogue warp: 32 rows x 128 B
+  static constexpr int COLP = 2 * 64 * 4;   // per epilogue warp: scales and biases of 64 columns
+  static constexpr int NORM_BYTES = 4 * 64 * 4;  // q and k norm weights and biases
   static constexpr int BAR_BYTES = 512;
   static constexpr int SMEM =
-      1024 + STAGES * STAGE_BYTES + EPI_WARPS * (STAGING + COLP) + NORM_BYTES + BAR_BYTES;
-  static constexpr int ACCS = PAIR ? 1 : 2;
+      1024 + STAGES * STAGE_BYTES + 2 * GROUP_WARPS * (STAGING + COLP) + NORM_BYTES + BAR_BYTES;
+  // TMEM: two accumulators and two buffers of scales, each for one chunk of A's and W's columns. Two 256-column
+  // accumulators and the scales do not fit 512 columns: the pair's accumulators share 32 columns, the last of
+  // the first and the first of the second, which the epilogue empties first.
   static constexpr uint32_t TMEM_COLS = 512;
-  static constexpr uint32_t SF_BASE = 256;               // TMEM column of the scales
-  static constexpr uint32_t SF_COLS = 16 + 4 * (BN / 32);  // per stage: A's, then W's
+  static constexpr uint32_t ACC_STRIDE = PAIR ? 224 : 128;
+  static constexpr uint32_t SFA_BASE = 480, SFB_BASE = 488;  // + 4 and + BN / 32 columns per buffer
   static_assert(STAGE_BYTES % 1024 == 0, "stages keep the swizzle's alignment");
+  static_assert(ACC_STRIDE + BN <= SFA_BASE && SFB_BASE + 2 * (BN / 32) <= TMEM_COLS, "TMEM");
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
-// tanh GELU: x * sigmoid(2 sqrt(2 / pi) (x + 0.044715 x^3)), MUFU ex2 and rcp (a few ulp).
-__device__ __forceinline__ float gelu_sigmoid(float x) {
-  const float t = -2.302208198f * (x + 0.044715f * x * x * x);  // -2 sqrt(2 / pi) log2 e
+// 1 / (1 + 2^t) on two lanes with three MUFU operations instead of four: one reciprocal of the product of both
+// denominators (t <= 62, so that the product stays finite; the result is then at least 2^-62).
+__device__ __forceinline__ float2 sigmoid2(float2 t) {
+  const float2 d = add2(make_float2(1.f, 1.f), make_float2(ex2_approx(fminf(t.x, 62.f)), ex2_approx(fminf(t.y, 62.f))));
   float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + ex2_approx(fminf(t, 126.f))));
-  return x * r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d.x * d.y));
+  return mul2(make_float2(r, r), make_float2(d.y, d.x));
+}
+// silu(g) * u.
+__device__ __forceinline__ float2 silu_up2(float2 g, float2 u) {
+  return mul2(mul2(g, u), sigmoid2(mul2(g, make_float2(-1.4426950408889634f, -1.4426950408889634f))));
+}
+// tanh GELU: x * sigmoid(2 sqrt(2 / pi) (x + 0.044715 x^3)).
+__device__ __forceinline__ float2 gelu2(float2 x) {
+  constexpr float c1 = -2.302208198f, c3 = -2.302208198f * 0.044715f;  // times -2 sqrt(2 / pi) log2 e
+  return mul2(x, sigmoid2(mul2(x, fma2(mul2(x, x), make_float2(c3, c3), make_float2(c1, c1)))));
 }
 
-// y[j] = acc[j] * (rs * cs[j]) + bias[j]; cs and bias in shared memory (read by every lane at once).
-__device__ __forceinline__ void scale32(const uint32_t (&r)[32], float rs, const float* cs, const float* bias,
-                                        float (&y)[32]) {
+// r[j] = r[j] * (rs * cs[j]) + bias[j] for N accumulators in place (as f32 bits); cs and bias in shared memory, read
+// by every lane at once.
+template <int N>
+__device__ __forceinline__ void scale_cols(uint32_t* r, float rs, const float* cs, const float* bias) {
   const float2 rs2 = make_float2(rs, rs);
 #pragma unroll
-  for (int j = 0; j < 32; j += 4) {
+  for (int j = 0; j < N; j += 4) {
     const float4 c = *reinterpret_cast<const float4*>(cs + j);
     const float4 b = *reinterpret_cast<const float4*>(bias + j);
     const float2 lo = fma2(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])),
                            mul2(rs2, make_float2(c.x, c.y)), make_float2(b.x, b.y));
     const float2 hi = fma2(make_float2(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3])),
                            mul2(rs2, make_float2(c.z, c.w)), make_float2(b.z, b.w));
-    y[j] = lo.x;
-    y[j + 1] = lo.y;
-    y[j + 2] = hi.x;
-    y[j + 3] = hi.y;
+    r[j] = __float_as_uint(lo.x);
+    r[j + 1] = __float_as_uint(lo.y);
+    r[j + 2] = __float_as_uint(hi.x);
+    r[j + 3] = __float_as_uint(hi.y);
   }
 }
+// Keeps the compiler from starting a later group's loads early: the epilogue has registers for one group.
+__device__ __forceinline__ void group_end() { asm volatile("" ::: "memory"); }
 
-// The scale copies and MMAs of one stage.
+// The scale copies and MMAs of one stage: chunk g of the scales goes to buffer g % 2, in order with the MMAs that
+// read it.
 template <bool PAIR, bool MX, class C>
-__device__ __forceinline__ void fp4_stage_mmas(uint32_t d, uint32_t sa, uint32_t sf, int steps, bool first) {
+__device__ __forceinline__ void fp4_stage_mmas(uint32_t d, uint32_t tmem, uint32_t sa, int steps, bool first) {
   constexpr int CH = sf_chunks_per_step(MX);
-  const uint32_t sfa = sf, sfb = sf + 16;
-  const uint32_t ssa = sa + 2 * C::CODE_BYTES, ssb = ssa + C::SFA_BYTES;
   constexpr int BT = C::BN / 128;
-#pragma unroll
-  for (int g = 0; g < CH; ++g) {
-    tc_cp_sf<PAIR>(sfa + 4 * g, sdesc_sf(ssa + g * kSfChunk));
-#pragma unroll
-    for (int t = 0; t < BT; ++t) tc_cp_sf<PAIR>(sfb + 4 * BT * g + 4 * t, sdesc_sf(ssb + (t * CH + g) * kSfChunk));
-  }
+  const uint32_t ssa = sa + 2 * C::CODE_BYTES, ssb = ssa + C::SFA_BYTES;
   const uint64_t adesc = sdesc_k_sw128(sa), bdesc = sdesc_k_sw128(sa + C::CODE_BYTES);
   constexpr uint32_t idesc = idesc_fp4(C::TILE_M, C::BN, MX);
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     if (k < steps) {
       const int g = MX ? k / 2 : k;
-      mma_fp4<PAIR, MX>(d, adesc + 2 * k, bdesc + 2 * k, idesc | (MX ? idesc_sf_id((k & 1) * 2) : 0u), sfa + 4 * g,
-                        sfb + 4 * BT * g, !(first && k == 0));
+      const uint32_t sfa = tmem + C::SFA_BASE + (g & 1) * 4, sfb = tmem + C::SFB_BASE + (g & 1) * (C::BN / 32);
+      if (!MX || (k & 1) == 0) {
+        tc_cp_sf<PAIR>(sfa, sdesc_sf(ssa + g * kSfChunk));
+#pragma unroll
+        for (int t = 0; t < BT; ++t) tc_cp_sf<PAIR>(sfb + 4 * t, sdesc_sf(ssb + (t * CH + g) * kSfChunk));
+      }
+      mma_fp4<PAIR, MX>(d, adesc + 2 * k, bdesc + 2 * k, idesc | (MX ? idesc_sf_id((k & 1) * 2) : 0u), sfa, sfb,
+                        !(first && k == 0));
     }
   }
 }
 
 template <bool PAIR, int EPI, class OutT>
-__global__ void __launch_bounds__(Fp4Cfg<PAIR, EPI == EPI_RESIDUAL>::THREADS, 1)
+__global__ void __launch_bounds__(Fp4Cfg<PAIR>::THREADS, 1)
     gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
                     const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSW,
                     const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmR,
                     const Fp4GemmArgs args) {
   constexpr bool RES = EPI == EPI_RESIDUAL;
   constexpr bool F32OUT = sizeof(OutT) == 4;
-  using C = Fp4Cfg<PAIR, RES>;
+  using C = Fp4Cfg<PAIR>;
   constexpr int STAGES = C::STAGES, BN = C::BN, HALF = C::HALF;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* staging = smem + STAGES * C::STAGE_BYTES;
-  float* colp = reinterpret_cast<float*>(staging + C::EPI_WARPS * C::STAGING);
-  float* normp = colp + C::EPI_WARPS * 2 * HALF;  // q weight, q bias, k weight, k bias
+  float* colp = reinterpret_cast<float*>(staging + 2 * C::GROUP_WARPS * C::STAGING);
+  float* normp = colp + 2 * C::GROUP_WARPS * (C::COLP / 4);  // q weight, q bias, k weight, k bias
   uint64_t* full = reinterpret_cast<uint64_t*>(normp + 4 * 64);
   uint64_t* empty = full + STAGES;
   uint64_t* tfull = empty + STAGES;
-  uint64_t* tempty = tfull + C::ACCS;
-  uint64_t* drain = tempty + C::ACCS;
-  uint64_t* resbar = drain + 1;  // two per epilogue warp (EPI_RESIDUAL)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(resbar + 2 * C::EPI_WARPS);
+  uint64_t* tempty = tfull + 2;  // an accumulator has been read
+  uint64_t* tearly = tempty + 2;  // PAIR: the columns that it shares with the other one have been read
+  uint64_t* drain = tearly + 2;
+  uint64_t* resbar = drain + 1;  // one per epilogue warp (EPI_RESIDUAL)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(resbar + 2 * C::GROUP_WARPS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -131,6 +148,9 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR, EPI == EPI_RESIDUAL>::THREADS, 1)
   const bool leader = rank == 0;
   const int unit = PAIR ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
   const int units = PAIR ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
+  // A run of tiles along N: consecutive tiles share their rows of A.
+  const int t_begin = static_cast<int>(static_cast<int64_t>(unit) * tiles / units);
+  const int t_end = static_cast<int>(static_cast<int64_t>(unit + 1) * tiles / units);
   auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
     if constexpr (PAIR)
       return mbar_wait_cluster<true>(bar, parity, abort_flag, args.err, code);
@@ -143,12 +163,13 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR, EPI == EPI_RESIDUAL>::THREADS, 1)
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    for (int a = 0; a < C::ACCS; ++a) {
+    for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull[a], 1);
-      mbar_init(&tempty[a], (PAIR ? 2 : 1) * C::EPI_WARPS);
+      mbar_init(&tempty[a], (PAIR ? 2 : 1) * C::GROUP_WARPS);
+      mbar_init(&tearly[a], 2 * C::GROUP_WARPS / 2);
     }
     mbar_init(drain, 1);
-    for (int i = 0; i < 2 * C::EPI_WARPS; ++i) mbar_init(&resbar[i], 1);
+    for (int i = 0; i < 2 * C::GROUP_WARPS; ++i) mbar_init(&resbar[i], 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -173,10 +194,9 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR, EPI == EPI_RESIDUAL>::THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_trigger();
-
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
-    if (lane == 0) {
+    if (elect_one()) {
       int stage = 0;
       uint32_t phase = 0;
       int last_phase[STAGES];
@@ -214,14 +234,14 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR, EPI == EPI_RESIDUAL>::THREADS, 1)
         if (PAIR && leader) mbar_arrive_expect_tx(bar, 2 * stage_bytes);
       };
       // With w_const the weights of the first stages come in before the wait for the previous kernel.
-      const int pre = (args.w_const && unit < tiles) ? (args.num_kb < STAGES ? args.num_kb : STAGES) : 0;
+      const int pre = args.w_const ? (args.num_kb < STAGES ? args.num_kb : STAGES) : 0;
       for (int kb = 0; kb < pre; ++kb) {
         expect(&full[kb]);
-        load_w(smem + kb * C::STAGE_BYTES, &full[kb], kb, unit % tiles_n);
+        load_w(smem + kb * C::STAGE_BYTES, &full[kb], kb, t_begin % tiles_n);
       }
       pdl_wait();
       bool ok = true, first = true;
-      for (int t = unit; t < tiles && ok; t += units) {
+      for (int t = t_begin; t < t_end && ok; ++t) {
         const int tm = t / tiles_n, tn = t % tiles_n;
         for (int kb = 0; kb < args.num_kb; ++kb) {
           uint8_t* sa = smem + stage * C::STAGE_BYTES;
@@ -255,8 +275,11 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR, EPI == EPI_RESIDUAL>::THREADS, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ scale copies and MMAs (the even CTA of a pair)
+    // One elected lane (elect.sync): the compiler then knows that the operands of the tcgen05 instructions are
+    // uniform. With a lane == 0 branch each instruction cost 50-60 cycles to issue and the issue rate bound the
+    // kernel (8192^3 FF_FP4_NV: pair tiles 367 -> 215 us, 128 x 128 tiles 510 -> 273 us).
     pdl_wait();
-    if (lane == 0 && leader) {
+    if (leader && elect_one()) {
       auto commit_both = [&](uint64_t* bar) {
         if constexpr (PAIR)
           tc_commit2_both(bar);
@@ -265,16 +288,14 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR, EPI == EPI_RESIDUAL>::THREADS, 1)
       };
       int stage = 0;
       uint32_t phase = 0;
-      int acc = 0;
-      uint32_t acc_phase = 0, sf_buf = 0;
       bool ok = true;
-      for (int t = unit; t < tiles && ok; t += units) {
-        if (!wait(&tempty[acc], acc_phase ^ 1u, kDevTimeoutTmemEmpty)) {
-          ok = false;
-          break;
-        }
+      for (int t = t_begin; t < t_end && ok; ++t) {
+        const int i = t - t_begin;
+        const uint32_t acc = i & 1, use = (i >> 1) & 1;
+        if (!wait(&tempty[acc], use ^ 1u, kDevTimeoutTmemEmpty)) break;
+        if (PAIR && i > 0 && !wait(&tearly[acc ^ 1u], ((i - 1) >> 1) & 1, kDevTimeoutTmemEmpty)) break;
         tc_fence_after();
-        const uint32_t d = tmem + static_cast<uint32_t>(acc * BN);
+        const uint32_t d = tmem + acc * C::ACC_STRIDE;
         for (int kb = 0; kb < args.num_kb; ++kb) {
           if (!wait(&full[stage], phase, kDevTimeoutTmaFull)) {
             ok = false;
@@ -282,14 +303,12 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR, EPI == EPI_RESIDUAL>::THREADS, 1)
           }
           tc_fence_after();
           const uint32_t sa = smem_u32(smem + stage * C::STAGE_BYTES);
-          const uint32_t sf = tmem + C::SF_BASE + sf_buf * C::SF_COLS;
           const int left = (args.K - kb * kFp4Step + 63) >> 6;  // 64-column steps to the end of the row
           if (args.mx)
-            fp4_stage_mmas<PAIR, true, C>(d, sa, sf, left, kb == 0);
+            fp4_stage_mmas<PAIR, true, C>(d, tmem, sa, left, kb == 0);
           else
-            fp4_stage_mmas<PAIR, false, C>(d, sa, sf, left, kb == 0);
+            fp4_stage_mmas<PAIR, false, C>(d, tmem, sa, left, kb == 0);
           commit_both(&empty[stage]);
-          sf_buf ^= 1u;
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1u;
@@ -297,10 +316,6 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR, EPI == EPI_RESIDUAL>::THREADS, 1)
         }
         if (!ok) break;
         commit_both(&tfull[acc]);
-        if (++acc == C::ACCS) {
-          acc = 0;
-          acc_phase ^= 1u;
-        }
       }
       // Drain: every MMA this thread issued must finish before TMEM is released.
       if constexpr (PAIR)
@@ -316,265 +331,274 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR, EPI == EPI_RESIDUAL>::THREADS, 1)
         }
       }
     }
-  } else {
+  } else if (warp >= 4) {
     // ------------------------------------------------------------ epilogue
+    // Two groups of eight warps, one per accumulator, take turns with the tiles: a group has the time of two
+    // mainloops for a tile. A warp reads one lane quarter (32 rows) and half of the tile's columns, 32 at a time.
     pdl_wait();
-    const int ew = warp - 2;
-    const int q = warp & 3;    // TMEM lane quarter
-    const int half = ew >> 2;  // which half of the tile's columns
+    const int ew = warp - 4;
+    const int acc = ew >> 3;         // group
+    const int q = warp & 3;          // TMEM lane quarter
+    const int half = (ew >> 2) & 1;  // of the tile's columns
     uint8_t* const stg = staging + ew * C::STAGING;
-    float* const cs_s = colp + ew * 2 * HALF;
-    float* const b_s = cs_s + HALF;
-    constexpr bool SPLIT = EPI == EPI_SWIGLU && BN == 128;  // the warp's columns: 32 gates and their 32 ups
+    float* const cs_s = colp + ew * (C::COLP / 4);
+    float* const b_s = cs_s + 64;
     if constexpr (EPI == EPI_QKV_NORM_ROPE) {
-      for (int i = threadIdx.x - 64; i < 64; i += 256) {
+      for (int i = threadIdx.x - 128; i < 64; i += 2 * 32 * C::GROUP_WARPS) {
         normp[i] = args.q_w[i];
         normp[64 + i] = args.q_b != nullptr ? args.q_b[i] : 0.f;
         normp[128 + i] = args.k_w[i];
         normp[192 + i] = args.k_b != nullptr ? args.k_b[i] : 0.f;
       }
-      asm volatile("bar.sync 1, 256;" ::: "memory");  // the eight epilogue warps
+      asm volatile("bar.sync 1, %0;" ::"n"(2 * 32 * C::GROUP_WARPS) : "memory");  // the epilogue warps
     }
-    int acc = 0;
-    uint32_t acc_phase = 0;
-    uint32_t res_phase[2] = {0, 0};
-    bool ok = true;
-    for (int t = unit; t < tiles; t += units) {
-      const int tm = t / tiles_n, tn = t % tiles_n;
+    constexpr bool SWIGLU = EPI == EPI_SWIGLU;
+    constexpr int STEPS = HALF / 64;           // 64 tile columns per step
+    constexpr int WIDTH = SWIGLU ? 32 : 64;    // output columns per step
+    uint32_t use = 0, res_phase = 0;
+    for (int t = t_begin + acc; t < t_end; t += 2, use ^= 1u) {
+      const int tm = t / tiles_n, tn = t - tm * tiles_n;
       const int m_block = tm * C::TILE_M + static_cast<int>(rank) * 128 + q * 32;
       const int m = m_block + lane;
       const bool row_ok = m < args.M;
-      const bool any = m_block < args.M;  // some row of this warp is real
       const int n_tile = tn * BN;
-      // Column scales and biases of this warp's columns (zero past N), row scale and rotation angles: read
-      // before the wait for the accumulator.
-      __syncwarp();
-      for (int i = lane; i < HALF; i += 32) {
-        const int n = n_tile + (SPLIT ? (i < 32 ? half * 32 + i : 32 + half * 32 + i) : half * HALF + i);
-        const bool in = n < args.N;
-        cs_s[i] = in ? (args.col_scale != nullptr ? __ldg(args.col_scale + n) : 1.f) : 0.f;
-        b_s[i] = in && args.bias != nullptr ? __ldg(args.bias + n) : 0.f;
-      }
-      __syncwarp();
       const float rs = row_ok ? (args.row_scale != nullptr ? __ldg(args.row_scale + m) : 1.f) : 0.f;
-      float rope_c[EPI == EPI_QKV_NORM_ROPE ? 32 : 1], rope_s[EPI == EPI_QKV_NORM_ROPE ? 32 : 1];
-      if constexpr (EPI == EPI_QKV_NORM_ROPE) {
-        if (n_tile + half * HALF < 64 * (args.q_heads + args.k_heads)) {
-          const int pos = (row_ok ? m : 0) % args.tokens;
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            rope_c[j] = __ldg(args.rope_cos + static_cast<int64_t>(j) * args.tokens + pos);
-            rope_s[j] = __ldg(args.rope_sin + static_cast<int64_t>(j) * args.tokens + pos);
-          }
-        }
-      }
-      if constexpr (RES) {
-        // The first chunk of the residual comes in while the mainloop runs.
-        if (any && lane == 0) {
-          bulk_wait_read_all();
-          mbar_arrive_expect_tx(&resbar[2 * ew], 4096);
-          tma_load_2d(stg, &tmR, &resbar[2 * ew], n_tile + half * HALF, m_block);
-        }
-      }
-      if (!wait(&tfull[acc], acc_phase, kDevTimeoutTmemFull)) {
-        ok = false;
-        if constexpr (RES) {  // let the residual copy land before the CTA exits
-          if (any && lane == 0) mbar_wait(&resbar[2 * ew], res_phase[0], abort_flag, args.err, kDevTimeoutDrain);
-        }
-        break;
-      }
-      tc_fence_after();
-      const uint32_t tbase = tmem + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * BN);
-      // A TMA store clips its box to whole 16-byte granules of a row: the last out_cols % 8 columns, when they lie
-      // in the 16-bit columns [n0, n0 + width) that this lane has staged, are written one by one.
-      auto store_ragged = [&](int n0, int width, uint4 u) {
-        const int c = args.tma_cols, left = args.out_cols - c;
-        if (left == 0 || c < n0 || c >= n0 + width || !row_ok) return;
-        uint16_t* dst = static_cast<uint16_t*>(args.out) + static_cast<int64_t>(m) * args.ldo + c;
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int e = 0; e < 7; ++e)
-          if (e < left) dst[e] = static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1)));
-      };
-      if (any) {
-        if constexpr (F32OUT) {
-          float* const out = static_cast<float*>(args.out);
-          const int rows = args.M - m_block < 32 ? args.M - m_block : 32;
+      const uint32_t tbase = tmem + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc) * C::ACC_STRIDE;
+      bool ok = true;
 #pragma unroll 1
-          for (int c = 0; c < HALF; c += 32) {
-            const int n0 = n_tile + half * HALF + c;
-            if (n0 >= args.N) break;
-            uint32_t r[32];
-            __syncwarp();
-            tmem_ld32(tbase + half * HALF + c, r);
-            tmem_ld_wait();
-            float y[32];
-            scale32(r, rs, cs_s + c, b_s + c, y);
+      for (int step = 0; step < STEPS; ++step) {
+        // The first group goes from the last columns down, the second from the first columns up, so that each
+        // begins with the columns that the accumulators share. ca, cb: the step's first and second 32 tile
+        // columns, neighbours or 32 gates and their 32 ups.
+        const int at = acc == 0 ? STEPS - 1 - step : step;
+        const int ca = SWIGLU ? (PAIR ? half * 128 + at * 32 : half * 32) : half * HALF + at * 64;
+        const int cb = ca + (SWIGLU ? 64 : 32);
+        const int out0 = SWIGLU ? (n_tile >> 1) + (PAIR ? half * 64 + at * 32 : half * 32) : n_tile + ca;
+        const bool any = m_block < args.M && out0 < args.out_cols;  // the warp has something to write
+        __syncwarp();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(y[j]);
-            stage_row128(stg, lane, r);
-            __syncwarp();
-            for (int i = 0; i < rows; ++i)  // one row of 32 columns per store: any row stride and column count
-              if (n0 + lane < args.N)
-                out[static_cast<int64_t>(m_block + i) * args.ldo + n0 + lane] =
-                    *reinterpret_cast<const float*>(stg + i * 128 + (((lane >> 2) ^ (i & 7)) << 4) + (lane & 3) * 4);
-          }
-        } else if constexpr (EPI == EPI_SWIGLU) {
-          constexpr int OUTS = BN == 256 ? 64 : 32;  // output columns per warp
-          const int col0 = (n_tile >> 1) + half * OUTS;
-          if (lane == 0) bulk_wait_read_all();
-          __syncwarp();
-#pragma unroll
-          for (int sub = 0; sub < OUTS / 32; ++sub) {
-            uint32_t rg[32], ru[32];
-            const int ig = SPLIT ? 0 : sub * 32, iu = SPLIT ? 32 : 64 + sub * 32;  // among the warp's columns
-            const int cg = SPLIT ? half * 32 : half * 128 + sub * 32;
-            __syncwarp();
-            tmem_ld32(tbase + cg, rg);
-            tmem_ld32(tbase + cg + 64, ru);
-            tmem_ld_wait();
-            float g[32], u[32];
-            scale32(rg, rs, cs_s + ig, b_s + ig, g);
-            scale32(ru, rs, cs_s + iu, b_s + iu, u);
-            uint32_t packed[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const float2 h = silu_mul2(make_float2(g[2 * j], g[2 * j + 1]), make_float2(u[2 * j], u[2 * j + 1]));
-              packed[j] = Pair16<OutT>::pack(h.x, h.y);
+        for (int i = 0; i < 2; ++i) {
+          const int n = n_tile + (i ? cb : ca) + lane;
+          const bool in = n < args.N;
+          cs_s[32 * i + lane] = in ? (args.col_scale != nullptr ? __ldg(args.col_scale + n) : 1.f) : 0.f;
+          b_s[32 * i + lane] = in && args.bias != nullptr ? __ldg(args.bias + n) : 0.f;
+        }
+        if (lane == 0) {
+          if constexpr (!F32OUT) bulk_wait_read_all();  // the staging buffer is free
+          if constexpr (RES) {
+            if (any) {  // the residual comes in while the mainloop runs
+              mbar_arrive_expect_tx(&resbar[ew], C::STAGING);
+              tma_load_2d(stg, &tmR, &resbar[ew], out0, m_block);
             }
-            if constexpr (OUTS == 64)
-              stage_half_row128(stg, lane, sub, packed);
+          }
+        }
+        __syncwarp();
+        if (step == 0) {
+          ok = wait(&tfull[acc], use, kDevTimeoutTmemFull);
+          if (!ok) {
+            if constexpr (RES) {  // let the residual copy land before the CTA exits
+              if (any) mbar_wait(&resbar[ew], res_phase, abort_flag, args.err, kDevTimeoutDrain);
+            }
+            break;
+          }
+          tc_fence_after();
+        }
+        // Hand back the shared columns (step 0), or the whole accumulator: every read of them has completed.
+        auto arrive = [&](uint64_t* bar) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if (PAIR && !leader)
+              mbar_arrive_cluster(mapa_shared(smem_u32(bar), 0u));
             else
-              stage_row64(stg, lane, packed);
+              mbar_arrive(bar);
           }
-          fence_async_smem();
+        };
+        auto arrive_early = [&]() {
+          if (PAIR && step == 0 && half != acc) arrive(&tearly[acc]);
+        };
+        auto arrive_empty = [&]() {
+          if (step == STEPS - 1) arrive(&tempty[acc]);
+        };
+        auto read32 = [&](int col, uint32_t(&r)[32]) {
           __syncwarp();
-          if (lane == 0 && col0 < args.tma_cols) {
-            tma_store_2d(&tmC, stg, col0, m_block);
-            bulk_commit_group();
+          if (any) {
+            tmem_ld32(tbase + col, r);
+            tmem_ld_wait();
           }
-          const int rc = (args.tma_cols - col0) >> 3;
-          store_ragged(col0, OUTS, OUTS == 64 ? staged_chunk128(stg, lane, rc & 7) : staged_chunk64(stg, lane, rc & 3));
-        } else {
-#pragma unroll
-          for (int ch = 0; ch < HALF / 64; ++ch) {
-            const int c0 = half * HALF + ch * 64;
-            const int n0 = n_tile + c0;
-            uint8_t* const buf = stg + (RES ? (ch & 1) * 4096 : 0);
-            if constexpr (RES) {
-              // The next chunk's residual into the other buffer, then this chunk's.
-              if (lane == 0 && ch + 1 < HALF / 64) {
-                bulk_wait_read_all();
-                mbar_arrive_expect_tx(&resbar[2 * ew + ((ch + 1) & 1)], 4096);
-                tma_load_2d(stg + ((ch + 1) & 1) * 4096, &tmR, &resbar[2 * ew + ((ch + 1) & 1)], n0 + 64, m_block);
-              }
-              if (!mbar_wait(&resbar[2 * ew + (ch & 1)], res_phase[ch & 1], abort_flag, args.err, kDevTimeoutTmaFull))
-                ok = false;
-              res_phase[ch & 1] ^= 1u;
-            } else {
-              if (lane == 0) bulk_wait_read_all();
+        };
+        auto wait_residual = [&]() {
+          if constexpr (RES) {
+            if (any) {
+              ok = mbar_wait(&resbar[ew], res_phase, abort_flag, args.err, kDevTimeoutTmaFull);
+              res_phase ^= 1u;
+              __syncwarp();
             }
-            __syncwarp();
-            if constexpr (EPI == EPI_QKV_NORM_ROPE) {
-              // A chunk is one head of 64 columns.
-              float y[64];
+          }
+        };
+        // Eight 16-bit output columns, at 16-byte slot g of the lane's staged row.
+        auto stage8 = [&](int g, const float(&y)[8]) {
+          if constexpr (!F32OUT) {
+            uint4* const slot = reinterpret_cast<uint4*>(
+                SWIGLU ? stg + lane * 64 + ((g ^ ((lane >> 1) & 3)) << 4) : stg + lane * 128 + ((g ^ (lane & 7)) << 4));
+            float z[8];
 #pragma unroll
+            for (int j = 0; j < 8; ++j) z[j] = y[j];
+            if constexpr (RES) {
+              const uint4 u = *slot;
+              const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float2 f = Pair16<OutT>::unpack(w[j]);
+                z[2 * j] += f.x;
+                z[2 * j + 1] += f.y;
+              }
+            }
+            *slot = make_uint4(Pair16<OutT>::pack(z[0], z[1]), Pair16<OutT>::pack(z[2], z[3]),
+                               Pair16<OutT>::pack(z[4], z[5]), Pair16<OutT>::pack(z[6], z[7]));
+            group_end();
+          }
+        };
+        if constexpr (SWIGLU) {
+          uint32_t rg[32], ru[32];
+          if (acc == 0)  // the shared ones first
+            read32(cb, ru);
+          else
+            read32(ca, rg);
+          arrive_early();
+          if (acc == 0)
+            read32(ca, rg);
+          else
+            read32(cb, ru);
+          arrive_empty();
+          if (!any) continue;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            scale_cols<8>(rg + 8 * g, rs, cs_s + 8 * g, b_s + 8 * g);
+            scale_cols<8>(ru + 8 * g, rs, cs_s + 32 + 8 * g, b_s + 32 + 8 * g);
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+              const int k = 8 * g + j;
+              const float2 h = silu_up2(make_float2(__uint_as_float(rg[k]), __uint_as_float(rg[k + 1])),
+                                        make_float2(__uint_as_float(ru[k]), __uint_as_float(ru[k + 1])));
+              y[j] = h.x;
+              y[j + 1] = h.y;
+            }
+            stage8(g, y);
+          }
+        } else {
+          // The head norm's statistics first, from reads of their own: the accumulator is read again below.
+          const int head = out0 >> 6;
+          float mean = 0.f, rstd = 1.f;
+          const bool qk = EPI == EPI_QKV_NORM_ROPE && any && head < args.q_heads + args.k_heads;
+          if constexpr (EPI == EPI_QKV_NORM_ROPE) {
+            auto over_head = [&](auto f) {
+#pragma unroll 1
               for (int sub = 0; sub < 2; ++sub) {
                 uint32_t r[32];
-                __syncwarp();
-                tmem_ld32(tbase + c0 + sub * 32, r);
-                tmem_ld_wait();
-                float h[32];
-                scale32(r, rs, cs_s + ch * 64 + sub * 32, b_s + ch * 64 + sub * 32, h);
+                read32(ca + 32 * sub, r);
+                scale_cols<32>(r, rs, cs_s + 32 * sub, b_s + 32 * sub);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) y[sub * 32 + j] = h[j];
+                for (int j = 0; j < 32; ++j) f(__uint_as_float(r[j]));
               }
-              const int head = n0 >> 6;
-              if (head < args.q_heads + args.k_heads) {
-                const float* w = normp + (head < args.q_heads ? 0 : 128);
-                float mean = 0.f;
-                if (args.norm == FF_NORM_LAYER) {
-#pragma unroll
-                  for (int j = 0; j < 64; ++j) mean += y[j];
-                  mean *= 1.f / 64.f;
-                }
-                float ss = 0.f;
-#pragma unroll
-                for (int j = 0; j < 64; ++j) {
-                  y[j] -= mean;
-                  ss = fmaf(y[j], y[j], ss);
-                }
-                const float rstd = rsqrtf(ss * (1.f / 64.f) + args.qk_eps);
-#pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                  const float x0 = fmaf(y[2 * j] * rstd, w[2 * j], w[64 + 2 * j]);
-                  const float x1 = fmaf(y[2 * j + 1] * rstd, w[2 * j + 1], w[64 + 2 * j + 1]);
-                  y[2 * j] = x0 * rope_c[j] - x1 * rope_s[j];
-                  y[2 * j + 1] = x0 * rope_s[j] + x1 * rope_c[j];
-                }
+            };
+            if (qk) {
+              if (args.norm == FF_NORM_LAYER) {
+                over_head([&](float v) { mean += v; });
+                mean *= 1.f / 64.f;
               }
-#pragma unroll
-              for (int sub = 0; sub < 2; ++sub) {
-                uint32_t packed[16];
-#pragma unroll
-                for (int j = 0; j < 16; ++j) packed[j] = Pair16<OutT>::pack(y[sub * 32 + 2 * j], y[sub * 32 + 2 * j + 1]);
-                stage_half_row128(buf, lane, sub, packed);
-              }
+              float ss = 0.f;
+              over_head([&](float v) { ss = fmaf(v - mean, v - mean, ss); });
+              rstd = rsqrtf(ss * (1.f / 64.f) + args.qk_eps);
+            }
+          }
+#pragma unroll 1
+          for (int i = 0; i < 2; ++i) {
+            const int sub = acc == 0 ? 1 - i : i;  // the shared columns first
+            uint32_t r[32];
+            read32(ca + 32 * sub, r);
+            if (i == 0) {
+              arrive_early();
+              wait_residual();
             } else {
+              arrive_empty();
+            }
+            if (!any) continue;
+            const float *cs = cs_s + 32 * sub, *bs = b_s + 32 * sub;
+            if constexpr (F32OUT) {
+              float* const out = static_cast<float*>(args.out);
+              const int rows = args.M - m_block < 32 ? args.M - m_block : 32;
+              scale_cols<32>(r, rs, cs, bs);
+              stage_row128(stg, lane, r);
+              __syncwarp();
+              const int n = out0 + 32 * sub + lane;
+              for (int k = 0; k < rows; ++k)  // one row of 32 columns per store: any row stride and column count
+                if (n < args.N)
+                  out[static_cast<int64_t>(m_block + k) * args.ldo + n] =
+                      *reinterpret_cast<const float*>(stg + k * 128 + (((lane >> 2) ^ (k & 7)) << 4) + (lane & 3) * 4);
+              __syncwarp();
+            } else {
+              float rc[EPI == EPI_QKV_NORM_ROPE ? 16 : 1], rn[EPI == EPI_QKV_NORM_ROPE ? 16 : 1];
+              if constexpr (EPI == EPI_QKV_NORM_ROPE) {
+                if (qk) {
+                  const int64_t at0 = static_cast<int64_t>(16 * sub) * args.tokens + (row_ok ? m : 0) % args.tokens;
+                  const float *cp = args.rope_cos + at0, *sp = args.rope_sin + at0;
 #pragma unroll
-              for (int sub = 0; sub < 2; ++sub) {
-                uint32_t r[32];
-                __syncwarp();
-                tmem_ld32(tbase + c0 + sub * 32, r);
-                tmem_ld_wait();
-                float y[32];
-                scale32(r, rs, cs_s + ch * 64 + sub * 32, b_s + ch * 64 + sub * 32, y);
-                if constexpr (EPI == EPI_GELU_F16) {
-#pragma unroll
-                  for (int j = 0; j < 32; ++j) y[j] = gelu_sigmoid(y[j]);
-                }
-                if constexpr (RES) {
-#pragma unroll
-                  for (int c = 0; c < 4; ++c) {
-                    const uint4 u = staged_chunk128(buf, lane, 4 * sub + c);
-                    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                      const float2 f = Pair16<OutT>::unpack(w[j]);
-                      y[8 * c + 2 * j] += f.x;
-                      y[8 * c + 2 * j + 1] += f.y;
-                    }
+                  for (int j = 0; j < 16; ++j) {
+                    rc[j] = __ldg(cp + static_cast<int64_t>(j) * args.tokens);
+                    rn[j] = __ldg(sp + static_cast<int64_t>(j) * args.tokens);
                   }
                 }
-                uint32_t packed[16];
+              }
 #pragma unroll
-                for (int j = 0; j < 16; ++j) packed[j] = Pair16<OutT>::pack(y[2 * j], y[2 * j + 1]);
-                stage_half_row128(buf, lane, sub, packed);
+              for (int g = 0; g < 4; ++g) {
+                scale_cols<8>(r + 8 * g, rs, cs + 8 * g, bs + 8 * g);
+                float y[8];
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {
+                  float2 v = make_float2(__uint_as_float(r[8 * g + j]), __uint_as_float(r[8 * g + j + 1]));
+                  if constexpr (EPI == EPI_GELU_F16) v = gelu2(v);
+                  if constexpr (EPI == EPI_QKV_NORM_ROPE) {
+                    if (qk) {
+                      const float* w = normp + (head < args.q_heads ? 0 : 128) + 32 * sub + 8 * g + j;
+                      const float x0 = fmaf((v.x - mean) * rstd, w[0], w[64]);
+                      const float x1 = fmaf((v.y - mean) * rstd, w[1], w[65]);
+                      const float c = rc[4 * g + j / 2], s = rn[4 * g + j / 2];
+                      v = make_float2(x0 * c - x1 * s, x0 * s + x1 * c);
+                    }
+                  }
+                  y[j] = v.x;
+                  y[j + 1] = v.y;
+                }
+                stage8(4 * sub + g, y);
               }
             }
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0 && n0 < args.tma_cols) {
-              tma_store_2d(&tmC, buf, n0, m_block);
-              bulk_commit_group();
-            }
-            store_ragged(n0, 64, staged_chunk128(buf, lane, (args.tma_cols - n0) >> 3 & 7));
+          }
+          if (!ok) break;
+          if (!any) continue;
+        }
+        if constexpr (!F32OUT) {
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0 && out0 < args.tma_cols) {
+            tma_store_2d(&tmC, stg, out0, m_block);
+            bulk_commit_group();
+          }
+          // A TMA store clips its box to whole 16-byte granules of a row: the last out_cols % 8 columns are written
+          // one by one by the lane that has staged them.
+          const int c = args.tma_cols, left = args.out_cols - c;
+          if (left != 0 && c >= out0 && c < out0 + WIDTH && row_ok) {
+            const uint4 u = SWIGLU ? staged_chunk64(stg, lane, (c - out0) >> 3) : staged_chunk128(stg, lane, (c - out0) >> 3);
+            uint16_t* dst = static_cast<uint16_t*>(args.out) + static_cast<int64_t>(m) * args.ldo + c;
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int e = 0; e < 7; ++e)
+              if (e < left) dst[e] = static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1)));
           }
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if (PAIR && !leader)
-          mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[acc]), 0u));
-        else
-          mbar_arrive(&tempty[acc]);
-      }
       if (!ok) break;
-      if (++acc == C::ACCS) {
-        acc = 0;
-        acc_phase ^= 1u;
-      }
     }
     if (!F32OUT && lane == 0) bulk_wait_all();
   }
@@ -598,7 +622,7 @@ struct Fp4Maps {
 
 template <bool PAIR, int EPI, class OutT>
 int launch_fp4(const Fp4Maps& t, const Fp4GemmArgs& a, cudaStream_t stream) {
-  using C = Fp4Cfg<PAIR, EPI == EPI_RESIDUAL>;
+  using C = Fp4Cfg<PAIR>;
   auto kernel = gemm_fp4_kernel<PAIR, EPI, OutT>;
   static int most[64] = {};  // CTAs (pairs) resident at once per device, 0 = not configured yet
   int dev = 0;
@@ -648,7 +672,12 @@ int dispatch_fp4(int epi, int dtype, const Fp4Maps& t, const Fp4GemmArgs& a, cud
     case EPI_SWIGLU: return bf ? launch_fp4<PAIR, EPI_SWIGLU, B>(t, a, s) : launch_fp4<PAIR, EPI_SWIGLU, H>(t, a, s);
     case EPI_RESIDUAL: return bf ? launch_fp4<PAIR, EPI_RESIDUAL, B>(t, a, s) : launch_fp4<PAIR, EPI_RESIDUAL, H>(t, a, s);
     default:
-      return bf ? launch_fp4<PAIR, EPI_QKV_NORM_ROPE, B>(t, a, s) : launch_fp4<PAIR, EPI_QKV_NORM_ROPE, H>(t, a, s);
+      if constexpr (PAIR) {
+        set_error("ff_gemm_fp4: no pair tiles for the QKV epilogue");
+        return FF_ERR_INVALID_ARGUMENT;
+      } else {
+        return bf ? launch_fp4<false, EPI_QKV_NORM_ROPE, B>(t, a, s) : launch_fp4<false, EPI_QKV_NORM_ROPE, H>(t, a, s);
+      }
   }
 }
 
@@ -680,6 +709,7 @@ int gemm_fp4(const Fp4Operand& A, const Fp4Operand& W, int fmt, int M, int N, in
              "ff_gemm_fp4: output type %d is not available for epilogue %d", e->out_dtype, epi);
   FF_REQUIRE(tile == 0 || tile == 128 || tile == FF_TILE_PAIR256, "ff_gemm_fp4: tile must be 0, 128 or FF_TILE_PAIR256 (got %d)",
              tile);
+  FF_REQUIRE(epi != EPI_QKV_NORM_ROPE || tile != FF_TILE_PAIR256, "ff_gemm_fp4: no pair tiles for the QKV epilogue");
   FF_REQUIRE(epi != EPI_SWIGLU || N % 128 == 0, "ff_gemm_fp4: SwiGLU needs N %% 128 == 0 (N=%d)", N);
   const int out_cols = epi == EPI_SWIGLU ? (e->out_cols > 0 ? e->out_cols : N / 2) : N;
   FF_REQUIRE(epi != EPI_SWIGLU || out_cols <= N / 2, "ff_gemm_fp4: SwiGLU writes at most N / 2 columns (out_cols=%d, N=%d)",
@@ -704,7 +734,7 @@ int gemm_fp4(const Fp4Operand& A, const Fp4Operand& W, int fmt, int M, int N, in
   FF_REQUIRE(epi != EPI_RESIDUAL || (aligned16(e->residual) && e->ldr % 8 == 0), "ff_gemm_fp4: residual rows must be 16-byte aligned");
 
   const int64_t pair_tiles = static_cast<int64_t>((M + 255) / 256) * ((N + 255) / 256);
-  const bool pair = tile == FF_TILE_PAIR256 || (tile == 0 && pair_tiles >= sm_count());
+  const bool pair = tile == FF_TILE_PAIR256 || (tile == 0 && epi != EPI_QKV_NORM_ROPE && pair_tiles >= sm_count());
   Fp4Maps t;
   const bool mx = fmt == FF_FP4_MX;
   int rc;
@@ -715,7 +745,7 @@ int gemm_fp4(const Fp4Operand& A, const Fp4Operand& W, int fmt, int M, int N, in
   t.r = t.a;
   const CUtensorMapDataType dt = e->out_dtype == FF_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   if (!f32) {
-    const bool narrow = epi == EPI_SWIGLU && !pair;  // 32 output columns per warp
+    const bool narrow = epi == EPI_SWIGLU;  // 32 output columns per warp
     // whole 16-byte granules only (none: a map that no store uses); the kernel writes the rest of a row itself
     rc = make_tmap_2d_pitched(&t.c, e->out, dt, 2, static_cast<uint64_t>(out_cols < 8 ? 8 : out_cols & ~7), static_cast<uint64_t>(M),
                               static_cast<uint64_t>(e->ldo) * 2, narrow ? 32 : 64, 32,

@@ -189,7 +189,8 @@ int ff_dequantize_fp4(const uint8_t* codes, const uint8_t* scales, const float* 
  *                         angle-major); the columns after them (v) are out = y
  * Any M, N, K >= 1 (FF_EPI_SWIGLU: N % 128 == 0; FF_EPI_QKV_NORM_ROPE: N % 64 == 0). 16-bit out and residual:
  * 16-byte aligned, row strides (elements) multiples of 8. f32 out: any row stride. bias may be NULL.
- * tile: 0 = automatic, 128 = 128 x 128 tiles per CTA, FF_TILE_PAIR256 = 256 x 256 tiles per pair of CTAs.
+ * tile: 0 = automatic, 128 = 128 x 128 tiles per CTA, FF_TILE_PAIR256 = 256 x 256 tiles per pair of CTAs (not for
+ * FF_EPI_QKV_NORM_ROPE).
  */
 #define FF_EPI_QKV_NORM_ROPE 8
 #define FF_NORM_RMS 1

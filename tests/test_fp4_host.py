@@ -150,6 +150,8 @@ def test_gemm_operand_checks():
     assert f(FAKE, FAKE, None, FAKE, FAKE, FAKE, 0, 4, 128, 256, C.byref(_epi()), 0, None) == BAD and "row and column scales" in _err()
     assert f(FAKE, FAKE + 4, FAKE, FAKE, FAKE, FAKE, 0, 4, 128, 256, C.byref(_epi()), 0, None) == BAD and "16-byte aligned" in _err()
     assert f(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 0, 4, 128, 256, C.byref(_epi()), 256, None) == BAD and "tile" in _err()
+    e = _epi(**QKV)
+    assert f(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 0, 4, 128, 256, C.byref(e), 512, None) == BAD and "no pair tiles" in _err()
     assert f(None, None, None, FAKE, FAKE, FAKE, 0, 0, 128, 256, C.byref(_epi()), 0, None) == 0  # no rows
 
 

@@ -256,7 +256,7 @@ def _tables(tokens, half, seed=0):
     return a.cos().contiguous(), a.sin().contiguous()
 
 
-@pytest.mark.parametrize("tile", [128, 512])
+@pytest.mark.parametrize("tile", [0, 128])
 @pytest.mark.parametrize("norm", ["rms", "layer"])
 @pytest.mark.parametrize(("M", "qh", "kh", "vh", "K", "tokens", "fmt", "dtype"), [
     (1, 1, 1, 1, 64, 1, "nv", torch.float16),
