@@ -12,7 +12,8 @@
 //
 // Bound by HBM: 2 bytes read and 0.56 (NV) or 0.53 (MX) written per value. The whole row stays in registers,
 // 16 consecutive columns per lane, so a 16-column block never leaves its lane and a 32-column block is a pair
-// of lanes; WPR warps share a row so that a lane holds at most 48 values.
+// of lanes; WPR warps share a row so that a lane holds at most 48 values. CTAs are persistent: a warp loads its
+// next row while it works on this one, and gamma and beta come from shared memory, filled once.
 #include <type_traits>
 
 #include "common.h"
@@ -24,73 +25,84 @@ namespace {
 
 constexpr int kQuantThreads = 256;
 
-// W 32-bit words starting at byte address `a` (any alignment that is a multiple of 2), words at or past `end`
-// undefined. Reads whole aligned 16-byte granules that hold at least one byte below `end`.
-template <int W>
-__device__ __forceinline__ void load_words(uintptr_t a, uintptr_t end, uint32_t (&w)[W]) {
-  const uint32_t mis = static_cast<uint32_t>(a) & 15u;
-  if (mis == 0) {
+// 16 consecutive values of a row, as loaded. Rows may start anywhere: whole aligned 16-byte granules are read, those
+// that hold at least one byte of the row, and shifted into place afterwards.
+template <class T, bool ALIGNED>
+struct Raw {
+  static constexpr int W = sizeof(T) * 4;  // words of 16 values
+  uint32_t t[ALIGNED ? W : W + 4];
+};
+
+template <class T, bool ALIGNED>
+__device__ __forceinline__ void load_raw(const T* __restrict__ xr, int col, int cols, Raw<T, ALIGNED>& r) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(xr + col), end = reinterpret_cast<uintptr_t>(xr + cols);
+  const uintptr_t base = ALIGNED ? a : a & ~uintptr_t(15);
+  constexpr int N = Raw<T, ALIGNED>::W / 4 + (ALIGNED ? 0 : 1);
 #pragma unroll
-    for (int j = 0; j < W / 4; ++j) {
-      uint4 u = make_uint4(0, 0, 0, 0);
-      if (a + 16 * j < end) u = __ldg(reinterpret_cast<const uint4*>(a) + j);
-      w[4 * j] = u.x;
-      w[4 * j + 1] = u.y;
-      w[4 * j + 2] = u.z;
-      w[4 * j + 3] = u.w;
-    }
-    return;
-  }
-  const uintptr_t base = a - mis;
-  uint32_t t[W + 4];
-#pragma unroll
-  for (int j = 0; j < W / 4 + 1; ++j) {
+  for (int j = 0; j < N; ++j) {
     uint4 u = make_uint4(0, 0, 0, 0);
-    if (base + 16 * j < end) u = __ldg(reinterpret_cast<const uint4*>(base) + j);
-    t[4 * j] = u.x;
-    t[4 * j + 1] = u.y;
-    t[4 * j + 2] = u.z;
-    t[4 * j + 3] = u.w;
+    if (col < cols && base + 16 * j < end) u = __ldg(reinterpret_cast<const uint4*>(base) + j);
+    r.t[4 * j] = u.x;
+    r.t[4 * j + 1] = u.y;
+    r.t[4 * j + 2] = u.z;
+    r.t[4 * j + 3] = u.w;
   }
-  if (mis & 8u) {
-#pragma unroll
-    for (int i = 0; i < W + 2; ++i) t[i] = t[i + 2];
-  }
-  if (mis & 4u) {
-#pragma unroll
-    for (int i = 0; i < W + 1; ++i) t[i] = t[i + 1];
-  }
-  const uint32_t sh = (mis & 2u) * 8u;  // 0 or 16 bits
-#pragma unroll
-  for (int i = 0; i < W; ++i) w[i] = __funnelshift_r(t[i], t[i + 1], sh);
 }
 
-template <class T>
-__device__ __forceinline__ void load16(const T* __restrict__ xr, int col, int cols, float (&v)[16]) {
-  if (col >= cols) {
+// The loaded words shifted into place, values at or past the row's end zero.
+template <class T, bool ALIGNED>
+__device__ __forceinline__ void realign(const T* xr, int col, int cols, Raw<T, ALIGNED>& r) {
+  constexpr int W = Raw<T, ALIGNED>::W;
+  if constexpr (!ALIGNED) {
+    const uint32_t mis = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(xr)) & 15u;  // the same for all columns
+    if (mis & 8u) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) v[e] = 0.f;
-    return;
+      for (int i = 0; i < W + 2; ++i) r.t[i] = r.t[i + 2];
+    }
+    if (mis & 4u) {
+#pragma unroll
+      for (int i = 0; i < W + 1; ++i) r.t[i] = r.t[i + 1];
+    }
+    const uint32_t sh = (mis & 2u) * 8u;  // 0 or 16 bits
+#pragma unroll
+    for (int i = 0; i < W; ++i) r.t[i] = __funnelshift_r(r.t[i], r.t[i + 1], sh);
   }
-  constexpr int W = sizeof(T) * 4;
-  uint32_t w[W];
-  load_words<W>(reinterpret_cast<uintptr_t>(xr + col), reinterpret_cast<uintptr_t>(xr + cols), w);
+  if (col + 16 > cols) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        if (col + i >= cols) r.t[i] = 0;
+      } else {
+        if (col + 2 * i >= cols)
+          r.t[i] = 0;
+        else if (col + 2 * i + 1 >= cols)
+          r.t[i] &= 0xffffu;
+      }
+    }
+  }
+}
+
+template <class T, bool ALIGNED>
+__device__ __forceinline__ void to_f32(const Raw<T, ALIGNED>& r, float (&v)[16]) {
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(w[e]);
+    for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(r.t[e]);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float2 f = Pair16<T>::unpack(w[e]);
+      const float2 f = Pair16<T>::unpack(r.t[e]);
       v[2 * e] = f.x;
       v[2 * e + 1] = f.y;
     }
   }
-  if (col + 16 > cols) {
-#pragma unroll
-    for (int e = 0; e < 16; ++e)
-      if (col + e >= cols) v[e] = 0.f;
-  }
+}
+
+template <class T>
+__device__ __forceinline__ void load16(const T* __restrict__ xr, int col, int cols, float (&v)[16]) {
+  Raw<T, false> r;
+  load_raw<T, false>(xr, col, cols, r);
+  realign<T, false>(xr, col, cols, r);
+  to_f32<T, false>(r, v);
 }
 
 // |.| maximum that keeps a NaN.
@@ -100,10 +112,25 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 __device__ __forceinline__ float amax16(const float (&v)[16]) {
-  float m = 0.f;
+  float m[4] = {0.f, 0.f, 0.f, 0.f};  // four chains
 #pragma unroll
-  for (int e = 0; e < 16; ++e) m = max_nan(m, fabsf(v[e]));
-  return m;
+  for (int e = 0; e < 16; ++e) m[e & 3] = max_nan(m[e & 3], fabsf(v[e]));
+  return max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3]));
+}
+// The same on 16-bit pairs as loaded: half the instructions.
+template <class T>
+__device__ __forceinline__ float amax_pairs(const uint32_t* w) {
+  uint32_t m[2] = {0, 0};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t v = w[e] & 0x7fff7fffu;
+    if constexpr (std::is_same<T, __half>::value)
+      asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(m[e & 1]) : "r"(v));
+    else
+      asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(m[e & 1]) : "r"(v));
+  }
+  const float2 a = Pair16<T>::unpack(m[0]), b = Pair16<T>::unpack(m[1]);
+  return max_nan(max_nan(a.x, a.y), max_nan(b.x, b.y));
 }
 __device__ __forceinline__ bool not_finite(float amax) { return !(amax <= 3.402823466e38f); }
 
@@ -115,35 +142,38 @@ __device__ __forceinline__ float nv_row_scale(float amax) {
 }
 __device__ __forceinline__ float inv_pow2(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
 
-// v / (S s) for the code. EXACT16: v came from a 16-bit type, so a quotient that is no rounding tie of e2m1 is
-// at least 2^-13 away from one, while v * (1 / S) is within 2^-20 of the quotient: adding and subtracting 192
-// rounds to multiples of 2^-16, which puts true ties exactly on the tie. EXACT32: IEEE division (checkpoint
-// weights, once per load). Neither: v is itself rounded (after a LayerNorm), the product is enough.
+// v / (S s) for the code, r = 1 / (S s) rounded. kExact16: v came from a 16-bit type, so a quotient that is no
+// rounding tie of e2m1 is at least 2^-13 away from one, while v * r is within 2^-20 of the quotient: rounding
+// v * r + 192 (one FMA, to multiples of 2^-16) puts true ties exactly on the tie. kExact32: IEEE division
+// (checkpoint weights, once per load). kPlain: v is itself rounded (after a LayerNorm) or r a power of two.
 enum QuotientKind { kPlain, kExact16, kExact32 };
 template <int KIND>
-__device__ __forceinline__ float quotient(float v, float r, float scale) {
-  if constexpr (KIND == kExact32) return scale > 0.f ? __fdiv_rn(v, scale) : 0.f;
-  const float y = __fmul_rn(v, r);
-  if constexpr (KIND == kExact16) return __fsub_rn(__fadd_rn(y, 192.f), 192.f);
-  return y;
+__device__ __forceinline__ float2 quotient2(float2 v, float r, float scale) {
+  if constexpr (KIND == kExact32)
+    return scale > 0.f ? make_float2(__fdiv_rn(v.x, scale), __fdiv_rn(v.y, scale)) : make_float2(0.f, 0.f);
+  else if constexpr (KIND == kExact16)
+    return add2(fma2(v, make_float2(r, r), make_float2(192.f, 192.f)), make_float2(-192.f, -192.f));
+  else
+    return mul2(v, make_float2(r, r));
 }
 
 template <int KIND>
 __device__ __forceinline__ uint2 codes16(const float (&v)[16], float r, float scale) {
-  float lo[8], hi[8];
+  float y[2][8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    lo[e] = quotient<KIND>(v[e], r, scale);
-    hi[e] = quotient<KIND>(v[8 + e], r, scale);
+  for (int e = 0; e < 16; e += 2) {
+    const float2 q = quotient2<KIND>(make_float2(v[e], v[e + 1]), r, scale);
+    y[e >> 3][e & 7] = q.x;
+    y[e >> 3][(e & 7) + 1] = q.y;
   }
-  return make_uint2(e2m1x8(lo), e2m1x8(hi));
+  return make_uint2(e2m1x8(y[0]), e2m1x8(y[1]));
 }
 
 // One 16-column piece of an NV row with row scale s: its scale byte and codes.
 template <int KIND>
-__device__ __forceinline__ uint32_t nv_piece(const float (&v)[16], float s, bool bad, uint2* codes) {
+__device__ __forceinline__ uint32_t nv_piece(const float (&v)[16], float amax, float s, bool bad, uint2* codes) {
   const float is = inv_pow2(s);
-  const uint32_t byte = bad ? 0u : e4m3_byte(__fdiv_rn(amax16(v) * is, 6.f));
+  const uint32_t byte = bad ? 0u : e4m3_byte(__fdiv_rn(amax * is, 6.f));
   const float S = e4m3_value(byte);
   const float r = byte ? __frcp_rn(S) * is : 0.f;
   *codes = bad ? make_uint2(0, 0) : codes16<KIND>(v, r, S * s);
@@ -210,93 +240,146 @@ __device__ __forceinline__ void store_piece(const QuantArgs& a, int row, int c, 
     *reinterpret_cast<uint32_t*>(a.scales + sf_offset(row, MX ? c >> 1 : c, tile)) = u;
 }
 
-// WPR warps per row, NC pieces of 16 columns per lane: rows of up to 512 * WPR * NC columns. A CTA takes rows
-// 32 apart (and neighbours), whose scales share 16-byte groups of a chunk.
-template <class T, bool MX, bool NORM, int WPR, int NC>
+// gamma and beta in shared memory, zero past the row's end: 16 bytes j of piece c at float4 index
+// 4 c + (j ^ (c / 2) % 4), so that lanes with consecutive pieces read from all banks.
+__device__ __forceinline__ int norm_slot(int c, int j) { return 4 * c + (j ^ ((c >> 1) & 3)); }
+
+// WPR warps per row, NC pieces of 16 columns per lane: rows of up to 512 * WPR * NC columns.
+template <class T, bool MX, bool NORM, bool ALIGNED, int WPR, int NC>
 __global__ void __launch_bounds__(kQuantThreads) quantize_fp4_kernel(const QuantArgs a) {
-  constexpr int RPC = kQuantThreads / 32 / WPR;  // rows per CTA
-  __shared__ float red[3][kQuantThreads / 32];
+  constexpr int WARPS = kQuantThreads / 32;
+  constexpr int RPC = WARPS / WPR;  // rows per CTA
+  extern __shared__ float4 norm_s[];  // gamma, then beta
+  __shared__ float red[2][3][WARPS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int grp = warp / WPR, wr = warp % WPR;
-  constexpr int PER_TILE = 128 / RPC;
-  const int tile = blockIdx.x / PER_TILE, j = blockIdx.x % PER_TILE;
-  int in_tile;
-  if constexpr (RPC == 8)
-    in_tile = 32 * (grp & 3) + 2 * j + (grp >> 2);
-  else if constexpr (RPC == 4)
-    in_tile = 32 * grp + j;
-  else if constexpr (RPC == 2)
-    in_tile = 32 * (2 * (j >> 5) + grp) + (j & 31);
-  else
-    in_tile = j;
-  const int row = tile * 128 + in_tile;
-  const bool on = row < a.rows;
+  const int pieces = (a.cols + kFp4Step - 1) / kFp4Step * (kFp4Step / 16);
+  int parity = 0;
   auto row_all = [&](float v, int slot, auto op) {  // over the WPR warps of the row, after a warp reduction
     if constexpr (WPR > 1) {
-      if (lane == 0) red[slot][warp] = v;
-      __syncthreads();
-      v = red[slot][grp * WPR];
+      if (lane == 0) red[parity][slot][warp] = v;
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + grp), "n"(32 * WPR) : "memory");
+      v = red[parity][slot][grp * WPR];
 #pragma unroll
-      for (int i = 1; i < WPR; ++i) v = op(v, red[slot][grp * WPR + i]);
+      for (int i = 1; i < WPR; ++i) v = op(v, red[parity][slot][grp * WPR + i]);
     }
     return v;
   };
   auto plus = [](float p, float q) { return p + q; };
   pdl_wait();
   pdl_trigger();
-  const T* xr = static_cast<const T*>(a.x) + (on ? row : 0) * a.ldx;
-  float v[NC][16];
-#pragma unroll
-  for (int i = 0; i < NC; ++i) load16<T>(xr, ((i * WPR + wr) * 32 + lane) * 16, on ? a.cols : 0, v[i]);
   if constexpr (NORM) {
-    float s = 0.f;
+    for (int i = threadIdx.x; i < pieces * 4; i += kQuantThreads) {
+      const int c = i >> 2, j = i & 3;
+      float g[4], b[4];
 #pragma unroll
-    for (int i = 0; i < NC; ++i)
+      for (int e = 0; e < 4; ++e) {
+        const int col = 16 * c + 4 * j + e;
+        g[e] = col < a.cols ? __ldg(a.gamma + col) : 0.f;
+        b[e] = col < a.cols ? __ldg(a.beta + col) : 0.f;
+      }
+      norm_s[norm_slot(c, j)] = make_float4(g[0], g[1], g[2], g[3]);
+      norm_s[4 * pieces + norm_slot(c, j)] = make_float4(b[0], b[1], b[2], b[3]);
+    }
+    __syncthreads();
+  }
+  const int step = static_cast<int>(gridDim.x) * RPC;
+  int row = static_cast<int>(blockIdx.x) * RPC + grp;
+  const T* xr = static_cast<const T*>(a.x) + row * a.ldx;
+  Raw<T, ALIGNED> raw[NC];
+  if (row < a.rows) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s += v[i][e];
-    const float n = static_cast<float>(a.cols);
-    const float mean = row_all(warp_sum(s), 0, plus) / n;
-    float q = 0.f;
+    for (int i = 0; i < NC; ++i) load_raw<T, ALIGNED>(xr, ((i * WPR + wr) * 32 + lane) * 16, a.cols, raw[i]);
+  }
+  for (; row < a.rows; row += step, parity ^= 1) {
+    float v[NC][16], amax[NC];
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int col = ((i * WPR + wr) * 32 + lane) * 16;
+      realign<T, ALIGNED>(xr, ((i * WPR + wr) * 32 + lane) * 16, a.cols, raw[i]);
+      if constexpr (!NORM && sizeof(T) == 2) amax[i] = amax_pairs<T>(raw[i].t);
+      to_f32<T, ALIGNED>(raw[i], v[i]);
+    }
+    if (row + step < a.rows) {  // the next row comes in meanwhile
+      xr += step * a.ldx;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float d = col + e < a.cols ? v[i][e] - mean : 0.f;
-        q += d * d;
+      for (int i = 0; i < NC; ++i) load_raw<T, ALIGNED>(xr, ((i * WPR + wr) * 32 + lane) * 16, a.cols, raw[i]);
+    }
+    if constexpr (NORM) {
+      float2 s2 = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) s2 = add2(s2, make_float2(v[i][e], v[i][e + 1]));
+      const float n = static_cast<float>(a.cols);
+      const float mean = row_all(warp_sum(s2.x + s2.y), 0, plus) / n;
+      float2 q2 = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        const int col = ((i * WPR + wr) * 32 + lane) * 16;
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+          const float2 d = add2(make_float2(v[i][e], v[i][e + 1]), make_float2(-mean, -mean));
+          v[i][e] = d.x;
+          v[i][e + 1] = d.y;
+        }
+        if (col + 16 > a.cols) {  // columns past the row's end stay out of the variance
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (col + e >= a.cols) v[i][e] = 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+          const float2 d = make_float2(v[i][e], v[i][e + 1]);
+          q2 = fma2(d, d, q2);
+        }
+      }
+      const float rstd = rsqrtf(row_all(warp_sum(q2.x + q2.y), 1, plus) / n + a.eps);
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        const int c = (i * WPR + wr) * 32 + lane;
+        if (c < pieces) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float4 g = norm_s[norm_slot(c, j)], b = norm_s[4 * pieces + norm_slot(c, j)];
+            const float2 r2 = make_float2(rstd, rstd);
+            const float2 lo = fma2(make_float2(v[i][4 * j], v[i][4 * j + 1]), mul2(r2, make_float2(g.x, g.y)), make_float2(b.x, b.y));
+            const float2 hi = fma2(make_float2(v[i][4 * j + 2], v[i][4 * j + 3]), mul2(r2, make_float2(g.z, g.w)), make_float2(b.z, b.w));
+            v[i][4 * j] = lo.x;
+            v[i][4 * j + 1] = lo.y;
+            v[i][4 * j + 2] = hi.x;
+            v[i][4 * j + 3] = hi.y;
+          }
+        }
       }
     }
-    const float rstd = rsqrtf(row_all(warp_sum(q), 1, plus) / n + a.eps);
+    if constexpr (NORM || sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < NC; ++i) affine16(v[i], mean, rstd, a, ((i * WPR + wr) * 32 + lane) * 16);
-  }
-  float s = 1.f;
-  bool bad = false;
-  if constexpr (!MX) {
-    float m = 0.f;
-#pragma unroll
-    for (int i = 0; i < NC; ++i) m = max_nan(m, amax16(v[i]));
-#pragma unroll
-    for (int o = 16; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-    m = row_all(m, 2, [](float p, float q) { return max_nan(p, q); });
-    bad = not_finite(m);
-    s = nv_row_scale(bad ? 0.f : m);
-    if (on && lane == 0 && wr == 0) a.row_scale[row] = bad ? __uint_as_float(0x7fffffffu) : s;
-  }
-  const int pieces = (a.cols + kFp4Step - 1) / kFp4Step * (kFp4Step / 16);
-#pragma unroll
-  for (int i = 0; i < NC; ++i) {
-    const int c = (i * WPR + wr) * 32 + lane;
-    uint2 codes;
-    uint32_t byte;
-    if constexpr (MX) {
-      float m = amax16(v[i]);
-      m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
-      byte = mx_piece(v[i], m, &codes);
-    } else {
-      byte = nv_piece<quotient_kind<T, NORM>()>(v[i], s, bad, &codes);
+      for (int i = 0; i < NC; ++i) amax[i] = amax16(v[i]);
     }
-    store_piece<MX>(a, row, c, codes, byte, on && c < pieces);
+    float s = 1.f;
+    bool bad = false;
+    if constexpr (!MX) {
+      float m = amax[0];
+#pragma unroll
+      for (int i = 1; i < NC; ++i) m = max_nan(m, amax[i]);
+#pragma unroll
+      for (int o = 16; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+      m = row_all(m, 2, [](float p, float q) { return max_nan(p, q); });
+      bad = not_finite(m);
+      s = nv_row_scale(bad ? 0.f : m);
+      if (lane == 0 && wr == 0) a.row_scale[row] = bad ? __uint_as_float(0x7fffffffu) : s;
+    }
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = (i * WPR + wr) * 32 + lane;
+      uint2 codes;
+      uint32_t byte;
+      if constexpr (MX)
+        byte = mx_piece(v[i], max_nan(amax[i], __shfl_xor_sync(0xffffffffu, amax[i], 1)), &codes);
+      else
+        byte = nv_piece<quotient_kind<T, NORM>()>(v[i], amax[i], s, bad, &codes);
+      store_piece<MX>(a, row, c, codes, byte, c < pieces);
+    }
   }
 }
 
@@ -367,37 +450,54 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_fp4_wide_kernel(const 
       m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
       byte = mx_piece(v, m, &codes);
     } else {
-      byte = nv_piece<quotient_kind<T, NORM>()>(v, s, bad, &codes);
+      byte = nv_piece<quotient_kind<T, NORM>()>(v, amax16(v), s, bad, &codes);
     }
     store_piece<MX>(a, row, c, codes, byte, c < pieces);
   }
 }
 
-template <class T, bool MX, bool NORM, int WPR, int NC>
+template <class T, bool MX, bool NORM, bool ALIGNED, int WPR, int NC>
 int launch_quant(const QuantArgs& a, cudaStream_t stream) {
   constexpr int RPC = kQuantThreads / 32 / WPR;
-  const int grid = (a.rows + 127) / 128 * (128 / RPC);
-  launch(quantize_fp4_kernel<T, MX, NORM, WPR, NC>, dim3(grid), dim3(kQuantThreads), 0, stream, a);
+  auto kernel = quantize_fp4_kernel<T, MX, NORM, ALIGNED, WPR, NC>;
+  const size_t smem = NORM ? static_cast<size_t>((a.cols + kFp4Step - 1) / kFp4Step) * kFp4Step * 8 : 0;
+  static int per_sm[64] = {};  // resident CTAs per SM, 0 = not configured yet (widest row of the instantiation)
+  int dev = 0;
+  cudaGetDevice(&dev);
+  int most = dev >= 0 && dev < 64 ? per_sm[dev] : 0;
+  if (most == 0) {
+    const size_t widest = NORM ? 512 * WPR * NC * 8 : 0;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(widest)) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&most, kernel, kQuantThreads, widest) != cudaSuccess || most < 1)
+      return check_launch("quantize_fp4: configuration");
+    if (dev >= 0 && dev < 64) per_sm[dev] = most;
+  }
+  const int want = (a.rows + RPC - 1) / RPC, full = most * sm_count();
+  launch(kernel, dim3(want < full ? want : full), dim3(kQuantThreads), smem, stream, a);
   return check_launch("quantize_fp4_kernel");
 }
 
-template <class T, bool MX, bool NORM>
+template <class T, bool MX, bool NORM, bool ALIGNED>
 int dispatch_quant(const QuantArgs& a, cudaStream_t stream) {
   const int cols = (a.cols + kFp4Step - 1) / kFp4Step * kFp4Step;  // the padded scales are written too
-  if (cols <= 512) return launch_quant<T, MX, NORM, 1, 1>(a, stream);
-  if (cols <= 1024) return launch_quant<T, MX, NORM, 1, 2>(a, stream);
-  if (cols <= 1536) return launch_quant<T, MX, NORM, 1, 3>(a, stream);
-  if (cols <= 3 * 1024) return launch_quant<T, MX, NORM, 2, 3>(a, stream);
-  if (cols <= 6 * 1024) return launch_quant<T, MX, NORM, 4, 3>(a, stream);
-  if (cols <= 12 * 1024) return launch_quant<T, MX, NORM, 8, 3>(a, stream);
+  if (cols <= 1024) return launch_quant<T, MX, NORM, ALIGNED, 1, 2>(a, stream);
+  if (cols <= 1536) return launch_quant<T, MX, NORM, ALIGNED, 1, 3>(a, stream);
+  if (cols <= 3 * 1024) return launch_quant<T, MX, NORM, ALIGNED, 2, 3>(a, stream);
+  if (cols <= 6 * 1024) return launch_quant<T, MX, NORM, ALIGNED, 4, 3>(a, stream);
   launch(quantize_fp4_wide_kernel<T, MX, NORM>, dim3(a.rows), dim3(kQuantThreads), 0, stream, a);
   return check_launch("quantize_fp4_wide_kernel");
 }
 
+template <class T, bool MX, bool NORM>
+int dispatch_quant_align(const QuantArgs& a, cudaStream_t stream) {
+  const bool aligned = aligned16(a.x) && a.ldx * static_cast<int64_t>(sizeof(T)) % 16 == 0;
+  return aligned ? dispatch_quant<T, MX, NORM, true>(a, stream) : dispatch_quant<T, MX, NORM, false>(a, stream);
+}
+
 template <class T>
 int dispatch_quant_t(const QuantArgs& a, bool mx, cudaStream_t stream) {
-  if (a.gamma != nullptr) return mx ? dispatch_quant<T, true, true>(a, stream) : dispatch_quant<T, false, true>(a, stream);
-  return mx ? dispatch_quant<T, true, false>(a, stream) : dispatch_quant<T, false, false>(a, stream);
+  if (a.gamma != nullptr) return mx ? dispatch_quant_align<T, true, true>(a, stream) : dispatch_quant_align<T, false, true>(a, stream);
+  return mx ? dispatch_quant_align<T, true, false>(a, stream) : dispatch_quant_align<T, false, false>(a, stream);
 }
 
 // ---------------------------------------------------------------- dequantisation
@@ -411,63 +511,63 @@ __device__ __forceinline__ void store_one(T* p, float v) {
     *p = __float2bfloat16_rn(v);
 }
 
-// A thread writes one aligned 16-byte granule of an output row (its columns need not start at a block), so the
-// stores are whole whatever the row's alignment; granules that stick out of the row are written value by value.
+// A lane writes one aligned 16-byte granule of an output row at a time (its columns need not start at a block), so
+// the stores are whole whatever the row's alignment; granules that stick out of the row are written value by value.
+// A warp takes whole rows.
 template <class T, bool MX>
 __global__ void __launch_bounds__(256)
     dequantize_fp4_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                          const float* __restrict__ row_scale, int rows, int cols, T* __restrict__ out, int64_t ldo,
-                          int granules) {
+                          const float* __restrict__ row_scale, int rows, int cols, T* __restrict__ out, int64_t ldo) {
   constexpr int E = 16 / sizeof(T);
+  constexpr int B = MX ? 32 : 16;
+  const int lane = threadIdx.x & 31;
   pdl_wait();
   pdl_trigger();
   const int64_t pitch = fp4_row_bytes(cols), tile = sf_tile_bytes(cols, MX);
-  const int64_t total = static_cast<int64_t>(rows) * granules;
-  for (int64_t t = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; t < total;
-       t += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int row = static_cast<int>(t / granules), g = static_cast<int>(t % granules);
+  const int words = static_cast<int>(pitch / 4);
+  for (int row = static_cast<int>(blockIdx.x) * 8 + (threadIdx.x >> 5); row < rows; row += static_cast<int>(gridDim.x) * 8) {
     T* orow = out + row * ldo;
     const int off = static_cast<int>((reinterpret_cast<uintptr_t>(orow) & 15) / sizeof(T));
-    const int c0 = g * E - off;  // first column of the granule, may be negative
-    if (c0 >= cols || c0 + E <= 0) continue;
-    const uint8_t* crow = codes + row * pitch;
-    const float s = MX || row_scale == nullptr ? 1.f : __ldg(row_scale + row);
-    // codes of columns [c0, c0 + 8): two aligned words, shifted
-    const int w0 = c0 >> 3;  // rounds down
-    const int words = static_cast<int>(pitch / 4);
-    const uint32_t lo = w0 >= 0 ? __ldg(reinterpret_cast<const uint32_t*>(crow) + w0) : 0u;
-    const uint32_t hi = w0 + 1 < words ? __ldg(reinterpret_cast<const uint32_t*>(crow) + w0 + 1) : 0u;
-    uint32_t h[4];
-    e2m1x8_to_half2(__funnelshift_r(lo, hi, 4 * (c0 & 7)), h);
-    // the (at most two) blocks that the granule touches
-    constexpr int B = MX ? 32 : 16;
-    const int b0 = (c0 < 0 ? 0 : c0) / B;
-    const int b1 = (c0 + E - 1 < cols ? c0 + E - 1 : cols - 1) / B;
-    float sc[2];
-    const int blk[2] = {b0, b1};
+    const uint32_t* crow = reinterpret_cast<const uint32_t*>(codes + row * pitch);
+    const uint8_t* srow = scales + sf_offset(row, 0, tile);
+    const float s = MX ? 1.f : __ldg(row_scale + row);
+    auto scale_at = [&](int blk) {
+      const uint32_t byte = __ldg(srow + static_cast<int64_t>(blk >> 2) * kSfChunk + (blk & 3));
+      return MX ? e8m0_value(byte) : e4m3_value(byte) * s;
+    };
+#pragma unroll 4
+    for (int c0 = lane * E - off; c0 < cols; c0 += 32 * E) {  // c0: the granule's first column, may be negative
+      if (c0 + E <= 0) continue;
+      // codes of columns [c0, c0 + E): one aligned word, or two when the row is not aligned
+      const int w0 = c0 >> 3, sh = 4 * (c0 & 7);
+      uint32_t q = w0 >= 0 ? __ldg(crow + w0) : 0u;
+      if (sh + 4 * E > 32) q = __funnelshift_r(q, w0 + 1 < words ? __ldg(crow + w0 + 1) : 0u, sh);
+      else q >>= sh;
+      uint32_t h[4];
+      e2m1x8_to_half2(q, h);
+      // the (at most two) blocks that the granule touches
+      const int first = c0 < 0 ? 0 : c0, last = c0 + E - 1 < cols ? c0 + E - 1 : cols - 1;
+      const float s0 = scale_at(first / B), s1 = last / B != first / B ? scale_at(last / B) : s0;
+      const int cut = (first / B + 1) * B;  // the second block's first column
+      float v[8];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint32_t byte = __ldg(scales + sf_offset(row, blk[i], tile));
-      sc[i] = MX ? e8m0_value(byte) : e4m3_value(byte) * s;
-    }
-    float v[8];
+      for (int e = 0; e < E; ++e) {
+        const float2 f = unpack_half2(h[e / 2]);
+        v[e] = ((e & 1) ? f.y : f.x) * (c0 + e >= cut ? s1 : s0);
+      }
+      if (c0 >= 0 && c0 + E <= cols) {
+        uint4 u;
+        if constexpr (sizeof(T) == 4)
+          u = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+        else
+          u = make_uint4(Pair16<T>::pack(v[0], v[1]), Pair16<T>::pack(v[2], v[3]), Pair16<T>::pack(v[4], v[5]),
+                         Pair16<T>::pack(v[6], v[7]));
+        *reinterpret_cast<uint4*>(orow + c0) = u;
+      } else {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float2 f = unpack_half2(h[e / 2]);
-      v[e] = ((e & 1) ? f.y : f.x) * ((c0 + e) / B > b0 ? sc[1] : sc[0]);
-    }
-    if (c0 >= 0 && c0 + E <= cols) {
-      uint4 u;
-      if constexpr (sizeof(T) == 4)
-        u = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-      else
-        u = make_uint4(Pair16<T>::pack(v[0], v[1]), Pair16<T>::pack(v[2], v[3]), Pair16<T>::pack(v[4], v[5]),
-                       Pair16<T>::pack(v[6], v[7]));
-      *reinterpret_cast<uint4*>(orow + c0) = u;
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (c0 + e >= 0 && c0 + e < cols) store_one(orow + c0 + e, v[e]);
+        for (int e = 0; e < E; ++e)
+          if (c0 + e >= 0 && c0 + e < cols) store_one(orow + c0 + e, v[e]);
+      }
     }
   }
 }
@@ -475,17 +575,12 @@ __global__ void __launch_bounds__(256)
 template <class T>
 int launch_dequant(const uint8_t* codes, const uint8_t* scales, const float* rs, int rows, int cols, bool mx, void* out,
                    int64_t ldo, cudaStream_t stream) {
-  constexpr int E = 16 / sizeof(T);
-  const int granules = (cols + 2 * E - 2) / E;  // one more than an aligned row's where the row may start inside one
-  const int64_t total = static_cast<int64_t>(rows) * granules;
-  const int64_t want = (total + 255) / 256, most = static_cast<int64_t>(sm_count()) * 32;
-  const dim3 grid(static_cast<unsigned>(want < most ? want : most));
+  const int want = (rows + 7) / 8, most = sm_count() * 8;
+  const dim3 grid(want < most ? want : most);
   if (mx)
-    launch(dequantize_fp4_kernel<T, true>, grid, dim3(256), 0, stream, codes, scales, rs, rows, cols,
-           static_cast<T*>(out), ldo, granules);
+    launch(dequantize_fp4_kernel<T, true>, grid, dim3(256), 0, stream, codes, scales, rs, rows, cols, static_cast<T*>(out), ldo);
   else
-    launch(dequantize_fp4_kernel<T, false>, grid, dim3(256), 0, stream, codes, scales, rs, rows, cols,
-           static_cast<T*>(out), ldo, granules);
+    launch(dequantize_fp4_kernel<T, false>, grid, dim3(256), 0, stream, codes, scales, rs, rows, cols, static_cast<T*>(out), ldo);
   return check_launch("dequantize_fp4_kernel");
 }
 

@@ -4,7 +4,7 @@
 // they multiply (kind::mxf4nvf4 / kind::mxf4, f32 accumulators in TMEM); the row scales, which are powers of
 // two, and the bias are applied in f32 in the epilogue, which rounds once, to the output's type.
 //
-// One CTA per SM, 640 threads, persistent over a run of tiles:
+// One CTA per SM, 640 threads, persistent over tiles:
 //   warp 0     TMA producer: per stage 256 columns (128 bytes of codes, 128-byte swizzle) of A and W rows and
 //              their scale chunks
 //   warp 1     TMEM allocator; copies each stage's scale chunks to TMEM (tcgen05.cp, in order with the MMAs of
@@ -148,9 +148,6 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR>::THREADS, 1)
   const bool leader = rank == 0;
   const int unit = PAIR ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
   const int units = PAIR ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
-  // A run of tiles along N: consecutive tiles share their rows of A.
-  const int t_begin = static_cast<int>(static_cast<int64_t>(unit) * tiles / units);
-  const int t_end = static_cast<int>(static_cast<int64_t>(unit + 1) * tiles / units);
   auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
     if constexpr (PAIR)
       return mbar_wait_cluster<true>(bar, parity, abort_flag, args.err, code);
@@ -237,11 +234,11 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR>::THREADS, 1)
       const int pre = args.w_const ? (args.num_kb < STAGES ? args.num_kb : STAGES) : 0;
       for (int kb = 0; kb < pre; ++kb) {
         expect(&full[kb]);
-        load_w(smem + kb * C::STAGE_BYTES, &full[kb], kb, t_begin % tiles_n);
+        load_w(smem + kb * C::STAGE_BYTES, &full[kb], kb, unit % tiles_n);
       }
       pdl_wait();
       bool ok = true, first = true;
-      for (int t = t_begin; t < t_end && ok; ++t) {
+      for (int t = unit; t < tiles && ok; t += units) {
         const int tm = t / tiles_n, tn = t % tiles_n;
         for (int kb = 0; kb < args.num_kb; ++kb) {
           uint8_t* sa = smem + stage * C::STAGE_BYTES;
@@ -289,8 +286,7 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR>::THREADS, 1)
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int t = t_begin; t < t_end && ok; ++t) {
-        const int i = t - t_begin;
+      for (int i = 0; unit + i * units < tiles && ok; ++i) {
         const uint32_t acc = i & 1, use = (i >> 1) & 1;
         if (!wait(&tempty[acc], use ^ 1u, kDevTimeoutTmemEmpty)) break;
         if (PAIR && i > 0 && !wait(&tearly[acc ^ 1u], ((i - 1) >> 1) & 1, kDevTimeoutTmemEmpty)) break;
@@ -356,7 +352,7 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR>::THREADS, 1)
     constexpr int STEPS = HALF / 64;           // 64 tile columns per step
     constexpr int WIDTH = SWIGLU ? 32 : 64;    // output columns per step
     uint32_t use = 0, res_phase = 0;
-    for (int t = t_begin + acc; t < t_end; t += 2, use ^= 1u) {
+    for (int t = unit + acc * units; t < tiles; t += 2 * units, use ^= 1u) {
       const int tm = t / tiles_n, tn = t - tm * tiles_n;
       const int m_block = tm * C::TILE_M + static_cast<int>(rank) * 128 + q * 32;
       const int m = m_block + lane;

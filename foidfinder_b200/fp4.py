@@ -133,22 +133,24 @@ class Fp4Linear:
             self._heads = [_f32(t, d) for t in (q_weight, k_weight, q_bias, k_bias, *rope)]
             heads = dict(zip(("q_weight", "k_weight", "q_bias", "k_bias", "rope_cos", "rope_sin"), self._heads))
             heads |= dict(norm=norm, q_heads=q_heads, k_heads=(total - q_heads) // 2, qk_eps=qk_eps)
-        self._epilogue_args = dict(bias=self.bias, **heads)
-        self.epilogue = EPILOGUES[epilogue]
-        ops.fp4_epilogue(self.epilogue, self.rows, d, **self._epilogue_args)  # refuses bad arguments here
+        self._epilogue = ops.fp4_epilogue(EPILOGUES[epilogue], self.rows, d, bias=self.bias, **heads)  # refuses bad arguments
+        q = self.weight
+        self._w = ops._operand(q.codes, q.scales, q.row_scale, self.rows, self.in_features, FORMATS[fmt], d.index, "Fp4Linear")
+        self._g = ops._vector(self.gamma, self.in_features, d.index, "Fp4Linear: gamma")
+        self._b = ops._vector(self.beta, self.in_features, d.index, "Fp4Linear: beta")
+        self._fmt, self._device = FORMATS[fmt], d.index
 
     def __call__(self, x: torch.Tensor, out: torch.Tensor | None = None, residual: torch.Tensor | None = None) -> torch.Tensor:
-        if x.dim() != 2 or x.shape[1] != self.in_features:
-            raise RuntimeError(f"Fp4Linear: x must be [M, {self.in_features}], got {list(x.shape)}")
+        """x [M, in_features] -> [M, out_features] (`out`, or a new tensor whose rows start 16 bytes apart or more)."""
+        if x.get_device() != self._device:
+            raise RuntimeError(f"Fp4Linear: x is on {x.device}, the weight on cuda:{self._device}")
         if out is None:
             pitch = (self.out_features + 7) // 8 * 8
             dtype = torch.float16 if x.dtype == torch.float32 else x.dtype
             out = torch.empty(x.shape[0], pitch, dtype=dtype, device=x.device)[:, : self.out_features]
-        if out.shape[1] != self.out_features:
+        if out.shape[-1] != self.out_features:
             raise RuntimeError(f"Fp4Linear: out must have {self.out_features} columns, got {list(out.shape)}")
-        w = self.weight
-        ops.linear_fp4(x, w.codes, w.scales, w.row_scale, out, self.epilogue, FORMATS[self.fmt], N=self.rows, gamma=self.gamma, beta=self.beta,
-                       eps=self.eps, residual=residual, **self._epilogue_args)
+        ops._linear(x, self._w, self._fmt, self.rows, self.in_features, self._g, self._b, self.eps, self._epilogue, out, residual)
         return out
 
 

@@ -306,37 +306,63 @@ def int8_mma_peak(device: int = 0, iters: int = 200_000) -> float:
 
 
 # ---------------------------------------------------------------- block-scaled 4-bit operands
+# These calls are made once per layer, some for a single row, so their checks read each tensor attribute once and
+# build no message that is not needed.
 _DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
 _NORMS = {"rms": _lib.NORM_RMS, "layer": _lib.NORM_LAYER}
 _PAIRINGS = {"pairs": _lib.ROPE_PAIRS, "halves": _lib.ROPE_HALVES}
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
-def _rows_2d(t: torch.Tensor, what: str) -> int:
-    """Row stride of a 2-D tensor whose columns are contiguous."""
-    _need(t.is_cuda and t.dim() == 2 and (t.shape[1] <= 1 or t.stride(1) == 1), f"{what}: expected a 2-D CUDA tensor with contiguous columns")
-    return max(t.stride(0), t.shape[1]) if t.shape[0] <= 1 else t.stride(0)
+def _launch(what: str, fn, device: int, *args) -> None:
+    """fn(*args, stream) on the current stream of CUDA device `device`."""
+    if device == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, _raw_stream(device))
+    if rc:
+        check(rc, what)
 
 
-def _params(n: int, device: torch.device, what: str, **ts: torch.Tensor | None) -> None:
-    for name, t in ts.items():
-        if t is not None:
-            _need(t.device == device and t.is_contiguous() and t.dtype == torch.float32 and t.numel() == n, f"{what}: {name} must be {n} contiguous f32 values on {device}")
+def _matrix(t: torch.Tensor, what: str) -> tuple[int, int, int, int]:
+    """(rows, columns, row stride, device index) of a 2-D CUDA tensor whose columns are contiguous."""
+    device = t.get_device()
+    if device < 0 or t.dim() != 2:
+        raise RuntimeError(f"{what}: expected a 2-D CUDA tensor, got {t.dim()}-D on {t.device}")
+    rows, cols = t.shape
+    ld, step = t.stride()
+    if step != 1 and cols > 1:
+        raise RuntimeError(f"{what}: expected contiguous columns, got strides {t.stride()}")
+    return rows, cols, ld if rows > 1 else max(ld, cols), device
+
+
+def _vector(t: torch.Tensor | None, n: int, device: int, what: str) -> int | None:
+    """Address of an optional f32 parameter of n values."""
+    if t is None:
+        return None
+    if t.get_device() != device or t.dtype is not torch.float32 or t.numel() != n or not t.is_contiguous():
+        raise RuntimeError(f"{what}: expected {n} contiguous f32 values on cuda:{device}, got {t.dtype} {list(t.shape)} on {t.device}")
+    return t.data_ptr()
 
 
 def fp4_sizes(rows: int, cols: int, fmt: int) -> tuple[int, int]:
     """Bytes of the code and scale buffers of a [rows, cols] operand."""
-    return int(lib().ff_fp4_code_bytes(rows, cols)), int(lib().ff_fp4_scale_bytes(rows, cols, fmt))
+    return rows * ((cols + 31) // 32 * 16), (rows + 127) // 128 * ((cols + 255) // 256 * (2048 if fmt == FP4_NV else 1024))
 
 
-def _fp4_operand(codes: torch.Tensor, scales: torch.Tensor, row_scale: torch.Tensor | None, rows: int, cols: int, fmt: int, what: str) -> None:
-    _cuda(codes, scales, row_scale)
+def _operand(codes: torch.Tensor, scales: torch.Tensor, row_scale: torch.Tensor | None, rows: int, cols: int, fmt: int, device: int,
+             what: str) -> tuple[int, int, int | None]:
+    """Addresses of a 4-bit operand's buffers."""
     nc, ns = fp4_sizes(rows, cols, fmt)
-    _need(codes.dtype == torch.uint8 and codes.numel() >= nc, f"{what}: codes must be uint8, {nc} bytes for [{rows}, {cols}]")
-    _need(scales.dtype == torch.uint8 and scales.numel() >= ns, f"{what}: scales must be uint8, {ns} bytes for [{rows}, {cols}]")
-    _need(scales.device == codes.device, f"{what}: codes and scales are on different devices")
-    if fmt == FP4_NV:
-        _params(rows, codes.device, what, row_scale=row_scale)
-        _need(row_scale is not None, f"{what}: FP4_NV needs row_scale")
+    for t, n in ((codes, nc), (scales, ns)):
+        if t.get_device() != device or t.dtype is not torch.uint8 or t.numel() < n or not t.is_contiguous():
+            raise RuntimeError(f"{what}: codes and scales of [{rows}, {cols}] must be contiguous uint8 of {nc} and {ns} bytes on cuda:{device}")
+    if fmt != FP4_NV:
+        return codes.data_ptr(), scales.data_ptr(), None
+    if row_scale is None:
+        raise RuntimeError(f"{what}: FP4_NV needs row_scale")
+    return codes.data_ptr(), scales.data_ptr(), _vector(row_scale, rows, device, what)
 
 
 def quantize_fp4(
@@ -352,36 +378,21 @@ def quantize_fp4(
 ) -> None:
     """x [T, C] fp16, bf16 or f32 (columns contiguous, any row stride) -> (LayerNorm) -> 4-bit codes and block scales
     (`fp4_sizes` bytes) and, for FP4_NV, row_scale [T] f32."""
-    ldx = _rows_2d(x, "quantize_fp4")
-    _need(x.dtype in _DTYPES, "quantize_fp4: x must be fp16, bf16 or f32")
-    T, cols = x.shape
-    _fp4_operand(codes, scales, row_scale, T, cols, fmt, "quantize_fp4")
-    _need(codes.device == x.device, "quantize_fp4: x and codes are on different devices")
-    _params(cols, x.device, "quantize_fp4", gamma=gamma, beta=beta)
-    with torch.cuda.device(x.device):
-        check(
-            lib().ff_quantize_fp4(
-                _ptr(x), _DTYPES[x.dtype], ldx, _ptr(gamma), _ptr(beta), eps, T, cols, fmt, _ptr(codes), _ptr(scales),
-                _ptr(row_scale), _stream(x),
-            ),
-            "quantize_fp4",
-        )
+    T, cols, ldx, device = _matrix(x, "quantize_fp4")
+    dtype = _DTYPES.get(x.dtype)
+    _need(dtype is not None, "quantize_fp4: x must be fp16, bf16 or f32")
+    c, s, r = _operand(codes, scales, row_scale, T, cols, fmt, device, "quantize_fp4")
+    g, b = _vector(gamma, cols, device, "quantize_fp4: gamma"), _vector(beta, cols, device, "quantize_fp4: beta")
+    _launch("quantize_fp4", lib().ff_quantize_fp4, device, x.data_ptr(), dtype, ldx, g, b, eps, T, cols, fmt, c, s, r)
 
 
 def dequantize_fp4(codes: torch.Tensor, scales: torch.Tensor, row_scale: torch.Tensor | None, out: torch.Tensor, fmt: int) -> None:
     """The values of a 4-bit operand into out [T, C] (fp16, bf16 or f32; columns contiguous, any row stride)."""
-    ldo = _rows_2d(out, "dequantize_fp4")
-    _need(out.dtype in _DTYPES, "dequantize_fp4: out must be fp16, bf16 or f32")
-    T, cols = out.shape
-    _fp4_operand(codes, scales, row_scale, T, cols, fmt, "dequantize_fp4")
-    _need(codes.device == out.device, "dequantize_fp4: codes and out are on different devices")
-    with torch.cuda.device(out.device):
-        check(
-            lib().ff_dequantize_fp4(
-                _ptr(codes), _ptr(scales), _ptr(row_scale), T, cols, fmt, _ptr(out), _DTYPES[out.dtype], ldo, _stream(out)
-            ),
-            "dequantize_fp4",
-        )
+    T, cols, ldo, device = _matrix(out, "dequantize_fp4")
+    dtype = _DTYPES.get(out.dtype)
+    _need(dtype is not None, "dequantize_fp4: out must be fp16, bf16 or f32")
+    c, s, r = _operand(codes, scales, row_scale, T, cols, fmt, device, "dequantize_fp4")
+    _launch("dequantize_fp4", lib().ff_dequantize_fp4, device, c, s, r, T, cols, fmt, out.data_ptr(), dtype, ldo)
 
 
 def fp4_epilogue(
@@ -403,32 +414,39 @@ def fp4_epilogue(
 ) -> _lib.Fp4Epilogue:
     """The part of a gemm_fp4 epilogue that does not change from call to call (the tensors must outlive it)."""
     e = _lib.Fp4Epilogue(kind=epi)
-    _params(N, device, "fp4_epilogue", bias=bias)
-    e.bias = _ptr(bias)
+    d = device.index if device.index is not None else torch.cuda.current_device()
+    e.bias = _vector(bias, N, d, "fp4_epilogue: bias")
     if epi == EPI_QKV_NORM_ROPE:
         _need(norm in _NORMS, "fp4_epilogue: norm must be 'rms' or 'layer'")
-        _params(64, device, "fp4_epilogue", q_weight=q_weight, k_weight=k_weight, q_bias=q_bias, k_bias=k_bias)
-        _need(rope_cos is not None and rope_sin is not None and rope_cos.dim() == 2 and rope_cos.shape[0] == 32 and rope_sin.shape == rope_cos.shape,
-              "fp4_epilogue: rotation tables must be [32, tokens]")
-        _params(rope_cos.numel(), device, "fp4_epilogue", rope_cos=rope_cos, rope_sin=rope_sin)
-        e.norm, e.q_heads, e.k_heads, e.tokens, e.qk_eps = _NORMS[norm], q_heads, k_heads, rope_cos.shape[1], qk_eps
-        e.q_w, e.k_w, e.q_b, e.k_b = _ptr(q_weight), _ptr(k_weight), _ptr(q_bias), _ptr(k_bias)
-        e.rope_cos, e.rope_sin = _ptr(rope_cos), _ptr(rope_sin)
+        _need(q_weight is not None and k_weight is not None, "fp4_epilogue: q and k norm weights are required")
+        e.q_w, e.k_w = _vector(q_weight, 64, d, "fp4_epilogue: q_weight"), _vector(k_weight, 64, d, "fp4_epilogue: k_weight")
+        e.q_b, e.k_b = _vector(q_bias, 64, d, "fp4_epilogue: q_bias"), _vector(k_bias, 64, d, "fp4_epilogue: k_bias")
+        e.rope_cos, e.rope_sin, e.tokens = _tables(rope_cos, rope_sin, 32, d, "fp4_epilogue")
+        e.norm, e.q_heads, e.k_heads, e.qk_eps = _NORMS[norm], q_heads, k_heads, qk_eps
     return e
 
 
-def _bind_out(e: _lib.Fp4Epilogue, M: int, N: int, out: torch.Tensor, residual: torch.Tensor | None, device: torch.device, what: str) -> None:
-    ldo = _rows_2d(out, what)
-    cols = out.shape[1]
-    _need(out.device == device and out.dtype in _DTYPES, f"{what}: out must be fp16, bf16 or f32 on {device}")
-    _need(out.shape[0] == M and (cols <= N // 2 if e.kind == EPI_SWIGLU else cols == N), f"{what}: out has shape {tuple(out.shape)} for M={M} N={N}")
-    e.out_dtype, e.out, e.ldo, e.out_cols = _DTYPES[out.dtype], _ptr(out), ldo, cols
-    e.residual = None
+def _tables(cos: torch.Tensor | None, sin: torch.Tensor | None, half: int, device: int, what: str) -> tuple[int, int, int]:
+    """Addresses of the angle-major rotation tables [half, tokens] and the number of tokens."""
+    if cos is None or sin is None or cos.dim() != 2 or cos.shape[0] != half or cos.shape != sin.shape:
+        raise RuntimeError(f"{what}: rotation tables must be two [{half}, tokens] tensors")
+    n = cos.numel()
+    return _vector(cos, n, device, what), _vector(sin, n, device, what), n // half
+
+
+def _bind(e: _lib.Fp4Epilogue, M: int, N: int, out: torch.Tensor, residual: torch.Tensor | None, device: int, what: str) -> None:
+    """The tensors of one call into an epilogue."""
+    rows, cols, e.ldo, d = _matrix(out, what)
+    dtype = _DTYPES.get(out.dtype)
+    if d != device or dtype is None or rows != M or (cols > N // 2 if e.kind == EPI_SWIGLU else cols != N):
+        raise RuntimeError(f"{what}: out is {out.dtype} {list(out.shape)} on {out.device} for M={M} N={N} on cuda:{device}")
+    e.out_dtype, e.out, e.out_cols = dtype, out.data_ptr(), cols
     if e.kind == EPI_RESIDUAL:
-        _need(residual is not None, f"{what}: EPI_RESIDUAL needs the residual")
-        e.ldr = _rows_2d(residual, what)
-        _need(residual.shape == out.shape and residual.dtype == out.dtype and residual.device == device, f"{what}: the residual must be like out")
-        e.residual = _ptr(residual)
+        _need(residual is not None, "EPI_RESIDUAL needs the residual")
+        rows, rcols, e.ldr, d = _matrix(residual, what)
+        if d != device or residual.dtype is not out.dtype or rows != M or rcols != cols:
+            raise RuntimeError(f"{what}: the residual ({residual.dtype} {list(residual.shape)} on {residual.device}) must be like out")
+        e.residual = residual.data_ptr()
 
 
 def gemm_fp4(
@@ -452,20 +470,15 @@ def gemm_fp4(
     """4-bit A [M, K] x W [N, K] (operands of `quantize_fp4`) -> epilogue into out (see include/foidfinder_b200.h).
     `epilogue` is an EPI_* number, with `bias` and the head arguments of `fp4_epilogue`, or a prepared
     `fp4_epilogue`."""
-    M = out.shape[0]
-    _fp4_operand(A, A_scales, row_scale, M, K, fmt, "gemm_fp4")
-    _fp4_operand(W, W_scales, col_scale, N, K, fmt, "gemm_fp4")
-    _need(W.device == A.device, "gemm_fp4: A and W are on different devices")
-    e = fp4_epilogue(epilogue, N, A.device, bias=bias, **heads) if isinstance(epilogue, int) else epilogue
-    _bind_out(e, M, N, out, residual, A.device, "gemm_fp4")
-    with torch.cuda.device(A.device):
-        check(
-            lib().ff_gemm_fp4(
-                _ptr(A), _ptr(A_scales), _ptr(row_scale), _ptr(W), _ptr(W_scales), _ptr(col_scale), fmt, M, N, K,
-                C.byref(e), tile, _stream(A),
-            ),
-            "gemm_fp4",
-        )
+    M, device = out.shape[0], out.get_device()
+    a = _operand(A, A_scales, row_scale, M, K, fmt, device, "gemm_fp4")
+    w = _operand(W, W_scales, col_scale, N, K, fmt, device, "gemm_fp4")
+    if isinstance(epilogue, int):
+        e = fp4_epilogue(epilogue, N, out.device, bias=bias, **heads)
+    else:
+        e = _lib.Fp4Epilogue.from_buffer_copy(epilogue)
+    _bind(e, M, N, out, residual, device, "gemm_fp4")
+    _launch("gemm_fp4", lib().ff_gemm_fp4, device, *a, *w, fmt, M, N, K, C.byref(e), tile)
 
 
 def linear_fp4(
@@ -487,24 +500,30 @@ def linear_fp4(
 ) -> None:
     """quantize_fp4 of x [M, K] (with the LayerNorm, if gamma is given) and gemm_fp4 in one call; the codes of x live
     in a workspace from torch's allocator on the current stream."""
-    ldx = _rows_2d(x, "linear_fp4")
-    M, K = x.shape
-    _need(x.dtype in _DTYPES, "linear_fp4: x must be fp16, bf16 or f32")
-    _fp4_operand(W, W_scales, col_scale, N, K, fmt, "linear_fp4")
-    _need(W.device == x.device, "linear_fp4: x and W are on different devices")
-    _params(K, x.device, "linear_fp4", gamma=gamma, beta=beta)
+    K, device = x.shape[-1], x.get_device()
+    w = _operand(W, W_scales, col_scale, N, K, fmt, device, "linear_fp4")
+    g, b = _vector(gamma, K, device, "linear_fp4: gamma"), _vector(beta, K, device, "linear_fp4: beta")
     e = fp4_epilogue(epilogue, N, x.device, bias=bias, **heads) if isinstance(epilogue, int) else epilogue
-    _bind_out(e, M, N, out, residual, x.device, "linear_fp4")
-    with torch.cuda.device(x.device):
-        nbytes = lib().ff_linear_fp4_workspace_bytes(M, K, fmt)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        check(
-            lib().ff_linear_fp4(
-                _ptr(x), _DTYPES[x.dtype], ldx, _ptr(gamma), _ptr(beta), eps, _ptr(W), _ptr(W_scales), _ptr(col_scale),
-                fmt, M, N, K, C.byref(e), _ptr(ws), nbytes, _stream(x),
-            ),
-            "linear_fp4",
-        )
+    _linear(x, w, fmt, N, K, g, b, eps, e, out, residual)
+
+
+def _linear(x, w, fmt, N, K, gamma, beta, eps, epilogue, out, residual) -> None:
+    """ff_linear_fp4 with the weight's and the norm's addresses."""
+    M, cols, ldx, device = _matrix(x, "linear_fp4")
+    dtype = _DTYPES.get(x.dtype)
+    if dtype is None or cols != K:
+        raise RuntimeError(f"linear_fp4: x must be fp16, bf16 or f32 [M, {K}], got {x.dtype} {list(x.shape)}")
+    e = _lib.Fp4Epilogue.from_buffer_copy(epilogue)
+    _bind(e, M, N, out, residual, device, "linear_fp4")
+    nbytes = _linear_workspace(M, K, fmt)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    _launch("linear_fp4", lib().ff_linear_fp4, device, x.data_ptr(), dtype, ldx, gamma, beta, eps, *w, fmt, M, N, K, C.byref(e), ws.data_ptr(), nbytes)
+
+
+def _linear_workspace(M: int, K: int, fmt: int) -> int:
+    """ff_linear_fp4_workspace_bytes: codes, scales and row scales, each rounded up to 256 bytes."""
+    codes, scales = fp4_sizes(M, K, fmt)
+    return (codes + 255 & ~255) + (scales + 255 & ~255) + (4 * M + 255 & ~255)
 
 
 def qk_norm_rope(
@@ -527,20 +546,18 @@ def qk_norm_rope(
     """x [T, >= (q_heads + k_heads) * head_dim] fp16 or bf16, q heads then k heads -> every head normalised ("rms" or
     "layer") and rotated by position row % tokens, into the first columns of out (x itself: in place). Tables are
     angle-major [head_dim / 2, tokens] f32; `pairing` "pairs" rotates (2i, 2i + 1), "halves" (i, i + head_dim / 2)."""
-    ldx, ldo = _rows_2d(x, "qk_norm_rope"), _rows_2d(out, "qk_norm_rope")
-    cols = (q_heads + k_heads) * head_dim
-    _need(x.dtype in (torch.float16, torch.bfloat16) and out.dtype == x.dtype, "qk_norm_rope: x and out must be fp16 or bf16, alike")
-    _need(x.shape[1] >= cols and out.shape[1] >= cols and out.shape[0] == x.shape[0] and out.device == x.device, "qk_norm_rope: shapes")
-    _need(norm in _NORMS and pairing in _PAIRINGS, "qk_norm_rope: norm is 'rms' or 'layer', pairing 'pairs' or 'halves'")
-    _params(head_dim, x.device, "qk_norm_rope", q_weight=q_weight, k_weight=k_weight, q_bias=q_bias, k_bias=k_bias)
-    _need(rope_cos.dim() == 2 and rope_cos.shape[0] == head_dim // 2 and rope_sin.shape == rope_cos.shape, "qk_norm_rope: rotation tables must be [head_dim / 2, tokens]")
-    _params(rope_cos.numel(), x.device, "qk_norm_rope", rope_cos=rope_cos, rope_sin=rope_sin)
-    with torch.cuda.device(x.device):
-        check(
-            lib().ff_qk_norm_rope(
-                _ptr(x), _DTYPES[x.dtype], ldx, _ptr(out), ldo, x.shape[0], q_heads, k_heads, head_dim, _NORMS[norm],
-                _ptr(q_weight), _ptr(q_bias), _ptr(k_weight), _ptr(k_bias), eps, _ptr(rope_cos), _ptr(rope_sin),
-                rope_cos.shape[1], _PAIRINGS[pairing], _stream(x),
-            ),
-            "qk_norm_rope",
-        )
+    rows, xcols, ldx, device = _matrix(x, "qk_norm_rope")
+    orows, ocols, ldo, odevice = _matrix(out, "qk_norm_rope")
+    cols, dtype = (q_heads + k_heads) * head_dim, x.dtype
+    if dtype is torch.float32 or dtype not in _DTYPES or out.dtype is not dtype:
+        raise RuntimeError(f"qk_norm_rope: x and out must be fp16 or bf16, alike, got {dtype} and {out.dtype}")
+    if xcols < cols or ocols < cols or orows != rows or odevice != device:
+        raise RuntimeError(f"qk_norm_rope: x {list(x.shape)} and out {list(out.shape)} must hold {cols} columns of the same rows on one device")
+    n, p = _NORMS.get(norm), _PAIRINGS.get(pairing)
+    _need(n is not None and p is not None, "qk_norm_rope: norm is 'rms' or 'layer', pairing 'pairs' or 'halves'")
+    what = "qk_norm_rope"
+    qw, qb = _vector(q_weight, head_dim, device, what), _vector(q_bias, head_dim, device, what)
+    kw, kb = _vector(k_weight, head_dim, device, what), _vector(k_bias, head_dim, device, what)
+    cos, sin, tokens = _tables(rope_cos, rope_sin, head_dim // 2, device, what)
+    _launch(what, lib().ff_qk_norm_rope, device, x.data_ptr(), _DTYPES[dtype], ldx, out.data_ptr(), ldo, rows, q_heads, k_heads, head_dim, n,
+            qw, qb, kw, kb, eps, cos, sin, tokens, p)

@@ -51,6 +51,9 @@ def test_epilogue_layout_matches_ctypes(tmp_path):
 @pytest.mark.parametrize(("rows", "cols"), [(1, 1), (128, 256), (129, 257), (1025, 1024), (300, 2730)])
 def test_buffer_sizes(rows, cols, fmt):
     codes, scales = ops.fp4_sizes(rows, cols, fp4.FORMATS[fmt])
+    lib = _lib.lib()
+    assert (codes, scales) == (lib.ff_fp4_code_bytes(rows, cols), lib.ff_fp4_scale_bytes(rows, cols, fp4.FORMATS[fmt]))
+    assert ops._linear_workspace(rows, cols, fp4.FORMATS[fmt]) == lib.ff_linear_fp4_workspace_bytes(rows, cols, fp4.FORMATS[fmt])
     assert codes == rows * (-(-cols // 32) * 16)
     tiles = -(-rows // 128) * 128
     assert scales == tiles * (-(-cols // 256) * 256 // O.BLOCK[fmt])
@@ -68,6 +71,7 @@ def test_buffer_sizes_of_bad_arguments_are_zero():
 def test_long_buffers_do_not_wrap():
     assert ops.fp4_sizes(1 << 20, 1 << 14, 0)[0] == 1 << 33
     assert ops.fp4_sizes(1 << 20, 1 << 14, 0)[1] == 1 << 30
+    assert _lib.lib().ff_fp4_code_bytes(1 << 20, 1 << 14) == 1 << 33
 
 
 @pytest.mark.parametrize(("args", "msg"), [
