@@ -12,8 +12,8 @@
 //
 // Bound by HBM: 2 bytes read and 0.56 (NV) or 0.53 (MX) written per value. The whole row stays in registers,
 // 16 consecutive columns per lane, so a 16-column block never leaves its lane and a 32-column block is a pair
-// of lanes; WPR warps share a row so that a lane holds at most 48 values. CTAs are persistent: a warp loads its
-// next row while it works on this one, and gamma and beta come from shared memory, filled once.
+// of lanes; the warps of a row are as many as leave each lane 32 values. CTAs are persistent, and gamma
+// and beta come from shared memory, filled once.
 #include <type_traits>
 
 #include "common.h"
@@ -35,13 +35,15 @@ struct Raw {
 
 template <class T, bool ALIGNED>
 __device__ __forceinline__ void load_raw(const T* __restrict__ xr, int col, int cols, Raw<T, ALIGNED>& r) {
-  const uintptr_t a = reinterpret_cast<uintptr_t>(xr + col), end = reinterpret_cast<uintptr_t>(xr + cols);
-  const uintptr_t base = ALIGNED ? a : a & ~uintptr_t(15);
+  constexpr int E = 16 / sizeof(T);  // values per granule
   constexpr int N = Raw<T, ALIGNED>::W / 4 + (ALIGNED ? 0 : 1);
+  // values between the granule's start and the row's (the same for all columns)
+  const int mis = ALIGNED ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(xr) & 15u) / static_cast<int>(sizeof(T));
+  const uint4* base = reinterpret_cast<const uint4*>(xr + col - mis);
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     uint4 u = make_uint4(0, 0, 0, 0);
-    if (col < cols && base + 16 * j < end) u = __ldg(reinterpret_cast<const uint4*>(base) + j);
+    if (col < cols && col + E * j - mis < cols) u = __ldg(base + j);
     r.t[4 * j] = u.x;
     r.t[4 * j + 1] = u.y;
     r.t[4 * j + 2] = u.z;
@@ -105,32 +107,31 @@ __device__ __forceinline__ void load16(const T* __restrict__ xr, int col, int co
   to_f32<T, false>(r, v);
 }
 
-// |.| maximum that keeps a NaN.
-__device__ __forceinline__ float max_nan(float a, float b) {
+// Maximum of magnitudes that keeps a NaN.
+__device__ __forceinline__ float max_nan(float a, float b, float c = 0.f) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 __device__ __forceinline__ float amax16(const float (&v)[16]) {
-  float m[4] = {0.f, 0.f, 0.f, 0.f};  // four chains
+  float m[2] = {0.f, 0.f};  // two chains
 #pragma unroll
-  for (int e = 0; e < 16; ++e) m[e & 3] = max_nan(m[e & 3], fabsf(v[e]));
-  return max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3]));
+  for (int e = 0; e < 16; e += 2) m[(e >> 1) & 1] = max_nan(m[(e >> 1) & 1], v[e], v[e + 1]);
+  return max_nan(m[0], m[1]);
 }
-// The same on 16-bit pairs as loaded: half the instructions.
+// The same on 16-bit pairs as loaded (the running maximum's sign is not meaningful until the end).
 template <class T>
 __device__ __forceinline__ float amax_pairs(const uint32_t* w) {
   uint32_t m[2] = {0, 0};
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const uint32_t v = w[e] & 0x7fff7fffu;
     if constexpr (std::is_same<T, __half>::value)
-      asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(m[e & 1]) : "r"(v));
+      asm("max.NaN.xorsign.abs.f16x2 %0, %0, %1;" : "+r"(m[e & 1]) : "r"(w[e]));
     else
-      asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(m[e & 1]) : "r"(v));
+      asm("max.NaN.xorsign.abs.bf16x2 %0, %0, %1;" : "+r"(m[e & 1]) : "r"(w[e]));
   }
   const float2 a = Pair16<T>::unpack(m[0]), b = Pair16<T>::unpack(m[1]);
-  return max_nan(max_nan(a.x, a.y), max_nan(b.x, b.y));
+  return max_nan(max_nan(a.x, a.y, b.x), b.y);
 }
 __device__ __forceinline__ bool not_finite(float amax) { return !(amax <= 3.402823466e38f); }
 
@@ -142,9 +143,10 @@ __device__ __forceinline__ float nv_row_scale(float amax) {
 }
 __device__ __forceinline__ float inv_pow2(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
 
-// v / (S s) for the code, r = 1 / (S s) rounded. kExact16: v came from a 16-bit type, so a quotient that is no
+// v / (S s) for the code, r about 1 / (S s). kExact16: v came from a 16-bit type, so a quotient that is no
 // rounding tie of e2m1 is at least 2^-13 away from one, while v * r is within 2^-20 of the quotient: rounding
-// v * r + 192 (one FMA, to multiples of 2^-16) puts true ties exactly on the tie. kExact32: IEEE division
+// v * r + 192 (one FMA, to multiples of 2^-16) puts true ties exactly on the tie (r within 2^-22 of 1 / (S s)
+// is enough). kExact32: IEEE division
 // (checkpoint weights, once per load). kPlain: v is itself rounded (after a LayerNorm) or r a power of two.
 enum QuotientKind { kPlain, kExact16, kExact32 };
 template <int KIND>
@@ -169,14 +171,23 @@ __device__ __forceinline__ uint2 codes16(const float (&v)[16], float r, float sc
   return make_uint2(e2m1x8(y[0]), e2m1x8(y[1]));
 }
 
-// One 16-column piece of an NV row with row scale s: its scale byte and codes.
+// One 16-column piece of an NV row with row scale s: its scale byte and codes. amax / (6 s) for the block scale: an
+// IEEE division for kExact32. For 16-bit inputs a true tie of e4m3 has at most 5 significant bits and any other
+// quotient is at least 2^-12 of itself away from one, so rounding the product with 1 / 6 to 16 significant bits
+// decides as the division would.
 template <int KIND>
 __device__ __forceinline__ uint32_t nv_piece(const float (&v)[16], float amax, float s, bool bad, uint2* codes) {
   const float is = inv_pow2(s);
-  const uint32_t byte = bad ? 0u : e4m3_byte(__fdiv_rn(amax * is, 6.f));
+  float t = amax * is;
+  if constexpr (KIND == kExact32)
+    t = __fdiv_rn(t, 6.f);
+  else
+    t = __uint_as_float((__float_as_uint(t * (1.f / 6.f)) + 0x40u) & ~0x7fu);
+  const uint32_t byte = bad ? 0u : e4m3_byte(t);
   const float S = e4m3_value(byte);
-  const float r = byte ? __frcp_rn(S) * is : 0.f;
-  *codes = bad ? make_uint2(0, 0) : codes16<KIND>(v, r, S * s);
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(S));
+  *codes = bad ? make_uint2(0, 0) : codes16<KIND>(v, byte ? r * is : 0.f, S * s);
   return byte;
 }
 // One 16-column piece of an MX block whose 32 columns have maximum amax. Scaling by a power of two is exact.
@@ -224,44 +235,118 @@ __device__ __forceinline__ void affine16(float (&v)[16], float mean, float rstd,
   }
 }
 
-// Codes and scale bytes of the piece at 16-column index c; lanes hold consecutive c, and 4 (NV) or 8 (MX)
-// lanes join their bytes into one 32-bit store. Every lane of the warp calls it.
+// Where a row's codes and scales go.
+struct RowOut {
+  uint8_t *codes, *scales;
+  int pitch;
+};
 template <bool MX>
-__device__ __forceinline__ void store_piece(const QuantArgs& a, int row, int c, uint2 codes, uint32_t byte, bool on) {
-  const int lane = threadIdx.x & 31;
+__device__ __forceinline__ RowOut row_out(const QuantArgs& a, int row) {
   const int64_t pitch = fp4_row_bytes(a.cols);
-  const int64_t tile = sf_tile_bytes(a.cols, MX);
-  uint32_t u = byte << (8 * (MX ? (lane >> 1) & 3 : lane & 3));
-  u |= __shfl_xor_sync(0xffffffffu, u, MX ? 2 : 1);
-  u |= __shfl_xor_sync(0xffffffffu, u, MX ? 4 : 2);
-  if (!on) return;
-  if (8 * static_cast<int64_t>(c) < pitch) *reinterpret_cast<uint2*>(a.codes + row * pitch + 8 * static_cast<int64_t>(c)) = codes;
-  if ((lane & (MX ? 7 : 3)) == 0)
-    *reinterpret_cast<uint32_t*>(a.scales + sf_offset(row, MX ? c >> 1 : c, tile)) = u;
+  return {a.codes + row * pitch, a.scales + sf_offset(row, 0, sf_tile_bytes(a.cols, MX)), static_cast<int>(pitch)};
+}
+// Codes and scale byte of the piece at 16-column index c. Lanes hold consecutive c: the warp's byte stores fall into
+// whole 4-byte groups of the scale chunks.
+template <bool MX>
+__device__ __forceinline__ void store_piece(const RowOut& o, int c, int pieces, uint2 codes, uint32_t byte) {
+  if (c >= pieces) return;
+  if (8 * c < o.pitch) *reinterpret_cast<uint2*>(o.codes + 8 * c) = codes;
+  if (MX) {
+    if ((c & 1) == 0) o.scales[(c >> 3) * kSfChunk + ((c >> 1) & 3)] = static_cast<uint8_t>(byte);
+  } else {
+    o.scales[(c >> 2) * kSfChunk + (c & 3)] = static_cast<uint8_t>(byte);
+  }
 }
 
 // gamma and beta in shared memory, zero past the row's end: 16 bytes j of piece c at float4 index
 // 4 c + (j ^ (c / 2) % 4), so that lanes with consecutive pieces read from all banks.
 __device__ __forceinline__ int norm_slot(int c, int j) { return 4 * c + (j ^ ((c >> 1) & 3)); }
+__device__ __forceinline__ void fill_norm(float4* norm_s, const QuantArgs& a, int pieces) {
+  for (int i = threadIdx.x; i < pieces * 4; i += blockDim.x) {
+    const int c = i >> 2, j = i & 3;
+    float g[4], b[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int col = 16 * c + 4 * j + e;
+      g[e] = col < a.cols ? __ldg(a.gamma + col) : 0.f;
+      b[e] = col < a.cols ? __ldg(a.beta + col) : 0.f;
+    }
+    norm_s[norm_slot(c, j)] = make_float4(g[0], g[1], g[2], g[3]);
+    norm_s[4 * pieces + norm_slot(c, j)] = make_float4(b[0], b[1], b[2], b[3]);
+  }
+}
 
-// WPR warps per row, NC pieces of 16 columns per lane: rows of up to 512 * WPR * NC columns.
-template <class T, bool MX, bool NORM, bool ALIGNED, int WPR, int NC>
-__global__ void __launch_bounds__(kQuantThreads) quantize_fp4_kernel(const QuantArgs a) {
-  constexpr int WARPS = kQuantThreads / 32;
-  constexpr int RPC = WARPS / WPR;  // rows per CTA
-  extern __shared__ float4 norm_s[];  // gamma, then beta
-  __shared__ float red[2][3][WARPS];
+// Rows of 16-bit values without a norm, one warp per row: the row stays in registers as loaded (8 words per 16
+// values), its maxima are taken on pairs, and it is unpacked once, for the codes. No barriers and few registers:
+// NW pieces of 16 columns per lane, rows of up to 512 * NW columns.
+template <int NW>
+__host__ __device__ constexpr int row_ctas() {  // CTAs of 256 threads per SM that the registers are held to
+  return NW <= 3 ? 4 : NW <= 6 ? 3 : 2;
+}
+template <class T, bool MX, bool ALIGNED, int NW>
+__global__ void __launch_bounds__(kQuantThreads, row_ctas<NW>()) quantize_fp4_rows_kernel(const QuantArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int grp = warp / WPR, wr = warp % WPR;
+  constexpr int WARPS = kQuantThreads / 32;
+  const int pieces = (a.cols + kFp4Step - 1) / kFp4Step * (kFp4Step / 16);
+  pdl_wait();
+  pdl_trigger();
+  for (int row = static_cast<int>(blockIdx.x) * WARPS + warp; row < a.rows; row += static_cast<int>(gridDim.x) * WARPS) {
+    const T* xr = static_cast<const T*>(a.x) + row * a.ldx;
+    const RowOut o = row_out<MX>(a, row);
+    Raw<T, ALIGNED> raw[NW];
+#pragma unroll
+    for (int i = 0; i < NW; ++i) load_raw<T, ALIGNED>(xr, (i * 32 + lane) * 16, a.cols, raw[i]);
+    float amax[NW];
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      realign<T, ALIGNED>(xr, (i * 32 + lane) * 16, a.cols, raw[i]);
+      amax[i] = amax_pairs<T>(raw[i].t);
+    }
+    float s = 1.f;
+    bool bad = false;
+    if constexpr (!MX) {
+      float m = amax[0];
+#pragma unroll
+      for (int i = 1; i < NW; ++i) m = max_nan(m, amax[i]);
+#pragma unroll
+      for (int k = 16; k; k >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, k));
+      bad = not_finite(m);
+      s = nv_row_scale(bad ? 0.f : m);
+      if (lane == 0) a.row_scale[row] = bad ? __uint_as_float(0x7fffffffu) : s;
+    }
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      float v[16];
+      to_f32<T, ALIGNED>(raw[i], v);
+      uint2 codes;
+      uint32_t byte;
+      if constexpr (MX)
+        byte = mx_piece(v, max_nan(amax[i], __shfl_xor_sync(0xffffffffu, amax[i], 1)), &codes);
+      else
+        byte = nv_piece<kExact16>(v, amax[i], s, bad, &codes);
+      store_piece<MX>(o, i * 32 + lane, pieces, codes, byte);
+    }
+  }
+}
+
+// wpr warps per row, NC pieces of 16 columns per lane: rows of up to 512 * wpr * NC columns. Two pieces per lane and
+// few registers beat three pieces.
+constexpr int NC = 2;
+template <class T, bool MX, bool NORM, bool ALIGNED>
+__global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 2 ? 4 : 2) quantize_fp4_kernel(const QuantArgs a, const int wpr) {
+  extern __shared__ float4 norm_s[];  // gamma, then beta
+  __shared__ float red[2][3][kQuantThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rpc = static_cast<int>(blockDim.x >> 5) / wpr;  // rows per CTA
+  const int grp = warp / wpr, wr = warp - grp * wpr;
   const int pieces = (a.cols + kFp4Step - 1) / kFp4Step * (kFp4Step / 16);
   int parity = 0;
-  auto row_all = [&](float v, int slot, auto op) {  // over the WPR warps of the row, after a warp reduction
-    if constexpr (WPR > 1) {
+  auto row_all = [&](float v, int slot, auto op) {  // over the warps of the row, after a warp reduction
+    if (wpr > 1) {
       if (lane == 0) red[parity][slot][warp] = v;
-      asm volatile("bar.sync %0, %1;" ::"r"(1 + grp), "n"(32 * WPR) : "memory");
-      v = red[parity][slot][grp * WPR];
-#pragma unroll
-      for (int i = 1; i < WPR; ++i) v = op(v, red[parity][slot][grp * WPR + i]);
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + grp), "r"(32 * wpr) : "memory");
+      v = red[parity][slot][grp * wpr];
+      for (int i = 1; i < wpr; ++i) v = op(v, red[parity][slot][grp * wpr + i]);
     }
     return v;
   };
@@ -269,40 +354,22 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_fp4_kernel(const Quant
   pdl_wait();
   pdl_trigger();
   if constexpr (NORM) {
-    for (int i = threadIdx.x; i < pieces * 4; i += kQuantThreads) {
-      const int c = i >> 2, j = i & 3;
-      float g[4], b[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int col = 16 * c + 4 * j + e;
-        g[e] = col < a.cols ? __ldg(a.gamma + col) : 0.f;
-        b[e] = col < a.cols ? __ldg(a.beta + col) : 0.f;
-      }
-      norm_s[norm_slot(c, j)] = make_float4(g[0], g[1], g[2], g[3]);
-      norm_s[4 * pieces + norm_slot(c, j)] = make_float4(b[0], b[1], b[2], b[3]);
-    }
+    fill_norm(norm_s, a, pieces);
     __syncthreads();
   }
-  const int step = static_cast<int>(gridDim.x) * RPC;
-  int row = static_cast<int>(blockIdx.x) * RPC + grp;
-  const T* xr = static_cast<const T*>(a.x) + row * a.ldx;
-  Raw<T, ALIGNED> raw[NC];
-  if (row < a.rows) {
-#pragma unroll
-    for (int i = 0; i < NC; ++i) load_raw<T, ALIGNED>(xr, ((i * WPR + wr) * 32 + lane) * 16, a.cols, raw[i]);
-  }
+  const int step = static_cast<int>(gridDim.x) * rpc;
+  int row = static_cast<int>(blockIdx.x) * rpc + grp;
   for (; row < a.rows; row += step, parity ^= 1) {
+    const RowOut o = row_out<MX>(a, row);
+    const T* xr = static_cast<const T*>(a.x) + row * a.ldx;
+    Raw<T, ALIGNED> raw[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) load_raw<T, ALIGNED>(xr, ((i * wpr + wr) * 32 + lane) * 16, a.cols, raw[i]);
     float v[NC][16], amax[NC];
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      realign<T, ALIGNED>(xr, ((i * WPR + wr) * 32 + lane) * 16, a.cols, raw[i]);
-      if constexpr (!NORM && sizeof(T) == 2) amax[i] = amax_pairs<T>(raw[i].t);
+      realign<T, ALIGNED>(xr, ((i * wpr + wr) * 32 + lane) * 16, a.cols, raw[i]);
       to_f32<T, ALIGNED>(raw[i], v[i]);
-    }
-    if (row + step < a.rows) {  // the next row comes in meanwhile
-      xr += step * a.ldx;
-#pragma unroll
-      for (int i = 0; i < NC; ++i) load_raw<T, ALIGNED>(xr, ((i * WPR + wr) * 32 + lane) * 16, a.cols, raw[i]);
     }
     if constexpr (NORM) {
       float2 s2 = make_float2(0.f, 0.f);
@@ -315,7 +382,7 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_fp4_kernel(const Quant
       float2 q2 = make_float2(0.f, 0.f);
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
-        const int col = ((i * WPR + wr) * 32 + lane) * 16;
+        const int col = ((i * wpr + wr) * 32 + lane) * 16;
 #pragma unroll
         for (int e = 0; e < 16; e += 2) {
           const float2 d = add2(make_float2(v[i][e], v[i][e + 1]), make_float2(-mean, -mean));
@@ -336,7 +403,7 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_fp4_kernel(const Quant
       const float rstd = rsqrtf(row_all(warp_sum(q2.x + q2.y), 1, plus) / n + a.eps);
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
-        const int c = (i * WPR + wr) * 32 + lane;
+        const int c = (i * wpr + wr) * 32 + lane;
         if (c < pieces) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -352,10 +419,8 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_fp4_kernel(const Quant
         }
       }
     }
-    if constexpr (NORM || sizeof(T) == 4) {
 #pragma unroll
-      for (int i = 0; i < NC; ++i) amax[i] = amax16(v[i]);
-    }
+    for (int i = 0; i < NC; ++i) amax[i] = amax16(v[i]);
     float s = 1.f;
     bool bad = false;
     if constexpr (!MX) {
@@ -371,14 +436,14 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_fp4_kernel(const Quant
     }
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int c = (i * WPR + wr) * 32 + lane;
+      const int c = (i * wpr + wr) * 32 + lane;
       uint2 codes;
       uint32_t byte;
       if constexpr (MX)
         byte = mx_piece(v[i], max_nan(amax[i], __shfl_xor_sync(0xffffffffu, amax[i], 1)), &codes);
       else
         byte = nv_piece<quotient_kind<T, NORM>()>(v[i], amax[i], s, bad, &codes);
-      store_piece<MX>(a, row, c, codes, byte, c < pieces);
+      store_piece<MX>(o, c, pieces, codes, byte);
     }
   }
 }
@@ -390,6 +455,7 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_fp4_wide_kernel(const 
   __shared__ float red[kQuantThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row = blockIdx.x;
+  const RowOut o = row_out<MX>(a, row);
   const T* xr = static_cast<const T*>(a.x) + row * a.ldx;
   auto cta_all = [&](float v, auto op) {
 #pragma unroll
@@ -452,40 +518,50 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_fp4_wide_kernel(const 
     } else {
       byte = nv_piece<quotient_kind<T, NORM>()>(v, amax16(v), s, bad, &codes);
     }
-    store_piece<MX>(a, row, c, codes, byte, c < pieces);
+    store_piece<MX>(o, c, pieces, codes, byte);
   }
 }
 
-template <class T, bool MX, bool NORM, bool ALIGNED, int WPR, int NC>
-int launch_quant(const QuantArgs& a, cudaStream_t stream) {
-  constexpr int RPC = kQuantThreads / 32 / WPR;
-  auto kernel = quantize_fp4_kernel<T, MX, NORM, ALIGNED, WPR, NC>;
-  const size_t smem = NORM ? static_cast<size_t>((a.cols + kFp4Step - 1) / kFp4Step) * kFp4Step * 8 : 0;
-  static int per_sm[64] = {};  // resident CTAs per SM, 0 = not configured yet (widest row of the instantiation)
-  int dev = 0;
-  cudaGetDevice(&dev);
-  int most = dev >= 0 && dev < 64 ? per_sm[dev] : 0;
-  if (most == 0) {
-    const size_t widest = NORM ? 512 * WPR * NC * 8 : 0;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(widest)) != cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&most, kernel, kQuantThreads, widest) != cudaSuccess || most < 1)
-      return check_launch("quantize_fp4: configuration");
-    if (dev >= 0 && dev < 64) per_sm[dev] = most;
-  }
-  const int want = (a.rows + RPC - 1) / RPC, full = most * sm_count();
-  launch(kernel, dim3(want < full ? want : full), dim3(kQuantThreads), smem, stream, a);
-  return check_launch("quantize_fp4_kernel");
+template <class T, bool MX, bool ALIGNED, int NW>
+int launch_rows(const QuantArgs& a, cudaStream_t stream) {
+  const int want = (a.rows + kQuantThreads / 32 - 1) / (kQuantThreads / 32), full = row_ctas<NW>() * sm_count();
+  launch(quantize_fp4_rows_kernel<T, MX, ALIGNED, NW>, dim3(want < full ? want : full), dim3(kQuantThreads), 0, stream, a);
+  return check_launch("quantize_fp4_rows_kernel");
 }
 
 template <class T, bool MX, bool NORM, bool ALIGNED>
 int dispatch_quant(const QuantArgs& a, cudaStream_t stream) {
   const int cols = (a.cols + kFp4Step - 1) / kFp4Step * kFp4Step;  // the padded scales are written too
-  if (cols <= 1024) return launch_quant<T, MX, NORM, ALIGNED, 1, 2>(a, stream);
-  if (cols <= 1536) return launch_quant<T, MX, NORM, ALIGNED, 1, 3>(a, stream);
-  if (cols <= 3 * 1024) return launch_quant<T, MX, NORM, ALIGNED, 2, 3>(a, stream);
-  if (cols <= 6 * 1024) return launch_quant<T, MX, NORM, ALIGNED, 4, 3>(a, stream);
-  launch(quantize_fp4_wide_kernel<T, MX, NORM>, dim3(a.rows), dim3(kQuantThreads), 0, stream, a);
-  return check_launch("quantize_fp4_wide_kernel");
+  if constexpr (sizeof(T) == 2 && !NORM) {
+    if (cols <= 1024) return launch_rows<T, MX, ALIGNED, 2>(a, stream);
+    if (cols <= 1536) return launch_rows<T, MX, ALIGNED, 3>(a, stream);
+    if (cols <= 3 * 1024) return launch_rows<T, MX, ALIGNED, 6>(a, stream);
+    if (cols <= 5 * 1024) return launch_rows<T, MX, ALIGNED, 10>(a, stream);
+  }
+  const int wpr = (cols + 512 * NC - 1) / (512 * NC);
+  constexpr int WARPS = kQuantThreads / 32;
+  if (wpr > WARPS) {
+    launch(quantize_fp4_wide_kernel<T, MX, NORM>, dim3(a.rows), dim3(kQuantThreads), 0, stream, a);
+    return check_launch("quantize_fp4_wide_kernel");
+  }
+  const int rpc = WARPS / wpr, threads = 32 * wpr * rpc;
+  auto kernel = quantize_fp4_kernel<T, MX, NORM, ALIGNED>;
+  const size_t smem = NORM ? static_cast<size_t>(cols) * 8 : 0;
+  static int per_sm[64][WARPS] = {};  // resident CTAs per device and wpr, 0 = not configured yet
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const bool known = dev >= 0 && dev < 64;
+  int most = known ? per_sm[dev][wpr - 1] : 0;
+  if (most == 0) {
+    constexpr int widest = 512 * NC * WARPS * 8;  // gamma and beta of the widest rows
+    if ((NORM && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, widest) != cudaSuccess) ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&most, kernel, threads, NORM ? 512 * NC * wpr * 8 : 0) != cudaSuccess || most < 1)
+      return check_launch("quantize_fp4: configuration");
+    if (known) per_sm[dev][wpr - 1] = most;
+  }
+  const int want = (a.rows + rpc - 1) / rpc, full = most * sm_count();
+  launch(kernel, dim3(want < full ? want : full), dim3(threads), smem, stream, a, wpr);
+  return check_launch("quantize_fp4_kernel");
 }
 
 template <class T, bool MX, bool NORM>
@@ -535,8 +611,32 @@ __global__ void __launch_bounds__(256)
       const uint32_t byte = __ldg(srow + static_cast<int64_t>(blk >> 2) * kSfChunk + (blk & 3));
       return MX ? e8m0_value(byte) : e4m3_value(byte) * s;
     };
+    auto pack = [&](const float(&v)[8]) {
+      if constexpr (sizeof(T) == 4)
+        return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+      else
+        return make_uint4(Pair16<T>::pack(v[0], v[1]), Pair16<T>::pack(v[2], v[3]), Pair16<T>::pack(v[4], v[5]),
+                          Pair16<T>::pack(v[6], v[7]));
+    };
+    int c0 = lane * E - off;  // the granule's first column, may be negative
+    if (off == 0) {  // whole granules of an aligned row lie in one block
 #pragma unroll 4
-    for (int c0 = lane * E - off; c0 < cols; c0 += 32 * E) {  // c0: the granule's first column, may be negative
+      for (; c0 + E <= cols; c0 += 32 * E) {
+        uint32_t h[4];
+        e2m1x8_to_half2(__ldg(crow + (c0 >> 3)) >> (4 * (c0 & 7)), h);
+        const float sc = scale_at(c0 / B);
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          const float2 f = mul2(unpack_half2(h[e / 2]), make_float2(sc, sc));
+          v[e] = f.x;
+          v[e + 1] = f.y;
+        }
+        *reinterpret_cast<uint4*>(orow + c0) = pack(v);
+      }
+    }
+#pragma unroll 2
+    for (; c0 < cols; c0 += 32 * E) {
       if (c0 + E <= 0) continue;
       // codes of columns [c0, c0 + E): one aligned word, or two when the row is not aligned
       const int w0 = c0 >> 3, sh = 4 * (c0 & 7);
@@ -556,13 +656,7 @@ __global__ void __launch_bounds__(256)
         v[e] = ((e & 1) ? f.y : f.x) * (c0 + e >= cut ? s1 : s0);
       }
       if (c0 >= 0 && c0 + E <= cols) {
-        uint4 u;
-        if constexpr (sizeof(T) == 4)
-          u = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-        else
-          u = make_uint4(Pair16<T>::pack(v[0], v[1]), Pair16<T>::pack(v[2], v[3]), Pair16<T>::pack(v[4], v[5]),
-                         Pair16<T>::pack(v[6], v[7]));
-        *reinterpret_cast<uint4*>(orow + c0) = u;
+        *reinterpret_cast<uint4*>(orow + c0) = pack(v);
       } else {
 #pragma unroll
         for (int e = 0; e < E; ++e)
