@@ -35,7 +35,7 @@ __host__ __device__ constexpr int64_t sf_offset(int row, int blk, int64_t tile_b
 
 // ---------------------------------------------------------------- conversions
 // Eight f32 -> eight e2m1 codes, element i in bits [4i, 4i + 4): round to nearest even, saturating at +-6.
-__device__ __forceinline__ uint32_t e2m1x8(const float (&y)[8]) {
+__device__ __forceinline__ uint32_t e2m1x8(const float2* y) {
   uint32_t r;
   asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
       "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
@@ -44,7 +44,7 @@ __device__ __forceinline__ uint32_t e2m1x8(const float (&y)[8]) {
       "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
       "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
       : "=r"(r)
-      : "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7]));
+      : "f"(y[0].x), "f"(y[0].y), "f"(y[1].x), "f"(y[1].y), "f"(y[2].x), "f"(y[2].y), "f"(y[3].x), "f"(y[3].y));
   return r;
 }
 // Eight e2m1 codes -> four half2 (exact).

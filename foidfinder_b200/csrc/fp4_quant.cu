@@ -52,7 +52,7 @@ __device__ __forceinline__ void load_raw(const T* __restrict__ xr, int col, int 
 }
 
 // The loaded words shifted into place, values at or past the row's end zero.
-template <class T, bool ALIGNED>
+template <class T, bool ALIGNED, bool WHOLE = false>
 __device__ __forceinline__ void realign(const T* xr, int col, int cols, Raw<T, ALIGNED>& r) {
   constexpr int W = Raw<T, ALIGNED>::W;
   if constexpr (!ALIGNED) {
@@ -69,7 +69,7 @@ __device__ __forceinline__ void realign(const T* xr, int col, int cols, Raw<T, A
 #pragma unroll
     for (int i = 0; i < W; ++i) r.t[i] = __funnelshift_r(r.t[i], r.t[i + 1], sh);
   }
-  if (col + 16 > cols) {
+  if (!WHOLE && col + 16 > cols) {
 #pragma unroll
     for (int i = 0; i < W; ++i) {
       if constexpr (sizeof(T) == 4) {
@@ -84,23 +84,23 @@ __device__ __forceinline__ void realign(const T* xr, int col, int cols, Raw<T, A
   }
 }
 
+template <class T>
+__device__ __forceinline__ float2 unpack16(uint32_t w) {
+  if constexpr (sizeof(T) == 2)
+    return Pair16<T>::unpack(w);
+  else
+    return make_float2(0.f, 0.f);
+}
 template <class T, bool ALIGNED>
-__device__ __forceinline__ void to_f32(const Raw<T, ALIGNED>& r, float (&v)[16]) {
-  if constexpr (sizeof(T) == 4) {
+__device__ __forceinline__ void to_f32(const Raw<T, ALIGNED>& r, float2 (&v)[8]) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(r.t[e]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float2 f = Pair16<T>::unpack(r.t[e]);
-      v[2 * e] = f.x;
-      v[2 * e + 1] = f.y;
-    }
-  }
+  for (int e = 0; e < 8; ++e)
+    v[e] = sizeof(T) == 4 ? make_float2(__uint_as_float(r.t[sizeof(T) == 4 ? 2 * e : 0]), __uint_as_float(r.t[sizeof(T) == 4 ? 2 * e + 1 : 0]))
+                          : unpack16<T>(r.t[e]);
 }
 
 template <class T>
-__device__ __forceinline__ void load16(const T* __restrict__ xr, int col, int cols, float (&v)[16]) {
+__device__ __forceinline__ void load16(const T* __restrict__ xr, int col, int cols, float2 (&v)[8]) {
   Raw<T, false> r;
   load_raw<T, false>(xr, col, cols, r);
   realign<T, false>(xr, col, cols, r);
@@ -113,10 +113,10 @@ __device__ __forceinline__ float max_nan(float a, float b, float c = 0.f) {
   asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-__device__ __forceinline__ float amax16(const float (&v)[16]) {
+__device__ __forceinline__ float amax16(const float2 (&v)[8]) {
   float m[2] = {0.f, 0.f};  // two chains
 #pragma unroll
-  for (int e = 0; e < 16; e += 2) m[(e >> 1) & 1] = max_nan(m[(e >> 1) & 1], v[e], v[e + 1]);
+  for (int e = 0; e < 8; ++e) m[e & 1] = max_nan(m[e & 1], v[e].x, v[e].y);
   return max_nan(m[0], m[1]);
 }
 // The same on 16-bit pairs as loaded (the running maximum's sign is not meaningful until the end).
@@ -160,15 +160,11 @@ __device__ __forceinline__ float2 quotient2(float2 v, float r, float scale) {
 }
 
 template <int KIND>
-__device__ __forceinline__ uint2 codes16(const float (&v)[16], float r, float scale) {
-  float y[2][8];
+__device__ __forceinline__ uint2 codes16(const float2 (&v)[8], float r, float scale) {
+  float2 q[8];
 #pragma unroll
-  for (int e = 0; e < 16; e += 2) {
-    const float2 q = quotient2<KIND>(make_float2(v[e], v[e + 1]), r, scale);
-    y[e >> 3][e & 7] = q.x;
-    y[e >> 3][(e & 7) + 1] = q.y;
-  }
-  return make_uint2(e2m1x8(y[0]), e2m1x8(y[1]));
+  for (int e = 0; e < 8; ++e) q[e] = quotient2<KIND>(v[e], r, scale);
+  return make_uint2(e2m1x8(q), e2m1x8(q + 4));
 }
 
 // One 16-column piece of an NV row with row scale s: its scale byte and codes. amax / (6 s) for the block scale: an
@@ -176,7 +172,7 @@ __device__ __forceinline__ uint2 codes16(const float (&v)[16], float r, float sc
 // quotient is at least 2^-12 of itself away from one, so rounding the product with 1 / 6 to 16 significant bits
 // decides as the division would.
 template <int KIND>
-__device__ __forceinline__ uint32_t nv_piece(const float (&v)[16], float amax, float s, bool bad, uint2* codes) {
+__device__ __forceinline__ uint32_t nv_piece(const float2 (&v)[8], float amax, float s, bool bad, uint2* codes) {
   const float is = inv_pow2(s);
   float t = amax * is;
   if constexpr (KIND == kExact32)
@@ -191,7 +187,7 @@ __device__ __forceinline__ uint32_t nv_piece(const float (&v)[16], float amax, f
   return byte;
 }
 // One 16-column piece of an MX block whose 32 columns have maximum amax. Scaling by a power of two is exact.
-__device__ __forceinline__ uint32_t mx_piece(const float (&v)[16], float amax, uint2* codes) {
+__device__ __forceinline__ uint32_t mx_piece(const float2 (&v)[8], float amax, uint2* codes) {
   if (not_finite(amax)) {
     *codes = make_uint2(0, 0);
     return 255u;
@@ -216,22 +212,12 @@ struct QuantArgs {
   float* row_scale;
 };
 
-__device__ __forceinline__ void affine16(float (&v)[16], float mean, float rstd, const QuantArgs& a, int col) {
-  if (col + 16 <= a.cols && (reinterpret_cast<uintptr_t>(a.gamma) & 15) == 0 &&
-      (reinterpret_cast<uintptr_t>(a.beta) & 15) == 0) {
+__device__ __forceinline__ void affine16(float2 (&v)[8], float mean, float rstd, const QuantArgs& a, int col) {
 #pragma unroll
-    for (int e = 0; e < 16; e += 4) {
-      const float4 g = __ldg(reinterpret_cast<const float4*>(a.gamma + col + e));
-      const float4 b = __ldg(reinterpret_cast<const float4*>(a.beta + col + e));
-      v[e] = (v[e] - mean) * rstd * g.x + b.x;
-      v[e + 1] = (v[e + 1] - mean) * rstd * g.y + b.y;
-      v[e + 2] = (v[e + 2] - mean) * rstd * g.z + b.z;
-      v[e + 3] = (v[e + 3] - mean) * rstd * g.w + b.w;
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 16; ++e)
-      v[e] = col + e < a.cols ? (v[e] - mean) * rstd * __ldg(a.gamma + col + e) + __ldg(a.beta + col + e) : 0.f;
+  for (int e = 0; e < 8; ++e) {
+    const int c = col + 2 * e;
+    v[e].x = c < a.cols ? fmaf(v[e].x - mean, rstd * __ldg(a.gamma + c), __ldg(a.beta + c)) : 0.f;
+    v[e].y = c + 1 < a.cols ? fmaf(v[e].y - mean, rstd * __ldg(a.gamma + c + 1), __ldg(a.beta + c + 1)) : 0.f;
   }
 }
 
@@ -283,7 +269,7 @@ template <int NW>
 __host__ __device__ constexpr int row_ctas() {  // CTAs of 256 threads per SM that the registers are held to
   return NW <= 3 ? 4 : NW <= 6 ? 3 : 2;
 }
-template <class T, bool MX, bool ALIGNED, int NW>
+template <class T, bool MX, bool ALIGNED, bool WHOLE, int NW>
 __global__ void __launch_bounds__(kQuantThreads, row_ctas<NW>()) quantize_fp4_rows_kernel(const QuantArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   constexpr int WARPS = kQuantThreads / 32;
@@ -299,7 +285,7 @@ __global__ void __launch_bounds__(kQuantThreads, row_ctas<NW>()) quantize_fp4_ro
     float amax[NW];
 #pragma unroll
     for (int i = 0; i < NW; ++i) {
-      realign<T, ALIGNED>(xr, (i * 32 + lane) * 16, a.cols, raw[i]);
+      realign<T, ALIGNED, WHOLE>(xr, (i * 32 + lane) * 16, a.cols, raw[i]);
       amax[i] = amax_pairs<T>(raw[i].t);
     }
     float s = 1.f;
@@ -316,7 +302,7 @@ __global__ void __launch_bounds__(kQuantThreads, row_ctas<NW>()) quantize_fp4_ro
     }
 #pragma unroll
     for (int i = 0; i < NW; ++i) {
-      float v[16];
+      float2 v[8];
       to_f32<T, ALIGNED>(raw[i], v);
       uint2 codes;
       uint32_t byte;
@@ -329,11 +315,9 @@ __global__ void __launch_bounds__(kQuantThreads, row_ctas<NW>()) quantize_fp4_ro
   }
 }
 
-// wpr warps per row, NC pieces of 16 columns per lane: rows of up to 512 * wpr * NC columns. Two pieces per lane and
-// few registers beat three pieces.
-constexpr int NC = 2;
-template <class T, bool MX, bool NORM, bool ALIGNED>
-__global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 2 ? 4 : 2) quantize_fp4_kernel(const QuantArgs a, const int wpr) {
+// wpr warps per row, NC pieces of 16 columns per lane: rows of up to 512 * wpr * NC columns.
+template <class T, bool MX, bool NORM, bool ALIGNED, bool WHOLE, int NC>
+__global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : NC == 2 ? 4 : 3) quantize_fp4_kernel(const QuantArgs a, const int wpr) {
   extern __shared__ float4 norm_s[];  // gamma, then beta
   __shared__ float red[2][3][kQuantThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -357,6 +341,7 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 2 ? 4 : 2) quantiz
     fill_norm(norm_s, a, pieces);
     __syncthreads();
   }
+  const float inv_n = 1.f / static_cast<float>(a.cols);
   const int step = static_cast<int>(gridDim.x) * rpc;
   int row = static_cast<int>(blockIdx.x) * rpc + grp;
   for (; row < a.rows; row += step, parity ^= 1) {
@@ -365,10 +350,11 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 2 ? 4 : 2) quantiz
     Raw<T, ALIGNED> raw[NC];
 #pragma unroll
     for (int i = 0; i < NC; ++i) load_raw<T, ALIGNED>(xr, ((i * wpr + wr) * 32 + lane) * 16, a.cols, raw[i]);
-    float v[NC][16], amax[NC];
+    float2 v[NC][8];
+    float amax[NC];
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      realign<T, ALIGNED>(xr, ((i * wpr + wr) * 32 + lane) * 16, a.cols, raw[i]);
+      realign<T, ALIGNED, WHOLE>(xr, ((i * wpr + wr) * 32 + lane) * 16, a.cols, raw[i]);
       to_f32<T, ALIGNED>(raw[i], v[i]);
     }
     if constexpr (NORM) {
@@ -376,31 +362,28 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 2 ? 4 : 2) quantiz
 #pragma unroll
       for (int i = 0; i < NC; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) s2 = add2(s2, make_float2(v[i][e], v[i][e + 1]));
-      const float n = static_cast<float>(a.cols);
-      const float mean = row_all(warp_sum(s2.x + s2.y), 0, plus) / n;
+        for (int e = 0; e < 8; ++e) s2 = add2(s2, v[i][e]);
+      const float mean = row_all(warp_sum(s2.x + s2.y), 0, plus) * inv_n;
       float2 q2 = make_float2(0.f, 0.f);
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
-        const int col = ((i * wpr + wr) * 32 + lane) * 16;
+        // columns past the row's end stay out of the variance
+        const int left = a.cols - ((i * wpr + wr) * 32 + lane) * 16;
+        const float m = left > 0 ? -mean : 0.f;
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          const float2 d = add2(make_float2(v[i][e], v[i][e + 1]), make_float2(-mean, -mean));
-          v[i][e] = d.x;
-          v[i][e + 1] = d.y;
-        }
-        if (col + 16 > a.cols) {  // columns past the row's end stay out of the variance
+        for (int e = 0; e < 8; ++e) v[i][e] = add2(v[i][e], make_float2(m, m));
+        if (!WHOLE && left > 0 && left < 16) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (col + e >= a.cols) v[i][e] = 0.f;
+          for (int e = 0; e < 8; ++e) {
+            if (2 * e >= left) v[i][e].x = 0.f;
+            if (2 * e + 1 >= left) v[i][e].y = 0.f;
+          }
         }
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          const float2 d = make_float2(v[i][e], v[i][e + 1]);
-          q2 = fma2(d, d, q2);
-        }
+        for (int e = 0; e < 8; ++e) q2 = fma2(v[i][e], v[i][e], q2);
       }
-      const float rstd = rsqrtf(row_all(warp_sum(q2.x + q2.y), 1, plus) / n + a.eps);
+      const float rstd = rsqrtf(row_all(warp_sum(q2.x + q2.y), 1, plus) * inv_n + a.eps);
+      const float2 r2 = make_float2(rstd, rstd);
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
         const int c = (i * wpr + wr) * 32 + lane;
@@ -408,13 +391,8 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 2 ? 4 : 2) quantiz
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float4 g = norm_s[norm_slot(c, j)], b = norm_s[4 * pieces + norm_slot(c, j)];
-            const float2 r2 = make_float2(rstd, rstd);
-            const float2 lo = fma2(make_float2(v[i][4 * j], v[i][4 * j + 1]), mul2(r2, make_float2(g.x, g.y)), make_float2(b.x, b.y));
-            const float2 hi = fma2(make_float2(v[i][4 * j + 2], v[i][4 * j + 3]), mul2(r2, make_float2(g.z, g.w)), make_float2(b.z, b.w));
-            v[i][4 * j] = lo.x;
-            v[i][4 * j + 1] = lo.y;
-            v[i][4 * j + 2] = hi.x;
-            v[i][4 * j + 3] = hi.y;
+            v[i][2 * j] = fma2(v[i][2 * j], mul2(r2, make_float2(g.x, g.y)), make_float2(b.x, b.y));
+            v[i][2 * j + 1] = fma2(v[i][2 * j + 1], mul2(r2, make_float2(g.z, g.w)), make_float2(b.z, b.w));
           }
         }
       }
@@ -471,22 +449,23 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_fp4_wide_kernel(const 
   pdl_wait();
   pdl_trigger();
   const int pieces = (a.cols + kFp4Step - 1) / kFp4Step * (kFp4Step / 16);
-  float mean = 0.f, rstd = 1.f, v[16];
+  float mean = 0.f, rstd = 1.f;
+  float2 v[8];
   if constexpr (NORM) {
     float s = 0.f;
     for (int c = threadIdx.x; c * 16 < a.cols; c += kQuantThreads) {
       load16<T>(xr, c * 16, a.cols, v);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s += v[e];
+      for (int e = 0; e < 8; ++e) s += v[e].x + v[e].y;
     }
     mean = cta_all(s, plus) / static_cast<float>(a.cols);
     float q = 0.f;
     for (int c = threadIdx.x; c * 16 < a.cols; c += kQuantThreads) {
       load16<T>(xr, c * 16, a.cols, v);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float d = c * 16 + e < a.cols ? v[e] - mean : 0.f;
-        q += d * d;
+      for (int e = 0; e < 8; ++e) {
+        const float d0 = c * 16 + 2 * e < a.cols ? v[e].x - mean : 0.f, d1 = c * 16 + 2 * e + 1 < a.cols ? v[e].y - mean : 0.f;
+        q = fmaf(d0, d0, fmaf(d1, d1, q));
       }
     }
     rstd = rsqrtf(cta_all(q, plus) / static_cast<float>(a.cols) + a.eps);
@@ -522,30 +501,22 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_fp4_wide_kernel(const 
   }
 }
 
-template <class T, bool MX, bool ALIGNED, int NW>
+template <class T, bool MX, bool ALIGNED, bool WHOLE, int NW>
 int launch_rows(const QuantArgs& a, cudaStream_t stream) {
   const int want = (a.rows + kQuantThreads / 32 - 1) / (kQuantThreads / 32), full = row_ctas<NW>() * sm_count();
-  launch(quantize_fp4_rows_kernel<T, MX, ALIGNED, NW>, dim3(want < full ? want : full), dim3(kQuantThreads), 0, stream, a);
+  launch(quantize_fp4_rows_kernel<T, MX, ALIGNED, WHOLE, NW>, dim3(want < full ? want : full), dim3(kQuantThreads), 0, stream, a);
   return check_launch("quantize_fp4_rows_kernel");
 }
 
-template <class T, bool MX, bool NORM, bool ALIGNED>
-int dispatch_quant(const QuantArgs& a, cudaStream_t stream) {
-  const int cols = (a.cols + kFp4Step - 1) / kFp4Step * kFp4Step;  // the padded scales are written too
-  if constexpr (sizeof(T) == 2 && !NORM) {
-    if (cols <= 1024) return launch_rows<T, MX, ALIGNED, 2>(a, stream);
-    if (cols <= 1536) return launch_rows<T, MX, ALIGNED, 3>(a, stream);
-    if (cols <= 3 * 1024) return launch_rows<T, MX, ALIGNED, 6>(a, stream);
-    if (cols <= 5 * 1024) return launch_rows<T, MX, ALIGNED, 10>(a, stream);
-  }
-  const int wpr = (cols + 512 * NC - 1) / (512 * NC);
+template <class T, bool MX, bool NORM, bool ALIGNED, bool WHOLE, int NC>
+int launch_joined(const QuantArgs& a, int cols, int wpr, cudaStream_t stream) {
   constexpr int WARPS = kQuantThreads / 32;
   if (wpr > WARPS) {
     launch(quantize_fp4_wide_kernel<T, MX, NORM>, dim3(a.rows), dim3(kQuantThreads), 0, stream, a);
     return check_launch("quantize_fp4_wide_kernel");
   }
   const int rpc = WARPS / wpr, threads = 32 * wpr * rpc;
-  auto kernel = quantize_fp4_kernel<T, MX, NORM, ALIGNED>;
+  auto kernel = quantize_fp4_kernel<T, MX, NORM, ALIGNED, WHOLE, NC>;
   const size_t smem = NORM ? static_cast<size_t>(cols) * 8 : 0;
   static int per_sm[64][WARPS] = {};  // resident CTAs per device and wpr, 0 = not configured yet
   int dev = 0;
@@ -564,10 +535,28 @@ int dispatch_quant(const QuantArgs& a, cudaStream_t stream) {
   return check_launch("quantize_fp4_kernel");
 }
 
+template <class T, bool MX, bool NORM, bool ALIGNED, bool WHOLE>
+int dispatch_quant(const QuantArgs& a, cudaStream_t stream) {
+  const int cols = (a.cols + kFp4Step - 1) / kFp4Step * kFp4Step;  // the padded scales are written too
+  if constexpr (sizeof(T) == 2 && !NORM) {
+    if (cols <= 1024) return launch_rows<T, MX, ALIGNED, WHOLE, 2>(a, stream);
+    if (cols <= 1536) return launch_rows<T, MX, ALIGNED, WHOLE, 3>(a, stream);
+    if (cols <= 3 * 1024) return launch_rows<T, MX, ALIGNED, WHOLE, 6>(a, stream);
+    if (cols <= 5 * 1024) return launch_rows<T, MX, ALIGNED, WHOLE, 10>(a, stream);
+  }
+  const int wpr2 = (cols + 1023) / 1024, wpr3 = (cols + 1535) / 1536;
+  // two or three pieces per lane, whichever leaves fewer lanes idle; three where that is even (fewer warps to join)
+  if (3 * wpr3 <= 2 * wpr2) return launch_joined<T, MX, NORM, ALIGNED, WHOLE, 3>(a, cols, wpr3, stream);
+  return launch_joined<T, MX, NORM, ALIGNED, WHOLE, 2>(a, cols, wpr2, stream);
+}
+
 template <class T, bool MX, bool NORM>
 int dispatch_quant_align(const QuantArgs& a, cudaStream_t stream) {
   const bool aligned = aligned16(a.x) && a.ldx * static_cast<int64_t>(sizeof(T)) % 16 == 0;
-  return aligned ? dispatch_quant<T, MX, NORM, true>(a, stream) : dispatch_quant<T, MX, NORM, false>(a, stream);
+  // aligned rows of whole 16-column pieces (the usual widths) do without shifts and masks
+  return aligned && a.cols % 16 == 0 ? dispatch_quant<T, MX, NORM, true, true>(a, stream)
+         : aligned                   ? dispatch_quant<T, MX, NORM, true, false>(a, stream)
+                                     : dispatch_quant<T, MX, NORM, false, false>(a, stream);
 }
 
 template <class T>
@@ -635,32 +624,43 @@ __global__ void __launch_bounds__(256)
         *reinterpret_cast<uint4*>(orow + c0) = pack(v);
       }
     }
-#pragma unroll 2
-    for (; c0 < cols; c0 += 32 * E) {
-      if (c0 + E <= 0) continue;
-      // codes of columns [c0, c0 + E): one aligned word, or two when the row is not aligned
-      const int w0 = c0 >> 3, sh = 4 * (c0 & 7);
-      uint32_t q = w0 >= 0 ? __ldg(crow + w0) : 0u;
-      if (sh + 4 * E > 32) q = __funnelshift_r(q, w0 + 1 < words ? __ldg(crow + w0 + 1) : 0u, sh);
-      else q >>= sh;
-      uint32_t h[4];
-      e2m1x8_to_half2(q, h);
-      // the (at most two) blocks that the granule touches
-      const int first = c0 < 0 ? 0 : c0, last = c0 + E - 1 < cols ? c0 + E - 1 : cols - 1;
-      const float s0 = scale_at(first / B), s1 = last / B != first / B ? scale_at(last / B) : s0;
-      const int cut = (first / B + 1) * B;  // the second block's first column
-      float v[8];
+    // Any other row, and an aligned row's last granule: all loads of four granules first.
+    constexpr int U = 4;
+    for (; c0 < cols; c0 += U * 32 * E) {
+      uint32_t lo[U], hi[U];
+      float sc[U][2];
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float2 f = unpack_half2(h[e / 2]);
-        v[e] = ((e & 1) ? f.y : f.x) * (c0 + e >= cut ? s1 : s0);
+      for (int u = 0; u < U; ++u) {
+        const int c = c0 + u * 32 * E;
+        const int w0 = c >> 3;  // codes of columns [c, c + E): one aligned word, or two when the row is not aligned
+        lo[u] = w0 >= 0 && w0 < words ? __ldg(crow + w0) : 0u;
+        hi[u] = w0 + 1 < words ? __ldg(crow + w0 + 1) : 0u;
+        // the (at most two) blocks that the granule touches
+        const int first = min(max(c, 0), cols - 1) / B, last = min(max(c + E - 1, 0), cols - 1) / B;
+        sc[u][0] = scale_at(first);
+        sc[u][1] = scale_at(last);
       }
-      if (c0 >= 0 && c0 + E <= cols) {
-        *reinterpret_cast<uint4*>(orow + c0) = pack(v);
-      } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (c0 + e >= 0 && c0 + e < cols) store_one(orow + c0 + e, v[e]);
+      for (int u = 0; u < U; ++u) {
+        const int c = c0 + u * 32 * E;
+        if (c >= cols || c + E <= 0) continue;
+        uint32_t h[4];
+        e2m1x8_to_half2(__funnelshift_r(lo[u], hi[u], 4 * (c & 7)), h);
+        const int cut = (max(c, 0) / B + 1) * B - c;  // values before the second block
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          const float2 f = mul2(unpack_half2(h[e / 2]), make_float2(e >= cut ? sc[u][1] : sc[u][0], e + 1 >= cut ? sc[u][1] : sc[u][0]));
+          v[e] = f.x;
+          v[e + 1] = f.y;
+        }
+        if (c >= 0 && c + E <= cols) {
+          *reinterpret_cast<uint4*>(orow + c) = pack(v);
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (c + e >= 0 && c + e < cols) store_one(orow + c + e, v[e]);
+        }
       }
     }
   }
