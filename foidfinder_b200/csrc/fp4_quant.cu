@@ -6,8 +6,8 @@
 //   FF_FP4_MX: scale = 2^(floor(log2 amax(block of 32)) - 2),  code = e2m1(v / scale)
 //
 // The power-of-two row scale costs no accuracy that the e4m3 block scale would have kept, and makes v / s and
-// S * s exact, so the codes are the correctly rounded quotients: amax / 6 is an IEEE division, and v / S is a
-// product with the rounded reciprocal whose last bits are snapped off for 16-bit inputs (see quotient()).
+// S * s exact, so the codes are the correctly rounded quotients: amax / 6 is rounded correctly (sixth()), and v / S
+// is a product with the reciprocal whose last bits are snapped off for 16-bit inputs (quotient2()).
 // A row (NV) or block (MX) that holds an infinity or NaN gets a NaN scale, so that it shows in every result.
 //
 // Bound by HBM: 2 bytes read and 0.56 (NV) or 0.53 (MX) written per value. The whole row stays in registers,
@@ -167,22 +167,22 @@ __device__ __forceinline__ uint2 codes16(const float2 (&v)[8], float r, float sc
   return make_uint2(e2m1x8(q), e2m1x8(q + 4));
 }
 
-// One 16-column piece of an NV row with row scale s: its scale byte and codes. amax / (6 s) for the block scale: an
-// IEEE division for kExact32. For 16-bit inputs a true tie of e4m3 has at most 5 significant bits and any other
-// quotient is at least 2^-12 of itself away from one, so rounding the product with 1 / 6 to 16 significant bits
-// decides as the division would.
+// amax / 6, rounded correctly: the remainder of the product with 1 / 6 corrects it, so that ties of e4m3 come out
+// exact and no other value moves onto one.
+__device__ __forceinline__ float sixth(float a) {
+  const float q = a * (1.f / 6.f);
+  return fmaf(fmaf(-6.f, q, a), 1.f / 6.f, q);
+}
+// One 16-column piece of an NV row with row scale s: its scale byte and codes.
 template <int KIND>
 __device__ __forceinline__ uint32_t nv_piece(const float2 (&v)[8], float amax, float s, bool bad, uint2* codes) {
   const float is = inv_pow2(s);
-  float t = amax * is;
-  if constexpr (KIND == kExact32)
-    t = __fdiv_rn(t, 6.f);
-  else
-    t = __uint_as_float((__float_as_uint(t * (1.f / 6.f)) + 0x40u) & ~0x7fu);
+  const float t = sixth(amax * is);
   const uint32_t byte = bad ? 0u : e4m3_byte(t);
   const float S = e4m3_value(byte);
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(S));
+  r = fmaf(r, fmaf(-S, r, 1.f), r);  // to the last bit
   *codes = bad ? make_uint2(0, 0) : codes16<KIND>(v, byte ? r * is : 0.f, S * s);
   return byte;
 }

@@ -22,7 +22,7 @@ namespace ff {
 
 namespace {
 
-template <bool PAIR>
+template <bool PAIR, bool QKV>
 struct Fp4Cfg {
   static constexpr int BN = PAIR ? 256 : 128;
   static constexpr int TILE_M = PAIR ? 256 : 128;
@@ -31,15 +31,17 @@ struct Fp4Cfg {
   static constexpr int SFA_BYTES = 4 * kSfChunk;
   static constexpr int SFB_BYTES = (BN / 128) * 4 * kSfChunk;
   static constexpr int STAGE_BYTES = 2 * CODE_BYTES + SFA_BYTES + SFB_BYTES;
-  static constexpr int STAGES = 4;
+  // EPI_QKV_NORM_ROPE: three stages leave the L1 cache room for a row block's rotation angles (32 KB)
+  static constexpr int STAGES = QKV ? 3 : 4;
   static constexpr int GROUP_WARPS = 8;  // epilogue warps of one accumulator
   static constexpr int THREADS = 128 + 2 * 32 * GROUP_WARPS;
   static constexpr int STAGING = 4096;      // per epilogue warp: 32 rows x 128 B
-  static constexpr int COLP = 2 * 64 * 4;   // per epilogue warp: scales and biases of 64 columns
+  static constexpr int COLP = 2 * BN * 4;   // column scales and biases of a tile
+  static constexpr int COLP_BUFS = 4;       // tiles that they are read ahead
   static constexpr int NORM_BYTES = 4 * 64 * 4;  // q and k norm weights and biases
   static constexpr int BAR_BYTES = 512;
   static constexpr int SMEM =
-      1024 + STAGES * STAGE_BYTES + 2 * GROUP_WARPS * (STAGING + COLP) + NORM_BYTES + BAR_BYTES;
+      1024 + STAGES * STAGE_BYTES + 2 * GROUP_WARPS * STAGING + COLP_BUFS * COLP + (QKV ? NORM_BYTES : 0) + BAR_BYTES;
   // TMEM: two accumulators and two buffers of scales, each for one chunk of A's and W's columns. Two 256-column
   // accumulators and the scales do not fit 512 columns: the pair's accumulators share 32 columns, the last of
   // the first and the first of the second, which the epilogue empties first.
@@ -69,19 +71,24 @@ __device__ __forceinline__ float2 gelu2(float2 x) {
   return mul2(x, sigmoid2(mul2(x, fma2(mul2(x, x), make_float2(c3, c3), make_float2(c1, c1)))));
 }
 
-// r[j] = r[j] * (rs * cs[j]) + bias[j] for N accumulators in place (as f32 bits); cs and bias in shared memory, read
-// by every lane at once.
-template <int N>
+// r[j] = r[j] * (rs * cs[j]) + bias[j] for N accumulators in place (as f32 bits); FF_FP4_MX has no row and column
+// scales. cs and bias in shared memory, read by every lane at once.
+template <int N, bool MX>
 __device__ __forceinline__ void scale_cols(uint32_t* r, float rs, const float* cs, const float* bias) {
   const float2 rs2 = make_float2(rs, rs);
 #pragma unroll
   for (int j = 0; j < N; j += 4) {
-    const float4 c = *reinterpret_cast<const float4*>(cs + j);
     const float4 b = *reinterpret_cast<const float4*>(bias + j);
-    const float2 lo = fma2(make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])),
-                           mul2(rs2, make_float2(c.x, c.y)), make_float2(b.x, b.y));
-    const float2 hi = fma2(make_float2(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3])),
-                           mul2(rs2, make_float2(c.z, c.w)), make_float2(b.z, b.w));
+    float2 lo = make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1]));
+    float2 hi = make_float2(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]));
+    if constexpr (MX) {
+      lo = add2(lo, make_float2(b.x, b.y));
+      hi = add2(hi, make_float2(b.z, b.w));
+    } else {
+      const float4 c = *reinterpret_cast<const float4*>(cs + j);
+      lo = fma2(lo, mul2(rs2, make_float2(c.x, c.y)), make_float2(b.x, b.y));
+      hi = fma2(hi, mul2(rs2, make_float2(c.z, c.w)), make_float2(b.z, b.w));
+    }
     r[j] = __float_as_uint(lo.x);
     r[j + 1] = __float_as_uint(lo.y);
     r[j + 2] = __float_as_uint(hi.x);
@@ -116,27 +123,30 @@ __device__ __forceinline__ void fp4_stage_mmas(uint32_t d, uint32_t tmem, uint32
   }
 }
 
-template <bool PAIR, int EPI, class OutT>
-__global__ void __launch_bounds__(Fp4Cfg<PAIR>::THREADS, 1)
+template <bool PAIR, bool MX, int EPI, class OutT>
+__global__ void __launch_bounds__(Fp4Cfg<PAIR, EPI == EPI_QKV_NORM_ROPE>::THREADS, 1)
     gemm_fp4_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
                     const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSW,
                     const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmR,
                     const Fp4GemmArgs args) {
   constexpr bool RES = EPI == EPI_RESIDUAL;
   constexpr bool F32OUT = sizeof(OutT) == 4;
-  using C = Fp4Cfg<PAIR>;
+  constexpr bool QKV = EPI == EPI_QKV_NORM_ROPE;
+  using C = Fp4Cfg<PAIR, QKV>;
   constexpr int STAGES = C::STAGES, BN = C::BN, HALF = C::HALF;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* staging = smem + STAGES * C::STAGE_BYTES;
   float* colp = reinterpret_cast<float*>(staging + 2 * C::GROUP_WARPS * C::STAGING);
-  float* normp = colp + 2 * C::GROUP_WARPS * (C::COLP / 4);  // q weight, q bias, k weight, k bias
-  uint64_t* full = reinterpret_cast<uint64_t*>(normp + 4 * 64);
+  float* normp = colp + C::COLP_BUFS * (C::COLP / 4);  // EPI_QKV_NORM_ROPE: q weight, q bias, k weight, k bias
+  uint64_t* full = reinterpret_cast<uint64_t*>(normp + (QKV ? C::NORM_BYTES / 4 : 0));
   uint64_t* empty = full + STAGES;
   uint64_t* tfull = empty + STAGES;
   uint64_t* tempty = tfull + 2;  // an accumulator has been read
   uint64_t* tearly = tempty + 2;  // PAIR: the columns that it shares with the other one have been read
-  uint64_t* drain = tearly + 2;
+  uint64_t* pfull = tearly + 2;  // a tile's column scales and biases are in shared memory
+  uint64_t* pempty = pfull + C::COLP_BUFS;
+  uint64_t* drain = pempty + C::COLP_BUFS;
   uint64_t* resbar = drain + 1;  // one per epilogue warp (EPI_RESIDUAL)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(resbar + 2 * C::GROUP_WARPS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -148,6 +158,12 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR>::THREADS, 1)
   const bool leader = rank == 0;
   const int unit = PAIR ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
   const int units = PAIR ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
+  // Tile i of this CTA (pair): strided over the units, so that the tiles in work at one time share A and W in L2;
+  // for EPI_QKV_NORM_ROPE runs along N, whose tiles share the rows' angles.
+  const int t_first = QKV ? static_cast<int>(static_cast<int64_t>(unit) * tiles / units) : unit;
+  const int t_step = QKV ? 1 : units;
+  const int my_tiles = QKV ? static_cast<int>(static_cast<int64_t>(unit + 1) * tiles / units) - t_first
+                           : (tiles - unit + units - 1) / units;
   auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
     if constexpr (PAIR)
       return mbar_wait_cluster<true>(bar, parity, abort_flag, args.err, code);
@@ -164,6 +180,10 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR>::THREADS, 1)
       mbar_init(&tfull[a], 1);
       mbar_init(&tempty[a], (PAIR ? 2 : 1) * C::GROUP_WARPS);
       mbar_init(&tearly[a], 2 * C::GROUP_WARPS / 2);
+    }
+    for (int p = 0; p < C::COLP_BUFS; ++p) {
+      mbar_init(&pfull[p], 1);
+      mbar_init(&pempty[p], C::GROUP_WARPS);
     }
     mbar_init(drain, 1);
     for (int i = 0; i < 2 * C::GROUP_WARPS; ++i) mbar_init(&resbar[i], 1);
@@ -199,8 +219,8 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR>::THREADS, 1)
       int last_phase[STAGES];
 #pragma unroll
       for (int s = 0; s < STAGES; ++s) last_phase[s] = -1;
-      const int ch = args.mx ? 2 : 4;  // scale chunks per stage and 128-row tile
-      const uint32_t stage_bytes = 2 * C::CODE_BYTES + (1 + BN / 128) * ch * kSfChunk;
+      constexpr int ch = sf_chunks_per_step(MX);  // scale chunks per stage and 128-row tile
+      constexpr uint32_t stage_bytes = 2 * C::CODE_BYTES + (1 + BN / 128) * ch * kSfChunk;
       const int row_chunks = args.num_kb * ch;  // scale chunks of one 128-row tile
       auto load_w = [&](uint8_t* sa, uint64_t* bar, int kb, int tn) {
         uint8_t* ssb = sa + 2 * C::CODE_BYTES + C::SFA_BYTES;
@@ -234,11 +254,12 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR>::THREADS, 1)
       const int pre = args.w_const ? (args.num_kb < STAGES ? args.num_kb : STAGES) : 0;
       for (int kb = 0; kb < pre; ++kb) {
         expect(&full[kb]);
-        load_w(smem + kb * C::STAGE_BYTES, &full[kb], kb, unit % tiles_n);
+        load_w(smem + kb * C::STAGE_BYTES, &full[kb], kb, t_first % tiles_n);
       }
       pdl_wait();
       bool ok = true, first = true;
-      for (int t = unit; t < tiles && ok; t += units) {
+      for (int i = 0; i < my_tiles && ok; ++i) {
+        const int t = t_first + i * t_step;
         const int tm = t / tiles_n, tn = t % tiles_n;
         for (int kb = 0; kb < args.num_kb; ++kb) {
           uint8_t* sa = smem + stage * C::STAGE_BYTES;
@@ -286,7 +307,7 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR>::THREADS, 1)
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int i = 0; unit + i * units < tiles && ok; ++i) {
+      for (int i = 0; i < my_tiles && ok; ++i) {
         const uint32_t acc = i & 1, use = (i >> 1) & 1;
         if (!wait(&tempty[acc], use ^ 1u, kDevTimeoutTmemEmpty)) break;
         if (PAIR && i > 0 && !wait(&tearly[acc ^ 1u], ((i - 1) >> 1) & 1, kDevTimeoutTmemEmpty)) break;
@@ -300,10 +321,7 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR>::THREADS, 1)
           tc_fence_after();
           const uint32_t sa = smem_u32(smem + stage * C::STAGE_BYTES);
           const int left = (args.K - kb * kFp4Step + 63) >> 6;  // 64-column steps to the end of the row
-          if (args.mx)
-            fp4_stage_mmas<PAIR, true, C>(d, tmem, sa, left, kb == 0);
-          else
-            fp4_stage_mmas<PAIR, false, C>(d, tmem, sa, left, kb == 0);
+          fp4_stage_mmas<PAIR, MX, C>(d, tmem, sa, left, kb == 0);
           commit_both(&empty[stage]);
           if (++stage == STAGES) {
             stage = 0;
@@ -327,6 +345,29 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR>::THREADS, 1)
         }
       }
     }
+  } else if (warp == 2) {
+    // ------------------------------------------------------------ column scales and biases, up to four tiles ahead
+    pdl_wait();
+    for (int i = 0; i < my_tiles; ++i) {
+      const int buf = i % C::COLP_BUFS;
+      if (!wait(&pempty[buf], ((i / C::COLP_BUFS) & 1) ^ 1u, kDevTimeoutTmemEmpty)) break;
+      float* const cs = colp + buf * (C::COLP / 4);
+      const int n0 = (t_first + i * t_step) % tiles_n * BN;
+      float c[BN / 32], b[BN / 32];  // all loads before the first store: one latency per tile
+#pragma unroll
+      for (int j = 0; j < BN / 32; ++j) {
+        const int n = n0 + 32 * j + lane;
+        c[j] = !MX && n < args.N ? __ldg(args.col_scale + n) : 0.f;  // zero past N
+        b[j] = args.bias != nullptr && n < args.N ? __ldg(args.bias + n) : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < BN / 32; ++j) {
+        if constexpr (!MX) cs[32 * j + lane] = c[j];
+        cs[BN + 32 * j + lane] = b[j];
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&pfull[buf]);
+    }
   } else if (warp >= 4) {
     // ------------------------------------------------------------ epilogue
     // Two groups of eight warps, one per accumulator, take turns with the tiles: a group has the time of two
@@ -337,8 +378,6 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR>::THREADS, 1)
     const int q = warp & 3;          // TMEM lane quarter
     const int half = (ew >> 2) & 1;  // of the tile's columns
     uint8_t* const stg = staging + ew * C::STAGING;
-    float* const cs_s = colp + ew * (C::COLP / 4);
-    float* const b_s = cs_s + 64;
     if constexpr (EPI == EPI_QKV_NORM_ROPE) {
       for (int i = threadIdx.x - 128; i < 64; i += 2 * 32 * C::GROUP_WARPS) {
         normp[i] = args.q_w[i];
@@ -352,33 +391,34 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR>::THREADS, 1)
     constexpr int STEPS = HALF / 64;           // 64 tile columns per step
     constexpr int WIDTH = SWIGLU ? 32 : 64;    // output columns per step
     uint32_t use = 0, res_phase = 0;
-    for (int t = unit + acc * units; t < tiles; t += 2 * units, use ^= 1u) {
+    // The lane's row scale, read a tile ahead: with the epilogue at work all the time its latency would be exposed.
+    auto row_scale_of = [&](int i) {
+      if (MX || i >= my_tiles) return 1.f;
+      const int row = (t_first + i * t_step) / tiles_n * C::TILE_M + static_cast<int>(rank) * 128 + q * 32 + lane;
+      return row < args.M ? __ldg(args.row_scale + row) : 0.f;
+    };
+    float rs_next = row_scale_of(acc);
+    for (int i = acc; i < my_tiles; i += 2, use ^= 1u) {
+      const int t = t_first + i * t_step;
       const int tm = t / tiles_n, tn = t - tm * tiles_n;
+      const int buf = i % C::COLP_BUFS;
+      const float* const cs_t = colp + buf * (C::COLP / 4);  // the tile's column scales, then its biases
       const int m_block = tm * C::TILE_M + static_cast<int>(rank) * 128 + q * 32;
       const int m = m_block + lane;
       const bool row_ok = m < args.M;
       const int n_tile = tn * BN;
-      const float rs = row_ok ? (args.row_scale != nullptr ? __ldg(args.row_scale + m) : 1.f) : 0.f;
+      const float rs = rs_next;
       const uint32_t tbase = tmem + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc) * C::ACC_STRIDE;
       bool ok = true;
 #pragma unroll 1
       for (int step = 0; step < STEPS; ++step) {
         // The first group goes from the last columns down, the second from the first columns up, so that each
-        // begins with the columns that the accumulators share. ca, cb: the step's first and second 32 tile
-        // columns, neighbours or 32 gates and their 32 ups.
-        const int at = acc == 0 ? STEPS - 1 - step : step;
-        const int ca = SWIGLU ? (PAIR ? half * 128 + at * 32 : half * 32) : half * HALF + at * 64;
-        const int cb = ca + (SWIGLU ? 64 : 32);
-        const int out0 = SWIGLU ? (n_tile >> 1) + (PAIR ? half * 64 + at * 32 : half * 32) : n_tile + ca;
+        // begins with the columns that the accumulators share. ca: the step's first tile column.
+        const int ca = half * HALF + (acc == 0 ? STEPS - 1 - step : step) * 64;
+        const int out0 = SWIGLU ? (n_tile + ca) >> 1 : n_tile + ca;
         const bool any = m_block < args.M && out0 < args.out_cols;  // the warp has something to write
+        const float *csa = cs_t + ca, *ba = csa + BN;
         __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int n = n_tile + (i ? cb : ca) + lane;
-          const bool in = n < args.N;
-          cs_s[32 * i + lane] = in ? (args.col_scale != nullptr ? __ldg(args.col_scale + n) : 1.f) : 0.f;
-          b_s[32 * i + lane] = in && args.bias != nullptr ? __ldg(args.bias + n) : 0.f;
-        }
         if (lane == 0) {
           if constexpr (!F32OUT) bulk_wait_read_all();  // the staging buffer is free
           if constexpr (RES) {
@@ -390,7 +430,7 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR>::THREADS, 1)
         }
         __syncwarp();
         if (step == 0) {
-          ok = wait(&tfull[acc], use, kDevTimeoutTmemFull);
+          ok = wait(&pfull[buf], (i / C::COLP_BUFS) & 1, kDevTimeoutTmemFull) && wait(&tfull[acc], use, kDevTimeoutTmemFull);
           if (!ok) {
             if constexpr (RES) {  // let the residual copy land before the CTA exits
               if (any) mbar_wait(&resbar[ew], res_phase, abort_flag, args.err, kDevTimeoutDrain);
@@ -414,7 +454,10 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR>::THREADS, 1)
           if (PAIR && step == 0 && half != acc) arrive(&tearly[acc]);
         };
         auto arrive_empty = [&]() {
-          if (step == STEPS - 1) arrive(&tempty[acc]);
+          if (step == STEPS - 1) {
+            arrive(&tempty[acc]);
+            rs_next = row_scale_of(i + 2);
+          }
         };
         auto read32 = [&](int col, uint32_t(&r)[32]) {
           __syncwarp();
@@ -455,113 +498,101 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR>::THREADS, 1)
             group_end();
           }
         };
-        if constexpr (SWIGLU) {
-          uint32_t rg[32], ru[32];
-          if (acc == 0)  // the shared ones first
-            read32(cb, ru);
-          else
-            read32(ca, rg);
-          arrive_early();
-          if (acc == 0)
-            read32(ca, rg);
-          else
-            read32(cb, ru);
-          arrive_empty();
+        // The head norm's statistics first, from reads of their own: the accumulator is read again below.
+        const int head = out0 >> 6;
+        float mean = 0.f, rstd = 1.f;
+        const bool qk = EPI == EPI_QKV_NORM_ROPE && any && head < args.q_heads + args.k_heads;
+        if constexpr (EPI == EPI_QKV_NORM_ROPE) {
+          auto over_head = [&](auto f) {
+#pragma unroll 1
+            for (int sub = 0; sub < 2; ++sub) {
+              uint32_t r[32];
+              read32(ca + 32 * sub, r);
+              scale_cols<32, MX>(r, rs, csa + 32 * sub, ba + 32 * sub);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) f(__uint_as_float(r[j]));
+            }
+          };
+          if (qk) {
+            if (args.norm == FF_NORM_LAYER) {
+              over_head([&](float v) { mean += v; });
+              mean *= 1.f / 64.f;
+            }
+            float ss = 0.f;
+            over_head([&](float v) { ss = fmaf(v - mean, v - mean, ss); });
+            rstd = rsqrtf(ss * (1.f / 64.f) + args.qk_eps);
+          }
+        }
+#pragma unroll 1
+        for (int k = 0; k < 2; ++k) {
+          const int sub = acc == 0 ? 1 - k : k;  // the shared columns first
+          uint32_t r[32];
+          read32(ca + 32 * sub, r);
+          if (k == 0) {
+            arrive_early();
+            wait_residual();
+          } else {
+            arrive_empty();
+          }
           if (!any) continue;
+          const float *cs = csa + 32 * sub, *bs = ba + 32 * sub;
+          if constexpr (F32OUT) {
+            float* const out = static_cast<float*>(args.out);
+            const int rows = args.M - m_block < 32 ? args.M - m_block : 32;
+            scale_cols<32, MX>(r, rs, cs, bs);
+            stage_row128(stg, lane, r);
+            __syncwarp();
+            const int n = out0 + 32 * sub + lane;
+            for (int k = 0; k < rows; ++k)  // one row of 32 columns per store: any row stride and column count
+              if (n < args.N)
+                out[static_cast<int64_t>(m_block + k) * args.ldo + n] =
+                    *reinterpret_cast<const float*>(stg + k * 128 + (((lane >> 2) ^ (k & 7)) << 4) + (lane & 3) * 4);
+            __syncwarp();
+          } else {
+            // Eight output columns at a time: scale, activate, round, stage.
+            if constexpr (SWIGLU) {  // 16 gates, then their 16 ups
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            scale_cols<8>(rg + 8 * g, rs, cs_s + 8 * g, b_s + 8 * g);
-            scale_cols<8>(ru + 8 * g, rs, cs_s + 32 + 8 * g, b_s + 32 + 8 * g);
-            float y[8];
+              for (int g = 0; g < 2; ++g) {
+                scale_cols<8, MX>(r + 8 * g, rs, cs + 8 * g, bs + 8 * g);
+                scale_cols<8, MX>(r + 16 + 8 * g, rs, cs + 16 + 8 * g, bs + 16 + 8 * g);
+                float y[8];
 #pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-              const int k = 8 * g + j;
-              const float2 h = silu_up2(make_float2(__uint_as_float(rg[k]), __uint_as_float(rg[k + 1])),
-                                        make_float2(__uint_as_float(ru[k]), __uint_as_float(ru[k + 1])));
-              y[j] = h.x;
-              y[j + 1] = h.y;
-            }
-            stage8(g, y);
-          }
-        } else {
-          // The head norm's statistics first, from reads of their own: the accumulator is read again below.
-          const int head = out0 >> 6;
-          float mean = 0.f, rstd = 1.f;
-          const bool qk = EPI == EPI_QKV_NORM_ROPE && any && head < args.q_heads + args.k_heads;
-          if constexpr (EPI == EPI_QKV_NORM_ROPE) {
-            auto over_head = [&](auto f) {
-#pragma unroll 1
-              for (int sub = 0; sub < 2; ++sub) {
-                uint32_t r[32];
-                read32(ca + 32 * sub, r);
-                scale_cols<32>(r, rs, cs_s + 32 * sub, b_s + 32 * sub);
-#pragma unroll
-                for (int j = 0; j < 32; ++j) f(__uint_as_float(r[j]));
-              }
-            };
-            if (qk) {
-              if (args.norm == FF_NORM_LAYER) {
-                over_head([&](float v) { mean += v; });
-                mean *= 1.f / 64.f;
-              }
-              float ss = 0.f;
-              over_head([&](float v) { ss = fmaf(v - mean, v - mean, ss); });
-              rstd = rsqrtf(ss * (1.f / 64.f) + args.qk_eps);
-            }
-          }
-#pragma unroll 1
-          for (int i = 0; i < 2; ++i) {
-            const int sub = acc == 0 ? 1 - i : i;  // the shared columns first
-            uint32_t r[32];
-            read32(ca + 32 * sub, r);
-            if (i == 0) {
-              arrive_early();
-              wait_residual();
-            } else {
-              arrive_empty();
-            }
-            if (!any) continue;
-            const float *cs = cs_s + 32 * sub, *bs = b_s + 32 * sub;
-            if constexpr (F32OUT) {
-              float* const out = static_cast<float*>(args.out);
-              const int rows = args.M - m_block < 32 ? args.M - m_block : 32;
-              scale_cols<32>(r, rs, cs, bs);
-              stage_row128(stg, lane, r);
-              __syncwarp();
-              const int n = out0 + 32 * sub + lane;
-              for (int k = 0; k < rows; ++k)  // one row of 32 columns per store: any row stride and column count
-                if (n < args.N)
-                  out[static_cast<int64_t>(m_block + k) * args.ldo + n] =
-                      *reinterpret_cast<const float*>(stg + k * 128 + (((lane >> 2) ^ (k & 7)) << 4) + (lane & 3) * 4);
-              __syncwarp();
-            } else {
-              float rc[EPI == EPI_QKV_NORM_ROPE ? 16 : 1], rn[EPI == EPI_QKV_NORM_ROPE ? 16 : 1];
-              if constexpr (EPI == EPI_QKV_NORM_ROPE) {
-                if (qk) {
-                  const int64_t at0 = static_cast<int64_t>(16 * sub) * args.tokens + (row_ok ? m : 0) % args.tokens;
-                  const float *cp = args.rope_cos + at0, *sp = args.rope_sin + at0;
-#pragma unroll
-                  for (int j = 0; j < 16; ++j) {
-                    rc[j] = __ldg(cp + static_cast<int64_t>(j) * args.tokens);
-                    rn[j] = __ldg(sp + static_cast<int64_t>(j) * args.tokens);
-                  }
+                for (int j = 0; j < 8; j += 2) {
+                  const uint32_t *gt = r + 8 * g + j, *up = gt + 16;
+                  const float2 h = silu_up2(make_float2(__uint_as_float(gt[0]), __uint_as_float(gt[1])),
+                                            make_float2(__uint_as_float(up[0]), __uint_as_float(up[1])));
+                  y[j] = h.x;
+                  y[j + 1] = h.y;
                 }
+                stage8(2 * sub + g, y);
               }
+            } else {
+              const int64_t at = static_cast<int64_t>(16 * sub) * args.tokens + (QKV && row_ok ? m % args.tokens : 0);
 #pragma unroll
               for (int g = 0; g < 4; ++g) {
-                scale_cols<8>(r + 8 * g, rs, cs + 8 * g, bs + 8 * g);
+                float rc[QKV ? 4 : 1], rn[QKV ? 4 : 1];
+                if constexpr (QKV) {
+                  if (qk) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                      rc[j] = __ldg(args.rope_cos + at + static_cast<int64_t>(4 * g + j) * args.tokens);
+                      rn[j] = __ldg(args.rope_sin + at + static_cast<int64_t>(4 * g + j) * args.tokens);
+                    }
+                  }
+                }
+                scale_cols<8, MX>(r + 8 * g, rs, cs + 8 * g, bs + 8 * g);
                 float y[8];
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) {
                   float2 v = make_float2(__uint_as_float(r[8 * g + j]), __uint_as_float(r[8 * g + j + 1]));
                   if constexpr (EPI == EPI_GELU_F16) v = gelu2(v);
-                  if constexpr (EPI == EPI_QKV_NORM_ROPE) {
+                  if constexpr (QKV) {
                     if (qk) {
                       const float* w = normp + (head < args.q_heads ? 0 : 128) + 32 * sub + 8 * g + j;
-                      const float x0 = fmaf((v.x - mean) * rstd, w[0], w[64]);
-                      const float x1 = fmaf((v.y - mean) * rstd, w[1], w[65]);
-                      const float c = rc[4 * g + j / 2], s = rn[4 * g + j / 2];
-                      v = make_float2(x0 * c - x1 * s, x0 * s + x1 * c);
+                      float2 x = mul2(add2(v, make_float2(-mean, -mean)), mul2(make_float2(rstd, rstd), *reinterpret_cast<const float2*>(w)));
+                      if (args.norm == FF_NORM_LAYER) x = add2(x, *reinterpret_cast<const float2*>(w + 64));
+                      const float c = rc[j / 2], s = rn[j / 2];
+                      v = make_float2(x.x * c - x.y * s, x.x * s + x.y * c);
                     }
                   }
                   y[j] = v.x;
@@ -571,9 +602,9 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR>::THREADS, 1)
               }
             }
           }
-          if (!ok) break;
-          if (!any) continue;
         }
+        if (!ok) break;
+        if (!any) continue;
         if constexpr (!F32OUT) {
           fence_async_smem();
           __syncwarp();
@@ -595,6 +626,8 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR>::THREADS, 1)
         }
       }
       if (!ok) break;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&pempty[buf]);
     }
     if (!F32OUT && lane == 0) bulk_wait_all();
   }
@@ -616,10 +649,10 @@ struct Fp4Maps {
   CUtensorMap a, w, sa, sw, c, r;
 };
 
-template <bool PAIR, int EPI, class OutT>
+template <bool PAIR, bool MX, int EPI, class OutT>
 int launch_fp4(const Fp4Maps& t, const Fp4GemmArgs& a, cudaStream_t stream) {
-  using C = Fp4Cfg<PAIR>;
-  auto kernel = gemm_fp4_kernel<PAIR, EPI, OutT>;
+  using C = Fp4Cfg<PAIR, EPI == EPI_QKV_NORM_ROPE>;
+  auto kernel = gemm_fp4_kernel<PAIR, MX, EPI, OutT>;
   static int most[64] = {};  // CTAs (pairs) resident at once per device, 0 = not configured yet
   int dev = 0;
   cudaGetDevice(&dev);
@@ -655,24 +688,24 @@ int launch_fp4(const Fp4Maps& t, const Fp4GemmArgs& a, cudaStream_t stream) {
   return check_launch("gemm_fp4_kernel");
 }
 
-template <bool PAIR>
+template <bool PAIR, bool MX>
 int dispatch_fp4(int epi, int dtype, const Fp4Maps& t, const Fp4GemmArgs& a, cudaStream_t s) {
   const bool bf = dtype == FF_BF16;
   using H = __half;
   using B = __nv_bfloat16;
   switch (epi) {
     case EPI_BIAS:
-      if (dtype == FF_F32) return launch_fp4<PAIR, EPI_BIAS, float>(t, a, s);
-      return bf ? launch_fp4<PAIR, EPI_BIAS, B>(t, a, s) : launch_fp4<PAIR, EPI_BIAS, H>(t, a, s);
-    case EPI_GELU_F16: return bf ? launch_fp4<PAIR, EPI_GELU_F16, B>(t, a, s) : launch_fp4<PAIR, EPI_GELU_F16, H>(t, a, s);
-    case EPI_SWIGLU: return bf ? launch_fp4<PAIR, EPI_SWIGLU, B>(t, a, s) : launch_fp4<PAIR, EPI_SWIGLU, H>(t, a, s);
-    case EPI_RESIDUAL: return bf ? launch_fp4<PAIR, EPI_RESIDUAL, B>(t, a, s) : launch_fp4<PAIR, EPI_RESIDUAL, H>(t, a, s);
+      if (dtype == FF_F32) return launch_fp4<PAIR, MX, EPI_BIAS, float>(t, a, s);
+      return bf ? launch_fp4<PAIR, MX, EPI_BIAS, B>(t, a, s) : launch_fp4<PAIR, MX, EPI_BIAS, H>(t, a, s);
+    case EPI_GELU_F16: return bf ? launch_fp4<PAIR, MX, EPI_GELU_F16, B>(t, a, s) : launch_fp4<PAIR, MX, EPI_GELU_F16, H>(t, a, s);
+    case EPI_SWIGLU: return bf ? launch_fp4<PAIR, MX, EPI_SWIGLU, B>(t, a, s) : launch_fp4<PAIR, MX, EPI_SWIGLU, H>(t, a, s);
+    case EPI_RESIDUAL: return bf ? launch_fp4<PAIR, MX, EPI_RESIDUAL, B>(t, a, s) : launch_fp4<PAIR, MX, EPI_RESIDUAL, H>(t, a, s);
     default:
       if constexpr (PAIR) {
         set_error("ff_gemm_fp4: no pair tiles for the QKV epilogue");
         return FF_ERR_INVALID_ARGUMENT;
       } else {
-        return bf ? launch_fp4<false, EPI_QKV_NORM_ROPE, B>(t, a, s) : launch_fp4<false, EPI_QKV_NORM_ROPE, H>(t, a, s);
+        return bf ? launch_fp4<false, MX, EPI_QKV_NORM_ROPE, B>(t, a, s) : launch_fp4<false, MX, EPI_QKV_NORM_ROPE, H>(t, a, s);
       }
   }
 }
@@ -706,7 +739,7 @@ int gemm_fp4(const Fp4Operand& A, const Fp4Operand& W, int fmt, int M, int N, in
   FF_REQUIRE(tile == 0 || tile == 128 || tile == FF_TILE_PAIR256, "ff_gemm_fp4: tile must be 0, 128 or FF_TILE_PAIR256 (got %d)",
              tile);
   FF_REQUIRE(epi != EPI_QKV_NORM_ROPE || tile != FF_TILE_PAIR256, "ff_gemm_fp4: no pair tiles for the QKV epilogue");
-  FF_REQUIRE(epi != EPI_SWIGLU || N % 128 == 0, "ff_gemm_fp4: SwiGLU needs N %% 128 == 0 (N=%d)", N);
+  FF_REQUIRE(epi != EPI_SWIGLU || N % 32 == 0, "ff_gemm_fp4: SwiGLU needs N %% 32 == 0 (N=%d)", N);
   const int out_cols = epi == EPI_SWIGLU ? (e->out_cols > 0 ? e->out_cols : N / 2) : N;
   FF_REQUIRE(epi != EPI_SWIGLU || out_cols <= N / 2, "ff_gemm_fp4: SwiGLU writes at most N / 2 columns (out_cols=%d, N=%d)",
              out_cols, N);
@@ -761,9 +794,8 @@ int gemm_fp4(const Fp4Operand& A, const Fp4Operand& W, int fmt, int M, int N, in
   a.tiles_m = pair ? (M + 255) / 256 : (M + 127) / 128;
   a.tiles_n = pair ? (N + 255) / 256 : (N + 127) / 128;
   FF_REQUIRE(static_cast<int64_t>(a.tiles_m) * a.tiles_n < (1ll << 31), "ff_gemm_fp4: too many tiles");
-  a.mx = mx;
-  a.row_scale = mx ? nullptr : A.row_scale;
-  a.col_scale = mx ? nullptr : W.row_scale;
+  a.row_scale = A.row_scale;
+  a.col_scale = W.row_scale;
   a.bias = e->bias;
   a.out = e->out;
   a.ldo = e->ldo;
@@ -783,7 +815,8 @@ int gemm_fp4(const Fp4Operand& A, const Fp4Operand& W, int fmt, int M, int N, in
   a.w_const = w_const;
   a.err = device_error_word();
   FF_REQUIRE(a.err != nullptr, "ff_gemm_fp4: no device error word");
-  return pair ? dispatch_fp4<true>(epi, e->out_dtype, t, a, stream) : dispatch_fp4<false>(epi, e->out_dtype, t, a, stream);
+  if (mx) return pair ? dispatch_fp4<true, true>(epi, e->out_dtype, t, a, stream) : dispatch_fp4<false, true>(epi, e->out_dtype, t, a, stream);
+  return pair ? dispatch_fp4<true, false>(epi, e->out_dtype, t, a, stream) : dispatch_fp4<false, false>(epi, e->out_dtype, t, a, stream);
 }
 
 }  // namespace ff

@@ -19,8 +19,8 @@ struct Fp4GemmArgs {
   int M, N, K;
   int num_kb;  // 256-column steps
   int tiles_m, tiles_n;
-  int mx;
-  const float *row_scale, *col_scale, *bias;  // NULL: 1, 1, 0
+  const float *row_scale, *col_scale;  // FF_FP4_NV
+  const float* bias;                   // or NULL
   void* out;
   int64_t ldo;
   int out_cols, tma_cols;  // columns written, and how many of them through TMA stores (a multiple of 8)

@@ -155,9 +155,9 @@ class Fp4Linear:
 
 
 def _interleave(t: torch.Tensor, h: int) -> torch.Tensor:
-    """Rows [h gates | h ups] -> [gate 64 | up 64] groups, zero rows past h (the SwiGLU epilogue's layout)."""
-    pad = -h % 64
+    """Rows [h gates | h ups] -> [gate 16 | up 16] groups, zero rows past h (the SwiGLU epilogue's layout)."""
+    pad = -h % 16
     z = t.new_zeros(pad, *t.shape[1:])
     g, u = torch.cat([t[:h], z]), torch.cat([t[h:], z])
-    n = (h + pad) // 64
-    return torch.stack([g.reshape(n, 64, *t.shape[1:]), u.reshape(n, 64, *t.shape[1:])], 1).reshape(2 * (h + pad), *t.shape[1:]).contiguous()
+    n = (h + pad) // 16
+    return torch.stack([g.reshape(n, 16, *t.shape[1:]), u.reshape(n, 16, *t.shape[1:])], 1).reshape(2 * (h + pad), *t.shape[1:]).contiguous()

@@ -180,14 +180,14 @@ int ff_dequantize_fp4(const uint8_t* codes, const uint8_t* scales, const float* 
  * (row_scale and col_scale, the two operands' row scales, are read for FF_FP4_NV only), then one of
  *   FF_EPI_BIAS           out = y                       (fp16, bf16 or f32)
  *   FF_EPI_GELU           out = gelu_tanh(y)            (fp16 or bf16, like all below)
- *   FF_EPI_SWIGLU         W rows interleaved [gate 64 | up 64]; out [M, out_cols] = silu(gate) * up, out_cols <= N / 2
+ *   FF_EPI_SWIGLU         W rows interleaved [gate 16 | up 16]; out [M, out_cols] = silu(gate) * up, out_cols <= N / 2
  *                         (0: N / 2)
  *   FF_EPI_RESIDUAL       out = residual + y, summed in f32 (residual may be out itself)
  *   FF_EPI_QKV_NORM_ROPE  heads of 64 columns, q_heads then k_heads of them, are normalised (FF_NORM_RMS:
  *                         y / rms(y) * w, FF_NORM_LAYER: (y - mean) / std * w + b) and their interleaved pairs
  *                         rotated by the angles of position m % tokens (rope_cos / rope_sin [32, tokens],
  *                         angle-major); the columns after them (v) are out = y
- * Any M, N, K >= 1 (FF_EPI_SWIGLU: N % 128 == 0; FF_EPI_QKV_NORM_ROPE: N % 64 == 0). 16-bit out and residual:
+ * Any M, N, K >= 1 (FF_EPI_SWIGLU: N % 32 == 0; FF_EPI_QKV_NORM_ROPE: N % 64 == 0). 16-bit out and residual:
  * 16-byte aligned, row strides (elements) multiples of 8. f32 out: any row stride. bias may be NULL.
  * tile: 0 = automatic, 128 = 128 x 128 tiles per CTA, FF_TILE_PAIR256 = 256 x 256 tiles per pair of CTAs (not for
  * FF_EPI_QKV_NORM_ROPE).

@@ -124,7 +124,7 @@ QKV = dict(kind=_lib.EPI_QKV_NORM_ROPE, norm=1, q_heads=1, k_heads=1, tokens=4, 
     (128, dict(kind=5), "unknown epilogue 5"),
     (128, dict(out_dtype=3), "output type 3"),
     (128, dict(kind=_lib.EPI_GELU, out_dtype=_lib.F32), "not available for epilogue"),
-    (192, dict(kind=_lib.EPI_SWIGLU), "N % 128"),
+    (144, dict(kind=_lib.EPI_SWIGLU), "N % 32"),
     (128, dict(kind=_lib.EPI_SWIGLU, out_cols=65), "at most N / 2"),
     (128, dict(ldo=120), "row stride 120"),
     (128, dict(ldo=129), "16-byte aligned rows"),
@@ -204,7 +204,9 @@ def test_python_checks_refuse_cpu_tensors_and_bad_names():
 def test_interleave_groups_gates_and_ups():
     w = torch.arange(2 * 100, dtype=torch.float32)[:, None].expand(200, 3)
     t = fp4._interleave(w, 100)
-    assert t.shape == (256, 3)
-    assert torch.equal(t[:64, 0], w[:64, 0]) and torch.equal(t[64:128, 0], w[100:164, 0])
-    assert torch.equal(t[128 : 128 + 36, 0], w[64:100, 0]) and (t[128 + 36 : 192] == 0).all()
-    assert torch.equal(t[192 : 192 + 36, 0], w[164:200, 0]) and (t[192 + 36 :] == 0).all()
+    assert t.shape == (224, 3)
+    for i in range(6):
+        assert torch.equal(t[32 * i : 32 * i + 16, 0], w[16 * i : 16 * i + 16, 0])
+        assert torch.equal(t[32 * i + 16 : 32 * i + 32, 0], w[100 + 16 * i : 100 + 16 * i + 16, 0])
+    assert torch.equal(t[192:196, 0], w[96:100, 0]) and (t[196:208] == 0).all()
+    assert torch.equal(t[208:212, 0], w[196:200, 0]) and (t[212:] == 0).all()
