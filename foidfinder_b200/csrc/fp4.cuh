@@ -93,6 +93,13 @@ struct Pair16<__nv_bfloat16> {
   }
 };
 
+// Arrive on another CTA's barrier (a shared::cluster address) without release: for an arrival that hands over
+// TMEM which this thread has finished reading (tcgen05.wait::ld), so that there are no writes to publish. The
+// releasing form waited for every outstanding write of the CTA, 1.5-2 us under the epilogue's stores.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
 // ---------------------------------------------------------------- tcgen05
 // Instruction descriptor of the block-scaled 4-bit MMAs, both operands e2m1 and K-major.
 // Bits: [4,6) B scale id, [7,10) A format, [10,12) B format (1 = e2m1), [17,23) N>>3, 23 scale type

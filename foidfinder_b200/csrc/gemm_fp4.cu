@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR, EPI == EPI_QKV_NORM_ROPE>::THREAD
           __syncwarp();
           if (lane == 0) {
             if (PAIR && !leader)
-              mbar_arrive_cluster(mapa_shared(smem_u32(bar), 0u));
+              mbar_arrive_cluster_relaxed(mapa_shared(smem_u32(bar), 0u));
             else
               mbar_arrive(bar);
           }
