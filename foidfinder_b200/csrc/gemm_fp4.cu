@@ -33,15 +33,18 @@ struct Fp4Cfg {
   static constexpr int STAGE_BYTES = 2 * CODE_BYTES + SFA_BYTES + SFB_BYTES;
   // EPI_QKV_NORM_ROPE: three stages leave the L1 cache room for a row block's rotation angles (32 KB)
   static constexpr int STAGES = QKV ? 3 : 4;
-  static constexpr int GROUP_WARPS = 8;  // epilogue warps of one accumulator
-  static constexpr int THREADS = 128 + 2 * 32 * GROUP_WARPS;
+  static constexpr int GROUP_WARPS = 8;  // epilogue warps that work on one accumulator
+  // Two groups take turns with the tiles; EPI_QKV_NORM_ROPE has one, whose lanes then have registers for a whole head
+  // (168 instead of 96).
+  static constexpr int GROUPS = QKV ? 1 : 2;
+  static constexpr int THREADS = 128 + GROUPS * 32 * GROUP_WARPS;
   static constexpr int STAGING = 4096;      // per epilogue warp: 32 rows x 128 B
   static constexpr int COLP = 2 * BN * 4;   // column scales and biases of a tile
   static constexpr int COLP_BUFS = 4;       // tiles that they are read ahead
   static constexpr int NORM_BYTES = 4 * 64 * 4;  // q and k norm weights and biases
   static constexpr int BAR_BYTES = 512;
   static constexpr int SMEM =
-      1024 + STAGES * STAGE_BYTES + 2 * GROUP_WARPS * STAGING + COLP_BUFS * COLP + (QKV ? NORM_BYTES : 0) + BAR_BYTES;
+      1024 + STAGES * STAGE_BYTES + GROUPS * GROUP_WARPS * STAGING + COLP_BUFS * COLP + (QKV ? NORM_BYTES : 0) + BAR_BYTES;
   // TMEM: two accumulators and two buffers of scales, each for one chunk of A's and W's columns. Two 256-column
   // accumulators and the scales do not fit 512 columns: the pair's accumulators share 32 columns, the last of
   // the first and the first of the second, which the epilogue empties first.
@@ -137,7 +140,7 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR, EPI == EPI_QKV_NORM_ROPE>::THREAD
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* staging = smem + STAGES * C::STAGE_BYTES;
-  float* colp = reinterpret_cast<float*>(staging + 2 * C::GROUP_WARPS * C::STAGING);
+  float* colp = reinterpret_cast<float*>(staging + C::GROUPS * C::GROUP_WARPS * C::STAGING);
   float* normp = colp + C::COLP_BUFS * (C::COLP / 4);  // EPI_QKV_NORM_ROPE: q weight, q bias, k weight, k bias
   uint64_t* full = reinterpret_cast<uint64_t*>(normp + (QKV ? C::NORM_BYTES / 4 : 0));
   uint64_t* empty = full + STAGES;
@@ -374,31 +377,33 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR, EPI == EPI_QKV_NORM_ROPE>::THREAD
     // mainloops for a tile. A warp reads one lane quarter (32 rows) and half of the tile's columns, 32 at a time.
     pdl_wait();
     const int ew = warp - 4;
-    const int acc = ew >> 3;         // group
+    const int group = ew >> 3;       // with two groups, also the accumulator that it works on
     const int q = warp & 3;          // TMEM lane quarter
     const int half = (ew >> 2) & 1;  // of the tile's columns
     uint8_t* const stg = staging + ew * C::STAGING;
     if constexpr (EPI == EPI_QKV_NORM_ROPE) {
-      for (int i = threadIdx.x - 128; i < 64; i += 2 * 32 * C::GROUP_WARPS) {
+      for (int i = threadIdx.x - 128; i < 64; i += C::GROUPS * 32 * C::GROUP_WARPS) {
         normp[i] = args.q_w[i];
         normp[64 + i] = args.q_b != nullptr ? args.q_b[i] : 0.f;
         normp[128 + i] = args.k_w[i];
         normp[192 + i] = args.k_b != nullptr ? args.k_b[i] : 0.f;
       }
-      asm volatile("bar.sync 1, %0;" ::"n"(2 * 32 * C::GROUP_WARPS) : "memory");  // the epilogue warps
+      asm volatile("bar.sync 1, %0;" ::"n"(C::GROUPS * 32 * C::GROUP_WARPS) : "memory");  // the epilogue warps
     }
     constexpr bool SWIGLU = EPI == EPI_SWIGLU;
     constexpr int STEPS = HALF / 64;           // 64 tile columns per step
     constexpr int WIDTH = SWIGLU ? 32 : 64;    // output columns per step
-    uint32_t use = 0, res_phase = 0;
+    uint32_t res_phase = 0;
     // The lane's row scale, read a tile ahead: with the epilogue at work all the time its latency would be exposed.
     auto row_scale_of = [&](int i) {
       if (MX || i >= my_tiles) return 1.f;
       const int row = (t_first + i * t_step) / tiles_n * C::TILE_M + static_cast<int>(rank) * 128 + q * 32 + lane;
       return row < args.M ? __ldg(args.row_scale + row) : 0.f;
     };
-    float rs_next = row_scale_of(acc);
-    for (int i = acc; i < my_tiles; i += 2, use ^= 1u) {
+    float rs_next = row_scale_of(group);
+    for (int i = group; i < my_tiles; i += C::GROUPS) {
+      const int acc = C::GROUPS == 2 ? group : i & 1;
+      const uint32_t use = (i >> 1) & 1;
       const int t = t_first + i * t_step;
       const int tm = t / tiles_n, tn = t - tm * tiles_n;
       const int buf = i % C::COLP_BUFS;
@@ -408,6 +413,7 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR, EPI == EPI_QKV_NORM_ROPE>::THREAD
       const bool row_ok = m < args.M;
       const int n_tile = tn * BN;
       const float rs = rs_next;
+      const uint32_t pos = QKV && row_ok ? static_cast<uint32_t>(m % args.tokens) : 0u;
       const uint32_t tbase = tmem + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc) * C::ACC_STRIDE;
       bool ok = true;
 #pragma unroll 1
@@ -456,7 +462,7 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR, EPI == EPI_QKV_NORM_ROPE>::THREAD
         auto arrive_empty = [&]() {
           if (step == STEPS - 1) {
             arrive(&tempty[acc]);
-            rs_next = row_scale_of(i + 2);
+            rs_next = row_scale_of(i + C::GROUPS);
           }
         };
         auto read32 = [&](int col, uint32_t(&r)[32]) {
@@ -498,31 +504,86 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR, EPI == EPI_QKV_NORM_ROPE>::THREAD
             group_end();
           }
         };
-        // The head norm's statistics first, from reads of their own: the accumulator is read again below.
-        const int head = out0 >> 6;
-        float mean = 0.f, rstd = 1.f;
-        const bool qk = EPI == EPI_QKV_NORM_ROPE && any && head < args.q_heads + args.k_heads;
-        if constexpr (EPI == EPI_QKV_NORM_ROPE) {
-          auto over_head = [&](auto f) {
-#pragma unroll 1
-            for (int sub = 0; sub < 2; ++sub) {
-              uint32_t r[32];
-              read32(ca + 32 * sub, r);
-              scale_cols<32, MX>(r, rs, csa + 32 * sub, ba + 32 * sub);
-#pragma unroll
-              for (int j = 0; j < 32; ++j) f(__uint_as_float(r[j]));
-            }
-          };
-          if (qk) {
-            if (args.norm == FF_NORM_LAYER) {
-              over_head([&](float v) { mean += v; });
-              mean *= 1.f / 64.f;
-            }
-            float ss = 0.f;
-            over_head([&](float v) { ss = fmaf(v - mean, v - mean, ss); });
-            rstd = rsqrtf(ss * (1.f / 64.f) + args.qk_eps);
+        if constexpr (QKV) {
+          // The step's 64 columns are one head, in registers whole.
+          uint32_t r[64];
+          if (any) {
+            tmem_ld32(tbase + ca, reinterpret_cast<uint32_t(&)[32]>(r[0]));
+            tmem_ld32(tbase + ca + 32, reinterpret_cast<uint32_t(&)[32]>(r[32]));
+            tmem_ld_wait();
           }
-        }
+          arrive_empty();
+          if (!any) continue;
+          const int head = out0 >> 6;
+          auto pair_of = [&](int j) { return make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])); };
+          if (head >= args.q_heads + args.k_heads) {  // v
+#pragma unroll
+            for (int g = 0; g < 8; ++g) {
+              scale_cols<8, MX>(r + 8 * g, rs, csa + 8 * g, ba + 8 * g);
+              float z[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) z[j] = __uint_as_float(r[8 * g + j]);
+              stage8(g, z);
+            }
+          } else {
+            // Angles of four pairs, read one group ahead of their use; volatile, with the pointers stepped in place,
+            // so that the compiler neither reads all of them at once nor keeps an address for each.
+            const float *cp = args.rope_cos + pos, *sp = args.rope_sin + pos;
+            float rope[2][8];
+            auto load_angles = [&](float(&a)[8]) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                asm volatile(
+                    "ld.global.nc.f32 %0, [%2];\n\tld.global.nc.f32 %1, [%3];\n\t"
+                    "add.s64 %2, %2, %4;\n\tadd.s64 %3, %3, %4;"
+                    : "=&f"(a[2 * j]), "=&f"(a[2 * j + 1]), "+l"(cp), "+l"(sp)
+                    : "l"(static_cast<int64_t>(args.tokens) * 4));
+            };
+            load_angles(rope[0]);
+#pragma unroll
+            for (int g = 0; g < 8; ++g) {
+              scale_cols<8, MX>(r + 8 * g, rs, csa + 8 * g, ba + 8 * g);
+              group_end();
+            }
+            float mean = 0.f;
+            if (args.norm == FF_NORM_LAYER) {
+              float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) sum = add2(sum, pair_of(j));
+              mean = (sum.x + sum.y) * (1.f / 64.f);
+            }
+            const float2 m2 = make_float2(-mean, -mean);
+            float2 sq = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const float2 d = add2(pair_of(j), m2);
+              sq = fma2(d, d, sq);
+            }
+            const float rstd = rsqrtf((sq.x + sq.y) * (1.f / 64.f) + args.qk_eps);
+            const float2 r2 = make_float2(rstd, rstd);
+            const float* const w = normp + (head < args.q_heads ? 0 : 128);  // weights, then biases (zero for RMS)
+#pragma unroll
+            for (int g = 0; g < 8; ++g) {
+              if (g < 7) load_angles(rope[(g + 1) & 1]);
+              float z[8];
+#pragma unroll
+              for (int j = 0; j < 4; j += 2) {
+                const float4 w4 = *reinterpret_cast<const float4*>(w + 8 * g + 2 * j);
+                const float4 b4 = *reinterpret_cast<const float4*>(w + 64 + 8 * g + 2 * j);
+                const float2 x[2] = {
+                    fma2(add2(pair_of(4 * g + j), m2), mul2(r2, make_float2(w4.x, w4.y)), make_float2(b4.x, b4.y)),
+                    fma2(add2(pair_of(4 * g + j + 1), m2), mul2(r2, make_float2(w4.z, w4.w)), make_float2(b4.z, b4.w))};
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                  const float c = rope[g & 1][2 * (j + k)], sn = rope[g & 1][2 * (j + k) + 1];
+                  z[2 * (j + k)] = x[k].x * c - x[k].y * sn;
+                  z[2 * (j + k) + 1] = x[k].x * sn + x[k].y * c;
+                }
+              }
+              stage8(g, z);
+            }
+          }
+        } else {
 #pragma unroll 1
         for (int k = 0; k < 2; ++k) {
           const int sub = acc == 0 ? 1 - k : k;  // the shared columns first
@@ -567,34 +628,14 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR, EPI == EPI_QKV_NORM_ROPE>::THREAD
                 stage8(2 * sub + g, y);
               }
             } else {
-              const int64_t at = static_cast<int64_t>(16 * sub) * args.tokens + (QKV && row_ok ? m % args.tokens : 0);
 #pragma unroll
               for (int g = 0; g < 4; ++g) {
-                float rc[QKV ? 4 : 1], rn[QKV ? 4 : 1];
-                if constexpr (QKV) {
-                  if (qk) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                      rc[j] = __ldg(args.rope_cos + at + static_cast<int64_t>(4 * g + j) * args.tokens);
-                      rn[j] = __ldg(args.rope_sin + at + static_cast<int64_t>(4 * g + j) * args.tokens);
-                    }
-                  }
-                }
                 scale_cols<8, MX>(r + 8 * g, rs, cs + 8 * g, bs + 8 * g);
                 float y[8];
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) {
                   float2 v = make_float2(__uint_as_float(r[8 * g + j]), __uint_as_float(r[8 * g + j + 1]));
                   if constexpr (EPI == EPI_GELU_F16) v = gelu2(v);
-                  if constexpr (QKV) {
-                    if (qk) {
-                      const float* w = normp + (head < args.q_heads ? 0 : 128) + 32 * sub + 8 * g + j;
-                      float2 x = mul2(add2(v, make_float2(-mean, -mean)), mul2(make_float2(rstd, rstd), *reinterpret_cast<const float2*>(w)));
-                      if (args.norm == FF_NORM_LAYER) x = add2(x, *reinterpret_cast<const float2*>(w + 64));
-                      const float c = rc[j / 2], s = rn[j / 2];
-                      v = make_float2(x.x * c - x.y * s, x.x * s + x.y * c);
-                    }
-                  }
                   y[j] = v.x;
                   y[j + 1] = v.y;
                 }
@@ -605,6 +646,7 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR, EPI == EPI_QKV_NORM_ROPE>::THREAD
         }
         if (!ok) break;
         if (!any) continue;
+        }
         if constexpr (!F32OUT) {
           fence_async_smem();
           __syncwarp();
@@ -723,6 +765,19 @@ int code_map(CUtensorMap* map, const uint8_t* codes, int rows, int cols) {
                               128, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// Whether 256 x 256 tiles over CTA pairs are the faster choice: rounds of tiles times the time of one, measured at
+// K = 1024 and 8192: 128 x 128 tiles 1.45 us (their epilogue) or 0.30 us per 256 columns of K, pair tiles 2.75 us or
+// 0.415 us. (65600 x 5504 x 1024 SwiGLU 201 us in pairs, 224 us without; 65600 x 1024 x 2730 97 and 139 us;
+// 8200 x 4096 x 768 21.2 and 20.3 us.)
+bool choose_pair_fp4(int M, int N, int K) {
+  const int64_t steps = (K + kFp4Step - 1) / kFp4Step, sms = sm_count(), pairs = sms / 2;
+  const int64_t single = static_cast<int64_t>((M + 127) / 128) * ((N + 127) / 128);
+  const int64_t pair = static_cast<int64_t>((M + 255) / 256) * ((N + 255) / 256);
+  const double t_single = static_cast<double>((single + sms - 1) / sms) * (steps > 4 ? 0.30 * steps : 1.45);
+  const double t_pair = static_cast<double>((pair + pairs - 1) / pairs) * (steps > 6 ? 0.415 * steps : 2.75);
+  return t_pair < t_single;
+}
+
 }  // namespace
 
 int gemm_fp4(const Fp4Operand& A, const Fp4Operand& W, int fmt, int M, int N, int K, const ff_fp4_epilogue* e, int tile,
@@ -748,7 +803,7 @@ int gemm_fp4(const Fp4Operand& A, const Fp4Operand& W, int fmt, int M, int N, in
     FF_REQUIRE(e->norm == FF_NORM_RMS || e->norm == FF_NORM_LAYER, "ff_gemm_fp4: unknown head norm %d", e->norm);
     FF_REQUIRE(e->q_heads >= 0 && e->k_heads >= 0 && N % 64 == 0 && static_cast<int64_t>(e->q_heads) + e->k_heads <= N / 64,
                "ff_gemm_fp4: %d + %d heads of 64 columns do not fit N=%d", e->q_heads, e->k_heads, N);
-    FF_REQUIRE(e->q_w && e->k_w && e->rope_cos && e->rope_sin && e->tokens >= 1,
+    FF_REQUIRE(e->q_w && e->k_w && e->rope_cos && e->rope_sin && e->tokens >= 1 && e->tokens <= (1 << 25),
                "ff_gemm_fp4: the QKV epilogue needs q and k norm weights, rotation tables and tokens");
   }
   if (M == 0) return FF_OK;
@@ -762,8 +817,7 @@ int gemm_fp4(const Fp4Operand& A, const Fp4Operand& W, int fmt, int M, int N, in
   FF_REQUIRE(!f32 || reinterpret_cast<uintptr_t>(e->out) % 4 == 0, "ff_gemm_fp4: out is not aligned to its type");
   FF_REQUIRE(epi != EPI_RESIDUAL || (aligned16(e->residual) && e->ldr % 8 == 0), "ff_gemm_fp4: residual rows must be 16-byte aligned");
 
-  const int64_t pair_tiles = static_cast<int64_t>((M + 255) / 256) * ((N + 255) / 256);
-  const bool pair = tile == FF_TILE_PAIR256 || (tile == 0 && epi != EPI_QKV_NORM_ROPE && pair_tiles >= sm_count());
+  const bool pair = tile == FF_TILE_PAIR256 || (tile == 0 && epi != EPI_QKV_NORM_ROPE && choose_pair_fp4(M, N, K));
   Fp4Maps t;
   const bool mx = fmt == FF_FP4_MX;
   int rc;
