@@ -3,9 +3,10 @@
 //   (y0, y1) -> (y0 cos - y1 sin, y0 sin + y1 cos) for every pair, f32 throughout, one rounding at the end.
 //
 // Bound by HBM: every value is read and written once (4 bytes). One warp per row: 8 values (16 bytes) per lane,
-// D / 8 lanes per head, so the norm is a sum over D / 8 lanes and a pair of FF_ROPE_PAIRS stays in its lane. The
-// row's angles and the weights stay in registers over its heads; a CTA takes 8 neighbouring rows, whose angles
-// share cache sectors of the angle-major tables.
+// D / 8 lanes per head, so the norm is a sum over D / 8 lanes and a pair of FF_ROPE_PAIRS stays in its lane. Warps
+// are persistent and keep the weights in registers, a row's angles serve all its heads, and the loads of four steps
+// are issued before the first is worked on. A CTA takes 8 neighbouring rows, whose angles share cache sectors of the
+// angle-major tables.
 #include "common.h"
 #include "fp4.cuh"
 
@@ -14,6 +15,7 @@ namespace ff {
 namespace {
 
 constexpr int kQkWarps = 8;
+constexpr int kQkCtas = 3;  // per SM
 
 struct QkArgs {
   const void* x;
@@ -28,86 +30,98 @@ struct QkArgs {
 };
 
 template <class T, int D, bool LAYER, bool HALVES>
-__global__ void __launch_bounds__(32 * kQkWarps) qk_norm_rope_kernel(const QkArgs a) {
+__global__ void __launch_bounds__(32 * kQkWarps, kQkCtas) qk_norm_rope_kernel(const QkArgs a) {
   constexpr int G = D / 8;       // lanes per head
   constexpr int HPW = 32 / G;    // heads per warp and step
   constexpr int NA = HALVES ? 8 : 4;  // angles per lane
+  constexpr int U = 4;           // steps whose loads are issued together
   const int lane = threadIdx.x & 31, l = lane % G, hl = lane / G;
-  const int row = blockIdx.x * kQkWarps + (threadIdx.x >> 5);
   pdl_wait();
   pdl_trigger();
-  if (row >= a.rows) return;
-  const int pos = row % a.tokens;
-  float c[NA], s[NA];
+  float wq[8], wk[8], bq[LAYER ? 8 : 1], bk[LAYER ? 8 : 1];
 #pragma unroll
-  for (int i = 0; i < NA; ++i) {
-    const int j = HALVES ? (l % (G / 2)) * 8 + i : l * 4 + i;
-    c[i] = __ldg(a.cos + static_cast<int64_t>(j) * a.tokens + pos);
-    s[i] = __ldg(a.sin + static_cast<int64_t>(j) * a.tokens + pos);
-  }
-  const T* xr = static_cast<const T*>(a.x) + row * a.ldx;
-  T* orow = static_cast<T*>(a.out) + row * a.ldo;
-  const int heads = a.q_heads + a.k_heads;
-#pragma unroll 2
-  for (int h0 = 0; h0 < heads; h0 += HPW) {
-    const int h = h0 + hl;
-    const bool on = h < heads;
-    uint4 u = make_uint4(0, 0, 0, 0);
-    if (on) u = *reinterpret_cast<const uint4*>(xr + h * D + l * 8);
-    const uint32_t w4[4] = {u.x, u.y, u.z, u.w};
-    float y[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = Pair16<T>::unpack(w4[i]);
-      y[2 * i] = f.x;
-      y[2 * i + 1] = f.y;
-    }
+  for (int i = 0; i < 8; ++i) {
+    wq[i] = a.q_w != nullptr ? __ldg(a.q_w + l * 8 + i) : 0.f;
+    wk[i] = a.k_w != nullptr ? __ldg(a.k_w + l * 8 + i) : 0.f;
     if constexpr (LAYER) {
-      float m = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) m += y[i];
-#pragma unroll
-      for (int o = G / 2; o; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
-      m *= 1.f / D;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] -= m;
+      bq[i] = a.q_b != nullptr ? __ldg(a.q_b + l * 8 + i) : 0.f;
+      bk[i] = a.k_b != nullptr ? __ldg(a.k_b + l * 8 + i) : 0.f;
     }
-    float ss = 0.f;
+  }
+  const int step = static_cast<int>(gridDim.x) * kQkWarps;
+  for (int row = static_cast<int>(blockIdx.x) * kQkWarps + (threadIdx.x >> 5); row < a.rows; row += step) {
+    const int pos = row % a.tokens;
+    float c[NA], s[NA];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss = fmaf(y[i], y[i], ss);
-#pragma unroll
-    for (int o = G / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const float rstd = rsqrtf(ss * (1.f / D) + a.eps);
-    const float* w = h < a.q_heads ? a.q_w : a.k_w;
-    const float* b = h < a.q_heads ? a.q_b : a.k_b;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      y[i] = y[i] * rstd * __ldg(w + l * 8 + i);
-      if (LAYER && b != nullptr) y[i] += __ldg(b + l * 8 + i);
+    for (int i = 0; i < NA; ++i) {
+      const int j = HALVES ? (l % (G / 2)) * 8 + i : l * 4 + i;
+      c[i] = __ldg(a.cos + static_cast<int64_t>(j) * a.tokens + pos);
+      s[i] = __ldg(a.sin + static_cast<int64_t>(j) * a.tokens + pos);
     }
-    if constexpr (HALVES) {
+    // The heads of one kind (q or k), which start at column `col` of the row.
+    auto heads = [&](int64_t col, int count, const float(&w)[8], const float(&b)[LAYER ? 8 : 1]) {
+      const T* const xr = static_cast<const T*>(a.x) + row * a.ldx + col + l * 8;
+      T* const orow = static_cast<T*>(a.out) + row * a.ldo + col + l * 8;
+      for (int h0 = hl; h0 - hl < count; h0 += U * HPW) {
+        uint4 u[U];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float other = __shfl_xor_sync(0xffffffffu, y[i], G / 2);
-        y[i] = l < G / 2 ? y[i] * c[i] - other * s[i] : other * s[i] + y[i] * c[i];
+        for (int k = 0; k < U; ++k)
+          u[k] = h0 + k * HPW < count ? *reinterpret_cast<const uint4*>(xr + (h0 + k * HPW) * D) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+          if (h0 - hl + k * HPW >= count) break;  // the whole warp
+          float2 y[4] = {Pair16<T>::unpack(u[k].x), Pair16<T>::unpack(u[k].y), Pair16<T>::unpack(u[k].z), Pair16<T>::unpack(u[k].w)};
+          if constexpr (LAYER) {
+            const float2 t = add2(add2(y[0], y[1]), add2(y[2], y[3]));
+            float m = t.x + t.y;
+#pragma unroll
+            for (int o = G / 2; o; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
+            m *= -1.f / D;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = add2(y[i], make_float2(m, m));
+          }
+          float2 q = mul2(y[0], y[0]);
+#pragma unroll
+          for (int i = 1; i < 4; ++i) q = fma2(y[i], y[i], q);
+          float ss = q.x + q.y;
+#pragma unroll
+          for (int o = G / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          const float rstd = rsqrtf(ss * (1.f / D) + a.eps);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 wr = mul2(make_float2(rstd, rstd), make_float2(w[2 * i], w[2 * i + 1]));
+            if constexpr (LAYER)
+              y[i] = fma2(y[i], wr, make_float2(b[2 * i], b[2 * i + 1]));
+            else
+              y[i] = mul2(y[i], wr);
+          }
+          if constexpr (HALVES) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 other = make_float2(__shfl_xor_sync(0xffffffffu, y[i].x, G / 2), __shfl_xor_sync(0xffffffffu, y[i].y, G / 2));
+              const float sx = l < G / 2 ? -s[2 * i] : s[2 * i], sy = l < G / 2 ? -s[2 * i + 1] : s[2 * i + 1];
+              y[i] = make_float2(y[i].x * c[2 * i] + other.x * sx, y[i].y * c[2 * i + 1] + other.y * sy);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = make_float2(y[i].x * c[i] - y[i].y * s[i], y[i].x * s[i] + y[i].y * c[i]);
+          }
+          if (h0 + k * HPW < count)
+            *reinterpret_cast<uint4*>(orow + (h0 + k * HPW) * D) =
+                make_uint4(Pair16<T>::pack(y[0].x, y[0].y), Pair16<T>::pack(y[1].x, y[1].y),
+                           Pair16<T>::pack(y[2].x, y[2].y), Pair16<T>::pack(y[3].x, y[3].y));
+        }
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float y0 = y[2 * i], y1 = y[2 * i + 1];
-        y[2 * i] = y0 * c[i] - y1 * s[i];
-        y[2 * i + 1] = y0 * s[i] + y1 * c[i];
-      }
-    }
-    if (on)
-      *reinterpret_cast<uint4*>(orow + h * D + l * 8) = make_uint4(
-          Pair16<T>::pack(y[0], y[1]), Pair16<T>::pack(y[2], y[3]), Pair16<T>::pack(y[4], y[5]), Pair16<T>::pack(y[6], y[7]));
+    };
+    heads(0, a.q_heads, wq, bq);
+    heads(static_cast<int64_t>(a.q_heads) * D, a.k_heads, wk, bk);
   }
 }
 
 template <class T, int D>
 void launch_qk(const QkArgs& a, int norm, int pairing, cudaStream_t s) {
-  const dim3 grid((a.rows + kQkWarps - 1) / kQkWarps), block(32 * kQkWarps);
+  const int want = (a.rows + kQkWarps - 1) / kQkWarps, most = sm_count() * kQkCtas;
+  const dim3 grid(want < most ? want : most), block(32 * kQkWarps);
   if (norm == FF_NORM_LAYER) {
     if (pairing == FF_ROPE_HALVES)
       launch(qk_norm_rope_kernel<T, D, true, true>, grid, block, 0, s, a);
