@@ -13,6 +13,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib, ops
+from .config import ModelConfig
 
 FORMATS = {"nv": _lib.FP4_NV, "mx": _lib.FP4_MX}
 EPILOGUES = {
@@ -161,3 +162,50 @@ def _interleave(t: torch.Tensor, h: int) -> torch.Tensor:
     g, u = torch.cat([t[:h], z]), torch.cat([t[h:], z])
     n = (h + pad) // 16
     return torch.stack([g.reshape(n, 16, *t.shape[1:]), u.reshape(n, 16, *t.shape[1:])], 1).reshape(2 * (h + pad), *t.shape[1:]).contiguous()
+
+
+class Fp4Block:
+    """One pre-norm transformer block of a tagger with 4-bit products and normalised queries and keys:
+
+        x -> LayerNorm, qkv product, q/k head norm and rotation -> attention -> proj product + x
+          -> LayerNorm, up product with SwiGLU (EVA02) or GELU (PixAI) -> (hidden LayerNorm), down product + x
+
+    in four calls of a linear layer (a quantisation, with its LayerNorm, and a product each) and one of attention. `raw` holds the
+    block's f32 weights under `prefix` with the names of `weights.random_raw` (norm1, qkv, proj, norm2, fc1, mlp_norm,
+    fc2); q_weight and k_weight [64] are the head norms' weights; rope the angle-major tables (cos, sin), [32, tokens].
+    """
+
+    def __init__(
+        self,
+        raw: dict[str, torch.Tensor],
+        prefix: str,
+        cfg: ModelConfig,
+        *,
+        q_weight: torch.Tensor,
+        k_weight: torch.Tensor,
+        rope: tuple[torch.Tensor, torch.Tensor],
+        fmt: str = "nv",
+        device: torch.device | str = "cuda",
+    ) -> None:
+        if cfg.head_dim != 64:
+            raise RuntimeError(f"Fp4Block: heads of {cfg.head_dim} columns (the attention takes 64)")
+        w = {k[len(prefix) :]: v.to(device) for k, v in raw.items() if k.startswith(prefix)}
+        eva = cfg.arch == "eva02"
+
+        def linear(name: str, epilogue: str, norm: str | None, **kw) -> Fp4Linear:
+            g, b = (w[norm + ".weight"], w[norm + ".bias"]) if norm else (None, None)
+            return Fp4Linear(w[name + ".weight"], w[name + ".bias"], fmt=fmt, epilogue=epilogue, gamma=g, beta=b, eps=cfg.ln_eps, **kw)
+
+        self.heads, self.tokens = cfg.heads, rope[0].shape[1]
+        self.qkv = linear("qkv", "qkv", "norm1", rope=rope, q_weight=q_weight, k_weight=k_weight, qk_eps=cfg.ln_eps)
+        self.proj = linear("proj", "residual", None)
+        self.fc1 = linear("fc1", "swiglu" if eva else "gelu", "norm2")
+        self.fc2 = linear("fc2", "residual", "mlp_norm" if eva else None)
+
+    def __call__(self, x: torch.Tensor) -> torch.Tensor:
+        """x [sequences * tokens, dim] fp16 -> the same; x itself is left as it is."""
+        qkv = self.qkv(x)
+        o = torch.empty_like(x)
+        ops.attention(qkv, o, self.tokens, self.heads, scale=0.125)
+        y = self.proj(o, residual=x)
+        return self.fc2(self.fc1(y), out=y, residual=y)

@@ -6,6 +6,8 @@ stream after warm-up. Also the entry point for ncu captures of single kernels.
     python -m foidfinder_b200.microbench attention [--batch 64] [--seq 1025] [--iters 20]
     python -m foidfinder_b200.microbench rotate [--batch 64] [--tokens 1025] [--cols 1024 ...] [--iters 20]
     python -m foidfinder_b200.microbench peak      (measured dense int8 tensor-core TOPS)
+    python -m foidfinder_b200.microbench fp4 [--batch 64] [--format nv|mx] [--iters 20]
+                                              (one EVA02-L block on 4-bit operands, and its parts)
 
 PixAI-1008 shapes: `attention --batch 144 --seq 576` (16 images x 9 windows), `attention --batch 16 --seq
 5184` (global blocks), `rotate --batch 16 --tokens 5184 --cols 1024 --cols 4864`.
@@ -110,9 +112,38 @@ def bench_rotate(batch: int, iters: int, tokens: int = TOKENS, widths: list[int]
                           "gbs": nbytes / ms / 1e6}))
 
 
+def bench_fp4(batch: int, iters: int, fmt: str) -> None:
+    from . import fp4
+    from .config import EVA02_L
+    from .weights import random_raw, rope_tables
+
+    d = torch.device("cuda")
+    cfg = EVA02_L.with_(depth=1)
+    M = cfg.tokens * batch
+    cos, sin = (t.t().contiguous().to(d) for t in rope_tables(cfg.grid, cfg.rope_ref_grid))
+    ones = torch.ones(64, device=d)
+    block = fp4.Fp4Block(random_raw(cfg, seed=0, device=d), "blocks.0.", cfg, q_weight=ones, k_weight=ones, rope=(cos, sin), fmt=fmt)
+    x = torch.randn(M, cfg.dim, device=d).half()
+    qkv, h, o = block.qkv(x), block.fc1(x), torch.empty_like(x)
+    q = fp4.Fp4Tensor.empty(M, cfg.dim, fmt)
+    qk = torch.empty(M, 2 * cfg.dim, device=d, dtype=torch.float16)
+    parts = {
+        "block": lambda: block(x),
+        "quantize_fp4": lambda: fp4.quantize(x, out=q),
+        "norm + qkv + qk norm + rope": lambda: block.qkv(x, out=qkv),
+        "proj + residual": lambda: block.proj(x, out=o, residual=x),
+        "norm + gate/up + swiglu": lambda: block.fc1(x, out=h),
+        "hidden norm + down + residual": lambda: block.fc2(h, out=o, residual=x),
+        "qk_norm_rope": lambda: ops.qk_norm_rope(qkv, qk, q_heads=cfg.heads, k_heads=cfg.heads, head_dim=64, norm="rms", q_weight=ones,
+                                                 k_weight=ones, rope_cos=cos, rope_sin=sin),
+    }
+    for name, fn in parts.items():
+        print(json.dumps({"kernel": "fp4", "part": name, "format": fmt, "M": M, "ms": _time(fn, iters)}))
+
+
 def main() -> None:
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
-    ap.add_argument("kernel", choices=("gemm", "attention", "rotate", "peak"))
+    ap.add_argument("kernel", choices=("gemm", "attention", "rotate", "peak", "fp4"))
     ap.add_argument("--batch", type=int, default=64)
     ap.add_argument("--iters", type=int, default=20)
     ap.add_argument("--shape", action="append", choices=sorted(GEMM_SHAPES))
@@ -121,8 +152,11 @@ def main() -> None:
     ap.add_argument("--seq", type=int, default=TOKENS, help="attention: sequence length")
     ap.add_argument("--tokens", type=int, default=TOKENS, help="rotate: rows per image")
     ap.add_argument("--cols", type=int, action="append", choices=sorted(ROT_CASES), help="rotate: row widths")
+    ap.add_argument("--format", default="nv", choices=("nv", "mx"), help="fp4: operand format")
     a = ap.parse_args()
-    if a.kernel == "peak":
+    if a.kernel == "fp4":
+        bench_fp4(a.batch, a.iters, a.format)
+    elif a.kernel == "peak":
         for _ in range(3):
             print(json.dumps({"kernel": "int8_mma_peak", "tops": ops.int8_mma_peak()}))
     elif a.kernel == "gemm":

@@ -419,3 +419,73 @@ def test_qk_norm_of_zero_and_huge_heads(cuda_device, no_device_error):
     got = out.cpu().float()
     assert (got[0] == 0).all() and (got[1] == 1).all() and (got[3] == 0).all()
     assert torch.isnan(got[2, :64]).all() and (got[2, 64:] == 0).all()
+
+
+@pytest.mark.parametrize("fmt", ["nv", "mx"])
+@pytest.mark.parametrize("arch", ["eva02", "pixai"])
+def test_fp4_block(cuda_device, no_device_error, arch, fmt):
+    """Every linear layer of the block against 64 bits on the inputs that the block gave it, and the block's output as a
+    whole. After a LayerNorm 1 in 1000 codes may be off by a step (a quarter of the value): sqrt(1e-3) / 4 = 0.8%, with
+    the storage rounding 2% is left for each layer. Across layers a stored fp16 value that rounds the other way moves
+    codes too, but the residual stream carries most of the output: 2% for the block."""
+    from foidfinder_b200 import fp4
+    from foidfinder_b200.config import EVA02_B, PIXAI_1008
+    from foidfinder_b200.weights import random_raw
+
+    d = cuda_device
+    cfg = EVA02_B.with_(depth=1, image_size=56) if arch == "eva02" else PIXAI_1008.with_(depth=1, image_size=112, window=0, dim=256, heads=4, mlp_hidden=600)
+    T, D, H = cfg.tokens, cfg.dim, cfg.heads
+    g = torch.Generator().manual_seed(1)
+    if arch == "eva02":
+        raw = {k: v for k, v in random_raw(cfg, seed=2).items() if k.startswith("blocks.0.")}
+    else:
+        raw = {}
+        for name, (n, k) in {"qkv": (3 * D, D), "proj": (D, D), "fc1": (cfg.mlp_hidden, D), "fc2": (D, cfg.mlp_hidden)}.items():
+            raw[f"blocks.0.{name}.weight"] = torch.randn(n, k, generator=g) * 0.05
+            raw[f"blocks.0.{name}.bias"] = torch.randn(n, generator=g) * 0.02
+        for name in ("norm1", "norm2"):
+            raw[f"blocks.0.{name}.weight"] = 1 + 0.02 * torch.randn(D, generator=g)
+            raw[f"blocks.0.{name}.bias"] = 0.02 * torch.randn(D, generator=g)
+    qw, kw = 1 + 0.1 * torch.randn(64, generator=g), 1 + 0.1 * torch.randn(64, generator=g)
+    cos, sin = _tables(T, 32, 7)
+    block = fp4.Fp4Block(raw, "blocks.0.", cfg, q_weight=qw.to(d), k_weight=kw.to(d), rope=(cos.to(d), sin.to(d)), fmt=fmt)
+    x = (torch.randn(2 * T, D, generator=g) * 1.5).half()
+    xd = x.to(d)
+    got = block(xd)
+    assert torch.equal(xd.cpu(), x)
+    w = {k[len("blocks.0.") :]: v.double() for k, v in raw.items()}
+    val = lambda t: O.values(*O.quantize(t, fmt), fmt)  # noqa: E731
+    lin = lambda t, n: val(t) @ val(w[n + ".weight"].float()).t() + w[n + ".bias"]  # noqa: E731
+    ln = lambda t, n: O.layer_norm(t, w[n + ".weight"], w[n + ".bias"], cfg.ln_eps)  # noqa: E731
+    f16 = lambda t: t.half().double()  # noqa: E731
+    def heads_of(y):
+        q = O.heads(y[:, :D], H, 64, qw, None, "rms", cfg.ln_eps, cos, sin, "pairs")
+        k = O.heads(y[:, D : 2 * D], H, 64, kw, None, "rms", cfg.ln_eps, cos, sin, "pairs")
+        return torch.cat([q, k, y[:, 2 * D :]], 1)
+
+    def close(name, got, ref):
+        rel = ((got.cpu().double() - ref).norm() / ref.norm()).item()
+        assert rel <= 2e-2, f"{name}: relative error {rel:.3g}"
+
+    act = (lambda u: O.silu_mul(u[:, : cfg.mlp_hidden], u[:, cfg.mlp_hidden :])) if arch == "eva02" else O.gelu_tanh
+    hidden = (lambda t: ln(t, "mlp_norm")) if arch == "eva02" else (lambda t: t)
+    # layer by layer
+    qkv = block.qkv(xd)
+    close("qkv", qkv, heads_of(lin(ln(x, "norm1"), "qkv")))
+    from foidfinder_b200 import ops
+
+    o = torch.empty_like(xd)
+    ops.attention(qkv, o, T, H, scale=0.125)
+    x1 = block.proj(o, residual=xd)
+    close("proj", x1 - xd, lin(o.cpu(), "proj"))
+    h = block.fc1(x1)
+    close("fc1", h, act(lin(ln(x1.cpu(), "norm2"), "fc1")))
+    x2 = block.fc2(h, residual=x1)
+    close("fc2", x2 - x1, lin(hidden(h.cpu()), "fc2"))
+    assert torch.equal(got, x2)
+    # as a whole
+    q, k, v = (f16(t).view(2, T, H, 64).transpose(1, 2) for t in heads_of(lin(ln(x, "norm1"), "qkv")).split(D, 1))
+    o = f16((torch.softmax(q @ k.transpose(-1, -2) / 8, -1) @ v).transpose(1, 2).reshape(2 * T, D))
+    x1 = f16(x.double() + lin(o, "proj"))
+    ref = x1 + lin(hidden(f16(act(lin(ln(x1, "norm2"), "fc1")))), "fc2")
+    close("block", got, ref)
