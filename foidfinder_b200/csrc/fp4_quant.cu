@@ -703,7 +703,7 @@ int quantize_fp4(const void* x, int dtype, int64_t ldx, const float* gamma, cons
                  int cols, int fmt, uint8_t* codes, uint8_t* scales, float* row_scale, cudaStream_t stream) {
   FF_REQUIRE(fmt == FF_FP4_NV || fmt == FF_FP4_MX, "ff_quantize_fp4: unknown format %d", fmt);
   FF_REQUIRE(dtype == FF_F16 || dtype == FF_BF16 || dtype == FF_F32, "ff_quantize_fp4: unknown type %d", dtype);
-  FF_REQUIRE(rows >= 0 && cols >= 1 && cols <= (1 << 24) && ldx >= cols, "ff_quantize_fp4: bad shape [%d, %d], row stride %lld", rows,
+  FF_REQUIRE(rows >= 0 && rows <= (1 << 30) && cols >= 1 && cols <= (1 << 24) && ldx >= cols, "ff_quantize_fp4: bad shape [%d, %d], row stride %lld", rows,
              cols, static_cast<long long>(ldx));
   if (rows == 0) return FF_OK;
   FF_REQUIRE(x && codes && scales, "ff_quantize_fp4: NULL pointer");
@@ -744,7 +744,7 @@ extern "C" int ff_dequantize_fp4(const uint8_t* codes, const uint8_t* scales, co
                                  int fmt, void* out, int dtype, int64_t ldo, void* stream) {
   FF_REQUIRE(fmt == FF_FP4_NV || fmt == FF_FP4_MX, "ff_dequantize_fp4: unknown format %d", fmt);
   FF_REQUIRE(dtype == FF_F16 || dtype == FF_BF16 || dtype == FF_F32, "ff_dequantize_fp4: unknown type %d", dtype);
-  FF_REQUIRE(rows >= 0 && cols >= 1 && cols <= (1 << 24) && ldo >= cols, "ff_dequantize_fp4: bad shape [%d, %d], row stride %lld", rows,
+  FF_REQUIRE(rows >= 0 && rows <= (1 << 30) && cols >= 1 && cols <= (1 << 24) && ldo >= cols, "ff_dequantize_fp4: bad shape [%d, %d], row stride %lld", rows,
              cols, static_cast<long long>(ldo));
   if (rows == 0) return FF_OK;
   FF_REQUIRE(codes && scales && out, "ff_dequantize_fp4: NULL pointer");

@@ -4,15 +4,24 @@
 // they multiply (kind::mxf4nvf4 / kind::mxf4, f32 accumulators in TMEM); the row scales, which are powers of
 // two, and the bias are applied in f32 in the epilogue, which rounds once, to the output's type.
 //
-// One CTA per SM, 640 threads, persistent over tiles:
+// One CTA per SM, 640 threads (384 for EPI_QKV_NORM_ROPE), persistent over tiles:
 //   warp 0     TMA producer: per stage 256 columns (128 bytes of codes, 128-byte swizzle) of A and W rows and
 //              their scale chunks
 //   warp 1     TMEM allocator; copies each stage's scale chunks to TMEM (tcgen05.cp, in order with the MMAs of
 //              the same thread) and issues the MMAs, 64 columns each
-//   warps 4-19 epilogue: two groups, one per accumulator, one output row per lane
+//   warp 2     column scales and biases, four tiles ahead
+//   warps 4-19 epilogue: two groups, one per accumulator, one output row per lane (EPI_QKV_NORM_ROPE: one group,
+//              warps 4-11, for both)
 // Tiles: 128 x 128 per CTA, or (PAIR) 256 x 256 over a cluster of two CTAs, where each CTA loads its 128 rows
 // of A, half of W's 256 rows and all of the tile's W scales (each SM's tensor core reads them from its own
 // TMEM), and shared memory moves half as many bytes per multiply-add.
+//
+// Measured, FF_FP4_NV unless said: 8192^3 190 us (5.8 PFLOP/s, 3.5 times the bf16 rate of the same GPU), bound by the
+// tensor cores. 65600 x 5504 x 1024 with SwiGLU 205 us (3.6 PFLOP/s), where reading the accumulators, activating and
+// storing takes about as long as the products do: 190 us without the column parameters, 183 without the
+// stores, 159 with the MMAs alone. 65600 x 1024 x 2730 with a residual 99 us; 65600 x 1024 x 1024 43 us, bound by the
+// 200 MB moved. 8200 x 2304 x 768 with norm and rotation 29 us, bound by its epilogue. One row of 1024 against 5460: 8 us,
+// the latency of one mainloop and its launch.
 #include "common.h"
 #include "fp4.cuh"
 #include "gemm_fp4.h"
@@ -97,6 +106,14 @@ __device__ __forceinline__ void scale_cols(uint32_t* r, float rs, const float* c
     r[j + 2] = __float_as_uint(hi.x);
     r[j + 3] = __float_as_uint(hi.y);
   }
+}
+// Waits, within the limit, for copies or MMAs in flight, whether or not the kernel is being given up.
+__device__ __forceinline__ bool drain_wait(uint64_t* bar, uint32_t parity) {
+  const uint32_t addr = smem_u32(bar);
+  const unsigned long long t0 = globaltimer();
+  while (!mbar_try_wait(addr, parity))
+    if (globaltimer() - t0 > kWaitLimitNs) return false;
+  return true;
 }
 // Keeps the compiler from starting a later group's loads early: the epilogue has registers for one group.
 __device__ __forceinline__ void group_end() { asm volatile("" ::: "memory"); }
@@ -286,12 +303,7 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR, EPI == EPI_QKV_NORM_ROPE>::THREAD
       if (!ok && leader) {
         // Let every issued copy land before the CTA exits (bounded).
         for (int s = 0; s < STAGES; ++s)
-          if (last_phase[s] >= 0) {
-            const uint32_t addr = smem_u32(&full[s]);
-            const unsigned long long t0 = globaltimer();
-            while (!mbar_try_wait(addr, static_cast<uint32_t>(last_phase[s])) && globaltimer() - t0 < kWaitLimitNs) {
-            }
-          }
+          if (last_phase[s] >= 0) drain_wait(&full[s], static_cast<uint32_t>(last_phase[s]));
       }
     }
   } else if (warp == 1) {
@@ -339,14 +351,7 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR, EPI == EPI_QKV_NORM_ROPE>::THREAD
         tc_commit2(drain);
       else
         tc_commit(drain);
-      const uint32_t addr = smem_u32(drain);
-      const unsigned long long t0 = globaltimer();
-      while (!mbar_try_wait(addr, 0)) {
-        if (globaltimer() - t0 > kWaitLimitNs) {
-          atomicCAS(args.err, 0, kDevTimeoutDrain);
-          break;
-        }
-      }
+      if (!drain_wait(drain, 0)) atomicCAS(args.err, 0, kDevTimeoutDrain);
     }
   } else if (warp == 2) {
     // ------------------------------------------------------------ column scales and biases, up to four tiles ahead
@@ -439,7 +444,7 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR, EPI == EPI_QKV_NORM_ROPE>::THREAD
           ok = wait(&pfull[buf], (i / C::COLP_BUFS) & 1, kDevTimeoutTmemFull) && wait(&tfull[acc], use, kDevTimeoutTmemFull);
           if (!ok) {
             if constexpr (RES) {  // let the residual copy land before the CTA exits
-              if (any) mbar_wait(&resbar[ew], res_phase, abort_flag, args.err, kDevTimeoutDrain);
+              if (any) drain_wait(&resbar[ew], res_phase);
             }
             break;
           }
@@ -476,6 +481,7 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR, EPI == EPI_QKV_NORM_ROPE>::THREAD
           if constexpr (RES) {
             if (any) {
               ok = mbar_wait(&resbar[ew], res_phase, abort_flag, args.err, kDevTimeoutTmaFull);
+              if (!ok) drain_wait(&resbar[ew], res_phase);
               res_phase ^= 1u;
               __syncwarp();
             }
@@ -585,67 +591,67 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR, EPI == EPI_QKV_NORM_ROPE>::THREAD
           }
         } else {
 #pragma unroll 1
-        for (int k = 0; k < 2; ++k) {
-          const int sub = acc == 0 ? 1 - k : k;  // the shared columns first
-          uint32_t r[32];
-          read32(ca + 32 * sub, r);
-          if (k == 0) {
-            arrive_early();
-            wait_residual();
-          } else {
-            arrive_empty();
-          }
-          if (!any) continue;
-          const float *cs = csa + 32 * sub, *bs = ba + 32 * sub;
-          if constexpr (F32OUT) {
-            float* const out = static_cast<float*>(args.out);
-            const int rows = args.M - m_block < 32 ? args.M - m_block : 32;
-            scale_cols<32, MX>(r, rs, cs, bs);
-            stage_row128(stg, lane, r);
-            __syncwarp();
-            const int n = out0 + 32 * sub + lane;
-            for (int k = 0; k < rows; ++k)  // one row of 32 columns per store: any row stride and column count
-              if (n < args.N)
-                out[static_cast<int64_t>(m_block + k) * args.ldo + n] =
-                    *reinterpret_cast<const float*>(stg + k * 128 + (((lane >> 2) ^ (k & 7)) << 4) + (lane & 3) * 4);
-            __syncwarp();
-          } else {
-            // Eight output columns at a time: scale, activate, round, stage.
-            if constexpr (SWIGLU) {  // 16 gates, then their 16 ups
-#pragma unroll
-              for (int g = 0; g < 2; ++g) {
-                scale_cols<8, MX>(r + 8 * g, rs, cs + 8 * g, bs + 8 * g);
-                scale_cols<8, MX>(r + 16 + 8 * g, rs, cs + 16 + 8 * g, bs + 16 + 8 * g);
-                float y[8];
-#pragma unroll
-                for (int j = 0; j < 8; j += 2) {
-                  const uint32_t *gt = r + 8 * g + j, *up = gt + 16;
-                  const float2 h = silu_up2(make_float2(__uint_as_float(gt[0]), __uint_as_float(gt[1])),
-                                            make_float2(__uint_as_float(up[0]), __uint_as_float(up[1])));
-                  y[j] = h.x;
-                  y[j + 1] = h.y;
-                }
-                stage8(2 * sub + g, y);
-              }
+          for (int k = 0; k < 2; ++k) {
+            const int sub = acc == 0 ? 1 - k : k;  // the shared columns first
+            uint32_t r[32];
+            read32(ca + 32 * sub, r);
+            if (k == 0) {
+              arrive_early();
+              wait_residual();
             } else {
+              arrive_empty();
+            }
+            if (!any) continue;
+            const float *cs = csa + 32 * sub, *bs = ba + 32 * sub;
+            if constexpr (F32OUT) {
+              float* const out = static_cast<float*>(args.out);
+              const int rows = args.M - m_block < 32 ? args.M - m_block : 32;
+              scale_cols<32, MX>(r, rs, cs, bs);
+              stage_row128(stg, lane, r);
+              __syncwarp();
+              const int n = out0 + 32 * sub + lane;
+              for (int k = 0; k < rows; ++k)  // one row of 32 columns per store: any row stride and column count
+                if (n < args.N)
+                  out[static_cast<int64_t>(m_block + k) * args.ldo + n] =
+                      *reinterpret_cast<const float*>(stg + k * 128 + (((lane >> 2) ^ (k & 7)) << 4) + (lane & 3) * 4);
+              __syncwarp();
+            } else {
+              // Eight output columns at a time: scale, activate, round, stage.
+              if constexpr (SWIGLU) {  // 16 gates, then their 16 ups
 #pragma unroll
-              for (int g = 0; g < 4; ++g) {
-                scale_cols<8, MX>(r + 8 * g, rs, cs + 8 * g, bs + 8 * g);
-                float y[8];
+                for (int g = 0; g < 2; ++g) {
+                  scale_cols<8, MX>(r + 8 * g, rs, cs + 8 * g, bs + 8 * g);
+                  scale_cols<8, MX>(r + 16 + 8 * g, rs, cs + 16 + 8 * g, bs + 16 + 8 * g);
+                  float y[8];
 #pragma unroll
-                for (int j = 0; j < 8; j += 2) {
-                  float2 v = make_float2(__uint_as_float(r[8 * g + j]), __uint_as_float(r[8 * g + j + 1]));
-                  if constexpr (EPI == EPI_GELU_F16) v = gelu2(v);
-                  y[j] = v.x;
-                  y[j + 1] = v.y;
+                  for (int j = 0; j < 8; j += 2) {
+                    const uint32_t *gt = r + 8 * g + j, *up = gt + 16;
+                    const float2 h = silu_up2(make_float2(__uint_as_float(gt[0]), __uint_as_float(gt[1])),
+                                              make_float2(__uint_as_float(up[0]), __uint_as_float(up[1])));
+                    y[j] = h.x;
+                    y[j + 1] = h.y;
+                  }
+                  stage8(2 * sub + g, y);
                 }
-                stage8(4 * sub + g, y);
+              } else {
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                  scale_cols<8, MX>(r + 8 * g, rs, cs + 8 * g, bs + 8 * g);
+                  float y[8];
+#pragma unroll
+                  for (int j = 0; j < 8; j += 2) {
+                    float2 v = make_float2(__uint_as_float(r[8 * g + j]), __uint_as_float(r[8 * g + j + 1]));
+                    if constexpr (EPI == EPI_GELU_F16) v = gelu2(v);
+                    y[j] = v.x;
+                    y[j + 1] = v.y;
+                  }
+                  stage8(4 * sub + g, y);
+                }
               }
             }
           }
-        }
-        if (!ok) break;
-        if (!any) continue;
+          if (!ok) break;
+          if (!any) continue;
         }
         if constexpr (!F32OUT) {
           fence_async_smem();

@@ -332,6 +332,8 @@ def _matrix(t: torch.Tensor, what: str) -> tuple[int, int, int, int]:
         raise RuntimeError(f"{what}: expected a 2-D CUDA tensor, got {t.dim()}-D on {t.device}")
     rows, cols = t.shape
     ld, step = t.stride()
+    if rows > 1 << 30:
+        raise RuntimeError(f"{what}: at most 2^30 rows, got {rows}")
     if step != 1 and cols > 1:
         raise RuntimeError(f"{what}: expected contiguous columns, got strides {t.stride()}")
     return rows, cols, ld if rows > 1 else max(ld, cols), device

@@ -91,6 +91,15 @@ def test_quantize_host_checks(args, msg):
     assert msg in _err()
 
 
+def test_rows_that_indices_cannot_step_over():
+    rows = (1 << 30) + 1
+    f = _lib.lib()
+    assert f.ff_quantize_fp4(FAKE, 0, 64, None, None, 1e-6, rows, 64, 0, FAKE, FAKE, FAKE, None) == BAD
+    assert f.ff_dequantize_fp4(FAKE, FAKE, FAKE, rows, 64, 0, FAKE, 0, 64, None) == BAD
+    assert f.ff_qk_norm_rope(FAKE, 0, 128, FAKE, 128, rows, 1, 1, 64, 1, FAKE, None, FAKE, None, 1e-6, FAKE, FAKE, 4, 0, None) == BAD
+    assert "bad shape" in _err()
+
+
 def test_quantize_and_dequantize_of_no_rows():
     assert _lib.lib().ff_quantize_fp4(None, 0, 64, None, None, 1e-6, 0, 64, 0, None, None, None, None) == 0
     assert _lib.lib().ff_dequantize_fp4(None, None, None, 0, 64, 0, None, 0, 64, None) == 0
