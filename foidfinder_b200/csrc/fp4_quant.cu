@@ -595,12 +595,77 @@ __device__ __forceinline__ void store_one(T* p, float v) {
     *p = __float2bfloat16_rn(v);
 }
 
-// A lane writes one aligned 16-byte granule of an output row at a time (its columns need not start at a block), so
-// the stores are whole whatever the row's alignment; granules that stick out of the row are written value by value.
-// A warp takes whole rows.
+template <class T>
+__device__ __forceinline__ uint4 pack16(const float* v) {
+  if constexpr (sizeof(T) == 4)
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+  else
+    return make_uint4(Pair16<T>::pack(v[0], v[1]), Pair16<T>::pack(v[2], v[3]), Pair16<T>::pack(v[4], v[5]),
+                      Pair16<T>::pack(v[6], v[7]));
+}
+
+// Outputs whose rows are 16-byte aligned. A warp takes 256 columns, 8 per lane, of rows r, r + 32, r + 64 and r + 96 of a
+// 128-row scale tile: the scales of four blocks of these four rows are 16 neighbouring bytes, so a lane's five loads are
+// one of scales and one of codes per row, all independent.
 template <class T, bool MX>
 __global__ void __launch_bounds__(256)
     dequantize_fp4_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+                          const float* __restrict__ row_scale, int rows, int cols, T* __restrict__ out, int64_t ldo,
+                          int units, int segs) {
+  constexpr int B = MX ? 32 : 16;
+  const int lane = threadIdx.x & 31;
+  pdl_wait();
+  pdl_trigger();
+  const int64_t pitch = fp4_row_bytes(cols), tile = sf_tile_bytes(cols, MX);
+  for (int u = static_cast<int>(blockIdx.x) * 8 + (threadIdx.x >> 5); u < units; u += static_cast<int>(gridDim.x) * 8) {
+    const int quad = u / segs, c = ((u - quad * segs) * 32 + lane) * 8;
+    const int row0 = (quad >> 5) * 128 + (quad & 31), blk = c / B;
+    if (c >= cols) continue;
+    const uint4 sw = __ldg(reinterpret_cast<const uint4*>(scales + (quad >> 5) * tile + static_cast<int64_t>(blk >> 2) * kSfChunk +
+                                                          (quad & 31) * 16));
+    const uint32_t sb[4] = {sw.x, sw.y, sw.z, sw.w};
+    uint32_t w[4];
+    float rs[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int row = row0 + 32 * j;
+      w[j] = row < rows ? __ldg(reinterpret_cast<const uint32_t*>(codes + row * pitch + (c >> 1))) : 0u;
+      rs[j] = MX || row >= rows ? 1.f : __ldg(row_scale + row);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int row = row0 + 32 * j;
+      if (row >= rows) break;
+      const uint32_t byte = (sb[j] >> (8 * (blk & 3))) & 0xffu;
+      const float sc = MX ? e8m0_value(byte) : e4m3_value(byte) * rs[j];
+      uint32_t h[4];
+      e2m1x8_to_half2(w[j], h);
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const float2 f = mul2(unpack_half2(h[e / 2]), make_float2(sc, sc));
+        v[e] = f.x;
+        v[e + 1] = f.y;
+      }
+      T* const o = out + row * ldo + c;
+      if (c + 8 <= cols) {
+        __stcs(reinterpret_cast<uint4*>(o), pack16<T>(v));
+        if constexpr (sizeof(T) == 4) __stcs(reinterpret_cast<uint4*>(o) + 1, pack16<T>(v + 4));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c + e < cols) store_one(o + e, v[e]);
+      }
+    }
+  }
+}
+
+// Any other output. A lane writes one aligned 16-byte granule of a row at a time (its columns need not start at a
+// block); granules that stick out of the row are written value by value. A warp takes whole rows, all loads of four
+// granules first.
+template <class T, bool MX>
+__global__ void __launch_bounds__(256)
+    dequantize_fp4_any_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                           const float* __restrict__ row_scale, int rows, int cols, T* __restrict__ out, int64_t ldo) {
   constexpr int E = 16 / sizeof(T);
   constexpr int B = MX ? 32 : 16;
@@ -619,31 +684,7 @@ __global__ void __launch_bounds__(256)
       const uint32_t byte = __ldg(srow + static_cast<int64_t>(blk >> 2) * kSfChunk + (blk & 3));
       return MX ? e8m0_value(byte) : e4m3_value(byte) * s;
     };
-    auto pack = [&](const float(&v)[8]) {
-      if constexpr (sizeof(T) == 4)
-        return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-      else
-        return make_uint4(Pair16<T>::pack(v[0], v[1]), Pair16<T>::pack(v[2], v[3]), Pair16<T>::pack(v[4], v[5]),
-                          Pair16<T>::pack(v[6], v[7]));
-    };
     int c0 = lane * E - off;  // the granule's first column, may be negative
-    if (off == 0) {  // whole granules of an aligned row lie in one block
-#pragma unroll 4
-      for (; c0 + E <= cols; c0 += 32 * E) {
-        uint32_t h[4];
-        e2m1x8_to_half2(__ldg(crow + (c0 >> 3)) >> (4 * (c0 & 7)), h);
-        const float sc = scale_at(c0 / B);
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < E; e += 2) {
-          const float2 f = mul2(unpack_half2(h[e / 2]), make_float2(sc, sc));
-          v[e] = f.x;
-          v[e + 1] = f.y;
-        }
-        *reinterpret_cast<uint4*>(orow + c0) = pack(v);
-      }
-    }
-    // Any other row, and an aligned row's last granule: all loads of four granules first.
     constexpr int U = 4;
     for (; c0 < cols; c0 += U * 32 * E) {
       uint32_t lo[U], hi[U];
@@ -666,7 +707,7 @@ __global__ void __launch_bounds__(256)
         uint32_t h[4];
         e2m1x8_to_half2(__funnelshift_r(lo[u], hi[u], 4 * (c & 7)), h);
         const int cut = (max(c, 0) / B + 1) * B - c;  // values before the second block
-        float v[8];
+        float v[E];
 #pragma unroll
         for (int e = 0; e < E; e += 2) {
           const float2 f = mul2(unpack_half2(h[e / 2]), make_float2(e >= cut ? sc[u][1] : sc[u][0], e + 1 >= cut ? sc[u][1] : sc[u][0]));
@@ -674,7 +715,7 @@ __global__ void __launch_bounds__(256)
           v[e + 1] = f.y;
         }
         if (c >= 0 && c + E <= cols) {
-          *reinterpret_cast<uint4*>(orow + c) = pack(v);
+          *reinterpret_cast<uint4*>(orow + c) = pack16<T>(v);
         } else {
 #pragma unroll
           for (int e = 0; e < E; ++e)
@@ -685,16 +726,21 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-template <class T>
-int launch_dequant(const uint8_t* codes, const uint8_t* scales, const float* rs, int rows, int cols, bool mx, void* out,
-                   int64_t ldo, cudaStream_t stream) {
-  const int want = (rows + 7) / 8, most = sm_count() * 8;
-  const dim3 grid(want < most ? want : most);
-  if (mx)
-    launch(dequantize_fp4_kernel<T, true>, grid, dim3(256), 0, stream, codes, scales, rs, rows, cols, static_cast<T*>(out), ldo);
-  else
-    launch(dequantize_fp4_kernel<T, false>, grid, dim3(256), 0, stream, codes, scales, rs, rows, cols, static_cast<T*>(out), ldo);
-  return check_launch("dequantize_fp4_kernel");
+template <class T, bool MX>
+int launch_dequant(const uint8_t* codes, const uint8_t* scales, const float* rs, int rows, int cols, void* out, int64_t ldo,
+                   cudaStream_t stream) {
+  T* const o = static_cast<T*>(out);
+  const int most = sm_count() * 8;
+  if (aligned16(out) && (rows == 1 || ldo * static_cast<int64_t>(sizeof(T)) % 16 == 0)) {
+    const int segs = (cols + 255) / 256, units = (rows + 127) / 128 * 32 * segs, want = units / 8;
+    launch(dequantize_fp4_kernel<T, MX>, dim3(want < most ? want : most), dim3(256), 0, stream, codes, scales, rs, rows, cols, o,
+           ldo, units, segs);
+    return check_launch("dequantize_fp4_kernel");
+  }
+  const int want = (rows + 7) / 8;
+  launch(dequantize_fp4_any_kernel<T, MX>, dim3(want < most ? want : most), dim3(256), 0, stream, codes, scales, rs, rows, cols, o,
+         ldo);
+  return check_launch("dequantize_fp4_any_kernel");
 }
 
 }  // namespace
@@ -754,8 +800,14 @@ extern "C" int ff_dequantize_fp4(const uint8_t* codes, const uint8_t* scales, co
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool mx = fmt == FF_FP4_MX;
   switch (dtype) {
-    case FF_F16: return launch_dequant<__half>(codes, scales, row_scale, rows, cols, mx, out, ldo, st);
-    case FF_BF16: return launch_dequant<__nv_bfloat16>(codes, scales, row_scale, rows, cols, mx, out, ldo, st);
-    default: return launch_dequant<float>(codes, scales, row_scale, rows, cols, mx, out, ldo, st);
+    case FF_F16:
+      return mx ? launch_dequant<__half, true>(codes, scales, row_scale, rows, cols, out, ldo, st)
+                : launch_dequant<__half, false>(codes, scales, row_scale, rows, cols, out, ldo, st);
+    case FF_BF16:
+      return mx ? launch_dequant<__nv_bfloat16, true>(codes, scales, row_scale, rows, cols, out, ldo, st)
+                : launch_dequant<__nv_bfloat16, false>(codes, scales, row_scale, rows, cols, out, ldo, st);
+    default:
+      return mx ? launch_dequant<float, true>(codes, scales, row_scale, rows, cols, out, ldo, st)
+                : launch_dequant<float, false>(codes, scales, row_scale, rows, cols, out, ldo, st);
   }
 }
