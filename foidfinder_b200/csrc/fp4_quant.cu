@@ -273,14 +273,14 @@ __device__ __forceinline__ float warp_amax(float v) {
   return r;
 }
 
-// Rows of 16-bit values without a norm, one warp per row: the row stays in registers as loaded (8 words per 16
+// FF_FP4_NV rows of 16-bit values without a norm, one warp per row: the row stays in registers as loaded (8 words per 16
 // values), its maxima are taken on pairs, and it is unpacked once, for the codes. No barriers and few registers:
 // NW pieces of 16 columns per lane, rows of up to 512 * NW columns.
 template <int NW>
 __host__ __device__ constexpr int row_ctas() {  // CTAs of 256 threads per SM that the registers are held to
   return NW <= 3 ? 4 : NW <= 6 ? 3 : 2;
 }
-template <class T, bool MX, bool ALIGNED, bool WHOLE, int NW>
+template <class T, bool ALIGNED, bool WHOLE, int NW>
 __global__ void __launch_bounds__(kQuantThreads, row_ctas<NW>()) quantize_fp4_rows_kernel(const QuantArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   constexpr int WARPS = kQuantThreads / 32;
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(kQuantThreads, row_ctas<NW>()) quantize_fp4_ro
   pdl_trigger();
   for (int row = static_cast<int>(blockIdx.x) * WARPS + warp; row < a.rows; row += static_cast<int>(gridDim.x) * WARPS) {
     const T* xr = static_cast<const T*>(a.x) + row * a.ldx;
-    const RowOut o = row_out<MX>(a, row);
+    const RowOut o = row_out<false>(a, row);
     Raw<T, ALIGNED> raw[NW];
 #pragma unroll
     for (int i = 0; i < NW; ++i) load_raw<T, ALIGNED>(xr, (i * 32 + lane) * 16, a.cols, raw[i]);
@@ -299,28 +299,61 @@ __global__ void __launch_bounds__(kQuantThreads, row_ctas<NW>()) quantize_fp4_ro
       realign<T, ALIGNED, WHOLE>(xr, (i * 32 + lane) * 16, a.cols, raw[i]);
       amax[i] = amax_pairs<T>(raw[i].t);
     }
-    float s = 1.f;
-    bool bad = false;
-    if constexpr (!MX) {
-      float m = amax[0];
+    float m = amax[0];
 #pragma unroll
-      for (int i = 1; i < NW; ++i) m = max_nan(m, amax[i]);
-      m = warp_amax(m);
-      bad = not_finite(m);
-      s = nv_row_scale(bad ? 0.f : m);
-      if (lane == 0) a.row_scale[row] = bad ? __uint_as_float(0x7fffffffu) : s;
-    }
+    for (int i = 1; i < NW; ++i) m = max_nan(m, amax[i]);
+    m = warp_amax(m);
+    const bool bad = not_finite(m);
+    const float s = nv_row_scale(bad ? 0.f : m);
+    if (lane == 0) a.row_scale[row] = bad ? __uint_as_float(0x7fffffffu) : s;
 #pragma unroll
     for (int i = 0; i < NW; ++i) {
       float2 v[8];
       to_f32<T, ALIGNED>(raw[i], v);
       uint2 codes;
-      uint32_t byte;
-      if constexpr (MX)
-        byte = mx_piece(v, max_nan(amax[i], __shfl_xor_sync(0xffffffffu, amax[i], 1)), &codes);
+      const uint32_t byte = nv_piece<kExact16>(v, amax[i], s, bad, &codes);
+      store_piece<false>(o, i * 32 + lane, pieces, codes, byte);
+    }
+  }
+}
+
+// FF_FP4_MX without a norm: blocks stand alone, so a warp takes 32 * NW pieces of a row at a time, of rows of any width.
+template <class T>
+__host__ __device__ constexpr int mx_ctas() {
+  return sizeof(T) == 4 ? 4 : 5;
+}
+template <class T>
+__host__ __device__ constexpr int mx_pieces() {
+  return sizeof(T) == 4 ? 1 : 2;
+}
+template <class T, bool ALIGNED, bool WHOLE>
+__global__ void __launch_bounds__(kQuantThreads, mx_ctas<T>()) quantize_fp4_mx_kernel(const QuantArgs a, const int units, const int segs) {
+  constexpr int NW = mx_pieces<T>();
+  constexpr int WARPS = kQuantThreads / 32;
+  const int lane = threadIdx.x & 31;
+  const int pieces = (a.cols + kFp4Step - 1) / kFp4Step * (kFp4Step / 16);
+  pdl_wait();
+  pdl_trigger();
+  for (int u = static_cast<int>(blockIdx.x) * WARPS + (threadIdx.x >> 5); u < units; u += static_cast<int>(gridDim.x) * WARPS) {
+    const int row = u / segs, c0 = (u - row * segs) * 32 * NW + lane;
+    const T* xr = static_cast<const T*>(a.x) + row * a.ldx;
+    const RowOut o = row_out<true>(a, row);
+    Raw<T, ALIGNED> raw[NW];
+#pragma unroll
+    for (int i = 0; i < NW; ++i) load_raw<T, ALIGNED>(xr, (c0 + 32 * i) * 16, a.cols, raw[i]);
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      realign<T, ALIGNED, WHOLE>(xr, (c0 + 32 * i) * 16, a.cols, raw[i]);
+      float2 v[8];
+      to_f32<T, ALIGNED>(raw[i], v);
+      float amax;
+      if constexpr (sizeof(T) == 2)
+        amax = amax_pairs<T>(raw[i].t);
       else
-        byte = nv_piece<kExact16>(v, amax[i], s, bad, &codes);
-      store_piece<MX>(o, i * 32 + lane, pieces, codes, byte);
+        amax = amax16(v);
+      uint2 codes;
+      const uint32_t byte = mx_piece(v, max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, 1)), &codes);
+      store_piece<true>(o, c0 + 32 * i, pieces, codes, byte);
     }
   }
 }
@@ -510,11 +543,20 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_fp4_wide_kernel(const 
   }
 }
 
-template <class T, bool MX, bool ALIGNED, bool WHOLE, int NW>
+template <class T, bool ALIGNED, bool WHOLE, int NW>
 int launch_rows(const QuantArgs& a, cudaStream_t stream) {
   const int want = (a.rows + kQuantThreads / 32 - 1) / (kQuantThreads / 32), full = row_ctas<NW>() * sm_count();
-  launch(quantize_fp4_rows_kernel<T, MX, ALIGNED, WHOLE, NW>, dim3(want < full ? want : full), dim3(kQuantThreads), 0, stream, a);
+  launch(quantize_fp4_rows_kernel<T, ALIGNED, WHOLE, NW>, dim3(want < full ? want : full), dim3(kQuantThreads), 0, stream, a);
   return check_launch("quantize_fp4_rows_kernel");
+}
+
+template <class T, bool ALIGNED, bool WHOLE>
+int launch_mx(const QuantArgs& a, int cols, cudaStream_t stream) {
+  constexpr int span = 512 * mx_pieces<T>();
+  const int segs = (cols + span - 1) / span, units = a.rows * segs;
+  const int want = (units - 1) / (kQuantThreads / 32) + 1, full = mx_ctas<T>() * sm_count();
+  launch(quantize_fp4_mx_kernel<T, ALIGNED, WHOLE>, dim3(want < full ? want : full), dim3(kQuantThreads), 0, stream, a, units, segs);
+  return check_launch("quantize_fp4_mx_kernel");
 }
 
 template <class T, bool MX, bool NORM, bool ALIGNED, bool WHOLE, int NC, int WPR>
@@ -547,26 +589,29 @@ int launch_joined(const QuantArgs& a, int wpr, cudaStream_t stream) {
 template <class T, bool MX, bool NORM, bool ALIGNED, bool WHOLE>
 int dispatch_quant(const QuantArgs& a, cudaStream_t stream) {
   const int cols = (a.cols + kFp4Step - 1) / kFp4Step * kFp4Step;  // the padded scales are written too
-  if constexpr (sizeof(T) == 2 && !NORM) {
-    if (cols <= 1024) return launch_rows<T, MX, ALIGNED, WHOLE, 2>(a, stream);
-    if (cols <= 1536) return launch_rows<T, MX, ALIGNED, WHOLE, 3>(a, stream);
-    if (cols <= 3 * 1024) return launch_rows<T, MX, ALIGNED, WHOLE, 6>(a, stream);
-    if (cols <= 5 * 1024) return launch_rows<T, MX, ALIGNED, WHOLE, 10>(a, stream);
+  if constexpr (MX && !NORM) return launch_mx<T, ALIGNED, WHOLE>(a, cols, stream);
+  if constexpr (sizeof(T) == 2 && !MX && !NORM) {
+    if (cols <= 1024) return launch_rows<T, ALIGNED, WHOLE, 2>(a, stream);
+    if (cols <= 1536) return launch_rows<T, ALIGNED, WHOLE, 3>(a, stream);
+    if (cols <= 3 * 1024) return launch_rows<T, ALIGNED, WHOLE, 6>(a, stream);
+    if (cols <= 5 * 1024) return launch_rows<T, ALIGNED, WHOLE, 10>(a, stream);
   }
-  const int wpr2 = (cols + 1023) / 1024, wpr3 = (cols + 1535) / 1536;
-  // two or three pieces per lane, whichever leaves fewer lanes idle; three where that is even (fewer warps to join)
-  const bool three = 3 * wpr3 <= 2 * wpr2;
-  const int wpr = three ? wpr3 : wpr2;
-  if constexpr (sizeof(T) == 2 && NORM) {
-    if (wpr == 1)
-      return three ? launch_joined<T, MX, NORM, ALIGNED, WHOLE, 3, 1>(a, wpr, stream)
-                   : launch_joined<T, MX, NORM, ALIGNED, WHOLE, 2, 1>(a, wpr, stream);
-    if (wpr == 2)
-      return three ? launch_joined<T, MX, NORM, ALIGNED, WHOLE, 3, 2>(a, wpr, stream)
-                   : launch_joined<T, MX, NORM, ALIGNED, WHOLE, 2, 2>(a, wpr, stream);
+  if constexpr (!MX || NORM) {
+    const int wpr2 = (cols + 1023) / 1024, wpr3 = (cols + 1535) / 1536;
+    // two or three pieces per lane, whichever leaves fewer lanes idle; three where that is even (fewer warps to join)
+    const bool three = 3 * wpr3 <= 2 * wpr2;
+    const int wpr = three ? wpr3 : wpr2;
+    if constexpr (sizeof(T) == 2 && NORM) {
+      if (wpr == 1)
+        return three ? launch_joined<T, MX, NORM, ALIGNED, WHOLE, 3, 1>(a, wpr, stream)
+                     : launch_joined<T, MX, NORM, ALIGNED, WHOLE, 2, 1>(a, wpr, stream);
+      if (wpr == 2)
+        return three ? launch_joined<T, MX, NORM, ALIGNED, WHOLE, 3, 2>(a, wpr, stream)
+                     : launch_joined<T, MX, NORM, ALIGNED, WHOLE, 2, 2>(a, wpr, stream);
+    }
+    return three ? launch_joined<T, MX, NORM, ALIGNED, WHOLE, 3, 0>(a, wpr, stream)
+                 : launch_joined<T, MX, NORM, ALIGNED, WHOLE, 2, 0>(a, wpr, stream);
   }
-  return three ? launch_joined<T, MX, NORM, ALIGNED, WHOLE, 3, 0>(a, wpr, stream)
-               : launch_joined<T, MX, NORM, ALIGNED, WHOLE, 2, 0>(a, wpr, stream);
 }
 
 template <class T, bool MX, bool NORM>
@@ -604,122 +649,73 @@ __device__ __forceinline__ uint4 pack16(const float* v) {
                       Pair16<T>::pack(v[6], v[7]));
 }
 
-// Outputs whose rows are 16-byte aligned. A warp takes 256 columns, 8 per lane, of rows r, r + 32, r + 64 and r + 96 of a
-// 128-row scale tile: the scales of four blocks of these four rows are 16 neighbouring bytes, so a lane's five loads are
-// one of scales and one of codes per row, all independent.
-template <class T, bool MX>
+// A warp takes 256 columns, 8 per lane, of rows r, r + 32, r + 64 and r + 96 of a 128-row scale tile: the scales of four
+// blocks of these four rows are 16 neighbouring bytes. All loads of a lane are independent of each other.
+// Rows that lie 32 apart are equally far from a 16-byte boundary, whatever the pitch. Rows that do not start on one
+// (!ALIGNED) have their lanes' columns moved down to the boundary before: a lane's columns then lie in two words of
+// codes and up to two blocks. Stores are whole 16-byte granules; those that stick out of the row are written by value.
+template <class T, bool MX, bool ALIGNED>
 __global__ void __launch_bounds__(256)
     dequantize_fp4_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                           const float* __restrict__ row_scale, int rows, int cols, T* __restrict__ out, int64_t ldo,
                           int units, int segs) {
   constexpr int B = MX ? 32 : 16;
+  constexpr int E = 16 / sizeof(T);
   const int lane = threadIdx.x & 31;
   pdl_wait();
   pdl_trigger();
   const int64_t pitch = fp4_row_bytes(cols), tile = sf_tile_bytes(cols, MX);
   for (int u = static_cast<int>(blockIdx.x) * 8 + (threadIdx.x >> 5); u < units; u += static_cast<int>(gridDim.x) * 8) {
-    const int quad = u / segs, c = ((u - quad * segs) * 32 + lane) * 8;
-    const int row0 = (quad >> 5) * 128 + (quad & 31), blk = c / B;
-    if (c >= cols) continue;
-    const uint4 sw = __ldg(reinterpret_cast<const uint4*>(scales + (quad >> 5) * tile + static_cast<int64_t>(blk >> 2) * kSfChunk +
-                                                          (quad & 31) * 16));
-    const uint32_t sb[4] = {sw.x, sw.y, sw.z, sw.w};
-    uint32_t w[4];
+    const int quad = u / segs, row0 = (quad >> 5) * 128 + (quad & 31);
+    const int off = ALIGNED ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(out + row0 * ldo) & 15) / static_cast<int>(sizeof(T));
+    const int c = ((u - quad * segs) * 32 + lane) * 8 - off;  // the lane's first column, may be negative
+    if (row0 >= rows || c >= cols) continue;
+    // the (at most two) blocks that the columns touch
+    const int blk = ALIGNED ? c / B : max(c, 0) / B, blk1 = ALIGNED ? blk : min(c + 7, cols - 1) / B;
+    const uint8_t* const sq = scales + (quad >> 5) * tile + (quad & 31) * 16;
+    const uint4 sw = __ldg(reinterpret_cast<const uint4*>(sq + static_cast<int64_t>(blk >> 2) * kSfChunk));
+    uint4 sw1 = sw;
+    if constexpr (!ALIGNED) sw1 = __ldg(reinterpret_cast<const uint4*>(sq + static_cast<int64_t>(blk1 >> 2) * kSfChunk));
+    const uint32_t sb[4] = {sw.x, sw.y, sw.z, sw.w}, sb1[4] = {sw1.x, sw1.y, sw1.z, sw1.w};
+    uint32_t w[4], w1[4];
     float rs[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int row = row0 + 32 * j;
-      w[j] = row < rows ? __ldg(reinterpret_cast<const uint32_t*>(codes + row * pitch + (c >> 1))) : 0u;
-      rs[j] = MX || row >= rows ? 1.f : __ldg(row_scale + row);
+      const int row = row0 + 32 * j, k = c >> 3;
+      const uint32_t* const p = reinterpret_cast<const uint32_t*>(codes + row * pitch) + k;
+      w[j] = row < rows && (ALIGNED || k >= 0) ? __ldg(p) : 0u;
+      w1[j] = !ALIGNED && row < rows && 8 * (k + 1) < cols ? __ldg(p + 1) : 0u;
+      rs[j] = !MX && row < rows ? __ldg(row_scale + row) : 1.f;
     }
+    const int cut = ALIGNED ? 8 : (blk + 1) * B - c;  // columns of the first block
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int row = row0 + 32 * j;
       if (row >= rows) break;
-      const uint32_t byte = (sb[j] >> (8 * (blk & 3))) & 0xffu;
-      const float sc = MX ? e8m0_value(byte) : e4m3_value(byte) * rs[j];
+      auto scale = [&](uint32_t bytes, int b) {
+        const uint32_t byte = (bytes >> (8 * (b & 3))) & 0xffu;
+        return MX ? e8m0_value(byte) : e4m3_value(byte) * rs[j];
+      };
+      const float sc = scale(sb[j], blk), sc1 = ALIGNED ? sc : scale(sb1[j], blk1);
       uint32_t h[4];
-      e2m1x8_to_half2(w[j], h);
+      e2m1x8_to_half2(ALIGNED ? w[j] : __funnelshift_r(w[j], w1[j], 4 * (c & 7)), h);
       float v[8];
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
-        const float2 f = mul2(unpack_half2(h[e / 2]), make_float2(sc, sc));
+        const float2 f = mul2(unpack_half2(h[e / 2]), make_float2(e < cut ? sc : sc1, e + 1 < cut ? sc : sc1));
         v[e] = f.x;
         v[e + 1] = f.y;
       }
       T* const o = out + row * ldo + c;
-      if (c + 8 <= cols) {
-        __stcs(reinterpret_cast<uint4*>(o), pack16<T>(v));
-        if constexpr (sizeof(T) == 4) __stcs(reinterpret_cast<uint4*>(o) + 1, pack16<T>(v + 4));
-      } else {
+      const bool whole = (ALIGNED || c >= 0) && c + 8 <= cols;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (c + e < cols) store_one(o + e, v[e]);
-      }
-    }
-  }
-}
-
-// Any other output. A lane writes one aligned 16-byte granule of a row at a time (its columns need not start at a
-// block); granules that stick out of the row are written value by value. A warp takes whole rows, all loads of four
-// granules first.
-template <class T, bool MX>
-__global__ void __launch_bounds__(256)
-    dequantize_fp4_any_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                          const float* __restrict__ row_scale, int rows, int cols, T* __restrict__ out, int64_t ldo) {
-  constexpr int E = 16 / sizeof(T);
-  constexpr int B = MX ? 32 : 16;
-  const int lane = threadIdx.x & 31;
-  pdl_wait();
-  pdl_trigger();
-  const int64_t pitch = fp4_row_bytes(cols), tile = sf_tile_bytes(cols, MX);
-  const int words = static_cast<int>(pitch / 4);
-  for (int row = static_cast<int>(blockIdx.x) * 8 + (threadIdx.x >> 5); row < rows; row += static_cast<int>(gridDim.x) * 8) {
-    T* orow = out + row * ldo;
-    const int off = static_cast<int>((reinterpret_cast<uintptr_t>(orow) & 15) / sizeof(T));
-    const uint32_t* crow = reinterpret_cast<const uint32_t*>(codes + row * pitch);
-    const uint8_t* srow = scales + sf_offset(row, 0, tile);
-    const float s = MX ? 1.f : __ldg(row_scale + row);
-    auto scale_at = [&](int blk) {
-      const uint32_t byte = __ldg(srow + static_cast<int64_t>(blk >> 2) * kSfChunk + (blk & 3));
-      return MX ? e8m0_value(byte) : e4m3_value(byte) * s;
-    };
-    int c0 = lane * E - off;  // the granule's first column, may be negative
-    constexpr int U = 4;
-    for (; c0 < cols; c0 += U * 32 * E) {
-      uint32_t lo[U], hi[U];
-      float sc[U][2];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int c = c0 + u * 32 * E;
-        const int w0 = c >> 3;  // codes of columns [c, c + E): one aligned word, or two when the row is not aligned
-        lo[u] = w0 >= 0 && w0 < words ? __ldg(crow + w0) : 0u;
-        hi[u] = w0 + 1 < words ? __ldg(crow + w0 + 1) : 0u;
-        // the (at most two) blocks that the granule touches
-        const int first = min(max(c, 0), cols - 1) / B, last = min(max(c + E - 1, 0), cols - 1) / B;
-        sc[u][0] = scale_at(first);
-        sc[u][1] = scale_at(last);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int c = c0 + u * 32 * E;
-        if (c >= cols || c + E <= 0) continue;
-        uint32_t h[4];
-        e2m1x8_to_half2(__funnelshift_r(lo[u], hi[u], 4 * (c & 7)), h);
-        const int cut = (max(c, 0) / B + 1) * B - c;  // values before the second block
-        float v[E];
-#pragma unroll
-        for (int e = 0; e < E; e += 2) {
-          const float2 f = mul2(unpack_half2(h[e / 2]), make_float2(e >= cut ? sc[u][1] : sc[u][0], e + 1 >= cut ? sc[u][1] : sc[u][0]));
-          v[e] = f.x;
-          v[e + 1] = f.y;
-        }
-        if (c >= 0 && c + E <= cols) {
-          *reinterpret_cast<uint4*>(orow + c) = pack16<T>(v);
+      for (int g = 0; g < 8; g += E) {
+        if (whole || ((ALIGNED || c + g >= 0) && c + g + E <= cols)) {
+          __stcs(reinterpret_cast<uint4*>(o + g), pack16<T>(v + g));
         } else {
 #pragma unroll
-          for (int e = 0; e < E; ++e)
-            if (c + e >= 0 && c + e < cols) store_one(orow + c + e, v[e]);
+          for (int e = g; e < g + E; ++e)
+            if ((ALIGNED || c + e >= 0) && c + e < cols) store_one(o + e, v[e]);
         }
       }
     }
@@ -730,17 +726,15 @@ template <class T, bool MX>
 int launch_dequant(const uint8_t* codes, const uint8_t* scales, const float* rs, int rows, int cols, void* out, int64_t ldo,
                    cudaStream_t stream) {
   T* const o = static_cast<T*>(out);
-  const int most = sm_count() * 8;
-  if (aligned16(out) && (rows == 1 || ldo * static_cast<int64_t>(sizeof(T)) % 16 == 0)) {
-    const int segs = (cols + 255) / 256, units = (rows + 127) / 128 * 32 * segs, want = units / 8;
-    launch(dequantize_fp4_kernel<T, MX>, dim3(want < most ? want : most), dim3(256), 0, stream, codes, scales, rs, rows, cols, o,
-           ldo, units, segs);
-    return check_launch("dequantize_fp4_kernel");
-  }
-  const int want = (rows + 7) / 8;
-  launch(dequantize_fp4_any_kernel<T, MX>, dim3(want < most ? want : most), dim3(256), 0, stream, codes, scales, rs, rows, cols, o,
-         ldo);
-  return check_launch("dequantize_fp4_any_kernel");
+  const bool aligned = aligned16(out) && (rows == 1 || ldo * static_cast<int64_t>(sizeof(T)) % 16 == 0);
+  const int segs = (cols + (aligned ? 0 : 16 / static_cast<int>(sizeof(T)) - 1) + 255) / 256;
+  const int units = (rows + 127) / 128 * 32 * segs, want = units / 8, most = sm_count() * 8;
+  const dim3 grid(want < most ? want : most);
+  if (aligned)
+    launch(dequantize_fp4_kernel<T, MX, true>, grid, dim3(256), 0, stream, codes, scales, rs, rows, cols, o, ldo, units, segs);
+  else
+    launch(dequantize_fp4_kernel<T, MX, false>, grid, dim3(256), 0, stream, codes, scales, rs, rows, cols, o, ldo, units, segs);
+  return check_launch("dequantize_fp4_kernel");
 }
 
 }  // namespace
