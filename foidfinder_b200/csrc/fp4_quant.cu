@@ -19,6 +19,7 @@
 // and 38.0, bound by issue (170 instructions per 16 columns against 107 without; 225 when gamma and beta lay
 // swizzled at computed addresses: 44.7 us). 65600 x 2730 bf16: MX 92 us, LayerNorm and NV 125. Gamma and beta held
 // in registers were slower (73 us at 1024 columns), as was reading a row ahead: they take the registers of the loads.
+#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
@@ -62,17 +63,18 @@ __device__ __forceinline__ void realign(const T* xr, int col, int cols, Raw<T, A
   constexpr int W = Raw<T, ALIGNED>::W;
   if constexpr (!ALIGNED) {
     const uint32_t mis = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(xr)) & 15u;  // the same for all columns
-    if (mis & 8u) {
-#pragma unroll
-      for (int i = 0; i < W + 2; ++i) r.t[i] = r.t[i + 2];
-    }
-    if (mis & 4u) {
-#pragma unroll
-      for (int i = 0; i < W + 1; ++i) r.t[i] = r.t[i + 1];
-    }
     const uint32_t sh = (mis & 2u) * 8u;  // 0 or 16 bits
+    auto shift = [&](auto words) {
+      constexpr int K = decltype(words)::value;
 #pragma unroll
-    for (int i = 0; i < W; ++i) r.t[i] = __funnelshift_r(r.t[i], r.t[i + 1], sh);
+      for (int i = 0; i < W; ++i) r.t[i] = sizeof(T) == 4 ? r.t[i + K] : __funnelshift_r(r.t[i + K], r.t[i + K + 1], sh);
+    };
+    switch (mis >> 2) {  // one move per word, where shifting by 8, 4 and 2 bytes in turn took three
+      case 0: shift(std::integral_constant<int, 0>{}); break;
+      case 1: shift(std::integral_constant<int, 1>{}); break;
+      case 2: shift(std::integral_constant<int, 2>{}); break;
+      default: shift(std::integral_constant<int, 3>{});
+    }
   }
   if (!WHOLE && col + 16 > cols) {
 #pragma unroll
@@ -327,15 +329,15 @@ __host__ __device__ constexpr int mx_pieces() {
   return sizeof(T) == 4 ? 1 : 2;
 }
 template <class T, bool ALIGNED, bool WHOLE>
-__global__ void __launch_bounds__(kQuantThreads, mx_ctas<T>()) quantize_fp4_mx_kernel(const QuantArgs a, const int units, const int segs) {
+__global__ void __launch_bounds__(kQuantThreads, mx_ctas<T>()) quantize_fp4_mx_kernel(const QuantArgs a) {
   constexpr int NW = mx_pieces<T>();
   constexpr int WARPS = kQuantThreads / 32;
   const int lane = threadIdx.x & 31;
   const int pieces = (a.cols + kFp4Step - 1) / kFp4Step * (kFp4Step / 16);
+  const int c0 = static_cast<int>(blockIdx.x) * 32 * NW + lane;
   pdl_wait();
   pdl_trigger();
-  for (int u = static_cast<int>(blockIdx.x) * WARPS + (threadIdx.x >> 5); u < units; u += static_cast<int>(gridDim.x) * WARPS) {
-    const int row = u / segs, c0 = (u - row * segs) * 32 * NW + lane;
+  for (int row = static_cast<int>(blockIdx.y) * WARPS + (threadIdx.x >> 5); row < a.rows; row += static_cast<int>(gridDim.y) * WARPS) {
     const T* xr = static_cast<const T*>(a.x) + row * a.ldx;
     const RowOut o = row_out<true>(a, row);
     Raw<T, ALIGNED> raw[NW];
@@ -543,6 +545,12 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_fp4_wide_kernel(const 
   }
 }
 
+// A CTA per segment of the rows (x) and, up to what the GPU holds, group of rows (y).
+dim3 segment_grid(int segs, int groups, int per_sm) {
+  const int most = std::max(per_sm * sm_count() / segs, 1);
+  return dim3(segs, std::min(groups, most));
+}
+
 template <class T, bool ALIGNED, bool WHOLE, int NW>
 int launch_rows(const QuantArgs& a, cudaStream_t stream) {
   const int want = (a.rows + kQuantThreads / 32 - 1) / (kQuantThreads / 32), full = row_ctas<NW>() * sm_count();
@@ -553,9 +561,8 @@ int launch_rows(const QuantArgs& a, cudaStream_t stream) {
 template <class T, bool ALIGNED, bool WHOLE>
 int launch_mx(const QuantArgs& a, int cols, cudaStream_t stream) {
   constexpr int span = 512 * mx_pieces<T>();
-  const int segs = (cols + span - 1) / span, units = a.rows * segs;
-  const int want = (units - 1) / (kQuantThreads / 32) + 1, full = mx_ctas<T>() * sm_count();
-  launch(quantize_fp4_mx_kernel<T, ALIGNED, WHOLE>, dim3(want < full ? want : full), dim3(kQuantThreads), 0, stream, a, units, segs);
+  const dim3 grid = segment_grid((cols + span - 1) / span, (a.rows - 1) / (kQuantThreads / 32) + 1, mx_ctas<T>());
+  launch(quantize_fp4_mx_kernel<T, ALIGNED, WHOLE>, grid, dim3(kQuantThreads), 0, stream, a);
   return check_launch("quantize_fp4_mx_kernel");
 }
 
@@ -657,18 +664,18 @@ __device__ __forceinline__ uint4 pack16(const float* v) {
 template <class T, bool MX, bool ALIGNED>
 __global__ void __launch_bounds__(256)
     dequantize_fp4_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                          const float* __restrict__ row_scale, int rows, int cols, T* __restrict__ out, int64_t ldo,
-                          int units, int segs) {
+                          const float* __restrict__ row_scale, int rows, int cols, T* __restrict__ out, int64_t ldo) {
   constexpr int B = MX ? 32 : 16;
   constexpr int E = 16 / sizeof(T);
   const int lane = threadIdx.x & 31;
   pdl_wait();
   pdl_trigger();
   const int64_t pitch = fp4_row_bytes(cols), tile = sf_tile_bytes(cols, MX);
-  for (int u = static_cast<int>(blockIdx.x) * 8 + (threadIdx.x >> 5); u < units; u += static_cast<int>(gridDim.x) * 8) {
-    const int quad = u / segs, row0 = (quad >> 5) * 128 + (quad & 31);
+  const int quads = (rows + 127) / 128 * 32;
+  for (int quad = static_cast<int>(blockIdx.y) * 8 + (threadIdx.x >> 5); quad < quads; quad += static_cast<int>(gridDim.y) * 8) {
+    const int row0 = (quad >> 5) * 128 + (quad & 31);
     const int off = ALIGNED ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(out + row0 * ldo) & 15) / static_cast<int>(sizeof(T));
-    const int c = ((u - quad * segs) * 32 + lane) * 8 - off;  // the lane's first column, may be negative
+    const int c = (static_cast<int>(blockIdx.x) * 32 + lane) * 8 - off;  // the lane's first column, may be negative
     if (row0 >= rows || c >= cols) continue;
     // the (at most two) blocks that the columns touch
     const int blk = ALIGNED ? c / B : max(c, 0) / B, blk1 = ALIGNED ? blk : min(c + 7, cols - 1) / B;
@@ -728,12 +735,11 @@ int launch_dequant(const uint8_t* codes, const uint8_t* scales, const float* rs,
   T* const o = static_cast<T*>(out);
   const bool aligned = aligned16(out) && (rows == 1 || ldo * static_cast<int64_t>(sizeof(T)) % 16 == 0);
   const int segs = (cols + (aligned ? 0 : 16 / static_cast<int>(sizeof(T)) - 1) + 255) / 256;
-  const int units = (rows + 127) / 128 * 32 * segs, want = units / 8, most = sm_count() * 8;
-  const dim3 grid(want < most ? want : most);
+  const dim3 grid = segment_grid(segs, (rows + 127) / 128 * 4, 8);
   if (aligned)
-    launch(dequantize_fp4_kernel<T, MX, true>, grid, dim3(256), 0, stream, codes, scales, rs, rows, cols, o, ldo, units, segs);
+    launch(dequantize_fp4_kernel<T, MX, true>, grid, dim3(256), 0, stream, codes, scales, rs, rows, cols, o, ldo);
   else
-    launch(dequantize_fp4_kernel<T, MX, false>, grid, dim3(256), 0, stream, codes, scales, rs, rows, cols, o, ldo, units, segs);
+    launch(dequantize_fp4_kernel<T, MX, false>, grid, dim3(256), 0, stream, codes, scales, rs, rows, cols, o, ldo);
   return check_launch("dequantize_fp4_kernel");
 }
 
