@@ -15,10 +15,14 @@
 // of lanes. Without a norm a warp takes rows of 16-bit values up to 5120 columns wide, packed as loaded; with one,
 // and for f32, a row's values are f32 in as many warps as leave each lane 32 or 48 of them. CTAs are persistent.
 //
-// Measured, 65600 rows of 1024 fp16 (171 MB moved): NV 27.5 us, 95% of the copy rate, MX 26.9; with LayerNorm 38.3
-// and 38.0, bound by issue (170 instructions per 16 columns against 107 without; 225 when gamma and beta lay
-// swizzled at computed addresses: 44.7 us). 65600 x 2730 bf16: MX 92 us, LayerNorm and NV 125. Gamma and beta held
-// in registers were slower (73 us at 1024 columns), as was reading a row ahead: they take the registers of the loads.
+// Measured, 65600 rows of 1024 fp16 (171 MB moved): NV 27.5 us, 95% of the copy rate, MX 26.7. 65600 x 2730 bf16: MX
+// 72 us where rows start at 16-byte boundaries and 84 where they do not (shifting them into place doubles the
+// instructions); NV 73 and 85. With LayerNorm 38 us and 125 (2730): bound by the shared-memory pipe (88% busy at 1024
+// columns), which delivers 8 bytes of gamma and beta per value. What did not help: two rows at a time for the same gamma
+// and beta (38.9 us and 140: half the warps), half a row per warp with two rows (43 and 172: barriers), the next row read
+// ahead into shared memory (50 and 148), 32-byte loads (37.6 and 148), gamma and beta in registers (73).
+// Dequantisation, 65600 x 1024 fp16 30 us (5.7 TB/s); 65600 x 2730 bf16 89 us aligned, 105 not. A kernel that only reads
+// and writes the same bytes takes 33 and 80.
 #include <algorithm>
 #include <type_traits>
 
