@@ -177,6 +177,52 @@ GEMM_SHAPES = [(1, 1, 1), (1, 7, 32), (2, 129, 64), (3, 64, 65), (127, 128, 256)
                (300, 520, 1100), (257, 333, 2730), (515, 384, 1600)]
 
 
+@pytest.mark.parametrize("fmt", ["nv", "mx"])
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize(("cols", "dtype"), [(96, torch.float32), (200, torch.float16), (1301, torch.bfloat16), (2736, torch.float16)])
+def test_rows_do_not_depend_on_each_other(cuda_device, no_device_error, cols, dtype, norm, fmt):
+    """More rows than the GPU holds at once (each warp goes on to further rows), against the same rows a few at a time:
+    equal to the last bit, and so are their values."""
+    from foidfinder_b200 import fp4
+
+    rows = 12345
+    x = _x(rows, cols, dtype, cols).to(cuda_device)
+    kw = dict(gamma=torch.linspace(0.5, 2, cols, device=cuda_device), beta=torch.linspace(-1, 1, cols, device=cuda_device)) if norm else {}
+    q = fp4.quantize(x, fmt, **kw)
+    codes, scales, row = _read(q)
+    v = {t: fp4.dequantize(q, t) for t in (torch.float16, torch.float32)}
+    for first in (0, 127, 5921, rows - 301):
+        part = slice(first, first + 301)
+        p = fp4.quantize(x[part].clone(), fmt, **kw)
+        pc, ps, pr = _read(p)
+        assert torch.equal(pc, codes[part]) and torch.equal(ps, scales[part]) and torch.equal(pr, row[part])
+        for t, a in v.items():
+            assert torch.equal(fp4.dequantize(p, t), a[part])
+
+
+def test_calls_of_no_rows(cuda_device, no_device_error):
+    from foidfinder_b200 import fp4, ops
+
+    d = cuda_device
+    x = torch.empty(0, 64, dtype=torch.float16, device=d)
+    q = fp4.quantize(x)
+    assert fp4.dequantize(q).shape == (0, 64)
+    for epilogue in ("bias", "residual"):
+        layer = fp4.Fp4Linear(torch.ones(64, 64, device=d), epilogue=epilogue)
+        assert layer(x, residual=x if epilogue == "residual" else None).shape == (0, 64)
+    t, w = torch.ones(16, 5, device=d), torch.ones(32, device=d)
+    ops.qk_norm_rope(x, x.clone(), q_heads=1, k_heads=1, head_dim=32, norm="rms", q_weight=w, k_weight=w, rope_cos=t, rope_sin=t)
+
+
+def test_more_rows_than_an_index_holds_are_refused(cuda_device):
+    from foidfinder_b200 import ops
+
+    x = torch.zeros(1, 1, dtype=torch.float16, device=cuda_device).expand((1 << 30) + 1, 1)
+    c = torch.zeros(16, dtype=torch.uint8, device=cuda_device)
+    with pytest.raises(RuntimeError, match="2\\^30 rows"):
+        ops.quantize_fp4(x, c, c, None, ops.FP4_MX)
+
+
 @pytest.mark.parametrize("tile", [128, 512])
 @pytest.mark.parametrize("fmt", ["nv", "mx"])
 @pytest.mark.parametrize(("M", "N", "K"), GEMM_SHAPES)
