@@ -311,12 +311,17 @@ def int8_mma_peak(device: int = 0, iters: int = 200_000) -> float:
 _DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
 _NORMS = {"rms": _lib.NORM_RMS, "layer": _lib.NORM_LAYER}
 _PAIRINGS = {"pairs": _lib.ROPE_PAIRS, "halves": _lib.ROPE_HALVES}
+# torch.cuda's own functions without their device guards and lazy initialisation (a CUDA tensor is at hand), which cost
+# more than what they call
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_alloc = getattr(torch._C, "_cuda_cudaCachingAllocator_raw_alloc", None) or (lambda n, s: torch.cuda.caching_allocator_alloc(n, stream=s))
+_free = getattr(torch._C, "_cuda_cudaCachingAllocator_raw_delete", None) or torch.cuda.caching_allocator_delete
 
 
 def _launch(what: str, fn, device: int, *args) -> None:
     """fn(*args, stream) on the current stream of CUDA device `device`."""
-    if device == torch.cuda.current_device():
+    if device == _current_device():
         rc = fn(*args, _raw_stream(device))
     else:
         with torch.cuda.device(device):
@@ -512,14 +517,25 @@ def linear_fp4(
 def _linear(x, w, fmt, N, K, gamma, beta, eps, epilogue, out, residual) -> None:
     """ff_linear_fp4 with the weight's and the norm's addresses."""
     M, cols, ldx, device = _matrix(x, "linear_fp4")
+    if device != _current_device():
+        with torch.cuda.device(device):
+            return _linear(x, w, fmt, N, K, gamma, beta, eps, epilogue, out, residual)
     dtype = _DTYPES.get(x.dtype)
     if dtype is None or cols != K:
         raise RuntimeError(f"linear_fp4: x must be fp16, bf16 or f32 [M, {K}], got {x.dtype} {list(x.shape)}")
     e = _lib.Fp4Epilogue.from_buffer_copy(epilogue)
     _bind(e, M, N, out, residual, device, "linear_fp4")
     nbytes = _linear_workspace(M, K, fmt)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    _launch("linear_fp4", lib().ff_linear_fp4, device, x.data_ptr(), dtype, ldx, gamma, beta, eps, *w, fmt, M, N, K, C.byref(e), ws.data_ptr(), nbytes)
+    if M == 0:
+        return
+    stream = _raw_stream(device)
+    ws = _alloc(nbytes, stream)  # torch's stream-ordered cache: free for the stream's next use as soon as the call has returned
+    try:
+        rc = lib().ff_linear_fp4(x.data_ptr(), dtype, ldx, gamma, beta, eps, *w, fmt, M, N, K, C.byref(e), ws, nbytes, stream)
+    finally:
+        _free(ws)
+    if rc:
+        check(rc, "linear_fp4")
 
 
 def _linear_workspace(M: int, K: int, fmt: int) -> int:
