@@ -8,9 +8,11 @@
 // are issued before the first is worked on. A CTA takes 8 neighbouring rows, whose angles share cache sectors of the
 // angle-major tables.
 //
-// Measured, 65600 rows of 32 heads of 64 fp16 (537 MB moved): RMS norm 90 us (6.0 TB/s, 91% of the copy rate), LayerNorm
-// 104; 32000 rows of 16 heads of 128, FF_ROPE_HALVES, 93. With a warp per row that ends with it, weights read for every
+// Measured, 65600 rows of 32 heads of 64 fp16 (537 MB moved): RMS norm 91 us (5.9 TB/s, 90% of the copy rate), LayerNorm
+// 97; 32000 rows of 32 heads of 128, FF_ROPE_HALVES, 96. With a warp per row that ends with it, weights read for every
 // row and fewer loads in flight, 101 and 114.
+#include <algorithm>
+
 #include "common.h"
 #include "fp4.cuh"
 
@@ -20,6 +22,7 @@ namespace {
 
 constexpr int kQkWarps = 8;
 constexpr int kQkCtas = 3;  // per SM
+constexpr int kQkSteps = 4;  // of 256 columns, whose loads are issued together
 
 struct QkArgs {
   const void* x;
@@ -33,12 +36,12 @@ struct QkArgs {
   int tokens;
 };
 
-template <class T, int D, bool LAYER, bool HALVES>
+template <class T, int D, bool LAYER, bool HALVES, bool SHARED>
 __global__ void __launch_bounds__(32 * kQkWarps, kQkCtas) qk_norm_rope_kernel(const QkArgs a) {
   constexpr int G = D / 8;       // lanes per head
   constexpr int HPW = 32 / G;    // heads per warp and step
   constexpr int NA = HALVES ? 8 : 4;  // angles per lane
-  constexpr int U = 4;           // steps whose loads are issued together
+  constexpr int U = kQkSteps;
   const int lane = threadIdx.x & 31, l = lane % G, hl = lane / G;
   pdl_wait();
   pdl_trigger();
@@ -52,6 +55,11 @@ __global__ void __launch_bounds__(32 * kQkWarps, kQkCtas) qk_norm_rope_kernel(co
       bk[i] = a.k_b != nullptr ? __ldg(a.k_b + l * 8 + i) : 0.f;
     }
   }
+  // A row's heads in chunks of CH, q then k. SHARED: several warps (blockIdx.y) take turns with them.
+  constexpr int CH = U * HPW;
+  const int warps = SHARED ? gridDim.y : 1, turn = SHARED ? blockIdx.y : 0;
+  const int stride = warps * CH, q_first = turn * CH;
+  const int k_first = (turn + warps - (a.q_heads + CH - 1) / CH % warps) % warps * CH;
   const int step = static_cast<int>(gridDim.x) * kQkWarps;
   for (int row = static_cast<int>(blockIdx.x) * kQkWarps + (threadIdx.x >> 5); row < a.rows; row += step) {
     const int pos = row % a.tokens;
@@ -62,92 +70,97 @@ __global__ void __launch_bounds__(32 * kQkWarps, kQkCtas) qk_norm_rope_kernel(co
       c[i] = __ldg(a.cos + static_cast<int64_t>(j) * a.tokens + pos);
       s[i] = __ldg(a.sin + static_cast<int64_t>(j) * a.tokens + pos);
     }
-    // The heads of one kind (q or k), which start at column `col` of the row.
+    // The first CH of `count` heads of one kind (q or k), which start at column `col` of the row.
     auto heads = [&](int64_t col, int count, const float(&w)[8], const float(&b)[LAYER ? 8 : 1]) {
       const T* const xr = static_cast<const T*>(a.x) + row * a.ldx + col + l * 8;
       T* const orow = static_cast<T*>(a.out) + row * a.ldo + col + l * 8;
-      for (int h0 = hl; h0 - hl < count; h0 += U * HPW) {
-        uint4 u[U];
+      uint4 u[U];
 #pragma unroll
-        for (int k = 0; k < U; ++k)
-          u[k] = h0 + k * HPW < count ? *reinterpret_cast<const uint4*>(xr + (h0 + k * HPW) * D) : make_uint4(0, 0, 0, 0);
+      for (int k = 0; k < U; ++k)
+        u[k] = hl + k * HPW < count ? *reinterpret_cast<const uint4*>(xr + (hl + k * HPW) * D) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int k = 0; k < U; ++k) {
-          if (h0 - hl + k * HPW >= count) break;  // the whole warp
-          float2 y[4] = {Pair16<T>::unpack(u[k].x), Pair16<T>::unpack(u[k].y), Pair16<T>::unpack(u[k].z),
-                         Pair16<T>::unpack(u[k].w)};
-          if constexpr (LAYER) {
-            const float2 t = add2(add2(y[0], y[1]), add2(y[2], y[3]));
-            float m = t.x + t.y;
+      for (int k = 0; k < U; ++k) {
+        if (k * HPW >= count) break;  // the whole warp
+        float2 y[4] = {Pair16<T>::unpack(u[k].x), Pair16<T>::unpack(u[k].y), Pair16<T>::unpack(u[k].z),
+                       Pair16<T>::unpack(u[k].w)};
+        if constexpr (LAYER) {
+          const float2 t = add2(add2(y[0], y[1]), add2(y[2], y[3]));
+          float m = t.x + t.y;
 #pragma unroll
-            for (int o = G / 2; o; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
-            m *= -1.f / D;
+          for (int o = G / 2; o; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
+          m *= -1.f / D;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = add2(y[i], make_float2(m, m));
-          }
-          float2 q = mul2(y[0], y[0]);
+          for (int i = 0; i < 4; ++i) y[i] = add2(y[i], make_float2(m, m));
+        }
+        float2 q = mul2(y[0], y[0]);
 #pragma unroll
-          for (int i = 1; i < 4; ++i) q = fma2(y[i], y[i], q);
-          float ss = q.x + q.y;
+        for (int i = 1; i < 4; ++i) q = fma2(y[i], y[i], q);
+        float ss = q.x + q.y;
 #pragma unroll
-          for (int o = G / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-          const float rstd = rsqrtf(ss * (1.f / D) + a.eps);
+        for (int o = G / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float rstd = rsqrtf(ss * (1.f / D) + a.eps);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 wr = mul2(make_float2(rstd, rstd), make_float2(w[2 * i], w[2 * i + 1]));
+          if constexpr (LAYER)
+            y[i] = fma2(y[i], wr, make_float2(b[2 * i], b[2 * i + 1]));
+          else
+            y[i] = mul2(y[i], wr);
+        }
+        if constexpr (HALVES) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float2 wr = mul2(make_float2(rstd, rstd), make_float2(w[2 * i], w[2 * i + 1]));
-            if constexpr (LAYER)
-              y[i] = fma2(y[i], wr, make_float2(b[2 * i], b[2 * i + 1]));
-            else
-              y[i] = mul2(y[i], wr);
+            const float2 other = make_float2(__shfl_xor_sync(0xffffffffu, y[i].x, G / 2),
+                                             __shfl_xor_sync(0xffffffffu, y[i].y, G / 2));
+            const float sx = l < G / 2 ? -s[2 * i] : s[2 * i], sy = l < G / 2 ? -s[2 * i + 1] : s[2 * i + 1];
+            y[i] = make_float2(y[i].x * c[2 * i] + other.x * sx, y[i].y * c[2 * i + 1] + other.y * sy);
           }
-          if constexpr (HALVES) {
+        } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float2 other = make_float2(__shfl_xor_sync(0xffffffffu, y[i].x, G / 2),
-                                               __shfl_xor_sync(0xffffffffu, y[i].y, G / 2));
-              const float sx = l < G / 2 ? -s[2 * i] : s[2 * i], sy = l < G / 2 ? -s[2 * i + 1] : s[2 * i + 1];
-              y[i] = make_float2(y[i].x * c[2 * i] + other.x * sx, y[i].y * c[2 * i + 1] + other.y * sy);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = make_float2(y[i].x * c[i] - y[i].y * s[i], y[i].x * s[i] + y[i].y * c[i]);
-          }
-          if (h0 + k * HPW < count)
-            *reinterpret_cast<uint4*>(orow + (h0 + k * HPW) * D) =
-                make_uint4(Pair16<T>::pack(y[0].x, y[0].y), Pair16<T>::pack(y[1].x, y[1].y),
-                           Pair16<T>::pack(y[2].x, y[2].y), Pair16<T>::pack(y[3].x, y[3].y));
+          for (int i = 0; i < 4; ++i) y[i] = make_float2(y[i].x * c[i] - y[i].y * s[i], y[i].x * s[i] + y[i].y * c[i]);
         }
+        if (hl + k * HPW < count)
+          *reinterpret_cast<uint4*>(orow + (hl + k * HPW) * D) =
+              make_uint4(Pair16<T>::pack(y[0].x, y[0].y), Pair16<T>::pack(y[1].x, y[1].y),
+                         Pair16<T>::pack(y[2].x, y[2].y), Pair16<T>::pack(y[3].x, y[3].y));
       }
     };
-    heads(0, a.q_heads, wq, bq);
-    heads(static_cast<int64_t>(a.q_heads) * D, a.k_heads, wk, bk);
+    for (int h = q_first; h < a.q_heads; h += stride) heads(static_cast<int64_t>(h) * D, a.q_heads - h, wq, bq);
+    for (int h = k_first; h < a.k_heads; h += stride) heads((static_cast<int64_t>(a.q_heads) + h) * D, a.k_heads - h, wk, bk);
   }
 }
 
-template <class T, int D>
-void launch_qk(const QkArgs& a, int norm, int pairing, cudaStream_t s) {
+template <class T, int D, bool LAYER, bool HALVES>
+void launch_qk(const QkArgs& a, cudaStream_t s) {
   const int want = (a.rows + kQkWarps - 1) / kQkWarps, most = sm_count() * kQkCtas;
-  const dim3 grid(want < most ? want : most), block(32 * kQkWarps);
-  if (norm == FF_NORM_LAYER) {
-    if (pairing == FF_ROPE_HALVES)
-      launch(qk_norm_rope_kernel<T, D, true, true>, grid, block, 0, s, a);
-    else
-      launch(qk_norm_rope_kernel<T, D, true, false>, grid, block, 0, s, a);
-  } else {
-    if (pairing == FF_ROPE_HALVES)
-      launch(qk_norm_rope_kernel<T, D, false, true>, grid, block, 0, s, a);
-    else
-      launch(qk_norm_rope_kernel<T, D, false, false>, grid, block, 0, s, a);
-  }
+  constexpr int CH = kQkSteps * 256 / D;
+  const int chunks = (a.q_heads + CH - 1) / CH + (a.k_heads + CH - 1) / CH;
+  // Fewer rows than four rounds of the GPU's warps: several warps per row, down to the heads that a warp works on at once
+  // (50 rows of 64 heads of 128: 12.8 us with one warp per row, 3.3 so).
+  const int share = std::min(chunks, 4 * most / want);
+  const dim3 block(32 * kQkWarps);
+  if (share > 1)
+    launch(qk_norm_rope_kernel<T, D, LAYER, HALVES, true>, dim3(want, share), block, 0, s, a);
+  else
+    launch(qk_norm_rope_kernel<T, D, LAYER, HALVES, false>, dim3(std::min(want, most)), block, 0, s, a);
+}
+
+template <class T, int D>
+void launch_qk_norm(const QkArgs& a, int norm, int pairing, cudaStream_t s) {
+  const bool halves = pairing == FF_ROPE_HALVES;
+  if (norm == FF_NORM_LAYER)
+    halves ? launch_qk<T, D, true, true>(a, s) : launch_qk<T, D, true, false>(a, s);
+  else
+    halves ? launch_qk<T, D, false, true>(a, s) : launch_qk<T, D, false, false>(a, s);
 }
 
 template <class T>
 void launch_qk_dim(const QkArgs& a, int dim, int norm, int pairing, cudaStream_t s) {
   switch (dim) {
-    case 32: return launch_qk<T, 32>(a, norm, pairing, s);
-    case 64: return launch_qk<T, 64>(a, norm, pairing, s);
-    case 128: return launch_qk<T, 128>(a, norm, pairing, s);
-    default: return launch_qk<T, 256>(a, norm, pairing, s);
+    case 32: return launch_qk_norm<T, 32>(a, norm, pairing, s);
+    case 64: return launch_qk_norm<T, 64>(a, norm, pairing, s);
+    case 128: return launch_qk_norm<T, 128>(a, norm, pairing, s);
+    default: return launch_qk_norm<T, 256>(a, norm, pairing, s);
   }
 }
 
