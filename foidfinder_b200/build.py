@@ -6,6 +6,9 @@ Same role as the reference's loader/build step (foidfinder/backends/cuda/kernels
 declared in `include/foidfinder_b200.h`. The CUDA runtime is linked statically, so the library needs
 only the driver at run time.
 
+`csrc/calls.cpp`, the short way from torch tensors into the calls that are made once per layer, becomes the extension
+module `foidfinder_b200._calls` (host code only, g++ against torch's headers).
+
     python -m foidfinder_b200.build [--force] [--jobs N]
 """
 
@@ -17,6 +20,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -26,6 +30,7 @@ INCLUDE = ROOT / "include"
 BUILD = ROOT / "_build"
 LIB_DIR = PKG / "_lib"
 LIB = LIB_DIR / "libfoidfinder_b200.so"
+CALLS = PKG / ("_calls" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", f"-I{INCLUDE}"]
@@ -82,7 +87,28 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         os.replace(tmp, LIB)
+    build_calls(force)
     return LIB
+
+
+def build_calls(force: bool = False) -> Path:
+    """The extension module of csrc/calls.cpp; returns its path."""
+    src = CSRC / "calls.cpp"
+    if force or _stale(CALLS, [src, *INCLUDE.glob("*.h")]):
+        from torch.utils import cpp_extension as torch_paths
+
+        cxx = shutil.which("g++") or shutil.which("c++")
+        if cxx is None:
+            raise RuntimeError("no C++ compiler found for foidfinder_b200/csrc/calls.cpp")
+        include = [f"-I{p}" for p in (*torch_paths.include_paths("cuda"), sysconfig.get_paths()["include"], INCLUDE)]
+        libs = [*(f"-L{p}" for p in torch_paths.library_paths("cuda")), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+        tmp = CALLS.with_name(CALLS.name + ".tmp")
+        cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", *include, str(src), "-o", str(tmp), *libs]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"{cxx} failed on {src.name}:\n{r.stdout}\n{r.stderr}")
+        os.replace(tmp, CALLS)
+    return CALLS
 
 
 def main() -> None:

@@ -1,12 +1,14 @@
 """Per-kernel entry points on torch CUDA tensors, mirroring the reference's `torch.ops.foidfinder` ops
 (foidfinder/backends/cuda/csrc/kernels.cu:267-281): outputs are caller-allocated and written in place,
 shape/dtype violations raise, and every launch goes on the current CUDA stream. Each call goes through
-the C ABI of `libfoidfinder_b200.so`; torch is only the memory and stream plumbing.
+the C ABI of `libfoidfinder_b200.so`; torch is only the memory and stream plumbing. Calls made once per layer
+take a short way to it (csrc/calls.cpp) where their arguments are plain.
 """
 
 from __future__ import annotations
 
 import ctypes as C
+from functools import cache
 
 import torch
 
@@ -319,6 +321,25 @@ _alloc = getattr(torch._C, "_cuda_cudaCachingAllocator_raw_alloc", None) or (lam
 _free = getattr(torch._C, "_cuda_cudaCachingAllocator_raw_delete", None) or torch.cuda.caching_allocator_delete
 
 
+class _NoCalls:
+    """In the place of the extension module where it has not been built: every call goes the long way."""
+
+    quantize = dequantize = linear = qk_norm_rope = staticmethod(lambda *args: None)
+
+
+@cache
+def _calls():
+    """The extension module of csrc/calls.cpp, bound to the kernels' library."""
+    try:
+        from . import _calls as module
+    except ImportError:
+        return _NoCalls
+    h = lib()
+    names = ("ff_quantize_fp4", "ff_dequantize_fp4", "ff_linear_fp4_workspace_bytes", "ff_linear_fp4", "ff_qk_norm_rope")
+    module.bind(*(C.cast(getattr(h, name), C.c_void_p).value for name in names))
+    return module
+
+
 def _launch(what: str, fn, device: int, *args) -> None:
     """fn(*args, stream) on the current stream of CUDA device `device`."""
     if device == _current_device():
@@ -385,6 +406,9 @@ def quantize_fp4(
 ) -> None:
     """x [T, C] fp16, bf16 or f32 (columns contiguous, any row stride) -> (LayerNorm) -> 4-bit codes and block scales
     (`fp4_sizes` bytes) and, for FP4_NV, row_scale [T] f32."""
+    rc = _calls().quantize(x, codes, scales, row_scale, fmt, gamma, beta, eps)
+    if rc is not None:
+        return check(rc, "quantize_fp4") if rc else None
     T, cols, ldx, device = _matrix(x, "quantize_fp4")
     dtype = _DTYPES.get(x.dtype)
     _need(dtype is not None, "quantize_fp4: x must be fp16, bf16 or f32")
@@ -395,6 +419,9 @@ def quantize_fp4(
 
 def dequantize_fp4(codes: torch.Tensor, scales: torch.Tensor, row_scale: torch.Tensor | None, out: torch.Tensor, fmt: int) -> None:
     """The values of a 4-bit operand into out [T, C] (fp16, bf16 or f32; columns contiguous, any row stride)."""
+    rc = _calls().dequantize(codes, scales, row_scale, out, fmt)
+    if rc is not None:
+        return check(rc, "dequantize_fp4") if rc else None
     T, cols, ldo, device = _matrix(out, "dequantize_fp4")
     dtype = _DTYPES.get(out.dtype)
     _need(dtype is not None, "dequantize_fp4: out must be fp16, bf16 or f32")
@@ -516,6 +543,9 @@ def linear_fp4(
 
 def _linear(x, w, fmt, N, K, gamma, beta, eps, epilogue, out, residual) -> None:
     """ff_linear_fp4 with the weight's and the norm's addresses."""
+    rc = _calls().linear(x, w, fmt, N, K, gamma, beta, eps, epilogue, out, residual)
+    if rc is not None:
+        return check(rc, "linear_fp4") if rc else None
     M, cols, ldx, device = _matrix(x, "linear_fp4")
     if device != _current_device():
         with torch.cuda.device(device):
@@ -564,6 +594,10 @@ def qk_norm_rope(
     """x [T, >= (q_heads + k_heads) * head_dim] fp16 or bf16, q heads then k heads -> every head normalised ("rms" or
     "layer") and rotated by position row % tokens, into the first columns of out (x itself: in place). Tables are
     angle-major [head_dim / 2, tokens] f32; `pairing` "pairs" rotates (2i, 2i + 1), "halves" (i, i + head_dim / 2)."""
+    n, p = _NORMS.get(norm), _PAIRINGS.get(pairing)
+    rc = _calls().qk_norm_rope(x, out, q_heads, k_heads, head_dim, n, q_weight, q_bias, k_weight, k_bias, eps, rope_cos, rope_sin, p)
+    if rc is not None:
+        return check(rc, "qk_norm_rope") if rc else None
     rows, xcols, ldx, device = _matrix(x, "qk_norm_rope")
     orows, ocols, ldo, odevice = _matrix(out, "qk_norm_rope")
     cols, dtype = (q_heads + k_heads) * head_dim, x.dtype
@@ -571,7 +605,6 @@ def qk_norm_rope(
         raise RuntimeError(f"qk_norm_rope: x and out must be fp16 or bf16, alike, got {dtype} and {out.dtype}")
     if xcols < cols or ocols < cols or orows != rows or odevice != device:
         raise RuntimeError(f"qk_norm_rope: x {list(x.shape)} and out {list(out.shape)} must hold {cols} columns of the same rows on one device")
-    n, p = _NORMS.get(norm), _PAIRINGS.get(pairing)
     _need(n is not None and p is not None, "qk_norm_rope: norm is 'rms' or 'layer', pairing 'pairs' or 'halves'")
     what = "qk_norm_rope"
     qw, qb = _vector(q_weight, head_dim, device, what), _vector(q_bias, head_dim, device, what)

@@ -219,3 +219,15 @@ def test_interleave_groups_gates_and_ups():
         assert torch.equal(t[32 * i + 16 : 32 * i + 32, 0], w[100 + 16 * i : 100 + 16 * i + 16, 0])
     assert torch.equal(t[192:196, 0], w[96:100, 0]) and (t[196:208] == 0).all()
     assert torch.equal(t[208:212, 0], w[196:200, 0]) and (t[212:] == 0).all()
+
+
+def test_the_extension_module_leaves_cpu_tensors_alone():
+    c = ops._calls()
+    assert c is not ops._NoCalls, "build it with python -m foidfinder_b200.build"
+    x, b, f = torch.zeros(2, 32), torch.zeros(64, dtype=torch.uint8), torch.zeros(2)
+    assert c.quantize(x, b, b, f, 0, None, None, 1e-6) is None
+    assert c.dequantize(b, b, f, x, 0) is None
+    assert c.linear(x, (1, 2, 3), 0, 32, 32, None, None, 1e-6, _lib.Fp4Epilogue(), x, None) is None
+    assert c.qk_norm_rope(x, x, 1, 0, 32, 1, f, None, f, None, 1e-6, f, f, 0) is None
+    with pytest.raises(TypeError):
+        c.bind(1, 2)

@@ -200,6 +200,57 @@ def test_rows_do_not_depend_on_each_other(cuda_device, no_device_error, cols, dt
             assert torch.equal(fp4.dequantize(p, t), a[part])
 
 
+@pytest.mark.parametrize("fmt", ["nv", "mx"])
+def test_the_short_and_the_long_way_into_a_call_agree(cuda_device, no_device_error, monkeypatch, fmt):
+    """The extension module takes plain calls (it must be there); what it leaves to Python gives the same."""
+    from foidfinder_b200 import fp4, ops
+
+    d = cuda_device
+    assert ops._calls() is not ops._NoCalls
+    x = _x(70, 200, torch.float16, 1).to(d)
+    g = torch.linspace(0.5, 1.5, 200, device=d)
+    t, hw = torch.linspace(0, 1, 16 * 7, device=d).view(16, 7), torch.ones(32, device=d)
+    layer = fp4.Fp4Linear(_x(200, 200, torch.float32, 2).to(d), g, fmt=fmt, epilogue="residual", gamma=g, beta=g)
+
+    def everything():
+        q = fp4.quantize(x, fmt, gamma=g, beta=g)
+        h = torch.zeros(70, 200, device=d, dtype=torch.float16)
+        ops.qk_norm_rope(x, h, q_heads=4, k_heads=2, head_dim=32, norm="layer", q_weight=hw, k_weight=hw, k_bias=hw, rope_cos=t, rope_sin=t, pairing="halves")
+        return [*_read(q), fp4.dequantize(q, torch.float32), layer(x, residual=x), h]
+
+    def taken(*args):
+        r = real(*args)
+        assert r == 0
+        return r
+
+    short = ops._calls()
+    for name in ("quantize", "dequantize", "linear", "qk_norm_rope"):
+        real = getattr(short, name)
+        with monkeypatch.context() as m:
+            m.setattr(short, name, taken)
+            a = everything()
+    monkeypatch.setattr(ops, "_calls", lambda: ops._NoCalls)
+    for u, v in zip(a, everything()):
+        assert torch.equal(u, v)
+
+
+def test_what_the_short_way_leaves(cuda_device, monkeypatch):
+    from foidfinder_b200 import fp4, ops
+
+    c = ops._calls()
+    d = cuda_device
+    x = torch.zeros(4, 64, dtype=torch.float16, device=d)
+    q = fp4.Fp4Tensor.empty(4, 64, "nv")
+    args = [x, q.codes, q.scales, q.row_scale, 0, None, None, 1e-6]
+    assert c.quantize(*args) == 0
+    for i, bad in ((0, x.cpu()), (0, x.t()), (0, x[0]), (0, x.int()), (0, x.cpu().numpy()), (1, q.codes[:8]), (1, q.codes.float()), (2, None), (3, None),
+                   (3, q.row_scale.half()), (4, "nv"), (4, 1 << 40), (5, x), (7, 1)):
+        assert c.quantize(*args[:i], bad, *args[i + 1 :]) is None, (i, bad)
+    assert c.quantize(*args[:-1]) is None
+    with pytest.raises(RuntimeError, match="unknown format"):  # the library's own check
+        ops.quantize_fp4(x, q.codes, q.scales, q.row_scale, 7)
+
+
 def test_calls_of_no_rows(cuda_device, no_device_error):
     from foidfinder_b200 import fp4, ops
 
