@@ -4,14 +4,13 @@
 // they multiply (kind::mxf4nvf4 / kind::mxf4, f32 accumulators in TMEM); the row scales, which are powers of
 // two, and the bias are applied in f32 in the epilogue, which rounds once, to the output's type.
 //
-// One CTA per SM, 640 threads (384 for EPI_QKV_NORM_ROPE), persistent over tiles:
+// One CTA per SM, 640 threads, persistent over tiles:
 //   warp 0     TMA producer: per stage 256 columns (128 bytes of codes, 128-byte swizzle) of A and W rows and
 //              their scale chunks
 //   warp 1     TMEM allocator; copies each stage's scale chunks to TMEM (tcgen05.cp, in order with the MMAs of
 //              the same thread) and issues the MMAs, 64 columns each
 //   warp 2     column scales and biases, four tiles ahead
-//   warps 4-19 epilogue: two groups, one per accumulator, one output row per lane (EPI_QKV_NORM_ROPE: one group,
-//              warps 4-11, for both)
+//   warps 4-19 epilogue: two groups, one per accumulator, one output row per lane
 // Tiles: 128 x 128 per CTA, or (PAIR) 256 x 256 over a cluster of two CTAs, where each CTA loads its 128 rows
 // of A, half of W's 256 rows and all of the tile's W scales (each SM's tensor core reads them from its own
 // TMEM), and shared memory moves half as many bytes per multiply-add.
@@ -20,7 +19,7 @@
 // tensor cores. 65600 x 5504 x 1024 with SwiGLU 209 us (3.5 PFLOP/s), where reading the accumulators, activating and
 // storing takes about as long as the products do: 190 us without the column parameters, 183 without the
 // stores, 159 with the MMAs alone. 65600 x 1024 x 2730 with a residual 100 us; 65600 x 1024 x 1024 44 us, bound by the
-// 200 MB moved. 8200 x 2304 x 768 with norm and rotation 29 us, bound by its epilogue. One row of 1024 against 5460: 8 us,
+// 200 MB moved. 8200 x 2304 x 768 with norm and rotation 26.5 us, bound by its epilogue (21 without the angles). One row of 1024 against 5460: 8 us,
 // the latency of one mainloop and its launch.
 #include "common.h"
 #include "fp4.cuh"
@@ -40,12 +39,9 @@ struct Fp4Cfg {
   static constexpr int SFA_BYTES = 4 * kSfChunk;
   static constexpr int SFB_BYTES = (BN / 128) * 4 * kSfChunk;
   static constexpr int STAGE_BYTES = 2 * CODE_BYTES + SFA_BYTES + SFB_BYTES;
-  // EPI_QKV_NORM_ROPE: three stages leave the L1 cache room for a row block's rotation angles (32 KB)
-  static constexpr int STAGES = QKV ? 3 : 4;
+  static constexpr int STAGES = 4;
   static constexpr int GROUP_WARPS = 8;  // epilogue warps that work on one accumulator
-  // Two groups take turns with the tiles; EPI_QKV_NORM_ROPE has one, whose lanes then have registers for a whole head
-  // (168 instead of 96).
-  static constexpr int GROUPS = QKV ? 1 : 2;
+  static constexpr int GROUPS = 2;       // take turns with the tiles
   static constexpr int THREADS = 128 + GROUPS * 32 * GROUP_WARPS;
   static constexpr int STAGING = 4096;      // per epilogue warp: 32 rows x 128 B
   static constexpr int COLP = 2 * BN * 4;   // column scales and biases of a tile
@@ -382,7 +378,7 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR, EPI == EPI_QKV_NORM_ROPE>::THREAD
     // mainloops for a tile. A warp reads one lane quarter (32 rows) and half of the tile's columns, 32 at a time.
     pdl_wait();
     const int ew = warp - 4;
-    const int group = ew >> 3;       // with two groups, also the accumulator that it works on
+    const int group = ew >> 3;       // also the accumulator that it works on
     const int q = warp & 3;          // TMEM lane quarter
     const int half = (ew >> 2) & 1;  // of the tile's columns
     uint8_t* const stg = staging + ew * C::STAGING;
@@ -407,7 +403,7 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR, EPI == EPI_QKV_NORM_ROPE>::THREAD
     };
     float rs_next = row_scale_of(group);
     for (int i = group; i < my_tiles; i += C::GROUPS) {
-      const int acc = C::GROUPS == 2 ? group : i & 1;
+      const int acc = group;
       const uint32_t use = (i >> 1) & 1;
       const int t = t_first + i * t_step;
       const int tm = t / tiles_n, tn = t - tm * tiles_n;
@@ -511,30 +507,44 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR, EPI == EPI_QKV_NORM_ROPE>::THREAD
           }
         };
         if constexpr (QKV) {
-          // The step's 64 columns are one head, in registers whole.
-          uint32_t r[64];
-          if (any) {
-            tmem_ld32(tbase + ca, reinterpret_cast<uint32_t(&)[32]>(r[0]));
-            tmem_ld32(tbase + ca + 32, reinterpret_cast<uint32_t(&)[32]>(r[32]));
-            tmem_ld_wait();
-          }
-          arrive_empty();
-          if (!any) continue;
+          // The step's 64 columns are one head. Its halves are read one after the other: statistics of the first, of
+          // the second, then the second's result and, read again, the first's. A lane that holds the whole head needs
+          // 168 registers, which leaves room for one group of warps only (8200 x 2304 x 768 29 us, 65600 x 3 * 1024 x 1024
+          // 235; this way 26.5 and 199; two warps per head that exchange their sums 27.1 and 220).
           const int head = out0 >> 6;
+          uint32_t r[32];
+          auto scaled_half = [&](int h) {
+            read32(ca + 32 * h, r);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              scale_cols<8, MX>(r + 8 * g, rs, csa + 32 * h + 8 * g, ba + 32 * h + 8 * g);
+              group_end();
+            }
+          };
           auto pair_of = [&](int j) { return make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])); };
+          if (!any) {
+            arrive_empty();
+            continue;
+          }
           if (head >= args.q_heads + args.k_heads) {  // v
 #pragma unroll
-            for (int g = 0; g < 8; ++g) {
-              scale_cols<8, MX>(r + 8 * g, rs, csa + 8 * g, ba + 8 * g);
-              float z[8];
+            for (int h = 0; h < 2; ++h) {
+              scaled_half(h);
+              if (h == 1) arrive_empty();
 #pragma unroll
-              for (int j = 0; j < 8; ++j) z[j] = __uint_as_float(r[8 * g + j]);
-              stage8(g, z);
+              for (int g = 0; g < 4; ++g) {
+                float z[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) z[j] = __uint_as_float(r[8 * g + j]);
+                stage8(4 * h + g, z);
+              }
             }
           } else {
             // Angles of four pairs, read one group ahead of their use; volatile, with the pointers stepped in place,
             // so that the compiler neither reads all of them at once nor keeps an address for each.
             const float *cp = args.rope_cos + pos, *sp = args.rope_sin + pos;
+            cp += 16 * static_cast<int64_t>(args.tokens);
+            sp += 16 * static_cast<int64_t>(args.tokens);
             float rope[2][8];
             auto load_angles = [&](float(&a)[8]) {
 #pragma unroll
@@ -546,47 +556,62 @@ __global__ void __launch_bounds__(Fp4Cfg<PAIR, EPI == EPI_QKV_NORM_ROPE>::THREAD
                     : "l"(static_cast<int64_t>(args.tokens) * 4));
             };
             load_angles(rope[0]);
+            // Mean and sum of squared differences of each half, then of both: with 32 values each,
+            // M2 = M2a + M2b + 16 (mean_a - mean_b)^2.
+            float mean[2] = {0.f, 0.f}, square[2];
 #pragma unroll
-            for (int g = 0; g < 8; ++g) {
-              scale_cols<8, MX>(r + 8 * g, rs, csa + 8 * g, ba + 8 * g);
-              group_end();
-            }
-            float mean = 0.f;
-            if (args.norm == FF_NORM_LAYER) {
-              float2 sum = make_float2(0.f, 0.f);
+            for (int h = 0; h < 2; ++h) {
+              scaled_half(h);
+              if (args.norm == FF_NORM_LAYER) {
+                float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) sum = add2(sum, pair_of(j));
-              mean = (sum.x + sum.y) * (1.f / 64.f);
-            }
-            const float2 m2 = make_float2(-mean, -mean);
-            float2 sq = make_float2(0.f, 0.f);
+                for (int j = 0; j < 16; ++j) sum = add2(sum, pair_of(j));
+                mean[h] = (sum.x + sum.y) * (1.f / 32.f);
+              }
+              float2 sq = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const float2 d = add2(pair_of(j), m2);
-              sq = fma2(d, d, sq);
+              for (int j = 0; j < 16; ++j) {
+                const float2 d = add2(pair_of(j), make_float2(-mean[h], -mean[h]));
+                sq = fma2(d, d, sq);
+              }
+              square[h] = sq.x + sq.y;
             }
-            const float rstd = rsqrtf((sq.x + sq.y) * (1.f / 64.f) + args.qk_eps);
-            const float2 r2 = make_float2(rstd, rstd);
+            const float diff = mean[0] - mean[1], neg = -0.5f * (mean[0] + mean[1]);
+            const float rstd = rsqrtf((square[0] + square[1] + 16.f * diff * diff) * (1.f / 64.f) + args.qk_eps);
+            const float2 m2 = make_float2(neg, neg), r2 = make_float2(rstd, rstd);
             const float* const w = normp + (head < args.q_heads ? 0 : 128);  // weights, then biases (zero for RMS)
 #pragma unroll
-            for (int g = 0; g < 8; ++g) {
-              if (g < 7) load_angles(rope[(g + 1) & 1]);
-              float z[8];
-#pragma unroll
-              for (int j = 0; j < 4; j += 2) {
-                const float4 w4 = *reinterpret_cast<const float4*>(w + 8 * g + 2 * j);
-                const float4 b4 = *reinterpret_cast<const float4*>(w + 64 + 8 * g + 2 * j);
-                const float2 x[2] = {
-                    fma2(add2(pair_of(4 * g + j), m2), mul2(r2, make_float2(w4.x, w4.y)), make_float2(b4.x, b4.y)),
-                    fma2(add2(pair_of(4 * g + j + 1), m2), mul2(r2, make_float2(w4.z, w4.w)), make_float2(b4.z, b4.w))};
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                  const float c = rope[g & 1][2 * (j + k)], sn = rope[g & 1][2 * (j + k) + 1];
-                  z[2 * (j + k)] = x[k].x * c - x[k].y * sn;
-                  z[2 * (j + k) + 1] = x[k].x * sn + x[k].y * c;
-                }
+            for (int k = 0; k < 2; ++k) {
+              const int h = 1 - k;
+              if (k == 1) {
+                scaled_half(0);
+                arrive_empty();
               }
-              stage8(g, z);
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                if (k == 0 && g == 3) {
+                  cp = args.rope_cos + pos;
+                  sp = args.rope_sin + pos;
+                }
+                if (k == 0 || g < 3) load_angles(rope[(g + 1) & 1]);
+                const float* const wg = w + 32 * h + 8 * g;
+                float z[8];
+#pragma unroll
+                for (int j = 0; j < 4; j += 2) {
+                  const float4 w4 = *reinterpret_cast<const float4*>(wg + 2 * j);
+                  const float4 b4 = *reinterpret_cast<const float4*>(wg + 64 + 2 * j);
+                  const float2 x[2] = {
+                      fma2(add2(pair_of(4 * g + j), m2), mul2(r2, make_float2(w4.x, w4.y)), make_float2(b4.x, b4.y)),
+                      fma2(add2(pair_of(4 * g + j + 1), m2), mul2(r2, make_float2(w4.z, w4.w)), make_float2(b4.z, b4.w))};
+#pragma unroll
+                  for (int i = 0; i < 2; ++i) {
+                    const float c = rope[g & 1][2 * (j + i)], sn = rope[g & 1][2 * (j + i) + 1];
+                    z[2 * (j + i)] = x[i].x * c - x[i].y * sn;
+                    z[2 * (j + i) + 1] = x[i].x * sn + x[i].y * c;
+                  }
+                }
+                stage8(4 * h + g, z);
+              }
             }
           }
         } else {
