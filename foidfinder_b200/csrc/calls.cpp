@@ -106,7 +106,7 @@ bool address(PyObject* o, const void** p) {
   if (o == Py_None) return true;
   if (!PyLong_Check(o)) return false;
   *p = PyLong_AsVoidPtr(o);
-  return true;
+  return *p != nullptr || PyErr_Occurred() == nullptr;
 }
 
 bool current(int device) { return c10::cuda::current_device() == device; }

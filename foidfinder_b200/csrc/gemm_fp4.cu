@@ -15,12 +15,12 @@
 // of A, half of W's 256 rows and all of the tile's W scales (each SM's tensor core reads them from its own
 // TMEM), and shared memory moves half as many bytes per multiply-add.
 //
-// Measured, FF_FP4_NV unless said: 8192^3 190 us (5.8 PFLOP/s, 3.5 times the bf16 rate of the same GPU), bound by the
+// Measured, FF_FP4_NV unless said: 8192^3 191 us (5.8 PFLOP/s, 3.5 times the bf16 rate of the same GPU), bound by the
 // tensor cores. 65600 x 5504 x 1024 with SwiGLU 209 us (3.5 PFLOP/s), where reading the accumulators, activating and
-// storing takes about as long as the products do: 190 us without the column parameters, 183 without the
-// stores, 159 with the MMAs alone. 65600 x 1024 x 2730 with a residual 100 us; 65600 x 1024 x 1024 44 us, bound by the
-// 200 MB moved. 8200 x 2304 x 768 with norm and rotation 26.5 us, bound by its epilogue (21 without the angles). One row of 1024 against 5460: 8 us,
-// the latency of one mainloop and its launch.
+// storing takes about as long as the products do: 190 us without the column parameters, 183 without the stores, 159
+// with the MMAs alone. 65600 x 1024 x 2730 with a residual 100 us; 65600 x 1024 x 1024 44 us, bound by the 200 MB moved.
+// 8200 x 2304 x 768 with norm and rotation 26.5 us, bound by its epilogue (21 without the reads of the angles). One row
+// of 1024 against 30877: 8 us, the latency of a launch and of two tiles.
 #include "common.h"
 #include "fp4.cuh"
 #include "gemm_fp4.h"
