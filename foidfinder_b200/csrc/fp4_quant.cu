@@ -7,7 +7,8 @@
 //
 // The power-of-two row scale costs no accuracy that the e4m3 block scale would have kept, and makes v / s and
 // S * s exact, so the codes are the correctly rounded quotients: amax / 6 is rounded correctly (sixth()), and v / S
-// is a product with the reciprocal whose last bits are snapped off for 16-bit inputs (quotient2()).
+// is a product with the reciprocal whose last bits are snapped off for 16-bit inputs, and corrected by its remainder
+// for f32 (quotient2(); 5460 x 1024 6.9 us, 10.3 with IEEE divisions).
 // A row (NV) or block (MX) that holds an infinity or NaN gets a NaN scale, so that it shows in every result.
 //
 // Bound by HBM: 2 bytes read and 0.56 (NV) or 0.53 (MX) written per value. The whole row stays in registers,
@@ -21,7 +22,7 @@
 // columns), which delivers 8 bytes of gamma and beta per value. What did not help: two rows at a time for the same gamma
 // and beta (38.9 us and 140: half the warps), half a row per warp with two rows (43 and 172: barriers), the next row read
 // ahead into shared memory (50 and 148), 32-byte loads (37.6 and 148), gamma and beta in registers (73) or TMEM (78).
-// Dequantisation, 65600 x 1024 fp16 30 us (5.7 TB/s); 65600 x 2730 bf16 89 us aligned, 105 not. A kernel that only reads
+// Dequantisation, 65600 x 1024 fp16 30 us (5.7 TB/s), 32000 x 4096 f32 100 us; 65600 x 2730 bf16 89 us aligned, 105 not. A kernel that only reads
 // and writes the same bytes takes 33 and 80.
 #include <algorithm>
 #include <type_traits>
@@ -157,17 +158,22 @@ __device__ __forceinline__ float inv_pow2(float s) { return __uint_as_float((254
 // v / (S s) for the code, r about 1 / (S s). kExact16: v came from a 16-bit type, so a quotient that is no
 // rounding tie of e2m1 is at least 2^-13 away from one, while v * r is within 2^-20 of the quotient: rounding
 // v * r + 192 (one FMA, to multiples of 2^-16) puts true ties exactly on the tie (r within 2^-22 of 1 / (S s)
-// is enough). kExact32: IEEE division
-// (checkpoint weights, once per load). kPlain: v is itself rounded (after a LayerNorm) or r a power of two.
+// is enough). kExact32: v from f32 and already divided by s (exact, or far below any tie), r the reciprocal of scale = S: the remainder of
+// v * r, exact in an FMA, corrects it to within a hair of the true quotient's rounding. A quotient that equals a tie
+// comes out as the tie; any other is at least 1.06 * 2^-24 of itself away from one (v's last bit against at most 1.875
+// of scale), more than half a unit in the last place, and does not. kPlain: v is itself rounded (after a LayerNorm) or r
+// a power of two.
 enum QuotientKind { kPlain, kExact16, kExact32 };
 template <int KIND>
 __device__ __forceinline__ float2 quotient2(float2 v, float r, float scale) {
-  if constexpr (KIND == kExact32)
-    return scale > 0.f ? make_float2(__fdiv_rn(v.x, scale), __fdiv_rn(v.y, scale)) : make_float2(0.f, 0.f);
-  else if constexpr (KIND == kExact16)
+  if constexpr (KIND == kExact32) {
+    const float2 r2 = make_float2(r, r), q = mul2(v, r2);
+    return fma2(fma2(q, make_float2(-scale, -scale), v), r2, q);
+  } else if constexpr (KIND == kExact16) {
     return add2(fma2(v, make_float2(r, r), make_float2(192.f, 192.f)), make_float2(-192.f, -192.f));
-  else
+  } else {
     return mul2(v, make_float2(r, r));
+  }
 }
 
 template <int KIND>
@@ -194,7 +200,14 @@ __device__ __forceinline__ uint32_t nv_piece(const float2 (&v)[8], float amax, f
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(S));
   r = fmaf(r, fmaf(-S, r, 1.f), r);  // to the last bit
-  *codes = bad ? make_uint2(0, 0) : codes16<KIND>(v, byte ? r * is : 0.f, S * s);
+  if constexpr (KIND == kExact32) {
+    float2 u[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) u[e] = mul2(v[e], make_float2(is, is));
+    *codes = bad ? make_uint2(0, 0) : codes16<KIND>(u, byte ? r : 0.f, S);
+  } else {
+    *codes = bad ? make_uint2(0, 0) : codes16<KIND>(v, byte ? r * is : 0.f, S * s);
+  }
   return byte;
 }
 // One 16-column piece of an MX block whose 32 columns have maximum amax. Scaling by a power of two is exact.
@@ -719,10 +732,18 @@ __global__ void __launch_bounds__(256)
       }
       T* const o = out + row * ldo + c;
       const bool whole = (ALIGNED || c >= 0) && c + 8 <= cols;
+      const bool wide = sizeof(T) == 4 && (reinterpret_cast<uintptr_t>(o) & 31) == 0;
 #pragma unroll
       for (int g = 0; g < 8; g += E) {
         if (whole || ((ALIGNED || c + g >= 0) && c + g + E <= cols)) {
-          __stcs(reinterpret_cast<uint4*>(o + g), pack16<T>(v + g));
+          if (sizeof(T) == 4 && whole && wide) {  // one store of 32 bytes: two of 16 would each write half sectors
+            if (g == 0)
+              asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(o), "f"(v[0]), "f"(v[1]), "f"(v[2]),
+                           "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+                           : "memory");
+          } else {
+            __stcs(reinterpret_cast<uint4*>(o + g), pack16<T>(v + g));
+          }
         } else {
 #pragma unroll
           for (int e = g; e < g + E; ++e)

@@ -97,6 +97,29 @@ def test_quantize_and_dequantize_any_alignment(cuda_device, no_device_error, fmt
         assert torch.isnan(buf).sum().item() == before  # nothing outside the rows was written
 
 
+@pytest.mark.parametrize(("low", "high"), [(-20, 20), (-120, 118)])
+def test_quotients_next_to_ties(cuda_device, no_device_error, low, high):
+    """f32 values that are e2m1 ties times their block's scale, or up to two units in the last place off them."""
+    from foidfinder_b200 import fp4
+
+    g = torch.Generator().manual_seed(high)
+    rows, cols = 256, 256
+    x = torch.randn(rows, cols, generator=g, dtype=torch.float64)
+    x[:, 0] = 2688 * torch.rand(rows, generator=g, dtype=torch.float64).clamp_min(0.51)
+    first = x.view(rows, -1, 16)[:, :, 0]  # each block's largest value fixes its scale
+    first[:, 1:] = 2688 * torch.rand(rows, cols // 16 - 1, generator=g, dtype=torch.float64) ** 4
+    x = (x * 2.0 ** torch.randint(low, high, (rows, 1), generator=g)).float()
+    _, s, row = O.quantize(x, "nv")
+    scale = s.view(torch.float8_e4m3fn).double() * row.double()[:, None]
+    tie = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], dtype=torch.float64)
+    v = (tie[torch.randint(0, 7, (rows, cols // 16, 15), generator=g)] * scale[:, :, None]).float()
+    v = (v.view(torch.int32) + torch.randint(-2, 3, v.shape, generator=g).int()).view(torch.float32).where(v > 0, 0.0)
+    blocks = x.view(rows, -1, 16)
+    v = v.where(v <= blocks[:, :, :1].abs(), 0.0)
+    blocks[:, :, 1:] = v.where(torch.rand(v.shape, generator=g) < 0.5, -v)
+    _check_exact(fp4.quantize(x.to(cuda_device), "nv"), x)
+
+
 @pytest.mark.parametrize("fmt", ["nv", "mx"])
 def test_quantize_special_values(cuda_device, no_device_error, fmt):
     from foidfinder_b200 import fp4
