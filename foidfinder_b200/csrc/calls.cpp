@@ -179,7 +179,7 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (fits) std::memcpy(&e, view.buf, sizeof e);
     PyBuffer_Release(&view);
     if (!fits || x.rows == 0 || x.cols != K || out.rows != x.rows || out.device != x.device ||
-        (e.kind == FF_EPI_SWIGLU ? out.cols > N / 2 : out.cols != N) || !current(x.device))
+        (e.kind == FF_EPI_SWIGLU ? out.cols < 1 || out.cols > N / 2 : out.cols != N) || !current(x.device))
       return nullptr;
     e.out_dtype = out.type;
     e.out = out.data;

@@ -472,7 +472,7 @@ def _bind(e: _lib.Fp4Epilogue, M: int, N: int, out: torch.Tensor, residual: torc
     """The tensors of one call into an epilogue."""
     rows, cols, e.ldo, d = _matrix(out, what)
     dtype = _DTYPES.get(out.dtype)
-    if d != device or dtype is None or rows != M or (cols > N // 2 if e.kind == EPI_SWIGLU else cols != N):
+    if d != device or dtype is None or rows != M or (not 0 < cols <= N // 2 if e.kind == EPI_SWIGLU else cols != N):  # the library takes 0 for N / 2
         raise RuntimeError(f"{what}: out is {out.dtype} {list(out.shape)} on {out.device} for M={M} N={N} on cuda:{device}")
     e.out_dtype, e.out, e.out_cols = dtype, out.data_ptr(), cols
     if e.kind == EPI_RESIDUAL:

@@ -231,3 +231,25 @@ def test_the_extension_module_leaves_cpu_tensors_alone():
     assert c.qk_norm_rope(x, x, 1, 0, 32, 1, f, None, f, None, 1e-6, f, f, 0) is None
     with pytest.raises(TypeError):
         c.bind(1, 2)
+
+
+class _OnGpu:
+    """A CPU tensor that says it is on cuda:0, for host checks that come before any CUDA call."""
+
+    def __init__(self, t):
+        self._t = t
+
+    def get_device(self):
+        return 0
+
+    def __getattr__(self, name):
+        return getattr(self._t, name)
+
+
+def test_an_output_of_no_columns_is_refused():
+    """For SwiGLU the library takes out_cols = 0 as N / 2, which a view of no columns does not hold."""
+    out = _OnGpu(torch.zeros(4, 64, dtype=torch.float16)[:, :0])
+    with pytest.raises(RuntimeError, match="out is"):
+        ops._bind(_lib.Fp4Epilogue(kind=_lib.EPI_SWIGLU), 4, 128, out, None, 0, "gemm_fp4")
+    with pytest.raises(RuntimeError, match="out is"):
+        ops._bind(_lib.Fp4Epilogue(kind=_lib.EPI_BIAS), 4, 128, out, None, 0, "gemm_fp4")

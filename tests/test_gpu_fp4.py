@@ -609,3 +609,18 @@ def test_fp4_block(cuda_device, no_device_error, arch, fmt):
     x1 = f16(x.double() + lin(o, "proj"))
     ref = x1 + lin(hidden(f16(act(lin(ln(x1, "norm2"), "fc1")))), "fc2")
     close("block", got, ref)
+
+
+def test_swiglu_into_no_columns_writes_nothing(cuda_device, no_device_error):
+    from foidfinder_b200 import fp4, ops
+
+    d = cuda_device
+    layer = fp4.Fp4Linear(torch.ones(128, 64, device=d), epilogue="swiglu")
+    x = torch.ones(4, 64, dtype=torch.float16, device=d)
+    q, W = fp4.quantize(x), layer.weight
+    buf = torch.full((4, 64), 77.0, dtype=torch.float16, device=d)
+    with pytest.raises(RuntimeError, match="out is"):
+        ops.gemm_fp4(q.codes, q.scales, q.row_scale, W.codes, W.scales, W.row_scale, buf[:, :0], ops.EPI_SWIGLU, 0, N=128, K=64)
+    with pytest.raises(RuntimeError, match="out is"):
+        ops.linear_fp4(x, W.codes, W.scales, W.row_scale, buf[:, :0], ops.EPI_SWIGLU, 0, N=128)
+    assert (buf == 77.0).all()
