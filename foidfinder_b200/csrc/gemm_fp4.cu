@@ -891,9 +891,11 @@ int gemm_fp4(const Fp4Operand& A, const Fp4Operand& W, int fmt, int M, int N, in
   a.k_heads = e->k_heads;
   a.qk_eps = e->qk_eps;
   a.q_w = e->q_w;
-  a.q_b = e->q_b;
   a.k_w = e->k_w;
-  a.k_b = e->k_b;
+  if (e->norm == FF_NORM_LAYER) {  // an RMS norm has no bias, whatever the caller set
+    a.q_b = e->q_b;
+    a.k_b = e->k_b;
+  }
   a.rope_cos = e->rope_cos;
   a.rope_sin = e->rope_sin;
   a.tokens = e->tokens > 0 ? e->tokens : 1;

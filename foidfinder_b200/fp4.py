@@ -82,7 +82,7 @@ class Fp4Linear:
 
     epilogue: "bias"; "gelu"; "swiglu" (weight rows are the H gates, then the H ups; y [M, H]); "residual" (y +
     residual); "qkv" (N = 3 * heads * 64, or q_heads + 2 * k_heads of them; q and k heads normalised by `norm`
-    "rms" or "layer" with q_weight/k_weight [64] (and biases) and rotated by the `rope` tables (cos, sin), each
+    "rms" or "layer" with q_weight/k_weight [64] (and, for "layer", biases) and rotated by the `rope` tables (cos, sin), each
     [32, tokens])."""
 
     def __init__(

@@ -206,7 +206,7 @@ typedef struct ff_fp4_epilogue {
   int64_t ldr;
   int norm, q_heads, k_heads, tokens;
   float qk_eps;
-  const float *q_w, *q_b, *k_w, *k_b; /* [64]; biases may be NULL */
+  const float *q_w, *q_b, *k_w, *k_b; /* [64]; biases may be NULL and are read for FF_NORM_LAYER only */
   const float *rope_cos, *rope_sin;
 } ff_fp4_epilogue;
 int ff_gemm_fp4(const uint8_t* A, const uint8_t* A_scales, const float* row_scale, const uint8_t* W,
@@ -226,7 +226,7 @@ int ff_linear_fp4(const void* x, int dtype, int64_t ldx, const float* gamma, con
 /*
  * Per-head norm and rotary position rotation of queries and keys in one pass: x [rows, >= (q_heads + k_heads) *
  * head_dim] of type dtype (FF_F16, FF_BF16), row stride ldx elements, q heads then k heads. Every head is
- * normalised (FF_NORM_RMS or FF_NORM_LAYER, f32, weights [head_dim], biases for FF_NORM_LAYER or NULL) and its
+ * normalised (FF_NORM_RMS or FF_NORM_LAYER, f32, weights [head_dim], biases or NULL, read for FF_NORM_LAYER only) and its
  * pairs rotated by the angles of position row % tokens: rope_cos / rope_sin [head_dim / 2, tokens] f32,
  * angle-major. pairing FF_ROPE_PAIRS: pair i is columns (2i, 2i + 1); FF_ROPE_HALVES: (i, i + head_dim / 2).
  * out [rows, (q_heads + k_heads) * head_dim], row stride ldo; out may be x itself (ldo == ldx). head_dim 32, 64,

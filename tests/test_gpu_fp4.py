@@ -624,3 +624,22 @@ def test_swiglu_into_no_columns_writes_nothing(cuda_device, no_device_error):
     with pytest.raises(RuntimeError, match="out is"):
         ops.linear_fp4(x, W.codes, W.scales, W.row_scale, buf[:, :0], ops.EPI_SWIGLU, 0, N=128)
     assert (buf == 77.0).all()
+
+
+@pytest.mark.parametrize("fmt", ["nv", "mx"])
+def test_an_rms_norm_has_no_bias(cuda_device, no_device_error, fmt):
+    """Biases given with an RMS head norm change nothing, neither in the product's epilogue nor by itself."""
+    from foidfinder_b200 import fp4, ops
+
+    d = cuda_device
+    g = torch.Generator().manual_seed(3)
+    w, b = (1 + 0.1 * torch.randn(64, generator=g)).to(d), torch.full((64,), 3.0, device=d)
+    cos, sin = (t.to(d) for t in _tables(7, 32))
+    weight, x = _x(3 * 64, 128, torch.float32, 2).to(d), _x(40, 128, torch.float16, 5).to(d)
+    kw = dict(fmt=fmt, epilogue="qkv", rope=(cos, sin), norm="rms", q_weight=w, k_weight=w)
+    assert torch.equal(fp4.Fp4Linear(weight, q_bias=b, k_bias=b, **kw)(x), fp4.Fp4Linear(weight, **kw)(x))
+    args = dict(q_heads=1, k_heads=1, head_dim=64, norm="rms", q_weight=w, k_weight=w, rope_cos=cos, rope_sin=sin)
+    with_bias, without = torch.empty_like(x), torch.empty_like(x)
+    ops.qk_norm_rope(x, with_bias, q_bias=b, k_bias=b, **args)
+    ops.qk_norm_rope(x, without, **args)
+    assert torch.equal(with_bias, without)
