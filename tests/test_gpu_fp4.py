@@ -643,3 +643,57 @@ def test_an_rms_norm_has_no_bias(cuda_device, no_device_error, fmt):
     ops.qk_norm_rope(x, with_bias, q_bias=b, k_bias=b, **args)
     ops.qk_norm_rope(x, without, **args)
     assert torch.equal(with_bias, without)
+
+
+def _biases_only(values, epilogue, device):
+    """A layer whose products are zero: its epilogue gets the biases, exactly."""
+    from foidfinder_b200 import fp4
+
+    v = torch.tensor(values)
+    return fp4.Fp4Linear(torch.zeros(len(v), 64, device=device), v.to(device), epilogue=epilogue)
+
+
+def _check_whole_range(got, ref, tol, dtype):
+    """Within `tol` and the type's rounding where the type holds the value, its rounding (an infinity) where it does not."""
+    top = torch.finfo(dtype).max
+    inside = ref.abs() <= top
+    _close(torch.where(inside, got.cpu().double(), 0), torch.where(inside, ref, 0), torch.where(inside, tol, 0), dtype)
+    assert torch.equal(got.cpu()[~inside].float(), torch.copysign(torch.full_like(ref[~inside], math.inf), ref[~inside]).float())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_swiglu_over_the_whole_range_of_gates(cuda_device, no_device_error, dtype):
+    """silu goes to zero below; f32 gates and ups of any size. 2^t with |t| <= 62 in f32 is within 62 * 2^-23 (2^-17) of
+    itself, the remaining operations within 2^-21: 2^-16 of the result, and 2^-56 of the up where the gate is cut off."""
+    gates = [-3e38, -1e20, -1e6, -200.0, -88.0, -60.0, -43.5, -43.0, -42.9, -30.0, -10.0, -1.0, -1e-20, 0.0, 1e-20, 0.5, 20.0, 43.5, 100.0, 1e6, 1e20]
+    ups = [1.0, -2.5, 1e-20, 1e6, -1e20, 1e30, 3e37]
+    g, u = torch.tensor(gates).repeat_interleave(len(ups)), torch.tensor(ups).repeat(len(gates))
+    x = torch.ones(3, 64, dtype=dtype, device=cuda_device)
+    got = _biases_only(torch.cat([g, u]).tolist(), "swiglu", cuda_device)(x)
+    ref = (g.double() * torch.sigmoid(g.double()) * u.double())[None].expand(3, -1)
+    edge = 2.0**-14 * torch.finfo(dtype).max
+    clear = (ref.abs() - torch.finfo(dtype).max).abs() > edge  # not next to the largest value, where rounding decides
+    assert clear.all()
+    _check_whole_range(got, ref, 2.0**-16 * ref.abs() + 2.0**-56 * u.double().abs(), dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_gelu_over_the_whole_range(cuda_device, no_device_error, dtype):
+    """The bounds are those of SwiGLU; where the argument is cut off the result is off by 7.6 * 2^-62 < 2^-59."""
+    v = torch.tensor([-3e38, -1e20, -1e10, -1e5, -100.0, -10.0, -8.0, -7.7, -7.5, -5.0, -1.0, -1e-20, 0.0, 1e-20, 1.0, 7.7, 100.0, 1e4, 1e10, 1e20, 1e38])
+    x = torch.ones(3, 64, dtype=dtype, device=cuda_device)
+    got = _biases_only(v.tolist(), "gelu", cuda_device)(x)
+    y = v.double()
+    ref = (y * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (y + 0.044715 * y**3)))[None].expand(3, -1)
+    _check_whole_range(got, ref, 2.0**-16 * ref.abs() + 2.0**-59, dtype)
+
+
+@pytest.mark.parametrize("epilogue", ["swiglu", "gelu"])
+def test_a_nan_column_stays_in_its_column(cuda_device, no_device_error, epilogue):
+    v = [0.5 + 0.01 * i for i in range(64)]
+    x = torch.ones(3, 64, dtype=torch.float16, device=cuda_device)
+    good = _biases_only(v, epilogue, cuda_device)(x)
+    for at in (0, 7, 31):
+        got = _biases_only(v[:at] + [math.nan] + v[at + 1 :], epilogue, cuda_device)(x)
+        keep = torch.arange(good.shape[1], device=cuda_device) != at
+        assert torch.isnan(got[:, at]).all() and torch.equal(got[:, keep], good[:, keep])
