@@ -100,13 +100,30 @@ bool number(PyObject* o, float* v) {
     return false;
   return true;
 }
-// An address or None.
-bool address(PyObject* o, const void** p) {
-  *p = nullptr;
-  if (o == Py_None) return true;
-  if (!PyLong_Check(o)) return false;
-  *p = PyLong_AsVoidPtr(o);
-  return *p != nullptr || PyErr_Occurred() == nullptr;
+// The addresses of a prepared epilogue's tensors (its attribute `tensors`: bias, q weight, q bias, k weight, k bias, cos,
+// sin) into its fields. One that was filled in by hand has none.
+bool address(PyObject* o, int N, int device, ff_fp4_epilogue* e) {
+  static PyObject* const name = PyUnicode_InternFromString("tensors");
+  PyObject* const ts = name != nullptr ? PyObject_GetAttr(o, name) : nullptr;
+  if (ts == nullptr || ts == Py_None) {
+    PyErr_Clear();
+    Py_XDECREF(ts);
+    return name != nullptr;
+  }
+  const bool qkv = e->kind == FF_EPI_QKV_NORM_ROPE;
+  float* p[7] = {};
+  bool ok = PyTuple_Check(ts) && PyTuple_GET_SIZE(ts) == 7 && (!qkv || e->tokens >= 1);
+  for (int i = 0; ok && i < (qkv ? 7 : 1); ++i)
+    ok = vector(PyTuple_GET_ITEM(ts, i), i == 0 ? N : i < 5 ? 64 : 32 * static_cast<int64_t>(e->tokens), device, &p[i]);
+  Py_DECREF(ts);
+  e->bias = p[0];
+  e->q_w = p[1];
+  e->q_b = p[2];
+  e->k_w = p[3];
+  e->k_b = p[4];
+  e->rope_cos = p[5];
+  e->rope_sin = p[6];
+  return ok;
 }
 
 bool current(int device) { return c10::cuda::current_device() == device; }
@@ -159,18 +176,20 @@ PyObject* dequantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// linear(x, (codes, scales, row_scale) addresses of the weight, fmt, N, K, gamma and beta addresses, eps, epilogue, out, residual)
+// linear(x, (codes, scales, row_scale) of the weight, fmt, N, K, gamma, beta, eps, epilogue, out, residual)
 PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     Matrix x, out;
     int fmt, N, K;
     float eps;
-    const void *w[3], *gamma, *beta;
-    if (n != 11 || !matrix(a[0], &x) || !PyTuple_Check(a[1]) || PyTuple_GET_SIZE(a[1]) != 3) return nullptr;
-    for (int i = 0; i < 3; ++i)
-      if (!address(PyTuple_GET_ITEM(a[1], i), &w[i])) return nullptr;
-    if (!integer(a[2], &fmt) || !integer(a[3], &N) || !integer(a[4], &K) || !address(a[5], &gamma) || !address(a[6], &beta) ||
-        !number(a[7], &eps) || !matrix(a[9], &out))
+    float *gamma, *beta;
+    Operand w;
+    if (n != 11 || !matrix(a[0], &x) || !PyTuple_Check(a[1]) || PyTuple_GET_SIZE(a[1]) != 3 || !integer(a[2], &fmt) || !integer(a[3], &N) ||
+        !integer(a[4], &K) || N < 1 || K < 1)
+      return nullptr;
+    PyObject* const wt[3] = {PyTuple_GET_ITEM(a[1], 0), PyTuple_GET_ITEM(a[1], 1), PyTuple_GET_ITEM(a[1], 2)};
+    if (!operand(wt, N, K, fmt, x.device, &w) || !vector(a[5], K, x.device, &gamma) || !vector(a[6], K, x.device, &beta) || !number(a[7], &eps) ||
+        !matrix(a[9], &out))
       return nullptr;
     ff_fp4_epilogue e;
     Py_buffer view;
@@ -178,7 +197,7 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const bool fits = view.len == static_cast<Py_ssize_t>(sizeof e);
     if (fits) std::memcpy(&e, view.buf, sizeof e);
     PyBuffer_Release(&view);
-    if (!fits || x.rows == 0 || x.cols != K || out.rows != x.rows || out.device != x.device ||
+    if (!fits || !address(a[8], N, x.device, &e) || x.rows == 0 || x.cols != K || out.rows != x.rows || out.device != x.device ||
         (e.kind == FF_EPI_SWIGLU ? out.cols < 1 || out.cols > N / 2 : out.cols != N) || !current(x.device))
       return nullptr;
     e.out_dtype = out.type;
@@ -197,8 +216,7 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     // from torch's stream-ordered cache: free for the stream's next use as soon as the call has returned
     void* const ws = c10::cuda::CUDACachingAllocator::raw_alloc_with_stream(static_cast<size_t>(bytes), s);
     PyObject* const rc = status([&] {
-      return lib.linear(x.data, x.type, x.ld, static_cast<const float*>(gamma), static_cast<const float*>(beta), eps, static_cast<const uint8_t*>(w[0]),
-                        static_cast<const uint8_t*>(w[1]), static_cast<const float*>(w[2]), fmt, x.rows, N, K, &e, ws, bytes, s);
+      return lib.linear(x.data, x.type, x.ld, gamma, beta, eps, w.codes, w.scales, w.row_scale, fmt, x.rows, N, K, &e, ws, bytes, s);
     });
     c10::cuda::CUDACachingAllocator::raw_delete(ws);
     return rc;

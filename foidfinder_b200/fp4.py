@@ -83,7 +83,9 @@ class Fp4Linear:
     epilogue: "bias"; "gelu"; "swiglu" (weight rows are the H gates, then the H ups; y [M, H]); "residual" (y +
     residual); "qkv" (N = 3 * heads * 64, or q_heads + 2 * k_heads of them; q and k heads normalised by `norm`
     "rms" or "layer" with q_weight/k_weight [64] (and, for "layer", biases) and rotated by the `rope` tables (cos, sin), each
-    [32, tokens])."""
+    [32, tokens]).
+
+    `weight`, `bias`, `gamma` and `beta` are read at every call and may be replaced by others of their shape and kind."""
 
     def __init__(
         self,
@@ -120,9 +122,9 @@ class Fp4Linear:
             h = self.out_features = w.shape[0] // 2
             w = _interleave(w, h)
             bias = None if bias is None else _interleave(bias, h)
-        self.fmt, self.in_features, self.rows, self.eps = fmt, w.shape[1], w.shape[0], eps
+        self.in_features, self.rows, self.eps = w.shape[1], w.shape[0], eps
         self.weight = quantize(w if w.stride(1) == 1 or w.shape[1] == 1 else w.contiguous(), fmt)
-        self.bias, self.gamma, self.beta = bias, _f32(gamma, d), _f32(beta, d)
+        self.gamma, self.beta = _f32(gamma, d), _f32(beta, d)
         heads = {}
         if epilogue == "qkv":
             if w.shape[0] % 64 or rope is None or q_weight is None or k_weight is None:
@@ -131,27 +133,47 @@ class Fp4Linear:
             q_heads = total // 3 if q_heads is None else q_heads
             if q_heads < 0 or (total - q_heads) % 2 or total < q_heads:
                 raise RuntimeError(f"Fp4Linear: {total} heads do not split into {q_heads} q heads and as many k as v heads")
-            self._heads = [_f32(t, d) for t in (q_weight, k_weight, q_bias, k_bias, *rope)]
-            heads = dict(zip(("q_weight", "k_weight", "q_bias", "k_bias", "rope_cos", "rope_sin"), self._heads))
+            tensors = (_f32(t, d) for t in (q_weight, k_weight, q_bias, k_bias, *rope))
+            heads = dict(zip(("q_weight", "k_weight", "q_bias", "k_bias", "rope_cos", "rope_sin"), tensors))
             heads |= dict(norm=norm, q_heads=q_heads, k_heads=(total - q_heads) // 2, qk_eps=qk_eps)
-        self._epilogue = ops.fp4_epilogue(EPILOGUES[epilogue], self.rows, d, bias=self.bias, **heads)  # refuses bad arguments
-        q = self.weight
-        self._w = ops._operand(q.codes, q.scales, q.row_scale, self.rows, self.in_features, FORMATS[fmt], d.index, "Fp4Linear")
-        self._g = ops._vector(self.gamma, self.in_features, d.index, "Fp4Linear: gamma")
-        self._b = ops._vector(self.beta, self.in_features, d.index, "Fp4Linear: beta")
-        self._fmt, self._device = FORMATS[fmt], d.index
+        self._kind, self._heads = EPILOGUES[epilogue], heads
+        self.bias = bias
+
+    @property
+    def fmt(self) -> str:
+        return self.weight.fmt
+
+    @property
+    def bias(self) -> torch.Tensor | None:
+        """[rows] f32 (swiglu: in the order of the weight's rows), or None."""
+        return self._bias
+
+    @bias.setter
+    def bias(self, bias: torch.Tensor | None) -> None:
+        self._epilogue = ops.fp4_epilogue(self._kind, self.rows, self.weight.codes.device, bias=bias, **self._heads)  # refuses bad arguments
+        self._bias = bias
+
+    def __getstate__(self) -> dict:
+        return {k: v for k, v in self.__dict__.items() if k != "_epilogue"}  # addresses do not travel
+
+    def __setstate__(self, state: dict) -> None:
+        self.__dict__.update(state)
+        self.bias = state["_bias"]
 
     def __call__(self, x: torch.Tensor, out: torch.Tensor | None = None, residual: torch.Tensor | None = None) -> torch.Tensor:
         """x [M, in_features] -> [M, out_features] (`out`, or a new tensor whose rows start 16 bytes apart or more)."""
-        if x.get_device() != self._device:
-            raise RuntimeError(f"Fp4Linear: x is on {x.device}, the weight on cuda:{self._device}")
+        w = self.weight
+        if x.get_device() != w.codes.get_device():
+            raise RuntimeError(f"Fp4Linear: x is on {x.device}, the weight on {w.codes.device}")
+        if w.rows != self.rows or w.cols != self.in_features:
+            raise RuntimeError(f"Fp4Linear: the weight is [{w.rows}, {w.cols}], the layer's [{self.rows}, {self.in_features}]")
         if out is None:
             pitch = (self.out_features + 7) // 8 * 8
             dtype = torch.float16 if x.dtype == torch.float32 else x.dtype
             out = torch.empty(x.shape[0], pitch, dtype=dtype, device=x.device)[:, : self.out_features]
         if out.shape[-1] != self.out_features:
             raise RuntimeError(f"Fp4Linear: out must have {self.out_features} columns, got {list(out.shape)}")
-        ops._linear(x, self._w, self._fmt, self.rows, self.in_features, self._g, self._b, self.eps, self._epilogue, out, residual)
+        ops._linear(x, (w.codes, w.scales, w.row_scale), FORMATS[w.fmt], self.rows, self.in_features, self.gamma, self.beta, self.eps, self._epilogue, out, residual)
         return out
 
 

@@ -446,18 +446,31 @@ def fp4_epilogue(
     rope_cos: torch.Tensor | None = None,
     rope_sin: torch.Tensor | None = None,
 ) -> _lib.Fp4Epilogue:
-    """The part of a gemm_fp4 epilogue that does not change from call to call (the tensors must outlive it)."""
+    """The part of a gemm_fp4 epilogue that does not change from call to call. It holds its tensors (`tensors`), and every
+    call reads their addresses anew."""
     e = _lib.Fp4Epilogue(kind=epi)
-    d = device.index if device.index is not None else torch.cuda.current_device()
-    e.bias = _vector(bias, N, d, "fp4_epilogue: bias")
+    heads = (None,) * 6
     if epi == EPI_QKV_NORM_ROPE:
         _need(norm in _NORMS, "fp4_epilogue: norm must be 'rms' or 'layer'")
         _need(q_weight is not None and k_weight is not None, "fp4_epilogue: q and k norm weights are required")
-        e.q_w, e.k_w = _vector(q_weight, 64, d, "fp4_epilogue: q_weight"), _vector(k_weight, 64, d, "fp4_epilogue: k_weight")
-        e.q_b, e.k_b = _vector(q_bias, 64, d, "fp4_epilogue: q_bias"), _vector(k_bias, 64, d, "fp4_epilogue: k_bias")
-        e.rope_cos, e.rope_sin, e.tokens = _tables(rope_cos, rope_sin, 32, d, "fp4_epilogue")
+        heads = (q_weight, q_bias, k_weight, k_bias, rope_cos, rope_sin)
         e.norm, e.q_heads, e.k_heads, e.qk_eps = _NORMS[norm], q_heads, k_heads, qk_eps
+    e.tensors = (bias, *heads)
+    _address(e, N, device.index if device.index is not None else torch.cuda.current_device(), "fp4_epilogue")
     return e
+
+
+def _address(e: _lib.Fp4Epilogue, N: int, device: int, what: str) -> None:
+    """The addresses of an epilogue's tensors into its fields. (One that was filled in by hand has no tensors.)"""
+    tensors = getattr(e, "tensors", None)
+    if tensors is None:
+        return
+    bias, q_weight, q_bias, k_weight, k_bias, cos, sin = tensors
+    e.bias = _vector(bias, N, device, f"{what}: bias")
+    if e.kind == EPI_QKV_NORM_ROPE:
+        e.q_w, e.k_w = _vector(q_weight, 64, device, f"{what}: q_weight"), _vector(k_weight, 64, device, f"{what}: k_weight")
+        e.q_b, e.k_b = _vector(q_bias, 64, device, f"{what}: q_bias"), _vector(k_bias, 64, device, f"{what}: k_bias")
+        e.rope_cos, e.rope_sin, e.tokens = _tables(cos, sin, 32, device, what)
 
 
 def _tables(cos: torch.Tensor | None, sin: torch.Tensor | None, half: int, device: int, what: str) -> tuple[int, int, int]:
@@ -469,7 +482,8 @@ def _tables(cos: torch.Tensor | None, sin: torch.Tensor | None, half: int, devic
 
 
 def _bind(e: _lib.Fp4Epilogue, M: int, N: int, out: torch.Tensor, residual: torch.Tensor | None, device: int, what: str) -> None:
-    """The tensors of one call into an epilogue."""
+    """The tensors of one call, and its own, into an epilogue."""
+    _address(e, N, device, what)
     rows, cols, e.ldo, d = _matrix(out, what)
     dtype = _DTYPES.get(out.dtype)
     if d != device or dtype is None or rows != M or (not 0 < cols <= N // 2 if e.kind == EPI_SWIGLU else cols != N):  # the library takes 0 for N / 2
@@ -481,6 +495,12 @@ def _bind(e: _lib.Fp4Epilogue, M: int, N: int, out: torch.Tensor, residual: torc
         if d != device or residual.dtype is not out.dtype or rows != M or rcols != cols:
             raise RuntimeError(f"{what}: the residual ({residual.dtype} {list(residual.shape)} on {residual.device}) must be like out")
         e.residual = residual.data_ptr()
+
+
+def _copy(epilogue: _lib.Fp4Epilogue) -> _lib.Fp4Epilogue:
+    e = _lib.Fp4Epilogue.from_buffer_copy(epilogue)
+    e.tensors = getattr(epilogue, "tensors", None)
+    return e
 
 
 def gemm_fp4(
@@ -510,7 +530,7 @@ def gemm_fp4(
     if isinstance(epilogue, int):
         e = fp4_epilogue(epilogue, N, out.device, bias=bias, **heads)
     else:
-        e = _lib.Fp4Epilogue.from_buffer_copy(epilogue)
+        e = _copy(epilogue)
     _bind(e, M, N, out, residual, device, "gemm_fp4")
     _launch("gemm_fp4", lib().ff_gemm_fp4, device, *a, *w, fmt, M, N, K, C.byref(e), tile)
 
@@ -534,26 +554,25 @@ def linear_fp4(
 ) -> None:
     """quantize_fp4 of x [M, K] (with the LayerNorm, if gamma is given) and gemm_fp4 in one call; the codes of x live
     in a workspace from torch's allocator on the current stream."""
-    K, device = x.shape[-1], x.get_device()
-    w = _operand(W, W_scales, col_scale, N, K, fmt, device, "linear_fp4")
-    g, b = _vector(gamma, K, device, "linear_fp4: gamma"), _vector(beta, K, device, "linear_fp4: beta")
     e = fp4_epilogue(epilogue, N, x.device, bias=bias, **heads) if isinstance(epilogue, int) else epilogue
-    _linear(x, w, fmt, N, K, g, b, eps, e, out, residual)
+    _linear(x, (W, W_scales, col_scale), fmt, N, x.shape[-1], gamma, beta, eps, e, out, residual)
 
 
-def _linear(x, w, fmt, N, K, gamma, beta, eps, epilogue, out, residual) -> None:
-    """ff_linear_fp4 with the weight's and the norm's addresses."""
-    rc = _calls().linear(x, w, fmt, N, K, gamma, beta, eps, epilogue, out, residual)
+def _linear(x, W, fmt, N, K, gamma, beta, eps, epilogue, out, residual) -> None:
+    """linear_fp4 with the weight's tensors (codes, scales, row scale) and a prepared epilogue."""
+    rc = _calls().linear(x, W, fmt, N, K, gamma, beta, eps, epilogue, out, residual)
     if rc is not None:
         return check(rc, "linear_fp4") if rc else None
     M, cols, ldx, device = _matrix(x, "linear_fp4")
     if device != _current_device():
         with torch.cuda.device(device):
-            return _linear(x, w, fmt, N, K, gamma, beta, eps, epilogue, out, residual)
+            return _linear(x, W, fmt, N, K, gamma, beta, eps, epilogue, out, residual)
     dtype = _DTYPES.get(x.dtype)
     if dtype is None or cols != K:
         raise RuntimeError(f"linear_fp4: x must be fp16, bf16 or f32 [M, {K}], got {x.dtype} {list(x.shape)}")
-    e = _lib.Fp4Epilogue.from_buffer_copy(epilogue)
+    w = _operand(*W, N, K, fmt, device, "linear_fp4")
+    g, b = _vector(gamma, K, device, "linear_fp4: gamma"), _vector(beta, K, device, "linear_fp4: beta")
+    e = _copy(epilogue)
     _bind(e, M, N, out, residual, device, "linear_fp4")
     nbytes = _linear_workspace(M, K, fmt)
     if M == 0:
@@ -561,7 +580,7 @@ def _linear(x, w, fmt, N, K, gamma, beta, eps, epilogue, out, residual) -> None:
     stream = _raw_stream(device)
     ws = _alloc(nbytes, stream)  # torch's stream-ordered cache: free for the stream's next use as soon as the call has returned
     try:
-        rc = lib().ff_linear_fp4(x.data_ptr(), dtype, ldx, gamma, beta, eps, *w, fmt, M, N, K, C.byref(e), ws, nbytes, stream)
+        rc = lib().ff_linear_fp4(x.data_ptr(), dtype, ldx, g, b, eps, *w, fmt, M, N, K, C.byref(e), ws, nbytes, stream)
     finally:
         _free(ws)
     if rc:

@@ -253,3 +253,21 @@ def test_an_output_of_no_columns_is_refused():
         ops._bind(_lib.Fp4Epilogue(kind=_lib.EPI_SWIGLU), 4, 128, out, None, 0, "gemm_fp4")
     with pytest.raises(RuntimeError, match="out is"):
         ops._bind(_lib.Fp4Epilogue(kind=_lib.EPI_BIAS), 4, 128, out, None, 0, "gemm_fp4")
+
+
+def test_a_prepared_epilogue_holds_its_tensors():
+    """Each call reads their addresses anew, so that they may be let go, or move, in between."""
+    import gc
+    import weakref
+
+    bias = _OnGpu(torch.zeros(128))
+    e = ops.fp4_epilogue(_lib.EPI_BIAS, 128, torch.device("cuda", 0), bias=bias)
+    alive = weakref.ref(bias)
+    at = bias.data_ptr()
+    del bias
+    gc.collect()
+    assert alive() is not None and e.bias == at
+    alive()._t = torch.ones(128)
+    copy = ops._copy(e)
+    ops._bind(copy, 4, 128, _OnGpu(torch.zeros(4, 128, dtype=torch.float16)), None, 0, "gemm_fp4")
+    assert copy.bias == alive().data_ptr() != at

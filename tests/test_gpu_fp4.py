@@ -697,3 +697,61 @@ def test_a_nan_column_stays_in_its_column(cuda_device, no_device_error, epilogue
         got = _biases_only(v[:at] + [math.nan] + v[at + 1 :], epilogue, cuda_device)(x)
         keep = torch.arange(good.shape[1], device=cuda_device) != at
         assert torch.isnan(got[:, at]).all() and torch.equal(got[:, keep], good[:, keep])
+
+
+def _layers(device, fmt="nv"):
+    from foidfinder_b200 import fp4
+
+    g = torch.Generator().manual_seed(3)
+    p = lambda n: (1 + 0.1 * torch.randn(n, generator=g)).to(device)  # noqa: E731
+    rope = tuple(t.to(device) for t in _tables(7, 32))
+    w = lambda n: _x(n, 128, torch.float32, n).to(device)  # noqa: E731
+    return [fp4.Fp4Linear(w(96), p(96), fmt=fmt, gamma=p(128), beta=p(128)), fp4.Fp4Linear(w(80), p(80), fmt=fmt, epilogue="swiglu"),
+            fp4.Fp4Linear(w(192), fmt=fmt, epilogue="qkv", norm="layer", rope=rope, q_weight=p(64), k_weight=p(64), q_bias=p(64), k_bias=p(64))]
+
+
+@pytest.mark.parametrize("fmt", ["nv", "mx"])
+def test_layers_can_be_copied_and_stored(cuda_device, no_device_error, fmt):
+    """A copy has tensors of its own: what the first layer's memory holds afterwards does not matter."""
+    import copy
+    import pickle
+
+    x = _x(33, 128, torch.float16, 1).to(cuda_device)
+    for layer in _layers(cuda_device, fmt):
+        ref = layer(x)
+        copies = [copy.deepcopy(layer), pickle.loads(pickle.dumps(layer))]
+        for t in (layer.weight.codes, layer.weight.scales, layer.weight.row_scale, layer.bias, layer.gamma, layer.beta, *layer._heads.values()):
+            if isinstance(t, torch.Tensor):
+                t.zero_()
+        for c in copies:
+            assert torch.equal(c(x), ref)
+
+
+def test_replaced_parameters_count(cuda_device, no_device_error):
+    from foidfinder_b200 import fp4, ops
+
+    d = cuda_device
+    x = _x(33, 128, torch.float16, 1).to(d)
+    layer = _layers(d)[0]
+    before = [layer.weight, layer.bias, layer.gamma, layer.beta]  # kept alive
+    w = _x(96, 128, torch.float32, 5).to(d)
+    bias, gamma, beta = (torch.linspace(a, 2, n, device=d) for a, n in ((0, 96), (1, 128), (-1, 128)))
+    layer.weight, layer.bias, layer.gamma, layer.beta = fp4.quantize(w, "mx"), bias, gamma, beta
+    ref = fp4.Fp4Linear(w, bias, fmt="mx", gamma=gamma, beta=beta)(x)
+    assert torch.equal(layer(x), ref) and layer.fmt == "mx" and layer.bias is bias
+    with pytest.MonkeyPatch.context() as m:  # and the long way
+        m.setattr(ops, "_calls", lambda: ops._NoCalls)
+        assert torch.equal(layer(x), ref)
+    bias.data = torch.zeros(96, device=d)
+    assert torch.equal(layer(x), fp4.Fp4Linear(w, fmt="mx", gamma=gamma, beta=beta)(x))
+    layer.bias = None
+    assert torch.equal(layer(x), fp4.Fp4Linear(w, fmt="mx", gamma=gamma, beta=beta)(x))
+    with pytest.raises(RuntimeError, match="bias"):
+        layer.bias = torch.zeros(95, device=d)
+    layer.gamma = torch.ones(127, device=d)
+    with pytest.raises(RuntimeError, match="gamma"):
+        layer(x)
+    layer.gamma, layer.weight = gamma, fp4.quantize(w[:95])
+    with pytest.raises(RuntimeError, match="the weight is"):
+        layer(x)
+    del before
