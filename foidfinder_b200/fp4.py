@@ -161,7 +161,8 @@ class Fp4Linear:
         self.bias = state["_bias"]
 
     def __call__(self, x: torch.Tensor, out: torch.Tensor | None = None, residual: torch.Tensor | None = None) -> torch.Tensor:
-        """x [M, in_features] -> [M, out_features] (`out`, or a new tensor whose rows start 16 bytes apart or more)."""
+        """x [M, in_features] -> [M, out_features]: `out`, or a new tensor of x's type whose rows start 16 bytes apart or more. Only the
+        bias epilogue writes f32: for an f32 x the others' new tensors are fp16 (give an `out` in bf16 for its range)."""
         w = self.weight
         if x.get_device() != w.codes.get_device():
             raise RuntimeError(f"Fp4Linear: x is on {x.device}, the weight on {w.codes.device}")
@@ -169,7 +170,7 @@ class Fp4Linear:
             raise RuntimeError(f"Fp4Linear: the weight is [{w.rows}, {w.cols}], the layer's [{self.rows}, {self.in_features}]")
         if out is None:
             pitch = (self.out_features + 7) // 8 * 8
-            dtype = torch.float16 if x.dtype == torch.float32 else x.dtype
+            dtype = torch.float16 if x.dtype == torch.float32 and self._kind != _lib.EPI_BIAS else x.dtype
             out = torch.empty(x.shape[0], pitch, dtype=dtype, device=x.device)[:, : self.out_features]
         if out.shape[-1] != self.out_features:
             raise RuntimeError(f"Fp4Linear: out must have {self.out_features} columns, got {list(out.shape)}")

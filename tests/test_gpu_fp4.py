@@ -755,3 +755,15 @@ def test_replaced_parameters_count(cuda_device, no_device_error):
     with pytest.raises(RuntimeError, match="the weight is"):
         layer(x)
     del before
+
+
+def test_f32_values_come_back_in_f32(cuda_device, no_device_error):
+    """Without `out` a layer gives x's type: f32 values beyond fp16 stay finite where the epilogue can write f32."""
+    from foidfinder_b200 import fp4
+
+    d = cuda_device
+    x, w = torch.full((3, 64), 960.0, device=d), torch.full((16, 64), 96.0, device=d)  # 6 x 320 / 2 and 6 x 256 / 16: exact in "nv"
+    y = fp4.Fp4Linear(w)(x)
+    assert y.dtype is torch.float32 and (y == 64 * 960.0 * 96.0).all()
+    assert fp4.Fp4Linear(w)(x.half()).dtype is torch.float16 and fp4.Fp4Linear(w)(x.bfloat16()).dtype is torch.bfloat16
+    assert fp4.Fp4Linear(w, epilogue="gelu")(x).dtype is torch.float16
