@@ -7,7 +7,8 @@ declared in `include/foidfinder_b200.h`. The CUDA runtime is linked statically, 
 only the driver at run time.
 
 `csrc/calls.cpp`, the short way from torch tensors into the calls that are made once per layer, becomes the extension
-module `foidfinder_b200._calls` (host code only, g++ against torch's headers).
+module `foidfinder_b200._calls` (host code only, g++ against torch's headers). Every call works without it, so a machine
+that cannot build it still gets the library, and a warning. It is built again for another version of torch.
 
     python -m foidfinder_b200.build [--force] [--jobs N]
 """
@@ -21,6 +22,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+from importlib.metadata import PackageNotFoundError, version
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -87,14 +89,19 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         os.replace(tmp, LIB)
-    build_calls(force)
+    try:
+        build_calls(force)
+    except (RuntimeError, ImportError, OSError, PackageNotFoundError) as e:
+        CALLS.unlink(missing_ok=True)  # an older one would not fit the sources or torch
+        print(f"foidfinder_b200: {CALLS.name} was not built, calls from Python take their longer way: {e}", file=sys.stderr)
     return LIB
 
 
 def build_calls(force: bool = False) -> Path:
-    """The extension module of csrc/calls.cpp; returns its path."""
-    src = CSRC / "calls.cpp"
-    if force or _stale(CALLS, [src, *INCLUDE.glob("*.h")]):
+    """The extension module of csrc/calls.cpp, for the installed torch; returns its path."""
+    src, stamp, torch_version = CSRC / "calls.cpp", BUILD / "calls.torch", version("torch")
+    if force or _stale(CALLS, [src, *INCLUDE.glob("*.h")]) or not stamp.exists() or stamp.read_text() != torch_version:
+        import torch
         from torch.utils import cpp_extension as torch_paths
 
         cxx = shutil.which("g++") or shutil.which("c++")
@@ -103,11 +110,12 @@ def build_calls(force: bool = False) -> Path:
         include = [f"-I{p}" for p in (*torch_paths.include_paths("cuda"), sysconfig.get_paths()["include"], INCLUDE)]
         libs = [*(f"-L{p}" for p in torch_paths.library_paths("cuda")), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
         tmp = CALLS.with_name(CALLS.name + ".tmp")
-        cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", *include, str(src), "-o", str(tmp), *libs]
+        cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", f'-DFF_TORCH_VERSION="{torch.__version__}"', *include, str(src), "-o", str(tmp), *libs]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"{cxx} failed on {src.name}:\n{r.stdout}\n{r.stderr}")
         os.replace(tmp, CALLS)
+        stamp.write_text(torch_version)
     return CALLS
 
 

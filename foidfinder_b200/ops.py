@@ -8,6 +8,7 @@ take a short way to it (csrc/calls.cpp) where their arguments are plain.
 from __future__ import annotations
 
 import ctypes as C
+import warnings
 from functools import cache
 
 import torch
@@ -333,6 +334,10 @@ def _calls():
     try:
         from . import _calls as module
     except ImportError:
+        return _NoCalls
+    built_for = getattr(module, "built_for", "?")
+    if built_for != torch.__version__:  # it reads torch's C++ objects
+        warnings.warn(f"foidfinder_b200._calls was built for torch {built_for}, not {torch.__version__}; build it with `python -m foidfinder_b200.build`")
         return _NoCalls
     h = lib()
     names = ("ff_quantize_fp4", "ff_dequantize_fp4", "ff_linear_fp4_workspace_bytes", "ff_linear_fp4", "ff_qk_norm_rope")

@@ -271,3 +271,52 @@ def test_a_prepared_epilogue_holds_its_tensors():
     copy = ops._copy(e)
     ops._bind(copy, 4, 128, _OnGpu(torch.zeros(4, 128, dtype=torch.float16)), None, 0, "gemm_fp4")
     assert copy.bias == alive().data_ptr() != at
+
+
+def _build_in(tmp_path, monkeypatch, cxx_status):
+    """foidfinder_b200.build in a folder of its own, with compilers that write an empty file or fail; the commands it ran."""
+    from types import SimpleNamespace
+
+    from foidfinder_b200 import build as B
+
+    ran = []
+
+    def run(cmd, **_):
+        ran.append(cmd[0])
+        ok = cmd[0] == "nvcc" or cxx_status == 0
+        if ok:
+            Path(cmd[cmd.index("-o") + 1]).write_text("")
+        return SimpleNamespace(returncode=0 if ok else cxx_status, stdout="", stderr="no such header")
+
+    for name in ("csrc", "include"):
+        (tmp_path / name).mkdir()
+    (tmp_path / "csrc" / "calls.cpp").write_text("")
+    for name, value in dict(CSRC=tmp_path / "csrc", INCLUDE=tmp_path / "include", BUILD=tmp_path / "o", LIB_DIR=tmp_path / "lib", LIB=tmp_path / "lib" / "l.so",
+                            CALLS=tmp_path / "calls.so", nvcc=lambda: "nvcc", subprocess=SimpleNamespace(run=run), shutil=SimpleNamespace(which=lambda _: "cxx")).items():
+        monkeypatch.setattr(B, name, value)
+    return B, ran
+
+
+def test_the_library_is_built_where_the_extension_module_cannot_be(tmp_path, monkeypatch, capsys):
+    B, ran = _build_in(tmp_path, monkeypatch, 1)
+    B.CALLS.write_text("built from other sources")
+    assert B.build(force=True) == B.LIB and B.LIB.exists() and "cxx" in ran
+    assert not B.CALLS.exists() and "no such header" in capsys.readouterr().err
+
+
+def test_the_extension_module_is_built_again_for_another_torch(tmp_path, monkeypatch):
+    B, ran = _build_in(tmp_path, monkeypatch, 0)
+    assert B.build() == B.LIB and ran.count("cxx") == 1
+    B.build()
+    assert ran.count("cxx") == 1
+    monkeypatch.setattr(B, "version", lambda _: "0.0")
+    B.build()
+    assert ran.count("cxx") == 2
+
+
+def test_an_extension_module_for_another_torch_is_not_used(monkeypatch):
+    load = ops._calls.__wrapped__
+    assert load().built_for == torch.__version__
+    monkeypatch.setattr(torch, "__version__", "0.0")
+    with pytest.warns(UserWarning, match="built for torch"):
+        assert load() is ops._NoCalls
