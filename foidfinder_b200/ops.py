@@ -483,7 +483,7 @@ def _tables(cos: torch.Tensor | None, sin: torch.Tensor | None, half: int, devic
     if cos is None or sin is None or cos.dim() != 2 or cos.shape[0] != half or cos.shape != sin.shape:
         raise RuntimeError(f"{what}: rotation tables must be two [{half}, tokens] tensors")
     n = cos.numel()
-    return _vector(cos, n, device, what), _vector(sin, n, device, what), n // half
+    return _vector(cos, n, device, what), _vector(sin, n, device, what), cos.shape[1]
 
 
 def _bind(e: _lib.Fp4Epilogue, M: int, N: int, out: torch.Tensor, residual: torch.Tensor | None, device: int, what: str) -> None:

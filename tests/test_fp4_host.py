@@ -320,3 +320,11 @@ def test_an_extension_module_for_another_torch_is_not_used(monkeypatch):
     monkeypatch.setattr(torch, "__version__", "0.0")
     with pytest.warns(UserWarning, match="built for torch"):
         assert load() is ops._NoCalls
+
+
+def test_tables_of_no_angles():
+    """Heads of no columns are left to the library's check, which names them."""
+    t = _OnGpu(torch.zeros(0, 5))
+    assert ops._tables(t, t, 0, 0, "qk_norm_rope")[2] == 5
+    args = (FAKE, 0, 128, FAKE, 128, 4, 1, 1, 0, 1, FAKE, None, FAKE, None, 1e-6, FAKE, FAKE, 5, 0, None)
+    assert _lib.lib().ff_qk_norm_rope(*args) == BAD and "head_dim 0" in _err()
