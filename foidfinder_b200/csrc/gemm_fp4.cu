@@ -840,6 +840,8 @@ int gemm_fp4(const Fp4Operand& A, const Fp4Operand& W, int fmt, int M, int N, in
   FF_REQUIRE(epi != EPI_SWIGLU || out_cols <= N / 2, "ff_gemm_fp4: SwiGLU writes at most N / 2 columns (out_cols=%d, N=%d)",
              out_cols, N);
   FF_REQUIRE(e->ldo >= out_cols, "ff_gemm_fp4: output row stride %lld for %d columns", static_cast<long long>(e->ldo), out_cols);
+  // A single row is never stepped over: any stride will do, rounded up to what the tensor maps take.
+  const int64_t ldo = M == 1 ? (e->ldo + 7) / 8 * 8 : e->ldo, ldr = M == 1 ? (e->ldr + 7) / 8 * 8 : e->ldr;
   if (epi == EPI_QKV_NORM_ROPE) {
     FF_REQUIRE(e->norm == FF_NORM_RMS || e->norm == FF_NORM_LAYER, "ff_gemm_fp4: unknown head norm %d", e->norm);
     FF_REQUIRE(e->q_heads >= 0 && e->k_heads >= 0 && N % 64 == 0 && static_cast<int64_t>(e->q_heads) + e->k_heads <= N / 64,
@@ -854,9 +856,9 @@ int gemm_fp4(const Fp4Operand& A, const Fp4Operand& W, int fmt, int M, int N, in
   FF_REQUIRE(aligned16(A.codes) && aligned16(A.scales) && aligned16(W.codes) && aligned16(W.scales),
              "ff_gemm_fp4: codes and scales must be 16-byte aligned");
   const bool f32 = e->out_dtype == FF_F32;
-  FF_REQUIRE(f32 || (aligned16(e->out) && e->ldo % 8 == 0), "ff_gemm_fp4: 16-bit outputs need 16-byte aligned rows (ldo %% 8 == 0)");
+  FF_REQUIRE(f32 || (aligned16(e->out) && ldo % 8 == 0), "ff_gemm_fp4: 16-bit outputs need 16-byte aligned rows (ldo %% 8 == 0)");
   FF_REQUIRE(!f32 || reinterpret_cast<uintptr_t>(e->out) % 4 == 0, "ff_gemm_fp4: out is not aligned to its type");
-  FF_REQUIRE(epi != EPI_RESIDUAL || (aligned16(e->residual) && e->ldr % 8 == 0), "ff_gemm_fp4: residual rows must be 16-byte aligned");
+  FF_REQUIRE(epi != EPI_RESIDUAL || (aligned16(e->residual) && ldr % 8 == 0), "ff_gemm_fp4: residual rows must be 16-byte aligned");
 
   const bool pair = tile == FF_TILE_PAIR256 || (tile == 0 && epi != EPI_QKV_NORM_ROPE && choose_pair_fp4(M, N, K));
   Fp4Maps t;
@@ -872,13 +874,13 @@ int gemm_fp4(const Fp4Operand& A, const Fp4Operand& W, int fmt, int M, int N, in
     const bool narrow = epi == EPI_SWIGLU;  // 32 output columns per warp
     // whole 16-byte granules only (none: a map that no store uses); the kernel writes the rest of a row itself
     rc = make_tmap_2d_pitched(&t.c, e->out, dt, 2, static_cast<uint64_t>(out_cols < 8 ? 8 : out_cols & ~7), static_cast<uint64_t>(M),
-                              static_cast<uint64_t>(e->ldo) * 2, narrow ? 32 : 64, 32,
+                              static_cast<uint64_t>(ldo) * 2, narrow ? 32 : 64, 32,
                               narrow ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != FF_OK) return rc;
   }
   if (epi == EPI_RESIDUAL) {
     rc = make_tmap_2d_pitched(&t.r, e->residual, dt, 2, static_cast<uint64_t>(N), static_cast<uint64_t>(M),
-                              static_cast<uint64_t>(e->ldr) * 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+                              static_cast<uint64_t>(ldr) * 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != FF_OK) return rc;
   }
   Fp4GemmArgs a{};
@@ -893,7 +895,7 @@ int gemm_fp4(const Fp4Operand& A, const Fp4Operand& W, int fmt, int M, int N, in
   a.col_scale = W.row_scale;
   a.bias = e->bias;
   a.out = e->out;
-  a.ldo = e->ldo;
+  a.ldo = ldo;
   a.out_cols = out_cols;
   a.tma_cols = out_cols & ~7;
   a.norm = e->norm;

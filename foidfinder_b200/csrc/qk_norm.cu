@@ -182,13 +182,13 @@ extern "C" int ff_qk_norm_rope(const void* x, int dtype, int64_t ldx, void* out,
   FF_REQUIRE(rows >= 0 && rows <= (1 << 30) && q_heads >= 0 && k_heads >= 0 && q_heads <= (1 << 16) && k_heads <= (1 << 16) && tokens >= 1,
              "ff_qk_norm_rope: bad shape rows=%d heads=%d+%d tokens=%d", rows, q_heads, k_heads, tokens);
   const int64_t cols = static_cast<int64_t>(q_heads + k_heads) * head_dim;
-  FF_REQUIRE(ldx >= cols && ldo >= cols && ldx % 8 == 0 && ldo % 8 == 0,
+  FF_REQUIRE(ldx >= cols && ldo >= cols && (rows <= 1 || (ldx % 8 == 0 && ldo % 8 == 0)),  // a single row is never stepped over
              "ff_qk_norm_rope: row strides %lld and %lld must hold %lld columns and be multiples of 8",
              static_cast<long long>(ldx), static_cast<long long>(ldo), static_cast<long long>(cols));
   if (rows == 0 || cols == 0) return FF_OK;
   FF_REQUIRE(x && out && rope_cos && rope_sin && (q_w || q_heads == 0) && (k_w || k_heads == 0), "ff_qk_norm_rope: NULL pointer");
   FF_REQUIRE(aligned16(x) && aligned16(out), "ff_qk_norm_rope: x and out must be 16-byte aligned");
-  FF_REQUIRE(x != out || ldx == ldo, "ff_qk_norm_rope: in place needs equal row strides");
+  FF_REQUIRE(x != out || ldx == ldo || rows == 1, "ff_qk_norm_rope: in place needs equal row strides");
   const QkArgs a{x, ldx, out, ldo, rows, q_heads, k_heads, q_w, q_b, k_w, k_b, eps, rope_cos, rope_sin, tokens};
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == FF_F16)

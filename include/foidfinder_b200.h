@@ -164,7 +164,7 @@ int64_t ff_fp4_code_bytes(int rows, int cols);
 int64_t ff_fp4_scale_bytes(int rows, int cols, int fmt);
 
 /*
- * x [rows, cols] of type dtype (FF_F16, FF_BF16, FF_F32), row stride ldx elements (any), -> (LayerNorm over the
+ * x [rows, cols] of type dtype (FF_F16, FF_BF16, FF_F32), row stride ldx >= cols elements, -> (LayerNorm over the
  * row with gamma/beta/eps when gamma != NULL, f32 statistics) -> codes, scales and, for FF_FP4_NV,
  * row_scale [rows] (unused and may be NULL for FF_FP4_MX). Any rows >= 0 and cols in [1, 2^24].
  */
@@ -188,7 +188,7 @@ int ff_dequantize_fp4(const uint8_t* codes, const uint8_t* scales, const float* 
  *                         rotated by the angles of position m % tokens (rope_cos / rope_sin [32, tokens],
  *                         angle-major); the columns after them (v) are out = y
  * Any M, N, K >= 1 (FF_EPI_SWIGLU: N % 32 == 0; FF_EPI_QKV_NORM_ROPE: N % 64 == 0). 16-bit out and residual:
- * 16-byte aligned, row strides (elements) multiples of 8. f32 out: any row stride. bias may be NULL.
+ * 16-byte aligned, row strides (elements) multiples of 8 (unless M is 1). f32 out: any row stride. bias may be NULL.
  * tile: 0 = automatic, 128 = 128 x 128 tiles per CTA, FF_TILE_PAIR256 = 256 x 256 tiles per pair of CTAs (not for
  * FF_EPI_QKV_NORM_ROPE).
  */
@@ -230,7 +230,8 @@ int ff_linear_fp4(const void* x, int dtype, int64_t ldx, const float* gamma, con
  * pairs rotated by the angles of position row % tokens: rope_cos / rope_sin [head_dim / 2, tokens] f32,
  * angle-major. pairing FF_ROPE_PAIRS: pair i is columns (2i, 2i + 1); FF_ROPE_HALVES: (i, i + head_dim / 2).
  * out [rows, (q_heads + k_heads) * head_dim], row stride ldo; out may be x itself (ldo == ldx). head_dim 32, 64,
- * 128 or 256; x and out 16-byte aligned with row strides that are multiples of 8. No reference counterpart.
+ * 128 or 256; x and out 16-byte aligned with row strides that are multiples of 8 (unless rows is 1). No reference
+ * counterpart.
  */
 #define FF_ROPE_PAIRS 0
 #define FF_ROPE_HALVES 1

@@ -767,3 +767,25 @@ def test_f32_values_come_back_in_f32(cuda_device, no_device_error):
     assert y.dtype is torch.float32 and (y == 64 * 960.0 * 96.0).all()
     assert fp4.Fp4Linear(w)(x.half()).dtype is torch.float16 and fp4.Fp4Linear(w)(x.bfloat16()).dtype is torch.bfloat16
     assert fp4.Fp4Linear(w, epilogue="gelu")(x).dtype is torch.float16
+
+
+def test_a_single_row_may_have_any_stride(cuda_device, no_device_error):
+    from foidfinder_b200 import fp4, ops
+
+    d = cuda_device
+    x, w = _x(1, 100, torch.float16, 1).to(d), _x(45, 100, torch.float32, 2).to(d)
+    r = _x(1, 45, torch.float16, 3).to(d)
+    for epilogue, residual in (("bias", None), ("residual", r)):
+        layer = fp4.Fp4Linear(w, epilogue=epilogue)
+        wide = None if residual is None else torch.cat([r, r], 1)[:, :48].contiguous()[:, :45]
+        ref = layer(x, residual=wide)
+        buf = torch.full((60,), 77.0, dtype=torch.float16, device=d)
+        assert torch.equal(layer(x, out=buf[:45].view(1, 45), residual=residual), ref)
+        assert (buf[45:] == 77.0).all()
+    t, hw = torch.linspace(0, 1, 16 * 3, device=d).view(16, 3), torch.ones(32, device=d)
+    args = dict(q_heads=1, k_heads=1, head_dim=32, norm="rms", q_weight=hw, k_weight=hw, rope_cos=t, rope_sin=t)
+    ref = torch.empty(1, 64, dtype=torch.float16, device=d)
+    ops.qk_norm_rope(x[:, :96], ref, **args)  # x: 100 elements from row to row
+    narrow = x[:, :96].contiguous()
+    ops.qk_norm_rope(narrow, narrow[:, :64], **args)
+    assert torch.equal(narrow[:, :64], ref) and torch.equal(narrow[:, 64:], x[:, 64:96])
