@@ -622,8 +622,10 @@ int dispatch_quant(const QuantArgs& a, cudaStream_t stream) {
   }
   if constexpr (!MX || NORM) {
     const int wpr2 = (cols + 1023) / 1024, wpr3 = (cols + 1535) / 1536;
-    // two or three pieces per lane, whichever leaves fewer lanes idle; three where that is even (fewer warps to join)
-    const bool three = 3 * wpr3 <= 2 * wpr2;
+    // two or three pieces per lane, whichever leaves fewer lanes idle; three where that is even (fewer warps to join) and
+    // where two need more warps than a CTA has (8000 x 9500 fp16 behind a LayerNorm 108 us, 618 as a row too wide for
+    // registers; f32 without one 72 and 111)
+    const bool three = 3 * wpr3 <= 2 * wpr2 || wpr2 > kQuantThreads / 32;
     const int wpr = three ? wpr3 : wpr2;
     if constexpr (sizeof(T) == 2 && NORM) {
       if (wpr == 1)

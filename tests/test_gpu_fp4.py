@@ -789,3 +789,29 @@ def test_a_single_row_may_have_any_stride(cuda_device, no_device_error):
     narrow = x[:, :96].contiguous()
     ops.qk_norm_rope(narrow, narrow[:, :64], **args)
     assert torch.equal(narrow[:, :64], ref) and torch.equal(narrow[:, 64:], x[:, 64:96])
+
+
+@pytest.mark.parametrize("fmt", ["nv", "mx"])
+@pytest.mark.parametrize(("cols", "dtype"), [(8193, torch.float32), (9500, torch.float16), (9500, torch.float32), (11000, torch.bfloat16), (12288, torch.float16)])
+def test_rows_that_fit_registers_stay_there(cuda_device, no_device_error, cols, dtype, fmt):
+    """Up to 12288 columns a CTA's lanes hold the row (two or three pieces each); wider rows are read again for each step."""
+    from foidfinder_b200 import fp4
+
+    x = _x(5, cols, dtype, cols)
+    xd = x.to(cuda_device)
+    if dtype is torch.float32:
+        _check_exact(fp4.quantize(xd, fmt), x)
+    g = torch.Generator().manual_seed(9)
+    gamma, beta = 1 + 0.1 * torch.randn(cols, generator=g), 0.1 * torch.randn(cols, generator=g)
+    kw = dict(gamma=gamma.to(cuda_device), beta=beta.to(cuda_device), eps=1e-5)
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as prof:
+        q = fp4.quantize(xd, fmt, **kw)
+        torch.cuda.synchronize()
+    names = [e.key for e in prof.key_averages() if "quantize_fp4" in e.key]
+    assert not any("wide" in n for n in names), names  # none where the profiler is not available
+    codes, s, row = _read(q)
+    ec, es, er = O.quantize(O.layer_norm(x, gamma, beta, 1e-5), fmt)
+    nb = es.shape[1]
+    assert torch.equal(row, er)
+    assert (s[:, :nb].int() - es.int()).abs().max() <= 1 and (s[:, :nb] != es).float().mean() <= 1e-3
+    assert s[:, nb:].count_nonzero() == 0 and (codes != ec).float().mean() <= 1e-3
