@@ -22,8 +22,7 @@
 // columns), which delivers 8 bytes of gamma and beta per value. What did not help: two rows at a time for the same gamma
 // and beta (38.9 us and 140: half the warps), half a row per warp with two rows (43 and 172: barriers), the next row read
 // ahead into shared memory (50 and 148), 32-byte loads (37.6 and 148), gamma and beta in registers (73) or TMEM (78).
-// Dequantisation, 65600 x 1024 fp16 30 us (5.7 TB/s), 32000 x 4096 f32 100 us; 65600 x 2730 bf16 89 us aligned, 105 not. A kernel that only reads
-// and writes the same bytes takes 33 and 80.
+// Dequantisation, 65600 x 1024 fp16 30 us (5.7 TB/s), 32000 x 4096 f32 100 us; 65600 x 2730 bf16 89 us aligned, 105 not.
 #include <algorithm>
 #include <type_traits>
 
@@ -155,14 +154,22 @@ __device__ __forceinline__ float nv_row_scale(float amax) {
 }
 __device__ __forceinline__ float inv_pow2(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
 
-// v / (S s) for the code, r about 1 / (S s). kExact16: v came from a 16-bit type, so a quotient that is no
-// rounding tie of e2m1 is at least 2^-13 away from one, while v * r is within 2^-20 of the quotient: rounding
-// v * r + 192 (one FMA, to multiples of 2^-16) puts true ties exactly on the tie (r within 2^-22 of 1 / (S s)
-// is enough). kExact32: v from f32 and already divided by s (exact, or far below any tie), r the reciprocal of scale = S: the remainder of
-// v * r, exact in an FMA, corrects it to within a hair of the true quotient's rounding. A quotient that equals a tie
-// comes out as the tie; any other is at least 1.06 * 2^-24 of itself away from one (v's last bit against at most 1.875
-// of scale), more than half a unit in the last place, and does not. kPlain: v is itself rounded (after a LayerNorm) or r
-// a power of two.
+// v / (S s) for the code, r about 1 / (S s). A code's ties are T = 0.25, 0.75, 1.25, 1.75, 2.5, 3.5 and 5; S has four
+// significant bits, so T S s is representable in every input type, and a quotient is a tie only if v is T S s.
+// kExact16: v came from a 16-bit type, so v and T S s differ in their first 11 bits if at all: a quotient that is no tie is
+//   at least 2^-11 T, that is 2^-13, away from one, while v * r is within 2^-20 of the quotient. Rounding v * r + 192 (one
+//   FMA, to multiples of 2^-16) puts true ties exactly on the tie and moves no other across (r within 2^-22 of 1 / (S s) is
+//   enough).
+// kExact32: v from f32 and already divided by s (exact, or far below any tie), r the reciprocal of scale = S. The quotient
+//   v * r is corrected by its remainder, which is exact in an FMA (P. Markstein, Computation of elementary functions on the
+//   IBM RISC System/6000 processor, IBM J. Res. Dev. 34, 1990): before its rounding the result is within 2^-45 of the true
+//   quotient Q. With Q = T it rounds to T. Otherwise |Q - T| is at least u / S, u the unit in the last place of T S. Let a and
+//   b be the significands of T and S, in [1, 2), and h half the unit in the last place of T (a <= 1.75). Above T,
+//   u / S = 2 h / b where a b < 2 and 4 h / b where not: for a = 1 (T = 0.25) at least 2 h / 1.875 = 1.067 h, for a = 1.25
+//   (b <= 1.5) 1.33 h, for 1.5 (b <= 1.25) 1.6 h, for 1.75 (b <= 1.125) 1.78 h. Below T it is the same, but for T = 0.25,
+//   where h is half as large, and T S a power of two (a = b = 1), where both are: 2 h at least. Always more than h, so the
+//   result rounds to T's neighbour or beyond.
+// kPlain: v is itself rounded (after a LayerNorm) or r a power of two.
 enum QuotientKind { kPlain, kExact16, kExact32 };
 template <int KIND>
 __device__ __forceinline__ float2 quotient2(float2 v, float r, float scale) {
@@ -184,8 +191,9 @@ __device__ __forceinline__ uint2 codes16(const float2 (&v)[8], float r, float sc
   return make_uint2(e2m1x8(q), e2m1x8(q + 4));
 }
 
-// amax / 6, rounded correctly: the remainder of the product with 1 / 6 corrects it, so that ties of e4m3 come out
-// exact and no other value moves onto one.
+// amax / 6, its product with 1 / 6 corrected by the remainder in the same way. Ties of e4m3 have five significant bits: a
+// quotient that is one comes out as it is. Any other is u / 6 away at least, u the unit in the last place of 6 T:
+// 4/3 of half the unit in the last place of T (significand below 4/3) or 8/3 (above), and does not move onto it.
 __device__ __forceinline__ float sixth(float a) {
   const float q = a * (1.f / 6.f);
   return fmaf(fmaf(-6.f, q, a), 1.f / 6.f, q);
@@ -199,7 +207,7 @@ __device__ __forceinline__ uint32_t nv_piece(const float2 (&v)[8], float amax, f
   const float S = e4m3_value(byte);
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(S));
-  r = fmaf(r, fmaf(-S, r, 1.f), r);  // to the last bit
+  r = fmaf(r, fmaf(-S, r, 1.f), r);  // one step of Newton's method
   if constexpr (KIND == kExact32) {
     float2 u[8];
 #pragma unroll

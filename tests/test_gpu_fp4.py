@@ -815,3 +815,55 @@ def test_rows_that_fit_registers_stay_there(cuda_device, no_device_error, cols, 
     assert torch.equal(row, er)
     assert (s[:, :nb].int() - es.int()).abs().max() <= 1 and (s[:, :nb] != es).float().mean() <= 1e-3
     assert s[:, nb:].count_nonzero() == 0 and (codes != ec).float().mean() <= 1e-3
+
+
+TIES = [0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0]
+
+
+def _ulps(v, n, dtype):
+    """The n-th neighbours (above for n > 0) of the positive values v of type dtype."""
+    bits = {torch.float32: torch.int32}.get(dtype, torch.int16)
+    return (v.to(dtype).view(bits) + n).view(dtype)
+
+
+@pytest.mark.parametrize(("dtype", "exponents"), [(torch.float32, (-100, -40, -3, 0, 1, 60, 115)), (torch.float16, (-4, 0, 3)), (torch.bfloat16, (-100, -7, 0, 100))])
+def test_every_tie_of_every_block_scale(cuda_device, no_device_error, dtype, exponents):
+    """All 7 ties times all 126 block scales, and the values next to them on either side, of either sign."""
+    from foidfinder_b200 import fp4
+
+    scales = O.e4m3_grid()[1:]
+    v = torch.tensor(TIES, dtype=torch.float64)[None] * scales[:, None]  # [126, 7], exact in every type
+    assert torch.equal(v.to(dtype).double(), v)
+    v = torch.stack([_ulps(v, n, dtype) for n in (-1, 0, 1)], 2).reshape(126, 21).double()
+    blocks = torch.zeros(126, 2, 16, dtype=torch.float64)
+    blocks[:, :, 0] = 6 * scales[:, None]  # the block's largest value: its scale comes out exactly
+    blocks[:, 0, 1:] = v[:, :15]
+    blocks[:, 1, 1:7] = v[:, 15:]
+    blocks[:, 1, 7:] = v[:, :9]
+    sign = torch.where(torch.rand(126, 2, 16, generator=torch.Generator().manual_seed(1)) < 0.5, -1.0, 1.0)
+    rows = torch.zeros(17, 16, 16, dtype=torch.float64)
+    rows[:, 0, 0] = 2688  # the row's largest value: row scale 1
+    flat = (blocks * sign).reshape(252, 16)
+    rows[:, 1:] = torch.cat([flat, flat[:3]]).view(17, 15, 16)
+    x = torch.cat([rows.view(17, 256) * 2.0**e for e in exponents])
+    low = x.to(dtype)
+    if dtype is not torch.float16:  # fp16 runs out of exponents for the smallest ties: those are rounded, all others exact
+        assert torch.equal(low.double(), x)
+    _check_exact(fp4.quantize(low.to(cuda_device), "nv"), low)
+
+
+@pytest.mark.parametrize("exponent", [-100, -20, 0, 90])
+def test_block_maxima_next_to_the_ties_of_scales(cuda_device, no_device_error, exponent):
+    """f32 block maxima that are 6 times a midpoint between two block scales, all 126 of them, or next to it."""
+    from foidfinder_b200 import fp4
+
+    grid = O.e4m3_grid()
+    mid = 6 * (grid[:-1] + grid[1:]) / 2
+    top = torch.stack([_ulps(mid, n, torch.float32) for n in (-1, 0, 1)], 1).double().reshape(-1)  # 378
+    blocks = torch.rand(378, 16, generator=torch.Generator().manual_seed(2), dtype=torch.float64) * top[:, None] * 0.99
+    blocks[:, 5] = -top
+    rows = torch.zeros(27, 15, 16, dtype=torch.float64)
+    rows[:, 0, 0] = 2688
+    rows[:, 1:] = blocks.view(27, 14, 16)
+    x = (rows.view(27, 240) * 2.0**exponent).float()
+    _check_exact(fp4.quantize(x.to(cuda_device), "nv"), x)
