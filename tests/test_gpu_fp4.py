@@ -867,3 +867,57 @@ def test_block_maxima_next_to_the_ties_of_scales(cuda_device, no_device_error, e
     rows[:, 1:] = blocks.view(27, 14, 16)
     x = (rows.view(27, 240) * 2.0**exponent).float()
     _check_exact(fp4.quantize(x.to(cuda_device), "nv"), x)
+
+
+@pytest.mark.parametrize("fmt", ["nv", "mx"])
+@pytest.mark.parametrize(("tile", "epi", "N", "K", "dtype"), [
+    (128, "bias", 4203, 320, torch.float32), (512, "bias", 4203, 320, torch.float32),
+    (128, "bias", 4203, 320, torch.float16), (512, "bias", 4203, 1300, torch.bfloat16),
+    (128, "gelu", 4200, 70, torch.bfloat16), (512, "gelu", 4200, 320, torch.float16),
+    (128, "residual", 4203, 1300, torch.float16), (512, "residual", 4203, 320, torch.bfloat16),
+    (128, "swiglu", 4202, 320, torch.bfloat16), (512, "swiglu", 4202, 320, torch.float16), (512, "swiglu", 4202, 1300, torch.bfloat16),
+    (128, "qkv rms", 4224, 320, torch.float16), (128, "qkv layer", 4224, 1300, torch.bfloat16),
+])
+def test_products_of_many_tiles(cuda_device, no_device_error, tile, epi, N, K, dtype, fmt):
+    """9 tiles or more for every CTA pair and 17 for every CTA of 148: both accumulators, the columns that they share, and
+    every ring of buffers are used again and again, with partial last tiles both ways. Equal to the last bit to the same
+    rows multiplied 250 at a time, where no CTA has a second tile (those are compared with the oracle above)."""
+    from foidfinder_b200 import fp4, ops
+
+    d = cuda_device
+    M, part = 10000, 250
+    g = torch.Generator().manual_seed(7)
+    x, w = _x(M, K, torch.float16, 1).to(d), (torch.randn(N, K, generator=g) * 0.05).to(d)
+    bias = (torch.randn(N, generator=g) * 0.1).to(d)
+    kind = {"bias": ops.EPI_BIAS, "gelu": ops.EPI_GELU, "residual": ops.EPI_RESIDUAL, "swiglu": ops.EPI_SWIGLU}.get(epi, ops.EPI_QKV_NORM_ROPE)
+    cols, kw = N, {}
+    if epi == "swiglu":
+        layer = fp4.Fp4Linear(w, bias, fmt=fmt, epilogue="swiglu")
+        W, bias, cols = layer.weight, layer.bias, N // 2
+    else:
+        W = fp4.quantize(w, fmt)
+    period = part
+    if epi.startswith("qkv"):
+        hw = [(1 + 0.1 * torch.randn(64, generator=g)).to(d) for _ in range(4)]
+        cos, sin = (t.to(d) for t in _tables(period, 32))  # positions start again with every part
+        kw = dict(norm=epi[4:], q_heads=30, k_heads=18, q_weight=hw[0], k_weight=hw[1], rope_cos=cos, rope_sin=sin)
+        kw |= dict(q_bias=hw[2], k_bias=hw[3]) if epi == "qkv layer" else {}
+    residual = torch.randn(M, cols, generator=g).to(dtype).to(d) if epi == "residual" else None
+
+    def product(rows, out):
+        q = fp4.quantize(x[rows], fmt)
+        if residual is not None:
+            out.copy_(residual[rows])  # in place
+        ops.gemm_fp4(q.codes, q.scales, q.row_scale, W.codes, W.scales, W.row_scale, out, kind, FMT[fmt], N=W.rows, K=K, bias=bias,
+                     residual=None if residual is None else out, tile=tile, **kw)
+
+    pitch = (cols + 7) // 8 * 8 + 8
+    buf = torch.full((M + 8, pitch), 77.0, dtype=dtype, device=d)
+    ref = torch.full((M, pitch), 77.0, dtype=dtype, device=d)[:, :cols]
+    for first in range(0, M, part):
+        product(slice(first, first + part), ref[first : first + part])
+    for _ in range(3):
+        buf.fill_(77.0)
+        product(slice(0, M), buf[:M, :cols])
+        assert torch.equal(buf[:M, :cols], ref)
+    assert (buf[M:] == 77.0).all() and (buf[:, cols:] == 77.0).all()
