@@ -921,3 +921,36 @@ def test_products_of_many_tiles(cuda_device, no_device_error, tile, epi, N, K, d
         product(slice(0, M), buf[:M, :cols])
         assert torch.equal(buf[:M, :cols], ref)
     assert (buf[M:] == 77.0).all() and (buf[:, cols:] == 77.0).all()
+
+
+@pytest.mark.parametrize("pairing", ["pairs", "halves"])
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+@pytest.mark.parametrize(("rows", "qh", "kh", "dim", "tokens", "dtype"), [
+    (50, 64, 16, 128, 7, torch.bfloat16),  # few rows: a warp for every chunk of heads
+    (5, 9, 7, 256, 3, torch.float16),  # the same, chunks that are not full
+    (3000, 20, 12, 128, 1025, torch.float16),  # four warps take turns with a row's five chunks
+    (7500, 9, 5, 128, 1025, torch.bfloat16),  # a warp per row, several rows per warp, three chunks of both kinds
+    (15000, 3, 2, 32, 577, torch.float16),  # the same, one chunk of each kind
+])
+def test_qk_norm_rope_of_many_heads_and_rows(cuda_device, no_device_error, rows, qh, kh, dim, tokens, dtype, norm, pairing):
+    from foidfinder_b200 import ops
+
+    d = cuda_device
+    cols = (qh + kh) * dim
+    x = (_x(rows, cols + 8, torch.float32, rows, outliers=False) * 1.5).to(dtype)
+    g = torch.Generator().manual_seed(4)
+    qw, kw = 1 + 0.1 * torch.randn(dim, generator=g), 1 + 0.1 * torch.randn(dim, generator=g)
+    qb, kb = (0.1 * torch.randn(dim, generator=g), 0.1 * torch.randn(dim, generator=g)) if norm == "layer" else (None, None)
+    cos, sin = _tables(tokens, dim // 2)
+    dev = lambda t: None if t is None else t.to(d)  # noqa: E731
+    args = dict(q_heads=qh, k_heads=kh, head_dim=dim, norm=norm, q_weight=dev(qw), k_weight=dev(kw), q_bias=dev(qb), k_bias=dev(kb), eps=1e-6,
+                rope_cos=dev(cos), rope_sin=dev(sin), pairing=pairing)
+    out = torch.full((rows, cols + 16), 77.0, device=d, dtype=dtype)
+    xd = x.to(d)
+    ops.qk_norm_rope(xd, out, **args)
+    ref = torch.cat([O.heads(x[:, : qh * dim], qh, dim, qw, qb, norm, 1e-6, cos, sin, pairing),
+                     O.heads(x[:, qh * dim : cols], kh, dim, kw, kb, norm, 1e-6, cos, sin, pairing)], 1)
+    _close(out[:, :cols], ref, 2.0**-20 * torch.full_like(ref, 10.0), dtype)  # as in test_qk_norm_rope
+    assert (out[:, cols:] == 77.0).all()
+    ops.qk_norm_rope(xd, xd, **args)
+    assert torch.equal(xd[:, :cols], out[:, :cols]) and torch.equal(xd[:, cols:].cpu(), x[:, cols:])
