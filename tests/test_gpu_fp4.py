@@ -954,3 +954,15 @@ def test_qk_norm_rope_of_many_heads_and_rows(cuda_device, no_device_error, rows,
     assert (out[:, cols:] == 77.0).all()
     ops.qk_norm_rope(xd, xd, **args)
     assert torch.equal(xd[:, :cols], out[:, :cols]) and torch.equal(xd[:, cols:].cpu(), x[:, cols:])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("cols", [511, 512, 513, 1024, 1025, 1537, 2048, 2049, 3071, 3073, 4096, 4097, 5120, 5121])
+def test_quantize_at_the_widths_where_variants_change(cuda_device, no_device_error, cols, dtype):
+    from foidfinder_b200 import fp4
+
+    x = _x(9, cols, dtype, cols)
+    _check_exact(fp4.quantize(x.to(cuda_device), "nv"), x)
+    wide = torch.full((9, (cols + 15) // 8 * 8), math.nan, dtype=dtype, device=cuda_device)[:, :cols]  # rows on 16-byte boundaries
+    wide.copy_(x)
+    _check_exact(fp4.quantize(wide, "nv"), x)
