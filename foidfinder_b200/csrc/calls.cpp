@@ -1,7 +1,7 @@
 // The short way from Python into the calls that are made once per layer, some of them for a single row: tensors are read
 // through torch's C++ interface and the kernels' library is called directly. Through ctypes and Python's tensor attributes a
-// quantisation of one row takes 6.7 us, a linear layer 12 and a head norm 8.6; this way 2.9, 6.5 and 2.9, of which 2.3,
-// 4.5 and 2.3 are the launches.
+// quantisation of one row takes 6.7 us, a linear layer 12 and a head norm 8.6; this way 2.9, 6.5 to 7.1 and 2.9, of which
+// 2.3, 4.5 and 2.3 are the launches.
 //
 // Every function takes what its namesake in ops.py takes and returns the library's status, or None for anything that is
 // not plain (a wrong type, shape, stride or device, a subclass, no memory): the caller then goes the long way, which has

@@ -18,11 +18,11 @@
 //
 // Measured, 65600 rows of 1024 fp16 (171 MB moved): NV 27.5 us, 95% of the copy rate, MX 26.7. 65600 x 2730 bf16: MX
 // 72 us where rows start at 16-byte boundaries and 84 where they do not (shifting them into place doubles the
-// instructions); NV 73 and 85. With LayerNorm 38 us and 125 (2730): bound by the shared-memory pipe (88% busy at 1024
+// instructions); NV 71 and 85. With LayerNorm 38 us and 126 (2730): bound by the shared-memory pipe (88% busy at 1024
 // columns), which delivers 8 bytes of gamma and beta per value. What did not help: two rows at a time for the same gamma
 // and beta (38.9 us and 140: half the warps), half a row per warp with two rows (43 and 172: barriers), the next row read
 // ahead into shared memory (50 and 148), 32-byte loads (37.6 and 148), gamma and beta in registers (73) or TMEM (78).
-// Dequantisation, 65600 x 1024 fp16 30 us (5.7 TB/s), 32000 x 4096 f32 100 us; 65600 x 2730 bf16 89 us aligned, 105 not.
+// Dequantisation, 65600 x 1024 fp16 30 us (5.7 TB/s), 32000 x 4096 f32 102 us; 65600 x 2730 bf16 89 us aligned, 105 not.
 #include <algorithm>
 #include <type_traits>
 

@@ -15,12 +15,13 @@
 // of A, half of W's 256 rows and all of the tile's W scales (each SM's tensor core reads them from its own
 // TMEM), and shared memory moves half as many bytes per multiply-add.
 //
-// Measured, FF_FP4_NV unless said: 8192^3 191 us (5.8 PFLOP/s, 3.5 times the bf16 rate of the same GPU), bound by the
-// tensor cores. 65600 x 5504 x 1024 with SwiGLU 209 us (3.5 PFLOP/s), where reading the accumulators, activating and
-// storing takes about as long as the products do: 190 us without the column parameters, 183 without the stores, 159
-// with the MMAs alone. 65600 x 1024 x 2730 with a residual 100 us; 65600 x 1024 x 1024 44 us, bound by the 200 MB moved.
-// 8200 x 2304 x 768 with norm and rotation 26.5 us, bound by its epilogue (21 without the reads of the angles). One row
-// of 1024 against 30877: 8 us, the latency of a launch and of two tiles.
+// Measured, FF_FP4_NV unless said, from rest: 8192^3 195 us (5.6 PFLOP/s, 3.4 times the bf16 rate of the same GPU; FF_FP4_MX
+// 185), under the power cap, the tensor pipe active 69% of the cycles at 4096 x 4096 x 8192. 65600 x 5504 x 1024 with SwiGLU
+// 205 us (3.6 PFLOP/s), where reading the accumulators, activating and storing takes about as long as the products do (when it
+// took 209: 190 without the column parameters, 183 without the stores, 159 with the MMAs alone); launched without a pause the
+// power cap lowers the SM clock to 1.52 GHz and it takes 247. 65600 x 1024 x 2730 with a residual 100 us (118 at 1.35 GHz);
+// 65600 x 1024 x 1024 44 us. 8200 x 2304 x 768 with norm and rotation 27 us, bound by its epilogue (21 without the reads of the
+// angles). One row of 1024 against 30877: 8 us, the latency of a launch and of two tiles.
 #include "common.h"
 #include "fp4.cuh"
 #include "gemm_fp4.h"
@@ -808,8 +809,8 @@ int code_map(CUtensorMap* map, const uint8_t* codes, int rows, int cols) {
 
 // Whether 256 x 256 tiles over CTA pairs are the faster choice: rounds of tiles times the time of one, measured at
 // K = 1024 and 8192: 128 x 128 tiles 1.45 us (their epilogue) or 0.30 us per 256 columns of K, pair tiles 2.75 us or
-// 0.415 us. (65600 x 5504 x 1024 SwiGLU 209 us in pairs, 232 us without; 65600 x 1024 x 2730 100 and 138 us;
-// 8200 x 4096 x 768 20.4 and 19.8 us.)
+// 0.415 us. (65600 x 5504 x 1024 SwiGLU 206 us in pairs, 230 us without; 65600 x 1024 x 2730 101 and 139 us;
+// 8200 x 4096 x 768 20.7 and 19.9 us.)
 bool choose_pair_fp4(int M, int N, int K) {
   const int64_t steps = (K + kFp4Step - 1) / kFp4Step, sms = sm_count(), pairs = sms / 2;
   const int64_t single = static_cast<int64_t>((M + 127) / 128) * ((N + 127) / 128);

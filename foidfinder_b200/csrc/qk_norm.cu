@@ -8,9 +8,10 @@
 // are issued before the first is worked on. A CTA takes 8 neighbouring rows, whose angles share cache sectors of the
 // angle-major tables.
 //
-// Measured, 65600 rows of 32 heads of 64 fp16 (537 MB moved): RMS norm 91 us (5.9 TB/s, 90% of the copy rate), LayerNorm
-// 97; 32000 rows of 32 heads of 128, FF_ROPE_HALVES, 96. With a warp per row that ends with it, weights read for every
-// row and fewer loads in flight, 101 and 114.
+// Measured, 65600 rows of 32 heads of 64 fp16 (537 MB moved): FF_ROPE_PAIRS RMS norm 91 us (5.9 TB/s, 90% of the copy rate),
+// LayerNorm 98; FF_ROPE_HALVES 99 and 136. 32000 rows of 32 heads of 128: 90 and 97, 96 and 136. LayerNorm with halves does
+// not fit its registers (twice the angles, and biases; 132 bytes per thread spilled). With a warp per row that ends with it,
+// weights read for every row and fewer loads in flight, pairs took 101 and 114.
 #include <algorithm>
 
 #include "common.h"

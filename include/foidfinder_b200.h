@@ -177,7 +177,8 @@ int ff_dequantize_fp4(const uint8_t* codes, const uint8_t* scales, const float* 
 /*
  * The product of two such operands on the tcgen05 tensor cores, A [M, K] x W [N, K]:
  *   y[m, n] = (sum over k, block scales included, f32) * row_scale[m] * col_scale[n] + bias[n]
- * (row_scale and col_scale, the two operands' row scales, are read for FF_FP4_NV only), then one of
+ * (row_scale and col_scale, the two operands' row scales, are read for FF_FP4_NV only; their product is taken first, in
+ * f32, and must stay below 2^128), then one of
  *   FF_EPI_BIAS           out = y                       (fp16, bf16 or f32)
  *   FF_EPI_GELU           out = gelu_tanh(y)            (fp16 or bf16, like all below)
  *   FF_EPI_SWIGLU         W rows interleaved [gate 16 | up 16]; out [M, out_cols] = silu(gate) * up, out_cols <= N / 2
