@@ -51,10 +51,17 @@ int* device_error_word() {
   if (g_err_word[dev] == nullptr) {
     std::lock_guard<std::mutex> lock(g_mu);
     if (g_err_word[dev] == nullptr) {
+      // On a stream of its own and waiting for that one only: the first call may come while a graph is being captured.
+      cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+      cudaThreadExchangeStreamCaptureMode(&mode);
       int* p = nullptr;
-      if (cudaMalloc(&p, sizeof(int)) != cudaSuccess) return nullptr;
-      cudaMemset(p, 0, sizeof(int));
-      cudaDeviceSynchronize();
+      cudaStream_t s = nullptr;
+      const bool ok = cudaMalloc(&p, sizeof(int)) == cudaSuccess && cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking) == cudaSuccess &&
+                      cudaMemsetAsync(p, 0, sizeof(int), s) == cudaSuccess && cudaStreamSynchronize(s) == cudaSuccess;
+      if (s != nullptr) cudaStreamDestroy(s);
+      if (!ok && p != nullptr) cudaFree(p);
+      cudaThreadExchangeStreamCaptureMode(&mode);
+      if (!ok) return nullptr;
       g_err_word[dev] = p;
     }
   }

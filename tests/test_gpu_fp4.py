@@ -966,3 +966,38 @@ def test_quantize_at_the_widths_where_variants_change(cuda_device, no_device_err
     wide = torch.full((9, (cols + 15) // 8 * 8), math.nan, dtype=dtype, device=cuda_device)[:, :cols]  # rows on 16-byte boundaries
     wide.copy_(x)
     _check_exact(fp4.quantize(wide, "nv"), x)
+
+
+_FIRST_CALLS = """
+import sys, torch
+from foidfinder_b200 import fp4, ops
+d = "cuda"
+x, w = torch.randn(8, 64, device=d).half(), torch.randn(128, 64, device=d)
+out, v, h = torch.empty(8, 128, device=d).half(), torch.empty(8, 64, device=d).half(), torch.empty(8, 64, device=d).half()
+t, hw = torch.ones(16, 3, device=d), torch.ones(32, device=d)
+q, weight = fp4.Fp4Tensor.empty(8, 64, "nv"), fp4.Fp4Tensor.empty(128, 64, "nv")
+def calls():
+    fp4.quantize(w, out=weight)
+    fp4.quantize(x, out=q)
+    fp4.dequantize(q, out=v)
+    ops.linear_fp4(x, weight.codes, weight.scales, weight.row_scale, out, ops.EPI_BIAS, 0, N=128)
+    ops.qk_norm_rope(x, h, q_heads=1, k_heads=1, head_dim=32, norm="rms", q_weight=hw, k_weight=hw, rope_cos=t, rope_sin=t)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    calls()
+g.replay()
+torch.cuda.synchronize()
+got = [t.clone() for t in (out, v, h)]
+calls()
+assert all(torch.equal(a, b) for a, b in zip(got, (out, v, h))) and ops.device_error(0) == 0
+"""
+
+
+def test_the_first_calls_of_a_process_can_be_captured(cuda_device):
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    r = subprocess.run([sys.executable, "-c", _FIRST_CALLS], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr[-2000:]
