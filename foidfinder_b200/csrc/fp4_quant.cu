@@ -154,10 +154,10 @@ __device__ __forceinline__ float nv_row_scale(float amax) {
 }
 __device__ __forceinline__ float inv_pow2(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
 
-// v / (S s) for the code, r about 1 / (S s). A code's ties are T = 0.25, 0.75, 1.25, 1.75, 2.5, 3.5 and 5; S has four
-// significant bits, so T S s is representable in every input type, and a quotient is a tie only if v is T S s.
-// kExact16: v came from a 16-bit type, so v and T S s differ in their first 11 bits if at all: a quotient that is no tie is
-//   at least 2^-11 T, that is 2^-13, away from one, while v * r is within 2^-20 of the quotient. Rounding v * r + 192 (one
+// v / (S s) for the code, r about 1 / (S s). A code's ties are T = 0.25, 0.75, 1.25, 1.75, 2.5, 3.5 and 5; T S s has
+// at most seven significant bits (three of T, four of S), and a quotient is a tie only if v is T S s.
+// kExact16: v came from a 16-bit type and has at most 11 significant bits, so v and T S s differ by 2^-11 of themselves or
+//   not at all: a quotient that is no tie is at least 2^-11 T, that is 2^-13, away from one, while v * r is within 2^-20 of the quotient. Rounding v * r + 192 (one
 //   FMA, to multiples of 2^-16) puts true ties exactly on the tie and moves no other across (r within 2^-22 of 1 / (S s) is
 //   enough).
 // kExact32: v from f32 and already divided by s (exact, or far below any tie), r the reciprocal of scale = S. The quotient
