@@ -39,6 +39,9 @@ F16, BF16, F32 = 0, 1, 2
 EPI_QKV_NORM_ROPE = 8
 NORM_RMS, NORM_LAYER = 1, 2
 ROPE_PAIRS, ROPE_HALVES = 0, 1
+# ff_norm_residual (FF_NORM_NONE, FF_GATE_*).
+NORM_NONE = 0
+GATE_PLAIN, GATE_SIGMOID, GATE_TANH = 0, 1, 2
 
 vp, i32, i64, f32 = C.c_void_p, C.c_int, C.c_int64, C.c_float
 
@@ -116,6 +119,16 @@ class Fp4Epilogue(C.Structure):
     )
 
 
+class NormResidualArgs(C.Structure):
+    _fields_ = [
+        ("x", vp), ("ldx", i64), ("y", vp), ("ldy", i64), ("out", vp), ("ldo", i64), ("normed", vp), ("ldn", i64),
+        ("x_type", i32), ("y_type", i32), ("rows", i32), ("cols", i32), ("alpha", f32),
+        ("post", i32), ("post_w", vp), ("post_b", vp), ("post_eps", f32),
+        ("pre", i32), ("pre_w", vp), ("pre_b", vp), ("pre_eps", f32),
+        ("gate", vp), ("ldg", i64), ("gate_type", i32), ("gate_cols", i32), ("gate_rows", i32), ("gate_act", i32), ("scale", vp),
+    ]
+
+
 _SIGNATURES = {
     "ff_last_error": (C.c_char_p, []),
     "ff_version": (i32, []),
@@ -138,6 +151,12 @@ _SIGNATURES = {
     ),
     "ff_qk_norm_rope": (
         i32, [vp, i32, i64, vp, i64, i32, i32, i32, i32, i32, vp, vp, vp, vp, f32, vp, vp, i32, i32, vp]
+    ),
+    "ff_rope": (i32, [vp, i32, i64, vp, i64, i32, i32, i32, i32, i32, i32, vp, i32, i32, vp, i32, f32, vp]),
+    "ff_norm_residual": (i32, [C.POINTER(NormResidualArgs), vp]),
+    "ff_cross_attention_workspace_bytes": (i64, [i32, i32, i32, i32, i32, i32]),
+    "ff_cross_attention": (
+        i32, [vp, i64, vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, vp, vp, vp, vp, i32, i32, i32, f32, vp, i64, vp]
     ),
     "ff_attention": (i32, [vp, vp, i32, i32, i32, vp, vp, f32, vp]),
     "ff_patchify": (i32, [vp, i32, i32, i32, C.POINTER(f32), C.POINTER(f32), vp, i32, vp]),

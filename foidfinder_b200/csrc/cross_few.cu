@@ -1,0 +1,389 @@
+// Attention of few queries per sequence to its keys and values (one decoder token, some learned queries).
+//   out = softmax(scale q k^T) v, head by head, keys that do not take part left out
+//
+// Bound by HBM: keys and values are read once, 4 bytes per key, head and column, for a few multiply-adds each. A CTA takes
+// one part of one sequence's keys and one key head, and all query rows that read it (the group's heads of every query,
+// 16 * RG rows at a time). Key and value tiles of 64 keys come through a ring of asynchronous 16-byte copies, which fill a
+// key that does not take part with zeros instead of reading it (so that whatever it holds, its value counts 0 * 0). RG
+// warps divide the rows, 4 / RG warps the keys of a tile; each keeps a running maximum, sum and output of its keys in
+// registers (mma.sync: the products are far from what bounds this kernel, and 16 rows are what there is). The warps' parts
+// are joined through shared memory in a fixed order, and the parts of CTAs by a second kernel through the workspace.
+//
+// P is rounded to 16 bits for its product with V, as 2^(x - max + 14) in fp16, where it would else lose bits below 2^-14;
+// sums are taken before that rounding, in f32.
+#include <algorithm>
+
+#include "common.h"
+#include "cross.h"
+#include "fp4.cuh"
+
+namespace ff {
+
+namespace {
+
+constexpr int kKeys = 64;        // of a tile
+constexpr int kFewThreads = 128;
+__host__ __device__ constexpr int few_stages(int atoms) { return atoms == 1 ? 4 : 3; }
+__host__ __device__ constexpr int few_tile(int atoms) { return atoms * kKeys * 128; }  // bytes of a K or V tile
+__host__ __device__ constexpr int few_smem(int atoms) { return few_stages(atoms) * 2 * few_tile(atoms); }
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool take) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+template <class T>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+#define FF_MMA(TYPE)                                                                                              \
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32." TYPE "." TYPE                                             \
+               ".f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"                             \
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])                                                   \
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1))
+  if constexpr (std::is_same<T, __half>::value)
+    FF_MMA("f16");
+  else
+    FF_MMA("bf16");
+#undef FF_MMA
+}
+
+// Byte of 16-byte chunk c (of 8 * atoms) of a tile's row: 128-byte rows per atom, chunks permuted by the row so that
+// neither eight rows of a chunk nor eight chunks of a row meet in a bank.
+__device__ __forceinline__ uint32_t tile_byte(int row, int c) {
+  return static_cast<uint32_t>((c >> 3) * (kKeys * 128) + row * 128 + (((c ^ row) & 7) << 4));
+}
+
+struct FewArgs {
+  CrossArgs p;
+  int passes, splits;
+  float* part_o;   // [splits][q_rows * heads][dim]
+  float2* part_ml;  // [splits][q_rows * heads]: maximum (in powers of two) and sum
+};
+
+template <class T, int ATOMS, int RG>
+__global__ void __launch_bounds__(kFewThreads) cross_few_kernel(const __grid_constant__ FewArgs a) {
+  constexpr int STAGES = few_stages(ATOMS), TILE = few_tile(ATOMS), KG = 4 / RG, KW = kKeys / KG;
+  constexpr int ROWS = 16 * RG, STEPS = ATOMS * 4;
+  constexpr float kShift = std::is_same<T, __half>::value ? 14.f : 0.f;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ uint64_t taken[STAGES];  // bits: keys of a tile that take part
+  __shared__ float part_m[KG][ROWS], part_l[KG][ROWS];
+  const CrossArgs& p = a.p;
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, rg = warp % RG, kg = warp / RG;
+  const int group = p.heads / p.kv_heads, dim = p.dim, chunks = dim / 8;
+  int at = static_cast<int>(blockIdx.x);
+  const int split = at % a.splits;
+  at /= a.splits;
+  const int pass0 = at % a.passes;
+  at /= a.passes;
+  const int kvh = at % p.kv_heads, b = at / p.kv_heads;
+  pdl_wait();
+  pdl_trigger();
+  const Piece qs = query_piece(p, b), ks = key_piece(p, b);
+  const int total_rows = qs.n * group;
+  const int all_tiles = (ks.n + kKeys - 1) / kKeys, per = (all_tiles + a.splits - 1) / a.splits;
+  const int first = split * per, tiles = max(0, min(per, all_tiles - first));
+  const T* const kp = static_cast<const T*>(p.k) + (ks.at + static_cast<int64_t>(first) * kKeys) * p.ldk + static_cast<int64_t>(kvh) * dim;
+  const T* const vp = static_cast<const T*>(p.v) + (ks.at + static_cast<int64_t>(first) * kKeys) * p.ldv + static_cast<int64_t>(kvh) * dim;
+  const uint8_t* const mask = p.mask != nullptr ? p.mask + ks.at + static_cast<int64_t>(first) * kKeys : nullptr;
+  const int keys = max(0, min(tiles * kKeys, ks.n - first * kKeys));
+  const uint32_t base = smem_u32(smem);
+
+  // The keys of tile i that take part; every warp works it out.
+  auto bits_of = [&](int i) -> uint64_t {
+    const int left = keys - i * kKeys;
+    if (left <= 0) return 0;
+    if (mask == nullptr) return left >= kKeys ? ~0ull : (1ull << left) - 1;
+    const bool lo = lane < left && mask[i * kKeys + lane] != 0, hi = 32 + lane < left && mask[i * kKeys + 32 + lane] != 0;
+    const uint64_t l = __ballot_sync(0xffffffffu, lo), h = __ballot_sync(0xffffffffu, hi);
+    return l | h << 32;
+  };
+  auto load = [&](int i, uint64_t bits) {
+    const int st = i % STAGES;
+    if (t == 0) taken[st] = bits;
+    const uint32_t kd = base + st * 2 * TILE, vd = kd + TILE;
+#pragma unroll
+    for (int n = 0; n < ATOMS * 4; ++n) {  // 64 rows x 8 chunks of an atom by 128 threads: 4 steps
+      const int c = (n >> 2) * 8 + (t & 7), row = (n & 3) * 16 + (t >> 3);
+      if (c < chunks) {
+        const bool take = bits >> row & 1;
+        const int64_t r = take ? i * kKeys + row : 0;  // a key left out is not read
+        const uint32_t d = tile_byte(row, c);
+        copy16(kd + d, kp + r * p.ldk + c * 8, take);
+        copy16(vd + d, vp + r * p.ldv + c * 8, take);
+      }
+    }
+  };
+
+  for (int pass = pass0; pass * ROWS < total_rows; pass += a.passes) {
+    // Rows of this lane: lane / 4 and 8 further, of the warp's 16.
+    uint32_t qf[STEPS][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = pass * ROWS + rg * 16 + h * 8 + (lane >> 2);
+      const T* qp = static_cast<const T*>(p.q);
+      if (row < total_rows) qp += static_cast<int64_t>(qs.at + row / group) * p.ldq + static_cast<int64_t>(kvh * group + row % group) * dim;
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          qf[s][2 * c + h] = row < total_rows && s * 16 < dim ? *reinterpret_cast<const uint32_t*>(qp + s * 16 + c * 8 + (lane & 3) * 2) : 0;
+    }
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[2 * STEPS][4];
+#pragma unroll
+    for (int n = 0; n < 2 * STEPS; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) {
+      const uint64_t bits = bits_of(i);
+      if (i < tiles) load(i, bits);
+      copies_commit();
+    }
+    uint64_t ahead = bits_of(STAGES - 1);
+    for (int i = 0; i < tiles; ++i) {
+      copies_wait<STAGES - 2>();
+      __syncthreads();  // tile i has landed for all, and all are done with tile i - 1, whose place is next
+      if (i + STAGES - 1 < tiles) load(i + STAGES - 1, ahead);
+      copies_commit();
+      ahead = bits_of(i + STAGES);
+      const uint32_t kt = base + (i % STAGES) * 2 * TILE, vt = kt + TILE;
+      const uint64_t bits = taken[i % STAGES] >> (kg * KW);  // of this warp's keys
+      float s[KW / 8][4];
+#pragma unroll
+      for (int n = 0; n < KW / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+#pragma unroll
+      for (int k = 0; k < STEPS; ++k) {
+        if (k * 16 >= dim) break;
+#pragma unroll
+        for (int n = 0; n < KW / 16; ++n) {
+          uint32_t f[4];
+          ldmatrix4(kt + tile_byte(kg * KW + n * 16 + (lane >> 4) * 8 + (lane & 7), k * 2 + (lane >> 3 & 1)), f);
+          mma16816<T>(s[2 * n], qf[k], f[0], f[1]);
+          mma16816<T>(s[2 * n + 1], qf[k], f[2], f[3]);
+        }
+      }
+      // Scores in powers of two; keys that do not take part are -inf (also where their products are NaN).
+      const uint64_t all = KW == 64 ? ~0ull : (1ull << (KW & 63)) - 1;
+      float mx[2] = {-INFINITY, -INFINITY};
+      if ((bits & all) != all) {
+#pragma unroll
+        for (int n = 0; n < KW / 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!(bits >> (n * 8 + (lane & 3) * 2 + (e & 1)) & 1)) s[n][e] = -INFINITY;
+      }
+#pragma unroll
+      for (int n = 0; n < KW / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
+      float base_m[2];
+      bool grew = false;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+        const float now = fmaxf(m[h], mx[h] * p.scale_log2);
+        grew |= now > m[h];
+        mx[h] = m[h];  // the old one
+        m[h] = now;
+        base_m[h] = now == -INFINITY ? 0.f : now;
+      }
+      if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float corr = ex2_approx(mx[h] - base_m[h]);
+          l[h] *= corr;
+#pragma unroll
+          for (int n = 0; n < 2 * STEPS; ++n) {
+            o[n][2 * h] *= corr;
+            o[n][2 * h + 1] *= corr;
+          }
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < KW / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[n][e] = ex2_approx(fmaf(s[n][e], p.scale_log2, kShift - base_m[e >> 1]));
+          l[e >> 1] += s[n][e];
+        }
+#pragma unroll
+      for (int n = 0; n < KW / 16; ++n) {
+        const uint32_t pf[4] = {Pair16<T>::pack(s[2 * n][0], s[2 * n][1]), Pair16<T>::pack(s[2 * n][2], s[2 * n][3]),
+                                Pair16<T>::pack(s[2 * n + 1][0], s[2 * n + 1][1]), Pair16<T>::pack(s[2 * n + 1][2], s[2 * n + 1][3])};
+#pragma unroll
+        for (int c = 0; c < STEPS; ++c) {
+          if (c * 16 >= dim) break;
+          uint32_t f[4];
+          ldmatrix4_trans(vt + tile_byte(kg * KW + n * 16 + (lane & 15), c * 2 + (lane >> 4)), f);
+          mma16816<T>(o[2 * c], pf, f[0], f[1]);
+          mma16816<T>(o[2 * c + 1], pf, f[2], f[3]);
+        }
+      }
+    }
+    copies_wait<0>();
+    __syncthreads();  // the ring is free: the warps' parts meet there, [KG][ROWS][dim] f32
+    float* const parts = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+      const int row = rg * 16 + h * 8 + (lane >> 2);
+      if ((lane & 3) == 0) {
+        part_m[kg][row] = m[h];
+        part_l[kg][row] = l[h];
+      }
+      float* const dst = parts + (kg * ROWS + row) * dim + (lane & 3) * 2;
+#pragma unroll
+      for (int n = 0; n < 2 * STEPS; ++n)
+        if (n * 8 < dim) *reinterpret_cast<float2*>(dst + n * 8) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+    }
+    __syncthreads();
+    const int quads = dim / 4;
+    for (int i = t; i < ROWS * quads; i += kFewThreads) {
+      const int r = i / quads, c = (i - r * quads) * 4, row = pass * ROWS + r;
+      if (row >= total_rows) break;
+      float top = part_m[0][r];
+#pragma unroll
+      for (int g = 1; g < KG; ++g) top = fmaxf(top, part_m[g][r]);
+      float sum = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int g = 0; g < KG; ++g) {
+        const float w = part_m[g][r] == -INFINITY && top == -INFINITY ? 1.f : ex2_approx(part_m[g][r] - top);
+        const float4 v = *reinterpret_cast<const float4*>(parts + (g * ROWS + r) * dim + c);
+        sum = fmaf(part_l[g][r], w, sum);
+        acc.x = fmaf(v.x, w, acc.x);
+        acc.y = fmaf(v.y, w, acc.y);
+        acc.z = fmaf(v.z, w, acc.z);
+        acc.w = fmaf(v.w, w, acc.w);
+      }
+      const int64_t q_row = qs.at + row / group;
+      const int head = kvh * group + row % group;
+      if (a.splits == 1) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no key: zeros
+        *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + q_row * p.ldo + static_cast<int64_t>(head) * dim + c) =
+            make_uint2(Pair16<T>::pack(acc.x * inv, acc.y * inv), Pair16<T>::pack(acc.z * inv, acc.w * inv));
+      } else {
+        const int64_t at_row = (static_cast<int64_t>(split) * p.q_rows + q_row) * p.heads + head;
+        *reinterpret_cast<float4*>(a.part_o + at_row * dim + c) = acc;
+        if (c == 0) a.part_ml[at_row] = make_float2(top, sum);
+      }
+    }
+    __syncthreads();  // before the next pass fills the ring
+  }
+}
+
+// out = the splits' parts, joined in order: a warp per query row and head.
+template <class T>
+__global__ void __launch_bounds__(256) cross_join_kernel(const __grid_constant__ FewArgs a) {
+  const CrossArgs& p = a.p;
+  const int lane = threadIdx.x & 31;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  pdl_wait();
+  pdl_trigger();
+  const int64_t rows = static_cast<int64_t>(p.q_rows) * p.heads;
+  if (at >= rows) return;
+  const int q_row = static_cast<int>(at / p.heads), head = static_cast<int>(at % p.heads);
+  if (p.q_start != nullptr && (q_row < __ldg(p.q_start) || q_row >= __ldg(p.q_start + p.sequences))) return;  // of no sequence
+  float top = -INFINITY;
+  for (int i = lane; i < a.splits; i += 32) top = fmaxf(top, a.part_ml[i * rows + at].x);
+  top = warp_max(top);
+  float sum = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int c = lane * 4;
+#pragma unroll 4
+  for (int i = 0; i < a.splits; ++i) {
+    const float2 ml = a.part_ml[i * rows + at];
+    const float w = ml.x == -INFINITY && top == -INFINITY ? 1.f : ex2_approx(ml.x - top);
+    sum = fmaf(ml.y, w, sum);
+    if (c < p.dim) {
+      const float4 v = *reinterpret_cast<const float4*>(a.part_o + (i * rows + at) * p.dim + c);
+      acc.x = fmaf(v.x, w, acc.x);
+      acc.y = fmaf(v.y, w, acc.y);
+      acc.z = fmaf(v.z, w, acc.z);
+      acc.w = fmaf(v.w, w, acc.w);
+    }
+  }
+  if (c >= p.dim) return;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + q_row * p.ldo + static_cast<int64_t>(head) * p.dim + c) =
+      make_uint2(Pair16<T>::pack(acc.x * inv, acc.y * inv), Pair16<T>::pack(acc.z * inv, acc.w * inv));
+}
+
+template <class T, int ATOMS, int RG>
+int launch_few(const FewArgs& a, cudaStream_t s) {
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    if (cudaFuncSetAttribute(cross_few_kernel<T, ATOMS, RG>, cudaFuncAttributeMaxDynamicSharedMemorySize, few_smem(ATOMS)) != cudaSuccess)
+      return check_launch("cross_few: cudaFuncSetAttribute");
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  const int64_t grid = static_cast<int64_t>(a.splits) * a.passes * a.p.kv_heads * a.p.sequences;
+  FF_REQUIRE(grid <= 0x7fffffff, "ff_cross_attention: %lld parts", static_cast<long long>(grid));
+  launch(cross_few_kernel<T, ATOMS, RG>, dim3(static_cast<unsigned>(grid)), dim3(kFewThreads), few_smem(ATOMS), s, a);
+  if (a.splits > 1) {
+    const int rc = check_launch("cross_few_kernel");
+    if (rc != FF_OK) return rc;
+    const int64_t rows = static_cast<int64_t>(a.p.q_rows) * a.p.heads;
+    launch(cross_join_kernel<T>, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0, s, a);
+  }
+  return check_launch("cross_few_kernel");
+}
+
+template <class T>
+int launch_few_type(const FewArgs& a, int row_tiles, cudaStream_t s) {
+  if (a.p.dim <= 64) {
+    if (row_tiles == 1) return launch_few<T, 1, 1>(a, s);
+    return row_tiles == 2 ? launch_few<T, 1, 2>(a, s) : launch_few<T, 1, 4>(a, s);
+  }
+  if (row_tiles == 1) return launch_few<T, 2, 1>(a, s);
+  return row_tiles == 2 ? launch_few<T, 2, 2>(a, s) : launch_few<T, 2, 4>(a, s);
+}
+
+}  // namespace
+
+CrossFewPlan cross_few_plan(int q_rows, int k_rows, int sequences, int heads, int kv_heads, int dim) {
+  CrossFewPlan plan{};
+  const int64_t rows = (static_cast<int64_t>(q_rows) + sequences - 1) / sequences * (heads / kv_heads);
+  plan.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  plan.passes = static_cast<int>(std::max<int64_t>(1, (rows + 16 * plan.row_tiles - 1) / (16 * plan.row_tiles)));
+  const int64_t ctas = static_cast<int64_t>(sequences) * kv_heads * plan.passes;
+  const int64_t tiles = ((static_cast<int64_t>(k_rows) + sequences - 1) / sequences + kKeys - 1) / kKeys;
+  // As many parts as fill the GPU's places for CTAs (three per SM, two with the larger tiles), of two tiles at least
+  const int64_t places = static_cast<int64_t>(sm_count()) * (dim <= 64 ? 3 : 2);
+  plan.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({places / ctas, (tiles + 1) / 2, 1024})));
+  if (plan.splits > 1) plan.workspace = static_cast<int64_t>(plan.splits) * q_rows * heads * (dim + 2) * 4;
+  return plan;
+}
+
+int cross_few(const CrossArgs& p, bool bf16, const CrossFewPlan& plan, void* workspace, cudaStream_t s) {
+  FewArgs a{};
+  a.p = p;
+  a.passes = plan.passes;
+  a.splits = plan.splits;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + static_cast<int64_t>(plan.splits) * p.q_rows * p.heads * p.dim);
+  return bf16 ? launch_few_type<__nv_bfloat16>(a, plan.row_tiles, s) : launch_few_type<__half>(a, plan.row_tiles, s);
+}
+
+}  // namespace ff

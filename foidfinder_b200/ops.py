@@ -8,6 +8,7 @@ take a short way to it (csrc/calls.cpp) where their arguments are plain.
 from __future__ import annotations
 
 import ctypes as C
+import math
 import warnings
 from functools import cache
 
@@ -24,6 +25,7 @@ __all__ = [
     "gemm_s8", "gemm_f16", "rot_q8", "rot_q8_1024", "rot_q8_h128", "attention", "patchify", "fill_cls",
     "layernorm", "topk", "tree_pool", "resize_pad", "patchify_windowed", "layernorm_pos", "pool_query_attention",
     "FP4_NV", "FP4_MX", "EPI_QKV_NORM_ROPE", "quantize_fp4", "dequantize_fp4", "gemm_fp4", "linear_fp4", "qk_norm_rope",
+    "rope", "rope_frequencies", "norm_residual", "cross_attention",
 ]
 
 
@@ -636,3 +638,198 @@ def qk_norm_rope(
     cos, sin, tokens = _tables(rope_cos, rope_sin, head_dim // 2, device, what)
     _launch(what, lib().ff_qk_norm_rope, device, x.data_ptr(), _DTYPES[dtype], ldx, out.data_ptr(), ldo, rows, q_heads, k_heads, head_dim, n,
             qw, qb, kw, kb, eps, cos, sin, tokens, p)
+
+
+# ---------------------------------------------------------------- tokens that read an image's
+_GATES = {None: _lib.GATE_PLAIN, "sigmoid": _lib.GATE_SIGMOID, "tanh": _lib.GATE_TANH}
+
+
+def rope_frequencies(
+    rotary: int,
+    base: float = 10000.0,
+    *,
+    scaling: str | None = None,
+    factor: float = 1.0,
+    trained: int = 0,
+    fast: float = 32.0,
+    slow: float = 1.0,
+) -> tuple[torch.Tensor, float]:
+    """Frequencies [rotary / 2] (f64, radians per position; base^(-2 i / rotary)) and the scale for `rope`. `scaling` stretches
+    them for contexts `factor` times as long: "linear" divides all of them, "ntk" raises the base so that the slowest is
+    divided and the fastest stays, "yarn" leaves pairs that turn more than `fast` times within the `trained` context, divides
+    those that turn less than `slow` times, blends between, and scales by 0.1 ln(factor) + 1."""
+    _need(rotary >= 2 and rotary % 2 == 0, f"rope_frequencies: {rotary} columns are no pairs")
+    _need(base > 1 and factor >= 1, "rope_frequencies: base must be above 1 and factor at least 1")
+    _need(scaling in (None, "linear", "ntk", "yarn"), f"rope_frequencies: unknown scaling {scaling!r}")
+    scale = 1.0
+    if scaling == "ntk" and rotary > 2:
+        base *= factor ** (rotary / (rotary - 2))
+    f = base ** (torch.arange(0, rotary, 2, dtype=torch.float64) / -rotary)
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "yarn":
+        _need(trained > 0 and fast > slow > 0, "rope_frequencies: yarn needs the trained context's length and fast > slow > 0")
+        # the pair (a fraction of one) that turns n times within the trained context
+        pair = lambda n: rotary * math.log(trained / (2 * math.pi * n)) / (2 * math.log(base))
+        low, high = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), rotary - 1)
+        ramp = ((torch.arange(rotary // 2, dtype=torch.float64) - low) / max(high - low, 0.001)).clamp(0, 1)
+        f = f * (1 - ramp) + f / factor * ramp
+        scale = 0.1 * math.log(factor) + 1
+    return f, scale
+
+
+def rope(
+    x: torch.Tensor,
+    out: torch.Tensor,
+    positions: torch.Tensor,
+    frequencies: torch.Tensor,
+    *,
+    heads: int,
+    head_dim: int,
+    start: int = 0,
+    pairing: str = "pairs",
+    scale: float = 1.0,
+) -> None:
+    """x [T, >= heads * head_dim] fp16, bf16 or f32 -> every head's columns [start, start + 2 * frequencies.numel()) rotated by
+    positions[row] * frequencies (radians; the angles in 64 bits), times `scale`, its other columns as they are, into the
+    first columns of out (x itself: in place). `positions` [T] or [T, axes] int32 or int64 (axes take equal shares of the
+    pairs, in order), `frequencies` f64 or f32 (`rope_frequencies`); `pairing` "pairs" rotates (2i, 2i + 1) of them, "halves" (i, i + r / 2)."""
+    what = "rope"
+    rows, xcols, ldx, device = _matrix(x, what)
+    orows, ocols, ldo, odevice = _matrix(out, what)
+    dtype = _DTYPES.get(x.dtype)
+    if dtype is None or out.dtype is not x.dtype:
+        raise RuntimeError(f"rope: x and out must be fp16, bf16 or f32, alike, got {x.dtype} and {out.dtype}")
+    cols = heads * head_dim
+    if heads < 0 or head_dim < 1 or xcols < cols or ocols < cols or orows != rows or odevice != device:
+        raise RuntimeError(f"rope: x {list(x.shape)} and out {list(out.shape)} must hold {cols} columns of the same rows on one device")
+    _need(pairing in _PAIRINGS, "rope: pairing is 'pairs' or 'halves'")
+    axes = 1 if positions.dim() == 1 else positions.shape[1] if positions.dim() == 2 else 0
+    if positions.get_device() != device or positions.dtype not in (torch.int32, torch.int64) or axes < 1 or positions.shape[0] != rows or not positions.is_contiguous():
+        raise RuntimeError(f"rope: positions must be contiguous int32 or int64 [{rows}] or [{rows}, axes] on cuda:{device}, got {positions.dtype} {list(positions.shape)} on {positions.device}")
+    if frequencies.get_device() != device or frequencies.dtype not in (torch.float32, torch.float64) or frequencies.dim() != 1 or not frequencies.is_contiguous():
+        raise RuntimeError(f"rope: frequencies must be a contiguous f64 or f32 vector on cuda:{device}, got {frequencies.dtype} {list(frequencies.shape)} on {frequencies.device}")
+    _launch(what, lib().ff_rope, device, x.data_ptr(), dtype, ldx, out.data_ptr(), ldo, rows, heads, head_dim, start, 2 * frequencies.numel(),
+            _PAIRINGS[pairing], positions.data_ptr(), positions.element_size(), axes, frequencies.data_ptr(), frequencies.element_size(), scale)
+
+
+def norm_residual(
+    x: torch.Tensor,
+    y: torch.Tensor,
+    out: torch.Tensor,
+    *,
+    alpha: float = 1.0,
+    post: str | None = None,
+    post_weight: torch.Tensor | None = None,
+    post_bias: torch.Tensor | None = None,
+    gate: torch.Tensor | None = None,
+    gate_act: str | None = None,
+    gate_rows: int = 1,
+    scale: torch.Tensor | None = None,
+    normed: torch.Tensor | None = None,
+    pre: str | None = None,
+    pre_weight: torch.Tensor | None = None,
+    pre_bias: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    pre_eps: float | None = None,
+) -> None:
+    """The end of a block and the norm before the next one: out = alpha * x + scale * act(gate) * post(y), normed = pre(out) (of
+    out before it is rounded). x and out [T, C] are the residual stream (out may be x), y the block's result; normed, y's
+    type, may be y. `post` and `pre`: None, "rms" or "layer" with weights and biases [C] (f32, or None). `gate` [G, C] or [G, 1],
+    f32 or y's type, after `gate_act` None, "sigmoid" or "tanh"; row t reads gate row t // gate_rows. `scale` [C] f32. Types: fp16,
+    bf16 or f32 alike, or x and out in f32 with a 16-bit y. Rows that start 16 bytes apart are the fastest."""
+    what = "norm_residual"
+    rows, cols, ldx, device = _matrix(x, what)
+    n = _lib.NormResidualArgs(rows=rows, cols=cols, alpha=alpha, ldx=ldx, x=x.data_ptr(), post_eps=eps, pre_eps=eps if pre_eps is None else pre_eps)
+    for name, ld, t, like in (("y", "ldy", y, y), ("out", "ldo", out, x), ("normed", "ldn", normed, y)):
+        if t is None:
+            continue
+        trows, tcols, tld, tdevice = _matrix(t, f"norm_residual: {name}")
+        if (trows, tcols, tdevice) != (rows, cols, device) or t.dtype is not like.dtype:
+            raise RuntimeError(f"norm_residual: {name} is {t.dtype} {list(t.shape)} on {t.device} beside x [{rows}, {cols}] on cuda:{device} and {like.dtype}")
+        setattr(n, name, t.data_ptr())
+        setattr(n, ld, tld)
+    if x.dtype not in _DTYPES or y.dtype not in _DTYPES or (x.dtype is not y.dtype and x.dtype is not torch.float32):
+        raise RuntimeError(f"norm_residual: x and y must be fp16, bf16 or f32 alike, or x f32, got {x.dtype} and {y.dtype}")
+    n.x_type, n.y_type = _DTYPES[x.dtype], _DTYPES[y.dtype]
+    if post not in (None, *_NORMS) or pre not in (None, *_NORMS) or (pre is None) != (normed is None):
+        raise RuntimeError("norm_residual: post and pre are None, 'rms' or 'layer', and pre comes with normed")
+    if post is not None:
+        n.post, n.post_w, n.post_b = _NORMS[post], _vector(post_weight, cols, device, what), _vector(post_bias, cols, device, what)
+    if pre is not None:
+        n.pre, n.pre_w, n.pre_b = _NORMS[pre], _vector(pre_weight, cols, device, what), _vector(pre_bias, cols, device, what)
+    n.scale = _vector(scale, cols, device, what)
+    if gate is not None:
+        grows, gcols, n.ldg, gdevice = _matrix(gate, "norm_residual: gate")
+        if gdevice != device or gcols not in (1, cols) or (gate.dtype is not torch.float32 and gate.dtype is not y.dtype) or gate_act not in _GATES:
+            raise RuntimeError(f"norm_residual: the gate must be f32 or {y.dtype} [G, {cols}] or [G, 1] on cuda:{device} behind None, 'sigmoid' or 'tanh', got {gate.dtype} {list(gate.shape)} on {gate.device} and {gate_act!r}")
+        if gate_rows < 1 or grows * gate_rows < rows:
+            raise RuntimeError(f"norm_residual: {grows} gate rows for {gate_rows} rows each are too few for {rows}")
+        n.gate, n.gate_type, n.gate_cols, n.gate_act = gate.data_ptr(), _DTYPES[gate.dtype], gcols, _GATES[gate_act]
+        n.gate_rows = min(gate_rows, max(rows, 1))
+    _launch(what, lib().ff_norm_residual, device, C.byref(n))
+
+
+def cross_attention(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    out: torch.Tensor,
+    *,
+    heads: int,
+    head_dim: int,
+    kv_heads: int | None = None,
+    sequences: int | None = None,
+    q_start: torch.Tensor | None = None,
+    k_start: torch.Tensor | None = None,
+    k_len: torch.Tensor | None = None,
+    mask: torch.Tensor | None = None,
+    scale: float | None = None,
+) -> None:
+    """out = softmax(scale * q k^T) v for every sequence and head, with queries and keys of different lengths: q and out [Tq, heads *
+    head_dim], k and v [Tk, kv_heads * head_dim], fp16 or bf16 (views with contiguous columns and 16-byte rows, such as the
+    halves of a packed projection). Query head h reads key head h // (heads // kv_heads).
+
+    Sequences are equal pieces of the rows (`sequences` of them), or sequence b has rows q_start[b] to q_start[b + 1] and
+    k_start[b] to k_start[b + 1] (ascending int32 [sequences + 1] on the device, one or both); of its keys the first k_len[b]
+    (int32 [sequences]) take part. `mask` [Tk] bool leaves out keys where it is False. What is left out counts nothing, whatever
+    it holds. A query without keys gives zeros; rows of out outside the sequences stay as they were. `scale` is head_dim**-0.5 unless given."""
+    what = "cross_attention"
+    kv_heads = heads if kv_heads is None else kv_heads
+    tq, qcols, ldq, device = _matrix(q, what)
+    tk, kcols, ldk, kdevice = _matrix(k, what)
+    shape_v, shape_o = _matrix(v, what), _matrix(out, what)
+    dtype = q.dtype
+    if dtype is torch.float32 or dtype not in _DTYPES or k.dtype is not dtype or v.dtype is not dtype or out.dtype is not dtype:
+        raise RuntimeError(f"cross_attention: q, k, v and out must be fp16 or bf16, alike, got {q.dtype}, {k.dtype}, {v.dtype} and {out.dtype}")
+    if qcols != heads * head_dim or kcols != kv_heads * head_dim or shape_v[:2] != (tk, kcols) or shape_o[:2] != (tq, qcols):
+        raise RuntimeError(f"cross_attention: q {list(q.shape)}, k {list(k.shape)}, v {list(v.shape)}, out {list(out.shape)} for {heads} and {kv_heads} heads of {head_dim}")
+    if kdevice != device or shape_v[3] != device or shape_o[3] != device:
+        raise RuntimeError("cross_attention: q, k, v and out must be on one device")
+    for t, more in ((q_start, 1), (k_start, 1), (k_len, 0)):
+        if t is not None and sequences is None:
+            sequences = t.numel() - more
+    sequences = 1 if sequences is None else sequences
+    for name, t, n in (("q_start", q_start, sequences + 1), ("k_start", k_start, sequences + 1), ("k_len", k_len, sequences)):
+        if t is not None and (t.get_device() != device or t.dtype is not torch.int32 or t.numel() != n or not t.is_contiguous()):
+            raise RuntimeError(f"cross_attention: {name} must be {n} contiguous int32 values on cuda:{device}, got {t.dtype} {list(t.shape)} on {t.device}")
+    if mask is not None and (mask.get_device() != device or mask.dtype not in (torch.bool, torch.uint8) or mask.numel() != tk or not mask.is_contiguous()):
+        raise RuntimeError(f"cross_attention: mask must be {tk} contiguous bool values on cuda:{device}, got {mask.dtype} {list(mask.shape)} on {mask.device}")
+    if sequences < 0 or heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise RuntimeError(f"cross_attention: {sequences} sequences, {heads} query heads over {kv_heads} key heads")
+    if device != _current_device():
+        with torch.cuda.device(device):
+            return cross_attention(q, k, v, out, heads=heads, head_dim=head_dim, kv_heads=kv_heads, sequences=sequences, q_start=q_start,
+                                   k_start=k_start, k_len=k_len, mask=mask, scale=scale)
+    nbytes = lib().ff_cross_attention_workspace_bytes(tq, tk, sequences, heads, kv_heads, head_dim)
+    stream = _raw_stream(device)
+    ws = _alloc(nbytes, stream) if nbytes else None  # torch's stream-ordered cache: free for the stream's next use on return
+    try:
+        rc = lib().ff_cross_attention(q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), shape_v[2], out.data_ptr(), shape_o[2], _DTYPES[dtype],
+                                      tq, tk, sequences, _ptr(q_start), _ptr(k_start), _ptr(k_len), _ptr(mask), heads, kv_heads, head_dim,
+                                      head_dim**-0.5 if scale is None else scale, ws, nbytes, stream)
+    finally:
+        if ws is not None:
+            _free(ws)
+    if rc:
+        check(rc, what)

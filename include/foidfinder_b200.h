@@ -240,6 +240,79 @@ int ff_qk_norm_rope(const void* x, int dtype, int64_t ldx, void* out, int64_t ld
                     int head_dim, int norm, const float* q_w, const float* q_b, const float* k_w, const float* k_b,
                     float eps, const float* rope_cos, const float* rope_sin, int tokens, int pairing, void* stream);
 
+/* ---------------------------------------------------------------- tokens that read an image's (no reference counterpart) */
+/*
+ * Rotation of heads by positions given per row. x and out [rows, >= heads * head_dim] of type dtype (FF_F16, FF_BF16,
+ * FF_F32), row strides ldx and ldo elements, any alignment of their type. Of every head the columns [start, start +
+ * rotary) are rotary / 2 pairs, (2i, 2i + 1) for FF_ROPE_PAIRS or (i, i + rotary / 2) for FF_ROPE_HALVES, which become
+ *   scale * (y0 cos t - y1 sin t, y0 sin t + y1 cos t),  t = positions[row, i * axes / (rotary / 2)] * frequencies[i]
+ * (radians). positions [rows, axes] of position_bytes (4 or 8, signed), frequencies [rotary / 2] of frequency_bytes (4:
+ * f32, 8: f64). The other columns of the heads are copied. out may be x itself (ldo == ldx; the other columns stay), and
+ * must not overlap it otherwise. head_dim at most 1024.
+ */
+int ff_rope(const void* x, int dtype, int64_t ldx, void* out, int64_t ldo, int rows, int heads, int head_dim, int start,
+            int rotary, int pairing, const void* positions, int position_bytes, int axes, const void* frequencies,
+            int frequency_bytes, float scale, void* stream);
+
+/*
+ * The end of a block and the norm before the next one, for rows of cols columns (at most 16376):
+ *   out    = alpha * x + scale * act(gate) * post(y)
+ *   normed = pre(out), of out before it is rounded
+ * post and pre: FF_NORM_NONE, FF_NORM_RMS (v / rms(v) * w + b) or FF_NORM_LAYER ((v - mean) / std * w + b), f32, weights
+ * and biases [cols] or NULL; pre is FF_NORM_NONE exactly if normed is NULL. gate: NULL, or [.., gate_cols] with gate_cols
+ * 1 or cols, in f32 or y's type, row r reading gate row r / gate_rows (row stride ldg). scale [cols] f32 or NULL. x and
+ * out have x_type, y and normed y_type: the same, or x in f32. All matrices have any alignment of their type and any row
+ * stride of at least cols (16-byte rows are the fastest). out may be x and normed may be y (equal strides); nothing else
+ * may overlap.
+ */
+#define FF_NORM_NONE 0
+#define FF_GATE_PLAIN 0
+#define FF_GATE_SIGMOID 1
+#define FF_GATE_TANH 2
+typedef struct ff_norm_residual_args {
+  const void* x;
+  int64_t ldx;
+  const void* y;
+  int64_t ldy;
+  void* out;
+  int64_t ldo;
+  void* normed;
+  int64_t ldn;
+  int x_type, y_type, rows, cols;
+  float alpha;
+  int post;
+  const float *post_w, *post_b;
+  float post_eps;
+  int pre;
+  const float *pre_w, *pre_b;
+  float pre_eps;
+  const void* gate;
+  int64_t ldg;
+  int gate_type, gate_cols, gate_rows, gate_act;
+  const float* scale;
+} ff_norm_residual_args;
+int ff_norm_residual(const ff_norm_residual_args* args, void* stream);
+
+/*
+ * Attention of queries to keys and values of another length, f32 softmax and accumulation:
+ *   out = softmax(scale * q k^T over the keys that take part) v
+ * for every sequence and head. q and out [q_rows, heads * head_dim], k and v [k_rows, kv_heads * head_dim] of type dtype
+ * (FF_F16, FF_BF16), 16-byte aligned, row strides multiples of 8 elements (unless there is one row). heads is a multiple
+ * of kv_heads; query head h reads key head h / (heads / kv_heads). head_dim: a multiple of 16 up to 128. scale > 0.
+ * Sequence b has the queries [q_start[b], q_start[b + 1]) and the keys [k_start[b], k_start[b + 1]), of which the first
+ * k_len[b] take part (k_len NULL: all). q_start or k_start NULL: equal pieces of q_rows / sequences or k_rows / sequences
+ * rows. Starts are ascending int32 values on the device, bounded by the kernels to the rows there are; rows of out
+ * outside the sequences are left as they were. mask: NULL, or a byte per row of k, zero for a key that does not take
+ * part. A query without keys gives zeros. Nothing of a key or value that does not take part counts, infinities and NaN
+ * neither. workspace: device memory, 16-byte aligned, of at least ff_cross_attention_workspace_bytes(...) bytes (which
+ * may be 0), free again once the call's work on the stream is done. out must not overlap the inputs.
+ */
+int64_t ff_cross_attention_workspace_bytes(int q_rows, int k_rows, int sequences, int heads, int kv_heads, int head_dim);
+int ff_cross_attention(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, void* out,
+                       int64_t ldo, int dtype, int q_rows, int k_rows, int sequences, const int32_t* q_start,
+                       const int32_t* k_start, const int32_t* k_len, const uint8_t* mask, int heads, int kv_heads,
+                       int head_dim, float scale, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------- stem, norm, head */
 /*
  * images [B, S, S, 3] uint8 -> patches [B * (S/p)^2, k_pad] fp16 with (kh, kw, c) column order
