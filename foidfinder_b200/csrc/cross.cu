@@ -41,5 +41,6 @@ extern "C" int ff_cross_attention(const void* q, int64_t ldq, const void* k, int
              "ff_cross_attention: a workspace of %lld bytes, 16-byte aligned, is needed", static_cast<long long>(plan.workspace));
   const CrossArgs a{q,       ldq,     k,     ldk,  v,     ldv,      out,      ldo, q_rows, k_rows, sequences, q_start,
                     k_start, k_len,   mask,  heads, kv_heads, head_dim, scale * 1.4426950408889634f};
+  if (!plan.few) return cross_tc(a, dtype == FF_BF16, static_cast<cudaStream_t>(stream));
   return cross_few(a, dtype == FF_BF16, plan, workspace, static_cast<cudaStream_t>(stream));
 }

@@ -48,10 +48,14 @@ __device__ __forceinline__ Piece key_piece(const CrossArgs& a, int b) {
 // Few queries per sequence. splits: parts of every sequence's keys that CTAs of their own work on (their results are
 // joined by a second kernel through the workspace).
 struct CrossFewPlan {
+  bool few;  // whether this kernel takes the call
   int row_tiles, passes, splits;
   int64_t workspace;
 };
 CrossFewPlan cross_few_plan(int q_rows, int k_rows, int sequences, int heads, int kv_heads, int dim);
 int cross_few(const CrossArgs& a, bool bf16, const CrossFewPlan& plan, void* workspace, cudaStream_t s);
+
+// Many queries per sequence.
+int cross_tc(const CrossArgs& a, bool bf16, cudaStream_t s);
 
 }  // namespace ff

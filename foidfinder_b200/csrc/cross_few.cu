@@ -364,6 +364,8 @@ int launch_few_type(const FewArgs& a, int row_tiles, cudaStream_t s) {
 
 CrossFewPlan cross_few_plan(int q_rows, int k_rows, int sequences, int heads, int kv_heads, int dim) {
   CrossFewPlan plan{};
+  plan.few = static_cast<int64_t>(q_rows) <= 64LL * sequences || k_rows == 0;
+  if (!plan.few) return plan;
   const int64_t rows = (static_cast<int64_t>(q_rows) + sequences - 1) / sequences * (heads / kv_heads);
   plan.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
   plan.passes = static_cast<int>(std::max<int64_t>(1, (rows + 16 * plan.row_tiles - 1) / (16 * plan.row_tiles)));

@@ -1,0 +1,559 @@
+// Attention of many queries per sequence to its keys and values on the 5th-generation tensor cores (tcgen05).
+//   out = softmax(scale q k^T) v, head by head, keys that do not take part left out
+//
+// Bound by the exponentials (one per query, key and head) and the hand-overs between tensor core and softmax. Persistent
+// CTAs (one per SM, 320 threads, all 512 TMEM columns) walk items: up to 256 queries (two tiles of 128) of one sequence
+// and head, against that sequence's keys in tiles of 128; consecutive items overlap in the pipeline.
+//   warp 0     loads, by TMA: an item's queries, and key and value tiles in turn through one ring. A tile's rows are rows of
+//              the whole matrix, whatever sequence they belong to.
+//   warp 1     MMAs, by one elected thread: S_i = Q_i K^T to TMEM columns [128 i, +128), and O_i += P_i V, P_i read from where
+//              S_i was, to columns [256 + 128 i, +dim). Order per key tile j: PV_0(j), S_0(j + 1), PV_1(j), S_1(j + 1); MMAs of
+//              one thread execute in order, so S_i(j + 1) finds P_i(j) consumed. Each P V starts with the first 64 keys, as
+//              soon as their P is there.
+//   warps 2-5  softmax of query tile 0, warps 6-9 of tile 1, a query per thread: the row of S in registers (one pass over
+//              TMEM), its maximum, P = 2^(s - m + 7) in 16 bits back over S, the sum of P in f32 before that rounding. O and
+//              the sum are rescaled only when the maximum has grown by 2^8 since the last time, which keeps P below 2^15.
+// Keys that take no part (past the sequence's end, or masked) get P = 0, and their rows of the value tile are overwritten
+// with zeros in shared memory before the product, so that nothing they hold (NaN, infinities) counts. Both groups of
+// softmax warps write the same zeros, each before it lets its own product start.
+#include <algorithm>
+
+#include "common.h"
+#include "cross.h"
+#include "fp4.cuh"
+
+namespace ff {
+
+namespace {
+
+constexpr int kBQ = 128, kBK = 128;
+constexpr int kAtom = 128 * 128;  // bytes: 128 rows of 64 columns, 128-byte swizzle
+constexpr int kTcThreads = 320;
+constexpr int kTable = 64;  // items of a CTA that are looked up ahead, all at once
+__host__ __device__ constexpr int q_buffers(int atoms) { return atoms == 1 ? 2 : 1; }
+__host__ __device__ constexpr int ring_slots(int atoms) { return atoms == 1 ? 8 : 5; }
+__host__ __device__ constexpr int off_ring(int atoms) { return q_buffers(atoms) * 2 * atoms * kAtom; }
+__host__ __device__ constexpr int off_table(int atoms) { return off_ring(atoms) + ring_slots(atoms) * atoms * kAtom; }
+__host__ __device__ constexpr int off_bars(int atoms) { return off_table(atoms) + kTable * 16; }
+__host__ __device__ constexpr int tc_smem(int atoms) { return 1024 + off_bars(atoms) + 256; }
+static_assert(tc_smem(1) <= 232448 && tc_smem(2) <= 232448, "shared memory of a CTA");
+
+__host__ __device__ constexpr uint32_t t_s(int i) { return 128u * i; }
+__host__ __device__ constexpr uint32_t t_o(int i) { return 256u + 128u * i; }
+constexpr float kGrowth = 8.f;  // powers of two by which the maximum may grow before O is rescaled
+constexpr float kUp = 7.f;      // P = 2^(x + 7): at most 2^15, in fp16's range
+
+struct TcArgs {
+  CrossArgs p;
+  int tiles_per_seq;  // equal pieces: items of 256 queries per sequence and head; 0: by q_start
+  int64_t items;
+  int* err;
+};
+
+// Up to 256 queries [q, q + nq) of a head against the keys [k, k + nk).
+struct Item {
+  int q, nq, k, nk;
+};
+
+// Value tile as MN-major operand: key rows of 128 bytes (64 columns), 8-row groups 1024 bytes apart, the next 64 columns an atom
+// further.
+__device__ __forceinline__ uint64_t sdesc_v(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(kAtom >> 4) << 16;
+  d |= static_cast<uint64_t>(1024u >> 4) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(2u) << 61;
+  return d;
+}
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Item `n` of this CTA (nq == 0: none). Head fastest, then the 256-query tiles of a sequence. By q_start, tile t of
+// sequence b is slot q_start[b] / 256 + b + t: slots of sequences do not overlap, and the one that holds a slot is found by halving.
+__device__ Item item_at(const TcArgs& a, int64_t it) {
+  const CrossArgs& p = a.p;
+  const int slot = static_cast<int>(it / p.heads);
+  int b, tile;
+  if (a.tiles_per_seq > 0) {
+    b = slot / a.tiles_per_seq;
+    tile = slot - b * a.tiles_per_seq;
+  } else {
+    auto first = [&](int i) { return min(max(__ldg(p.q_start + i), 0), p.q_rows) / 256 + i; };
+    int lo = 0, hi = p.sequences - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (first(mid) <= slot) lo = mid;
+      else hi = mid - 1;
+    }
+    b = lo;
+    tile = slot - first(b);
+  }
+  const Piece q = query_piece(p, b);
+  Item r{0, 0, 0, 0};
+  if (tile < 0 || static_cast<int64_t>(tile) * 256 >= q.n) return r;
+  r.q = q.at + tile * 256;
+  r.nq = min(256, q.n - tile * 256);
+  const Piece k = key_piece(p, b);
+  r.k = k.at;
+  r.nk = k.n;
+  return r;
+}
+
+// O (dim TMEM columns from `to`) scaled by corr; out of line, it is rare.
+__device__ __noinline__ void rescale(uint32_t to, int dim, float corr) {
+  for (int c = 0; c < dim; c += 16) {
+    uint32_t o[16];
+    tmem_ld16(to + c, o);
+    tmem_ld_wait();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+    tmem_st16(to + c, o);
+  }
+}
+
+template <class T, int ATOMS>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    cross_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                    const __grid_constant__ TcArgs a) {
+  constexpr int QB = q_buffers(ATOMS), SLOTS = ring_slots(ATOMS), TILE = ATOMS * kAtom;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Item* const table = reinterpret_cast<Item*>(smem + off_table(ATOMS));
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + off_bars(ATOMS));
+  uint64_t* q_full = bar;             // [QB]
+  uint64_t* q_empty = q_full + QB;    // [QB]
+  uint64_t* full = q_empty + QB;      // [SLOTS]
+  uint64_t* empty = full + SLOTS;     // [SLOTS]
+  uint64_t* s_full = empty + SLOTS;   // [2], per query tile
+  uint64_t* p_half = s_full + 2;      // [2]
+  uint64_t* p_full = p_half + 2;      // [2]
+  uint64_t* o_full = p_full + 2;      // [2]
+  uint64_t* drain = o_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const CrossArgs& p = a.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int dim = p.dim, group = p.heads / p.kv_heads;
+  int* const err = a.err;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < QB; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+    }
+    for (int i = 0; i < SLOTS; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_half[i], 4);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_full[i], 1);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_map(&tm_q);
+    tma_prefetch_map(&tm_k);
+    tma_prefetch_map(&tm_v);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  pdl_wait();
+  pdl_trigger();
+  for (int n = threadIdx.x; n < kTable; n += kTcThreads) {
+    const int64_t it = blockIdx.x + static_cast<int64_t>(n) * gridDim.x;
+    table[n] = it < a.items ? item_at(a, it) : Item{0, 0, 0, 0};
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  // The next item with queries (after the n-th), and its head.
+  auto advance = [&](int& n, Item& item, int& head) -> bool {
+    for (++n;; ++n) {
+      const int64_t it = blockIdx.x + static_cast<int64_t>(n) * gridDim.x;
+      if (it >= a.items) return false;
+      item = n < kTable ? table[n] : item_at(a, it);
+      head = static_cast<int>(it % p.heads);
+      if (item.nq > 0) return true;
+    }
+  };
+  // The same, with keys as well.
+  auto advance_work = [&](int& n, Item& item, int& head) -> bool {
+    while (advance(n, item, head))
+      if (item.nk > 0) return true;
+    return false;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ loads
+    if (elect_one()) {
+      int q_phase[QB], phase[SLOTS];
+#pragma unroll
+      for (int i = 0; i < QB; ++i) q_phase[i] = -1;
+#pragma unroll
+      for (int i = 0; i < SLOTS; ++i) phase[i] = -1;
+      bool ok = true;
+      int slot = 0, n = -1, head = 0;
+      uint32_t round = 0;  // of the ring
+      Item item;
+      for (int m = 0; ok && advance_work(n, item, head); ++m) {
+        const int qb = m % QB, tiles = item.nq > kBQ ? 2 : 1;
+        if (m >= QB && !mbar_wait<true>(&q_empty[qb], static_cast<uint32_t>(m / QB - 1) & 1u, abort_flag, err, kDevTimeoutAttn)) {
+          ok = false;
+          break;
+        }
+        mbar_arrive_expect_tx(&q_full[qb], tiles * TILE);
+        for (int i = 0; i < tiles; ++i)
+#pragma unroll
+          for (int c = 0; c < ATOMS; ++c)
+            tma_load_2d(smem + (2 * qb + i) * TILE + c * kAtom, &tm_q, &q_full[qb], head * dim + 64 * c, item.q + i * kBQ);
+        q_phase[qb] = (m / QB) & 1;
+        const int x = head / group * dim, nkv = (item.nk + kBK - 1) / kBK;
+        for (int j = 0; j < 2 * nkv; ++j) {  // K_0, V_0, K_1, V_1, ..
+          if (!mbar_wait<true>(&empty[slot], (round & 1u) ^ 1u, abort_flag, err, kDevTimeoutAttn)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&full[slot], TILE);
+#pragma unroll
+          for (int c = 0; c < ATOMS; ++c)
+            tma_load_2d(smem + off_ring(ATOMS) + slot * TILE + c * kAtom, j & 1 ? &tm_v : &tm_k, &full[slot], x + 64 * c, item.k + (j >> 1) * kBK);
+          phase[slot] = static_cast<int>(round & 1u);
+          if (++slot == SLOTS) {
+            slot = 0;
+            ++round;
+          }
+        }
+      }
+      // Normally everything has been consumed. After an abort, let issued copies land (bounded) before the CTA can exit.
+      if (!ok) {
+        const unsigned long long t0 = globaltimer();
+        for (int i = 0; i < QB; ++i)
+          if (q_phase[i] >= 0)
+            while (!mbar_try_wait(smem_u32(&q_full[i]), static_cast<uint32_t>(q_phase[i])) && globaltimer() - t0 < kWaitLimitNs) {
+            }
+        for (int i = 0; i < SLOTS; ++i)
+          if (phase[i] >= 0)
+            while (!mbar_try_wait(smem_u32(&full[i]), static_cast<uint32_t>(phase[i])) && globaltimer() - t0 < kWaitLimitNs) {
+            }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMAs
+    if (elect_one()) {
+      constexpr uint32_t fmt = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);  // both operands fp16 or bf16
+      const uint32_t id_o = idesc_f16(128, dim) | fmt | (1u << 16);  // B = V is MN-major
+      const int steps = dim / 16;
+      const uint32_t ring = smem_u32(smem) + off_ring(ATOMS);
+      // Keys of a tile that its products cover: all, or the sequence's last ones rounded up to 16.
+      auto width = [](int nk, int j) { return min(kBK, (nk - j * kBK + 15) & ~15); };
+      auto issue_s = [&](int i, int qb, int slot, int keys) {
+        const uint32_t id = idesc_f16(128, keys) | fmt;
+        const uint64_t qd = sdesc_k_sw128(smem_u32(smem) + (2 * qb + i) * TILE);
+        const uint64_t kd = sdesc_k_sw128(ring + slot * TILE);
+#pragma unroll
+        for (int k = 0; k < 4 * ATOMS; ++k)
+          if (k < steps) {
+            const uint64_t o = (k >> 2) * (kAtom >> 4) + (k & 3) * 2;
+            mma_f16(tmem + t_s(i), qd + o, kd + o, id, k > 0);
+          }
+        tc_commit(&s_full[i]);
+      };
+      auto issue_pv = [&](int i, int slot, int keys, int k0, bool first) {  // steps k0 .. k0 + 3 of 16 keys
+        const uint64_t vd = sdesc_v(ring + slot * TILE);
+#pragma unroll
+        for (int k = k0; k < k0 + 4; ++k)
+          if (16 * k < keys) mma_ts(tmem + t_o(i), tmem + t_s(i) + 8 * k, vd + static_cast<uint64_t>(k * 128), id_o, (first && k == 0) ? 0u : 1u);
+      };
+      bool ok = true;
+      auto wait = [&](uint64_t* b, uint32_t parity) {
+        if (ok) ok = mbar_wait(b, parity, abort_flag, err, kDevTimeoutAttn);
+        return ok;
+      };
+      int n = -1, head, m = 0, slot = 0;  // slot, round: of the current key tile's K
+      uint32_t round = 0, count[2] = {0, 0};
+      Item cur{}, nxt{};
+      bool have = advance_work(n, cur, head);
+      if (have && wait(&q_full[0], 0) && wait(&full[0], 0)) {
+        tc_fence_after();
+        issue_s(0, 0, 0, width(cur.nk, 0));
+        if (cur.nq > kBQ) issue_s(1, 0, 0, width(cur.nk, 0));
+        tc_commit(&empty[0]);
+        if (cur.nk <= kBK) tc_commit(&q_empty[0]);
+      }
+      while (have && ok) {
+        const bool more = advance_work(n, nxt, head), two = cur.nq > kBQ;
+        const int nkv = (cur.nk + kBK - 1) / kBK;
+        for (int j = 0; j < nkv && ok; ++j) {
+          const bool last = j == nkv - 1, next = !last || more;
+          int v_slot = slot + 1, k_slot = slot + 2;
+          uint32_t v_round = round, k_round = round;
+          if (v_slot >= SLOTS) v_slot -= SLOTS, ++v_round;
+          if (k_slot >= SLOTS) k_slot -= SLOTS, ++k_round;
+          const int keys = width(cur.nk, j);
+          const int next_keys = last ? width(nxt.nk, 0) : width(cur.nk, j + 1);  // unused without a next tile
+          const int next_m = last ? m + 1 : m;
+          auto pv = [&](int i) {
+            if (!wait(&p_half[i], count[i] & 1u)) return;
+            tc_fence_after();
+            issue_pv(i, v_slot, keys, 0, j == 0);
+            if (!wait(&p_full[i], count[i] & 1u)) return;
+            tc_fence_after();
+            issue_pv(i, v_slot, keys, 4, j == 0);
+            if (last) tc_commit(&o_full[i]);
+            ++count[i];
+          };
+          if (!wait(&full[v_slot], v_round & 1u)) break;
+          pv(0);
+          if (!ok) break;
+          if (next) {
+            if (!wait(&full[k_slot], k_round & 1u) || (last && !wait(&q_full[next_m % QB], static_cast<uint32_t>(next_m / QB) & 1u))) break;
+            tc_fence_after();
+            issue_s(0, next_m % QB, k_slot, next_keys);
+          }
+          if (two) pv(1);
+          if (!ok) break;
+          tc_commit(&empty[v_slot]);
+          if (next) {
+            if (last ? nxt.nq > kBQ : two) issue_s(1, next_m % QB, k_slot, next_keys);
+            tc_commit(&empty[k_slot]);
+            if (last ? nxt.nk <= kBK : j + 1 == nkv - 1) tc_commit(&q_empty[next_m % QB]);  // the last use of these queries
+          }
+          slot = k_slot;
+          round = k_round;
+        }
+        cur = nxt;
+        have = more;
+        ++m;
+      }
+      tc_commit(drain);
+      const unsigned long long t0 = globaltimer();
+      while (!mbar_try_wait(smem_u32(drain), 0)) {
+        if (globaltimer() - t0 > kWaitLimitNs) {
+          atomicCAS(err, 0, kDevTimeoutDrain);
+          break;
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ softmax and results
+    const int g = (warp - 2) >> 2, quarter = warp & 3;
+    const uint32_t ts = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + t_s(g);
+    const uint32_t to = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + t_o(g);
+    const int first_row = g * kBQ + quarter * 32;  // of this warp, in the item
+    bool ok = true;
+    int n = -1, head, v_slot = 1;
+    uint32_t v_round = 0, tiles = 0, items = 0;
+    Item item;
+    while (ok && advance(n, item, head)) {
+      const int64_t row = item.q + first_row + lane;
+      const bool store = first_row + lane < item.nq, active = first_row < item.nq;
+      T* const out = static_cast<T*>(p.out) + row * p.ldo + static_cast<int64_t>(head) * dim;
+      if (item.nk == 0) {
+        if (store)
+          for (int c = 0; c < dim; c += 8) *reinterpret_cast<uint4*>(out + c) = make_uint4(0, 0, 0, 0);
+        continue;
+      }
+      const int nkv = (item.nk + kBK - 1) / kBK;
+      if (g * kBQ >= item.nq) {  // this group has no queries here; the ring goes on
+        const uint32_t at = static_cast<uint32_t>(v_slot) + 2u * nkv;
+        v_round += at / SLOTS;
+        v_slot = static_cast<int>(at % SLOTS);
+        continue;
+      }
+      const uint8_t* const mask = p.mask != nullptr ? p.mask + item.k : nullptr;
+      uint32_t ahead[4];  // mask bytes of the next tile's keys 32 c + lane
+      auto fetch = [&](int j) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int key = j * kBK + 32 * c + lane;
+          ahead[c] = key < item.nk ? __ldg(mask + key) : 0;
+        }
+      };
+      if (mask != nullptr) fetch(0);
+      float m_ref = -INFINITY;
+      float2 sum = make_float2(0.f, 0.f);
+      for (int j = 0; j < nkv; ++j, ++tiles) {
+        const int left = item.nk - j * kBK;
+        uint32_t bits[4];  // keys that take part
+        bool every = left >= kBK;
+        if (mask != nullptr) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            bits[c] = __ballot_sync(0xffffffffu, ahead[c] != 0);
+            every = every && bits[c] == 0xffffffffu;
+          }
+          fetch(j + 1);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) bits[c] = left >= 32 * c + 32 ? 0xffffffffu : left <= 32 * c ? 0u : (1u << (left - 32 * c)) - 1u;
+        }
+        if (!mbar_wait(&s_full[g], tiles & 1u, abort_flag, err, kDevTimeoutAttn)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (!every) {  // zeros for the values of keys left out: thread i of the group has key i
+          if (!mbar_wait(&full[v_slot], v_round & 1u, abort_flag, err, kDevTimeoutAttn)) {
+            ok = false;
+            break;
+          }
+          const uint32_t mine = quarter == 0 ? bits[0] : quarter == 1 ? bits[1] : quarter == 2 ? bits[2] : bits[3];
+          if (!(mine >> lane & 1u)) {
+#pragma unroll
+            for (int c = 0; c < ATOMS; ++c) {
+              uint4* const v = reinterpret_cast<uint4*>(smem + off_ring(ATOMS) + v_slot * TILE + c * kAtom + (quarter * 32 + lane) * 128);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[i] = make_uint4(0, 0, 0, 0);
+            }
+          }
+          fence_async_smem();
+        }
+        v_slot += 2;
+        if (v_slot >= SLOTS) v_slot -= SLOTS, ++v_round;
+        float2 nm2 = make_float2(0.f, 0.f);
+        const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
+        uint32_t s[4][32];
+        if (active) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, s[c]);
+          tmem_ld_wait();
+          if (!every) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (!(bits[c] >> e & 1u)) s[c][e] = 0xff800000u;  // -inf
+          }
+          float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) mq[(e >> 1) & 3] = max3(mq[(e >> 1) & 3], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
+          const float m_new = fmaxf(m_ref, max3(mq[0], mq[1], fmaxf(mq[2], mq[3])) * p.scale_log2);
+          bool grown = false;
+          float corr = 1.f;
+          if (j == 0) {
+            m_ref = m_new;
+          } else if (m_new > m_ref + kGrowth) {
+            corr = ex2_approx(m_ref - m_new);  // 0 while there was no key
+            m_ref = m_new;
+            grown = true;
+          }
+          if (__any_sync(0xffffffffu, grown)) {
+            rescale(to, dim, corr);
+            sum.x *= corr;
+            sum.y *= corr;
+          }
+          const float nm = m_ref == -INFINITY ? 0.f : kUp - m_ref;  // no key so far: P = 2^-inf = 0
+          nm2 = make_float2(nm, nm);
+        }
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          if (active) {
+#pragma unroll
+            for (int c = 2 * hf; c < 2 * hf + 2; ++c) {
+              uint32_t pk[16];
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const float2 x = fma2(make_float2(__uint_as_float(s[c][2 * e]), __uint_as_float(s[c][2 * e + 1])), sc2, nm2);
+                const float2 w = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+                sum = add2(sum, w);
+                pk[e] = Pair16<T>::pack(w.x, w.y);
+              }
+              tmem_st16(ts + 16 * c, pk);
+            }
+          }
+          __syncwarp();
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(hf == 0 ? &p_half[g] : &p_full[g]);
+        }
+      }
+      if (!ok) break;
+      if (!mbar_wait(&o_full[g], items & 1u, abort_flag, err, kDevTimeoutAttn)) break;
+      ++items;
+      tc_fence_after();
+      if (active) {
+        const float l = sum.x + sum.y, inv = l == 0.f ? 0.f : 1.f / l;  // no key took part: zeros
+        for (int c = 0; c < dim; c += 16) {
+          uint32_t o[16];
+          tmem_ld16(to + c, o);
+          tmem_ld_wait();
+          if (store) {
+            uint32_t w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = Pair16<T>::pack(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+            *reinterpret_cast<uint4*>(out + c) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(out + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+          }
+        }
+      }
+      // The next item's first product into O waits for this group's next P, which comes after these reads.
+    }
+  }
+
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
+template <class T, int ATOMS>
+int launch_tc(const TcArgs& a, cudaStream_t s) {
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    if (cudaFuncSetAttribute(cross_tc_kernel<T, ATOMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, tc_smem(ATOMS)) != cudaSuccess)
+      return check_launch("cross_tc: cudaFuncSetAttribute");
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  const CrossArgs& p = a.p;
+  CUtensorMap maps[3];
+  const void* base[3] = {p.q, p.k, p.v};
+  const int64_t ld[3] = {p.ldq, p.ldk, p.ldv};
+  for (int i = 0; i < 3; ++i) {
+    const uint64_t cols = static_cast<uint64_t>(i == 0 ? p.heads : p.kv_heads) * p.dim, rows = i == 0 ? p.q_rows : p.k_rows;
+    const int rc = make_tmap_2d_pitched(&maps[i], base[i], std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                                        2, cols, rows, 2 * (rows > 1 ? static_cast<uint64_t>(ld[i]) : cols), 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc != FF_OK) return rc;
+  }
+  const int grid = static_cast<int>(std::min<int64_t>(a.items, sm_count()));
+  launch(cross_tc_kernel<T, ATOMS>, dim3(grid), dim3(kTcThreads), tc_smem(ATOMS), s, maps[0], maps[1], maps[2], a);
+  return check_launch("cross_tc_kernel");
+}
+
+}  // namespace
+
+int cross_tc(const CrossArgs& p, bool bf16, cudaStream_t s) {
+  TcArgs a{};
+  a.p = p;
+  a.tiles_per_seq = p.q_start == nullptr ? (p.q_rows / p.sequences + 255) / 256 : 0;
+  const int64_t slots = p.q_start == nullptr ? static_cast<int64_t>(p.sequences) * a.tiles_per_seq : static_cast<int64_t>(p.q_rows) / 256 + p.sequences;
+  FF_REQUIRE(slots <= 0x3fffffff, "ff_cross_attention: %lld query tiles", static_cast<long long>(slots));
+  a.items = slots * p.heads;
+  a.err = device_error_word();
+  FF_REQUIRE(a.err != nullptr, "ff_cross_attention: no device error word");
+  if (p.dim <= 64) return bf16 ? launch_tc<__nv_bfloat16, 1>(a, s) : launch_tc<__half, 1>(a, s);
+  return bf16 ? launch_tc<__nv_bfloat16, 2>(a, s) : launch_tc<__half, 2>(a, s);
+}
+
+}  // namespace ff
