@@ -6,13 +6,15 @@
 // and head, against that sequence's keys in tiles of 128; consecutive items overlap in the pipeline.
 //   warp 0     loads, by TMA: an item's queries, and key and value tiles in turn through one ring. A tile's rows are rows of
 //              the whole matrix, whatever sequence they belong to.
-//   warp 1     MMAs, by one elected thread: S_i = Q_i K^T to TMEM columns [128 i, +128), and O_i += P_i V, P_i read from where
-//              S_i was, to columns [256 + 128 i, +dim). Order per key tile j: PV_0(j), S_0(j + 1), PV_1(j), S_1(j + 1); MMAs of
-//              one thread execute in order, so S_i(j + 1) finds P_i(j) consumed. Each P V starts with the first 64 keys, as
-//              soon as their P is there.
-//   warps 2-5  softmax of query tile 0, warps 6-9 of tile 1, a query per thread: the row of S in registers (one pass over
-//              TMEM), its maximum, P = 2^(s - m + 7) in 16 bits back over S, the sum of P in f32 before that rounding. O and
-//              the sum are rescaled only when the maximum has grown by 2^8 since the last time, which keeps P below 2^15.
+//   warp 1     MMAs, by one elected thread: S_i = Q_i K^T and O_i += P_i V, P_i read from TMEM. Heads of up to 64 columns have
+//              room for S, P and O of both tiles beside one another: S_i(j + 1) is issued when the softmax has read S_i(j),
+//              while it still works on P_i(j). Wider heads have P over S: PV_i(j), then S_i(j + 1) (MMAs of one thread
+//              execute in order).
+//   warps 2-5  softmax of query tile 0, warps 6-9 of tile 1, a query per thread: 32 scores at a time, the next 32 on their
+//              way meanwhile, P = 2^(s - m + 7) in 16 bits, the sum of P in f32 before that rounding. m is the
+//              maximum at some earlier time: the exponentials start at once, and the new maximum is found beside them.
+//              Only where it has grown by more than 2^8 (P could pass 2^15, fp16's range) do m, O, the sum and the P so
+//              far get rescaled and the 32 exponentials repeated.
 // Keys that take no part (past the sequence's end, or masked) get P = 0, and their rows of the value tile are overwritten
 // with zeros in shared memory before the product, so that nothing they hold (NaN, infinities) counts. Both groups of
 // softmax warps write the same zeros, each before it lets its own product start.
@@ -35,11 +37,19 @@ __host__ __device__ constexpr int ring_slots(int atoms) { return atoms == 1 ? 8 
 __host__ __device__ constexpr int off_ring(int atoms) { return q_buffers(atoms) * 2 * atoms * kAtom; }
 __host__ __device__ constexpr int off_table(int atoms) { return off_ring(atoms) + ring_slots(atoms) * atoms * kAtom; }
 __host__ __device__ constexpr int off_bars(int atoms) { return off_table(atoms) + kTable * 16; }
-__host__ __device__ constexpr int tc_smem(int atoms) { return 1024 + off_bars(atoms) + 256; }
+__host__ __device__ constexpr int tc_smem(int atoms) { return 1024 + off_bars(atoms) + 384; }
 static_assert(tc_smem(1) <= 232448 && tc_smem(2) <= 232448, "shared memory of a CTA");
 
+// TMEM columns of query tile i.
 __host__ __device__ constexpr uint32_t t_s(int i) { return 128u * i; }
-__host__ __device__ constexpr uint32_t t_o(int i) { return 256u + 128u * i; }
+template <int ATOMS>
+__host__ __device__ constexpr uint32_t t_p(int i) {
+  return ATOMS == 1 ? 256u + 64u * i : t_s(i);
+}
+template <int ATOMS>
+__host__ __device__ constexpr uint32_t t_o(int i) {
+  return ATOMS == 1 ? 384u + 64u * i : 256u + 128u * i;
+}
 constexpr float kGrowth = 8.f;  // powers of two by which the maximum may grow before O is rescaled
 constexpr float kUp = 7.f;      // P = 2^(x + 7): at most 2^15, in fp16's range
 
@@ -118,10 +128,27 @@ __device__ __noinline__ void rescale(uint32_t to, int dim, float corr) {
   }
 }
 
+// The same for the first `chunks` times 32 weights of P.
+template <class T>
+__device__ __noinline__ void rescale_p(uint32_t ts, int chunks, float corr) {
+  for (int c = 0; c < chunks; ++c) {
+    uint32_t w[16];
+    tmem_ld16(ts + 16 * c, w);
+    tmem_ld_wait();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float2 v = Pair16<T>::unpack(w[e]);
+      w[e] = Pair16<T>::pack(v.x * corr, v.y * corr);
+    }
+    tmem_st16(ts + 16 * c, w);
+  }
+}
+
 template <class T, int ATOMS>
 __global__ void __launch_bounds__(kTcThreads, 1)
     cross_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                     const __grid_constant__ TcArgs a) {
+  constexpr bool APART = ATOMS == 1;  // P beside S
   constexpr int QB = q_buffers(ATOMS), SLOTS = ring_slots(ATOMS), TILE = ATOMS * kAtom;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -132,10 +159,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint64_t* full = q_empty + QB;      // [SLOTS]
   uint64_t* empty = full + SLOTS;     // [SLOTS]
   uint64_t* s_full = empty + SLOTS;   // [2], per query tile
-  uint64_t* p_half = s_full + 2;      // [2]
-  uint64_t* p_full = p_half + 2;      // [2]
-  uint64_t* o_full = p_full + 2;      // [2]
-  uint64_t* drain = o_full + 2;
+  uint64_t* p_full = s_full + 2;      // [2]
+  uint64_t* s_read = p_full + 2;      // [2]
+  uint64_t* pv_done = s_read + 2;     // [2]
+  uint64_t* drain = pv_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -154,9 +181,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_half[i], 4);
       mbar_init(&p_full[i], 4);
-      mbar_init(&o_full[i], 1);
+      mbar_init(&s_read[i], 4);
+      mbar_init(&pv_done[i], 1);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -274,15 +301,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
         tc_commit(&s_full[i]);
       };
-      auto issue_pv = [&](int i, int slot, int keys, int k0, bool first) {  // steps k0 .. k0 + 3 of 16 keys
+      auto issue_pv = [&](int i, int slot, int keys, bool first) {
         const uint64_t vd = sdesc_v(ring + slot * TILE);
 #pragma unroll
-        for (int k = k0; k < k0 + 4; ++k)
-          if (16 * k < keys) mma_ts(tmem + t_o(i), tmem + t_s(i) + 8 * k, vd + static_cast<uint64_t>(k * 128), id_o, (first && k == 0) ? 0u : 1u);
+        for (int k = 0; k < 8; ++k)
+          if (16 * k < keys) mma_ts(tmem + t_o<ATOMS>(i), tmem + t_p<ATOMS>(i) + 8 * k, vd + static_cast<uint64_t>(k * 128), id_o, (first && k == 0) ? 0u : 1u);
       };
       bool ok = true;
       auto wait = [&](uint64_t* b, uint32_t parity) {
-        if (ok) ok = mbar_wait(b, parity, abort_flag, err, kDevTimeoutAttn);
+        if (ok) ok = mbar_wait<true>(b, parity, abort_flag, err, kDevTimeoutAttn);
         return ok;
       };
       int n = -1, head, m = 0, slot = 0;  // slot, round: of the current key tile's K
@@ -308,31 +335,35 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           const int keys = width(cur.nk, j);
           const int next_keys = last ? width(nxt.nk, 0) : width(cur.nk, j + 1);  // unused without a next tile
           const int next_m = last ? m + 1 : m;
+          const int qb = next_m % QB;
           auto pv = [&](int i) {
-            if (!wait(&p_half[i], count[i] & 1u)) return;
-            tc_fence_after();
-            issue_pv(i, v_slot, keys, 0, j == 0);
             if (!wait(&p_full[i], count[i] & 1u)) return;
             tc_fence_after();
-            issue_pv(i, v_slot, keys, 4, j == 0);
-            if (last) tc_commit(&o_full[i]);
+            issue_pv(i, v_slot, keys, j == 0);
+            tc_commit(&pv_done[i]);
             ++count[i];
           };
-          if (!wait(&full[v_slot], v_round & 1u)) break;
-          pv(0);
-          if (!ok) break;
-          if (next) {
-            if (!wait(&full[k_slot], k_round & 1u) || (last && !wait(&q_full[next_m % QB], static_cast<uint32_t>(next_m / QB) & 1u))) break;
-            tc_fence_after();
-            issue_s(0, next_m % QB, k_slot, next_keys);
-          }
-          if (two) pv(1);
+          // One query tile: P V of this key tile, S of the next one, in the order that TMEM allows.
+          auto turn = [&](int i, bool here, bool there) {
+            if (APART && here && !wait(&s_read[i], count[i] & 1u)) return;
+            if (APART && there) {
+              tc_fence_after();
+              issue_s(i, qb, k_slot, next_keys);
+            }
+            if (here) pv(i);
+            if (!APART && there && ok) issue_s(i, qb, k_slot, next_keys);
+          };
+          if (!wait(&full[v_slot], v_round & 1u) || (next && !wait(&full[k_slot], k_round & 1u)) ||
+              (next && last && !wait(&q_full[qb], static_cast<uint32_t>(next_m / QB) & 1u)))
+            break;
+          tc_fence_after();
+          turn(0, true, next);
+          if (ok) turn(1, two, next && (last ? nxt.nq > kBQ : two));
           if (!ok) break;
           tc_commit(&empty[v_slot]);
           if (next) {
-            if (last ? nxt.nq > kBQ : two) issue_s(1, next_m % QB, k_slot, next_keys);
             tc_commit(&empty[k_slot]);
-            if (last ? nxt.nk <= kBK : j + 1 == nkv - 1) tc_commit(&q_empty[next_m % QB]);  // the last use of these queries
+            if (last ? nxt.nk <= kBK : j + 1 == nkv - 1) tc_commit(&q_empty[qb]);  // the last use of these queries
           }
           slot = k_slot;
           round = k_round;
@@ -354,11 +385,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // ------------------------------------------------------------ softmax and results
     const int g = (warp - 2) >> 2, quarter = warp & 3;
     const uint32_t ts = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + t_s(g);
-    const uint32_t to = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + t_o(g);
+    const uint32_t tp = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + t_p<ATOMS>(g);
+    const uint32_t to = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + t_o<ATOMS>(g);
     const int first_row = g * kBQ + quarter * 32;  // of this warp, in the item
     bool ok = true;
     int n = -1, head, v_slot = 1;
-    uint32_t v_round = 0, tiles = 0, items = 0;
+    uint32_t v_round = 0, tiles = 0;
     Item item;
     while (ok && advance(n, item, head)) {
       const int64_t row = item.q + first_row + lane;
@@ -386,7 +418,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       };
       if (mask != nullptr) fetch(0);
-      float m_ref = -INFINITY;
+      float shift = 0.f;  // 7 - m, once there is an m
+      bool set = false;
       float2 sum = make_float2(0.f, 0.f);
       for (int j = 0; j < nkv; ++j, ++tiles) {
         const int left = item.nk - j * kBK;
@@ -426,69 +459,78 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         v_slot += 2;
         if (v_slot >= SLOTS) v_slot -= SLOTS, ++v_round;
-        float2 nm2 = make_float2(0.f, 0.f);
-        const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
-        uint32_t s[4][32];
         if (active) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, s[c]);
+          const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
+          uint32_t s[2][32];
+          tmem_ld32(ts, s[0]);
           tmem_ld_wait();
-          if (!every) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < 4; ++c) {
+            if (c < 3) tmem_ld32(ts + 32 * (c + 1), s[(c + 1) & 1]);
+            uint32_t(&sc)[32] = s[c & 1];
+            if (!every) {
 #pragma unroll
               for (int e = 0; e < 32; ++e)
-                if (!(bits[c] >> e & 1u)) s[c][e] = 0xff800000u;  // -inf
-          }
-          float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) mq[(e >> 1) & 3] = max3(mq[(e >> 1) & 3], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
-          const float m_new = fmaxf(m_ref, max3(mq[0], mq[1], fmaxf(mq[2], mq[3])) * p.scale_log2);
-          bool grown = false;
-          float corr = 1.f;
-          if (j == 0) {
-            m_ref = m_new;
-          } else if (m_new > m_ref + kGrowth) {
-            corr = ex2_approx(m_ref - m_new);  // 0 while there was no key
-            m_ref = m_new;
-            grown = true;
-          }
-          if (__any_sync(0xffffffffu, grown)) {
-            rescale(to, dim, corr);
-            sum.x *= corr;
-            sum.y *= corr;
-          }
-          const float nm = m_ref == -INFINITY ? 0.f : kUp - m_ref;  // no key so far: P = 2^-inf = 0
-          nm2 = make_float2(nm, nm);
-        }
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          if (active) {
-#pragma unroll
-            for (int c = 2 * hf; c < 2 * hf + 2; ++c) {
-              uint32_t pk[16];
+                if (!(bits[c] >> e & 1u)) sc[e] = 0xff800000u;  // -inf
+            }
+            uint32_t pk[16];
+            float2 part;
+            auto exponentials = [&]() -> float {  // -> the largest exponent
+              const float2 sh2 = make_float2(shift, shift);
+              float mx[2] = {-INFINITY, -INFINITY};
+              float2 ps[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
               for (int e = 0; e < 16; ++e) {
-                const float2 x = fma2(make_float2(__uint_as_float(s[c][2 * e]), __uint_as_float(s[c][2 * e + 1])), sc2, nm2);
+                const float2 x = fma2(make_float2(__uint_as_float(sc[2 * e]), __uint_as_float(sc[2 * e + 1])), sc2, sh2);
+                mx[e & 1] = max3(mx[e & 1], x.x, x.y);
                 const float2 w = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-                sum = add2(sum, w);
+                ps[e & 1] = add2(ps[e & 1], w);
                 pk[e] = Pair16<T>::pack(w.x, w.y);
               }
-              tmem_st16(ts + 16 * c, pk);
+              part = add2(ps[0], ps[1]);
+              return fmaxf(mx[0], mx[1]);
+            };
+            const float mx = exponentials();
+            if (c == 0 && tiles > 0) {  // before P and O are touched: the last product has read and written them
+              ok = mbar_wait(&pv_done[g], (tiles - 1) & 1u, abort_flag, err, kDevTimeoutAttn);
+              tc_fence_after();
+            }
+            const bool grown = mx > kUp + kGrowth || (!set && mx > -INFINITY);
+            if (__any_sync(0xffffffffu, grown)) {
+              if (c < 3) tmem_ld_wait();  // nothing on its way into registers across the calls
+              float corr = 1.f;
+              if (grown) {
+                const float now = kUp - (mx - shift);
+                corr = set ? ex2_approx(now - shift) : 0.f;  // without an m there was no key, and all is zero
+                shift = now;
+                set = true;
+              }
+              if (j > 0) rescale(to, dim, corr);
+              if (c > 0) rescale_p<T>(tp, c, corr);
+              sum.x *= corr;
+              sum.y *= corr;
+              exponentials();
+            }
+            sum = add2(sum, part);
+            tmem_st16(tp + 16 * c, pk);
+            if (c < 3) tmem_ld_wait();
+            if (APART && c == 2) {  // all of S is in registers
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&s_read[g]);
             }
           }
-          __syncwarp();
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(hf == 0 ? &p_half[g] : &p_full[g]);
+        } else if (APART && lane == 0) {
+          mbar_arrive(&s_read[g]);
         }
+        __syncwarp();
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[g]);
       }
       if (!ok) break;
-      if (!mbar_wait(&o_full[g], items & 1u, abort_flag, err, kDevTimeoutAttn)) break;
-      ++items;
+      if (!mbar_wait(&pv_done[g], (tiles - 1) & 1u, abort_flag, err, kDevTimeoutAttn)) break;
       tc_fence_after();
       if (active) {
         const float l = sum.x + sum.y, inv = l == 0.f ? 0.f : 1.f / l;  // no key took part: zeros
