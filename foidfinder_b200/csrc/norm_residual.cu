@@ -8,9 +8,11 @@
 // rows of up to 1024 columns (32 values per lane), wider rows are shared by more warps, whose sums meet in shared memory.
 // All sums, statistics and products are f32; each output is rounded once.
 //
-// Three ways to deal out the columns: FULL, 16-byte chunks (8 columns) that divide the row; SHIFTED, the same when rows start
-// off a chunk but all matrices by the same amount, so that only a row's first and last chunk are taken apart; STRIDED, for
-// all else, neighbouring columns to neighbouring lanes, one by one.
+// Three ways to deal out the columns. FULL: 16-byte chunks (8 columns of 16 bits) that divide the rows of every matrix. PAIRS:
+// neighbouring pairs of columns to neighbouring lanes, where all rows and the width are whole pairs; parameters then come
+// in whole 8-byte words, and a warp's pairs still fill cache lines. SINGLES: columns one by one, for any alignment and
+// width. (16-byte words shifted into place took 146-200 us for 16400 x 2730 with a gate: code for each alignment and
+// edge, and waits for the edges.)
 #include <algorithm>
 
 #include "common.h"
@@ -22,14 +24,13 @@ namespace {
 
 constexpr int kChunk = 8;
 constexpr int kNrThreads = 128;    // of a CTA whose warps take rows of their own
-constexpr int kNrMaxCols = 16376;  // 16 warps x 32 lanes x 4 chunks, less a shift of up to 7
+constexpr int kNrMaxCols = 16384;  // 16 warps x 32 lanes x 4 chunks of 8
 
-enum class Deal { kFull, kShifted, kStrided };
+enum class Deal { kFull, kPairs, kSingles };
 
 struct NrArgs {
   ff_norm_residual_args p;
-  int lanes;         // per row: 4, 8, 16 or 32, or 32 times the row's warps
-  bool gate_chunks;  // a 16-bit gate for every element, dealt out as y is
+  int lanes;  // per row: 4, 8, 16 or 32, or 32 times the row's warps
 };
 
 // Conversions of 8 values between memory and f32 pairs.
@@ -48,7 +49,6 @@ struct Raw {
 #pragma unroll
     for (int i = 0; i < static_cast<int>(sizeof(w) / 16); ++i) w[i] = make_uint4(0, 0, 0, 0);
   }
-  __device__ __forceinline__ T& at(int i) { return reinterpret_cast<T*>(w)[i]; }
   __device__ __forceinline__ uint32_t word(int i) const {
     const uint4& u = w[i >> 2];
     return (i & 3) == 0 ? u.x : (i & 3) == 1 ? u.y : (i & 3) == 2 ? u.z : u.w;
@@ -58,6 +58,10 @@ struct Raw {
       return make_float2(__uint_as_float(word(2 * i)), __uint_as_float(word(2 * i + 1)));
     else
       return Pair16<T>::unpack(word(i));
+  }
+  __device__ __forceinline__ void set_word(int i, uint32_t x) {
+    uint4& u = w[i >> 2];
+    ((i & 3) == 0 ? u.x : (i & 3) == 1 ? u.y : (i & 3) == 2 ? u.z : u.w) = x;
   }
   __device__ __forceinline__ void set(const float2 (&v)[4]) {
     if constexpr (sizeof(T) == 4) {
@@ -74,86 +78,92 @@ __device__ __forceinline__ float as_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float as_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float as_f32(float v) { return v; }
 
-// The columns of one thread: chunk k, value e.
+// The columns of one thread: chunk k, value e of its eight.
 template <Deal D>
 struct Columns {
-  int cols, first, step;  // FULL and SHIFTED: column of chunk 0's value 0, and between chunks; STRIDED: of value 0 and values
-  int shift;
-  __device__ __forceinline__ Columns(int cols, int lane, int threads, int shift) : cols(cols), shift(shift) {
-    first = D == Deal::kStrided ? lane : lane * kChunk - shift;
-    step = D == Deal::kStrided ? threads : threads * kChunk;
-  }
-  __device__ __forceinline__ int at(int k, int e) const {
-    return D == Deal::kStrided ? first + (k * kChunk + e) * step : first + k * step + e;
-  }
-  __device__ __forceinline__ bool holds(int k, int e) const {
-    const int c = at(k, e);
-    return c < cols && (D != Deal::kShifted || c >= 0);
-  }
-  // Whether all of chunk k is there (FULL: all or nothing).
-  __device__ __forceinline__ bool whole(int k) const {
-    if (D == Deal::kStrided) return false;
-    const int c = first + k * step;
-    return c + kChunk <= cols && (D == Deal::kFull || c >= 0);
-  }
+  static constexpr int kUnit = D == Deal::kFull ? kChunk : D == Deal::kPairs ? 2 : 1;  // neighbouring columns of a lane
+  int cols, first, step;  // of unit 0, and between units
+  __device__ __forceinline__ Columns(int cols, int lane, int lanes) : cols(cols), first(lane * kUnit), step(lanes * kUnit) {}
+  __device__ __forceinline__ int at(int k, int e) const { return first + (k * kChunk + e) / kUnit * step + e % kUnit; }
 
   template <class T>
   __device__ __forceinline__ void load(const T* row, int k, Raw<T>& r) const {
-    r.clear();
-    if (whole(k)) {
-      r.load(row + at(k, 0));
-    } else if constexpr (D != Deal::kFull) {
+    if constexpr (D == Deal::kFull) {
+      r.clear();
+      if (at(k, 0) < cols) r.load(row + at(k, 0));
+    } else if constexpr (D == Deal::kPairs) {
 #pragma unroll
-      for (int e = 0; e < kChunk; ++e)
-        if (holds(k, e)) r.at(e) = row[at(k, e)];
+      for (int e = 0; e < 4; ++e) {
+        const bool there = at(k, 2 * e) < cols;
+        if constexpr (sizeof(T) == 4) {
+          const uint2 w = there ? *reinterpret_cast<const uint2*>(row + at(k, 2 * e)) : make_uint2(0, 0);
+          r.set_word(2 * e, w.x);
+          r.set_word(2 * e + 1, w.y);
+        } else {
+          r.set_word(e, there ? *reinterpret_cast<const uint32_t*>(row + at(k, 2 * e)) : 0u);
+        }
+      }
+    } else {
+      using B = typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type;
+      const B* const p = reinterpret_cast<const B*>(row);
+      B w[kChunk];
+#pragma unroll
+      for (int e = 0; e < kChunk; ++e) w[e] = at(k, e) < cols ? p[at(k, e)] : B(0);
+#pragma unroll
+      for (int i = 0; i < (sizeof(T) == 4 ? 8 : 4); ++i)
+        r.set_word(i, sizeof(T) == 4 ? w[i] : w[2 * i & 7] | static_cast<uint32_t>(w[(2 * i + 1) & 7]) << 16);
     }
   }
   template <class T>
   __device__ __forceinline__ void store(T* row, int k, const float2 (&v)[4]) const {
     Raw<T> r;
     r.set(v);
-    if (whole(k)) {
-      r.store(row + at(k, 0));
-    } else if constexpr (D != Deal::kFull) {
+    if constexpr (D == Deal::kFull) {
+      if (at(k, 0) < cols) r.store(row + at(k, 0));
+    } else if constexpr (D == Deal::kPairs) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (at(k, 2 * e) < cols) {
+          if constexpr (sizeof(T) == 4)
+            *reinterpret_cast<uint2*>(row + at(k, 2 * e)) = make_uint2(r.word(2 * e), r.word(2 * e + 1));
+          else
+            *reinterpret_cast<uint32_t*>(row + at(k, 2 * e)) = r.word(e);
+        }
+    } else {
+      using B = typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type;
+      B* const p = reinterpret_cast<B*>(row);
 #pragma unroll
       for (int e = 0; e < kChunk; ++e)
-        if (holds(k, e)) row[at(k, e)] = r.at(e);
+        if (at(k, e) < cols) p[at(k, e)] = static_cast<B>(sizeof(T) == 4 ? r.word(e) : r.word(e / 2) >> (16 * (e & 1)));
     }
   }
-  // f32 parameters of chunk k's columns (0 where there is none), 16-byte aligned but for STRIDED.
+  // f32 parameters of chunk k's columns (0 where there is none).
   __device__ __forceinline__ void parameters(const float* p, int k, float2 (&v)[4]) const {
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-    if (D == Deal::kFull || (D == Deal::kShifted && (shift & 3) == 0 && whole(k))) {
-      if (whole(k)) {
-        const float4* const q = reinterpret_cast<const float4*>(p + at(k, 0));
-        a = __ldg(q);
-        b = __ldg(q + 1);
-      }
+    if constexpr (D == Deal::kFull) {
+      const bool there = at(k, 0) < cols;
+      const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+      const float4 a = there ? __ldg(reinterpret_cast<const float4*>(p + at(k, 0))) : z, b = there ? __ldg(reinterpret_cast<const float4*>(p + at(k, 0)) + 1) : z;
       v[0] = make_float2(a.x, a.y);
       v[1] = make_float2(a.z, a.w);
       v[2] = make_float2(b.x, b.y);
       v[3] = make_float2(b.z, b.w);
-    } else if (D == Deal::kShifted && (shift & 1) == 0 && whole(k)) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = __ldg(reinterpret_cast<const float2*>(p + at(k, 2 * e)));
     } else {
+      Raw<float> r;
+      load(p, k, r);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        v[e] = make_float2(holds(k, 2 * e) ? __ldg(p + at(k, 2 * e)) : 0.f, holds(k, 2 * e + 1) ? __ldg(p + at(k, 2 * e + 1)) : 0.f);
+      for (int e = 0; e < 4; ++e) v[e] = r.pair(e);
     }
   }
   // Values past the row to 0.
   template <int K>
   __device__ __forceinline__ void trim(float2 (&v)[K][4]) const {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      if (whole(k)) continue;
+    for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (D == Deal::kFull || !holds(k, 2 * e)) v[k][e].x = 0.f;
-        if (D == Deal::kFull || !holds(k, 2 * e + 1)) v[k][e].y = 0.f;
+        if (at(k, 2 * e) >= cols) v[k][e].x = 0.f;
+        if (at(k, 2 * e + 1) >= cols) v[k][e].y = 0.f;
       }
-    }
   }
 };
 
@@ -227,17 +237,25 @@ __device__ __forceinline__ float exp_close(float x) {
   const float y = ex2_approx(t);
   return fabsf(t) < 126.f ? fmaf(y, lost * 0.693147181f, y) : y;
 }
-// Within a few 2^-24 of the value: 1 / (1 + e^-g), and for tanh 1 - 2 / (1 + e^2|g|), but its series
-// g (1 - g^2 / 3 + 2 g^4 / 15 - 17 g^6 / 315 + 62 g^8 / 2835 - 1382 g^10 / 155925) below 0.35 (the next term is 2^-25 of it there).
+__device__ __forceinline__ float reciprocal(float v) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(v));
+  return y;
+}
+// 1 / (1 + e^-g), and for tanh 1 - 2 / (1 + e^2|g|), but its series g (1 - g^2 / 3 + 2 g^4 / 15 - 17 g^6 / 315 + 62 g^8 / 2835 -
+// 1382 g^10 / 155925) below 0.35 (the next term is 2^-25 of it there). CLOSE (32-bit results): within a few 2^-24 of the
+// value; else within 2^-19, for results that are rounded to 12 bits at most.
+template <bool CLOSE>
 __device__ __forceinline__ float activate(float g, int act) {
-  if (act == FF_GATE_SIGMOID) return __fdividef(1.f, 1.f + exp_close(fminf(-g, 87.f)));
+  auto exponential = [](float x) { return CLOSE ? exp_close(x) : ex2_approx(x * 1.44269504f); };
+  if (act == FF_GATE_SIGMOID) return reciprocal(1.f + exponential(-g));
   if (act == FF_GATE_TANH) {
     const float a = fabsf(g), q = g * g;
     float s = fmaf(q, -8.863235530e-3f, 2.186948854e-2f);
     s = fmaf(q, s, -5.396825397e-2f);
     s = fmaf(q, s, 1.333333333e-1f);
     s = fmaf(q, s, -3.333333333e-1f);
-    const float far = 1.f - __fdividef(2.f, 1.f + exp_close(fminf(2.f * a, 87.f)));
+    const float far = 1.f - 2.f * reciprocal(1.f + exponential(2.f * a));
     return a < 0.35f ? fmaf(g * q, s, g) : g != g ? g : copysignf(far, g);
   }
   return g;
@@ -256,8 +274,8 @@ __global__ void __launch_bounds__(MULTI ? (K == 1 ? 1024 : 512) : kNrThreads, MU
   const int64_t r = real ? row : 0;
   const TY* const y = static_cast<const TY*>(p.y) + r * p.ldy;
   const TX* const x = static_cast<const TX*>(p.x) + r * p.ldx;
-  const int shift = D == Deal::kShifted ? static_cast<int>(reinterpret_cast<uintptr_t>(y) / sizeof(TY) % kChunk) : 0;
-  Columns<D> c(p.cols, in_row, lanes, shift);
+  TX* const out = static_cast<TX*>(p.out) + r * p.ldo;
+  Columns<D> c(p.cols, in_row, lanes);
   if (!real) c.first = p.cols;
   Raw<TY> raw[K];
   Raw<TX> xr[K];
@@ -270,15 +288,16 @@ __global__ void __launch_bounds__(MULTI ? (K == 1 ? 1024 : 512) : kNrThreads, MU
   for (int k = 0; k < K; ++k)
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[k][e] = raw[k].pair(e);
-  const int64_t gate_at = p.gate != nullptr ? r / p.gate_rows * p.ldg : 0;
-  if (a.gate_chunks) {  // under way during the norm
+  const int64_t gate_at = p.gate != nullptr ? static_cast<int64_t>(static_cast<uint32_t>(r) / static_cast<uint32_t>(p.gate_rows)) * p.ldg : 0;
+  const bool narrow = p.gate != nullptr && p.gate_cols > 1 && p.gate_type != FF_F32;  // a gate of 16 bits per column
+  if (narrow || (sizeof(TY) == 4 && p.gate != nullptr && p.gate_cols > 1)) {  // under way during the norm
 #pragma unroll
     for (int k = 0; k < K; ++k) c.load(static_cast<const TY*>(p.gate) + gate_at, k, raw[k]);
   }
   if (p.post != FF_NORM_NONE) norm<D, K, MULTI>(v, c, p.post, p.post_w, p.post_b, p.post_eps, lanes, part);
   if (p.gate != nullptr) {
     if (p.gate_cols == 1) {
-      const float g = activate(p.gate_type == FF_F32 ? static_cast<const float*>(p.gate)[gate_at] : as_f32(static_cast<const TY*>(p.gate)[gate_at]),
+      const float g = activate<true>(p.gate_type == FF_F32 ? static_cast<const float*>(p.gate)[gate_at] : as_f32(static_cast<const TY*>(p.gate)[gate_at]),
                                p.gate_act);
 #pragma unroll
       for (int k = 0; k < K; ++k)
@@ -288,20 +307,15 @@ __global__ void __launch_bounds__(MULTI ? (K == 1 ? 1024 : 512) : kNrThreads, MU
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         float2 g[4];
-        if (a.gate_chunks) {
+        if (narrow || sizeof(TY) == 4) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) g[e] = raw[k].pair(e);
-        } else if (p.gate_type == FF_F32) {
-          c.parameters(static_cast<const float*>(p.gate) + gate_at, k, g);
         } else {
-          const TY* const q = static_cast<const TY*>(p.gate) + gate_at;
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            g[e] = make_float2(c.holds(k, 2 * e) ? as_f32(q[c.at(k, 2 * e)]) : 0.f, c.holds(k, 2 * e + 1) ? as_f32(q[c.at(k, 2 * e + 1)]) : 0.f);
+          c.parameters(static_cast<const float*>(p.gate) + gate_at, k, g);
         }
         if (p.gate_act != FF_GATE_PLAIN) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) g[e] = make_float2(activate(g[e].x, p.gate_act), activate(g[e].y, p.gate_act));
+          for (int e = 0; e < 4; ++e) g[e] = make_float2(activate<sizeof(TX) == 4>(g[e].x, p.gate_act), activate<sizeof(TX) == 4>(g[e].y, p.gate_act));
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[k][e] = mul2(v[k][e], g[e]);
@@ -317,7 +331,6 @@ __global__ void __launch_bounds__(MULTI ? (K == 1 ? 1024 : 512) : kNrThreads, MU
       for (int e = 0; e < 4; ++e) v[k][e] = mul2(v[k][e], s[e]);
     }
   }
-  TX* const out = static_cast<TX*>(p.out) + r * p.ldo;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
 #pragma unroll
@@ -332,68 +345,61 @@ __global__ void __launch_bounds__(MULTI ? (K == 1 ? 1024 : 512) : kNrThreads, MU
   for (int k = 0; k < K; ++k) c.store(normed, k, v[k]);
 }
 
-template <class TX, class TY, int K, bool MULTI>
-void launch_nr_deal(const NrArgs& a, Deal deal, cudaStream_t s) {
+template <class TX, class TY, int K, Deal D, bool MULTI>
+void launch_nr(const NrArgs& a, cudaStream_t s) {
   const int rows = a.p.rows, per = kNrThreads / a.lanes;
-  const dim3 grid(MULTI ? rows : (rows + per - 1) / per), block(MULTI ? a.lanes : kNrThreads);
-  switch (deal) {
-    case Deal::kFull: launch(norm_residual_kernel<TX, TY, K, Deal::kFull, MULTI>, grid, block, 0, s, a); break;
-    case Deal::kShifted: launch(norm_residual_kernel<TX, TY, K, Deal::kShifted, MULTI>, grid, block, 0, s, a); break;
-    case Deal::kStrided: launch(norm_residual_kernel<TX, TY, K, Deal::kStrided, MULTI>, grid, block, 0, s, a); break;
+  launch(norm_residual_kernel<TX, TY, K, D, MULTI>, dim3(MULTI ? rows : (rows + per - 1) / per), dim3(MULTI ? a.lanes : kNrThreads), 0, s, a);
+}
+
+template <class TX, class TY, Deal D>
+void launch_nr_deal(NrArgs& a, int chunks, int wide, cudaStream_t s) {
+  if (wide == 1) {
+    a.lanes = chunks <= 4 ? 4 : chunks <= 8 ? 8 : chunks <= 16 ? 16 : 32;
+    return launch_nr<TX, TY, 1, D, false>(a, s);
   }
+  const bool sums = a.p.post != FF_NORM_NONE || a.p.normed != nullptr;
+  if (wide <= 32 && (D == Deal::kSingles || static_cast<int64_t>(a.p.rows) * wide <= 16LL * sm_count())) {
+    a.lanes = 32 * wide;
+    return launch_nr<TX, TY, 1, D, true>(a, s);
+  }
+  if (wide <= 4 && (wide == 2 || !sums)) {
+    a.lanes = 32;
+    return wide == 2 ? launch_nr<TX, TY, 2, D, false>(a, s) : launch_nr<TX, TY, 4, D, false>(a, s);
+  }
+  if (wide <= 32) {
+    a.lanes = 32 * ((wide + 1) / 2);
+    return launch_nr<TX, TY, 2, D, true>(a, s);
+  }
+  a.lanes = 32 * ((wide + 3) / 4);
+  launch_nr<TX, TY, 4, D, true>(a, s);
 }
 
 template <class TX, class TY>
-void launch_nr(NrArgs& a, cudaStream_t s) {
+void launch_nr_types(NrArgs& a, cudaStream_t s) {
   const ff_norm_residual_args& p = a.p;
-  // How far a matrix's rows start off a chunk, row 0 and from row to row.
-  bool same = true, full = p.cols % kChunk == 0;
-  int64_t base = -1, pitch = -1;
-  auto look = [&](const void* q, int64_t ld, size_t size) {
-    const int64_t b = static_cast<int64_t>(reinterpret_cast<uintptr_t>(q) / size % kChunk), l = p.rows > 1 ? (ld % kChunk + kChunk) % kChunk : 0;
-    if (base < 0) base = b, pitch = l;
-    same = same && b == base && l == pitch;
-    full = full && b == 0 && l == 0;
+  bool full = p.cols % kChunk == 0, pairs = p.cols % 2 == 0;
+  auto look = [&](const void* q, int64_t ld, int64_t size, int64_t rows) {
+    const uint64_t bits = reinterpret_cast<uintptr_t>(q) | static_cast<uint64_t>(rows > 1 ? ld * size : 0);
+    full = full && bits % 16 == 0;
+    pairs = pairs && bits % (2 * size) == 0;
   };
-  look(p.y, p.ldy, sizeof(TY));
-  look(p.x, p.ldx, sizeof(TX));
-  look(p.out, p.ldo, sizeof(TX));
-  if (p.normed != nullptr) look(p.normed, p.ldn, sizeof(TY));
-  for (const void* q : {static_cast<const void*>(p.post_w), static_cast<const void*>(p.post_b), static_cast<const void*>(p.pre_w),
-                        static_cast<const void*>(p.pre_b), static_cast<const void*>(p.scale)})
-    full = full && aligned16(q), same = same && aligned16(q);
-  if (p.gate != nullptr && p.gate_cols > 1) {
-    const bool one = p.rows <= p.gate_rows;  // a single gate row
-    if (p.gate_type == FF_F32) {
-      const bool fits = aligned16(p.gate) && (one || p.ldg % 4 == 0);
-      full = full && fits;
-      same = same && fits;
-    } else {
-      const int64_t b = static_cast<int64_t>(reinterpret_cast<uintptr_t>(p.gate) / sizeof(TY) % kChunk), l = one ? 0 : p.ldg % kChunk;
-      a.gate_chunks = full ? b == 0 && l == 0 : same && p.gate_rows == 1 && b == base && l == pitch;
-    }
-  }
-  const Deal deal = full ? Deal::kFull : same ? Deal::kShifted : Deal::kStrided;
-  if (deal == Deal::kStrided) a.gate_chunks = false;
-  // Lanes and chunks per row. Many rows: as few warps as hold the row in 4 chunks per lane. Few rows (less than 16 warps
-  // per SM even so): one chunk per lane, for the shortest way through one row.
-  const int chunks = (p.cols + (deal == Deal::kShifted ? kChunk - 1 : 0) + kChunk - 1) / kChunk;
+  look(p.y, p.ldy, sizeof(TY), p.rows);
+  look(p.x, p.ldx, sizeof(TX), p.rows);
+  look(p.out, p.ldo, sizeof(TX), p.rows);
+  look(p.normed, p.ldn, sizeof(TY), p.rows);
+  for (const float* q : {p.post_w, p.post_b, p.pre_w, p.pre_b, p.scale}) look(q, 0, 4, 1);
+  if (p.gate != nullptr && p.gate_cols > 1) look(p.gate, p.ldg, p.gate_type == FF_F32 ? 4 : 2, p.rows <= p.gate_rows ? 1 : p.rows);
+  // Lanes and chunks per row. Two chunks per lane (65600 x 1024 bf16 with two norms, gate and scale: 117 us, 146 with four,
+  // 125 with one), but one where rows are few (less than 16 warps per SM even so), for the shortest way through a row, or
+  // columns come one by one (16400 x 2731: 126 us, 151 with two), and four where no sum holds a row together (58 us, 69 with two).
+  const int chunks = (p.cols + kChunk - 1) / kChunk;
   const int wide = (chunks + 31) / 32;
-  if (wide > 1 && wide <= 32 && static_cast<int64_t>(p.rows) * wide <= 16LL * sm_count()) {
-    a.lanes = 32 * wide;
-    return launch_nr_deal<TX, TY, 1, true>(a, deal, s);
-  }
-  if (wide > 4) {
-    a.lanes = 32 * ((wide + 3) / 4);
-    return launch_nr_deal<TX, TY, 4, true>(a, deal, s);
-  }
-  a.lanes = chunks <= 4 ? 4 : chunks <= 8 ? 8 : chunks <= 16 ? 16 : 32;
-  switch (wide) {
-    case 1: return launch_nr_deal<TX, TY, 1, false>(a, deal, s);
-    case 2: return launch_nr_deal<TX, TY, 2, false>(a, deal, s);
-    case 3: return launch_nr_deal<TX, TY, 3, false>(a, deal, s);
-    default: return launch_nr_deal<TX, TY, 4, false>(a, deal, s);
-  }
+  if (full)
+    launch_nr_deal<TX, TY, Deal::kFull>(a, chunks, wide, s);
+  else if (pairs)
+    launch_nr_deal<TX, TY, Deal::kPairs>(a, chunks, wide, s);
+  else
+    launch_nr_deal<TX, TY, Deal::kSingles>(a, chunks, wide, s);
 }
 
 }  // namespace
@@ -438,15 +444,15 @@ extern "C" int ff_norm_residual(const ff_norm_residual_args* args, void* stream)
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (p.x_type == FF_F32) {
     if (p.y_type == FF_F32)
-      launch_nr<float, float>(a, s);
+      launch_nr_types<float, float>(a, s);
     else if (p.y_type == FF_F16)
-      launch_nr<float, __half>(a, s);
+      launch_nr_types<float, __half>(a, s);
     else
-      launch_nr<float, __nv_bfloat16>(a, s);
+      launch_nr_types<float, __nv_bfloat16>(a, s);
   } else if (p.x_type == FF_F16) {
-    launch_nr<__half, __half>(a, s);
+    launch_nr_types<__half, __half>(a, s);
   } else {
-    launch_nr<__nv_bfloat16, __nv_bfloat16>(a, s);
+    launch_nr_types<__nv_bfloat16, __nv_bfloat16>(a, s);
   }
   return check_launch("norm_residual_kernel");
 }

@@ -255,7 +255,7 @@ int ff_rope(const void* x, int dtype, int64_t ldx, void* out, int64_t ldo, int r
             int frequency_bytes, float scale, void* stream);
 
 /*
- * The end of a block and the norm before the next one, for rows of cols columns (at most 16376):
+ * The end of a block and the norm before the next one, for rows of cols columns (at most 16384):
  *   out    = alpha * x + scale * act(gate) * post(y)
  *   normed = pre(out), of out before it is rounded
  * post and pre: FF_NORM_NONE, FF_NORM_RMS (v / rms(v) * w + b) or FF_NORM_LAYER ((v - mean) / std * w + b), f32, weights

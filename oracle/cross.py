@@ -36,7 +36,7 @@ def norm(x, kind, w, b, eps):
 def block_end(x, y, *, alpha=1.0, post=None, post_weight=None, post_bias=None, gate=None, gate_act=None, gate_rows=1, scale=None, pre=None,
               pre_weight=None, pre_bias=None, eps=1e-6, pre_eps=None):
     """-> (out, bound of its error in f32, normed, bound of its error in f32), before the outputs' own rounding."""
-    # A sum of n <= 16376 values goes through at most 32 values per lane, 5 steps in a warp and 5 across warps: 42 roundings.
+    # A sum of n <= 16384 values goes through at most 32 values per lane, 5 steps in a warp and 5 across warps: 42 roundings.
     sums, step = 42 * 2.0**-24, 2.0**-24
     T = x.shape[0]
     v = y.double()

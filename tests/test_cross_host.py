@@ -104,7 +104,7 @@ END = dict(x=FAKE, ldx=64, y=FAKE + 4096, ldy=64, out=FAKE + 8192, ldo=64, norme
 
 
 @pytest.mark.parametrize(("change", "message"), [
-    (dict(x_type=3), "type"), (dict(x_type=0, y_type=1), "alike"), (dict(x_type=0, y_type=2), "alike"), (dict(rows=-1), "shape"), (dict(cols=16377), "shape"),
+    (dict(x_type=3), "type"), (dict(x_type=0, y_type=1), "alike"), (dict(x_type=0, y_type=2), "alike"), (dict(rows=-1), "shape"), (dict(cols=16385), "shape"),
     (dict(post=3), "norm"), (dict(pre=-1), "norm"), (dict(pre=0), "together"), (dict(normed=None), "together"), (dict(ldx=63), "strides"), (dict(ldn=1), "strides"),
     (dict(x=None), "NULL"), (dict(out=None), "NULL"), (dict(gate=FAKE, gate_cols=64, gate_rows=1, gate_type=1), "gate"),
     (dict(gate=FAKE, gate_cols=2, gate_rows=1, gate_type=2), "columns"), (dict(gate=FAKE, gate_cols=1, gate_rows=0, gate_type=2), "rows"),

@@ -162,7 +162,7 @@ TYPES = [(F16, F16), (BF16, BF16), (F32, F32), (F32, F16), (F32, BF16)]
 
 
 @pytest.mark.parametrize(("xt", "yt"), TYPES)
-@pytest.mark.parametrize(("rows", "cols"), [(1, 1), (1, 1024), (3, 7), (5, 257), (130, 768), (4, 2730), (2, 4097), (3, 8192), (2, 16376), (2500, 40), (2400, 1024),
+@pytest.mark.parametrize(("rows", "cols"), [(1, 1), (1, 1024), (3, 7), (5, 257), (130, 768), (4, 2730), (2, 4097), (3, 8192), (2, 16384), (2500, 40), (2400, 1024),
                                             (2400, 515)])
 def test_block_end(cuda_device, rows, cols, xt, yt):
     x, y, kw = _end_inputs(rows, cols, xt, yt, gate=(3, True, F32))
@@ -238,6 +238,21 @@ def test_block_end_rows_are_apart(cuda_device):
     _close(normed[keep], n, n_err, F32)
     assert normed[3].isnan().all() and not out[7].isfinite().all()
     assert torch.equal(out[11].cpu(), x[11] + kw["post_bias"])
+
+
+@pytest.mark.parametrize("act", ["sigmoid", "tanh"])
+@pytest.mark.parametrize("cols", [512, 301])
+@pytest.mark.parametrize(("xt", "yt"), [(F16, F16), (F32, F32)])
+def test_block_end_gates_of_any_size(cuda_device, act, cols, xt, yt):
+    """Gates far from zero on both sides and next to it; a NaN is one."""
+    x, y, kw = _end_inputs(40, cols, xt, yt, gate=(1, True, yt), scale=False)
+    sizes = torch.tensor([0.0, 1e-4, -3e-3, 0.1, -0.34, 0.36, 2.0, -6.0, 11.0, -20.0, 60.0, -90.0, 300.0, -2e4, math.inf, -math.inf])
+    kw["gate"] = sizes[torch.arange(40 * cols) % 16].reshape(40, cols).to(yt)
+    out, _ = _end(x, y, kw | dict(gate_act=act))
+    gate = kw["gate"].cuda()
+    gate[5, 7] = math.nan
+    ops.norm_residual(x.cuda(), y.cuda(), out, gate=gate, gate_act=act)
+    assert out[5, 7].isnan() and out.isnan().sum() == 1
 
 
 def test_block_end_large_mean(cuda_device):
