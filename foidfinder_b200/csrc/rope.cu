@@ -7,9 +7,13 @@
 // Angles: position * frequency and its part of a whole turn in 64 bits (at position 2^20 an angle in 32 bits is off by up
 // to 0.06), the sine and cosine of that part in 32 bits, the rotation in 32 bits, one rounding at the end.
 //
-// Bound by HBM: every value is read and written once. A CTA takes rows whose chunks (16 bytes of a head, or two a half
-// apart) make up to kUnits per thread; their loads are issued before the angles of these rows are worked out into shared
-// memory, once for all heads. Chunks get narrower (8, 4 bytes, single values) where a size, stride or address asks for it.
+// Measured: 65600 rows of 32 heads of 64, fp16 (537 MB): pairs 91 us, 5.9 TB/s; halves 87 us, 6.1 TB/s. 32001 rows of 8 heads of 128,
+// bf16, 64 columns turning: halves 23.4 us, 5.6 TB/s.
+//
+// Bound by HBM: every value is read and written once. A CTA takes rows whose turning units (32 bytes of a head, or twice 16 a
+// half apart) make up to kTurning per thread; their loads are issued before the angles of the rows are worked out into
+// shared memory, once for all heads, and the columns that do not turn are copied. Units get narrower, down to single
+// values, where a size, stride or address asks for it.
 #include <algorithm>
 
 #include "common.h"
@@ -20,7 +24,8 @@ namespace ff {
 namespace {
 
 constexpr int kRopeThreads = 256;
-constexpr int kRopeUnits = 4;       // per thread, whose loads are issued together
+constexpr int kTurning = 2;         // units per thread whose loads are issued together
+constexpr int kCopying = 4;         // the same of columns that are copied
 constexpr int kRopeAngles = 2048;   // per CTA, in shared memory
 
 // n / d for n < 2^31 by a multiplication: m = ceil(2^(31 + l) / d), l = ceil(log2 d), so m d - 2^(31 + l) < d <= 2^l and the
@@ -33,6 +38,7 @@ struct Divisor {
     while ((1ull << shift) < v) ++shift;
     m = ((1ull << (31 + shift)) + v - 1) / v;
   }
+  __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return static_cast<uint32_t>((n * m) >> (31 + shift)); }
   __device__ __forceinline__ void operator()(uint32_t n, uint32_t& q, uint32_t& r) const {
     q = static_cast<uint32_t>((n * m) >> (31 + shift));
     r = n - q * d;
@@ -45,8 +51,8 @@ struct RopeArgs {
   void* out;
   int64_t ldo;
   int rows, rows_per_cta, head_dim, start, rotary, axes;
-  uint32_t turn_units;  // of a head that turn; those after them copy
-  Divisor row_units, head_units;
+  Divisor turn_row, turn_head, copy_row, copy_head;  // units of a row and of a head that turn, and that are copied
+  Divisor angles, share;                            // of a row, and of an axis
   const void* positions;
   const void* frequencies;
   bool wide_positions, wide_frequencies;
@@ -63,6 +69,8 @@ template <>
 struct Word<8> { using type = uint2; };
 template <>
 struct Word<16> { using type = uint4; };
+template <>
+struct Word<32> { using type = struct { uint4 a, b; }; };
 
 // N values of T that are read and written whole, or (ALIGNED false) one by one.
 template <class T, int N, bool ALIGNED>
@@ -91,61 +99,88 @@ struct Chunk {
   }
 };
 
-__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float to_f32(float v) { return v; }
-template <class T>
-__device__ __forceinline__ T from_f32(float v) {
-  if constexpr (sizeof(T) == 4)
-    return v;
-  else if constexpr (std::is_same<T, __half>::value)
-    return __float2half_rn(v);
-  else
-    return __float2bfloat16_rn(v);
+// Values as pairs of f32, and back.
+template <class T, int N>
+__device__ __forceinline__ void widen(const T (&v)[N], float (&f)[N]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] = v[e];
+  } else if constexpr (N == 1) {
+    uint16_t h;
+    __builtin_memcpy(&h, v, 2);
+    f[0] = Pair16<T>::unpack(h).x;
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+      uint32_t w;
+      __builtin_memcpy(&w, v + e, 4);
+      const float2 p = Pair16<T>::unpack(w);
+      f[e] = p.x;
+      f[e + 1] = p.y;
+    }
+  }
+}
+template <class T, int N>
+__device__ __forceinline__ void narrow(const float (&f)[N], T (&v)[N]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = f[e];
+  } else if constexpr (N == 1) {
+    const uint32_t w = Pair16<T>::pack(f[0], 0.f);
+    __builtin_memcpy(v, &w, 2);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+      const uint32_t w = Pair16<T>::pack(f[e], f[e + 1]);
+      __builtin_memcpy(v + e, &w, 4);
+    }
+  }
+}
+// N neighbouring f32 values of shared memory that start at a multiple of N.
+template <int N>
+__device__ __forceinline__ void read(const float* p, float (&f)[N]) {
+  constexpr int W = N >= 4 ? 4 : N;
+#pragma unroll
+  for (int i = 0; i < N; i += W) __builtin_memcpy(f + i, __builtin_assume_aligned(p + i, 4 * W), 4 * W);
 }
 
-// A unit: N values that hold N / 2 neighbouring pairs, or N values and their partners a half further (HALVES). Units past
-// turn_units copy N values (one, if not ALIGNED) of the columns outside [start, start + rotary).
+// A unit: N values that hold N / 2 neighbouring pairs, or N values and their partners a half further (HALVES). Columns outside
+// [start, start + rotary) are copied N at a time (one, if not ALIGNED).
 template <class T, int N, bool HALVES, bool ALIGNED>
-__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constant__ RopeArgs a) {
-  constexpr int U = kRopeUnits, COPY = ALIGNED ? N : 1;
-  extern __shared__ float2 angle[];  // [rows of the CTA][rotary / 2] (cos, sin), times scale
+__global__ void __launch_bounds__(kRopeThreads, 4) rope_kernel(const __grid_constant__ RopeArgs a) {
+  constexpr int U = kTurning, COPY = ALIGNED ? N : 1, PAIRS = HALVES ? N : N / 2;
+  extern __shared__ __align__(16) float table[];  // [rows of the CTA][rotary / 2] cosines, then sines, both times scale
   pdl_wait();
   pdl_trigger();
   const int row0 = static_cast<int>(blockIdx.x) * a.rows_per_cta, half = a.rotary / 2;
-  const uint32_t rows = static_cast<uint32_t>(min(a.rows_per_cta, a.rows - row0)), units = rows * a.row_units.d;
+  const uint32_t rows = static_cast<uint32_t>(min(a.rows_per_cta, a.rows - row0)), units = rows * a.turn_row.d;
+  float* const sines = table + a.rows_per_cta * half;
   const T* const x = static_cast<const T*>(a.x) + row0 * a.ldx;
   T* const out = static_cast<T*>(a.out) + row0 * a.ldo;
   for (uint32_t base = 0; base < units; base += kRopeThreads * U) {
     Chunk<T, N, ALIGNED> u[U], v[HALVES ? U : 1];
-    uint32_t row[U], col[U], k[U];
+    // Row, column and number within its head of a unit (worked out twice: kept, they take the registers of a CTA per SM).
+    auto locate = [&](uint32_t at, uint32_t& row, uint32_t& col, uint32_t& k) {
+      uint32_t c, head;
+      a.turn_row(at, row, c);
+      a.turn_head(c, head, k);
+      col = head * a.head_dim + a.start + k * N;
+    };
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const uint32_t at = base + i * kRopeThreads + threadIdx.x;
       if (at >= units) break;
-      uint32_t c, head;
-      a.row_units(at, row[i], c);
-      a.head_units(c, head, k[i]);
-      const T* const p = x + row[i] * a.ldx;
-      col[i] = head * a.head_dim;
-      if (k[i] < a.turn_units) {
-        col[i] += a.start + k[i] * N;
-        u[i].load(p + col[i]);
-        if constexpr (HALVES) v[i].load(p + col[i] + half);
-      } else {
-        const uint32_t o = (k[i] - a.turn_units) * COPY;
-        col[i] += o < a.start ? o : o + a.rotary;
-        if constexpr (ALIGNED)
-          u[i].load(p + col[i]);
-        else
-          u[i].v[0] = p[col[i]];
-      }
+      uint32_t row, col, k;
+      locate(at, row, col, k);
+      const T* const p = x + row * a.ldx + col;
+      u[i].load(p);
+      if constexpr (HALVES) v[i].load(p + half);
     }
     if (base == 0) {
-      const int share = half / a.axes;
-      for (int i = threadIdx.x; i < static_cast<int>(rows) * half; i += kRopeThreads) {
-        const int r = i / half, j = i - r * half;
-        const int64_t at = static_cast<int64_t>(row0 + r) * a.axes + j / share;
+      for (uint32_t i = threadIdx.x; i < rows * half; i += kRopeThreads) {
+        uint32_t r, j;
+        a.angles(i, r, j);
+        const int64_t at = static_cast<int64_t>(row0 + r) * a.axes + (a.axes == 1 ? 0u : a.share(j));
         const double position = a.wide_positions ? static_cast<double>(static_cast<const int64_t*>(a.positions)[at])
                                                  : static_cast<double>(static_cast<const int*>(a.positions)[at]);
         const double frequency = a.wide_frequencies ? static_cast<const double*>(a.frequencies)[j]
@@ -153,40 +188,67 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constan
         const double turns = position * frequency * 0.15915494309189533577;  // 1 / (2 pi)
         float s, c;
         sincospif(2.f * static_cast<float>(turns - rint(turns)), &s, &c);
-        angle[i] = make_float2(c * a.scale, s * a.scale);
+        table[i] = c * a.scale;
+        sines[i] = s * a.scale;
+      }
+      if (a.x != a.out) {
+        const uint32_t copies = rows * a.copy_row.d;
+        for (uint32_t first = threadIdx.x; first < copies; first += kRopeThreads * kCopying) {
+          Chunk<T, COPY, ALIGNED> w[kCopying];
+          uint32_t to_row[kCopying], to[kCopying];
+#pragma unroll
+          for (int i = 0; i < kCopying; ++i) {
+            const uint32_t at = first + i * kRopeThreads;
+            if (at >= copies) break;
+            uint32_t c, head, o;
+            a.copy_row(at, to_row[i], c);
+            a.copy_head(c, head, o);
+            o *= COPY;
+            to[i] = head * a.head_dim + (o < static_cast<uint32_t>(a.start) ? o : o + a.rotary);
+            w[i].load(x + to_row[i] * a.ldx + to[i]);
+          }
+#pragma unroll
+          for (int i = 0; i < kCopying; ++i) {
+            if (first + i * kRopeThreads >= copies) break;
+            w[i].store(out + to_row[i] * a.ldo + to[i]);
+          }
+        }
       }
       __syncthreads();
     }
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      if (base + i * kRopeThreads + threadIdx.x >= units) break;
-      T* const p = out + row[i] * a.ldo + col[i];
-      if (k[i] >= a.turn_units) {
-        if constexpr (ALIGNED)
-          u[i].store(p);
-        else
-          *p = u[i].v[0];
-        continue;
-      }
-      const float2* const t = angle + row[i] * half + k[i] * (HALVES ? N : N / 2);
+      uint32_t at = base + i * kRopeThreads + threadIdx.x;
+      if (at >= units) break;
+      asm volatile("" : "+r"(at));  // not the values from above
+      uint32_t row, col, k;
+      locate(at, row, col, k);
+      T* const p = out + row * a.ldo + col;
+      float c[PAIRS], s[PAIRS], y0[N];
+      read(table + row * half + k * PAIRS, c);
+      read(sines + row * half + k * PAIRS, s);
+      widen(u[i].v, y0);
       if constexpr (HALVES) {
+        float y1[N];
+        widen(v[i].v, y1);
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-          const float2 w = t[e];
-          const float y0 = to_f32(u[i].v[e]), y1 = to_f32(v[i].v[e]);
-          u[i].v[e] = from_f32<T>(y0 * w.x - y1 * w.y);
-          v[i].v[e] = from_f32<T>(y0 * w.y + y1 * w.x);
+          const float r = y0[e] * c[e] - y1[e] * s[e];
+          y1[e] = y0[e] * s[e] + y1[e] * c[e];
+          y0[e] = r;
         }
+        narrow(y0, u[i].v);
+        narrow(y1, v[i].v);
         u[i].store(p);
         v[i].store(p + half);
       } else {
 #pragma unroll
-        for (int e = 0; e < N; e += 2) {
-          const float2 w = t[e / 2];
-          const float y0 = to_f32(u[i].v[e]), y1 = to_f32(u[i].v[e + 1]);
-          u[i].v[e] = from_f32<T>(y0 * w.x - y1 * w.y);
-          u[i].v[e + 1] = from_f32<T>(y0 * w.y + y1 * w.x);
+        for (int e = 0; e < PAIRS; ++e) {
+          const float r = y0[2 * e] * c[e] - y0[2 * e + 1] * s[e];
+          y0[2 * e + 1] = y0[2 * e] * s[e] + y0[2 * e + 1] * c[e];
+          y0[2 * e] = r;
         }
+        narrow(y0, u[i].v);
         u[i].store(p);
       }
     }
@@ -195,26 +257,34 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constan
 
 template <class T, int N, bool HALVES, bool ALIGNED>
 void launch_rope(RopeArgs& a, int heads, cudaStream_t s) {
-  const uint32_t copies = a.x == a.out ? 0 : static_cast<uint32_t>(a.head_dim - a.rotary) / (ALIGNED ? N : 1);
-  a.turn_units = static_cast<uint32_t>(a.rotary) / (HALVES ? 2 * N : N);
-  a.head_units = Divisor(a.turn_units + copies);
-  a.row_units = Divisor(static_cast<uint32_t>(heads) * a.head_units.d);
-  const int half = a.rotary / 2;
-  // Rows of a CTA: all its threads' units in one go and at most kRopeAngles angles, but fewer while SMs would have nothing
-  a.rows_per_cta = std::max(1, std::min<int>(kRopeThreads * kRopeUnits / a.row_units.d, kRopeAngles / half));
+  const int copies = (a.head_dim - a.rotary) / (ALIGNED ? N : 1), half = a.rotary / 2, turning = a.rotary / (HALVES ? 2 * N : N);
+  a.turn_head = Divisor(turning);
+  a.turn_row = Divisor(static_cast<uint32_t>(heads) * turning);
+  if (copies > 0 && a.x != a.out) {
+    a.copy_head = Divisor(copies);
+    a.copy_row = Divisor(static_cast<uint32_t>(heads) * copies);
+  } else {
+    a.copy_row.d = 0;  // nothing to copy
+  }
+  a.angles = Divisor(half);
+  a.share = Divisor(half / a.axes);
+  // Rows of a CTA: their units in one go and at most kRopeAngles angles, but fewer while SMs would have nothing
+  a.rows_per_cta = std::max(1, std::min<int>(kRopeThreads * kTurning / a.turn_row.d, kRopeAngles / half));
   a.rows_per_cta = std::max(1, std::min(a.rows_per_cta, (a.rows + sm_count() - 1) / sm_count()));
   launch(rope_kernel<T, N, HALVES, ALIGNED>, dim3((a.rows + a.rows_per_cta - 1) / a.rows_per_cta), dim3(kRopeThreads),
-         sizeof(float2) * a.rows_per_cta * half, s, a);
+         2 * sizeof(float) * a.rows_per_cta * half, s, a);
 }
 
 template <class T, bool HALVES>
 void launch_rope_width(RopeArgs& a, int heads, cudaStream_t s) {
   // The widest chunk that divides every offset: of a head, of the turning columns and their halves, of rows and addresses.
   const uint64_t bytes = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.out);
-  uint64_t all = static_cast<uint64_t>(a.head_dim) | a.start | (HALVES ? a.rotary / 2 : a.rotary) | 16 / sizeof(T);
+  uint64_t all = static_cast<uint64_t>(a.head_dim) | a.start | (HALVES ? a.rotary / 2 : a.rotary) | (HALVES ? 16 : 32) / sizeof(T);
   if (a.rows > 1) all |= static_cast<uint64_t>(a.ldx) | static_cast<uint64_t>(a.ldo);
   all |= bytes / sizeof(T);  // a multiple of sizeof(T)
   const int n = static_cast<int>(all & (~all + 1));
+  if constexpr (!HALVES)
+    if (n >= static_cast<int>(32 / sizeof(T))) return launch_rope<T, 32 / sizeof(T), HALVES, true>(a, heads, s);
   if constexpr (sizeof(T) == 2)
     if (n >= 8) return launch_rope<T, 8, HALVES, true>(a, heads, s);
   if (n >= 4) return launch_rope<T, 4, HALVES, true>(a, heads, s);
