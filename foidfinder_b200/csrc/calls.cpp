@@ -1,7 +1,7 @@
 // The short way from Python into the calls that are made once per layer, some of them for a single row: tensors are read
 // through torch's C++ interface and the kernels' library is called directly. Through ctypes and Python's tensor attributes a
 // quantisation of one row takes 6.7 us, a linear layer 12 and a head norm 8.6; this way 2.9, 6.5 to 7.1 and 2.9, of which
-// 2.3, 4.5 and 2.3 are the launches.
+// 2.3, 4.5 and 2.3 are the launches. (A rotation 8.1, a block end 11.4: 3.0 and 3.4.)
 //
 // Every function takes what its namesake in ops.py takes and returns the library's status, or None for anything that is
 // not plain (a wrong type, shape, stride or device, a subclass, no memory): the caller then goes the long way, which has
@@ -27,6 +27,10 @@ struct {
   decltype(&ff_linear_fp4_workspace_bytes) workspace;
   decltype(&ff_linear_fp4) linear;
   decltype(&ff_qk_norm_rope) qk_norm_rope;
+  decltype(&ff_rope) rope;
+  decltype(&ff_norm_residual) norm_residual;
+  decltype(&ff_cross_attention_workspace_bytes) cross_workspace;
+  decltype(&ff_cross_attention) cross_attention;
 } lib;
 
 const at::Tensor* tensor(PyObject* o) {
@@ -249,18 +253,145 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// bind(addresses of the five functions of the kernels' library, in the order of `lib`)
+// rope(x, out, positions, frequencies, heads, head_dim, start, pairing, scale)
+PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Matrix x, out;
+    int heads, dim, start, pairing;
+    float scale;
+    if (n != 9 || !matrix(a[0], &x) || !matrix(a[1], &out) || !integer(a[4], &heads) || !integer(a[5], &dim) || !integer(a[6], &start) ||
+        !integer(a[7], &pairing) || !number(a[8], &scale) || heads < 0 || heads > (1 << 16) || dim < 1 || dim > (1 << 16))
+      return nullptr;
+    const at::Tensor *p = tensor(a[2]), *f = tensor(a[3]);
+    const int64_t cols = static_cast<int64_t>(heads) * dim;
+    if (p == nullptr || f == nullptr || out.type != x.type || x.cols < cols || out.cols < cols || out.rows != x.rows || out.device != x.device) return nullptr;
+    const bool wide_p = p->scalar_type() == at::kLong, wide_f = f->scalar_type() == at::kDouble;
+    if ((!wide_p && p->scalar_type() != at::kInt) || (!wide_f && f->scalar_type() != at::kFloat) || p->dim() < 1 || p->dim() > 2 || f->dim() != 1 ||
+        p->size(0) != x.rows || !p->is_contiguous() || !f->is_contiguous() || p->get_device() != x.device || f->get_device() != x.device ||
+        f->size(0) > (1 << 16) || !current(x.device))
+      return nullptr;
+    const int64_t axes = p->dim() == 1 ? 1 : p->size(1);
+    if (axes < 1 || axes > (1 << 16)) return nullptr;
+    const void *positions = p->data_ptr(), *frequencies = f->data_ptr();
+    const int rotary = 2 * static_cast<int>(f->size(0));
+    void* const s = stream_of(x.device);
+    return status([&] {
+      return lib.rope(x.data, x.type, x.ld, out.data, out.ld, x.rows, heads, dim, start, rotary, pairing, positions, wide_p ? 8 : 4, static_cast<int>(axes),
+                      frequencies, wide_f ? 8 : 4, scale, s);
+    });
+  });
+}
+
+// norm_residual(x, y, out, normed, alpha, post, post_weight, post_bias, gate, gate_act, gate_rows, scale, pre, pre_weight, pre_bias, eps, pre_eps)
+PyObject* norm_residual(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Matrix x, y, out, normed{}, gate{};
+    ff_norm_residual_args r{};
+    int gate_rows;
+    float* p[5];
+    if (n != 17 || !matrix(a[0], &x) || !matrix(a[1], &y) || !matrix(a[2], &out) || !number(a[4], &r.alpha) || !integer(a[5], &r.post) ||
+        !integer(a[9], &r.gate_act) || !integer(a[10], &gate_rows) || !integer(a[12], &r.pre) || !number(a[15], &r.post_eps) || !number(a[16], &r.pre_eps))
+      return nullptr;
+    auto like = [&](const Matrix& m, int type) { return m.type == type && m.rows == x.rows && m.cols == x.cols && m.device == x.device; };
+    if (!like(y, y.type) || !like(out, x.type) || (x.type != y.type && x.type != FF_F32)) return nullptr;
+    if ((a[3] == Py_None) != (r.pre == FF_NORM_NONE) || (a[3] != Py_None && (!matrix(a[3], &normed) || !like(normed, y.type)))) return nullptr;
+    PyObject* const params[5] = {a[6], a[7], a[11], a[13], a[14]};
+    for (int i = 0; i < 5; ++i)
+      if (!vector(params[i], x.cols, x.device, &p[i])) return nullptr;
+    if (a[8] != Py_None) {
+      if (!matrix(a[8], &gate) || gate.device != x.device || (gate.cols != 1 && gate.cols != x.cols) || (gate.type != FF_F32 && gate.type != y.type) ||
+          gate_rows < 1 || static_cast<int64_t>(gate.rows) * gate_rows < x.rows || x.rows == 0)
+        return nullptr;
+      r.gate = gate.data;
+      r.ldg = gate.ld;
+      r.gate_type = gate.type;
+      r.gate_cols = gate.cols;
+      r.gate_rows = gate_rows;
+    }
+    if (!current(x.device)) return nullptr;
+    r.x = x.data;
+    r.ldx = x.ld;
+    r.y = y.data;
+    r.ldy = y.ld;
+    r.out = out.data;
+    r.ldo = out.ld;
+    r.normed = normed.data;
+    r.ldn = normed.ld;
+    r.x_type = x.type;
+    r.y_type = y.type;
+    r.rows = x.rows;
+    r.cols = x.cols;
+    r.post_w = p[0];
+    r.post_b = p[1];
+    r.scale = p[2];
+    r.pre_w = p[3];
+    r.pre_b = p[4];
+    void* const s = stream_of(x.device);
+    return status([&] { return lib.norm_residual(&r, s); });
+  });
+}
+
+// An optional tensor of n int32 values.
+bool starts(PyObject* o, int64_t n, int device, const int32_t** p) {
+  *p = nullptr;
+  if (o == Py_None) return true;
+  const at::Tensor* t = tensor(o);
+  if (t == nullptr || t->scalar_type() != at::kInt || t->numel() != n || !t->is_contiguous() || t->get_device() != device) return false;
+  *p = static_cast<const int32_t*>(t->data_ptr());
+  return true;
+}
+
+// cross_attention(q, k, v, out, heads, kv_heads, head_dim, sequences, q_start, k_start, k_len, mask, scale)
+PyObject* cross_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Matrix q, k, v, out;
+    int heads, kv_heads, dim, sequences;
+    float scale;
+    const int32_t *q_start, *k_start, *k_len;
+    const uint8_t* mask = nullptr;
+    if (n != 13 || !matrix(a[0], &q) || !matrix(a[1], &k) || !matrix(a[2], &v) || !matrix(a[3], &out) || !integer(a[4], &heads) || !integer(a[5], &kv_heads) ||
+        !integer(a[6], &dim) || !integer(a[7], &sequences) || !number(a[12], &scale) || heads < 1 || heads > 1024 || kv_heads < 1 || dim < 1 || dim > 128 ||
+        heads % kv_heads != 0 || sequences < 1)
+      return nullptr;
+    if (q.type == FF_F32 || k.type != q.type || v.type != q.type || out.type != q.type || q.cols != heads * dim || out.cols != q.cols || k.cols != kv_heads * dim ||
+        v.cols != k.cols || out.rows != q.rows || v.rows != k.rows || k.device != q.device || v.device != q.device || out.device != q.device || q.rows < 1)
+      return nullptr;
+    if (!starts(a[8], static_cast<int64_t>(sequences) + 1, q.device, &q_start) || !starts(a[9], static_cast<int64_t>(sequences) + 1, q.device, &k_start) ||
+        !starts(a[10], sequences, q.device, &k_len))
+      return nullptr;
+    if (a[11] != Py_None) {
+      const at::Tensor* t = tensor(a[11]);
+      if (t == nullptr || (t->scalar_type() != at::kBool && t->scalar_type() != at::kByte) || t->numel() != k.rows || !t->is_contiguous() ||
+          t->get_device() != q.device)
+        return nullptr;
+      mask = static_cast<const uint8_t*>(t->data_ptr());
+    }
+    if (!current(q.device)) return nullptr;
+    const int64_t bytes = lib.cross_workspace(q.rows, k.rows, sequences, heads, kv_heads, dim);
+    const auto s = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(q.device)).stream();
+    void* const ws = bytes > 0 ? c10::cuda::CUDACachingAllocator::raw_alloc_with_stream(static_cast<size_t>(bytes), s) : nullptr;
+    PyObject* const rc = status([&] {
+      return lib.cross_attention(q.data, q.ld, k.data, k.ld, v.data, v.ld, out.data, out.ld, q.type, q.rows, k.rows, sequences, q_start, k_start, k_len, mask, heads,
+                                 kv_heads, dim, scale, ws, bytes, s);
+    });
+    if (ws != nullptr) c10::cuda::CUDACachingAllocator::raw_delete(ws);
+    return rc;
+  });
+}
+
+// bind(addresses of the functions of the kernels' library, in the order of `lib`)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  void* f[5];
+  constexpr int kFunctions = 9;
+  void* f[kFunctions];
   static_assert(sizeof f == sizeof lib, "one address each");
-  if (n != 5) {
-    PyErr_SetString(PyExc_TypeError, "bind takes five addresses");
+  if (n != kFunctions) {
+    PyErr_SetString(PyExc_TypeError, "bind takes nine addresses");
     return nullptr;
   }
-  for (int i = 0; i < 5; ++i) {
+  for (int i = 0; i < kFunctions; ++i) {
     f[i] = PyLong_AsVoidPtr(a[i]);
     if (f[i] == nullptr) {
-      if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, "bind takes five addresses");
+      if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, "bind takes nine addresses");
       return nullptr;
     }
   }
@@ -269,7 +400,9 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 #define METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {METHOD(bind), METHOD(quantize), METHOD(dequantize), METHOD(linear), METHOD(qk_norm_rope), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {METHOD(bind),         METHOD(quantize), METHOD(dequantize),    METHOD(linear),
+                         METHOD(qk_norm_rope), METHOD(rope),     METHOD(norm_residual), METHOD(cross_attention),
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -25,7 +25,6 @@ namespace {
 
 constexpr int kRopeThreads = 256;
 constexpr int kTurning = 2;         // units per thread whose loads are issued together
-constexpr int kCopying = 4;         // the same of columns that are copied
 constexpr int kRopeAngles = 2048;   // per CTA, in shared memory
 
 // n / d for n < 2^31 by a multiplication: m = ceil(2^(31 + l) / d), l = ceil(log2 d), so m d - 2^(31 + l) < d <= 2^l and the
@@ -148,7 +147,7 @@ __device__ __forceinline__ void read(const float* p, float (&f)[N]) {
 // [start, start + rotary) are copied N at a time (one, if not ALIGNED).
 template <class T, int N, bool HALVES, bool ALIGNED>
 __global__ void __launch_bounds__(kRopeThreads, 4) rope_kernel(const __grid_constant__ RopeArgs a) {
-  constexpr int U = kTurning, COPY = ALIGNED ? N : 1, PAIRS = HALVES ? N : N / 2;
+  constexpr int U = kTurning, COPY = ALIGNED ? N : 1, COPIES = N * sizeof(T) > 16 ? 2 : 4, PAIRS = HALVES ? N : N / 2;
   extern __shared__ __align__(16) float table[];  // [rows of the CTA][rotary / 2] cosines, then sines, both times scale
   pdl_wait();
   pdl_trigger();
@@ -193,11 +192,11 @@ __global__ void __launch_bounds__(kRopeThreads, 4) rope_kernel(const __grid_cons
       }
       if (a.x != a.out) {
         const uint32_t copies = rows * a.copy_row.d;
-        for (uint32_t first = threadIdx.x; first < copies; first += kRopeThreads * kCopying) {
-          Chunk<T, COPY, ALIGNED> w[kCopying];
-          uint32_t to_row[kCopying], to[kCopying];
+        for (uint32_t first = threadIdx.x; first < copies; first += kRopeThreads * COPIES) {
+          Chunk<T, COPY, ALIGNED> w[COPIES];
+          uint32_t to_row[COPIES], to[COPIES];
 #pragma unroll
-          for (int i = 0; i < kCopying; ++i) {
+          for (int i = 0; i < COPIES; ++i) {
             const uint32_t at = first + i * kRopeThreads;
             if (at >= copies) break;
             uint32_t c, head, o;
@@ -208,7 +207,7 @@ __global__ void __launch_bounds__(kRopeThreads, 4) rope_kernel(const __grid_cons
             w[i].load(x + to_row[i] * a.ldx + to[i]);
           }
 #pragma unroll
-          for (int i = 0; i < kCopying; ++i) {
+          for (int i = 0; i < COPIES; ++i) {
             if (first + i * kRopeThreads >= copies) break;
             w[i].store(out + to_row[i] * a.ldo + to[i]);
           }

@@ -327,7 +327,7 @@ _free = getattr(torch._C, "_cuda_cudaCachingAllocator_raw_delete", None) or torc
 class _NoCalls:
     """In the place of the extension module where it has not been built: every call goes the long way."""
 
-    quantize = dequantize = linear = qk_norm_rope = staticmethod(lambda *args: None)
+    quantize = dequantize = linear = qk_norm_rope = rope = norm_residual = cross_attention = staticmethod(lambda *args: None)
 
 
 @cache
@@ -342,7 +342,8 @@ def _calls():
         warnings.warn(f"foidfinder_b200._calls was built for torch {built_for}, not {torch.__version__}; build it with `python -m foidfinder_b200.build`")
         return _NoCalls
     h = lib()
-    names = ("ff_quantize_fp4", "ff_dequantize_fp4", "ff_linear_fp4_workspace_bytes", "ff_linear_fp4", "ff_qk_norm_rope")
+    names = ("ff_quantize_fp4", "ff_dequantize_fp4", "ff_linear_fp4_workspace_bytes", "ff_linear_fp4", "ff_qk_norm_rope", "ff_rope",
+             "ff_norm_residual", "ff_cross_attention_workspace_bytes", "ff_cross_attention")
     module.bind(*(C.cast(getattr(h, name), C.c_void_p).value for name in names))
     return module
 
@@ -641,6 +642,7 @@ def qk_norm_rope(
 
 
 # ---------------------------------------------------------------- tokens that read an image's
+_KINDS = {None: _lib.NORM_NONE, **_NORMS}
 _GATES = {None: _lib.GATE_PLAIN, "sigmoid": _lib.GATE_SIGMOID, "tanh": _lib.GATE_TANH}
 
 
@@ -695,6 +697,9 @@ def rope(
     first columns of out (x itself: in place). `positions` [T] or [T, axes] int32 or int64 (axes take equal shares of the
     pairs, in order), `frequencies` f64 or f32 (`rope_frequencies`); `pairing` "pairs" rotates (2i, 2i + 1) of them, "halves" (i, i + r / 2)."""
     what = "rope"
+    rc = _calls().rope(x, out, positions, frequencies, heads, head_dim, start, _PAIRINGS.get(pairing), scale)
+    if rc is not None:
+        return check(rc, what) if rc else None
     rows, xcols, ldx, device = _matrix(x, what)
     orows, ocols, ldo, odevice = _matrix(out, what)
     dtype = _DTYPES.get(x.dtype)
@@ -739,6 +744,10 @@ def norm_residual(
     f32 or y's type, after `gate_act` None, "sigmoid" or "tanh"; row t reads gate row t // gate_rows. `scale` [C] f32. Types: fp16,
     bf16 or f32 alike, or x and out in f32 with a 16-bit y. Rows that start 16 bytes apart are the fastest."""
     what = "norm_residual"
+    rc = _calls().norm_residual(x, y, out, normed, alpha, _KINDS.get(post), post_weight, post_bias, gate, _GATES.get(gate_act), gate_rows, scale, _KINDS.get(pre),
+                                pre_weight, pre_bias, eps, eps if pre_eps is None else pre_eps)
+    if rc is not None:
+        return check(rc, what) if rc else None
     rows, cols, ldx, device = _matrix(x, what)
     n = _lib.NormResidualArgs(rows=rows, cols=cols, alpha=alpha, ldx=ldx, x=x.data_ptr(), post_eps=eps, pre_eps=eps if pre_eps is None else pre_eps)
     for name, ld, t, like in (("y", "ldy", y, y), ("out", "ldo", out, x), ("normed", "ldn", normed, y)):
@@ -796,6 +805,14 @@ def cross_attention(
     it holds. A query without keys gives zeros; rows of out outside the sequences stay as they were. `scale` is head_dim**-0.5 unless given."""
     what = "cross_attention"
     kv_heads = heads if kv_heads is None else kv_heads
+    for t, more in ((q_start, 1), (k_start, 1), (k_len, 0)):
+        if sequences is None and t is not None:
+            sequences = t.numel() - more
+    sequences = 1 if sequences is None else sequences
+    scale = head_dim**-0.5 if scale is None and head_dim > 0 else scale
+    rc = _calls().cross_attention(q, k, v, out, heads, kv_heads, head_dim, sequences, q_start, k_start, k_len, mask, scale)
+    if rc is not None:
+        return check(rc, what) if rc else None
     tq, qcols, ldq, device = _matrix(q, what)
     tk, kcols, ldk, kdevice = _matrix(k, what)
     shape_v, shape_o = _matrix(v, what), _matrix(out, what)
@@ -806,10 +823,6 @@ def cross_attention(
         raise RuntimeError(f"cross_attention: q {list(q.shape)}, k {list(k.shape)}, v {list(v.shape)}, out {list(out.shape)} for {heads} and {kv_heads} heads of {head_dim}")
     if kdevice != device or shape_v[3] != device or shape_o[3] != device:
         raise RuntimeError("cross_attention: q, k, v and out must be on one device")
-    for t, more in ((q_start, 1), (k_start, 1), (k_len, 0)):
-        if t is not None and sequences is None:
-            sequences = t.numel() - more
-    sequences = 1 if sequences is None else sequences
     for name, t, n in (("q_start", q_start, sequences + 1), ("k_start", k_start, sequences + 1), ("k_len", k_len, sequences)):
         if t is not None and (t.get_device() != device or t.dtype is not torch.int32 or t.numel() != n or not t.is_contiguous()):
             raise RuntimeError(f"cross_attention: {name} must be {n} contiguous int32 values on cuda:{device}, got {t.dtype} {list(t.shape)} on {t.device}")
@@ -827,7 +840,7 @@ def cross_attention(
     try:
         rc = lib().ff_cross_attention(q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), shape_v[2], out.data_ptr(), shape_o[2], _DTYPES[dtype],
                                       tq, tk, sequences, _ptr(q_start), _ptr(k_start), _ptr(k_len), _ptr(mask), heads, kv_heads, head_dim,
-                                      head_dim**-0.5 if scale is None else scale, ws, nbytes, stream)
+                                      scale, ws, nbytes, stream)
     finally:
         if ws is not None:
             _free(ws)

@@ -514,3 +514,78 @@ def test_tokens_read_an_image(cuda_device, no_device_error, nq):
     torch.cuda.synchronize()
     check(1, out, work)
     check(2, other, other_work)
+
+
+# ---------------------------------------------------------------- refusals and ways into the calls
+def _every_call():
+    """The three calls on one set of tensors, as functions of what to replace."""
+    d = "cuda"
+    x = torch.zeros(4, 128, dtype=F16, device=d)
+    pos, f, w = torch.zeros(4, dtype=torch.int32, device=d), torch.zeros(32, dtype=torch.float64, device=d), torch.ones(128, device=d)
+    k = torch.zeros(6, 128, dtype=F16, device=d)
+    rope = dict(x=x, out=torch.zeros_like(x), positions=pos, frequencies=f, heads=2, head_dim=64)
+    end = dict(x=x, y=torch.zeros_like(x), out=torch.zeros_like(x), post="rms", post_weight=w, normed=torch.zeros_like(x), pre="layer", pre_weight=w, pre_bias=w,
+               gate=torch.zeros(4, 1, device=d), gate_act="tanh")
+    cross = dict(q=x, k=k, v=k, out=torch.zeros_like(x), heads=2, head_dim=64, q_start=torch.tensor([0, 1, 4]).int().cuda(), k_start=torch.tensor([0, 3, 6]).int().cuda(),
+                 k_len=torch.tensor([3, 3]).int().cuda(), mask=torch.ones(6, dtype=torch.bool, device=d))
+    return (ops.rope, rope), (ops.norm_residual, end), (ops.cross_attention, cross)
+
+
+@pytest.mark.parametrize("short", [True, False])
+def test_refusals(cuda_device, monkeypatch, short):
+    """What a call does not take raises before any launch, through the extension module and without it."""
+    if not short:
+        monkeypatch.setattr(ops, "_calls", lambda: ops._NoCalls)
+    (rope, r), (end, e), (cross, c) = _every_call()
+    x, d = r["x"], "cuda"
+    for fn, kw in ((rope, r), (end, e), (cross, c)):
+        fn(**kw)
+    strided = torch.zeros(4, 256, dtype=F16, device=d)[:, ::2]
+    for change in (dict(x=x.cpu()), dict(out=x.bfloat16()), dict(out=x[:3]), dict(x=x[:, :100]), dict(x=strided), dict(positions=r["positions"][:3]),
+                   dict(positions=r["positions"].float()), dict(positions=r["positions"].cpu()), dict(frequencies=r["frequencies"].half()), dict(frequencies=r["frequencies"][None]),
+                   dict(frequencies=r["frequencies"].repeat(2)), dict(frequencies=r["frequencies"][:0]), dict(pairing="both"), dict(start=1), dict(start=-2), dict(head_dim=0),
+                   dict(heads=-1), dict(heads=3), dict(positions=torch.zeros(4, 3, dtype=torch.int32, device=d)), dict(positions=torch.zeros(4, 0, dtype=torch.int32, device=d)),
+                   dict(x=x.int(), out=x.int())):
+        with pytest.raises(RuntimeError):
+            rope(**(r | change))
+    for change in (dict(x=x.cpu()), dict(y=x.bfloat16()), dict(y=x.float()), dict(out=x.float()), dict(out=x[:3]), dict(normed=None), dict(pre=None), dict(post="other"), dict(pre="other"),
+                   dict(post_weight=e["post_weight"][:5]), dict(pre_bias=e["pre_bias"].half()), dict(gate=torch.zeros(3, 1, device=d)), dict(gate=torch.zeros(4, 2, device=d)),
+                   dict(gate=x.bfloat16()), dict(gate_act="relu"), dict(gate_rows=0), dict(scale=e["post_weight"].cpu()), dict(y=strided), dict(normed=e["out"]), dict(out=e["y"])):
+        with pytest.raises(RuntimeError):
+            end(**(e | change))
+    for change in (dict(q=x.cpu()), dict(q=x.float()), dict(k=c["k"].bfloat16()), dict(v=c["v"][:5]), dict(out=x[:3]), dict(heads=3), dict(kv_heads=1), dict(heads=0), dict(head_dim=32),
+                   dict(head_dim=24, heads=2), dict(q_start=c["q_start"].long()), dict(q_start=c["q_start"].cpu()), dict(k_start=c["k_start"][:2]), dict(k_len=c["q_start"]),
+                   dict(mask=c["mask"][:5]), dict(mask=c["mask"].float()), dict(sequences=3), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan),
+                   dict(sequences=4, q_start=None, k_start=None, k_len=None), dict(q=torch.zeros(4, 132, dtype=F16, device=d)[:, :128]), dict(v=strided[:4].repeat(2, 1)[:6, :64])):
+        with pytest.raises(RuntimeError):
+            cross(**(c | change))
+
+
+def test_the_short_and_the_long_way_into_these_calls_agree(cuda_device, no_device_error, monkeypatch):
+    x, y, kw = _end_inputs(67, 256, F16, F16, gate=(67, False, F32))
+    kw = {k: v.cuda() if torch.is_tensor(v) else v for k, v in kw.items()} | dict(post="rms", pre="layer", gate_act="tanh")
+    q, k, v = (t.cuda() for t in _qkv(40, 3000, 4, 2, 64, F16))
+    f, pos = ops.rope_frequencies(32)[0].cuda(), torch.arange(67, device="cuda")
+
+    def everything():
+        o = [torch.full_like(t, 3.0) for t in (x.cuda(), x.cuda(), x.cuda(), q)]
+        ops.rope(x.cuda(), o[0], pos, f, heads=4, head_dim=64, start=32, pairing="halves", scale=1.25)
+        ops.norm_residual(x.cuda(), y.cuda(), o[1], normed=o[2], **kw)
+        ops.cross_attention(q, k, v, o[3], heads=4, kv_heads=2, head_dim=64, sequences=10)
+        return o
+
+    def taken(real):
+        def call(*args):
+            r = real(*args)
+            assert r == 0
+            return r
+        return call
+
+    short = ops._calls()
+    with monkeypatch.context() as m:
+        for name in ("rope", "norm_residual", "cross_attention"):
+            m.setattr(short, name, taken(getattr(short, name)))
+        a = everything()
+    monkeypatch.setattr(ops, "_calls", lambda: ops._NoCalls)
+    for u, w in zip(a, everything()):
+        assert torch.equal(u, w)
