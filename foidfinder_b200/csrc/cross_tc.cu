@@ -170,6 +170,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int dim = p.dim, group = p.heads / p.kv_heads;
   int* const err = a.err;
+  if (a.items == gridDim.x) {  // one item per CTA, perhaps none
+    pdl_wait();
+    if (item_at(a, blockIdx.x).nq == 0) return;
+  }
   if (threadIdx.x == 0) {
     for (int i = 0; i < QB; ++i) {
       mbar_init(&q_full[i], 1);
@@ -578,7 +582,9 @@ int launch_tc(const TcArgs& a, cudaStream_t s) {
                                         2, cols, rows, 2 * (rows > 1 ? static_cast<uint64_t>(ld[i]) : cols), 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc != FF_OK) return rc;
   }
-  const int grid = static_cast<int>(std::min<int64_t>(a.items, sm_count()));
+  // Sequences of different lengths: a CTA per item, so that whoever is done takes the next.
+  const bool even = p.q_start == nullptr && p.k_start == nullptr && p.k_len == nullptr;
+  const int grid = static_cast<int>(std::min<int64_t>(a.items, even ? sm_count() : 0x7fffffff));
   launch(cross_tc_kernel<T, ATOMS>, dim3(grid), dim3(kTcThreads), tc_smem(ATOMS), s, maps[0], maps[1], maps[2], a);
   return check_launch("cross_tc_kernel");
 }
