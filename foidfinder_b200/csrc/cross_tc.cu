@@ -1,4 +1,5 @@
-// Attention of many queries per sequence to its keys and values on the 5th-generation tensor cores (tcgen05).
+// Attention of many queries per sequence to its keys and values on the 5th-generation tensor cores (tcgen05), heads of 65 to
+// 128 columns (cross_tc64.cu has the narrower ones).
 //   out = softmax(scale q k^T) v, head by head, keys that do not take part left out
 //
 // Bound by the exponentials (one per query, key and head) and the hand-overs between tensor core and softmax. Persistent
@@ -6,10 +7,10 @@
 // and head, against that sequence's keys in tiles of 128; consecutive items overlap in the pipeline.
 //   warp 0     loads, by TMA: an item's queries, and key and value tiles in turn through one ring. A tile's rows are rows of
 //              the whole matrix, whatever sequence they belong to.
-//   warp 1     MMAs, by one elected thread: S_i = Q_i K^T and O_i += P_i V, P_i read from TMEM. Heads of up to 64 columns have
-//              room for S, P and O of both tiles beside one another: S_i(j + 1) is issued when the softmax has read S_i(j),
-//              while it still works on P_i(j). Wider heads have P over S: PV_i(j), then S_i(j + 1) (MMAs of one thread
-//              execute in order).
+//   warp 1     MMAs, by one elected thread: S_i = Q_i K^T to TMEM columns [128 i, +128), and O_i += P_i V, P_i read from where
+//              S_i was, to columns [256 + 128 i, +dim). Order per key tile j: PV_0(j), S_0(j + 1), PV_1(j), S_1(j + 1); MMAs of
+//              one thread execute in order, so S_i(j + 1) finds P_i(j) consumed. (A thread for each tile let both tiles
+//              fall in step and then wait together: 619 us where this takes 469.)
 //   warps 2-5  softmax of query tile 0, warps 6-9 of tile 1, a query per thread: 32 scores at a time, the next 32 on their
 //              way meanwhile, P = 2^(s - m + 7) in 16 bits, the sum of P in f32 before that rounding. m is the
 //              maximum at some earlier time: the exponentials start at once, and the new maximum is found beside them.
@@ -21,114 +22,27 @@
 #include <algorithm>
 
 #include "common.h"
-#include "cross.h"
-#include "fp4.cuh"
+#include "cross_tc.cuh"
 
 namespace ff {
 
 namespace {
 
-constexpr int kBQ = 128, kBK = 128;
-constexpr int kAtom = 128 * 128;  // bytes: 128 rows of 64 columns, 128-byte swizzle
+constexpr int kBK = 128;
 constexpr int kTcThreads = 320;
-constexpr int kTable = 64;  // items of a CTA that are looked up ahead, all at once
-__host__ __device__ constexpr int q_buffers(int atoms) { return atoms == 1 ? 2 : 1; }
-__host__ __device__ constexpr int ring_slots(int atoms) { return atoms == 1 ? 8 : 5; }
-__host__ __device__ constexpr int off_ring(int atoms) { return q_buffers(atoms) * 2 * atoms * kAtom; }
-__host__ __device__ constexpr int off_table(int atoms) { return off_ring(atoms) + ring_slots(atoms) * atoms * kAtom; }
-__host__ __device__ constexpr int off_bars(int atoms) { return off_table(atoms) + kTable * 16; }
-__host__ __device__ constexpr int tc_smem(int atoms) { return 1024 + off_bars(atoms) + 384; }
-static_assert(tc_smem(1) <= 232448 && tc_smem(2) <= 232448, "shared memory of a CTA");
+constexpr int kSlots = 5;          // of the ring
+constexpr int kTile = 2 * kAtom;   // 128 rows of 128 columns
+constexpr int kOffRing = 2 * kTile;
+constexpr int kOffTable = kOffRing + kSlots * kTile;
+constexpr int kOffBars = kOffTable + kTable * static_cast<int>(sizeof(Item));
+constexpr int kTcSmem = 1024 + kOffBars + 256;
+static_assert(kTcSmem <= 232448, "shared memory of a CTA");
 
 // TMEM columns of query tile i.
 __host__ __device__ constexpr uint32_t t_s(int i) { return 128u * i; }
-template <int ATOMS>
-__host__ __device__ constexpr uint32_t t_p(int i) {
-  return ATOMS == 1 ? 256u + 64u * i : t_s(i);
-}
-template <int ATOMS>
-__host__ __device__ constexpr uint32_t t_o(int i) {
-  return ATOMS == 1 ? 384u + 64u * i : 256u + 128u * i;
-}
-constexpr float kGrowth = 8.f;  // powers of two by which the maximum may grow before O is rescaled
-constexpr float kUp = 7.f;      // P = 2^(x + 7): at most 2^15, in fp16's range
+__host__ __device__ constexpr uint32_t t_o(int i) { return 256u + 128u * i; }
 
-struct TcArgs {
-  CrossArgs p;
-  int tiles_per_seq;  // equal pieces: items of 256 queries per sequence and head; 0: by q_start
-  int64_t items;
-  int* err;
-};
-
-// Up to 256 queries [q, q + nq) of a head against the keys [k, k + nk).
-struct Item {
-  int q, nq, k, nk;
-};
-
-// Value tile as MN-major operand: key rows of 128 bytes (64 columns), 8-row groups 1024 bytes apart, the next 64 columns an atom
-// further.
-__device__ __forceinline__ uint64_t sdesc_v(uint32_t saddr) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
-  d |= static_cast<uint64_t>(kAtom >> 4) << 16;
-  d |= static_cast<uint64_t>(1024u >> 4) << 32;
-  d |= static_cast<uint64_t>(1u) << 46;
-  d |= static_cast<uint64_t>(2u) << 61;
-  return d;
-}
-__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
-// Item `n` of this CTA (nq == 0: none). Head fastest, then the 256-query tiles of a sequence. By q_start, tile t of
-// sequence b is slot q_start[b] / 256 + b + t: slots of sequences do not overlap, and the one that holds a slot is found by halving.
-__device__ Item item_at(const TcArgs& a, int64_t it) {
-  const CrossArgs& p = a.p;
-  const int slot = static_cast<int>(it / p.heads);
-  int b, tile;
-  if (a.tiles_per_seq > 0) {
-    b = slot / a.tiles_per_seq;
-    tile = slot - b * a.tiles_per_seq;
-  } else {
-    auto first = [&](int i) { return min(max(__ldg(p.q_start + i), 0), p.q_rows) / 256 + i; };
-    int lo = 0, hi = p.sequences - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (first(mid) <= slot) lo = mid;
-      else hi = mid - 1;
-    }
-    b = lo;
-    tile = slot - first(b);
-  }
-  const Piece q = query_piece(p, b);
-  Item r{0, 0, 0, 0};
-  if (tile < 0 || static_cast<int64_t>(tile) * 256 >= q.n) return r;
-  r.q = q.at + tile * 256;
-  r.nq = min(256, q.n - tile * 256);
-  const Piece k = key_piece(p, b);
-  r.k = k.at;
-  r.nk = k.n;
-  return r;
-}
-
-// O (dim TMEM columns from `to`) scaled by corr; out of line, it is rare.
-__device__ __noinline__ void rescale(uint32_t to, int dim, float corr) {
-  for (int c = 0; c < dim; c += 16) {
-    uint32_t o[16];
-    tmem_ld16(to + c, o);
-    tmem_ld_wait();
-#pragma unroll
-    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-    tmem_st16(to + c, o);
-  }
-}
-
-// The same for the first `chunks` times 32 weights of P.
+// The first `chunks` times 32 weights of P scaled by corr.
 template <class T>
 __device__ __noinline__ void rescale_p(uint32_t ts, int chunks, float corr) {
   for (int c = 0; c < chunks; ++c) {
@@ -144,24 +58,21 @@ __device__ __noinline__ void rescale_p(uint32_t ts, int chunks, float corr) {
   }
 }
 
-template <class T, int ATOMS>
+template <class T>
 __global__ void __launch_bounds__(kTcThreads, 1)
     cross_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                     const __grid_constant__ TcArgs a) {
-  constexpr bool APART = ATOMS == 1;  // P beside S
-  constexpr int QB = q_buffers(ATOMS), SLOTS = ring_slots(ATOMS), TILE = ATOMS * kAtom;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  Item* const table = reinterpret_cast<Item*>(smem + off_table(ATOMS));
-  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + off_bars(ATOMS));
-  uint64_t* q_full = bar;             // [QB]
-  uint64_t* q_empty = q_full + QB;    // [QB]
-  uint64_t* full = q_empty + QB;      // [SLOTS]
-  uint64_t* empty = full + SLOTS;     // [SLOTS]
-  uint64_t* s_full = empty + SLOTS;   // [2], per query tile
+  Item* const table = reinterpret_cast<Item*>(smem + kOffTable);
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + kOffBars);
+  uint64_t* q_full = bar;
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* full = q_empty + 1;       // [kSlots]
+  uint64_t* empty = full + kSlots;    // [kSlots]
+  uint64_t* s_full = empty + kSlots;  // [2], per query tile
   uint64_t* p_full = s_full + 2;      // [2]
-  uint64_t* s_read = p_full + 2;      // [2]
-  uint64_t* pv_done = s_read + 2;     // [2]
+  uint64_t* pv_done = p_full + 2;     // [2]
   uint64_t* drain = pv_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -175,18 +86,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (item_at(a, blockIdx.x).nq == 0) return;
   }
   if (threadIdx.x == 0) {
-    for (int i = 0; i < QB; ++i) {
-      mbar_init(&q_full[i], 1);
-      mbar_init(&q_empty[i], 1);
-    }
-    for (int i = 0; i < SLOTS; ++i) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int i = 0; i < kSlots; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
-      mbar_init(&s_read[i], 4);
       mbar_init(&pv_done[i], 1);
     }
     mbar_init(drain, 1);
@@ -213,59 +121,41 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  // The next item with queries (after the n-th), and its head.
-  auto advance = [&](int& n, Item& item, int& head) -> bool {
-    for (++n;; ++n) {
-      const int64_t it = blockIdx.x + static_cast<int64_t>(n) * gridDim.x;
-      if (it >= a.items) return false;
-      item = n < kTable ? table[n] : item_at(a, it);
-      head = static_cast<int>(it % p.heads);
-      if (item.nq > 0) return true;
-    }
-  };
-  // The same, with keys as well.
-  auto advance_work = [&](int& n, Item& item, int& head) -> bool {
-    while (advance(n, item, head))
-      if (item.nk > 0) return true;
-    return false;
-  };
+  Items items{a, table};
 
   if (warp == 0) {
     // ------------------------------------------------------------ loads
     if (elect_one()) {
-      int q_phase[QB], phase[SLOTS];
+      int q_phase = -1, phase[kSlots];
 #pragma unroll
-      for (int i = 0; i < QB; ++i) q_phase[i] = -1;
-#pragma unroll
-      for (int i = 0; i < SLOTS; ++i) phase[i] = -1;
+      for (int i = 0; i < kSlots; ++i) phase[i] = -1;
       bool ok = true;
-      int slot = 0, n = -1, head = 0;
+      int slot = 0;
       uint32_t round = 0;  // of the ring
       Item item;
-      for (int m = 0; ok && advance_work(n, item, head); ++m) {
-        const int qb = m % QB, tiles = item.nq > kBQ ? 2 : 1;
-        if (m >= QB && !mbar_wait<true>(&q_empty[qb], static_cast<uint32_t>(m / QB - 1) & 1u, abort_flag, err, kDevTimeoutAttn)) {
+      for (int m = 0; ok && items.next<true>(item); ++m) {
+        const int tiles = item.nq > kBQ ? 2 : 1;
+        if (m > 0 && !mbar_wait<true>(q_empty, static_cast<uint32_t>(m - 1) & 1u, abort_flag, err, kDevTimeoutAttn)) {
           ok = false;
           break;
         }
-        mbar_arrive_expect_tx(&q_full[qb], tiles * TILE);
+        mbar_arrive_expect_tx(q_full, tiles * kTile);
         for (int i = 0; i < tiles; ++i)
 #pragma unroll
-          for (int c = 0; c < ATOMS; ++c)
-            tma_load_2d(smem + (2 * qb + i) * TILE + c * kAtom, &tm_q, &q_full[qb], head * dim + 64 * c, item.q + i * kBQ);
-        q_phase[qb] = (m / QB) & 1;
-        const int x = head / group * dim, nkv = (item.nk + kBK - 1) / kBK;
+          for (int c = 0; c < 2; ++c) tma_load_2d(smem + i * kTile + c * kAtom, &tm_q, q_full, items.head * dim + 64 * c, item.q + i * kBQ);
+        q_phase = m & 1;
+        const int x = items.head / group * dim, nkv = (item.nk + kBK - 1) / kBK;
         for (int j = 0; j < 2 * nkv; ++j) {  // K_0, V_0, K_1, V_1, ..
           if (!mbar_wait<true>(&empty[slot], (round & 1u) ^ 1u, abort_flag, err, kDevTimeoutAttn)) {
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(&full[slot], TILE);
+          mbar_arrive_expect_tx(&full[slot], kTile);
 #pragma unroll
-          for (int c = 0; c < ATOMS; ++c)
-            tma_load_2d(smem + off_ring(ATOMS) + slot * TILE + c * kAtom, j & 1 ? &tm_v : &tm_k, &full[slot], x + 64 * c, item.k + (j >> 1) * kBK);
+          for (int c = 0; c < 2; ++c)
+            tma_load_2d(smem + kOffRing + slot * kTile + c * kAtom, j & 1 ? &tm_v : &tm_k, &full[slot], x + 64 * c, item.k + (j >> 1) * kBK);
           phase[slot] = static_cast<int>(round & 1u);
-          if (++slot == SLOTS) {
+          if (++slot == kSlots) {
             slot = 0;
             ++round;
           }
@@ -274,11 +164,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       // Normally everything has been consumed. After an abort, let issued copies land (bounded) before the CTA can exit.
       if (!ok) {
         const unsigned long long t0 = globaltimer();
-        for (int i = 0; i < QB; ++i)
-          if (q_phase[i] >= 0)
-            while (!mbar_try_wait(smem_u32(&q_full[i]), static_cast<uint32_t>(q_phase[i])) && globaltimer() - t0 < kWaitLimitNs) {
-            }
-        for (int i = 0; i < SLOTS; ++i)
+        if (q_phase >= 0)
+          while (!mbar_try_wait(smem_u32(q_full), static_cast<uint32_t>(q_phase)) && globaltimer() - t0 < kWaitLimitNs) {
+          }
+        for (int i = 0; i < kSlots; ++i)
           if (phase[i] >= 0)
             while (!mbar_try_wait(smem_u32(&full[i]), static_cast<uint32_t>(phase[i])) && globaltimer() - t0 < kWaitLimitNs) {
             }
@@ -290,15 +179,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       constexpr uint32_t fmt = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);  // both operands fp16 or bf16
       const uint32_t id_o = idesc_f16(128, dim) | fmt | (1u << 16);  // B = V is MN-major
       const int steps = dim / 16;
-      const uint32_t ring = smem_u32(smem) + off_ring(ATOMS);
+      const uint32_t ring = smem_u32(smem) + kOffRing;
       // Keys of a tile that its products cover: all, or the sequence's last ones rounded up to 16.
       auto width = [](int nk, int j) { return min(kBK, (nk - j * kBK + 15) & ~15); };
-      auto issue_s = [&](int i, int qb, int slot, int keys) {
+      auto issue_s = [&](int i, int slot, int keys) {
         const uint32_t id = idesc_f16(128, keys) | fmt;
-        const uint64_t qd = sdesc_k_sw128(smem_u32(smem) + (2 * qb + i) * TILE);
-        const uint64_t kd = sdesc_k_sw128(ring + slot * TILE);
+        const uint64_t qd = sdesc_k_sw128(smem_u32(smem) + i * kTile);
+        const uint64_t kd = sdesc_k_sw128(ring + slot * kTile);
 #pragma unroll
-        for (int k = 0; k < 4 * ATOMS; ++k)
+        for (int k = 0; k < 8; ++k)
           if (k < steps) {
             const uint64_t o = (k >> 2) * (kAtom >> 4) + (k & 3) * 2;
             mma_f16(tmem + t_s(i), qd + o, kd + o, id, k > 0);
@@ -306,59 +195,51 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tc_commit(&s_full[i]);
       };
       auto issue_pv = [&](int i, int slot, int keys, bool first) {
-        const uint64_t vd = sdesc_v(ring + slot * TILE);
+        const uint64_t vd = sdesc_v(ring + slot * kTile);
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          if (16 * k < keys) mma_ts(tmem + t_o<ATOMS>(i), tmem + t_p<ATOMS>(i) + 8 * k, vd + static_cast<uint64_t>(k * 128), id_o, (first && k == 0) ? 0u : 1u);
+          if (16 * k < keys) mma_ts(tmem + t_o(i), tmem + t_s(i) + 8 * k, vd + static_cast<uint64_t>(k * 128), id_o, (first && k == 0) ? 0u : 1u);
       };
       bool ok = true;
       auto wait = [&](uint64_t* b, uint32_t parity) {
         if (ok) ok = mbar_wait<true>(b, parity, abort_flag, err, kDevTimeoutAttn);
         return ok;
       };
-      int n = -1, head, m = 0, slot = 0;  // slot, round: of the current key tile's K
+      int m = 0, slot = 0;  // slot, round: of the current key tile's K
       uint32_t round = 0, count[2] = {0, 0};
       Item cur{}, nxt{};
-      bool have = advance_work(n, cur, head);
-      if (have && wait(&q_full[0], 0) && wait(&full[0], 0)) {
+      bool have = items.next<true>(cur);
+      if (have && wait(q_full, 0) && wait(&full[0], 0)) {
         tc_fence_after();
-        issue_s(0, 0, 0, width(cur.nk, 0));
-        if (cur.nq > kBQ) issue_s(1, 0, 0, width(cur.nk, 0));
+        issue_s(0, 0, width(cur.nk, 0));
+        if (cur.nq > kBQ) issue_s(1, 0, width(cur.nk, 0));
         tc_commit(&empty[0]);
-        if (cur.nk <= kBK) tc_commit(&q_empty[0]);
+        if (cur.nk <= kBK) tc_commit(q_empty);
       }
       while (have && ok) {
-        const bool more = advance_work(n, nxt, head), two = cur.nq > kBQ;
+        const bool more = items.next<true>(nxt), two = cur.nq > kBQ;
         const int nkv = (cur.nk + kBK - 1) / kBK;
         for (int j = 0; j < nkv && ok; ++j) {
           const bool last = j == nkv - 1, next = !last || more;
           int v_slot = slot + 1, k_slot = slot + 2;
           uint32_t v_round = round, k_round = round;
-          if (v_slot >= SLOTS) v_slot -= SLOTS, ++v_round;
-          if (k_slot >= SLOTS) k_slot -= SLOTS, ++k_round;
+          if (v_slot >= kSlots) v_slot -= kSlots, ++v_round;
+          if (k_slot >= kSlots) k_slot -= kSlots, ++k_round;
           const int keys = width(cur.nk, j);
           const int next_keys = last ? width(nxt.nk, 0) : width(cur.nk, j + 1);  // unused without a next tile
-          const int next_m = last ? m + 1 : m;
-          const int qb = next_m % QB;
-          auto pv = [&](int i) {
-            if (!wait(&p_full[i], count[i] & 1u)) return;
-            tc_fence_after();
-            issue_pv(i, v_slot, keys, j == 0);
-            tc_commit(&pv_done[i]);
-            ++count[i];
-          };
-          // One query tile: P V of this key tile, S of the next one, in the order that TMEM allows.
+          // One query tile: P V of this key tile, then S of the next one.
           auto turn = [&](int i, bool here, bool there) {
-            if (APART && here && !wait(&s_read[i], count[i] & 1u)) return;
-            if (APART && there) {
+            if (here) {
+              if (!wait(&p_full[i], count[i] & 1u)) return;
               tc_fence_after();
-              issue_s(i, qb, k_slot, next_keys);
+              issue_pv(i, v_slot, keys, j == 0);
+              tc_commit(&pv_done[i]);
+              ++count[i];
             }
-            if (here) pv(i);
-            if (!APART && there && ok) issue_s(i, qb, k_slot, next_keys);
+            if (there) issue_s(i, k_slot, next_keys);
           };
           if (!wait(&full[v_slot], v_round & 1u) || (next && !wait(&full[k_slot], k_round & 1u)) ||
-              (next && last && !wait(&q_full[qb], static_cast<uint32_t>(next_m / QB) & 1u)))
+              (next && last && !wait(q_full, static_cast<uint32_t>(m + 1) & 1u)))
             break;
           tc_fence_after();
           turn(0, true, next);
@@ -367,7 +248,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           tc_commit(&empty[v_slot]);
           if (next) {
             tc_commit(&empty[k_slot]);
-            if (last ? nxt.nk <= kBK : j + 1 == nkv - 1) tc_commit(&q_empty[qb]);  // the last use of these queries
+            if (last ? nxt.nk <= kBK : j + 1 == nkv - 1) tc_commit(q_empty);  // the last use of these queries
           }
           slot = k_slot;
           round = k_round;
@@ -389,17 +270,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // ------------------------------------------------------------ softmax and results
     const int g = (warp - 2) >> 2, quarter = warp & 3;
     const uint32_t ts = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + t_s(g);
-    const uint32_t tp = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + t_p<ATOMS>(g);
-    const uint32_t to = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + t_o<ATOMS>(g);
+    const uint32_t to = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + t_o(g);
     const int first_row = g * kBQ + quarter * 32;  // of this warp, in the item
     bool ok = true;
-    int n = -1, head, v_slot = 1;
+    int v_slot = 1;
     uint32_t v_round = 0, tiles = 0;
     Item item;
-    while (ok && advance(n, item, head)) {
+    while (ok && items.next<false>(item)) {
       const int64_t row = item.q + first_row + lane;
       const bool store = first_row + lane < item.nq, active = first_row < item.nq;
-      T* const out = static_cast<T*>(p.out) + row * p.ldo + static_cast<int64_t>(head) * dim;
+      T* const out = static_cast<T*>(p.out) + row * p.ldo + static_cast<int64_t>(items.head) * dim;
       if (item.nk == 0) {
         if (store)
           for (int c = 0; c < dim; c += 8) *reinterpret_cast<uint4*>(out + c) = make_uint4(0, 0, 0, 0);
@@ -408,8 +288,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int nkv = (item.nk + kBK - 1) / kBK;
       if (g * kBQ >= item.nq) {  // this group has no queries here; the ring goes on
         const uint32_t at = static_cast<uint32_t>(v_slot) + 2u * nkv;
-        v_round += at / SLOTS;
-        v_slot = static_cast<int>(at % SLOTS);
+        v_round += at / kSlots;
+        v_slot = static_cast<int>(at % kSlots);
         continue;
       }
       const uint8_t* const mask = p.mask != nullptr ? p.mask + item.k : nullptr;
@@ -453,8 +333,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           const uint32_t mine = quarter == 0 ? bits[0] : quarter == 1 ? bits[1] : quarter == 2 ? bits[2] : bits[3];
           if (!(mine >> lane & 1u)) {
 #pragma unroll
-            for (int c = 0; c < ATOMS; ++c) {
-              uint4* const v = reinterpret_cast<uint4*>(smem + off_ring(ATOMS) + v_slot * TILE + c * kAtom + (quarter * 32 + lane) * 128);
+            for (int c = 0; c < 2; ++c) {
+              uint4* const v = reinterpret_cast<uint4*>(smem + kOffRing + v_slot * kTile + c * kAtom + (quarter * 32 + lane) * 128);
 #pragma unroll
               for (int i = 0; i < 8; ++i) v[i] = make_uint4(0, 0, 0, 0);
             }
@@ -462,7 +342,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           fence_async_smem();
         }
         v_slot += 2;
-        if (v_slot >= SLOTS) v_slot -= SLOTS, ++v_round;
+        if (v_slot >= kSlots) v_slot -= kSlots, ++v_round;
         if (active) {
           const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
           uint32_t s[2][32];
@@ -495,10 +375,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               return fmaxf(mx[0], mx[1]);
             };
             const float mx = exponentials();
-            if (c == 0 && tiles > 0) {  // before P and O are touched: the last product has read and written them
-              ok = mbar_wait(&pv_done[g], (tiles - 1) & 1u, abort_flag, err, kDevTimeoutAttn);
-              tc_fence_after();
-            }
             const bool grown = mx > kUp + kGrowth || (!set && mx > -INFINITY);
             if (__any_sync(0xffffffffu, grown)) {
               if (c < 3) tmem_ld_wait();  // nothing on its way into registers across the calls
@@ -510,22 +386,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 set = true;
               }
               if (j > 0) rescale(to, dim, corr);
-              if (c > 0) rescale_p<T>(tp, c, corr);
+              if (c > 0) rescale_p<T>(ts, c, corr);
               sum.x *= corr;
               sum.y *= corr;
               exponentials();
             }
             sum = add2(sum, part);
-            tmem_st16(tp + 16 * c, pk);
+            tmem_st16(ts + 16 * c, pk);
             if (c < 3) tmem_ld_wait();
-            if (APART && c == 2) {  // all of S is in registers
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&s_read[g]);
-            }
           }
-        } else if (APART && lane == 0) {
-          mbar_arrive(&s_read[g]);
         }
         __syncwarp();
         tmem_st_wait();
@@ -562,34 +431,36 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (warp == 1) tmem_dealloc(tmem, 512);
 }
 
-template <class T, int ATOMS>
-int launch_tc(const TcArgs& a, cudaStream_t s) {
+template <class T>
+int launch_tc(const TcArgs& a, int grid, cudaStream_t s) {
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !configured[dev]) {
-    if (cudaFuncSetAttribute(cross_tc_kernel<T, ATOMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, tc_smem(ATOMS)) != cudaSuccess)
+    if (cudaFuncSetAttribute(cross_tc_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcSmem) != cudaSuccess)
       return check_launch("cross_tc: cudaFuncSetAttribute");
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  const CrossArgs& p = a.p;
   CUtensorMap maps[3];
-  const void* base[3] = {p.q, p.k, p.v};
-  const int64_t ld[3] = {p.ldq, p.ldk, p.ldv};
-  for (int i = 0; i < 3; ++i) {
-    const uint64_t cols = static_cast<uint64_t>(i == 0 ? p.heads : p.kv_heads) * p.dim, rows = i == 0 ? p.q_rows : p.k_rows;
-    const int rc = make_tmap_2d_pitched(&maps[i], base[i], std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-                                        2, cols, rows, 2 * (rows > 1 ? static_cast<uint64_t>(ld[i]) : cols), 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (rc != FF_OK) return rc;
-  }
-  // Sequences of different lengths: a CTA per item, so that whoever is done takes the next.
-  const bool even = p.q_start == nullptr && p.k_start == nullptr && p.k_len == nullptr;
-  const int grid = static_cast<int>(std::min<int64_t>(a.items, even ? sm_count() : 0x7fffffff));
-  launch(cross_tc_kernel<T, ATOMS>, dim3(grid), dim3(kTcThreads), tc_smem(ATOMS), s, maps[0], maps[1], maps[2], a);
+  const int rc = cross_maps(a.p, std::is_same<T, __nv_bfloat16>::value, kBK, maps);
+  if (rc != FF_OK) return rc;
+  launch(cross_tc_kernel<T>, dim3(grid), dim3(kTcThreads), kTcSmem, s, maps[0], maps[1], maps[2], a);
   return check_launch("cross_tc_kernel");
 }
 
 }  // namespace
+
+int cross_maps(const CrossArgs& p, bool bf16, int key_rows, CUtensorMap (&maps)[3]) {
+  const void* base[3] = {p.q, p.k, p.v};
+  const int64_t ld[3] = {p.ldq, p.ldk, p.ldv};
+  for (int i = 0; i < 3; ++i) {
+    const uint64_t cols = static_cast<uint64_t>(i == 0 ? p.heads : p.kv_heads) * p.dim, rows = i == 0 ? p.q_rows : p.k_rows;
+    const int rc = make_tmap_2d_pitched(&maps[i], base[i], bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, cols, rows,
+                                        2 * (rows > 1 ? static_cast<uint64_t>(ld[i]) : cols), 64, i == 0 ? kBQ : key_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc != FF_OK) return rc;
+  }
+  return FF_OK;
+}
 
 int cross_tc(const CrossArgs& p, bool bf16, cudaStream_t s) {
   TcArgs a{};
@@ -600,8 +471,11 @@ int cross_tc(const CrossArgs& p, bool bf16, cudaStream_t s) {
   a.items = slots * p.heads;
   a.err = device_error_word();
   FF_REQUIRE(a.err != nullptr, "ff_cross_attention: no device error word");
-  if (p.dim <= 64) return bf16 ? launch_tc<__nv_bfloat16, 1>(a, s) : launch_tc<__half, 1>(a, s);
-  return bf16 ? launch_tc<__nv_bfloat16, 2>(a, s) : launch_tc<__half, 2>(a, s);
+  // Sequences of different lengths: a CTA per item, so that whoever is done takes the next.
+  const bool even = p.q_start == nullptr && p.k_start == nullptr && p.k_len == nullptr;
+  const int grid = static_cast<int>(std::min<int64_t>(a.items, even ? sm_count() : 0x7fffffff));
+  if (p.dim <= 64) return cross_tc64(a, bf16, grid, s);
+  return bf16 ? launch_tc<__nv_bfloat16>(a, grid, s) : launch_tc<__half>(a, grid, s);
 }
 
 }  // namespace ff

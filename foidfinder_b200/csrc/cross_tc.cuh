@@ -1,0 +1,111 @@
+// What the two tensor-core kernels of cross attention share (cross_tc.cu: heads of more than 64 columns; cross_tc64.cu: up to 64).
+#pragma once
+#include "common.h"
+#include "cross.h"
+#include "fp4.cuh"
+
+namespace ff {
+
+constexpr int kBQ = 128;          // queries of a tile
+constexpr int kAtom = 128 * 128;  // bytes: 128 rows of 64 columns, 128-byte swizzle
+constexpr int kTable = 64;        // items of a CTA that are looked up ahead, all at once
+constexpr float kGrowth = 8.f;    // powers of two by which the maximum may grow before O is rescaled
+constexpr float kUp = 7.f;        // P = 2^(x + 7): at most 2^15, in fp16's range
+
+struct TcArgs {
+  CrossArgs p;
+  int tiles_per_seq;  // equal pieces: items of 256 queries per sequence and head; 0: by q_start
+  int64_t items;
+  int* err;
+};
+
+// Up to 256 queries [q, q + nq) of a head against the keys [k, k + nk).
+struct Item {
+  int q, nq, k, nk;
+};
+
+// Tensor maps of q, k and v: boxes of 64 columns and 128 queries or key_rows keys.
+int cross_maps(const CrossArgs& p, bool bf16, int key_rows, CUtensorMap (&maps)[3]);
+int cross_tc64(const TcArgs& a, bool bf16, int grid, cudaStream_t s);
+
+// Value tile as MN-major operand: key rows of 128 bytes (64 columns), 8-row groups 1024 bytes apart, the next 64 columns an atom
+// further.
+__device__ __forceinline__ uint64_t sdesc_v(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(kAtom >> 4) << 16;
+  d |= static_cast<uint64_t>(1024u >> 4) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(2u) << 61;
+  return d;
+}
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Item `n` of this CTA (nq == 0: none). Head fastest, then the 256-query tiles of a sequence. By q_start, tile t of
+// sequence b is slot q_start[b] / 256 + b + t: slots of sequences do not overlap, and the one that holds a slot is found by halving.
+static __device__ Item item_at(const TcArgs& a, int64_t it) {
+  const CrossArgs& p = a.p;
+  const int slot = static_cast<int>(it / p.heads);
+  int b, tile;
+  if (a.tiles_per_seq > 0) {
+    b = slot / a.tiles_per_seq;
+    tile = slot - b * a.tiles_per_seq;
+  } else {
+    auto first = [&](int i) { return min(max(__ldg(p.q_start + i), 0), p.q_rows) / 256 + i; };
+    int lo = 0, hi = p.sequences - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (first(mid) <= slot) lo = mid;
+      else hi = mid - 1;
+    }
+    b = lo;
+    tile = slot - first(b);
+  }
+  const Piece q = query_piece(p, b);
+  Item r{0, 0, 0, 0};
+  if (tile < 0 || static_cast<int64_t>(tile) * 256 >= q.n) return r;
+  r.q = q.at + tile * 256;
+  r.nq = min(256, q.n - tile * 256);
+  const Piece k = key_piece(p, b);
+  r.k = k.at;
+  r.nk = k.n;
+  return r;
+}
+
+// O (dim TMEM columns from `to`) scaled by corr; out of line, it is rare.
+static __device__ __noinline__ void rescale(uint32_t to, int dim, float corr) {
+  for (int c = 0; c < dim; c += 16) {
+    uint32_t o[16];
+    tmem_ld16(to + c, o);
+    tmem_ld_wait();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+    tmem_st16(to + c, o);
+  }
+}
+
+// Walks the items of a CTA. next(): the next one with queries (and, WORK, with keys).
+struct Items {
+  const TcArgs& a;
+  const Item* table;
+  int n = -1, head = 0;
+  template <bool WORK>
+  __device__ __forceinline__ bool next(Item& item) {
+    for (++n;; ++n) {
+      const int64_t it = blockIdx.x + static_cast<int64_t>(n) * gridDim.x;
+      if (it >= a.items) return false;
+      item = n < kTable ? table[n] : item_at(a, it);
+      head = static_cast<int>(it % a.p.heads);
+      if (item.nq > 0 && (!WORK || item.nk > 0)) return true;
+    }
+  }
+};
+
+}  // namespace ff
