@@ -46,9 +46,10 @@ __device__ __forceinline__ Piece key_piece(const CrossArgs& a, int b) {
 #endif
 
 // Few queries per sequence. splits: parts of every sequence's keys that CTAs of their own work on (their results are
-// joined by a second kernel through the workspace).
+// joined within a cluster, or by a second kernel through the workspace).
 struct CrossFewPlan {
   bool few;  // whether this kernel takes the call
+  bool cluster;  // the splits of a sequence are a cluster
   int row_tiles, passes, splits;
   int64_t workspace;
 };

@@ -7,7 +7,9 @@
 // key that does not take part with zeros instead of reading it (so that whatever it holds, its value counts 0 * 0). RG
 // warps divide the rows, 4 / RG warps the keys of a tile; each keeps a running maximum, sum and output of its keys in
 // registers (mma.sync: the products are far from what bounds this kernel, and 16 rows are what there is). The warps' parts
-// are joined through shared memory in a fixed order, and the parts of CTAs by a second kernel through the workspace.
+// are joined through shared memory in a fixed order. Up to 8 parts of a sequence are a cluster of CTAs, which read one
+// another's shared memory (no second launch: one token over 1025 keys 9.6 -> 7.4 us, over 4096 keys no gain); more of them go through the workspace
+// and a second kernel.
 //
 // P is rounded to 16 bits for its product with V, as 2^(x - max + 14) in fp16, where it would else lose bits below 2^-14;
 // sums are taken before that rounding, in f32.
@@ -23,7 +25,10 @@ namespace {
 
 constexpr int kKeys = 64;        // of a tile
 constexpr int kFewThreads = 128;
-__host__ __device__ constexpr int few_stages(int atoms) { return atoms == 1 ? 4 : 3; }
+constexpr int kCluster = 8;      // CTAs of a cluster, at most
+constexpr int kClusterTiles = 40;  // of a sequence, beyond which a second launch costs less than having 8 parts only
+__host__ __device__ constexpr int few_stages(int atoms) { return atoms == 1 ? 3 : 2; }
+__host__ __device__ constexpr int few_ctas(int atoms) { return atoms == 1 ? 4 : 3; }  // per SM
 __host__ __device__ constexpr int few_tile(int atoms) { return atoms * kKeys * 128; }  // bytes of a K or V tile
 __host__ __device__ constexpr int few_smem(int atoms) { return few_stages(atoms) * 2 * few_tile(atoms); }
 
@@ -67,21 +72,36 @@ __device__ __forceinline__ uint32_t tile_byte(int row, int c) {
   return static_cast<uint32_t>((c >> 3) * (kKeys * 128) + row * 128 + (((c ^ row) & 7) << 4));
 }
 
+__device__ __forceinline__ float4 read_cluster(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 read_cluster2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+// Weight of a part whose maximum is m beside the largest one, top. (Both -inf: nothing but NaN can be there.)
+__device__ __forceinline__ float part_weight(float m, float top) { return m == -INFINITY && top == -INFINITY ? 1.f : ex2_approx(m - top); }
+
 struct FewArgs {
   CrossArgs p;
   int passes, splits;
+  bool cluster;    // the splits of a sequence are a cluster
   float* part_o;   // [splits][q_rows * heads][dim]
   float2* part_ml;  // [splits][q_rows * heads]: maximum (in powers of two) and sum
 };
 
 template <class T, int ATOMS, int RG>
-__global__ void __launch_bounds__(kFewThreads) cross_few_kernel(const __grid_constant__ FewArgs a) {
+__global__ void __launch_bounds__(kFewThreads, few_ctas(ATOMS)) cross_few_kernel(const __grid_constant__ FewArgs a) {
   constexpr int STAGES = few_stages(ATOMS), TILE = few_tile(ATOMS), KG = 4 / RG, KW = kKeys / KG;
   constexpr int ROWS = 16 * RG, STEPS = ATOMS * 4;
   constexpr float kShift = std::is_same<T, __half>::value ? 14.f : 0.f;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ uint64_t taken[STAGES];  // bits: keys of a tile that take part
   __shared__ float part_m[KG][ROWS], part_l[KG][ROWS];
+  __shared__ __align__(8) float2 joined[ROWS];
   const CrossArgs& p = a.p;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, rg = warp % RG, kg = warp / RG;
   const int group = p.heads / p.kv_heads, dim = p.dim, chunks = dim / 8;
@@ -103,30 +123,39 @@ __global__ void __launch_bounds__(kFewThreads) cross_few_kernel(const __grid_con
   const int keys = max(0, min(tiles * kKeys, ks.n - first * kKeys));
   const uint32_t base = smem_u32(smem);
 
-  // The keys of tile i that take part; every warp works it out.
-  auto bits_of = [&](int i) -> uint64_t {
-    const int left = keys - i * kKeys;
-    if (left <= 0) return 0;
-    if (mask == nullptr) return left >= kKeys ? ~0ull : (1ull << left) - 1;
-    const bool lo = lane < left && mask[i * kKeys + lane] != 0, hi = 32 + lane < left && mask[i * kKeys + 32 + lane] != 0;
-    const uint64_t l = __ballot_sync(0xffffffffu, lo), h = __ballot_sync(0xffffffffu, hi);
+  // Mask bytes of tile i's keys lane and lane + 32 (1 without a mask), 0 past the end.
+  uint32_t ahead[2];
+  auto fetch = [&](int i) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int key = i * kKeys + 32 * c + lane;
+      ahead[c] = key < keys ? (mask != nullptr ? __ldg(mask + key) : 1u) : 0u;
+    }
+  };
+  auto ahead_bits = [&]() -> uint64_t {  // the keys that take part
+    const uint64_t l = __ballot_sync(0xffffffffu, ahead[0] != 0), h = __ballot_sync(0xffffffffu, ahead[1] != 0);
     return l | h << 32;
   };
+  // This thread copies chunk t % 8 (of an atom) of the rows t / 8 + 16 n, whose swizzle is the same.
+  const int64_t k16 = 16 * p.ldk, v16 = 16 * p.ldv;
+  const T* const k_own = kp + (t >> 3) * p.ldk + (t & 7) * 8;
+  const T* const v_own = vp + (t >> 3) * p.ldv + (t & 7) * 8;
+  const uint32_t own = tile_byte(t >> 3, t & 7);
   auto load = [&](int i, uint64_t bits) {
     const int st = i % STAGES;
     if (t == 0) taken[st] = bits;
-    const uint32_t kd = base + st * 2 * TILE, vd = kd + TILE;
+    const uint32_t d = base + st * 2 * TILE + own;
+    const T* ks = k_own + 4 * i * k16;
+    const T* vs = v_own + 4 * i * v16;
+    const uint32_t rows = static_cast<uint32_t>((bits >> (t >> 3) & 1) | (bits >> (16 + (t >> 3)) & 1) << 1 | (bits >> (32 + (t >> 3)) & 1) << 2 | (bits >> (48 + (t >> 3)) & 1) << 3);
 #pragma unroll
-    for (int n = 0; n < ATOMS * 4; ++n) {  // 64 rows x 8 chunks of an atom by 128 threads: 4 steps
-      const int c = (n >> 2) * 8 + (t & 7), row = (n & 3) * 16 + (t >> 3);
-      if (c < chunks) {
-        const bool take = bits >> row & 1;
-        const int64_t r = take ? i * kKeys + row : 0;  // a key left out is not read
-        const uint32_t d = tile_byte(row, c);
-        copy16(kd + d, kp + r * p.ldk + c * 8, take);
-        copy16(vd + d, vp + r * p.ldv + c * 8, take);
-      }
-    }
+    for (int n = 0; n < 4; ++n, ks += k16, vs += v16)
+#pragma unroll
+      for (int c = 0; c < ATOMS; ++c)
+        if (c * 8 + (t & 7) < chunks) {  // a key left out is not read
+          copy16(d + c * (kKeys * 128) + n * 2048, ks + c * 64, rows >> n & 1);
+          copy16(d + TILE + c * (kKeys * 128) + n * 2048, vs + c * 64, rows >> n & 1);
+        }
   };
 
   for (int pass = pass0; pass * ROWS < total_rows; pass += a.passes) {
@@ -148,19 +177,21 @@ __global__ void __launch_bounds__(kFewThreads) cross_few_kernel(const __grid_con
     for (int n = 0; n < 2 * STEPS; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+    fetch(0);
 #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i) {
-      const uint64_t bits = bits_of(i);
+      const uint64_t bits = ahead_bits();
+      fetch(i + 1);
       if (i < tiles) load(i, bits);
       copies_commit();
     }
-    uint64_t ahead = bits_of(STAGES - 1);
     for (int i = 0; i < tiles; ++i) {
       copies_wait<STAGES - 2>();
       __syncthreads();  // tile i has landed for all, and all are done with tile i - 1, whose place is next
-      if (i + STAGES - 1 < tiles) load(i + STAGES - 1, ahead);
+      const uint64_t next = ahead_bits();
+      if (i + STAGES - 1 < tiles) load(i + STAGES - 1, next);
       copies_commit();
-      ahead = bits_of(i + STAGES);
+      fetch(i + STAGES);
       const uint32_t kt = base + (i % STAGES) * 2 * TILE, vt = kt + TILE;
       const uint64_t bits = taken[i % STAGES] >> (kg * KW);  // of this warp's keys
       float s[KW / 8][4];
@@ -267,7 +298,7 @@ __global__ void __launch_bounds__(kFewThreads) cross_few_kernel(const __grid_con
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int g = 0; g < KG; ++g) {
-        const float w = part_m[g][r] == -INFINITY && top == -INFINITY ? 1.f : ex2_approx(part_m[g][r] - top);
+        const float w = part_weight(part_m[g][r], top);
         const float4 v = *reinterpret_cast<const float4*>(parts + (g * ROWS + r) * dim + c);
         sum = fmaf(part_l[g][r], w, sum);
         acc.x = fmaf(v.x, w, acc.x);
@@ -281,26 +312,68 @@ __global__ void __launch_bounds__(kFewThreads) cross_few_kernel(const __grid_con
         const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no key: zeros
         *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + q_row * p.ldo + static_cast<int64_t>(head) * dim + c) =
             make_uint2(Pair16<T>::pack(acc.x * inv, acc.y * inv), Pair16<T>::pack(acc.z * inv, acc.w * inv));
+      } else if (a.cluster) {
+        *reinterpret_cast<float4*>(parts + r * dim + c) = acc;  // in the place of the first group's, which no one else reads
+        if (c == 0) joined[r] = make_float2(top, sum);
       } else {
         const int64_t at_row = (static_cast<int64_t>(split) * p.q_rows + q_row) * p.heads + head;
         *reinterpret_cast<float4*>(a.part_o + at_row * dim + c) = acc;
         if (c == 0) a.part_ml[at_row] = make_float2(top, sum);
       }
     }
-    __syncthreads();  // before the next pass fills the ring
+    if (a.cluster) {
+      __syncwarp();
+      cluster_sync();  // every CTA's part of these rows is there
+      const int rows = min(ROWS, total_rows - pass * ROWS);
+      for (int i = split * kFewThreads + t; i < rows * quads; i += a.splits * kFewThreads) {
+        const int r = i / quads, c = (i - r * quads) * 4, row = pass * ROWS + r;
+        float2 ml[kCluster];
+        float4 v[kCluster];
+#pragma unroll
+        for (int g = 0; g < kCluster; ++g) {
+          ml[g] = make_float2(-INFINITY, 0.f);
+          v[g] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (g < a.splits) {
+            ml[g] = read_cluster2(mapa_shared(smem_u32(&joined[r]), g));
+            v[g] = read_cluster(mapa_shared(smem_u32(parts + r * dim + c), g));
+          }
+        }
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int g = 0; g < kCluster; ++g) top = fmaxf(top, ml[g].x);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int g = 0; g < kCluster; ++g) {
+          const float w = part_weight(ml[g].x, top);
+          sum = fmaf(ml[g].y, w, sum);
+          acc.x = fmaf(v[g].x, w, acc.x);
+          acc.y = fmaf(v[g].y, w, acc.y);
+          acc.z = fmaf(v[g].z, w, acc.z);
+          acc.w = fmaf(v[g].w, w, acc.w);
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + static_cast<int64_t>(qs.at + row / group) * p.ldo + static_cast<int64_t>(kvh * group + row % group) * dim + c) =
+            make_uint2(Pair16<T>::pack(acc.x * inv, acc.y * inv), Pair16<T>::pack(acc.z * inv, acc.w * inv));
+      }
+      __syncwarp();
+      cluster_sync();  // and has been read
+    } else {
+      __syncthreads();  // before the next pass fills the ring
+    }
   }
 }
 
-// out = the splits' parts, joined in order: a warp per query row and head.
+// out = the splits' parts, joined in order: a CTA per query row and head, a warp for every kJoinWarps-th part.
+constexpr int kJoinWarps = 8;
 template <class T>
-__global__ void __launch_bounds__(256) cross_join_kernel(const __grid_constant__ FewArgs a) {
+__global__ void __launch_bounds__(32 * kJoinWarps) cross_join_kernel(const __grid_constant__ FewArgs a) {
+  __shared__ float sums[kJoinWarps];
+  __shared__ float4 accs[kJoinWarps][32];
   const CrossArgs& p = a.p;
-  const int lane = threadIdx.x & 31;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t at = blockIdx.x, rows = static_cast<int64_t>(p.q_rows) * p.heads;
   pdl_wait();
   pdl_trigger();
-  const int64_t rows = static_cast<int64_t>(p.q_rows) * p.heads;
-  if (at >= rows) return;
   const int q_row = static_cast<int>(at / p.heads), head = static_cast<int>(at % p.heads);
   if (p.q_start != nullptr && (q_row < __ldg(p.q_start) || q_row >= __ldg(p.q_start + p.sequences))) return;  // of no sequence
   float top = -INFINITY;
@@ -310,9 +383,9 @@ __global__ void __launch_bounds__(256) cross_join_kernel(const __grid_constant__
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   const int c = lane * 4;
 #pragma unroll 4
-  for (int i = 0; i < a.splits; ++i) {
+  for (int i = warp; i < a.splits; i += kJoinWarps) {
     const float2 ml = a.part_ml[i * rows + at];
-    const float w = ml.x == -INFINITY && top == -INFINITY ? 1.f : ex2_approx(ml.x - top);
+    const float w = part_weight(ml.x, top);
     sum = fmaf(ml.y, w, sum);
     if (c < p.dim) {
       const float4 v = *reinterpret_cast<const float4*>(a.part_o + (i * rows + at) * p.dim + c);
@@ -322,7 +395,18 @@ __global__ void __launch_bounds__(256) cross_join_kernel(const __grid_constant__
       acc.w = fmaf(v.w, w, acc.w);
     }
   }
-  if (c >= p.dim) return;
+  accs[warp][lane] = acc;
+  if (lane == 0) sums[warp] = sum;
+  __syncthreads();
+  if (warp != 0 || c >= p.dim) return;
+  for (int g = 1; g < kJoinWarps; ++g) {
+    const float4 v = accs[g][lane];
+    sum += sums[g];
+    acc.x += v.x;
+    acc.y += v.y;
+    acc.z += v.z;
+    acc.w += v.w;
+  }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + q_row * p.ldo + static_cast<int64_t>(head) * p.dim + c) =
       make_uint2(Pair16<T>::pack(acc.x * inv, acc.y * inv), Pair16<T>::pack(acc.z * inv, acc.w * inv));
@@ -340,12 +424,29 @@ int launch_few(const FewArgs& a, cudaStream_t s) {
   }
   const int64_t grid = static_cast<int64_t>(a.splits) * a.passes * a.p.kv_heads * a.p.sequences;
   FF_REQUIRE(grid <= 0x7fffffff, "ff_cross_attention: %lld parts", static_cast<long long>(grid));
+  if (a.cluster) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(grid));
+    cfg.blockDim = dim3(kFewThreads);
+    cfg.dynamicSmemBytes = few_smem(ATOMS);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(a.splits);
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    cudaLaunchKernelEx(&cfg, cross_few_kernel<T, ATOMS, RG>, a);
+    return check_launch("cross_few_kernel");
+  }
   launch(cross_few_kernel<T, ATOMS, RG>, dim3(static_cast<unsigned>(grid)), dim3(kFewThreads), few_smem(ATOMS), s, a);
   if (a.splits > 1) {
     const int rc = check_launch("cross_few_kernel");
     if (rc != FF_OK) return rc;
     const int64_t rows = static_cast<int64_t>(a.p.q_rows) * a.p.heads;
-    launch(cross_join_kernel<T>, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0, s, a);
+    launch(cross_join_kernel<T>, dim3(static_cast<unsigned>(rows)), dim3(32 * kJoinWarps), 0, s, a);
   }
   return check_launch("cross_few_kernel");
 }
@@ -371,9 +472,15 @@ CrossFewPlan cross_few_plan(int q_rows, int k_rows, int sequences, int heads, in
   plan.passes = static_cast<int>(std::max<int64_t>(1, (rows + 16 * plan.row_tiles - 1) / (16 * plan.row_tiles)));
   const int64_t ctas = static_cast<int64_t>(sequences) * kv_heads * plan.passes;
   const int64_t tiles = ((static_cast<int64_t>(k_rows) + sequences - 1) / sequences + kKeys - 1) / kKeys;
-  // As many parts as fill the GPU's places for CTAs (three per SM, two with the larger tiles), of two tiles at least
-  const int64_t places = static_cast<int64_t>(sm_count()) * (dim <= 64 ? 3 : 2);
+  // As many parts as fill the GPU's places for CTAs, of two tiles at least
+  const int64_t places = static_cast<int64_t>(sm_count()) * few_ctas(dim <= 64 ? 1 : 2);
   plan.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({places / ctas, (tiles + 1) / 2, 1024})));
+  // Few enough parts, or a sequence short enough that 8 of them are read as fast as the second launch is made: a cluster.
+  if (plan.splits > 1 && (plan.splits <= kCluster || (ctas * kCluster >= sm_count() / 2 && tiles <= kClusterTiles))) {
+    plan.cluster = true;
+    plan.splits = std::min(plan.splits, kCluster);
+    return plan;
+  }
   if (plan.splits > 1) plan.workspace = static_cast<int64_t>(plan.splits) * q_rows * heads * (dim + 2) * 4;
   return plan;
 }
@@ -383,6 +490,7 @@ int cross_few(const CrossArgs& p, bool bf16, const CrossFewPlan& plan, void* wor
   a.p = p;
   a.passes = plan.passes;
   a.splits = plan.splits;
+  a.cluster = plan.cluster;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + static_cast<int64_t>(plan.splits) * p.q_rows * p.heads * p.dim);
   return bf16 ? launch_few_type<__nv_bfloat16>(a, plan.row_tiles, s) : launch_few_type<__half>(a, plan.row_tiles, s);

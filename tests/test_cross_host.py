@@ -146,9 +146,9 @@ def test_cross_attention_nothing_to_do():
 
 def test_cross_attention_workspace():
     lib = _lib.lib()
-    need = lib.ff_cross_attention_workspace_bytes(1, 4096, 1, 16, 16, 64)
+    need = lib.ff_cross_attention_workspace_bytes(1, 1 << 16, 1, 16, 16, 64)
     assert need > 0 and need % 8 == 0
-    one = CROSS | dict(q_rows=1, k_rows=4096, sequences=1, heads=16, kv_heads=16, ldk=1024, ldv=1024)
+    one = CROSS | dict(q_rows=1, k_rows=1 << 16, sequences=1, heads=16, kv_heads=16, ldk=1024, ldv=1024)
     for change in (dict(), dict(workspace=FAKE, workspace_bytes=need - 1), dict(workspace=FAKE + 8, workspace_bytes=need)):
         assert lib.ff_cross_attention(*(one | change).values()) == BAD
         assert "workspace" in _err()
