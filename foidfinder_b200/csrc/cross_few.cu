@@ -93,7 +93,8 @@ struct FewArgs {
   float2* part_ml;  // [splits][q_rows * heads]: maximum (in powers of two) and sum
 };
 
-template <class T, int ATOMS, int RG>
+// SHORT: sequences of about a tile of keys, whose products leave out groups of 16 keys that there are not.
+template <class T, int ATOMS, int RG, bool SHORT>
 __global__ void __launch_bounds__(kFewThreads, few_ctas(ATOMS)) cross_few_kernel(const __grid_constant__ FewArgs a) {
   constexpr int STAGES = few_stages(ATOMS), TILE = few_tile(ATOMS), KG = 4 / RG, KW = kKeys / KG;
   constexpr int ROWS = 16 * RG, STEPS = ATOMS * 4;
@@ -122,6 +123,7 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(ATOMS)) cross_few_kernel
   const uint8_t* const mask = p.mask != nullptr ? p.mask + ks.at + static_cast<int64_t>(first) * kKeys : nullptr;
   const int keys = max(0, min(tiles * kKeys, ks.n - first * kKeys));
   const uint32_t base = smem_u32(smem);
+  const int quads = dim / 4, at_once = 32 / quads, lane_row = lane / quads, c = lane % quads * 4;  // when parts are joined
 
   // Mask bytes of tile i's keys lane and lane + 32 (1 without a mask), 0 past the end.
   uint32_t ahead[2];
@@ -159,6 +161,14 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(ATOMS)) cross_few_kernel
   };
 
   for (int pass = pass0; pass * ROWS < total_rows; pass += a.passes) {
+    fetch(0);
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) {
+      const uint64_t bits = ahead_bits();
+      fetch(i + 1);
+      if (i < tiles) load(i, bits);
+      copies_commit();
+    }
     // Rows of this lane: lane / 4 and 8 further, of the warp's 16.
     uint32_t qf[STEPS][4];
 #pragma unroll
@@ -177,14 +187,6 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(ATOMS)) cross_few_kernel
     for (int n = 0; n < 2 * STEPS; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
-    fetch(0);
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) {
-      const uint64_t bits = ahead_bits();
-      fetch(i + 1);
-      if (i < tiles) load(i, bits);
-      copies_commit();
-    }
     for (int i = 0; i < tiles; ++i) {
       copies_wait<STAGES - 2>();
       __syncthreads();  // tile i has landed for all, and all are done with tile i - 1, whose place is next
@@ -194,6 +196,7 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(ATOMS)) cross_few_kernel
       fetch(i + STAGES);
       const uint32_t kt = base + (i % STAGES) * 2 * TILE, vt = kt + TILE;
       const uint64_t bits = taken[i % STAGES] >> (kg * KW);  // of this warp's keys
+      const int groups = SHORT ? (min(KW, keys - i * kKeys - kg * KW) + 15) >> 4 : KW / 16;  // of 16 keys (none: 0 or less)
       float s[KW / 8][4];
 #pragma unroll
       for (int n = 0; n < KW / 8; ++n)
@@ -204,6 +207,7 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(ATOMS)) cross_few_kernel
         if (k * 16 >= dim) break;
 #pragma unroll
         for (int n = 0; n < KW / 16; ++n) {
+          if (SHORT && n >= groups) break;
           uint32_t f[4];
           ldmatrix4(kt + tile_byte(kg * KW + n * 16 + (lane >> 4) * 8 + (lane & 7), k * 2 + (lane >> 3 & 1)), f);
           mma16816<T>(s[2 * n], qf[k], f[0], f[1]);
@@ -249,14 +253,17 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(ATOMS)) cross_few_kernel
         }
       }
 #pragma unroll
-      for (int n = 0; n < KW / 8; ++n)
+      for (int n = 0; n < KW / 8; ++n) {
+        if (SHORT && n >= 2 * groups) break;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           s[n][e] = ex2_approx(fmaf(s[n][e], p.scale_log2, kShift - base_m[e >> 1]));
           l[e >> 1] += s[n][e];
         }
+      }
 #pragma unroll
       for (int n = 0; n < KW / 16; ++n) {
+        if (SHORT && n >= groups) break;
         const uint32_t pf[4] = {Pair16<T>::pack(s[2 * n][0], s[2 * n][1]), Pair16<T>::pack(s[2 * n][2], s[2 * n][3]),
                                 Pair16<T>::pack(s[2 * n + 1][0], s[2 * n + 1][1]), Pair16<T>::pack(s[2 * n + 1][2], s[2 * n + 1][3])};
 #pragma unroll
@@ -287,10 +294,10 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(ATOMS)) cross_few_kernel
         if (n * 8 < dim) *reinterpret_cast<float2*>(dst + n * 8) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
     }
     __syncthreads();
-    const int quads = dim / 4;
-    for (int i = t; i < ROWS * quads; i += kFewThreads) {
-      const int r = i / quads, c = (i - r * quads) * 4, row = pass * ROWS + r;
-      if (row >= total_rows) break;
+    // A row of `dim / 4` lanes, as many rows at a time as a warp has of them.
+    for (int r = warp * at_once + lane_row; r < ROWS; r += 4 * at_once) {
+      const int row = pass * ROWS + r;
+      if (lane_row >= at_once || row >= total_rows) break;
       float top = part_m[0][r];
 #pragma unroll
       for (int g = 1; g < KG; ++g) top = fmaxf(top, part_m[g][r]);
@@ -324,9 +331,9 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(ATOMS)) cross_few_kernel
     if (a.cluster) {
       __syncwarp();
       cluster_sync();  // every CTA's part of these rows is there
-      const int rows = min(ROWS, total_rows - pass * ROWS);
-      for (int i = split * kFewThreads + t; i < rows * quads; i += a.splits * kFewThreads) {
-        const int r = i / quads, c = (i - r * quads) * 4, row = pass * ROWS + r;
+      for (int r = (split * 4 + warp) * at_once + lane_row; r < ROWS; r += a.splits * 4 * at_once) {
+        const int row = pass * ROWS + r;
+        if (lane_row >= at_once || row >= total_rows) break;
         float2 ml[kCluster];
         float4 v[kCluster];
 #pragma unroll
@@ -412,13 +419,13 @@ __global__ void __launch_bounds__(32 * kJoinWarps) cross_join_kernel(const __gri
       make_uint2(Pair16<T>::pack(acc.x * inv, acc.y * inv), Pair16<T>::pack(acc.z * inv, acc.w * inv));
 }
 
-template <class T, int ATOMS, int RG>
+template <class T, int ATOMS, int RG, bool SHORT>
 int launch_few(const FewArgs& a, cudaStream_t s) {
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !configured[dev]) {
-    if (cudaFuncSetAttribute(cross_few_kernel<T, ATOMS, RG>, cudaFuncAttributeMaxDynamicSharedMemorySize, few_smem(ATOMS)) != cudaSuccess)
+    if (cudaFuncSetAttribute(cross_few_kernel<T, ATOMS, RG, SHORT>, cudaFuncAttributeMaxDynamicSharedMemorySize, few_smem(ATOMS)) != cudaSuccess)
       return check_launch("cross_few: cudaFuncSetAttribute");
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
@@ -438,10 +445,10 @@ int launch_few(const FewArgs& a, cudaStream_t s) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    cudaLaunchKernelEx(&cfg, cross_few_kernel<T, ATOMS, RG>, a);
+    cudaLaunchKernelEx(&cfg, cross_few_kernel<T, ATOMS, RG, SHORT>, a);
     return check_launch("cross_few_kernel");
   }
-  launch(cross_few_kernel<T, ATOMS, RG>, dim3(static_cast<unsigned>(grid)), dim3(kFewThreads), few_smem(ATOMS), s, a);
+  launch(cross_few_kernel<T, ATOMS, RG, SHORT>, dim3(static_cast<unsigned>(grid)), dim3(kFewThreads), few_smem(ATOMS), s, a);
   if (a.splits > 1) {
     const int rc = check_launch("cross_few_kernel");
     if (rc != FF_OK) return rc;
@@ -451,27 +458,42 @@ int launch_few(const FewArgs& a, cudaStream_t s) {
   return check_launch("cross_few_kernel");
 }
 
+template <class T, bool SHORT>
+int launch_few_rows(const FewArgs& a, int row_tiles, cudaStream_t s) {
+  if (a.p.dim <= 64) {
+    if (row_tiles == 1) return launch_few<T, 1, 1, SHORT>(a, s);
+    return row_tiles == 2 ? launch_few<T, 1, 2, SHORT>(a, s) : launch_few<T, 1, 4, SHORT>(a, s);
+  }
+  if (row_tiles == 1) return launch_few<T, 2, 1, SHORT>(a, s);
+  return row_tiles == 2 ? launch_few<T, 2, 2, SHORT>(a, s) : launch_few<T, 2, 4, SHORT>(a, s);
+}
 template <class T>
 int launch_few_type(const FewArgs& a, int row_tiles, cudaStream_t s) {
-  if (a.p.dim <= 64) {
-    if (row_tiles == 1) return launch_few<T, 1, 1>(a, s);
-    return row_tiles == 2 ? launch_few<T, 1, 2>(a, s) : launch_few<T, 1, 4>(a, s);
-  }
-  if (row_tiles == 1) return launch_few<T, 2, 1>(a, s);
-  return row_tiles == 2 ? launch_few<T, 2, 2>(a, s) : launch_few<T, 2, 4>(a, s);
+  const bool brief = a.p.k_rows <= static_cast<int64_t>(kKeys) * a.p.sequences;
+  return brief ? launch_few_rows<T, true>(a, row_tiles, s) : launch_few_rows<T, false>(a, row_tiles, s);
 }
 
 }  // namespace
 
 CrossFewPlan cross_few_plan(int q_rows, int k_rows, int sequences, int heads, int kv_heads, int dim) {
   CrossFewPlan plan{};
-  plan.few = static_cast<int64_t>(q_rows) <= 64LL * sequences || k_rows == 0;
-  if (!plan.few) return plan;
-  const int64_t rows = (static_cast<int64_t>(q_rows) + sequences - 1) / sequences * (heads / kv_heads);
+  const int64_t queries = (static_cast<int64_t>(q_rows) + sequences - 1) / sequences, keys = (static_cast<int64_t>(k_rows) + sequences - 1) / sequences;
+  const int64_t rows = queries * (heads / kv_heads);
   plan.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
   plan.passes = static_cast<int>(std::max<int64_t>(1, (rows + 16 * plan.row_tiles - 1) / (16 * plan.row_tiles)));
   const int64_t ctas = static_cast<int64_t>(sequences) * kv_heads * plan.passes;
-  const int64_t tiles = ((static_cast<int64_t>(k_rows) + sequences - 1) / sequences + kKeys - 1) / kKeys;
+  const int64_t tiles = (keys + kKeys - 1) / kKeys;
+  // Which kernel: the one that is expected to take less time, in us. This one does 70, 125 or 160 TFLOP/s on the rows of its row
+  // tiles (1, 2 or 4 of them), or reads 5.2 TB/s. The other takes 1.5 us for 128 keys and up to 256 queries of a head (2.1
+  // for heads of more than 64 columns) on every SM at once, but has no parts of a sequence's keys. Measured (few, other):
+  // 64 x 32 queries, 1025 keys, 16 heads of 64: 64, 85 us; 64 x 40: 95, 92; 1 x 64 queries, 5184 keys: 22, 50; 16 x 32, 2048
+  // keys, 16 heads of 128: 72, 70; 16 x 40: 115, 70; 1 x 64, 2048 keys, 32 heads over 8: 29, 36.
+  const double macs = static_cast<double>(ctas) * 16 * plan.row_tiles * ((keys + 15) / 16 * 16) * dim, rate = plan.row_tiles == 1 ? 70e6 : plan.row_tiles == 2 ? 125e6 : 160e6;
+  const double few = std::max(4 * macs / rate, 4.0 * sequences * keys * kv_heads * dim / 5.2e6) + 3;
+  const int64_t items = static_cast<int64_t>(sequences) * heads * ((queries + 255) / 256), sms = sm_count();
+  const double other = static_cast<double>((items + sms - 1) / sms) * ((keys + 127) / 128) * (dim <= 64 ? 1.5 : 2.1) + 3;
+  plan.few = few <= other || k_rows == 0;
+  if (!plan.few) return plan;
   // As many parts as fill the GPU's places for CTAs, of two tiles at least
   const int64_t places = static_cast<int64_t>(sm_count()) * few_ctas(dim <= 64 ? 1 : 2);
   plan.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({places / ctas, (tiles + 1) / 2, 1024})));
