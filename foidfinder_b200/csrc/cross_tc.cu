@@ -4,14 +4,16 @@
 //
 // Bound by the exponentials (one per query, key and head) and the hand-overs between tensor core and softmax. Persistent
 // CTAs (one per SM, 320 threads, all 512 TMEM columns) walk items: up to 256 queries (two tiles of 128) of one sequence
-// and head, against that sequence's keys in tiles of 128; consecutive items overlap in the pipeline.
+// and head, against that sequence's keys in tiles of 128; consecutive items overlap in the pipeline. Two streams, each with
+// scores S, weights P and output O in TMEM, take a query tile each, or, of an item with one tile, every second key tile
+// each, and are joined at its end.
 //   warp 0     loads, by TMA: an item's queries, and key and value tiles in turn through one ring. A tile's rows are rows of
 //              the whole matrix, whatever sequence they belong to.
-//   warp 1     MMAs, by one elected thread: S_i = Q_i K^T to TMEM columns [128 i, +128), and O_i += P_i V, P_i read from where
-//              S_i was, to columns [256 + 128 i, +dim). Order per key tile j: PV_0(j), S_0(j + 1), PV_1(j), S_1(j + 1); MMAs of
-//              one thread execute in order, so S_i(j + 1) finds P_i(j) consumed. (A thread for each tile let both tiles
-//              fall in step and then wait together: 619 us where this takes 469.)
-//   warps 2-5  softmax of query tile 0, warps 6-9 of tile 1, a query per thread: 32 scores at a time, the next 32 on their
+//   warp 1     MMAs, by one elected thread: S_i = Q K^T of stream i to TMEM columns [128 i, +128), and O_i += P_i V, P_i read
+//              from where S_i was, to columns [256 + 128 i, +dim). Order per key tile j of a pair: PV_0(j), S_0(j + 1), PV_1(j),
+//              S_1(j + 1); MMAs of one thread execute in order, so S_i(j + 1) finds P_i(j) consumed. (A thread for each
+//              stream let both fall in step and then wait together: 619 us where this takes 465.)
+//   warps 2-5  softmax of stream 0, warps 6-9 of stream 1, a query per thread: 32 scores at a time, the next 32 on their
 //              way meanwhile, P = 2^(s - m + 7) in 16 bits, the sum of P in f32 before that rounding. m is the
 //              maximum at some earlier time: the exponentials start at once, and the new maximum is found beside them.
 //              Only where it has grown by more than 2^8 (P could pass 2^15, fp16's range) do m, O, the sum and the P so
@@ -33,12 +35,18 @@ constexpr int kTcThreads = 320;
 constexpr int kSlots = 5;          // of the ring
 constexpr int kTile = 2 * kAtom;   // 128 rows of 128 columns
 constexpr int kOffRing = 2 * kTile;
-constexpr int kOffTable = kOffRing + kSlots * kTile;
+constexpr int kOffJoin = kOffRing + kSlots * kTile;  // [128 rows] (shift, sum) of stream 1
+constexpr int kOffTable = kOffJoin + 128 * 8;
 constexpr int kOffBars = kOffTable + kTable * static_cast<int>(sizeof(Item));
 constexpr int kTcSmem = 1024 + kOffBars + 256;
 static_assert(kTcSmem <= 232448, "shared memory of a CTA");
 
-// TMEM columns of query tile i.
+// Whether the streams divide the keys of an item's only query tile, or (neither) the first has all of a single key tile.
+__device__ __forceinline__ bool pair_of(const Item& i) { return i.nq > kBQ; }
+__device__ __forceinline__ bool split_of(const Item& i) { return i.nq <= kBQ && i.nk > kBK; }
+__device__ __forceinline__ int tiles_of(const Item& i) { return (i.nk + kBK - 1) / kBK; }
+
+// TMEM columns of stream i.
 __host__ __device__ constexpr uint32_t t_s(int i) { return 128u * i; }
 __host__ __device__ constexpr uint32_t t_o(int i) { return 256u + 128u * i; }
 
@@ -72,8 +80,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint64_t* empty = full + kSlots;    // [kSlots]
   uint64_t* s_full = empty + kSlots;  // [2], per query tile
   uint64_t* p_full = s_full + 2;      // [2]
-  uint64_t* pv_done = p_full + 2;     // [2]
-  uint64_t* drain = pv_done + 2;
+  uint64_t* o_full = p_full + 2;      // [2]: a stream's last product of an item
+  uint64_t* joined = o_full + 2;     // stream 1's maxima and sums are there: its 4 warps
+  uint64_t* o_free = joined + 1;      // and its O has been read: stream 0's
+  uint64_t* drain = o_free + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -95,8 +105,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
-      mbar_init(&pv_done[i], 1);
+      mbar_init(&o_full[i], 1);
     }
+    mbar_init(joined, 4);
+    mbar_init(o_free, 4);
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -182,9 +194,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const uint32_t ring = smem_u32(smem) + kOffRing;
       // Keys of a tile that its products cover: all, or the sequence's last ones rounded up to 16.
       auto width = [](int nk, int j) { return min(kBK, (nk - j * kBK + 15) & ~15); };
-      auto issue_s = [&](int i, int slot, int keys) {
+      auto issue_s = [&](int i, int tile, int slot, int keys) {
         const uint32_t id = idesc_f16(128, keys) | fmt;
-        const uint64_t qd = sdesc_k_sw128(smem_u32(smem) + i * kTile);
+        const uint64_t qd = sdesc_k_sw128(smem_u32(smem) + tile * kTile);
         const uint64_t kd = sdesc_k_sw128(ring + slot * kTile);
 #pragma unroll
         for (int k = 0; k < 8; ++k)
@@ -205,54 +217,67 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (ok) ok = mbar_wait<true>(b, parity, abort_flag, err, kDevTimeoutAttn);
         return ok;
       };
-      int m = 0, slot = 0;  // slot, round: of the current key tile's K
-      uint32_t round = 0, count[2] = {0, 0};
-      Item cur{}, nxt{};
-      bool have = items.next<true>(cur);
-      if (have && wait(q_full, 0) && wait(&full[0], 0)) {
+      // Ring positions: key tile t over all items has K at 2 t, V at 2 t + 1.
+      auto arrived = [&](uint32_t at) {
+        const bool r = wait(&full[at % kSlots], at / kSlots & 1u);
         tc_fence_after();
-        issue_s(0, 0, width(cur.nk, 0));
-        if (cur.nq > kBQ) issue_s(1, 0, width(cur.nk, 0));
-        tc_commit(&empty[0]);
-        if (cur.nk <= kBK) tc_commit(q_empty);
+        return r;
+      };
+      int m = 0, s_left = 0;  // item; its S that are to be issued, after which its queries may go
+      uint32_t g0 = 0, count[2] = {0, 0};
+      // S of stream i for key tile t of an item; its keys and queries are there. keys_done: no other stream needs them.
+      auto scores = [&](int i, int tile, int slot, int keys, bool keys_done) {
+        issue_s(i, tile, slot, keys);
+        if (keys_done) tc_commit(&empty[slot]);
+        if (--s_left == 0) tc_commit(q_empty);
+      };
+      Item cur{}, nxt{};
+      int first_done = 0;  // bits: streams whose first S of the next item has been issued
+      // The same for its first key tile, of item `k`, if it has one.
+      auto first_scores = [&](int i, const Item& item, int k, uint32_t g) {
+        if (i == 1 && !pair_of(item) && !split_of(item)) return;
+        if (first_done == 0) {
+          if (!wait(q_full, static_cast<uint32_t>(k) & 1u)) return;
+          s_left = tiles_of(item) * (pair_of(item) ? 2 : 1);
+        }
+        const int t = split_of(item) ? i : 0;
+        if (!arrived(2 * (g + t))) return;
+        scores(i, pair_of(item) ? i : 0, 2 * (g + t) % kSlots, width(item.nk, t), !pair_of(item) || first_done != 0);
+        first_done |= 1 << i;
+      };
+      bool have = items.next<true>(cur);
+      if (have) {
+        first_scores(0, cur, 0, 0);
+        if (ok) first_scores(1, cur, 0, 0);
       }
       while (have && ok) {
-        const bool more = items.next<true>(nxt), two = cur.nq > kBQ;
-        const int nkv = (cur.nk + kBK - 1) / kBK;
-        for (int j = 0; j < nkv && ok; ++j) {
-          const bool last = j == nkv - 1, next = !last || more;
-          int v_slot = slot + 1, k_slot = slot + 2;
-          uint32_t v_round = round, k_round = round;
-          if (v_slot >= kSlots) v_slot -= kSlots, ++v_round;
-          if (k_slot >= kSlots) k_slot -= kSlots, ++k_round;
-          const int keys = width(cur.nk, j);
-          const int next_keys = last ? width(nxt.nk, 0) : width(cur.nk, j + 1);  // unused without a next tile
-          // One query tile: P V of this key tile, then S of the next one.
-          auto turn = [&](int i, bool here, bool there) {
-            if (here) {
-              if (!wait(&p_full[i], count[i] & 1u)) return;
-              tc_fence_after();
-              issue_pv(i, v_slot, keys, j == 0);
-              tc_commit(&pv_done[i]);
-              ++count[i];
-            }
-            if (there) issue_s(i, k_slot, next_keys);
+        const bool more = items.next<true>(nxt), two = pair_of(cur), split = split_of(cur);
+        const int nkv = tiles_of(cur), stride = split ? 2 : 1;
+        first_done = 0;
+        for (int t = 0; t < nkv && ok; ++t) {
+          // All that the issuing after a wait for P needs, worked out before it.
+          const int keys = width(cur.nk, t), next_keys = width(cur.nk, t + stride);
+          const bool on = t + stride < nkv;
+          const uint32_t v = 2 * (g0 + t) + 1;
+          const int v_slot = v % kSlots, k_slot = (v_slot + 2 * stride - 1) % kSlots;
+          auto turn = [&](int i) {
+            if ((!two || i == 0) && ((on && !arrived(2 * (g0 + t + stride))) || !arrived(v))) return;  // of a pair, stream 0 has waited
+            if (!wait(&p_full[i], count[i] & 1u)) return;
+            tc_fence_after();
+            issue_pv(i, v_slot, keys, t < stride);
+            ++count[i];
+            if (on)  // before anything else: the softmax waits for it
+              scores(i, two ? i : 0, k_slot, next_keys, !two || i == 1);
+            else
+              tc_commit(&o_full[i]);
+            if (!two || i == 1) tc_commit(&empty[v_slot]);
+            if (!on && more) first_scores(i, nxt, m + 1, g0 + nkv);
           };
-          if (!wait(&full[v_slot], v_round & 1u) || (next && !wait(&full[k_slot], k_round & 1u)) ||
-              (next && last && !wait(q_full, static_cast<uint32_t>(m + 1) & 1u)))
-            break;
-          tc_fence_after();
-          turn(0, true, next);
-          if (ok) turn(1, two, next && (last ? nxt.nq > kBQ : two));
-          if (!ok) break;
-          tc_commit(&empty[v_slot]);
-          if (next) {
-            tc_commit(&empty[k_slot]);
-            if (last ? nxt.nk <= kBK : j + 1 == nkv - 1) tc_commit(q_empty);  // the last use of these queries
-          }
-          slot = k_slot;
-          round = k_round;
+          if (!split || (t & 1) == 0) turn(0);
+          if (ok && (two || (split && (t & 1)))) turn(1);
         }
+        if (ok && more && !two && !split) first_scores(1, nxt, m + 1, g0 + nkv);  // stream 1 had nothing here
+        g0 += nkv;
         cur = nxt;
         have = more;
         ++m;
@@ -271,27 +296,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int g = (warp - 2) >> 2, quarter = warp & 3;
     const uint32_t ts = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + t_s(g);
     const uint32_t to = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + t_o(g);
-    const int first_row = g * kBQ + quarter * 32;  // of this warp, in the item
+    float2* const join = reinterpret_cast<float2*>(smem + kOffJoin) + quarter * 32 + lane;
     bool ok = true;
-    int v_slot = 1;
-    uint32_t v_round = 0, tiles = 0;
+    uint32_t g0 = 0, tiles = 0, worked = 0, splits = 0, freed = 0;  // key tiles of the items before; of this stream, and its items; split ones, and waited for
     Item item;
     while (ok && items.next<false>(item)) {
+      const bool two = pair_of(item), split = split_of(item);
+      const int first_row = (two ? g * kBQ : 0) + quarter * 32;  // of this warp, in the item
       const int64_t row = item.q + first_row + lane;
       const bool store = first_row + lane < item.nq, active = first_row < item.nq;
       T* const out = static_cast<T*>(p.out) + row * p.ldo + static_cast<int64_t>(items.head) * dim;
       if (item.nk == 0) {
-        if (store)
+        if (store && (two || g == 0))
           for (int c = 0; c < dim; c += 8) *reinterpret_cast<uint4*>(out + c) = make_uint4(0, 0, 0, 0);
         continue;
       }
-      const int nkv = (item.nk + kBK - 1) / kBK;
-      if (g * kBQ >= item.nq) {  // this group has no queries here; the ring goes on
-        const uint32_t at = static_cast<uint32_t>(v_slot) + 2u * nkv;
-        v_round += at / kSlots;
-        v_slot = static_cast<int>(at % kSlots);
-        continue;
-      }
+      const int nkv = tiles_of(item), stride = split ? 2 : 1, first = split ? g : 0;
+      const uint32_t g1 = g0;
+      g0 += nkv;
+      if (g == 1 && !two && !split) continue;  // nothing for this stream
       const uint8_t* const mask = p.mask != nullptr ? p.mask + item.k : nullptr;
       uint32_t ahead[4];  // mask bytes of the next tile's keys 32 c + lane
       auto fetch = [&](int j) {
@@ -301,11 +324,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           ahead[c] = key < item.nk ? __ldg(mask + key) : 0;
         }
       };
-      if (mask != nullptr) fetch(0);
+      if (mask != nullptr) fetch(first);
       float shift = 0.f;  // 7 - m, once there is an m
       bool set = false;
       float2 sum = make_float2(0.f, 0.f);
-      for (int j = 0; j < nkv; ++j, ++tiles) {
+      for (int j = first; j < nkv; j += stride, ++tiles) {
         const int left = item.nk - j * kBK;
         uint32_t bits[4];  // keys that take part
         bool every = left >= kBK;
@@ -315,7 +338,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             bits[c] = __ballot_sync(0xffffffffu, ahead[c] != 0);
             every = every && bits[c] == 0xffffffffu;
           }
-          fetch(j + 1);
+          fetch(j + stride);
         } else {
 #pragma unroll
           for (int c = 0; c < 4; ++c) bits[c] = left >= 32 * c + 32 ? 0xffffffffu : left <= 32 * c ? 0u : (1u << (left - 32 * c)) - 1u;
@@ -326,7 +349,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         tc_fence_after();
         if (!every) {  // zeros for the values of keys left out: thread i of the group has key i
-          if (!mbar_wait(&full[v_slot], v_round & 1u, abort_flag, err, kDevTimeoutAttn)) {
+          const uint32_t at = 2 * (g1 + j) + 1, v_slot = at % kSlots;
+          if (!mbar_wait(&full[v_slot], at / kSlots & 1u, abort_flag, err, kDevTimeoutAttn)) {
             ok = false;
             break;
           }
@@ -341,8 +365,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           fence_async_smem();
         }
-        v_slot += 2;
-        if (v_slot >= kSlots) v_slot -= kSlots, ++v_round;
         if (active) {
           const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
           uint32_t s[2][32];
@@ -385,7 +407,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 shift = now;
                 set = true;
               }
-              if (j > 0) rescale(to, dim, corr);
+              if (j > first) rescale(to, dim, corr);
               if (c > 0) rescale_p<T>(ts, c, corr);
               sum.x *= corr;
               sum.y *= corr;
@@ -396,6 +418,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (c < 3) tmem_ld_wait();
           }
         }
+        if (g == 1 && freed != splits) {  // before the first product into this O: stream 0 has read it
+          if (!mbar_wait(o_free, (splits - 1) & 1u, abort_flag, err, kDevTimeoutAttn)) {
+            ok = false;
+            break;
+          }
+          freed = splits;
+        }
         __syncwarp();
         tmem_st_wait();
         tc_fence_before();
@@ -403,22 +432,56 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (lane == 0) mbar_arrive(&p_full[g]);
       }
       if (!ok) break;
-      if (!mbar_wait(&pv_done[g], (tiles - 1) & 1u, abort_flag, err, kDevTimeoutAttn)) break;
+      if (!mbar_wait(&o_full[g], worked++ & 1u, abort_flag, err, kDevTimeoutAttn)) break;
       tc_fence_after();
+      float l = sum.x + sum.y, mine = 1.f, other = 0.f;  // what both streams' outputs count
+      if (split) {  // a stream's O is 2^shift times what it stands for; stream 0 writes the result
+        if (g == 1) {
+          *join = make_float2(set ? shift : INFINITY, l);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(joined);
+          ++splits;
+          continue;
+        }
+        if (!mbar_wait(joined, splits & 1u, abort_flag, err, kDevTimeoutAttn)) break;
+        ++splits;
+        tc_fence_after();
+        const float2 theirs = *join;
+        const float my_shift = set ? shift : INFINITY, least = fminf(my_shift, theirs.x);
+        mine = my_shift == least ? 1.f : ex2_approx(least - my_shift);
+        other = theirs.x == least ? 1.f : ex2_approx(least - theirs.x);
+        l = l * mine + theirs.y * other;
+      }
       if (active) {
-        const float l = sum.x + sum.y, inv = l == 0.f ? 0.f : 1.f / l;  // no key took part: zeros
+        const float inv = l == 0.f ? 0.f : 1.f / l;  // no key took part: zeros
+        mine *= inv;
+        other *= inv;
         for (int c = 0; c < dim; c += 16) {
           uint32_t o[16];
           tmem_ld16(to + c, o);
           tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * mine);
+          if (split) {
+            uint32_t o1[16];
+            tmem_ld16(to + t_o(1) - t_o(0) + c, o1);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(fmaf(__uint_as_float(o1[e]), other, __uint_as_float(o[e])));
+          }
           if (store) {
             uint32_t w[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = Pair16<T>::pack(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+            for (int e = 0; e < 8; ++e) w[e] = Pair16<T>::pack(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
             *reinterpret_cast<uint4*>(out + c) = make_uint4(w[0], w[1], w[2], w[3]);
             *reinterpret_cast<uint4*>(out + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
           }
         }
+      }
+      if (split) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(o_free);
       }
       // The next item's first product into O waits for this group's next P, which comes after these reads.
     }

@@ -8,7 +8,7 @@ namespace ff {
 
 constexpr int kBQ = 128;          // queries of a tile
 constexpr int kAtom = 128 * 128;  // bytes: 128 rows of 64 columns, 128-byte swizzle
-constexpr int kTable = 64;        // items of a CTA that are looked up ahead, all at once
+constexpr int kTable = 16;        // items of a CTA that are looked up ahead, all at once
 constexpr float kGrowth = 8.f;    // powers of two by which the maximum may grow before O is rescaled
 constexpr float kUp = 7.f;        // P = 2^(x + 7): at most 2^15, in fp16's range
 

@@ -238,14 +238,14 @@ __global__ void __launch_bounds__(kThreads64, 1)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
               if (16 * k < keys) mma_ts(tmem + t_o64(stream), tmem + t_s64(stream) + 8 * k, vd + static_cast<uint64_t>(k * 128), id_o, (t >= ways || k > 0) ? 1u : 0u);
-            tc_commit(&empty[slot + 1]);
-            if (on) {
+            if (on) {  // before anything else: the softmax waits for it
               issue_s(i, cur, m, t + ways, g + ways);
             } else {
               tc_commit(&o_full[stream]);
               first[i] = true;
               if (next) first_s(i);
             }
+            tc_commit(&empty[slot + 1]);
           }
           if (!mine && ok) {  // the other thread's, which needs this one's consent to load over it
             if (!wait(&full[slot], round) || !wait(&full[slot + 1], round)) break;
