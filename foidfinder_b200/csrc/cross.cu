@@ -27,6 +27,7 @@ extern "C" int ff_cross_attention(const void* q, int64_t ldq, const void* k, int
   FF_REQUIRE(q_start != nullptr || q_rows % sequences == 0, "ff_cross_attention: %d queries are not %d equal pieces", q_rows, sequences);
   FF_REQUIRE(k_start != nullptr || k_rows % sequences == 0, "ff_cross_attention: %d keys are not %d equal pieces", k_rows, sequences);
   FF_REQUIRE(q && out && (k_rows == 0 || (k && v)), "ff_cross_attention: NULL pointer");
+  FF_REQUIRE(out != q && out != k && out != v, "ff_cross_attention: out must not be an input");
   FF_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out), "ff_cross_attention: q, k, v and out must be 16-byte aligned");
   auto words = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; };
   FF_REQUIRE(words(q_start) && words(k_start) && words(k_len), "ff_cross_attention: misaligned starts or lengths");

@@ -149,15 +149,27 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(ATOMS)) cross_few_kernel
     const uint32_t d = base + st * 2 * TILE + own;
     const T* ks = k_own + 4 * i * k16;
     const T* vs = v_own + 4 * i * v16;
-    const uint32_t rows = static_cast<uint32_t>((bits >> (t >> 3) & 1) | (bits >> (16 + (t >> 3)) & 1) << 1 | (bits >> (32 + (t >> 3)) & 1) << 2 | (bits >> (48 + (t >> 3)) & 1) << 3);
+    if (bits == ~0ull) {
 #pragma unroll
-    for (int n = 0; n < 4; ++n, ks += k16, vs += v16)
+      for (int n = 0; n < 4; ++n, ks += k16, vs += v16)
+#pragma unroll
+        for (int c = 0; c < ATOMS; ++c)
+          if (c * 8 + (t & 7) < chunks) {
+            copy16(d + c * (kKeys * 128) + n * 2048, ks + c * 64, true);
+            copy16(d + TILE + c * (kKeys * 128) + n * 2048, vs + c * 64, true);
+          }
+      return;
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n, ks += k16, vs += v16) {
+      const bool take = bits >> (16 * n + (t >> 3)) & 1;  // a key left out is not read
 #pragma unroll
       for (int c = 0; c < ATOMS; ++c)
-        if (c * 8 + (t & 7) < chunks) {  // a key left out is not read
-          copy16(d + c * (kKeys * 128) + n * 2048, ks + c * 64, rows >> n & 1);
-          copy16(d + TILE + c * (kKeys * 128) + n * 2048, vs + c * 64, rows >> n & 1);
+        if (c * 8 + (t & 7) < chunks) {
+          copy16(d + c * (kKeys * 128) + n * 2048, take ? ks + c * 64 : kp, take);
+          copy16(d + TILE + c * (kKeys * 128) + n * 2048, take ? vs + c * 64 : vp, take);
         }
+    }
   };
 
   for (int pass = pass0; pass * ROWS < total_rows; pass += a.passes) {

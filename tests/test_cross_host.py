@@ -124,14 +124,14 @@ def test_block_end_nothing_to_do():
 
 
 # ---------------------------------------------------------------- cross attention
-CROSS = dict(q=FAKE, ldq=256, k=FAKE, ldk=128, v=FAKE, ldv=128, out=FAKE, ldo=256, dtype=0, q_rows=8, k_rows=100, sequences=2, q_start=None, k_start=None, k_len=None,
+CROSS = dict(q=FAKE, ldq=256, k=FAKE, ldk=128, v=FAKE, ldv=128, out=2 * FAKE, ldo=256, dtype=0, q_rows=8, k_rows=100, sequences=2, q_start=None, k_start=None, k_len=None,
              mask=None, heads=4, kv_heads=2, head_dim=64, scale=0.125, workspace=None, workspace_bytes=0, stream=None)
 
 
 @pytest.mark.parametrize(("change", "message"), [
     (dict(dtype=2), "type"), (dict(heads=0), "heads"), (dict(kv_heads=3), "heads"), (dict(heads=2048), "heads"), (dict(head_dim=24), "head_dim"), (dict(head_dim=144), "head_dim"),
     (dict(head_dim=0), "head_dim"), (dict(q_rows=-1), "shape"), (dict(k_rows=-1), "shape"), (dict(sequences=-1), "shape"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"),
-    (dict(scale=math.nan), "scale"), (dict(scale=math.inf), "scale"), (dict(q_rows=7), "equal pieces"), (dict(k_rows=99), "equal pieces"), (dict(q=None), "NULL"), (dict(v=None), "NULL"),
+    (dict(scale=math.nan), "scale"), (dict(scale=math.inf), "scale"), (dict(q_rows=7), "equal pieces"), (dict(k_rows=99), "equal pieces"), (dict(q=None), "NULL"), (dict(v=None), "NULL"), (dict(out=FAKE), "an input"),
     (dict(q=FAKE + 8), "aligned"), (dict(k=FAKE + 2), "aligned"), (dict(out=FAKE + 2), "aligned"), (dict(k_start=FAKE + 2), "misaligned"), (dict(k_len=FAKE + 1), "misaligned"),
     (dict(ldq=255), "strides"), (dict(ldk=120), "strides"), (dict(ldv=129), "strides"), (dict(ldo=260), "strides"), (dict(q_rows=1 << 30, ldq=1 << 12), "each key head")])
 def test_cross_attention_refusals(change, message):

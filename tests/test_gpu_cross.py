@@ -315,6 +315,8 @@ RAGGED = {
     "uneven": ([1, 1, 1, 1, 1000], [64, 65, 63, 1, 190]),
     "uneven the other way": ([900, 500, 400] + [1] * 12, [100] * 15),
     "nothing": ([0, 0, 5], [7, 0, 0]),
+    "short on average": ([2, 1, 3] + [1] * 20, [900, 0, 130] + [3] * 20),
+    "queries of one tile and of two": ([128, 129, 1, 256, 257, 384, 100], [128, 129, 300, 64, 257, 700, 1000]),
     "many": ([i % 5 for i in range(150)], [(7 * i) % 90 for i in range(150)]),
     "many long": ([(37 * i) % 300 for i in range(40)], [(53 * i) % 400 for i in range(40)]),
 }
@@ -377,6 +379,28 @@ def test_attention_starts_beyond_the_rows(cuda_device, no_device_error, nq):
     q, k, v = _qkv(2 * nq, 300, 2, 2, 64, F16)
     out = _attend(q, k, v, heads=2, head_dim=64, q_start=torch.tensor([-4, nq, 5 * nq + 9]).int(), k_start=torch.tensor([-100, 100, 1 << 30]).int())
     _check_attention(out, q, k, v, heads=2, kv_heads=2, dim=64, pieces=_pieces([nq, nq], [100, 200]))
+
+
+@pytest.mark.parametrize(("sequences", "nq", "nk", "dim"), [(150, 300, 130, 128), (150, 100, 400, 128), (160, 130, 200, 64), (300, 40, 300, 64), (9, 3000, 70, 64), (160, 1, 100, 32)])
+def test_attention_of_many_items_in_a_row(cuda_device, no_device_error, sequences, nq, nk, dim):
+    """More items than SMs, one behind the other in the CTAs' pipelines."""
+    q, k, v = _qkv(sequences * nq, sequences * nk, 2, 1, dim, BF16)
+    out = _attend(q, k, v, heads=2, kv_heads=1, head_dim=dim, sequences=sequences)
+    _check_attention(out, q, k, v, heads=2, kv_heads=1, dim=dim, pieces=_pieces([nq] * sequences, [nk] * sequences))
+
+
+def test_attention_with_offsets_beyond_32_bits(cuda_device, no_device_error):
+    """Keys and values whose rows lie more than 2^32 bytes and 2^31 elements from the first."""
+    rows, pitch = 700_000, 4096
+    big = torch.empty(rows, pitch, dtype=F16, device="cuda")
+    for nq in (1, 300):
+        q, k, v = _qkv(nq, 500, 2, 2, 64, F16, seed=nq)
+        at = rows - 500
+        big[at:, :128], big[at:, 2048:2176] = k.cuda(), v.cuda()
+        starts = torch.tensor([at, rows]).int().cuda()
+        out = torch.empty(nq, 128, dtype=F16, device="cuda")
+        ops.cross_attention(q.cuda(), big[:, :128], big[:, 2048:2176], out, heads=2, head_dim=64, k_start=starts, q_start=torch.tensor([0, nq]).int().cuda())
+        _check_attention(out, q, k, v, heads=2, kv_heads=2, dim=64, pieces=_pieces([nq], [500]))
 
 
 @pytest.mark.parametrize("nq", [2, 140])
@@ -555,7 +579,7 @@ def test_refusals(cuda_device, monkeypatch, short):
             end(**(e | change))
     for change in (dict(q=x.cpu()), dict(q=x.float()), dict(k=c["k"].bfloat16()), dict(v=c["v"][:5]), dict(out=x[:3]), dict(heads=3), dict(kv_heads=1), dict(heads=0), dict(head_dim=32),
                    dict(head_dim=24, heads=2), dict(q_start=c["q_start"].long()), dict(q_start=c["q_start"].cpu()), dict(k_start=c["k_start"][:2]), dict(k_len=c["q_start"]),
-                   dict(mask=c["mask"][:5]), dict(mask=c["mask"].float()), dict(sequences=3), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan),
+                   dict(mask=c["mask"][:5]), dict(mask=c["mask"].float()), dict(sequences=3), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(out=x),
                    dict(sequences=4, q_start=None, k_start=None, k_len=None), dict(q=torch.zeros(4, 132, dtype=F16, device=d)[:, :128]), dict(v=strided[:4].repeat(2, 1)[:6, :64])):
         with pytest.raises(RuntimeError):
             cross(**(c | change))
