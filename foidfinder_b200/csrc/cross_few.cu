@@ -495,15 +495,22 @@ CrossFewPlan cross_few_plan(int q_rows, int k_rows, int sequences, int heads, in
   plan.passes = static_cast<int>(std::max<int64_t>(1, (rows + 16 * plan.row_tiles - 1) / (16 * plan.row_tiles)));
   const int64_t ctas = static_cast<int64_t>(sequences) * kv_heads * plan.passes;
   const int64_t tiles = (keys + kKeys - 1) / kKeys;
-  // Which kernel: the one that is expected to take less time, in us. This one does 70, 125 or 160 TFLOP/s on the rows of its row
-  // tiles (1, 2 or 4 of them), or reads 5.2 TB/s. The other takes 1.5 us for 128 keys and up to 256 queries of a head (2.1
-  // for heads of more than 64 columns) on every SM at once, but has no parts of a sequence's keys. Measured (few, other):
-  // 64 x 32 queries, 1025 keys, 16 heads of 64: 64, 85 us; 64 x 40: 95, 92; 1 x 64 queries, 5184 keys: 22, 50; 16 x 32, 2048
-  // keys, 16 heads of 128: 72, 70; 16 x 40: 115, 70; 1 x 64, 2048 keys, 32 heads over 8: 29, 36.
-  const double macs = static_cast<double>(ctas) * 16 * plan.row_tiles * ((keys + 15) / 16 * 16) * dim, rate = plan.row_tiles == 1 ? 70e6 : plan.row_tiles == 2 ? 125e6 : 160e6;
-  const double few = std::max(4 * macs / rate, 4.0 * sequences * keys * kv_heads * dim / 5.2e6) + 3;
+  // Which kernel: the one that is expected to take less time, in us. This one has 4 to 6 us for one CTA's way (up to 8.4 for heads of
+  // more than 64 columns), 0.008 to 0.012 (0.024) for every CTA's start and end, does 70, 125 or 160 TFLOP/s on the rows
+  // of its row tiles (1, 2 or 4 of them), or reads 5.2 TB/s. The other has 3.6 us for every SM's item of up to 256 queries of
+  // a head, and for 128 keys of it 1.8 (2.4), or 1.2 (1.5) up to 128 queries, but has no parts of a sequence's keys. Measured (few, other):
+  // 64 x 32 queries, 1025 keys, 16 heads of 64: 63, 85 us; 64 x 40: 95, 92; 64 x 64 queries, 128 keys: 22, 33; 64 x 128: 40, 34;
+  // 1 x 64 queries, 5184 keys: 22, 50; 16 x 32, 2048 keys, 16 heads of 128: 72, 70; 24 x 64, 64 keys, 16 heads over 4: 14,
+  // 13; 24 x 829, 7 keys: 121, 55.
+  const bool wide = dim > 64;
+  const int tiles_of_rows = plan.row_tiles == 4 ? 3 : plan.row_tiles;
+  const double macs = static_cast<double>(ctas) * 16 * plan.row_tiles * ((keys + 15) / 16 * 16) * dim;
+  const double rate[] = {70e6, 125e6, 160e6}, edge[] = {0.008, 0.011, 0.012};
+  const double few = 3 + tiles_of_rows * (wide ? 1.8 : 1.0) + static_cast<double>(ctas) * edge[tiles_of_rows - 1] * (wide ? 2 : 1) +
+                     std::max(4 * macs / rate[tiles_of_rows - 1], 4.0 * sequences * keys * kv_heads * dim / 5.2e6);
   const int64_t items = static_cast<int64_t>(sequences) * heads * ((queries + 255) / 256), sms = sm_count();
-  const double other = static_cast<double>((items + sms - 1) / sms) * ((keys + 127) / 128) * (dim <= 64 ? 1.5 : 2.1) + 3;
+  const double step = queries > 128 ? (wide ? 2.4 : 1.8) : (wide ? 1.5 : 1.2);
+  const double other = 3 + static_cast<double>((items + sms - 1) / sms) * (3.6 + static_cast<double>((keys + 127) / 128) * step);
   plan.few = few <= other || k_rows == 0;
   if (!plan.few) return plan;
   // As many parts as fill the GPU's places for CTAs, of two tiles at least

@@ -66,6 +66,18 @@ __device__ __noinline__ void rescale_p(uint32_t ts, int chunks, float corr) {
   }
 }
 
+// Zeros for the values of those of 32 keys that `out_of` says; out of line, it is rare.
+__device__ __noinline__ void zero_values(uint8_t* v, uint32_t out_of, int lane) {
+  for (int i = 0; i < 8; ++i) {
+    const int key = 4 * i + (lane >> 3);  // 8 lanes, 128 bytes: no two on a bank
+    if (out_of >> key & 1u) {
+      uint8_t* const at = v + key * 128 + (lane & 7) * 16;
+      *reinterpret_cast<uint4*>(at) = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(at + kAtom) = make_uint4(0, 0, 0, 0);
+    }
+  }
+}
+
 template <class T>
 __global__ void __launch_bounds__(kTcThreads, 1)
     cross_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -93,7 +105,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   int* const err = a.err;
   if (a.items == gridDim.x) {  // one item per CTA, perhaps none
     pdl_wait();
-    if (item_at(a, blockIdx.x).nq == 0) return;
+    const Item only = a.by_cost ? item_by_cost(a, reinterpret_cast<int2*>(smem + kOffRing), table) : item_at(a, blockIdx.x);
+    if (only.nq == 0) return;
   }
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -124,7 +137,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   }
   pdl_wait();
   pdl_trigger();
-  for (int n = threadIdx.x; n < kTable; n += kTcThreads) {
+  for (int n = a.by_cost ? kTable : threadIdx.x; n < kTable; n += kTcThreads) {
     const int64_t it = blockIdx.x + static_cast<int64_t>(n) * gridDim.x;
     table[n] = it < a.items ? item_at(a, it) : Item{0, 0, 0, 0};
   }
@@ -348,22 +361,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           break;
         }
         tc_fence_after();
-        if (!every) {  // zeros for the values of keys left out: thread i of the group has key i
-          const uint32_t at = 2 * (g1 + j) + 1, v_slot = at % kSlots;
-          if (!mbar_wait(&full[v_slot], at / kSlots & 1u, abort_flag, err, kDevTimeoutAttn)) {
-            ok = false;
-            break;
-          }
+        if (!every) {  // zeros for the values of keys left out but within the product: warp i has keys [32 i, +32)
           const uint32_t mine = quarter == 0 ? bits[0] : quarter == 1 ? bits[1] : quarter == 2 ? bits[2] : bits[3];
-          if (!(mine >> lane & 1u)) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              uint4* const v = reinterpret_cast<uint4*>(smem + kOffRing + v_slot * kTile + c * kAtom + (quarter * 32 + lane) * 128);
-#pragma unroll
-              for (int i = 0; i < 8; ++i) v[i] = make_uint4(0, 0, 0, 0);
+          const int within = ((left + 15) & ~15) - 32 * quarter;
+          const uint32_t out_of = within <= 0 ? 0u : ~mine & (within >= 32 ? 0xffffffffu : (1u << within) - 1u);
+          if (out_of != 0) {
+            const uint32_t at = 2 * (g1 + j) + 1, v_slot = at % kSlots;
+            if (!mbar_wait(&full[v_slot], at / kSlots & 1u, abort_flag, err, kDevTimeoutAttn)) {
+              ok = false;
+              break;
             }
+            zero_values(smem + kOffRing + v_slot * kTile + quarter * 32 * 128, out_of, lane);
+            fence_async_smem();
           }
-          fence_async_smem();
         }
         if (active) {
           const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
@@ -374,7 +384,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           for (int c = 0; c < 4; ++c) {
             if (c < 3) tmem_ld32(ts + 32 * (c + 1), s[(c + 1) & 1]);
             uint32_t(&sc)[32] = s[c & 1];
-            if (!every) {
+            if (bits[c] != 0xffffffffu) {
 #pragma unroll
               for (int e = 0; e < 32; ++e)
                 if (!(bits[c] >> e & 1u)) sc[e] = 0xff800000u;  // -inf
@@ -534,9 +544,11 @@ int cross_tc(const CrossArgs& p, bool bf16, cudaStream_t s) {
   a.items = slots * p.heads;
   a.err = device_error_word();
   FF_REQUIRE(a.err != nullptr, "ff_cross_attention: no device error word");
-  // Sequences of different lengths: a CTA per item, so that whoever is done takes the next.
+  // Sequences of different lengths: a CTA per item, so that whoever is done takes the next, the longest first (ragged captions
+  // over ragged images: 141 us in the order of the sequences).
   const bool even = p.q_start == nullptr && p.k_start == nullptr && p.k_len == nullptr;
   const int grid = static_cast<int>(std::min<int64_t>(a.items, even ? sm_count() : 0x7fffffff));
+  a.by_cost = !even && p.sequences <= kTcThreads;
   if (p.dim <= 64) return cross_tc64(a, bf16, grid, s);
   return bf16 ? launch_tc<__nv_bfloat16>(a, grid, s) : launch_tc<__half>(a, grid, s);
 }

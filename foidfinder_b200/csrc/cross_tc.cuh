@@ -16,6 +16,7 @@ struct TcArgs {
   CrossArgs p;
   int tiles_per_seq;  // equal pieces: items of 256 queries per sequence and head; 0: by q_start
   int64_t items;
+  bool by_cost;  // an item per CTA, by item_by_cost
   int* err;
 };
 
@@ -77,6 +78,34 @@ static __device__ Item item_at(const TcArgs& a, int64_t it) {
   r.k = k.at;
   r.nk = k.n;
   return r;
+}
+
+// The item of a CTA that has one, or none: sequences in falling order of their keys (half of these for up to 128 queries), so
+// that no long item starts when the others are about to end. By all threads, for at most one sequence each; `cost` has
+// room for all sequences and is left to the asynchronous copies.
+static __device__ Item item_by_cost(const TcArgs& a, int2* cost, Item* found) {
+  const int i = threadIdx.x, n = a.p.sequences;
+  Piece q{0, 0}, k{0, 0};
+  int2 mine = make_int2(0, 0);  // cost, items
+  if (i < n) {
+    q = query_piece(a.p, i);
+    k = key_piece(a.p, i);
+    mine = make_int2(q.n > kBQ ? k.n : (k.n + 1) / 2, (q.n + 255) / 256);
+    cost[i] = mine;
+  }
+  if (i == 0) *found = Item{0, 0, 0, 0};
+  __syncthreads();
+  if (i < n) {
+    int tile = static_cast<int>(blockIdx.x / static_cast<uint32_t>(a.p.heads));
+    for (int j = 0; j < n; ++j) {
+      const int2 other = cost[j];
+      if (other.x > mine.x || (other.x == mine.x && j < i)) tile -= other.y;
+    }
+    if (tile >= 0 && tile < mine.y) *found = Item{q.at + tile * 256, min(256, q.n - tile * 256), k.at, k.n};
+  }
+  fence_async_smem();
+  __syncthreads();
+  return *found;
 }
 
 // O (dim TMEM columns from `to`) scaled by corr; out of line, it is rare.

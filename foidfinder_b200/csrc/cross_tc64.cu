@@ -79,7 +79,8 @@ __global__ void __launch_bounds__(kThreads64, 1)
   int* const err = a.err;
   if (a.items == gridDim.x) {  // one item per CTA, perhaps none
     pdl_wait();
-    if (item_at(a, blockIdx.x).nq == 0) return;
+    const Item only = a.by_cost ? item_by_cost(a, reinterpret_cast<int2*>(smem + kOffRing), table) : item_at(a, blockIdx.x);
+    if (only.nq == 0) return;
   }
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -112,7 +113,7 @@ __global__ void __launch_bounds__(kThreads64, 1)
   }
   pdl_wait();
   pdl_trigger();
-  for (int n = threadIdx.x; n < kTable; n += kThreads64) {
+  for (int n = a.by_cost ? kTable : threadIdx.x; n < kTable; n += kThreads64) {
     const int64_t it = blockIdx.x + static_cast<int64_t>(n) * gridDim.x;
     table[n] = it < a.items ? item_at(a, it) : Item{0, 0, 0, 0};
   }
@@ -323,18 +324,22 @@ __global__ void __launch_bounds__(kThreads64, 1)
           break;
         }
         tc_fence_after();
-        if (!every) {  // zeros for the values of keys left out: two threads of the stream for a key
-          if (!mbar_wait(&full[v_slot], (g / kRing) & 1u, abort_flag, err, kDevTimeoutAttn)) {
-            ok = false;
-            break;
-          }
-          const uint32_t mine = quarter & 1 ? bits[1] : bits[0];
-          if (!(mine >> lane & 1u)) {
-            uint4* const v = reinterpret_cast<uint4*>(smem + kOffRing + v_slot * kSlot + (in_tile & 63) * 128 + (quarter >> 1) * 64);
+        if (!every) {  // zeros for the values of keys left out but within the product: warp i has keys [16 i, +16)
+          const uint32_t mine = (quarter & 2 ? bits[1] : bits[0]) >> (16 * (quarter & 1));
+          const uint32_t out_of = 16 * quarter < left ? ~mine & 0xffffu : 0u;
+          if (out_of != 0) {
+            if (!mbar_wait(&full[v_slot], (g / kRing) & 1u, abort_flag, err, kDevTimeoutAttn)) {
+              ok = false;
+              break;
+            }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < 4; ++i) {
+              const int key = 4 * i + (lane >> 3);  // 8 lanes, 128 bytes: no two on a bank
+              if (out_of >> key & 1u)
+                *reinterpret_cast<uint4*>(smem + kOffRing + v_slot * kSlot + (quarter * 16 + key) * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_async_smem();
           }
-          fence_async_smem();
         }
         if (active) {
           const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
@@ -349,7 +354,7 @@ __global__ void __launch_bounds__(kThreads64, 1)
               uint32_t s[32];
               tmem_ld32(ts + 32 * c, s);
               tmem_ld_wait();
-              if (!every) {
+              if (bits[c] != 0xffffffffu) {
 #pragma unroll
                 for (int e = 0; e < 32; ++e)
                   if (!(bits[c] >> e & 1u)) s[e] = 0xff800000u;  // -inf

@@ -353,6 +353,15 @@ def test_attention_ragged(cuda_device, no_device_error, name, heads, kv_heads, d
             assert (out[qi.cuda()] == 0).all()
 
 
+@pytest.mark.parametrize(("sequences", "dim"), [(320, 64), (321, 64), (320, 80), (321, 80)])
+def test_attention_of_many_sequences_of_many_queries(cuda_device, no_device_error, sequences, dim):
+    """As many sequences as are put in order by their lengths, and one more; equal lengths and none among them."""
+    nq, nk = [(37 * i) % 390 for i in range(sequences)], [(53 * i) % 100 // 8 * 8 for i in range(sequences)]
+    q, k, v = _qkv(sum(nq), sum(nk), 2, 2, dim, F16)
+    out = _attend(q, k, v, heads=2, kv_heads=2, head_dim=dim, q_start=_starts(nq, 0), k_start=_starts(nk, 0))
+    _check_attention(out, q, k, v, heads=2, kv_heads=2, dim=dim, pieces=_pieces(nq, nk))
+
+
 @pytest.mark.parametrize("nq", [1, 20, 150])
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_attention_padded(cuda_device, no_device_error, nq, dtype):
