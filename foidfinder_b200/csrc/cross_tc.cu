@@ -483,8 +483,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             uint32_t w[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) w[e] = Pair16<T>::pack(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
-            *reinterpret_cast<uint4*>(out + c) = make_uint4(w[0], w[1], w[2], w[3]);
-            *reinterpret_cast<uint4*>(out + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+            store_columns(out + c, w);
           }
         }
       }

@@ -120,6 +120,18 @@ static __device__ __noinline__ void rescale(uint32_t to, int dim, float corr) {
   }
 }
 
+// 16 columns of a row of the result. One store of 32 bytes, where they start at one: two of 16 would each write half a sector.
+static __device__ __forceinline__ void store_columns(void* out, const uint32_t (&w)[8]) {
+  if ((reinterpret_cast<uintptr_t>(out) & 31) == 0) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]),
+                 "r"(w[6]), "r"(w[7])
+                 : "memory");
+  } else {
+    static_cast<uint4*>(out)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    static_cast<uint4*>(out)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+}
+
 // Walks the items of a CTA. next(): the next one with queries (and, WORK, with keys).
 struct Items {
   const TcArgs& a;
