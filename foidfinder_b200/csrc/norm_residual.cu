@@ -83,6 +83,7 @@ template <Deal D>
 struct Columns {
   static constexpr int kUnit = D == Deal::kFull ? kChunk : D == Deal::kPairs ? 2 : 1;  // neighbouring columns of a lane
   int cols, first, step;  // of unit 0, and between units
+  Columns() = default;
   __device__ __forceinline__ Columns(int cols, int lane, int lanes) : cols(cols), first(lane * kUnit), step(lanes * kUnit) {}
   __device__ __forceinline__ int at(int k, int e) const { return first + (k * kChunk + e) / kUnit * step + e % kUnit; }
 
@@ -167,73 +168,103 @@ struct Columns {
   }
 };
 
-// Sum over the threads of a row. Sums of several warps go through `part` (a slot of 32 per call).
-template <bool MULTI>
-__device__ __forceinline__ float row_sum(float v, int lanes, float* part) {
-  if constexpr (MULTI) {
-    v = warp_sum(v);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (lane == 0) part[warp] = v;
-    __syncthreads();
-    return warp_sum(lane * 32 < lanes ? part[lane] : 0.f);
-  } else {
+// Sums over the threads of a row, of R rows. Sums of several warps go through `part` (32 R words per call).
+template <bool MULTI, int R>
+__device__ __forceinline__ void row_sums(float (&v)[R], int lanes, float (*part)[32]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
-    for (int o = 16; o; o >>= 1)
-      if (o < lanes) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+  for (int r = 0; r < R; ++r) {
+    if constexpr (MULTI) {
+      v[r] = warp_sum(v[r]);
+      if (lane == 0) part[r][warp] = v[r];
+    } else {
+#pragma unroll
+      for (int o = 16; o; o >>= 1)
+        if (o < lanes) v[r] += __shfl_xor_sync(0xffffffffu, v[r], o);
+    }
+  }
+  if constexpr (MULTI) {
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r) v[r] = warp_sum(lane * 32 < lanes ? part[r][lane] : 0.f);
   }
 }
 
-// v (0 past the row) -> its norm, in place.
-template <Deal D, int K, bool MULTI>
-__device__ __forceinline__ void norm(float2 (&v)[K][4], const Columns<D>& c, int kind, const float* w, const float* b, float eps, int lanes,
+// v (0 past the row) -> its norm, in place, for R rows.
+template <Deal D, int R, int K, bool MULTI>
+__device__ __forceinline__ void norm(float2 (&v)[R][K][4], const Columns<D> (&c)[R], int kind, const float* w, const float* b, float eps, int lanes,
                                      float (*part)[32]) {
-  const float inv = 1.f / static_cast<float>(c.cols);
+  const float inv = 1.f / static_cast<float>(c[0].cols);
+  float sum[R];
   if (kind == FF_NORM_LAYER) {
-    float2 s[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+    for (int r = 0; r < R; ++r) {
+      float2 s[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[e & 1] = add2(s[e & 1], v[k][e]);
-    s[0] = add2(s[0], s[1]);
-    const float mean = row_sum<MULTI>(s[0].x + s[0].y, lanes, part[0]) * inv;
+      for (int k = 0; k < K; ++k)
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+        for (int e = 0; e < 4; ++e) s[e & 1] = add2(s[e & 1], v[r][k][e]);
+      s[0] = add2(s[0], s[1]);
+      sum[r] = s[0].x + s[0].y;
+    }
+    row_sums<MULTI>(sum, lanes, part);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[k][e] = sub2(v[k][e], make_float2(mean, mean));
-    c.trim(v);
+    for (int r = 0; r < R; ++r) {
+      const float mean = sum[r] * inv;
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[r][k][e] = sub2(v[r][k][e], make_float2(mean, mean));
+      c[r].trim(v[r]);
+    }
   }
-  float2 q[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-  for (int k = 0; k < K; ++k)
+  for (int r = 0; r < R; ++r) {
+    float2 q[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) q[e & 1] = fma2(v[k][e], v[k][e], q[e & 1]);
-  q[0] = add2(q[0], q[1]);
-  const float rstd = rsqrtf(row_sum<MULTI>(q[0].x + q[0].y, lanes, part[1]) * inv + eps);
-  const float2 r2 = make_float2(rstd, rstd);
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[e & 1] = fma2(v[r][k][e], v[r][k][e], q[e & 1]);
+    q[0] = add2(q[0], q[1]);
+    sum[r] = q[0].x + q[0].y;
+  }
+  row_sums<MULTI>(sum, lanes, part + R);
+  float2 r2[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const float rstd = rsqrtf(sum[r] * inv + eps);
+    r2[r] = make_float2(rstd, rstd);
+  }
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     float2 wk[4];
     if (w != nullptr) {
-      c.parameters(w, k, wk);
+      c[0].parameters(w, k, wk);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[k][e] = mul2(v[k][e], mul2(wk[e], r2));
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[r][k][e] = mul2(v[r][k][e], mul2(wk[e], r2[r]));
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[k][e] = mul2(v[k][e], r2);
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[r][k][e] = mul2(v[r][k][e], r2[r]);
     }
     if (b != nullptr) {
-      c.parameters(b, k, wk);
+      c[0].parameters(b, k, wk);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[k][e] = add2(v[k][e], wk[e]);
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[r][k][e] = add2(v[r][k][e], wk[e]);
     }
   }
 }
 
 // e^x within a few 2^-24 of itself: 2^t of the rounded t = x log2(e), corrected by what the product and the constant lost.
 __device__ __forceinline__ float exp_close(float x) {
-  const float t = x * 1.44269504f;
-  const float lost = fmaf(x, 1.44269504f, -t) + x * 1.925963033e-8f;  // log2(e) = 1.44269504 + 1.926e-8
+  constexpr float kLog2e = 1.44269504f, kBelow = static_cast<float>(1.4426950408889634 - static_cast<double>(kLog2e));
+  const float t = x * kLog2e;
+  const float lost = fmaf(x, kLog2e, -t) + x * kBelow;
   const float y = ex2_approx(t);
   return fabsf(t) < 126.f ? fmaf(y, lost * 0.693147181f, y) : y;
 }
@@ -261,64 +292,90 @@ __device__ __forceinline__ float activate(float g, int act) {
   return g;
 }
 
-template <class TX, class TY, int K, Deal D, bool MULTI>
-__global__ void __launch_bounds__(MULTI ? (K == 1 ? 1024 : 512) : kNrThreads, MULTI ? 1 : K <= 2 ? 8 : sizeof(TX) == 2 && D == Deal::kFull ? 5 : 4) norm_residual_kernel(const __grid_constant__ NrArgs a) {
-  __shared__ float part[MULTI ? 4 : 1][32];
+// R rows at a time by the same threads, which then read the parameters once for all of them.
+template <class TX, class TY, int R, int K, Deal D, bool MULTI>
+__global__ void __launch_bounds__(MULTI ? (R * K == 1 ? 1024 : 512) : kNrThreads, MULTI ? 1 : R * K <= 2 ? 8 : sizeof(TX) == 2 && D == Deal::kFull ? 5 : 4)
+    norm_residual_kernel(const __grid_constant__ NrArgs a) {
+  __shared__ float part[MULTI ? 4 * R : 1][32];
   const ff_norm_residual_args& p = a.p;
   const int lanes = a.lanes;  // a power of two unless MULTI
   const int in_row = MULTI ? static_cast<int>(threadIdx.x) : static_cast<int>(threadIdx.x) & (lanes - 1);
-  const int row = MULTI ? static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x) * (kNrThreads / lanes) + static_cast<int>(threadIdx.x) / lanes;
+  const int group = MULTI ? static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x) * (kNrThreads / lanes) + static_cast<int>(threadIdx.x) / lanes;
   pdl_wait();
   pdl_trigger();
-  const bool real = MULTI || row < p.rows;  // lanes without a row go along (their warp's others have one), on nothing
-  const int64_t r = real ? row : 0;
-  const TY* const y = static_cast<const TY*>(p.y) + r * p.ldy;
-  const TX* const x = static_cast<const TX*>(p.x) + r * p.ldx;
-  TX* const out = static_cast<TX*>(p.out) + r * p.ldo;
-  Columns<D> c(p.cols, in_row, lanes);
-  if (!real) c.first = p.cols;
-  Raw<TY> raw[K];
-  Raw<TX> xr[K];
+  Columns<D> c[R];
+  int64_t row[R];
 #pragma unroll
-  for (int k = 0; k < K; ++k) c.load(y, k, raw[k]);
+  for (int r = 0; r < R; ++r) {
+    const int64_t n = static_cast<int64_t>(group) * R + r;
+    const bool real = (MULTI && R == 1) || n < p.rows;  // lanes without a row go along, on nothing
+    row[r] = real ? n : 0;
+    c[r] = Columns<D>(p.cols, in_row, lanes);
+    if (!real) c[r].first = p.cols;
+  }
+  Raw<TY> raw[R][K];
+  Raw<TX> xr[R][K];
 #pragma unroll
-  for (int k = 0; k < K; ++k) c.load(x, k, xr[k]);
-  float2 v[K][4];
+  for (int r = 0; r < R; ++r)
 #pragma unroll
-  for (int k = 0; k < K; ++k)
+    for (int k = 0; k < K; ++k) c[r].load(static_cast<const TY*>(p.y) + row[r] * p.ldy, k, raw[r][k]);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[k][e] = raw[k].pair(e);
-  const int64_t gate_at = p.gate != nullptr ? static_cast<int64_t>(static_cast<uint32_t>(r) / static_cast<uint32_t>(p.gate_rows)) * p.ldg : 0;
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int k = 0; k < K; ++k) c[r].load(static_cast<const TX*>(p.x) + row[r] * p.ldx, k, xr[r][k]);
+  float2 v[R][K][4];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[r][k][e] = raw[r][k].pair(e);
+  int64_t gate_at[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    gate_at[r] = p.gate != nullptr ? static_cast<int64_t>(static_cast<uint32_t>(row[r]) / static_cast<uint32_t>(p.gate_rows)) * p.ldg : 0;
   const bool narrow = p.gate != nullptr && p.gate_cols > 1 && p.gate_type != FF_F32;  // a gate of 16 bits per column
   if (narrow || (sizeof(TY) == 4 && p.gate != nullptr && p.gate_cols > 1)) {  // under way during the norm
 #pragma unroll
-    for (int k = 0; k < K; ++k) c.load(static_cast<const TY*>(p.gate) + gate_at, k, raw[k]);
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int k = 0; k < K; ++k) c[r].load(static_cast<const TY*>(p.gate) + gate_at[r], k, raw[r][k]);
   }
-  if (p.post != FF_NORM_NONE) norm<D, K, MULTI>(v, c, p.post, p.post_w, p.post_b, p.post_eps, lanes, part);
+  if (p.post != FF_NORM_NONE) norm<D, R, K, MULTI>(v, c, p.post, p.post_w, p.post_b, p.post_eps, lanes, part);
   if (p.gate != nullptr) {
     if (p.gate_cols == 1) {
-      const float g = activate<true>(p.gate_type == FF_F32 ? static_cast<const float*>(p.gate)[gate_at] : as_f32(static_cast<const TY*>(p.gate)[gate_at]),
-                               p.gate_act);
 #pragma unroll
-      for (int k = 0; k < K; ++k)
+      for (int r = 0; r < R; ++r) {
+        const float g = activate<true>(
+            p.gate_type == FF_F32 ? static_cast<const float*>(p.gate)[gate_at[r]] : as_f32(static_cast<const TY*>(p.gate)[gate_at[r]]), p.gate_act);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[k][e] = mul2(v[k][e], make_float2(g, g));
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[r][k][e] = mul2(v[r][k][e], make_float2(g, g));
+      }
     } else {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         float2 g[4];
-        if (narrow || sizeof(TY) == 4) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) g[e] = raw[k].pair(e);
-        } else {
-          c.parameters(static_cast<const float*>(p.gate) + gate_at, k, g);
+        for (int r = 0; r < R; ++r) {
+          if (narrow || sizeof(TY) == 4) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) g[e] = raw[r][k].pair(e);
+          } else if (r == 0 || gate_at[r] != gate_at[r - 1]) {
+            c[r].parameters(static_cast<const float*>(p.gate) + gate_at[r], k, g);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[r][k][e] = mul2(v[r][k][e], g[e]);
+            continue;
+          }
+          if (p.gate_act != FF_GATE_PLAIN) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) g[e] = make_float2(activate<sizeof(TX) == 4>(g[e].x, p.gate_act), activate<sizeof(TX) == 4>(g[e].y, p.gate_act));
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[r][k][e] = mul2(v[r][k][e], g[e]);
         }
-        if (p.gate_act != FF_GATE_PLAIN) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) g[e] = make_float2(activate<sizeof(TX) == 4>(g[e].x, p.gate_act), activate<sizeof(TX) == 4>(g[e].y, p.gate_act));
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[k][e] = mul2(v[k][e], g[e]);
       }
     }
   }
@@ -326,52 +383,72 @@ __global__ void __launch_bounds__(MULTI ? (K == 1 ? 1024 : 512) : kNrThreads, MU
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       float2 s[4];
-      c.parameters(p.scale, k, s);
+      c[0].parameters(p.scale, k, s);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[k][e] = mul2(v[k][e], s[e]);
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[r][k][e] = mul2(v[r][k][e], s[e]);
     }
   }
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
+  for (int r = 0; r < R; ++r)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[k][e] = fma2(make_float2(p.alpha, p.alpha), xr[k].pair(e), v[k][e]);
-    c.store(out, k, v[k]);
-  }
+    for (int k = 0; k < K; ++k) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[r][k][e] = fma2(make_float2(p.alpha, p.alpha), xr[r][k].pair(e), v[r][k][e]);
+      c[r].store(static_cast<TX*>(p.out) + row[r] * p.ldo, k, v[r][k]);
+    }
   if (p.normed == nullptr) return;
-  c.trim(v);  // statistics, biases, gates and infinities can have left others than 0 there
-  norm<D, K, MULTI>(v, c, p.pre, p.pre_w, p.pre_b, p.pre_eps, lanes, part + (MULTI ? 2 : 0));
-  TY* const normed = static_cast<TY*>(p.normed) + r * p.ldn;
 #pragma unroll
-  for (int k = 0; k < K; ++k) c.store(normed, k, v[k]);
+  for (int r = 0; r < R; ++r) c[r].trim(v[r]);  // statistics, biases, gates and infinities can have left others than 0 there
+  norm<D, R, K, MULTI>(v, c, p.pre, p.pre_w, p.pre_b, p.pre_eps, lanes, part + (MULTI ? 2 * R : 0));
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int k = 0; k < K; ++k) c[r].store(static_cast<TY*>(p.normed) + row[r] * p.ldn, k, v[r][k]);
 }
 
-template <class TX, class TY, int K, Deal D, bool MULTI>
+template <class TX, class TY, int R, int K, Deal D, bool MULTI>
 void launch_nr(const NrArgs& a, cudaStream_t s) {
-  const int rows = a.p.rows, per = kNrThreads / a.lanes;
-  launch(norm_residual_kernel<TX, TY, K, D, MULTI>, dim3(MULTI ? rows : (rows + per - 1) / per), dim3(MULTI ? a.lanes : kNrThreads), 0, s, a);
+  const int rows = (a.p.rows + R - 1) / R, per = kNrThreads / a.lanes;
+  launch(norm_residual_kernel<TX, TY, R, K, D, MULTI>, dim3(MULTI ? rows : (rows + per - 1) / per), dim3(MULTI ? a.lanes : kNrThreads), 0, s, a);
 }
 
 template <class TX, class TY, Deal D>
 void launch_nr_deal(NrArgs& a, int chunks, int wide, cudaStream_t s) {
+  const ff_norm_residual_args& p = a.p;
+  const int lanes = chunks <= 4 ? 4 : chunks <= 8 ? 8 : chunks <= 16 ? 16 : 32;  // of a row within a warp
+  const bool sums = p.post != FF_NORM_NONE || p.normed != nullptr, few = static_cast<int64_t>(p.rows) * wide * lanes <= 512LL * sm_count();
+  int vectors = p.scale != nullptr;
+  for (const float* q : {p.post_w, p.post_b, p.pre_w, p.pre_b}) vectors += q != nullptr;
+  vectors += p.gate != nullptr && p.gate_cols > 1 && p.gate_type == FF_F32 && p.gate_rows > 1;
   if (wide == 1) {
-    a.lanes = chunks <= 4 ? 4 : chunks <= 8 ? 8 : chunks <= 16 ? 16 : 32;
-    return launch_nr<TX, TY, 1, D, false>(a, s);
+    a.lanes = lanes;
+    if constexpr (sizeof(TX) == 2) {
+      if (!few && vectors >= 2) return launch_nr<TX, TY, 2, 1, D, false>(a, s);
+    }
+    return launch_nr<TX, TY, 1, 1, D, false>(a, s);
   }
-  const bool sums = a.p.post != FF_NORM_NONE || a.p.normed != nullptr;
-  if (wide <= 32 && (D == Deal::kSingles || static_cast<int64_t>(a.p.rows) * wide <= 16LL * sm_count())) {
+  if (wide <= 32 && (few || D == Deal::kSingles)) {
     a.lanes = 32 * wide;
-    return launch_nr<TX, TY, 1, D, true>(a, s);
+    return launch_nr<TX, TY, 1, 1, D, true>(a, s);
   }
-  if (wide <= 4 && (wide == 2 || !sums)) {
-    a.lanes = 32;
-    return wide == 2 ? launch_nr<TX, TY, 2, D, false>(a, s) : launch_nr<TX, TY, 4, D, false>(a, s);
-  }
-  if (wide <= 32) {
-    a.lanes = 32 * ((wide + 1) / 2);
-    return launch_nr<TX, TY, 2, D, true>(a, s);
+  if constexpr (D != Deal::kSingles) {
+    if (wide <= 8 && sums && vectors >= 3) {
+      a.lanes = 32 * wide;
+      return launch_nr<TX, TY, 2, 1, D, true>(a, s);
+    }
+    if (wide <= 4 && (wide == 2 || !sums)) {
+      a.lanes = 32;
+      return wide == 2 ? launch_nr<TX, TY, 1, 2, D, false>(a, s) : launch_nr<TX, TY, 1, 4, D, false>(a, s);
+    }
+    if (wide <= 32) {
+      a.lanes = 32 * ((wide + 1) / 2);
+      return launch_nr<TX, TY, 1, 2, D, true>(a, s);
+    }
   }
   a.lanes = 32 * ((wide + 3) / 4);
-  launch_nr<TX, TY, 4, D, true>(a, s);
+  launch_nr<TX, TY, 1, 4, D, true>(a, s);
 }
 
 template <class TX, class TY>
@@ -389,9 +466,12 @@ void launch_nr_types(NrArgs& a, cudaStream_t s) {
   look(p.normed, p.ldn, sizeof(TY), p.rows);
   for (const float* q : {p.post_w, p.post_b, p.pre_w, p.pre_b, p.scale}) look(q, 0, 4, 1);
   if (p.gate != nullptr && p.gate_cols > 1) look(p.gate, p.ldg, p.gate_type == FF_F32 ? 4 : 2, p.rows <= p.gate_rows ? 1 : p.rows);
-  // Lanes and chunks per row. Two chunks per lane (65600 x 1024 bf16 with two norms, gate and scale: 117 us, 146 with four,
-  // 125 with one), but one where rows are few (less than 16 warps per SM even so), for the shortest way through a row, or
-  // columns come one by one (16400 x 2731: 126 us, 151 with two), and four where no sum holds a row together (58 us, 69 with two).
+  // Lanes, chunks and rows per lane. Two chunks of a row (65600 x 1024 bf16 with two RMS norms: 87 us, four chunks of it with gate and
+  // scale 146 against 117), or one chunk of two rows where at least three vectors of parameters are then read once for
+  // both (with gate and scale 117 -> 105 us; without 89), or two where a warp has all of a row of 16 bits (60000 x 256: 26.5 ->
+  // 23.8; f32 24.7 -> 26.6), but not in more than 8 warps (16400 x 2736: 85 -> 102). One chunk of one row where rows are few (less than 16 warps per SM even
+  // so), for the shortest way through a row, or columns come one by one (16400 x 2731: 126 us, 151 with two), and four where no
+  // sum holds a row together (58 us, 69 with two).
   const int chunks = (p.cols + kChunk - 1) / kChunk;
   const int wide = (chunks + 31) / 32;
   if (full)

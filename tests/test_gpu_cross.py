@@ -163,7 +163,7 @@ TYPES = [(F16, F16), (BF16, BF16), (F32, F32), (F32, F16), (F32, BF16)]
 
 @pytest.mark.parametrize(("xt", "yt"), TYPES)
 @pytest.mark.parametrize(("rows", "cols"), [(1, 1), (1, 1024), (3, 7), (5, 257), (130, 768), (4, 2730), (2, 4097), (3, 8192), (2, 16384), (2500, 40), (2400, 1024),
-                                            (2400, 515)])
+                                            (2400, 515), (9601, 40), (3001, 250), (1201, 770), (901, 1000), (701, 2056)])
 def test_block_end(cuda_device, rows, cols, xt, yt):
     x, y, kw = _end_inputs(rows, cols, xt, yt, gate=(3, True, F32))
     _end(x, y, kw | dict(post="rms", pre="layer", gate_act="tanh", alpha=0.875))
