@@ -8,11 +8,18 @@
 // rows of up to 1024 columns (32 values per lane), wider rows are shared by more warps, whose sums meet in shared memory.
 // All sums, statistics and products are f32; each output is rounded once.
 //
-// Three ways to deal out the columns. FULL: 16-byte chunks (8 columns of 16 bits) that divide the rows of every matrix. PAIRS:
-// neighbouring pairs of columns to neighbouring lanes, where all rows and the width are whole pairs; parameters then come
-// in whole 8-byte words, and a warp's pairs still fill cache lines. SINGLES: columns one by one, for any alignment and
-// width. (16-byte words shifted into place took 146-200 us for 16400 x 2730 with a gate: code for each alignment and
-// edge, and waits for the edges.)
+// Measured: 65600 x 1024 bf16, two RMS norms, gate per image and scale (537 MB) 105 us, 5.1 TB/s, and without gate and scale 86 us,
+// 6.2 TB/s; 16400 x 2730 bf16, gate per element 78 us, 4.6 TB/s (2736 columns: 61 us, 5.9 TB/s); 8200 x 768 f32 with a bf16
+// branch, two LayerNorms and a scale 18.2 us, 4.1 TB/s; one row of 1024 3.8 us with its call. What is short of HBM's rate waits:
+// a row's sums need all of it, and its registers are not free for the next before. (Sums of warps merged around their own
+// means, one barrier less: 121 -> 130 us with two LayerNorms, for the instructions more. Persistent CTAs with the
+// parameters in registers: 160.)
+//
+// Four ways to deal out the columns. FULL: 16-byte chunks (8 columns of 16 bits) that divide the rows of every matrix. SHIFTED:
+// the same, where a row is equally far off 16 bytes in every matrix: its chunks begin before it, and the first and last are
+// dealt with by 4-byte words. PAIRS: neighbouring pairs of columns to neighbouring lanes, where all rows and the width are
+// whole pairs; parameters then come in whole 8-byte words, and a warp's pairs still fill cache lines. SINGLES: columns one by
+// one, for any alignment and width.
 #include <algorithm>
 
 #include "common.h"
@@ -26,7 +33,7 @@ constexpr int kChunk = 8;
 constexpr int kNrThreads = 128;    // of a CTA whose warps take rows of their own
 constexpr int kNrMaxCols = 16384;  // 16 warps x 32 lanes x 4 chunks of 8
 
-enum class Deal { kFull, kPairs, kSingles };
+enum class Deal { kFull, kShifted, kPairs, kSingles };
 
 struct NrArgs {
   ff_norm_residual_args p;
@@ -81,17 +88,29 @@ __device__ __forceinline__ float as_f32(float v) { return v; }
 // The columns of one thread: chunk k, value e of its eight.
 template <Deal D>
 struct Columns {
-  static constexpr int kUnit = D == Deal::kFull ? kChunk : D == Deal::kPairs ? 2 : 1;  // neighbouring columns of a lane
+  static constexpr int kUnit = D == Deal::kFull || D == Deal::kShifted ? kChunk : D == Deal::kPairs ? 2 : 1;  // neighbouring columns of a lane
   int cols, first, step;  // of unit 0, and between units
   Columns() = default;
   __device__ __forceinline__ Columns(int cols, int lane, int lanes) : cols(cols), first(lane * kUnit), step(lanes * kUnit) {}
   __device__ __forceinline__ int at(int k, int e) const { return first + (k * kChunk + e) / kUnit * step + e % kUnit; }
+
+  __device__ __forceinline__ bool within(int k, int e) const {
+    return D == Deal::kShifted ? static_cast<uint32_t>(at(k, e)) < static_cast<uint32_t>(cols) : at(k, e) < cols;
+  }
+  __device__ __forceinline__ bool whole(int k) const { return at(k, 0) >= 0 && at(k, kChunk - 1) < cols; }
 
   template <class T>
   __device__ __forceinline__ void load(const T* row, int k, Raw<T>& r) const {
     if constexpr (D == Deal::kFull) {
       r.clear();
       if (at(k, 0) < cols) r.load(row + at(k, 0));
+    } else if constexpr (D == Deal::kShifted) {
+      if (whole(k)) {
+        r.load(row + at(k, 0));
+      } else {
+#pragma unroll
+        for (int e = 0; e < kChunk; e += 2) r.set_word(e / 2, within(k, e) ? *reinterpret_cast<const uint32_t*>(row + at(k, e)) : 0u);
+      }
     } else if constexpr (D == Deal::kPairs) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -121,6 +140,14 @@ struct Columns {
     r.set(v);
     if constexpr (D == Deal::kFull) {
       if (at(k, 0) < cols) r.store(row + at(k, 0));
+    } else if constexpr (D == Deal::kShifted) {
+      if (whole(k)) {
+        r.store(row + at(k, 0));
+      } else {
+#pragma unroll
+        for (int e = 0; e < kChunk; e += 2)
+          if (within(k, e)) *reinterpret_cast<uint32_t*>(row + at(k, e)) = r.word(e / 2);
+      }
     } else if constexpr (D == Deal::kPairs) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -148,6 +175,15 @@ struct Columns {
       v[1] = make_float2(a.z, a.w);
       v[2] = make_float2(b.x, b.y);
       v[3] = make_float2(b.z, b.w);
+    } else if constexpr (D == Deal::kShifted) {
+      if (whole(k) && reinterpret_cast<uintptr_t>(p + at(k, 0)) % 8 == 0) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = __ldg(reinterpret_cast<const float2*>(p + at(k, 2 * e)));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[e] = make_float2(within(k, 2 * e) ? __ldg(p + at(k, 2 * e)) : 0.f, within(k, 2 * e + 1) ? __ldg(p + at(k, 2 * e + 1)) : 0.f);
+      }
     } else {
       Raw<float> r;
       load(p, k, r);
@@ -155,15 +191,15 @@ struct Columns {
       for (int e = 0; e < 4; ++e) v[e] = r.pair(e);
     }
   }
-  // Values past the row to 0.
+  // Values outside the row to 0.
   template <int K>
   __device__ __forceinline__ void trim(float2 (&v)[K][4]) const {
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (at(k, 2 * e) >= cols) v[k][e].x = 0.f;
-        if (at(k, 2 * e + 1) >= cols) v[k][e].y = 0.f;
+        if (!within(k, 2 * e)) v[k][e].x = 0.f;
+        if (!within(k, 2 * e + 1)) v[k][e].y = 0.f;
       }
   }
 };
@@ -311,6 +347,8 @@ __global__ void __launch_bounds__(MULTI ? (R * K == 1 ? 1024 : 512) : kNrThreads
     const bool real = (MULTI && R == 1) || n < p.rows;  // lanes without a row go along, on nothing
     row[r] = real ? n : 0;
     c[r] = Columns<D>(p.cols, in_row, lanes);
+    if constexpr (D == Deal::kShifted)  // the row's columns before its first whole 16 bytes
+      c[r].first -= static_cast<int>(reinterpret_cast<uintptr_t>(static_cast<const TY*>(p.y) + row[r] * p.ldy) % 16 / sizeof(TY));
     if (!real) c[r].first = p.cols;
   }
   Raw<TY> raw[R][K];
@@ -415,28 +453,30 @@ void launch_nr(const NrArgs& a, cudaStream_t s) {
 }
 
 template <class TX, class TY, Deal D>
-void launch_nr_deal(NrArgs& a, int chunks, int wide, cudaStream_t s) {
+void launch_nr_deal(NrArgs& a, int vectors, int chunks, cudaStream_t s) {
+  const int wide = (chunks + 31) / 32;  // warps with a chunk per lane
   const ff_norm_residual_args& p = a.p;
   const int lanes = chunks <= 4 ? 4 : chunks <= 8 ? 8 : chunks <= 16 ? 16 : 32;  // of a row within a warp
   const bool sums = p.post != FF_NORM_NONE || p.normed != nullptr, few = static_cast<int64_t>(p.rows) * wide * lanes <= 512LL * sm_count();
-  int vectors = p.scale != nullptr;
-  for (const float* q : {p.post_w, p.post_b, p.pre_w, p.pre_b}) vectors += q != nullptr;
-  vectors += p.gate != nullptr && p.gate_cols > 1 && p.gate_type == FF_F32 && p.gate_rows > 1;
-  if (wide == 1) {
-    a.lanes = lanes;
-    if constexpr (sizeof(TX) == 2) {
-      if (!few && vectors >= 2) return launch_nr<TX, TY, 2, 1, D, false>(a, s);
+  if constexpr (D != Deal::kShifted) {
+    if (wide == 1) {
+      a.lanes = lanes;
+      if constexpr (sizeof(TX) == 2) {
+        if (!few && vectors >= 2) return launch_nr<TX, TY, 2, 1, D, false>(a, s);
+      }
+      return launch_nr<TX, TY, 1, 1, D, false>(a, s);
     }
-    return launch_nr<TX, TY, 1, 1, D, false>(a, s);
   }
   if (wide <= 32 && (few || D == Deal::kSingles)) {
     a.lanes = 32 * wide;
     return launch_nr<TX, TY, 1, 1, D, true>(a, s);
   }
   if constexpr (D != Deal::kSingles) {
-    if (wide <= 8 && sums && vectors >= 3) {
-      a.lanes = 32 * wide;
-      return launch_nr<TX, TY, 2, 1, D, true>(a, s);
+    if constexpr (D != Deal::kShifted) {
+      if (wide <= 8 && sums && vectors >= 3) {
+        a.lanes = 32 * wide;
+        return launch_nr<TX, TY, 2, 1, D, true>(a, s);
+      }
     }
     if (wide <= 4 && (wide == 2 || !sums)) {
       a.lanes = 32;
@@ -472,14 +512,36 @@ void launch_nr_types(NrArgs& a, cudaStream_t s) {
   // 23.8; f32 24.7 -> 26.6), but not in more than 8 warps (16400 x 2736: 85 -> 102). One chunk of one row where rows are few (less than 16 warps per SM even
   // so), for the shortest way through a row, or columns come one by one (16400 x 2731: 126 us, 151 with two), and four where no
   // sum holds a row together (58 us, 69 with two).
+  int vectors = p.scale != nullptr;  // of parameters
+  for (const float* q : {p.post_w, p.post_b, p.pre_w, p.pre_b}) vectors += q != nullptr;
+  vectors += p.gate != nullptr && p.gate_cols > 1 && p.gate_type == FF_F32 && p.gate_rows > 1;
   const int chunks = (p.cols + kChunk - 1) / kChunk;
-  const int wide = (chunks + 31) / 32;
-  if (full)
-    launch_nr_deal<TX, TY, Deal::kFull>(a, chunks, wide, s);
-  else if (pairs)
-    launch_nr_deal<TX, TY, Deal::kPairs>(a, chunks, wide, s);
+  if (full) return launch_nr_deal<TX, TY, Deal::kFull>(a, vectors, chunks, s);
+  // SHIFTED: for 16 bits, rows that a warp has not all of, and either one vector of parameters (these are off their 16 bytes; 16400 x
+  // 770, gate per element: 32 -> 26 us, but 35 -> 38 at 902 columns with three) or more than 2048 columns (2050 with three:
+  // 102 -> 84, 2730 with a gate per element 98 -> 78). f32: 16400 x 1030 57, and 66 so.
+  if constexpr (sizeof(TX) == 2 && sizeof(TY) == 2) {
+    bool alike = p.cols % 2 == 0;
+    auto like_y = [&](const void* q, int64_t ld) {  // every row as far off 16 bytes as y's
+      const uint64_t from = reinterpret_cast<uintptr_t>(q), y = reinterpret_cast<uintptr_t>(p.y);
+      alike = alike && from % 4 == 0 && from % 16 == y % 16 && (p.rows == 1 || (2 * ld % 4 == 0 && 2 * ld % 16 == 2 * p.ldy % 16));
+    };
+    like_y(p.y, p.ldy);
+    like_y(p.x, p.ldx);
+    like_y(p.out, p.ldo);
+    if (p.normed != nullptr) like_y(p.normed, p.ldn);
+    if (p.gate != nullptr && p.gate_cols > 1 && p.gate_type != FF_F32) {
+      alike = alike && (p.gate_rows == 1 || p.rows == 1);
+      like_y(p.gate, p.ldg);
+    }
+    const int shifted = (p.cols + 2 * kChunk - 2) / kChunk;  // the first can begin before the row
+    if (alike && shifted <= kNrMaxCols / kChunk && chunks > 32 && (vectors <= 1 || chunks > 256))
+      return launch_nr_deal<TX, TY, Deal::kShifted>(a, vectors, shifted, s);
+  }
+  if (pairs)
+    launch_nr_deal<TX, TY, Deal::kPairs>(a, vectors, chunks, s);
   else
-    launch_nr_deal<TX, TY, Deal::kSingles>(a, chunks, wide, s);
+    launch_nr_deal<TX, TY, Deal::kSingles>(a, vectors, chunks, s);
 }
 
 }  // namespace

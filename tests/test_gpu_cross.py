@@ -212,6 +212,30 @@ def test_block_end_rows_off_a_chunk(cuda_device, xt, yt, cols):
                     assert (t[:, beside] == 9).all()
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize(("rows", "cols", "plain"), [(21, 258, True), (700, 518, True), (900, 770, True), (130, 2050, False), (400, 2730, True), (9, 6002, False),
+                                                     (3, 16370, False), (3, 16384, False)])
+def test_block_end_rows_equally_off_16_bytes(cuda_device, rows, cols, plain, dtype):
+    """Rows of every matrix, the gate's among them, begin equally far off 16 bytes, each row differently; with few parameters and
+    many; nothing beside the rows is written, and what is there (NaN) does not count."""
+    x, y, kw = _end_inputs(rows, cols, dtype, dtype, gate=(1, True, dtype), scale=not plain)
+    kw |= dict(post="layer", gate_act="sigmoid") | (dict(post_weight=None, post_bias=None, pre_weight=None, pre_bias=None) if plain else dict(pre="rms"))
+    want, err, n, n_err = O.block_end(x, y, **kw)
+    for pitch, offset in ((cols + 8, 2), (cols + 10, 6), (cols + 12, 1), (cols + 14, 0)):
+        at = slice(offset, offset + cols)
+        dx, dy, gate = (torch.full((rows, pitch), math.nan, dtype=dtype, device="cuda") for _ in range(3))
+        out, normed = (torch.full((rows, pitch), 9.0, dtype=dtype, device="cuda") for _ in range(2))
+        dx[:, at], dy[:, at], gate[:, at] = x.cuda(), y.cuda(), kw["gate"].cuda()
+        on_device = {k: v.cuda() if torch.is_tensor(v) else v for k, v in kw.items()} | dict(gate=gate[:, at])
+        ops.norm_residual(dx[:, at], dy[:, at], out[:, at], normed=None if plain else normed[:, at], **on_device)
+        _close(out[:, at], want, err, dtype)
+        if not plain:
+            _close(normed[:, at], n, n_err, dtype)
+        beside = torch.ones(pitch, dtype=torch.bool, device="cuda")
+        beside[at] = False
+        assert (out[:, beside] == 9).all() and (normed[:, beside] == 9).all()
+
+
 @pytest.mark.parametrize("cols", [1024, 99, 5000])
 def test_block_end_in_place(cuda_device, cols):
     x, y, kw = _end_inputs(300, cols, BF16, BF16)
