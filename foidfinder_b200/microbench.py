@@ -8,6 +8,8 @@ stream after warm-up. Also the entry point for ncu captures of single kernels.
     python -m foidfinder_b200.microbench peak      (measured dense int8 tensor-core TOPS)
     python -m foidfinder_b200.microbench fp4 [--batch 64] [--format nv|mx] [--iters 20]
                                               (one EVA02-L block on 4-bit operands, and its parts)
+    python -m foidfinder_b200.microbench cross [--batch 64] [--queries 32] [--iters 20]
+                                              (the operators with which other tokens read EVA02-L's)
 
 PixAI-1008 shapes: `attention --batch 144 --seq 576` (16 images x 9 windows), `attention --batch 16 --seq
 5184` (global blocks), `rotate --batch 16 --tokens 5184 --cols 1024 --cols 4864`.
@@ -141,9 +143,36 @@ def bench_fp4(batch: int, iters: int, fmt: str) -> None:
         print(json.dumps({"kernel": "fp4", "part": name, "format": fmt, "M": M, "ms": _time(fn, iters)}))
 
 
+def bench_cross(batch: int, iters: int, queries: int) -> None:
+    """What a block takes in which `queries` tokens per image read the image's (EVA02-L's tokens, heads and width): rotation of
+    its queries and of the image's keys, attention, its end with the next norm."""
+    from .config import EVA02_L
+
+    d = torch.device("cuda")
+    cfg = EVA02_L
+    tokens, heads, dim, width = cfg.tokens, cfg.heads, cfg.dim // cfg.heads, cfg.dim
+    q, k, v = (torch.randn(batch * n, width, device=d).half() for n in (queries, tokens, tokens))
+    x, y, out, normed = (torch.empty_like(q).copy_(q) for _ in range(4))
+    rotated = torch.empty_like(k)
+    f = ops.rope_frequencies(dim)[0].to(d)
+    at_q, at_k = (torch.arange(n, device=d, dtype=torch.int32).repeat(batch) for n in (queries, tokens))
+    gate, weight = torch.zeros(1, 1, device=d), torch.ones(width, device=d)
+    parts = {
+        "rope of the queries": (lambda: ops.rope(q, x, at_q, f, heads=heads, head_dim=dim), 4 * q.numel()),
+        "rope of the keys": (lambda: ops.rope(k, rotated, at_k, f, heads=heads, head_dim=dim), 4 * k.numel()),
+        "cross_attention": (lambda: ops.cross_attention(q, k, v, out, heads=heads, head_dim=dim, sequences=batch), 4 * (q.numel() + k.numel())),
+        "norm_residual": (lambda: ops.norm_residual(x, y, out, gate=gate, gate_act="tanh", gate_rows=batch * queries, normed=normed, pre="layer",
+                                                    pre_weight=weight, pre_bias=weight), 8 * q.numel()),
+    }
+    for name, (fn, nbytes) in parts.items():
+        ms = _time(fn, iters)
+        print(json.dumps({"kernel": "cross", "part": name, "queries": queries, "batch": batch, "ms": ms, "gbs": nbytes / ms / 1e6,
+                          **({"tflops": 4 * batch * queries * tokens * width / ms / 1e9} if name == "cross_attention" else {})}))
+
+
 def main() -> None:
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
-    ap.add_argument("kernel", choices=("gemm", "attention", "rotate", "peak", "fp4"))
+    ap.add_argument("kernel", choices=("gemm", "attention", "rotate", "peak", "fp4", "cross"))
     ap.add_argument("--batch", type=int, default=64)
     ap.add_argument("--iters", type=int, default=20)
     ap.add_argument("--shape", action="append", choices=sorted(GEMM_SHAPES))
@@ -153,9 +182,12 @@ def main() -> None:
     ap.add_argument("--tokens", type=int, default=TOKENS, help="rotate: rows per image")
     ap.add_argument("--cols", type=int, action="append", choices=sorted(ROT_CASES), help="rotate: row widths")
     ap.add_argument("--format", default="nv", choices=("nv", "mx"), help="fp4: operand format")
+    ap.add_argument("--queries", type=int, default=32, help="cross: tokens that read each image's")
     a = ap.parse_args()
     if a.kernel == "fp4":
         bench_fp4(a.batch, a.iters, a.format)
+    elif a.kernel == "cross":
+        bench_cross(a.batch, a.iters, a.queries)
     elif a.kernel == "peak":
         for _ in range(3):
             print(json.dumps({"kernel": "int8_mma_peak", "tops": ops.int8_mma_peak()}))

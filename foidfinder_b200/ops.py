@@ -742,7 +742,7 @@ def norm_residual(
     out before it is rounded). x and out [T, C] are the residual stream (out may be x), y the block's result; normed, y's
     type, may be y. `post` and `pre`: None, "rms" or "layer" with weights and biases [C] (f32, or None). `gate` [G, C] or [G, 1],
     f32 or y's type, after `gate_act` None, "sigmoid" or "tanh"; row t reads gate row t // gate_rows. `scale` [C] f32. Types: fp16,
-    bf16 or f32 alike, or x and out in f32 with a 16-bit y. Rows that start 16 bytes apart are the fastest."""
+    bf16 or f32 alike, or x and out in f32 with a 16-bit y; C is at most 16384. Rows that start 16 bytes apart are the fastest."""
     what = "norm_residual"
     rc = _calls().norm_residual(x, y, out, normed, alpha, _KINDS.get(post), post_weight, post_bias, gate, _GATES.get(gate_act), gate_rows, scale, _KINDS.get(pre),
                                 pre_weight, pre_bias, eps, eps if pre_eps is None else pre_eps)

@@ -646,3 +646,10 @@ def test_the_short_and_the_long_way_into_these_calls_agree(cuda_device, no_devic
     monkeypatch.setattr(ops, "_calls", lambda: ops._NoCalls)
     for u, w in zip(a, everything()):
         assert torch.equal(u, w)
+
+
+def test_microbench_cross(cuda_device, no_device_error, capsys):
+    from foidfinder_b200 import microbench
+
+    microbench.bench_cross(1, 1, 3)
+    assert len(capsys.readouterr().out.splitlines()) == 4
