@@ -551,7 +551,7 @@ int cross_tc(const CrossArgs& p, bool bf16, cudaStream_t s) {
   // over ragged images: 141 -> 102 us).
   const bool even = p.q_start == nullptr && p.k_start == nullptr && p.k_len == nullptr;
   const int grid = static_cast<int>(std::min<int64_t>(a.items, even ? sm_count() : 0x7fffffff));
-  a.by_cost = !even && p.sequences <= kTcThreads;
+  a.by_cost = !even && grid == a.items && p.sequences <= kTcThreads;
   if (p.dim <= 64) return cross_tc64(a, bf16, grid, s);
   return bf16 ? launch_tc<__nv_bfloat16>(a, grid, s) : launch_tc<__half>(a, grid, s);
 }

@@ -648,6 +648,24 @@ def test_the_short_and_the_long_way_into_these_calls_agree(cuda_device, no_devic
         assert torch.equal(u, w)
 
 
+def test_rows_beyond_32_bits(cuda_device):
+    """Rows that start more than 2^32 columns behind the first: rotation and block end."""
+    pitch, rows = (1 << 30) + 8, 6
+    x = _randn(rows, 256, seed=3, dtype=F16)
+    whole = torch.empty(rows * pitch, dtype=F16, device="cuda")
+    far = whole.as_strided((rows, 256), (pitch, 1))
+    far.copy_(x)
+    positions, f = torch.arange(rows, dtype=torch.int32) * 100, ops.rope_frequencies(64)[0]
+    want, size, _ = O.rope(x, positions, f, heads=4, head_dim=64, start=0, pairing="halves", scale=1.0)
+    ops.rope(far, far, positions.cuda(), f.cuda(), heads=4, head_dim=64, pairing="halves")
+    _close(far, want, size * 2.0**-21, F16)
+    _, y, kw = _end_inputs(rows, 256, F16, F16)
+    far.copy_(x)
+    _end(x, y, kw | dict(post="rms"), dx=far, out=far)
+    del far, whole
+    torch.cuda.empty_cache()
+
+
 def test_microbench_cross(cuda_device, no_device_error, capsys):
     from foidfinder_b200 import microbench
 
