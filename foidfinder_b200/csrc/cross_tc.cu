@@ -414,6 +414,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const bool grown = mx > kUp + kGrowth || (!set && mx > -INFINITY);
             if (__any_sync(0xffffffffu, grown)) {
               if (c < 3) tmem_ld_wait();  // nothing on its way into registers across the calls
+              tmem_st_wait();  // what the calls read back (P of the chunks before, O after an earlier growth) has been written
               float corr = 1.f;
               if (grown) {
                 const float now = kUp - (mx - shift);
