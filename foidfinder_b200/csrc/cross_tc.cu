@@ -17,7 +17,7 @@
 //              way meanwhile, P = 2^(s - m + 7) in 16 bits, the sum of P in f32 before that rounding. m is the
 //              maximum at some earlier time: the exponentials start at once, and the new maximum is found beside them.
 //              Only where it has grown by more than 2^8 (P could pass 2^15, fp16's range) do m, O, the sum and the P so
-//              far get rescaled and the 32 exponentials repeated.
+//              far get rescaled, by a whole power of two, and the 32 exponentials repeated.
 // Keys that take no part (past the sequence's end, or masked) get P = 0, and their rows of the value tile are overwritten
 // with zeros in shared memory before the product, so that nothing they hold (NaN, infinities) counts. Both groups of
 // softmax warps write the same zeros, each before it lets its own product start.
@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       };
       if (mask != nullptr) fetch(first);
-      float shift = 0.f;  // 7 - m, once there is an m
+      float shift = 0.f;  // 7 - m, once there is an m: a whole number
       bool set = false;
       float2 sum = make_float2(0.f, 0.f);
       for (int j = first; j < nkv; j += stride, ++tiles) {
@@ -417,9 +417,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               tmem_st_wait();  // what the calls read back (P of the chunks before, O after an earlier growth) has been written
               float corr = 1.f;
               if (grown) {
-                const float now = kUp - (mx - shift);
-                corr = set ? ex2_approx(now - shift) : 0.f;  // without an m there was no key, and all is zero
-                shift = now;
+                const float up = floorf(mx - kUp);  // whole powers of two: the P so far are scaled without a second rounding
+                corr = set ? power_below(up) : 0.f;  // without an m there was no key, and all is zero
+                shift -= up;
                 set = true;
               }
               if (j > first) rescale(to, dim, corr);

@@ -108,6 +108,9 @@ static __device__ Item item_by_cost(const TcArgs& a, int2* cost, Item* found) {
   return *found;
 }
 
+// 2^-n of a whole n >= 0, exactly (0 where f32 has no normal number for it).
+__device__ __forceinline__ float power_below(float n) { return n < 127.f ? __uint_as_float(static_cast<uint32_t>(127 - static_cast<int>(n)) << 23) : 0.f; }
+
 // O (dim TMEM columns from `to`) scaled by corr; out of line, it is rare.
 static __device__ __noinline__ void rescale(uint32_t to, int dim, float corr) {
   for (int c = 0; c < dim; c += 16) {

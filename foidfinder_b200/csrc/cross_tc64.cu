@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(kThreads64, 1)
         }
       };
       if (mask != nullptr) fetch(phase);
-      float shift = 0.f;  // 7 - m, once there is an m
+      float shift = 0.f;  // 7 - m, once there is an m: a whole number
       bool set = false;
       float2 sum = make_float2(0.f, 0.f);
       for (int t = phase; t < steps; t += ways, ++count) {
@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(kThreads64, 1)
                 for (int e = 0; e < 32; e += 2) top[(e >> 1) & 1] = max3(top[(e >> 1) & 1], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
                 top[0] = fmaxf(top[0], top[1]);
                 set = top[0] > -INFINITY;
-                if (set) shift = kUp - top[0] * p.scale_log2;
+                if (set) shift = kUp - floorf(top[0] * p.scale_log2);
               }
               const float2 sh2 = make_float2(shift, shift);
               float2 x[16];
@@ -384,9 +384,9 @@ __global__ void __launch_bounds__(kThreads64, 1)
                 if (once && __any_sync(0xffffffffu, grown)) {
                   float corr = 1.f;
                   if (grown) {
-                    const float now = kUp - (top - shift);
-                    corr = set ? ex2_approx(now - shift) : 0.f;  // without an m there was no key, and all is zero
-                    shift = now;
+                    const float up = floorf(top - kUp);
+                    corr = set ? power_below(up) : 0.f;  // without an m there was no key, and all is zero
+                    shift -= up;
                     set = true;
                   }
                   if (t >= ways) rescale(to, dim, corr);

@@ -80,3 +80,28 @@ def test_maxima_that_grow(no_device_error, kernels_of, steps, dim, sequences, nq
     (out, names) = kernels_of(lambda: _attend(q, k, v, heads=heads, head_dim=dim, sequences=sequences, scale=1.0))
     _ran(names, _kernel(dim))
     _check_attention(out, q, k, v, heads=heads, kv_heads=heads, dim=dim, pieces=_pieces([nq] * sequences, [nk] * sequences), scale=1.0)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_weights_are_rounded_once(no_device_error, kernels_of, dim, dtype):
+    """Three keys take part, in three stretches of 32: one that sets the maximum, one near it, whose value alone is not zero, and
+    one far above both. The result is the second key's weight: rounded to 16 bits when it is stored, and once more in the
+    output, and not when the third key scales it down."""
+    sequences, heads, nq, nk = 16, 8, 300, 128
+    q, k, v = _qkv(sequences * nq, sequences * nk, heads, heads, dim, dtype, seed=11)
+    q[:], k[:], v[:] = 0, 0, 0
+    for h in range(heads):
+        q[:, h * dim] = 1.0
+        q[:, h * dim + 1 : h * dim + 3] = torch.rand(sequences * nq, 2, generator=torch.Generator().manual_seed(h)).to(dtype)
+        for b in range(sequences):
+            k[b * nk + 32, h * dim + 1] = 2.0  # between 0 and 2
+            k[b * nk + 64, h * dim], k[b * nk + 64, h * dim + 2] = 8.0, 2.0  # between 8 and 10: at least 8 powers of two above
+    v[32::nk] = 1 + torch.rand(sequences, heads * dim, generator=torch.Generator().manual_seed(1)).to(dtype)
+    mask = torch.zeros(sequences * nk, dtype=torch.bool)
+    for i in (0, 32, 64):
+        mask[i::nk] = True
+    at = [nk * i for i in range(sequences)]
+    (out, names) = kernels_of(lambda: _attend(q, k, v, heads=heads, head_dim=dim, sequences=sequences, scale=1.0, mask=mask))
+    _ran(names, _kernel(dim))
+    _check_attention(out, q, k, v, heads=heads, kv_heads=heads, dim=dim, pieces=_pieces([nq] * sequences, [nk] * sequences, mask, at), scale=1.0)
