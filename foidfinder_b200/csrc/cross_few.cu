@@ -15,7 +15,7 @@
 // the warps' chains of products and exponentials; one query 50.5 us, 5.3 TB/s; one query over 24600 keys of 4 sequences, 16
 // heads over 4 of 128: 39 us, 5.2 TB/s; one query over 1025 keys of one image 7.5 us, over 32800 keys of one head of 128 15.4.
 //
-// P is rounded to 16 bits for its product with V, as 2^(x - max + 14) in fp16, where it would else lose bits below 2^-14;
+// P is rounded to 16 bits for its product with V, as 2^((s - max) scale + 14) in fp16, where it would else lose bits below 2^-14;
 // sums are taken before that rounding, in f32.
 #include <algorithm>
 
@@ -86,15 +86,17 @@ __device__ __forceinline__ float2 read_cluster2(uint32_t addr) {
   asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
   return v;
 }
-// Weight of a part whose maximum is m beside the largest one, top. (Both -inf: nothing but NaN can be there.)
-__device__ __forceinline__ float part_weight(float m, float top) { return m == -INFINITY && top == -INFINITY ? 1.f : ex2_approx(m - top); }
+// Weight of a part whose largest score is m beside the largest of all, top. (Both -inf: nothing but NaN can be there.)
+__device__ __forceinline__ float part_weight(float m, float top, float scale_log2) {
+  return m == -INFINITY && top == -INFINITY ? 1.f : ex2_approx((m - top) * scale_log2);
+}
 
 struct FewArgs {
   CrossArgs p;
   int passes, splits;
   bool cluster;    // the splits of a sequence are a cluster
   float* part_o;   // [splits][q_rows * heads][dim]
-  float2* part_ml;  // [splits][q_rows * heads]: maximum (in powers of two) and sum
+  float2* part_ml;  // [splits][q_rows * heads]: largest score and sum
 };
 
 // SHORT: sequences of about a tile of keys, whose products leave out groups of 16 keys that there are not.
@@ -230,7 +232,7 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(ATOMS)) cross_few_kernel
           mma16816<T>(s[2 * n + 1], qf[k], f[2], f[3]);
         }
       }
-      // Scores in powers of two; keys that do not take part are -inf (also where their products are NaN).
+      // Keys that do not take part are -inf (also where their products are NaN).
       const uint64_t all = KW == 64 ? ~0ull : (1ull << (KW & 63)) - 1;
       float mx[2] = {-INFINITY, -INFINITY};
       if ((bits & all) != all) {
@@ -244,22 +246,22 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(ATOMS)) cross_few_kernel
       for (int n = 0; n < KW / 8; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
-      float base_m[2];
+      float ref[2];  // subtracted from the scores themselves, however large: times scale their difference would be lost
       bool grew = false;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
         mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-        const float now = fmaxf(m[h], mx[h] * p.scale_log2);
+        const float now = fmaxf(m[h], mx[h]);
         grew |= now > m[h];
         mx[h] = m[h];  // the old one
         m[h] = now;
-        base_m[h] = now == -INFINITY ? 0.f : now;
+        ref[h] = now == -INFINITY ? 0.f : now;
       }
       if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float corr = ex2_approx(mx[h] - base_m[h]);
+          const float corr = ex2_approx((mx[h] - ref[h]) * p.scale_log2);
           l[h] *= corr;
 #pragma unroll
           for (int n = 0; n < 2 * STEPS; ++n) {
@@ -272,9 +274,13 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(ATOMS)) cross_few_kernel
       for (int n = 0; n < KW / 8; ++n) {
         if (SHORT && n >= 2 * groups) break;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[n][e] = ex2_approx(fmaf(s[n][e], p.scale_log2, kShift - base_m[e >> 1]));
-          l[e >> 1] += s[n][e];
+        for (int h = 0; h < 2; ++h) {
+          const float2 x = fma2(sub2(make_float2(s[n][2 * h], s[n][2 * h + 1]), make_float2(ref[h], ref[h])), make_float2(p.scale_log2, p.scale_log2),
+                                make_float2(kShift, kShift));
+          s[n][2 * h] = ex2_approx(x.x);
+          s[n][2 * h + 1] = ex2_approx(x.y);
+          l[h] += s[n][2 * h];
+          l[h] += s[n][2 * h + 1];
         }
       }
 #pragma unroll
@@ -321,7 +327,7 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(ATOMS)) cross_few_kernel
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int g = 0; g < KG; ++g) {
-        const float w = part_weight(part_m[g][r], top);
+        const float w = part_weight(part_m[g][r], top, p.scale_log2);
         const float4 v = *reinterpret_cast<const float4*>(parts + (g * ROWS + r) * dim + c);
         sum = fmaf(part_l[g][r], w, sum);
         acc.x = fmaf(v.x, w, acc.x);
@@ -367,7 +373,7 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(ATOMS)) cross_few_kernel
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int g = 0; g < kCluster; ++g) {
-          const float w = part_weight(ml[g].x, top);
+          const float w = part_weight(ml[g].x, top, p.scale_log2);
           sum = fmaf(ml[g].y, w, sum);
           acc.x = fmaf(v[g].x, w, acc.x);
           acc.y = fmaf(v[g].y, w, acc.y);
@@ -408,7 +414,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) cross_join_kernel(const __gri
 #pragma unroll 4
   for (int i = warp; i < a.splits; i += kJoinWarps) {
     const float2 ml = a.part_ml[i * rows + at];
-    const float w = part_weight(ml.x, top);
+    const float w = part_weight(ml.x, top, p.scale_log2);
     sum = fmaf(ml.y, w, sum);
     if (c < p.dim) {
       const float4 v = *reinterpret_cast<const float4*>(a.part_o + (i * rows + at) * p.dim + c);

@@ -39,8 +39,8 @@ constexpr int kTcThreads = 320;
 constexpr int kSlots = 5;          // of the ring
 constexpr int kTile = 2 * kAtom;   // 128 rows of 128 columns
 constexpr int kOffRing = 2 * kTile;
-constexpr int kOffJoin = kOffRing + kSlots * kTile;  // [128 rows] (shift, sum) of stream 1
-constexpr int kOffTable = kOffJoin + 128 * 8;
+constexpr int kOffJoin = kOffRing + kSlots * kTile;  // [3][128 rows]: ref, shift and sum of stream 1
+constexpr int kOffTable = kOffJoin + 3 * 128 * 4;
 constexpr int kOffBars = kOffTable + kTable * static_cast<int>(sizeof(Item));
 constexpr int kTcSmem = 1024 + kOffBars + 256;
 static_assert(kTcSmem <= 232448, "shared memory of a CTA");
@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int g = (warp - 2) >> 2, quarter = warp & 3;
     const uint32_t ts = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + t_s(g);
     const uint32_t to = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + t_o(g);
-    float2* const join = reinterpret_cast<float2*>(smem + kOffJoin) + quarter * 32 + lane;
+    float* const join = reinterpret_cast<float*>(smem + kOffJoin) + quarter * 32 + lane;
     bool ok = true;
     uint32_t g0 = 0, tiles = 0, worked = 0, splits = 0, freed = 0;  // key tiles of the items before; of this stream, and its items; split ones, and waited for
     Item item;
@@ -342,8 +342,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       };
       if (mask != nullptr) fetch(first);
-      float shift = 0.f;  // 7 - m, once there is an m: a whole number
-      bool set = false;
+      Maximum m{0.f, 0.f, false};
+      float use = 0.f;  // m.shift, or such a one that all scores seem to have grown
       float2 sum = make_float2(0.f, 0.f);
       for (int j = first; j < nkv; j += stride, ++tiles) {
         const int left = item.nk - j * kBK;
@@ -393,9 +393,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               for (int e = 0; e < 32; ++e)
                 if (!(bits[c] >> e & 1u)) sc[e] = 0xff800000u;  // -inf
             }
+            if (c == 0 && j == first) {  // a first maximum
+              const float at = largest(sc) * p.scale_log2;
+              m.set = fabsf(at) < kFarScore;  // else below
+              if (m.set) use = m.shift = kUp - floorf(at);
+            }
             uint32_t pk[16];
             float2 part;
-            auto exponentials = [&]() -> float {  // -> the largest exponent
+            auto exponentials = [&](float shift) -> float {  // -> the largest exponent
               const float2 sh2 = make_float2(shift, shift);
               float mx[2] = {-INFINITY, -INFINITY};
               float2 ps[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -410,23 +415,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               part = add2(ps[0], ps[1]);
               return fmaxf(mx[0], mx[1]);
             };
-            const float mx = exponentials();
-            const bool grown = mx > kUp + kGrowth || (!set && mx > -INFINITY);
+            const float mx = exponentials(use);
+            const bool grown = mx > kUp + kGrowth || (!m.set && bits[c] != 0);
             if (__any_sync(0xffffffffu, grown)) {
               if (c < 3) tmem_ld_wait();  // nothing on its way into registers across the calls
               tmem_st_wait();  // what the calls read back (P of the chunks before, O after an earlier growth) has been written
-              float corr = 1.f;
-              if (grown) {
-                const float up = floorf(mx - kUp);  // whole powers of two: the P so far are scaled without a second rounding
-                corr = set ? power_below(up) : 0.f;  // without an m there was no key, and all is zero
-                shift -= up;
-                set = true;
+              const float top = largest(sc);
+              const float corr = m.below(top, p.scale_log2) ? raise(m, top, p.scale_log2) : 1.f;
+              use = m.ref != 0.f ? 3e38f : m.shift;
+              if (__any_sync(0xffffffffu, m.ref != 0.f)) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) sc[e] = __float_as_uint(__uint_as_float(sc[e]) - m.ref);
               }
               if (j > first) rescale(to, dim, corr);
               if (c > 0) rescale_p<T>(ts, c, corr);
               sum.x *= corr;
               sum.y *= corr;
-              exponentials();
+              exponentials(m.shift);
             }
             sum = add2(sum, part);
             tmem_st16(ts + 16 * c, pk);
@@ -452,7 +457,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       float l = sum.x + sum.y, mine = 1.f, other = 0.f;  // what both streams' outputs count
       if (split) {  // a stream's O is 2^shift times what it stands for; stream 0 writes the result
         if (g == 1) {
-          *join = make_float2(set ? shift : INFINITY, l);
+          join[0] = m.ref;
+          join[128] = m.set ? m.shift : INFINITY;
+          join[256] = l;
           __syncwarp();
           if (lane == 0) mbar_arrive(joined);
           ++splits;
@@ -461,11 +468,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (!mbar_wait(joined, splits & 1u, abort_flag, err, kDevTimeoutAttn)) break;
         ++splits;
         tc_fence_after();
-        const float2 theirs = *join;
-        const float my_shift = set ? shift : INFINITY, least = fminf(my_shift, theirs.x);
-        mine = my_shift == least ? 1.f : ex2_approx(least - my_shift);
-        other = theirs.x == least ? 1.f : ex2_approx(least - theirs.x);
-        l = l * mine + theirs.y * other;
+        const Maximum theirs{join[0], join[128], join[128] < INFINITY};
+        if (m.set && theirs.set) {  // else one has zeros, or NaN, which counts as well
+          const float up = above(theirs, m, p.scale_log2);
+          mine = up > 0.f ? ex2_approx(-up) : 1.f;
+          other = up > 0.f ? 1.f : ex2_approx(up);
+        } else {
+          other = 1.f;
+        }
+        l = l * mine + join[256] * other;
       }
       if (active) {
         const float inv = l == 0.f ? 0.f : 1.f / l;  // no key took part: zeros

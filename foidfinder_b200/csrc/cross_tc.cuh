@@ -111,6 +111,42 @@ static __device__ Item item_by_cost(const TcArgs& a, int2* cost, Item* found) {
 // 2^-n of a whole n >= 0, exactly (0 where f32 has no normal number for it).
 __device__ __forceinline__ float power_below(float n) { return n < 127.f ? __uint_as_float(static_cast<uint32_t>(127 - static_cast<int>(n)) << 23) : 0.f; }
 
+// What a query's weights are relative to: P = 2^((s - ref) scale + shift). ref is 0 and shift a whole number, but for scores
+// beyond 2^20 powers of two: their fractions would be lost in a shift of that size, so ref is the score itself. The usual
+// way through the scores knows no ref: it has a shift then with which they all seem to have grown, and what looks into that
+// takes ref off them.
+constexpr float kFarScore = 1048576.f;
+struct Maximum {
+  float ref, shift;
+  bool set;  // there has been a key
+  __device__ __forceinline__ bool below(float top, float scale_log2) const {
+    return top > -INFINITY && (!set || fmaf(top - ref, scale_log2, shift) > kUp + kGrowth);
+  }
+};
+// `top` (a score above -inf) becomes the maximum, up to a power of two. -> What all before has to be scaled by: a whole
+// power of two, or nothing of it is left (2^-512 of P is no number of 32 bits; without a maximum there was no key).
+__device__ __forceinline__ float raise(Maximum& m, float top, float scale_log2) {
+  const float x = fmaf(top - m.ref, scale_log2, m.shift), up = floorf(x - kUp), at = top * scale_log2;
+  const bool far = !(fabsf(at) < kFarScore);
+  if (m.set && up < 512.f) {
+    m.shift = far ? x - up : m.shift - up;
+    if (far) m.ref = top;
+    return power_below(up);
+  }
+  m = {far ? top : 0.f, far ? kUp : kUp - floorf(at), true};
+  return 0.f;
+}
+// Powers of two by which a's maximum is above b's.
+__device__ __forceinline__ float above(const Maximum& a, const Maximum& b, float scale_log2) {
+  return fmaf(a.ref - b.ref, scale_log2, b.shift - a.shift);
+}
+template <int N>
+__device__ __forceinline__ float largest(const uint32_t (&s)[N]) {
+  float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+  for (int e = 0; e < N; e += 2) top[(e >> 1) & 1] = max3(top[(e >> 1) & 1], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+  return fmaxf(top[0], top[1]);
+}
 // O (dim TMEM columns from `to`) scaled by corr; out of line, it is rare.
 static __device__ __noinline__ void rescale(uint32_t to, int dim, float corr) {
   for (int c = 0; c < dim; c += 16) {

@@ -40,8 +40,8 @@ constexpr int kRing = 8;                  // steps
 constexpr int kSlot = kStep * 128;        // bytes of a K or V tile
 constexpr int kThreads64 = 640;
 constexpr int kOffRing = 4 * kAtom;       // two buffers of two query tiles
-constexpr int kOffJoin = kOffRing + 2 * kRing * kSlot;          // [2][4 streams][128 rows] (shift, sum)
-constexpr int kOffTable = kOffJoin + 2 * 4 * 128 * 8;
+constexpr int kOffJoin = kOffRing + 2 * kRing * kSlot;          // [2][4 streams][128 rows] (ref, shift, sum, nothing)
+constexpr int kOffTable = kOffJoin + 2 * 4 * 128 * 16;
 constexpr int kOffBars = kOffTable + kTable * static_cast<int>(sizeof(Item));
 constexpr int kSmem64 = 1024 + kOffBars + 512;
 static_assert(kSmem64 <= 232448, "shared memory of a CTA");
@@ -55,6 +55,55 @@ __device__ __forceinline__ int ways_of(const Item& i) { return i.nq > kBQ ? 2 : 
 __device__ __forceinline__ int phase_of(const Item& i, int stream) { return i.nq > kBQ ? stream & 1 : stream; }
 __device__ __forceinline__ int steps_of(const Item& i) { return (i.nk + kStep - 1) / kStep; }
 
+// What `shift` holds where the weights are relative to a ref: (ref, shift) are then in the query's place of the join, and all
+// scores seem to have grown.
+constexpr float kSeeJoin = 3e38f;
+
+// The way of a step whose scores have grown, or seem to: out of line, it is rare. S in TMEM from `ts` becomes P. -> What all
+// before has to be scaled by, the sum of the weights, the shift (kSeeJoin) and whether there has been a key.
+struct Grown {
+  float corr, sum, shift;
+  bool set;
+};
+template <class T>
+__device__ __noinline__ Grown grown_step(uint32_t ts, uint32_t bits0, uint32_t bits1, float4* place, float shift, bool set, float scale_log2) {
+  const bool far = shift == kSeeJoin;
+  Maximum m{far ? place->x : 0.f, far ? place->y : shift, set};
+  float top = -INFINITY;
+  uint32_t s[32];
+  auto scores = [&](int c) {
+    const uint32_t bits = c ? bits1 : bits0;
+    tmem_ld32(ts + 32 * c, s);
+    tmem_ld_wait();
+#pragma unroll
+    for (int e = 0; e < 32; ++e)
+      if (!(bits >> e & 1u)) s[e] = 0xff800000u;  // -inf
+  };
+  for (int c = 0; c < 2; ++c) {
+    scores(c);
+    top = fmaxf(top, largest(s));
+  }
+  Grown r{m.below(top, scale_log2) ? raise(m, top, scale_log2) : 1.f, 0.f, 0.f, m.set};
+  for (int c = 0; c < 2; ++c) {
+    scores(c);  // P is over the first half's
+    uint32_t pk[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      float w[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        w[i] = ex2_approx(fmaf(__uint_as_float(s[2 * e + i]) - m.ref, scale_log2, m.shift));
+        r.sum += w[i];
+      }
+      pk[e] = Pair16<T>::pack(w[0], w[1]);
+    }
+    tmem_st16(ts + 16 * c, pk);
+  }
+  r.shift = m.ref != 0.f ? kSeeJoin : m.shift;
+  if (m.ref != 0.f) *place = make_float4(m.ref, m.shift, 0.f, 0.f);
+  return r;
+}
+
 template <class T>
 __global__ void __launch_bounds__(kThreads64, 1)
     cross_tc64_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -62,7 +111,7 @@ __global__ void __launch_bounds__(kThreads64, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Item* const table = reinterpret_cast<Item*>(smem + kOffTable);
-  auto join = reinterpret_cast<float2(*)[4][128]>(smem + kOffJoin);
+  auto join = reinterpret_cast<float4(*)[4][128]>(smem + kOffJoin);
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + kOffBars);
   uint64_t* q_full = bar;               // [2]
   uint64_t* q_empty = q_full + 2;       // [2], by both MMA threads
@@ -307,8 +356,9 @@ __global__ void __launch_bounds__(kThreads64, 1)
         }
       };
       if (mask != nullptr) fetch(phase);
-      float shift = 0.f;  // 7 - m, once there is an m: a whole number
+      float shift = 0.f;  // once there is a maximum
       bool set = false;
+      float4* const place = &join[m & 1][stream][in_tile];
       float2 sum = make_float2(0.f, 0.f);
       for (int t = phase; t < steps; t += ways, ++count) {
         const uint32_t g = g0 + t, v_slot = 2 * (g % kRing) + 1;
@@ -347,64 +397,58 @@ __global__ void __launch_bounds__(kThreads64, 1)
         }
         if (active) {
           const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
-          float2 part[2];
-          for (bool again = true, once = true; again; once = false) {
-            again = false;
-            part[0] = part[1] = make_float2(0.f, 0.f);
-            float mx[2] = {-INFINITY, -INFINITY};
-            uint32_t pk[2][16];
+          float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          float mx[2] = {-INFINITY, -INFINITY};
+          uint32_t pk[2][16];
+          bool slow = false;
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              uint32_t s[32];
-              tmem_ld32(ts + 32 * c, s);
-              tmem_ld_wait();
-              if (bits[c] != 0xffffffffu) {
+          for (int c = 0; c < 2; ++c) {
+            uint32_t s[32];
+            tmem_ld32(ts + 32 * c, s);
+            tmem_ld_wait();
+            if (bits[c] != 0xffffffffu) {
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
-                  if (!(bits[c] >> e & 1u)) s[e] = 0xff800000u;  // -inf
-              }
-              if (c == 0 && once && t < ways) {  // a first m, from these 32
-                float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-                for (int e = 0; e < 32; e += 2) top[(e >> 1) & 1] = max3(top[(e >> 1) & 1], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
-                top[0] = fmaxf(top[0], top[1]);
-                set = top[0] > -INFINITY;
-                if (set) shift = kUp - floorf(top[0] * p.scale_log2);
-              }
-              const float2 sh2 = make_float2(shift, shift);
-              float2 x[16];
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                x[e] = fma2(make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), sc2, sh2);
-                mx[e & 1] = max3(mx[e & 1], x[e].x, x[e].y);
-              }
-              if (c == 1) {
-                const float top = fmaxf(mx[0], mx[1]);
-                const bool grown = top > kUp + kGrowth || (!set && top > -INFINITY);
-                if (once && __any_sync(0xffffffffu, grown)) {
-                  float corr = 1.f;
-                  if (grown) {
-                    const float up = floorf(top - kUp);
-                    corr = set ? power_below(up) : 0.f;  // without an m there was no key, and all is zero
-                    shift -= up;
-                    set = true;
-                  }
-                  if (t >= ways) rescale(to, dim, corr);
-                  sum.x *= corr;
-                  sum.y *= corr;
-                  again = true;
-                  break;
-                }
-                tmem_st16(ts, pk[0]);  // all of S is in registers
-              }
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                const float2 w = make_float2(ex2_approx(x[e].x), ex2_approx(x[e].y));
-                part[e & 1] = add2(part[e & 1], w);
-                pk[c][e] = Pair16<T>::pack(w.x, w.y);
-              }
+              for (int e = 0; e < 32; ++e)
+                if (!(bits[c] >> e & 1u)) s[e] = 0xff800000u;  // -inf
             }
-            if (!again) tmem_st16(ts + 16, pk[1]);
+            if (c == 0 && t < ways) {  // a first maximum, from these 32
+              const float top = largest(s), at = top * p.scale_log2;
+              set = fabsf(at) < kFarScore;  // else with its second half
+              if (set) shift = kUp - floorf(at);
+            }
+            const float2 sh2 = make_float2(shift, shift);
+            float2 x[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              x[e] = fma2(make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), sc2, sh2);
+              mx[e & 1] = max3(mx[e & 1], x[e].x, x[e].y);
+            }
+            if (c == 1) {
+              const bool grown = fmaxf(mx[0], mx[1]) > kUp + kGrowth || (!set && (bits[0] | bits[1]) != 0);
+              if (__any_sync(0xffffffffu, grown)) {
+                slow = true;
+                break;
+              }
+              tmem_st16(ts, pk[0]);  // all of S is in registers
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float2 w = make_float2(ex2_approx(x[e].x), ex2_approx(x[e].y));
+              part[e & 1] = add2(part[e & 1], w);
+              pk[c][e] = Pair16<T>::pack(w.x, w.y);
+            }
+          }
+          if (!slow) {
+            tmem_st16(ts + 16, pk[1]);
+          } else {
+            const Grown r = grown_step<T>(ts, bits[0], bits[1], place, shift, set, p.scale_log2);
+            if (t >= ways) rescale(to, dim, r.corr);
+            sum.x *= r.corr;
+            sum.y *= r.corr;
+            part[0] = make_float2(r.sum, 0.f);
+            part[1] = make_float2(0.f, 0.f);
+            shift = r.shift;
+            set = r.set;
           }
           sum = add2(sum, add2(part[0], part[1]));
         }
@@ -425,25 +469,31 @@ __global__ void __launch_bounds__(kThreads64, 1)
         if (!mbar_wait(&o_full[stream], worked & 1u, abort_flag, err, kDevTimeoutAttn)) break;
         ++worked;
       }
-      // The tile's streams are joined: each takes every ways-th 16 columns. A stream's O is 2^shift times what it stands for.
-      join[m & 1][stream][in_tile] = make_float2(set ? shift : INFINITY, sum.x + sum.y);
+      // The tile's streams are joined: each takes every ways-th 16 columns.
+      if (shift != kSeeJoin) *place = make_float4(0.f, set ? shift : INFINITY, 0.f, 0.f);
+      place->z = sum.x + sum.y;
       __syncwarp();
       if (lane == 0) mbar_arrive(joined);
       if (!mbar_wait(joined, m & 1u, abort_flag, err, kDevTimeoutAttn)) break;
       tc_fence_after();
       if (active) {
         const int base = stream & ~(ways - 1), with = min(ways, steps);  // streams of this tile, and those that had a step
-        float weight[4], least = INFINITY, l = 0.f;
+        float weight[4], l = 0.f;
+        Maximum most{0.f, INFINITY, false};  // the highest
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (i < with) least = fminf(least, join[m & 1][base + i][in_tile].x);
+          if (i < with) {
+            const float4 v = join[m & 1][base + i][in_tile];
+            const Maximum other{v.x, v.y, v.y < INFINITY};
+            if (other.set && (!most.set || above(other, most, p.scale_log2) > 0.f)) most = other;
+          }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           weight[i] = 0.f;
           if (i < with) {
-            const float2 v = join[m & 1][base + i][in_tile];
-            weight[i] = v.x == least ? 1.f : ex2_approx(least - v.x);
-            l = fmaf(v.y, weight[i], l);
+            const float4 v = join[m & 1][base + i][in_tile];
+            weight[i] = v.y < INFINITY ? ex2_approx(above({v.x, v.y, true}, most, p.scale_log2)) : 1.f;  // without a key: zeros, or NaN, which counts
+            l = fmaf(v.z, weight[i], l);
           }
         }
         const float inv = l == 0.f ? 0.f : 1.f / l;  // no key took part: zeros

@@ -4,9 +4,12 @@ at the test."""
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
+from oracle import cross as O
 from test_gpu_cross import BF16, F16, _attend, _check_attention, _pieces, _qkv
 
 pytestmark = pytest.mark.gpu
@@ -105,3 +108,65 @@ def test_weights_are_rounded_once(no_device_error, kernels_of, dim, dtype):
     (out, names) = kernels_of(lambda: _attend(q, k, v, heads=heads, head_dim=dim, sequences=sequences, scale=1.0, mask=mask))
     _ran(names, _kernel(dim))
     _check_attention(out, q, k, v, heads=heads, kv_heads=heads, dim=dim, pieces=_pieces([nq] * sequences, [nk] * sequences, mask, at), scale=1.0)
+
+
+# What reaches each kernel: sequences, queries and keys of each, heads of how many columns.
+EACH_KERNEL = {"cross_few_kernel": [(3, 1, 300, 64), (2, 1, 1100, 128), (2, 20, 150, 80), (5, 4, 40, 16)], NARROW: [(16, 300, 290, 64), (48, 100, 290, 48)],
+               WIDE: [(16, 300, 290, 128), (16, 100, 290, 80)]}
+EACH_KERNEL = [pytest.param(name, *shape, id="-".join(map(str, (name, *shape)))) for name, shapes in EACH_KERNEL.items() for shape in shapes]
+
+
+@pytest.mark.parametrize("order", ["rising", "falling", "mixed", "late"])
+@pytest.mark.parametrize(("dtype", "q0", "k0", "apart"), [
+    pytest.param(dtype, q0, k0, apart, id=f"{str(dtype)[6:]}-{math.copysign(math.log2(abs(q0 * k0)), q0 * k0):.0f}")
+    for dtype, q0, k0, apart in (
+        (F16, 2.0**6, 2.0**10, 1.0), (F16, 2.0**14, 2.0**10, 1.0), (F16, 2.0**14, -(2.0**10), 1.0), (F16, 2.0**14, -(2.0**14), 16.0), (F16, 2.0**15, 2.0**14, 16.0),
+        (BF16, 2.0**20, 2.0**20, 2.0**13), (BF16, 2.0**40, -(2.0**50), 2.0**43), (BF16, -(2.0**60), 2.0**60, 2.0**53))])
+@pytest.mark.parametrize(("kernel", "sequences", "nq", "nk", "dim"), EACH_KERNEL)
+def test_scores_far_from_zero(no_device_error, kernels_of, kernel, sequences, nq, nk, dim, dtype, q0, k0, apart, order):
+    """Scores of up to 2^120, whose fractions 32 bits do not hold, exact multiples of q0 apart (64 at least, so the second best has no
+    weight): the result is the mean of the best key's values and those of its doubles. Their weights are equal: one
+    rounding to 16 bits, and the sum's in 32; then the output's."""
+    heads = 8
+    n = torch.arange(nk) % 100
+    late = torch.arange(nk) > nk - 10
+    level = {"rising": n, "falling": 99 - n, "mixed": 37 * n % 100, "late": n * late}[order].double()
+    keys = k0 + apart * level
+    if order == "late" and k0 > 0:
+        keys = torch.where(late, keys, 0.0)
+    q, k, v = _qkv(sequences * nq, sequences * nk, heads, heads, dim, dtype, seed=3)
+    q[:], k[:] = 0, 0
+    q[:, ::dim] = q0
+    k[:, ::dim] = keys.to(dtype).repeat(sequences)[:, None]
+    assert torch.equal(k[:nk, 0].double(), keys)
+    top = (q0 * keys == (q0 * keys).max()).nonzero()[:, 0]
+    best = v.reshape(sequences, nk, heads * dim)[:, top].double()
+    (out, names) = kernels_of(lambda: _attend(q, k, v, heads=heads, head_dim=dim, sequences=sequences, scale=1.0))
+    assert any(kernel + "<" in n for n in names), names
+    want, size = best.mean(1)[:, None], best.abs().mean(1)[:, None]
+    half = torch.finfo(dtype).eps / 2
+    off = (out.double().cpu().reshape(sequences, nq, -1) - want).abs()
+    assert (off <= size * (half + 2.0**-20) + want.abs() * half * (1 + half) + 2.0**-25).all(), off.max()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize(("kernel", "sequences", "nq", "nk", "dim"), EACH_KERNEL)
+def test_scores_far_from_zero_and_near_each_other(no_device_error, kernels_of, kernel, sequences, nq, nk, dim, dtype):
+    """Scores from 2^21 to 2^22 (exact, in steps of 2^14) times scale 2^-14: the best has most of the weight, its neighbours e^-1,
+    e^-2 and so on. And the same ones 2^24 times as large, where the best has all. Exponents are exact but for scale *
+    log2(e), within 2^-23 of itself: times at most 128 * 1.45, and times ln 2 in a weight, that is 2^-15."""
+    heads = 8
+    q, k, v = _qkv(sequences * nq, sequences * nk, heads, heads, dim, dtype, seed=7)
+    level = 37 * torch.arange(nk) % 100 + 128
+    q[:], k[:] = 0, 0
+    q[:, ::dim] = 2.0**7
+    k[:, ::dim] = (2.0**7 * level).to(dtype).repeat(sequences)[:, None]
+    at = [slice(i * nk, (i + 1) * nk) for i in range(sequences)]
+    pieces = [(slice(i * nq, (i + 1) * nq), s) for i, s in enumerate(at)]
+    half = torch.finfo(dtype).eps / 2
+    for scale in (2.0**-14, 2.0**10):
+        (out, names) = kernels_of(lambda: _attend(q, k, v, heads=heads, head_dim=dim, sequences=sequences, scale=scale))
+        assert any(kernel + "<" in n for n in names), names
+        want, size, _, _ = O.attention(q, k, v, heads=heads, kv_heads=heads, head_dim=dim, pieces=pieces, scale=scale)
+        off = (out.double().cpu() - want).abs()
+        assert (off <= size * (half + 2 * 2.0**-15 + 2.0**-20) + want.abs() * half * (1 + half) + nk * 2.0**-32 * 5 + 2.0**-25).all(), off.max()
