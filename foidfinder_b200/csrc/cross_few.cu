@@ -15,8 +15,9 @@
 // the warps' chains of products and exponentials; one query 50.5 us, 5.3 TB/s; one query over 24600 keys of 4 sequences, 16
 // heads over 4 of 128: 39 us, 5.2 TB/s; one query over 1025 keys of one image 7.5 us, over 32800 keys of one head of 128 15.4.
 //
-// P is rounded to 16 bits for its product with V, as 2^((s - max) scale + 14) in fp16, where it would else lose bits below 2^-14;
-// sums are taken before that rounding, in f32.
+// P is rounded to 16 bits for its product with V, as 2^((s - max) scale + 14) in fp16, where it would else lose bits below 2^-14, and
+// with -20 in bf16, so that sums over 2^20 values next to the type's largest stay in f32's range; sums of P are taken
+// before that rounding, in f32.
 #include <algorithm>
 
 #include "common.h"
@@ -104,7 +105,7 @@ template <class T, int ATOMS, int RG, bool SHORT>
 __global__ void __launch_bounds__(kFewThreads, few_ctas(ATOMS)) cross_few_kernel(const __grid_constant__ FewArgs a) {
   constexpr int STAGES = few_stages(ATOMS), TILE = few_tile(ATOMS), KG = 4 / RG, KW = kKeys / KG;
   constexpr int ROWS = 16 * RG, STEPS = ATOMS * 4;
-  constexpr float kShift = std::is_same<T, __half>::value ? 14.f : 0.f;
+  constexpr float kShift = std::is_same<T, __half>::value ? 14.f : -20.f;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ uint64_t taken[STAGES];  // bits: keys of a tile that take part
   __shared__ float part_m[KG][ROWS], part_l[KG][ROWS];

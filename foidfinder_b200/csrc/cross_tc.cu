@@ -14,7 +14,7 @@
 //              S_1(j + 1); MMAs of one thread execute in order, so S_i(j + 1) finds P_i(j) consumed. (A thread for each
 //              stream let both fall in step and then wait together: 619 us where this takes 463.)
 //   warps 2-5  softmax of stream 0, warps 6-9 of stream 1, a query per thread: 32 scores at a time, the next 32 on their
-//              way meanwhile, P = 2^(s - m + 7) in 16 bits, the sum of P in f32 before that rounding. m is the
+//              way meanwhile, P = 2^(s - m + 7) (bf16: s - m - 28) in 16 bits, the sum of P in f32 before that rounding. m is the
 //              maximum at some earlier time: the exponentials start at once, and the new maximum is found beside them.
 //              Only where it has grown by more than 2^8 (P could pass 2^15, fp16's range) do m, O, the sum and the P so
 //              far get rescaled, by a whole power of two, and the 32 exponentials repeated.
@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (c == 0 && j == first) {  // a first maximum
               const float at = largest(sc) * p.scale_log2;
               m.set = fabsf(at) < kFarScore;  // else below
-              if (m.set) use = m.shift = kUp - floorf(at);
+              if (m.set) use = m.shift = kUp<T> - floorf(at);
             }
             uint32_t pk[16];
             float2 part;
@@ -416,12 +416,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               return fmaxf(mx[0], mx[1]);
             };
             const float mx = exponentials(use);
-            const bool grown = mx > kUp + kGrowth || (!m.set && bits[c] != 0);
+            const bool grown = mx > kUp<T> + kGrowth || (!m.set && bits[c] != 0);
             if (__any_sync(0xffffffffu, grown)) {
               if (c < 3) tmem_ld_wait();  // nothing on its way into registers across the calls
               tmem_st_wait();  // what the calls read back (P of the chunks before, O after an earlier growth) has been written
               const float top = largest(sc);
-              const float corr = m.below(top, p.scale_log2) ? raise(m, top, p.scale_log2) : 1.f;
+              const float corr = below<T>(m, top, p.scale_log2) ? raise<T>(m, top, p.scale_log2) : 1.f;
               use = m.ref != 0.f ? 3e38f : m.shift;
               if (__any_sync(0xffffffffu, m.ref != 0.f)) {
 #pragma unroll

@@ -1,5 +1,7 @@
 // What the two tensor-core kernels of cross attention share (cross_tc.cu: heads of more than 64 columns; cross_tc64.cu: up to 64).
 #pragma once
+#include <type_traits>
+
 #include "common.h"
 #include "cross.h"
 #include "fp4.cuh"
@@ -10,7 +12,10 @@ constexpr int kBQ = 128;          // queries of a tile
 constexpr int kAtom = 128 * 128;  // bytes: 128 rows of 64 columns, 128-byte swizzle
 constexpr int kTable = 16;        // items of a CTA that are looked up ahead, all at once
 constexpr float kGrowth = 8.f;    // powers of two by which the maximum may grow before O is rescaled
-constexpr float kUp = 7.f;        // P = 2^(x + 7): at most 2^15, in fp16's range
+// P = 2^(x + kUp), at most 2^8 more. In fp16 up to 2^15, so that weights far below the largest are still normal numbers; in bf16 up to
+// 2^-20, so that sums over 2^20 values next to the type's largest stay in f32's range.
+template <class T>
+constexpr float kUp = std::is_same<T, __half>::value ? 7.f : -28.f;
 
 struct TcArgs {
   CrossArgs p;
@@ -119,21 +124,24 @@ constexpr float kFarScore = 1048576.f;
 struct Maximum {
   float ref, shift;
   bool set;  // there has been a key
-  __device__ __forceinline__ bool below(float top, float scale_log2) const {
-    return top > -INFINITY && (!set || fmaf(top - ref, scale_log2, shift) > kUp + kGrowth);
-  }
 };
+// Whether `top` calls for raising the maximum.
+template <class T>
+__device__ __forceinline__ bool below(const Maximum& m, float top, float scale_log2) {
+  return top > -INFINITY && (!m.set || fmaf(top - m.ref, scale_log2, m.shift) > kUp<T> + kGrowth);
+}
 // `top` (a score above -inf) becomes the maximum, up to a power of two. -> What all before has to be scaled by: a whole
 // power of two, or nothing of it is left (2^-512 of P is no number of 32 bits; without a maximum there was no key).
+template <class T>
 __device__ __forceinline__ float raise(Maximum& m, float top, float scale_log2) {
-  const float x = fmaf(top - m.ref, scale_log2, m.shift), up = floorf(x - kUp), at = top * scale_log2;
+  const float x = fmaf(top - m.ref, scale_log2, m.shift), up = floorf(x - kUp<T>), at = top * scale_log2;
   const bool far = !(fabsf(at) < kFarScore);
   if (m.set && up < 512.f) {
     m.shift = far ? x - up : m.shift - up;
     if (far) m.ref = top;
     return power_below(up);
   }
-  m = {far ? top : 0.f, far ? kUp : kUp - floorf(at), true};
+  m = {far ? top : 0.f, far ? kUp<T> : kUp<T> - floorf(at), true};
   return 0.f;
 }
 // Powers of two by which a's maximum is above b's.

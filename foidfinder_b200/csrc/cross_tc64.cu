@@ -15,7 +15,7 @@
 //   warps 1, 2  MMAs, by an elected thread each: warp 1 for streams 0 and 1, warp 2 for 2 and 3. Per step of a stream: O += P V
 //               (P read from TMEM), then S = Q K^T of the stream's next step, which finds P consumed, since MMAs of one
 //               thread execute in order.
-//   warps 4-19  softmax, four warps per stream, a query per thread: P = 2^(s - m + 7) in 16 bits, the sum of P in f32 before
+//   warps 4-19  softmax, four warps per stream, a query per thread: P = 2^(s - m + 7) (bf16: s - m - 28) in 16 bits, the sum of P in f32 before
 //               that rounding. m is the maximum at some earlier time: the exponentials start at once, and the new maximum
 //               is found beside them. Only where it has grown by more than 2^8 (P could pass 2^15, fp16's range) are m, O
 //               and the sum rescaled and the step's exponentials repeated.
@@ -83,7 +83,7 @@ __device__ __noinline__ Grown grown_step(uint32_t ts, uint32_t bits0, uint32_t b
     scores(c);
     top = fmaxf(top, largest(s));
   }
-  Grown r{m.below(top, scale_log2) ? raise(m, top, scale_log2) : 1.f, 0.f, 0.f, m.set};
+  Grown r{below<T>(m, top, scale_log2) ? raise<T>(m, top, scale_log2) : 1.f, 0.f, 0.f, m.set};
   for (int c = 0; c < 2; ++c) {
     scores(c);  // P is over the first half's
     uint32_t pk[16];
@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(kThreads64, 1)
             if (c == 0 && t < ways) {  // a first maximum, from these 32
               const float top = largest(s), at = top * p.scale_log2;
               set = fabsf(at) < kFarScore;  // else with its second half
-              if (set) shift = kUp - floorf(at);
+              if (set) shift = kUp<T> - floorf(at);
             }
             const float2 sh2 = make_float2(shift, shift);
             float2 x[16];
@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(kThreads64, 1)
               mx[e & 1] = max3(mx[e & 1], x[e].x, x[e].y);
             }
             if (c == 1) {
-              const bool grown = fmaxf(mx[0], mx[1]) > kUp + kGrowth || (!set && (bits[0] | bits[1]) != 0);
+              const bool grown = fmaxf(mx[0], mx[1]) > kUp<T> + kGrowth || (!set && (bits[0] | bits[1]) != 0);
               if (__any_sync(0xffffffffu, grown)) {
                 slow = true;
                 break;

@@ -170,3 +170,23 @@ def test_scores_far_from_zero_and_near_each_other(no_device_error, kernels_of, k
         want, size, _, _ = O.attention(q, k, v, heads=heads, kv_heads=heads, head_dim=dim, pieces=pieces, scale=scale)
         off = (out.double().cpu() - want).abs()
         assert (off <= size * (half + 2 * 2.0**-15 + 2.0**-20) + want.abs() * half * (1 + half) + nk * 2.0**-32 * 5 + 2.0**-25).all(), off.max()
+
+
+@pytest.mark.parametrize("size", [3e38, 1e30, 1e-25])
+@pytest.mark.parametrize(("kernel", "sequences", "nq", "nk", "dim"), EACH_KERNEL)
+def test_values_of_any_size(no_device_error, kernels_of, kernel, sequences, nq, nk, dim, size):
+    """bf16 values next to the type's largest, and far below 1: sums of weights times values stay numbers of 32 bits. (Scores near each
+    other, so that all weights count. The smallest products are off by f32's smallest normal number at most, 2^-126, where
+    1e-25 times a weight of 2^-28 is 2^-111: within the 2^-9 of a weight's rounding, which few come near.)"""
+    heads = 8
+    q, k, v = _qkv(sequences * nq, sequences * nk, heads, heads, dim, BF16, seed=13)
+    q = q / 16
+    v = (v.float().clamp(-1, 1) * size).to(BF16)
+    v[::nk] = size
+    (out, names) = kernels_of(lambda: _attend(q, k, v, heads=heads, head_dim=dim, sequences=sequences))
+    assert any(kernel + "<" in n for n in names), names
+    assert out.isfinite().all()
+    pieces = [(slice(i * nq, (i + 1) * nq), slice(i * nk, (i + 1) * nk)) for i in range(sequences)]
+    want, magnitude, dot, _ = O.attention(q, k, v, heads=heads, kv_heads=heads, head_dim=dim, pieces=pieces, scale=dim**-0.5)
+    off, half = (out.double().cpu() - want).abs(), 2.0**-9
+    assert (off <= magnitude * (half + 2 * 2.0**-20 * dot + 2.0**-20) + want.abs() * half * (1 + half)).all(), (off / magnitude).max()
