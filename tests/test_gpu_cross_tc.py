@@ -9,8 +9,9 @@ import math
 import pytest
 import torch
 
+from foidfinder_b200 import ops
 from oracle import cross as O
-from test_gpu_cross import BF16, F16, _attend, _check_attention, _pieces, _qkv
+from test_gpu_cross import BF16, F16, _attend, _check_attention, _pieces, _qkv, _randn, _starts
 
 pytestmark = pytest.mark.gpu
 
@@ -190,3 +191,220 @@ def test_values_of_any_size(no_device_error, kernels_of, kernel, sequences, nq, 
     want, magnitude, dot, _ = O.attention(q, k, v, heads=heads, kv_heads=heads, head_dim=dim, pieces=pieces, scale=dim**-0.5)
     off, half = (out.double().cpu() - want).abs(), 2.0**-9
     assert (off <= magnitude * (half + 2 * 2.0**-20 * dot + 2.0**-20) + want.abs() * half * (1 + half)).all(), (off / magnitude).max()
+
+
+def _check(out, q, k, v, *, heads, kv_heads=None, dim, pieces):
+    _check_attention(out, q, k, v, heads=heads, kv_heads=kv_heads or heads, dim=dim, pieces=pieces)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", range(16, 129, 16))
+@pytest.mark.parametrize(("sequences", "nq", "nk", "heads", "kv_heads"), [(37, 500, 130, 2, 2), (37, 250, 130, 4, 1), (74, 128, 65, 2, 2), (2, 700, 1500, 48, 16), (37, 250, 1, 4, 4)])
+def test_every_head_size(no_device_error, kernels_of, sequences, nq, nk, heads, kv_heads, dim, dtype):
+    """Items of one query tile and of two, last tiles of one query and of few, keys that end within a step, and longer than the
+    ring of loads."""
+    q, k, v = _qkv(sequences * nq, sequences * nk, heads, kv_heads, dim, dtype)
+    (out, names) = kernels_of(lambda: _attend(q, k, v, heads=heads, kv_heads=kv_heads, head_dim=dim, sequences=sequences))
+    _ran(names, _kernel(dim))
+    _check(out, q, k, v, heads=heads, kv_heads=kv_heads, dim=dim, pieces=_pieces([nq] * sequences, [nk] * sequences))
+
+
+@pytest.mark.parametrize(("dim", "heads"), [(64, 32), (128, 16)])
+def test_more_items_than_are_looked_up_ahead(no_device_error, kernels_of, dim, heads):
+    """More than 16 items for each of 148 CTAs."""
+    sequences, nq, nk = 151, 128, 200
+    q, k, v = _qkv(sequences * nq, sequences * nk, heads, heads, dim, F16)
+    (out, names) = kernels_of(lambda: _attend(q, k, v, heads=heads, head_dim=dim, sequences=sequences))
+    _ran(names, _kernel(dim))
+    _check(out, q, k, v, heads=heads, dim=dim, pieces=_pieces([nq] * sequences, [nk] * sequences))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("nk", [1, 15, 16, 17, 31, 63, 64, 65, 127, 128, 129, 192, 193, 255, 257, 511, 513, 1000])
+@pytest.mark.parametrize("nq", [100, 128, 129, 256, 257])
+def test_every_end_of_a_tile(no_device_error, kernels_of, nq, nk, dim):
+    sequences, heads = 37, 4 if nq <= 256 else 2  # 148 items
+    q, k, v = _qkv(sequences * nq, sequences * nk, heads, 2, dim, BF16)
+    (out, names) = kernels_of(lambda: _attend(q, k, v, heads=heads, kv_heads=2, head_dim=dim, sequences=sequences))
+    _ran(names, _kernel(dim))
+    _check(out, q, k, v, heads=heads, kv_heads=2, dim=dim, pieces=_pieces([nq] * sequences, [nk] * sequences))
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize(("sequences", "heads", "kv_heads", "dim"), [(40, 16, 16, 64), (40, 16, 4, 128), (40, 12, 2, 48), (330, 4, 2, 64), (700, 4, 1, 80)])
+def test_packed(no_device_error, kernels_of, sequences, heads, kv_heads, dim, dtype, masked):
+    """Sequences of any lengths, none among them, packed with rows before and behind; a mask that leaves some of them nothing. What
+    takes no part is NaN or infinite, and rows outside the sequences stay. (From 321 sequences on, items are not put in
+    order.)"""
+    nq, nk = [(137 * i) % 390 for i in range(sequences)], [(253 * i) % 700 * (i % 9 != 4) for i in range(sequences)]
+    if sequences > 300:
+        nk = [n // 8 for n in nk]
+    before, behind = 5, 200
+    q, k, v = _qkv(sum(nq) + before + behind, sum(nk) + before + behind, heads, kv_heads, dim, dtype)
+    ks = _starts(nk, before)
+    mask = None
+    if masked:
+        mask = torch.rand(k.shape[0], generator=torch.Generator().manual_seed(4)) < 0.6
+        for b in range(0, sequences, 7):
+            mask[ks[b] : ks[b + 1]] = False
+        at = int(ks[sequences // 2])
+        mask[at : at + 500] = False  # whole tiles
+    pieces = [(qi + before, ki) for qi, ki in _pieces(nq, nk, mask, [int(s) for s in ks[:-1]])]
+    used = torch.zeros(k.shape[0], dtype=torch.bool)
+    for _, ki in pieces:
+        used[ki] = True
+    k[~used], v[~used] = math.nan, math.inf
+    v[~used, ::2] = math.nan
+    (out, names) = kernels_of(lambda: _attend(q, k, v, heads=heads, kv_heads=kv_heads, head_dim=dim, q_start=_starts(nq, before), k_start=ks, mask=mask))
+    _ran(names, _kernel(dim))
+    _check(out, q, torch.where(used[:, None], k, 0), torch.where(used[:, None], v, 0), heads=heads, kv_heads=kv_heads, dim=dim, pieces=pieces)
+    assert (out[:before] == 9).all() and (out[before + sum(nq) :] == 9).all()
+    for qi, ki in pieces:
+        if len(ki) == 0 and len(qi):
+            assert (out[qi.cuda()] == 0).all()
+
+
+@pytest.mark.parametrize("nq", [100, 300])
+@pytest.mark.parametrize("dim", [64, 96])
+def test_padded(no_device_error, kernels_of, dim, nq):
+    """Equal pieces of which the first k_len keys take part, lengths out of range included, with and without q_start and a mask."""
+    sequences, heads, nk = 30, 16, 400
+    lens = [(97 * i) % 400 for i in range(sequences)]
+    lens[3], lens[4], lens[5] = 999, -7, 0
+    kept = [min(max(n, 0), nk) for n in lens]
+    q, k, v = _qkv(sequences * nq, sequences * nk, heads, 4, dim, F16)
+    at = [nk * i for i in range(sequences)]
+    for mask in (None, torch.rand(sequences * nk, generator=torch.Generator().manual_seed(8)) < 0.8):
+        pieces = _pieces([nq] * sequences, kept, mask, at)
+        used = torch.zeros(sequences * nk, dtype=torch.bool)
+        for _, ki in pieces:
+            used[ki] = True
+        dirty = torch.where(used[:, None], k, math.inf), torch.where(used[:, None], v, math.nan)
+        clean = torch.where(used[:, None], k, 0), torch.where(used[:, None], v, 0)
+        for more in (dict(sequences=sequences), dict(q_start=_starts([nq] * sequences))):
+            kw = dict(heads=heads, kv_heads=4, head_dim=dim, k_len=torch.tensor(lens).int(), mask=mask, **more)
+            (out, names) = kernels_of(lambda: _attend(q, *dirty, **kw))
+            _ran(names, _kernel(dim))
+            _check(out, q, *clean, heads=heads, kv_heads=4, dim=dim, pieces=pieces)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_starts_beyond_the_rows(no_device_error, kernels_of, dim):
+    """Starts past the rows that there are, or before the first, are taken back to them."""
+    nq, heads = 300, 160
+    q, k, v = _qkv(2 * nq, 300, heads, 8, dim, F16)
+    starts = dict(q_start=torch.tensor([-4, nq, 5 * nq + 9]).int(), k_start=torch.tensor([-100, 100, 1 << 30]).int())
+    (out, names) = kernels_of(lambda: _attend(q, k, v, heads=heads, kv_heads=8, head_dim=dim, **starts))
+    _ran(names, _kernel(dim))
+    _check(out, q, k, v, heads=heads, kv_heads=8, dim=dim, pieces=_pieces([nq, nq], [100, 200]))
+
+
+@pytest.mark.parametrize("dim", [64, 112])
+def test_views(no_device_error, kernels_of, dim):
+    """Keys and values as halves of a packed projection, queries and results in wider rows, each 16 bytes further in."""
+    sequences, heads, nq, nk = 20, 16, 140, 333
+    cols = heads * dim
+    q, kv = _randn(sequences * nq, 3 * cols, seed=1, dtype=F16), _randn(sequences * nk, 2 * cols + 16, seed=2, dtype=F16)
+    out = torch.full((sequences * nq, cols + 24), 9.0, dtype=F16, device="cuda")
+    dq, dkv = q.cuda(), kv.cuda()
+    call = lambda: ops.cross_attention(dq[:, cols : 2 * cols], dkv[:, 8 : 8 + cols], dkv[:, 16 + cols :], out[:, 8 : 8 + cols], heads=heads, head_dim=dim, sequences=sequences)
+    _, names = kernels_of(call)
+    _ran(names, _kernel(dim))
+    _check(out[:, 8 : 8 + cols], q[:, cols : 2 * cols], kv[:, 8 : 8 + cols], kv[:, 16 + cols :], heads=heads, dim=dim, pieces=_pieces([nq] * sequences, [nk] * sequences))
+    assert (out[:, :8] == 9).all() and (out[:, 8 + cols :] == 9).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_offsets_beyond_32_bits(no_device_error, kernels_of, dim):
+    """Rows of every matrix that lie more than 2^32 bytes and 2^31 elements from the first."""
+    rows, pitch, heads, nq, nk = 300_000, 8192, 16, 600, 700
+    big = torch.empty(rows, pitch, dtype=F16, device="cuda")
+    assert big.nbytes > 1 << 32 and big.numel() > 1 << 31
+    cols = heads * dim
+    q, k, v = _qkv(4 * nq, 4 * nk, heads, heads, dim, F16)
+    q_at, k_at = rows - 4 * nq, rows - 4 * nk
+    parts = [big[:, i * 2048 : i * 2048 + cols] for i in range(4)]
+    for part, t in zip(parts, (q, k, v)):
+        part[rows - t.shape[0] :] = t.cuda()
+    parts[3][:] = 9
+    starts = dict(q_start=_starts([nq] * 4, q_at).cuda(), k_start=_starts([nk] * 4, k_at).cuda())
+    _, names = kernels_of(lambda: ops.cross_attention(*parts, heads=heads, head_dim=dim, **starts))
+    _ran(names, _kernel(dim))
+    _check(parts[3][q_at:], q, k, v, heads=heads, dim=dim, pieces=_pieces([nq] * 4, [nk] * 4))
+    assert (parts[3][:q_at] == 9).all()
+    del big, parts
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("nq", [100, 300])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_non_finite_keys_and_queries(no_device_error, kernels_of, dim, nq):
+    """A NaN or an infinite score stays with what reads it. (A score of -inf counts nothing; the sequence with it is not compared.)"""
+    sequences, heads, nk = 16, 8, 400
+    q, k, v = _qkv(sequences * nq, sequences * nk, heads, heads, dim, F16)
+    want = q.clone(), k.clone(), v.clone()
+    k[nk + 150, 3] = math.nan  # sequence 1, head 0
+    k[2 * nk + 390, 1 * dim + 5] = math.inf  # sequence 2, head 1: a score of either infinity
+    v[3 * nk + 7, 2 * dim + 1] = math.nan  # sequence 3, head 2, column 1
+    q[nq - 1, dim] = math.nan  # sequence 0, last query, head 1
+    (out, names) = kernels_of(lambda: _attend(q, k, v, heads=heads, head_dim=dim, sequences=sequences))
+    _ran(names, _kernel(dim))
+    bad = torch.zeros(sequences * nq, heads * dim, dtype=torch.bool)
+    bad[nq : 2 * nq, :dim] = True
+    bad[3 * nq : 4 * nq, 2 * dim + 1] = True
+    bad[nq - 1, dim : 2 * dim] = True
+    rows = torch.arange(2 * nq, 3 * nq)
+    plus = rows[q[rows, dim + 5] > 0]  # its score is +inf: no difference to it is a number
+    bad[plus, dim : 2 * dim] = True
+    got = out.cpu()
+    assert got[bad].isnan().all()
+    good, size, dot, _ = O.attention(*want, heads=heads, kv_heads=heads, head_dim=dim, pieces=_pieces([nq] * sequences, [nk] * sequences), scale=dim**-0.5)
+    rest = ~bad & (torch.arange(sequences * nq)[:, None] // nq != 2)
+    tol = size * (2.0**-11 + 2 * 2.0**-20 * 60 + 2.0**-20) + nk * 2.0**-32 * 5 + good.abs() * 2.0**-11 * 1.001 + 2.0**-25
+    assert ((got.double() - good).abs() <= tol)[rest].all()
+    assert got[~bad].isfinite().all()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_same_bits_every_time_on_other_streams_and_in_a_graph(no_device_error, kernels_of, dim):
+    """Equal pieces and packed ones: the same bits again, several calls at once on streams of their own, and as a graph that is
+    replayed on other inputs beside eager calls."""
+    heads, sequences = 16, 10
+    nq, nk = [260, 100, 0, 513, 128, 300, 77, 256, 30, 400], [300, 700, 64, 0, 900, 129, 500, 64, 200, 1000]
+    even = [_qkv(10 * 300, 10 * 600, heads, 4, dim, BF16, seed=10 * i) for i in range(2)]
+    packed = [_qkv(sum(nq), sum(nk), heads, 4, dim, BF16, seed=100 + 10 * i) for i in range(2)]
+    starts = dict(q_start=_starts(nq).cuda(), k_start=_starts(nk).cuda())
+    calls = [(tuple(t.cuda() for t in s), kw) for some, kw in ((even, dict(sequences=sequences)), (packed, starts)) for s in some]
+    run = lambda c, o: ops.cross_attention(*c[0], o, heads=heads, kv_heads=4, head_dim=dim, **c[1])
+    outs = [torch.zeros_like(c[0][0]) for c in calls]
+    _, names = kernels_of(lambda: [run(c, o) for c, o in zip(calls, outs)])
+    _ran(names, _kernel(dim))
+    _check(outs[1], *even[1], heads=heads, kv_heads=4, dim=dim, pieces=_pieces([300] * 10, [600] * 10))
+    _check(outs[3], *packed[1], heads=heads, kv_heads=4, dim=dim, pieces=_pieces(nq, nk))
+    again, streams = [torch.zeros_like(o) for o in outs], [torch.cuda.Stream() for _ in outs]
+    for _ in range(3):
+        for st, c, o in zip(streams, calls, again):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                run(c, o)
+    torch.cuda.synchronize()
+    for a, b in zip(outs, again):
+        assert torch.equal(a, b)
+    for first in (0, 2):
+        c, static = calls[first], tuple(t.clone() for t in calls[first][0])
+        o, beside = torch.zeros_like(outs[first]), torch.zeros_like(outs[first])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run((static, c[1]), o)
+        graph.replay()
+        assert torch.equal(o, outs[first])
+        for t, n in zip(static, calls[first + 1][0]):
+            t.copy_(n)
+        side = streams[0]
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            run(c, beside)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, outs[first + 1]) and torch.equal(beside, outs[first])
