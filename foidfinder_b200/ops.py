@@ -675,6 +675,7 @@ def rope_frequencies(
         pair = lambda n: rotary * math.log(trained / (2 * math.pi * n)) / (2 * math.log(base))
         low, high = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), rotary - 1)
         ramp = ((torch.arange(rotary // 2, dtype=torch.float64) - low) / max(high - low, 0.001)).clamp(0, 1)
+        ramp[f * trained < 2 * math.pi * slow] = 1  # the first pair too, where even that turns less than `slow` times
         f = f * (1 - ramp) + f / factor * ramp
         scale = 0.1 * math.log(factor) + 1
     return f, scale

@@ -166,3 +166,15 @@ def test_python_refuses_host_tensors():
         ops.norm_residual(x, x, x)
     with pytest.raises(RuntimeError, match="cross_attention: expected a 2-D CUDA tensor"):
         ops.cross_attention(x, x, x, x, heads=1, head_dim=64)
+
+
+@pytest.mark.parametrize("trained", [1, 3, 6, 40, 300, 4096])
+def test_stretched_frequencies_of_short_contexts(trained):
+    """yarn: pairs that turn less than once within the trained context are divided, the first one too, and those that turn more than
+    `fast` times are not."""
+    f, _ = ops.rope_frequencies(64, scaling="yarn", factor=8.0, trained=trained)
+    plain = ops.rope_frequencies(64)[0]
+    turns = plain * trained / (2 * math.pi)
+    torch.testing.assert_close(f[turns < 1], plain[turns < 1] / 8, rtol=1e-14, atol=0)
+    assert torch.equal(f[turns > 32], plain[turns > 32])
+    assert ((f <= plain) & (f >= plain / 8 * (1 - 1e-15))).all()
