@@ -559,11 +559,17 @@ int cross_tc(const CrossArgs& p, bool bf16, cudaStream_t s) {
   a.items = slots * p.heads;
   a.err = device_error_word();
   FF_REQUIRE(a.err != nullptr, "ff_cross_attention: no device error word");
-  // Sequences of different lengths: a CTA per item, so that whoever is done takes the next, the longest first (ragged captions
-  // over ragged images: 141 -> 102 us).
+  // Sequences that may differ in length: a CTA per item, so that whoever is done takes the next, the longest first; but where
+  // these are short and many, CTAs that walk them, since the start of a CTA (3.5 us) counts then and their sums even out.
+  // Walking and a CTA each (heads of 64 and 128, lengths alike to differing by 100% either way): 400 sequences of 140 queries over
+  // 64 keys 233 to 330 and 429 to 491 us, 64 of 256 over 384: 77 to 150 and 102 to 149, over 512: 90 to 191 and 114 to
+  // 178, over 1300: 175 to 413 and 188 to 318. Where there are fewer items, 24 of 200 over 256: 37 to 48 and 31 to 42, over 64: 22 to
+  // 28 and 23 to 32.
   const bool even = p.q_start == nullptr && p.k_start == nullptr && p.k_len == nullptr;
-  const int grid = static_cast<int>(std::min<int64_t>(a.items, even ? sm_count() : 0x7fffffff));
-  a.by_cost = !even && grid == a.items && p.sequences <= kTcThreads;
+  const int64_t keys = (static_cast<int64_t>(p.k_rows) + p.sequences - 1) / p.sequences;
+  const bool walk = even || keys <= 64 || (keys <= 384 && a.items > 5 * sm_count());
+  const int grid = static_cast<int>(std::min<int64_t>(a.items, walk ? sm_count() : 0x7fffffff));
+  a.by_cost = !walk && grid == a.items && p.sequences <= kTcThreads;
   if (p.dim <= 64) return cross_tc64(a, bf16, grid, s);
   return bf16 ? launch_tc<__nv_bfloat16>(a, grid, s) : launch_tc<__half>(a, grid, s);
 }

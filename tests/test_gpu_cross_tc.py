@@ -235,8 +235,7 @@ def test_every_end_of_a_tile(no_device_error, kernels_of, nq, nk, dim):
 @pytest.mark.parametrize(("sequences", "heads", "kv_heads", "dim"), [(40, 16, 16, 64), (40, 16, 4, 128), (40, 12, 2, 48), (330, 4, 2, 64), (700, 4, 1, 80)])
 def test_packed(no_device_error, kernels_of, sequences, heads, kv_heads, dim, dtype, masked):
     """Sequences of any lengths, none among them, packed with rows before and behind; a mask that leaves some of them nothing. What
-    takes no part is NaN or infinite, and rows outside the sequences stay. (From 321 sequences on, items are not put in
-    order.)"""
+    takes no part is NaN or infinite, and rows outside the sequences stay. (Items are many and short: the CTAs walk them, up to 33 each.)"""
     nq, nk = [(137 * i) % 390 for i in range(sequences)], [(253 * i) % 700 * (i % 9 != 4) for i in range(sequences)]
     if sequences > 300:
         nk = [n // 8 for n in nk]
@@ -263,6 +262,23 @@ def test_packed(no_device_error, kernels_of, sequences, heads, kv_heads, dim, dt
     for qi, ki in pieces:
         if len(ki) == 0 and len(qi):
             assert (out[qi.cuda()] == 0).all()
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("sequences", [20, 320, 321, 400])
+@pytest.mark.parametrize("dim", [64, 80])
+def test_packed_in_any_order(no_device_error, kernels_of, dim, sequences, masked):
+    """Enough keys (450 on average) that every item has a CTA of its own: the longest first, up to 320 sequences; equal lengths and
+    none among them."""
+    heads = 16 if sequences == 20 else 2
+    nq, nk = [(37 * i) % 390 for i in range(sequences)], [(53 * i) % 113 * 8 for i in range(sequences)]
+    q, k, v = _qkv(sum(nq), sum(nk), heads, 2, dim, F16)
+    mask = torch.rand(sum(nk), generator=torch.Generator().manual_seed(5)) < 0.7 if masked else None
+    at = [int(n) for n in _starts(nk)[:-1]]
+    call = lambda: _attend(q, k, v, heads=heads, kv_heads=2, head_dim=dim, q_start=_starts(nq, 0), k_start=_starts(nk, 0), mask=mask)
+    (out, names) = kernels_of(call)
+    _ran(names, _kernel(dim))
+    _check(out, q, k, v, heads=heads, kv_heads=2, dim=dim, pieces=_pieces(nq, nk, mask, at))
 
 
 @pytest.mark.parametrize("nq", [100, 300])
