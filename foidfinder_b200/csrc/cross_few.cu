@@ -87,10 +87,10 @@ __device__ __forceinline__ float2 read_cluster2(uint32_t addr) {
   asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
   return v;
 }
-// Weight of a part whose largest score is m beside the largest of all, top. (Both -inf: nothing but NaN can be there.)
-__device__ __forceinline__ float part_weight(float m, float top, float scale_log2) {
-  return m == -INFINITY && top == -INFINITY ? 1.f : ex2_approx((m - top) * scale_log2);
-}
+// What scores are relative to: the largest, or nothing (where it is -inf, nothing but NaN can be there, and counts all the same).
+__device__ __forceinline__ float reference(float top) { return top == -INFINITY ? 0.f : top; }
+// Weight of a part whose largest score is m.
+__device__ __forceinline__ float part_weight(float m, float ref, float scale_log2) { return ex2_approx((m - ref) * scale_log2); }
 
 struct FewArgs {
   CrossArgs p;
@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(ATOMS)) cross_few_kernel
         grew |= now > m[h];
         mx[h] = m[h];  // the old one
         m[h] = now;
-        ref[h] = now == -INFINITY ? 0.f : now;
+        ref[h] = reference(now);
       }
       if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
@@ -324,11 +324,12 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(ATOMS)) cross_few_kernel
       float top = part_m[0][r];
 #pragma unroll
       for (int g = 1; g < KG; ++g) top = fmaxf(top, part_m[g][r]);
+      const float ref = reference(top);
       float sum = 0.f;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int g = 0; g < KG; ++g) {
-        const float w = part_weight(part_m[g][r], top, p.scale_log2);
+        const float w = part_weight(part_m[g][r], ref, p.scale_log2);
         const float4 v = *reinterpret_cast<const float4*>(parts + (g * ROWS + r) * dim + c);
         sum = fmaf(part_l[g][r], w, sum);
         acc.x = fmaf(v.x, w, acc.x);
@@ -371,10 +372,11 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(ATOMS)) cross_few_kernel
         float top = -INFINITY, sum = 0.f;
 #pragma unroll
         for (int g = 0; g < kCluster; ++g) top = fmaxf(top, ml[g].x);
+        const float ref = reference(top);
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int g = 0; g < kCluster; ++g) {
-          const float w = part_weight(ml[g].x, top, p.scale_log2);
+          const float w = part_weight(ml[g].x, ref, p.scale_log2);
           sum = fmaf(ml[g].y, w, sum);
           acc.x = fmaf(v[g].x, w, acc.x);
           acc.y = fmaf(v[g].y, w, acc.y);
@@ -408,7 +410,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) cross_join_kernel(const __gri
   if (p.q_start != nullptr && (q_row < __ldg(p.q_start) || q_row >= __ldg(p.q_start + p.sequences))) return;  // of no sequence
   float top = -INFINITY;
   for (int i = lane; i < a.splits; i += 32) top = fmaxf(top, a.part_ml[i * rows + at].x);
-  top = warp_max(top);
+  top = reference(warp_max(top));
   float sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   const int c = lane * 4;
