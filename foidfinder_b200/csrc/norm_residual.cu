@@ -310,8 +310,10 @@ __device__ __forceinline__ float reciprocal(float v) {
   return y;
 }
 // 1 / (1 + e^-g), and for tanh 1 - 2 / (1 + e^2|g|), but its series g (1 - g^2 / 3 + 2 g^4 / 15 - 17 g^6 / 315 + 62 g^8 / 2835 -
-// 1382 g^10 / 155925) below 0.35 (the next term is 2^-25 of it there). CLOSE (32-bit results): within a few 2^-24 of the
-// value; else within 2^-19, for results that are rounded to 12 bits at most.
+// 1382 g^10 / 155925) below 0.35 (the next term is 2^-25 of it there). CLOSE (32-bit results): within 2^-20 of the
+// value; else, for results that are rounded to 12 bits at most, within 2^-19, but sigmoids of g below -22 within 2^-18 and
+// below -44 within 2^-17 (half a unit of t = g log2(e) is that much of 2^t). Below -87.3 a sigmoid is less than f32's
+// smallest normal number, and 0 here.
 template <bool CLOSE>
 __device__ __forceinline__ float activate(float g, int act) {
   auto exponential = [](float x) { return CLOSE ? exp_close(x) : ex2_approx(x * 1.44269504f); };
