@@ -11,9 +11,10 @@
 // another's shared memory (no second launch: one token over 1025 keys 9.6 -> 7.4 us, over 4096 keys no gain); more of them go through the workspace
 // and a second kernel.
 //
-// Measured (fp16): 32 queries over 1025 keys of 64 images, 16 heads of 64: 63 us, 4.4 TB/s, where half of the issue slots go to
-// the warps' chains of products and exponentials; one query 50.5 us, 5.3 TB/s; one query over 24600 keys of 4 sequences, 16
-// heads over 4 of 128: 39 us, 5.2 TB/s; one query over 1025 keys of one image 7.5 us, over 32800 keys of one head of 128 15.4.
+// Measured (fp16, at 1965 MHz): 32 queries over 1025 keys of 64 images, 16 heads of 64: 63 us, 4.4 TB/s, where half of the issue
+// slots go to the warps' chains of products and exponentials; one query 50.2 us, 5.4 TB/s; one query over 24600 keys of 4
+// sequences, 16 heads over 4 of 128: 39 us, 5.2 TB/s; one query over 1025 keys of one image 7.3 us, over 32800 keys of one
+// head of 128 13.1.
 //
 // P is rounded to 16 bits for its product with V, as 2^((s - max) scale + 14) in fp16, where it would else lose bits below 2^-14, and
 // with -20 in bf16, so that sums over 2^20 values next to the type's largest stay in f32's range; sums of P are taken
@@ -512,9 +513,9 @@ CrossFewPlan cross_few_plan(int q_rows, int k_rows, int sequences, int heads, in
   // more than 64 columns), 0.008 to 0.012 (0.024) for every CTA's start and end, does 70, 125 or 160 TFLOP/s on the rows
   // of its row tiles (1, 2 or 4 of them), or reads 5.2 TB/s. The other has 3.6 us for every SM's item of up to 256 queries of
   // a head, and for 128 keys of it 1.8 (2.4), or 1.2 (1.5) up to 128 queries, but has no parts of a sequence's keys. Measured (few, other):
-  // 64 x 32 queries, 1025 keys, 16 heads of 64: 63, 85 us; 64 x 40: 95, 92; 64 x 64 queries, 128 keys: 22, 33; 64 x 128: 40, 34;
-  // 1 x 64 queries, 5184 keys: 22, 50; 16 x 32, 2048 keys, 16 heads of 128: 72, 70; 24 x 64, 64 keys, 16 heads over 4: 14,
-  // 13; 24 x 829, 7 keys: 121, 55.
+  // 64 x 32 queries, 1025 keys, 16 heads of 64: 64, 87 us; 64 x 40: 91, 92; 64 x 64 queries, 128 keys: 22, 35; 64 x 128: 40, 34;
+  // 1 x 64 queries, 5184 keys: 22, 50; 16 x 32, 2048 keys, 16 heads of 128: 74, 69; 24 x 64, 64 keys, 16 heads over 4: 14,
+  // 15; 24 x 829, 7 keys: 121, 56. Over 210 shapes of equal lengths its choice costs 1.9% on average.
   const bool wide = dim > 64;
   const int tiles_of_rows = plan.row_tiles == 4 ? 3 : plan.row_tiles;
   const double macs = static_cast<double>(ctas) * 16 * plan.row_tiles * ((keys + 15) / 16 * 16) * dim;

@@ -12,7 +12,7 @@
 //   warp 1     MMAs, by one elected thread: S_i = Q K^T of stream i to TMEM columns [128 i, +128), and O_i += P_i V, P_i read
 //              from where S_i was, to columns [256 + 128 i, +dim). Order per key tile j of a pair: PV_0(j), S_0(j + 1), PV_1(j),
 //              S_1(j + 1); MMAs of one thread execute in order, so S_i(j + 1) finds P_i(j) consumed. (A thread for each
-//              stream let both fall in step and then wait together: 619 us where this takes 463.)
+//              stream let both fall in step and then wait together: 619 us where this took 463.)
 //   warps 2-5  softmax of stream 0, warps 6-9 of stream 1, a query per thread: 32 scores at a time, the next 32 on their
 //              way meanwhile, P = 2^(s - m + 7) (bf16: s - m - 28) in 16 bits, the sum of P in f32 before that rounding. m is the
 //              maximum at some earlier time: the exponentials start at once, and the new maximum is found beside them.
@@ -22,9 +22,10 @@
 // with zeros in shared memory before the product, so that nothing they hold (NaN, infinities) counts. Both groups of
 // softmax warps write the same zeros, each before it lets its own product start.
 //
-// Measured: 2592 queries over 5184 keys of 4 images, 16 heads, fp16: 463 us, 950 TFLOP/s (tensor pipe and exponentials each
-// busy half of the time; a quarter of the exponentials as polynomials 465); 1845 queries of 6 sequences, 32 heads over
-// 8: over 512 keys 130 us, over 16 keys 57, 3.2 TB/s; ragged captions over ragged images (24 sequences, masked) 95 us.
+// Measured (at 1965 MHz): 2592 queries over 5184 keys of 4 images, 16 heads, fp16: 468 us, 940 TFLOP/s (512 us at the 1725 MHz that
+// the power limit leaves in the long run; tensor pipe and exponentials each busy half of the time; a quarter of the
+// exponentials as polynomials no gain); 1845 queries of 6 sequences, 32 heads over 8: over 512 keys 127 us, over 16 keys
+// 55, 3.3 TB/s; ragged captions over ragged images (24 sequences, masked) 99 us.
 #include <algorithm>
 
 #include "common.h"

@@ -18,14 +18,14 @@
 //   warps 4-19  softmax, four warps per stream, a query per thread: P = 2^(s - m + 7) (bf16: s - m - 28) in 16 bits, the sum of P in f32 before
 //               that rounding. m is the maximum at some earlier time: the exponentials start at once, and the new maximum
 //               is found beside them. Only where it has grown by more than 2^8 (P could pass 2^15, fp16's range) are m, O
-//               and the sum rescaled and the step's exponentials repeated.
+//               and the sum rescaled and the step's exponentials repeated, out of line (372 us with that in the loop).
 // Keys that take no part (past the sequence's end, or masked) get P = 0, and their rows of the value tile are overwritten
 // with zeros in shared memory before the product, so that nothing they hold (NaN, infinities) counts. Streams of both
 // tiles write the same zeros, each before it lets its own product start.
 //
-// Measured: 2592 queries over 5184 keys of 4 images, 16 heads, fp16: 372 us, 592 TFLOP/s, exponentials 60% of the unit's rate (a
-// quarter of them as polynomials on the other units 421: the issue slots are half taken already); 128 queries over 1025 keys
-// of 64 images 95 us; 1845 queries over 16 keys of 6 sequences, 32 heads over 8: 44 us.
+// Measured (at 1965 MHz): 2592 queries over 5184 keys of 4 images, 16 heads, fp16: 359 us, 614 TFLOP/s, exponentials 61% of the
+// unit's rate (a quarter of them as polynomials on the other units 421 where this took 372: the issue slots are half taken
+// already); 128 queries over 1025 keys of 64 images 93 us; 1845 queries over 16 keys of 6 sequences, 32 heads over 8: 43 us.
 #include <algorithm>
 
 #include "common.h"

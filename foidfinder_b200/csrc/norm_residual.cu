@@ -8,9 +8,10 @@
 // rows of up to 1024 columns (32 values per lane), wider rows are shared by more warps, whose sums meet in shared memory.
 // All sums, statistics and products are f32; each output is rounded once.
 //
-// Measured: 65600 x 1024 bf16, two RMS norms, gate per image and scale (537 MB) 105 us, 5.1 TB/s, and without gate and scale 86 us,
-// 6.2 TB/s; 16400 x 2730 bf16, gate per element 78 us, 4.6 TB/s (2736 columns: 61 us, 5.9 TB/s); 8200 x 768 f32 with a bf16
-// branch, two LayerNorms and a scale 18.2 us, 4.1 TB/s; one row of 1024 3.8 us with its call. What is short of HBM's rate waits:
+// Measured: 65600 x 1024 bf16, two RMS norms, gate per image and scale (537 MB) 106 us, 5.1 TB/s, and without gate and scale 87 us,
+// 6.2 TB/s (at 1965 MHz; 92 at 1755, under the power limit), with two LayerNorms 122 us; 16400 x 2730 bf16, gate per element
+// 78 us, 4.6 TB/s (2736 columns: 62 us, 5.8 TB/s); 8200 x 768 f32 with a bf16 branch, two LayerNorms and a scale 17.7 us,
+// 4.3 TB/s; one row of 1024 3.3 us with its call. What is short of HBM's rate waits:
 // a row's sums need all of it, and its registers are not free for the next before. (Sums of warps merged around their own
 // means, one barrier less: 121 -> 130 us with two LayerNorms, for the instructions more. Persistent CTAs with the
 // parameters in registers: 160.)

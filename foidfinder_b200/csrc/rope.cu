@@ -7,8 +7,8 @@
 // Angles: position * frequency and its part of a whole turn in 64 bits (at position 2^20 an angle in 32 bits is off by up
 // to 0.06), the sine and cosine of that part in 32 bits, the rotation in 32 bits, one rounding at the end.
 //
-// Measured: 65600 rows of 32 heads of 64, fp16 (537 MB): pairs 91 us, 5.9 TB/s; halves 87 us, 6.1 TB/s. 32001 rows of 8 heads of 128,
-// bf16, 64 columns turning: halves 23.4 us, 5.6 TB/s.
+// Measured: 65600 rows of 32 heads of 64, fp16 (537 MB): pairs 91 us, 5.9 TB/s (at 1965 MHz; 94 at 1840, under the power limit);
+// halves 87 us, 6.1 TB/s (91 at 1810 MHz). 32001 rows of 8 heads of 128, bf16, 64 columns turning: halves 23.0 us, 5.7 TB/s.
 //
 // Bound by HBM: every value is read and written once. A CTA takes rows whose turning units (32 bytes of a head, or twice 16 a
 // half apart) make up to kTurning per thread; their loads are issued before the angles of the rows are worked out into
