@@ -24,22 +24,32 @@ def _kernel(dim):
 
 @pytest.fixture(scope="module")
 def kernels_of(cuda_device):
-    """f -> (f(), names of the cross attention kernels that it launched)."""
+    """f -> (f(), names of the cross attention kernels that it launched, or None where the profiler sees no kernels at all)."""
 
     def run(f):
         with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as prof:
             r = f()
             torch.cuda.synchronize()
-        names = {e.key for e in prof.key_averages() if "cross_" in e.key}
-        assert names, "the profiler has seen no kernel"
-        return r, names
+        return r, {e.key for e in prof.key_averages()}
 
-    return run
+    x = torch.ones(8, device=cuda_device)
+    sees = any("elementwise" in n for n in run(lambda: x + 1)[1])
+
+    def named(f):
+        r, names = run(f)
+        return r, {n for n in names if "cross_" in n} if sees else None
+
+    return named
 
 
-def _ran(names, *kernels):
-    """Exactly these kernels (whole names: one is the beginning of another's)."""
-    assert len(names) == len(kernels) and all(any(k + "<" in n for n in names) for k in kernels), names
+def _ran(names, kernel):
+    """This kernel alone (whole names: one is the beginning of another's)."""
+    assert names is None or (len(names) == 1 and kernel + "<" in next(iter(names))), names
+
+
+def _ran_first(names, kernel):
+    """This kernel, perhaps with another that joins its parts."""
+    assert names is None or any(kernel + "<" in n for n in names), names
 
 
 def _levels(tiles, tile, steps):
@@ -143,7 +153,7 @@ def test_scores_far_from_zero(no_device_error, kernels_of, kernel, sequences, nq
     top = (q0 * keys == (q0 * keys).max()).nonzero()[:, 0]
     best = v.reshape(sequences, nk, heads * dim)[:, top].double()
     (out, names) = kernels_of(lambda: _attend(q, k, v, heads=heads, head_dim=dim, sequences=sequences, scale=1.0))
-    assert any(kernel + "<" in n for n in names), names
+    _ran_first(names, kernel)
     want, size = best.mean(1)[:, None], best.abs().mean(1)[:, None]
     half = torch.finfo(dtype).eps / 2
     off = (out.double().cpu().reshape(sequences, nq, -1) - want).abs()
@@ -167,7 +177,7 @@ def test_scores_far_from_zero_and_near_each_other(no_device_error, kernels_of, k
     half = torch.finfo(dtype).eps / 2
     for scale in (2.0**-14, 2.0**10):
         (out, names) = kernels_of(lambda: _attend(q, k, v, heads=heads, head_dim=dim, sequences=sequences, scale=scale))
-        assert any(kernel + "<" in n for n in names), names
+        _ran_first(names, kernel)
         want, size, _, _ = O.attention(q, k, v, heads=heads, kv_heads=heads, head_dim=dim, pieces=pieces, scale=scale)
         off = (out.double().cpu() - want).abs()
         assert (off <= size * (half + 2 * 2.0**-15 + 2.0**-20) + want.abs() * half * (1 + half) + nk * 2.0**-32 * 5 + 2.0**-25).all(), off.max()
@@ -185,7 +195,7 @@ def test_values_of_any_size(no_device_error, kernels_of, kernel, sequences, nq, 
     v = (v.float().clamp(-1, 1) * size).to(BF16)
     v[::nk] = size
     (out, names) = kernels_of(lambda: _attend(q, k, v, heads=heads, head_dim=dim, sequences=sequences))
-    assert any(kernel + "<" in n for n in names), names
+    _ran_first(names, kernel)
     assert out.isfinite().all()
     pieces = [(slice(i * nq, (i + 1) * nq), slice(i * nk, (i + 1) * nk)) for i in range(sequences)]
     want, magnitude, dot, _ = O.attention(q, k, v, heads=heads, kv_heads=heads, head_dim=dim, pieces=pieces, scale=dim**-0.5)
@@ -281,12 +291,14 @@ def test_packed_in_any_order(no_device_error, kernels_of, dim, sequences, masked
     _check(out, q, k, v, heads=heads, kv_heads=2, dim=dim, pieces=_pieces(nq, nk, mask, at))
 
 
+@pytest.mark.parametrize(("sequences", "nk"), [(30, 400), (50, 200)])
 @pytest.mark.parametrize("nq", [100, 300])
 @pytest.mark.parametrize("dim", [64, 96])
-def test_padded(no_device_error, kernels_of, dim, nq):
-    """Equal pieces of which the first k_len keys take part, lengths out of range included, with and without q_start and a mask."""
-    sequences, heads, nk = 30, 16, 400
-    lens = [(97 * i) % 400 for i in range(sequences)]
+def test_padded(no_device_error, kernels_of, dim, nq, sequences, nk):
+    """Equal pieces of which the first k_len keys take part, lengths out of range included, with and without q_start and a mask; a
+    CTA per item, and CTAs that walk them."""
+    heads = 16
+    lens = [(97 * i) % nk for i in range(sequences)]
     lens[3], lens[4], lens[5] = 999, -7, 0
     kept = [min(max(n, 0), nk) for n in lens]
     q, k, v = _qkv(sequences * nq, sequences * nk, heads, 4, dim, F16)
