@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               tmem_st_wait();  // what the calls read back (P of the chunks before, O after an earlier growth) has been written
               const float top = largest(sc);
               const float corr = below<T>(m, top, p.scale_log2) ? raise<T>(m, top, p.scale_log2) : 1.f;
-              use = m.ref != 0.f ? 3e38f : m.shift;
+              use = m.ref != 0.f ? kSeemsGrown : m.shift;
               if (__any_sync(0xffffffffu, m.ref != 0.f)) {
 #pragma unroll
                 for (int e = 0; e < 32; ++e) sc[e] = __float_as_uint(__uint_as_float(sc[e]) - m.ref);
@@ -433,6 +433,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               sum.x *= corr;
               sum.y *= corr;
               exponentials(m.shift);
+              if (part.x != part.x || part.y != part.y) {
+                m = {0.f, 0.f, true};
+                use = 0.f;
+              }
             }
             sum = add2(sum, part);
             tmem_st16(ts + 16 * c, pk);

@@ -118,9 +118,9 @@ __device__ __forceinline__ float power_below(float n) { return n < 127.f ? __uin
 
 // What a query's weights are relative to: P = 2^((s - ref) scale + shift). ref is 0 and shift a whole number, but for scores
 // beyond 2^20 powers of two: their fractions would be lost in a shift of that size, so ref is the score itself. The usual
-// way through the scores knows no ref: it has a shift then with which they all seem to have grown, and what looks into that
-// takes ref off them.
-constexpr float kFarScore = 1048576.f;
+// way through the scores knows no ref: its shift is then such that they all seem to have grown (kSeemsGrown), and what looks
+// into that takes ref off them. Where a weight is NaN, so is the result, whatever the maximum: nothing is looked into again.
+constexpr float kFarScore = 1048576.f, kSeemsGrown = 3e38f;
 struct Maximum {
   float ref, shift;
   bool set;  // there has been a key
@@ -155,6 +155,7 @@ __device__ __forceinline__ float largest(const uint32_t (&s)[N]) {
   for (int e = 0; e < N; e += 2) top[(e >> 1) & 1] = max3(top[(e >> 1) & 1], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
   return fmaxf(top[0], top[1]);
 }
+
 // O (dim TMEM columns from `to`) scaled by corr; out of line, it is rare.
 static __device__ __noinline__ void rescale(uint32_t to, int dim, float corr) {
   for (int c = 0; c < dim; c += 16) {

@@ -55,19 +55,16 @@ __device__ __forceinline__ int ways_of(const Item& i) { return i.nq > kBQ ? 2 : 
 __device__ __forceinline__ int phase_of(const Item& i, int stream) { return i.nq > kBQ ? stream & 1 : stream; }
 __device__ __forceinline__ int steps_of(const Item& i) { return (i.nk + kStep - 1) / kStep; }
 
-// What `shift` holds where the weights are relative to a ref: (ref, shift) are then in the query's place of the join, and all
-// scores seem to have grown.
-constexpr float kSeeJoin = 3e38f;
-
 // The way of a step whose scores have grown, or seem to: out of line, it is rare. S in TMEM from `ts` becomes P. -> What all
-// before has to be scaled by, the sum of the weights, the shift (kSeeJoin) and whether there has been a key.
+// before has to be scaled by, the sum of the weights, the shift and whether there has been a key. Where the weights are
+// relative to a ref, the shift is kSeemsGrown, and (ref, shift) are in the query's place of the join.
 struct Grown {
   float corr, sum, shift;
   bool set;
 };
 template <class T>
 __device__ __noinline__ Grown grown_step(uint32_t ts, uint32_t bits0, uint32_t bits1, float4* place, float shift, bool set, float scale_log2) {
-  const bool far = shift == kSeeJoin;
+  const bool far = shift == kSeemsGrown;
   Maximum m{far ? place->x : 0.f, far ? place->y : shift, set};
   float top = -INFINITY;
   uint32_t s[32];
@@ -83,7 +80,8 @@ __device__ __noinline__ Grown grown_step(uint32_t ts, uint32_t bits0, uint32_t b
     scores(c);
     top = fmaxf(top, largest(s));
   }
-  Grown r{below<T>(m, top, scale_log2) ? raise<T>(m, top, scale_log2) : 1.f, 0.f, 0.f, m.set};
+  Grown r{};
+  r.corr = below<T>(m, top, scale_log2) ? raise<T>(m, top, scale_log2) : 1.f;
   for (int c = 0; c < 2; ++c) {
     scores(c);  // P is over the first half's
     uint32_t pk[16];
@@ -99,8 +97,10 @@ __device__ __noinline__ Grown grown_step(uint32_t ts, uint32_t bits0, uint32_t b
     }
     tmem_st16(ts + 16 * c, pk);
   }
-  r.shift = m.ref != 0.f ? kSeeJoin : m.shift;
-  if (m.ref != 0.f) *place = make_float4(m.ref, m.shift, 0.f, 0.f);
+  const bool nan = r.sum != r.sum, away = m.ref != 0.f && !nan;
+  r.set = m.set || nan;
+  r.shift = nan ? 0.f : away ? kSeemsGrown : m.shift;
+  if (away) *place = make_float4(m.ref, m.shift, 0.f, 0.f);
   return r;
 }
 
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(kThreads64, 1)
         ++worked;
       }
       // The tile's streams are joined: each takes every ways-th 16 columns.
-      if (shift != kSeeJoin) *place = make_float4(0.f, set ? shift : INFINITY, 0.f, 0.f);
+      if (shift != kSeemsGrown) *place = make_float4(0.f, set ? shift : INFINITY, 0.f, 0.f);
       place->z = sum.x + sum.y;
       __syncwarp();
       if (lane == 0) mbar_arrive(joined);
